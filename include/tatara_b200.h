@@ -249,6 +249,44 @@ int tb_ft_backward_static_scratch(const float* d_dft, const int32_t* d_indices, 
                                   int ft_out, int ft_in, int max_active, float* d_grad, void* stream, char* err,
                                   size_t err_len);
 
+/* ---- operators on the caller's device tensors ----------------------------------------------
+ * No counterpart in the reference.  What a trainer with learned buckets needs beside the step: normalised rows in
+ * front of a gate and the choice of a bucket (expert) per row with a balance loss.  ALL tensor pointers are DEVICE memory of the
+ * current device, owned by the caller; the work is enqueued on `stream` (a cudaStream_t, NULL = default stream) and not synchronised; nothing is
+ * allocated and nothing is kept between calls, so calls on different streams may overlap as long as each has its own workspace.
+ * A failed call returns a code, writes the reason to err (may be NULL) and launches nothing when an argument is refused.
+ * Workspaces: tb_*_workspace returns the bytes a call of these sizes needs on the current device (negative: invalid sizes).
+ * Row strides count elements; they may exceed the row (columns of a wider buffer).  Sums are fp32 in a fixed order
+ * (repeated calls agree bit for bit), results are rounded once to the tensors' type. */
+enum { TB_TYPE_F32 = 0, TB_TYPE_F16 = 1, TB_TYPE_BF16 = 2 };
+
+/* y = (x - mean) * rstd * weight + bias per row of n; weight, bias (fp32 [n]) may be NULL (1 and 0), mean, rstd (fp32 [rows], kept
+ * for the backward pass) may be NULL.  x and y have the same type; y may be x. */
+int tb_layer_norm_forward(const void* d_x, int64_t x_stride, const float* d_weight, const float* d_bias, float eps, int type, int64_t rows,
+                          int n, void* d_y, int64_t y_stride, float* d_mean, float* d_rstd, void* stream, char* err, size_t err_len);
+int64_t tb_layer_norm_backward_workspace(int64_t rows, int n);
+/* dx, and dweight, dbias (fp32 [n], written, not added to; either may be NULL, both NULL need no workspace).  dx may be dy or x when
+ * the strides are the same. */
+int tb_layer_norm_backward(const void* d_dy, int64_t dy_stride, const void* d_x, int64_t x_stride, const float* d_mean, const float* d_rstd,
+                           const float* d_weight, int type, int64_t rows, int n, void* d_dx, int64_t dx_stride, float* d_dweight,
+                           float* d_dbias, void* d_work, int64_t work_bytes, void* stream, char* err, size_t err_len);
+
+/* The k largest of every row's `experts` logits (1 <= k <= min(experts, 16), experts <= 1024), ties to the lowest index, with
+ * the gates, per-expert counts and losses.  mask: NULL or a byte per row, 0 = the row takes no part.  A logit of -inf forbids its
+ * expert; a NaN counts as the largest and makes its row's gates and the losses NaN.  Writes index [rows, k] (-1 where no expert is left),
+ * gate [rows, k] (softmax over the chosen with renormalise, else over the row; 0 beside -1), counts [experts], rows [1] (rows N that
+ * take part and have an expert), prob_mean [experts] (P: the mean softmax over those), losses [2]: the balance loss
+ * experts * sum_e counts_e / (N k) * P_e and the z loss, the mean squared log-sum-exp (0 where N is 0). */
+int64_t tb_route_forward_workspace(int64_t rows, int experts);
+int tb_route_forward(const void* d_logits, int64_t stride, int type, int64_t rows, int experts, int k, int renormalise, const uint8_t* d_mask,
+                     int32_t* d_index, float* d_gate, int32_t* d_counts, int32_t* d_rows, float* d_prob_mean, float* d_losses, void* d_work,
+                     int64_t work_bytes, void* stream, char* err, size_t err_len);
+/* The logits' gradient from dgate [rows, k] and dlosses [2] (the gradients of the gates and of the two losses; either may be NULL: zero) and
+ * what the forward call wrote; the choice and the counts are constants.  Rows that take no part get zeros. */
+int tb_route_backward(const void* d_logits, int64_t stride, int type, int64_t rows, int experts, int k, int renormalise, const uint8_t* d_mask,
+                      const int32_t* d_index, const float* d_gate, const float* d_dgate, const int32_t* d_counts, const int32_t* d_rows,
+                      const float* d_dlosses, void* d_dlogits, int64_t dstride, void* stream, char* err, size_t err_len);
+
 /* ---- inputs: PackedSfenValue records -> step inputs, on the device ---------------------
  * Decodes 40-byte records (crates/shogi-format/src/packed_sfen.rs:387-448) and extracts the active
  * feature indices of both perspectives (crates/shogi-features/src/feature_set.rs:655-808), the

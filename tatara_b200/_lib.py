@@ -17,6 +17,7 @@ ACT_CRELU, ACT_SCRELU, ACT_PAIRWISE = 0, 1, 2
 OPT_RANGER, OPT_RADAM, OPT_ADAMW = 0, 1, 2
 LOSS_SIGMOID, LOSS_WRM = 0, 1
 NUM_SLOTS = 4
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
 
 f = C.c_float
 i32 = C.c_int32
@@ -95,6 +96,12 @@ SIGNATURES = {
     "tb_host_alloc": (C.c_int, [C.POINTER(vp), C.c_size_t]),
     "tb_host_free": (C.c_int, [vp]),
     "tb_ft_backward_static_scratch": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, C.c_char_p, C.c_size_t]),
+    "tb_layer_norm_forward": (C.c_int, [vp, i64, vp, vp, f, C.c_int, i64, C.c_int, vp, i64, vp, vp, vp, C.c_char_p, C.c_size_t]),
+    "tb_layer_norm_backward_workspace": (i64, [i64, C.c_int]),
+    "tb_layer_norm_backward": (C.c_int, [vp, i64, vp, i64, vp, vp, vp, C.c_int, i64, C.c_int, vp, i64, vp, vp, vp, i64, vp, C.c_char_p, C.c_size_t]),
+    "tb_route_forward_workspace": (i64, [i64, C.c_int]),
+    "tb_route_forward": (C.c_int, [vp, i64, C.c_int, i64, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp, C.c_char_p, C.c_size_t]),
+    "tb_route_backward": (C.c_int, [vp, i64, C.c_int, i64, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp, C.c_char_p, C.c_size_t]),
     "tb_nccl_unique_id": (C.c_int, [vp]),
     "tb_device_count": (C.c_int, []),
     "tb_version": (C.c_char_p, []),

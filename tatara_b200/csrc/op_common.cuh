@@ -1,0 +1,66 @@
+// Shared by the operators on the caller's device tensors (norm_kernels.cu, route_kernels.cu, orth_kernels.cu): element types,
+// 16-byte vectors, group reductions and how an entry point reports an error.
+#pragma once
+#include "../../include/tatara_b200.h"
+#include "common.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+#include <stdarg.h>
+#include <stdio.h>
+
+static __device__ __forceinline__ float op_float(float v) { return v; }
+static __device__ __forceinline__ float op_float(__half v) { return __half2float(v); }
+static __device__ __forceinline__ float op_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> static __device__ __forceinline__ T op_round(float v);
+template <> __device__ __forceinline__ float op_round<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half op_round<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 op_round<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// N adjacent elements as one access: 16 bytes, or a single element where rows do not start on 16-byte boundaries
+template <typename T, int N>
+struct alignas(N * sizeof(T)) OpVec {
+    T v[N];
+};
+template <typename T, int N>
+static __device__ __forceinline__ void op_load(const T* p, float (&to)[N]) {
+    const OpVec<T, N> u = *reinterpret_cast<const OpVec<T, N>*>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i] = op_float(u.v[i]);
+}
+template <typename T, int N>
+static __device__ __forceinline__ void op_store(T* p, const float (&from)[N]) {
+    OpVec<T, N> u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) u.v[i] = op_round<T>(from[i]);
+    *reinterpret_cast<OpVec<T, N>*>(p) = u;
+}
+
+// sum over aligned groups of G lanes, the same bits in every lane (halves are added in a fixed order)
+template <int G>
+static __device__ __forceinline__ float op_group_sum(float v) {
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+static inline int op_type_size(int type) { return type == TB_TYPE_F32 ? 4 : type == TB_TYPE_F16 || type == TB_TYPE_BF16 ? 2 : 0; }
+
+#if defined(__GNUC__)
+__attribute__((format(printf, 4, 5)))
+#endif
+static inline int op_report(char* err, size_t err_len, int code, const char* fmt, ...) {
+    if (err && err_len) {
+        va_list ap;
+        va_start(ap, fmt);
+        vsnprintf(err, err_len, fmt, ap);
+        va_end(ap);
+    }
+    return code;
+}
+static inline int op_launched(char* err, size_t err_len) {
+    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) return TB_OK;
+    return op_report(err, err_len, e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver ? TB_ERR_NO_DEVICE : TB_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
+}
