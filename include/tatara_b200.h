@@ -251,7 +251,7 @@ int tb_ft_backward_static_scratch(const float* d_dft, const int32_t* d_indices, 
 
 /* ---- operators on the caller's device tensors ----------------------------------------------
  * No counterpart in the reference.  What a trainer with learned buckets needs beside the step: normalised rows in
- * front of a gate and the choice of a bucket (expert) per row with a balance loss.  ALL tensor pointers are DEVICE memory of the
+ * front of a gate, the choice of a bucket (expert) per row with a balance loss, and the matrix optimizer of hidden weights.  ALL tensor pointers are DEVICE memory of the
  * current device, owned by the caller; the work is enqueued on `stream` (a cudaStream_t, NULL = default stream) and not synchronised; nothing is
  * allocated and nothing is kept between calls, so calls on different streams may overlap as long as each has its own workspace.
  * A failed call returns a code, writes the reason to err (may be NULL) and launches nothing when an argument is refused.
@@ -286,6 +286,29 @@ int tb_route_forward(const void* d_logits, int64_t stride, int type, int64_t row
 int tb_route_backward(const void* d_logits, int64_t stride, int type, int64_t rows, int experts, int k, int renormalise, const uint8_t* d_mask,
                       const int32_t* d_index, const float* d_gate, const float* d_dgate, const int32_t* d_counts, const int32_t* d_rows,
                       const float* d_dlosses, void* d_dlogits, int64_t dstride, void* stream, char* err, size_t err_len);
+
+/* Newton-Schulz orthogonalisation of every matrix of a batch: X = x / (|x| + eps) (Frobenius norm), then `steps` (1 .. 32) times
+ * X = (a I + b A + c A^2) X with A = X X^T taken over the shorter side; coefficients = {a, b, c} on the HOST.  x and out have the same
+ * type and may be the same memory; x_batch and out_batch are the strides between matrices.  Coefficients for which a singular value of at most 1
+ * could grow beyond 4 (or |a| + |b| s^2 + |c| s^4 beyond 31) are refused.  fp32 and fp16: products of 22-bit operands (64-bit where the shorter
+ * side is at most 64); bf16: 11-bit operands; fp32 sums.  A matrix with an infinity or a NaN comes out NaN. */
+int64_t tb_orthogonalise_workspace(int type, int batch, int rows, int cols);
+int tb_orthogonalise(const void* d_x, int64_t x_batch, int64_t x_stride, int type, int batch, int rows, int cols, int steps,
+                     const float* coefficients, float eps, void* d_out, int64_t out_batch, int64_t out_stride, void* d_work,
+                     int64_t work_bytes, void* stream, char* err, size_t err_len);
+
+/* The Muon step of a batch of weight matrices, all contiguous [batch, rows, cols]: m' = beta m + g; u = nesterov ? g + beta m' : m';
+ * w' = clamp(w (1 - lr weight_decay) - lr scale orthogonalise(u), -clip, clip).  w, m and their results are fp32 (each result may be its
+ * input's memory), g any type. */
+typedef struct tb_muon {
+    int32_t struct_size; /* sizeof(tb_muon) of the caller */
+    int32_t steps, nesterov;
+    float a, b, c, eps;  /* of the orthogonalisation */
+    float lr, beta, weight_decay, scale, clip; /* clip: INFINITY for none */
+} tb_muon;
+int64_t tb_muon_step_workspace(int batch, int rows, int cols);
+int tb_muon_step(const tb_muon* cfg, const float* d_w, const float* d_m, const void* d_g, int g_type, int batch, int rows, int cols,
+                 float* d_w_out, float* d_m_out, void* d_work, int64_t work_bytes, void* stream, char* err, size_t err_len);
 
 /* ---- inputs: PackedSfenValue records -> step inputs, on the device ---------------------
  * Decodes 40-byte records (crates/shogi-format/src/packed_sfen.rs:387-448) and extracts the active

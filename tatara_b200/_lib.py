@@ -46,6 +46,11 @@ class MicrobenchResult(C.Structure):
     _fields_ = [("fwd_ms", f), ("bwd_ms", f), ("adam_ms", f), ("fwd_slice_ms", f), ("bwd_slice_ms", f), ("iters", i32)]
 
 
+class Muon(C.Structure):
+    _fields_ = [("struct_size", i32), ("steps", i32), ("nesterov", i32), ("a", f), ("b", f), ("c", f), ("eps", f), ("lr", f), ("beta", f),
+                ("weight_decay", f), ("scale", f), ("clip", f)]
+
+
 class Batch(C.Structure):
     _fields_ = [
         ("n_pos", i32), ("stm_indices", vp), ("nstm_indices", vp), ("nnz", vp), ("bucket_idx", vp), ("score", vp),
@@ -102,6 +107,10 @@ SIGNATURES = {
     "tb_route_forward_workspace": (i64, [i64, C.c_int]),
     "tb_route_forward": (C.c_int, [vp, i64, C.c_int, i64, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp, C.c_char_p, C.c_size_t]),
     "tb_route_backward": (C.c_int, [vp, i64, C.c_int, i64, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp, C.c_char_p, C.c_size_t]),
+    "tb_orthogonalise_workspace": (i64, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    "tb_orthogonalise": (C.c_int, [vp, i64, i64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(f), f, vp, i64, i64, vp, i64, vp, C.c_char_p, C.c_size_t]),
+    "tb_muon_step_workspace": (i64, [C.c_int, C.c_int, C.c_int]),
+    "tb_muon_step": (C.c_int, [C.POINTER(Muon), vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp, i64, vp, C.c_char_p, C.c_size_t]),
     "tb_nccl_unique_id": (C.c_int, [vp]),
     "tb_device_count": (C.c_int, []),
     "tb_version": (C.c_char_p, []),

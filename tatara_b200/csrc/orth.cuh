@@ -1,0 +1,60 @@
+// Newton-Schulz orthogonalisation and the Muon step: what its two paths (orth_kernels.cu, orth_tc.cu) share.
+//
+//   u = the matrix (orthogonalise), or the momentum m' = beta m + g or g + beta m' (Muon, Nesterov)
+//   X = u / (|u| + eps), transposed to n <= m;  `steps` times: A = X X^T, Q = a I + b A + c A^2, X = Q X
+//   out = X (orthogonalise), or w' = clamp(w * w_mul - step * X) (Muon)
+#pragma once
+#include "op_common.cuh"
+
+struct OrthIo {
+    const void* g;                // [batch][rows][cols]
+    int64_t g_batch, g_stride;
+    const float* m;               // Muon: momentum, contiguous like w; NULL for orthogonalise
+    float* m_out;
+    float beta;
+    int nesterov;
+    void* out;                    // orthogonalise: of g's type; Muon: the new weights, fp32
+    int64_t out_batch, out_stride;
+    const float* w;
+    float w_mul, step, clip;
+    int rows, cols, batch;
+};
+struct OrthPoly {
+    int steps;
+    float a, b, c, eps;
+};
+
+// element (r, c) of u; FIRST: the call that updates the momentum (once per element, before any other)
+template <typename T, bool FIRST>
+static __device__ __forceinline__ float orth_load(const OrthIo& io, int b, int64_t r, int64_t c) {
+    const float g = op_float(static_cast<const T*>(io.g)[b * io.g_batch + r * io.g_stride + c]);
+    if (!io.m) return g;
+    const int64_t at = ((int64_t)b * io.rows + r) * io.cols + c;
+    float m;
+    if (FIRST) {
+        m = fmaf(io.beta, io.m[at], g);
+        io.m_out[at] = m;
+    } else {
+        m = io.m_out[at];
+    }
+    return io.nesterov ? fmaf(io.beta, m, g) : m;
+}
+template <typename T>
+static __device__ __forceinline__ void orth_store(const OrthIo& io, int b, int64_t r, int64_t c, float x) {
+    const int64_t at = b * io.out_batch + r * io.out_stride + c;
+    if (!io.m) {
+        static_cast<T*>(io.out)[at] = op_round<T>(x);
+        return;
+    }
+    float w = fmaf(-io.step, x, io.w[at] * io.w_mul);
+    w = w < -io.clip ? -io.clip : w;  // comparisons keep a NaN
+    w = w > io.clip ? io.clip : w;
+    static_cast<float*>(io.out)[at] = w;
+}
+
+// orth_kernels.cu: n <= ORTH_SMALL_N
+#define ORTH_SMALL_N 64
+void launch_orth_small(cudaStream_t s, const OrthIo& io, const OrthPoly& p, int type);
+// orth_tc.cu: any size; limbs: fp16 numbers that hold an operand (1: 11 bits, 2: 22 bits)
+int64_t orth_tc_workspace(int batch, int rows, int cols, int limbs);
+void launch_orth_tc(cudaStream_t s, const OrthIo& io, const OrthPoly& p, int type, int limbs, void* work);

@@ -1,0 +1,528 @@
+// Newton-Schulz steps of matrices with a short side above 64: products on the 5th-generation tensor cores.
+//
+// Operands are fp16 "limbs" of numbers scaled by 2^11: one limb holds 11 bits of a number, two hold 22 (the second is the first one's
+// rounding error).  With two limbs a product is three products of limbs (high high, high low, low high; low low is below 2^-22)
+// into one fp32 accumulator, which keeps the steps at fp32 accuracy at a third of the fp16 rate; fp32 on the CUDA cores has a thirtieth.
+// With one limb the roundings (2^-12 of an element, a few times over) stay below those of a bf16 result (2^-9).  Numbers up to 32
+// fit; the entry points refuse coefficients that could leave that range.
+//
+// All matrices live in the workspace as 16 KB tiles of 128 rows x 64 columns, stored as the tensor cores want them in shared memory
+// (rows of 128 bytes, their 16-byte pieces permuted by the row's last three bits), so every operand is fetched by untiled bulk copies
+// and nothing is laid out twice:
+//   Gram    A = X X^T             X's tiles as rows (K along the columns), both sides
+//   square  Q = a I + b A + c A A A is symmetric: its rows serve as columns
+//   apply   X = Q X               X's tiles as K x N operands (N along the columns): the same bytes, the other major
+// Gram and square are symmetric: only tiles on and below the diagonal are computed, the epilogue stores the mirrored tile too.
+// a I is part of Q, so that no product has to add its own input.
+//
+// One thread issues the bulk copies into a ring of stages, one the MMAs, eight warps read the accumulators from tensor memory.  The tensor
+// cores truncate when they add to an accumulator: 2.5e-5 of the result after five steps of K = 1000 with two limbs.  So the accumulator
+// changes every four chunks of K, and the warps add what it held to their registers, rounded to nearest, while the next one fills.
+// Every wait is bounded; where one runs out the block's results become NaN, and so the output.
+#include "orth.cuh"
+
+namespace {
+
+#define OT_TILE 16384           // bytes of a tile of 128 x 64 fp16
+#define OT_SCALE 2048.0f
+#define OT_UNSCALE (1.0f / (2048.0f * 2048.0f))
+#define OT_WAIT_LIMIT (1 << 20)
+#define OT_NORM_BLOCKS 64       // partial sums of squares per matrix
+enum { OT_GRAM = 0, OT_SQUARE = 1, OT_APPLY = 2, OT_LAST = 3 };
+
+__device__ __forceinline__ unsigned ot_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void ot_bar_init(unsigned bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ bool ot_wait(unsigned bar, unsigned parity) {
+    for (int i = 0; i < OT_WAIT_LIMIT; ++i) {
+        unsigned ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ void ot_expect(unsigned bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void ot_copy(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// the same where blocks of the cluster arrive
+__device__ __forceinline__ bool ot_wait_cluster(unsigned bar, unsigned parity) {
+    for (int i = 0; i < OT_WAIT_LIMIT; ++i) {
+        unsigned ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+// arrives at the same barrier of block `rank` of the cluster
+__device__ __forceinline__ void ot_arrive_at(unsigned bar, unsigned rank) {
+    asm volatile(
+        "{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %0, %1;\n\tmbarrier.arrive.release.cluster.shared::cluster.b64 _, [at];\n\t}" ::"r"(bar), "r"(rank)
+        : "memory");
+}
+__device__ __forceinline__ void ot_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void ot_store(void* dst, unsigned src, unsigned bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void ot_mma(unsigned d, unsigned long long da, unsigned long long db, unsigned idesc, unsigned accumulate) {
+    if (CTAS == 2)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(da), "l"(db),
+                     "r"(idesc), "r"(accumulate)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(da), "l"(db),
+                     "r"(idesc), "r"(accumulate)
+                     : "memory");
+}
+// arrives at the barrier (of both blocks) when the MMAs issued so far are done
+template <int CTAS>
+__device__ __forceinline__ void ot_commit(unsigned bar) {
+    if (CTAS == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((unsigned short)3) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void ot_read32(unsigned taddr, unsigned (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
+        "%24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+          "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]),
+          "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// shared-memory matrix descriptor: 128-byte swizzle (2 at bit 61), version 1 (bit 46), offsets in 16 bytes
+__device__ __forceinline__ unsigned long long ot_desc(unsigned addr, unsigned lbo, unsigned sbo) {
+    return (unsigned long long)((addr & 0x3FFFFu) >> 4) | ((unsigned long long)(lbo >> 4) << 16) | ((unsigned long long)(sbo >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// limbs of x: hi + lo = x to 22 bits
+template <int LIMBS>
+__device__ __forceinline__ void ot_split(float x, __half (&h)[LIMBS]) {
+    h[0] = __float2half_rn(x);
+    if (LIMBS == 2) h[LIMBS - 1] = __float2half_rn(x - __half2float(h[0]));
+}
+// byte offset of element (row, col) in a 128 x 64 tile
+__device__ __forceinline__ int ot_at(int row, int col) { return row * 128 + ((((col >> 3) ^ row) & 7) << 4) + (col & 7) * 2; }
+
+// ---- the norm and the tiles of the first X ----------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(512) k_orth_norm(OrthIo io, double* __restrict__ partial) {
+    __shared__ double s_sum[16];
+    const int b = blockIdx.y;
+    double sum = 0.0;
+    for (int r = blockIdx.x; r < io.rows; r += gridDim.x)
+        for (int c = threadIdx.x; c < io.cols; c += 512) {
+            const double u = (double)orth_load<T, true>(io, b, r, c);
+            sum = fma(u, u, sum);
+        }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) sum += s_sum[w];
+        partial[b * OT_NORM_BLOCKS + blockIdx.x] = sum;
+    }
+}
+
+// one tile per block: X0 = u / (|u| + eps), n x m with n <= m, zeros beyond both
+template <typename T, int LIMBS>
+__global__ void __launch_bounds__(256) k_orth_pack(OrthIo io, float eps, const double* __restrict__ partial, int n_partial, uint8_t* __restrict__ x, int64_t limb_bytes) {
+    __shared__ __align__(128) uint8_t s_tile[LIMBS][OT_TILE];
+    __shared__ double s_inv;
+    const int b = blockIdx.z;
+    const bool tall = io.rows > io.cols;
+    const int n = tall ? io.cols : io.rows, m = tall ? io.rows : io.cols;
+    if (threadIdx.x < 32) {
+        double v = 0.0;
+        for (int i = threadIdx.x; i < n_partial; i += 32) v += partial[b * OT_NORM_BLOCKS + i];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (threadIdx.x == 0) s_inv = (double)OT_SCALE / (sqrt(v) + (double)eps);
+    }
+    __syncthreads();
+    const double inv = s_inv;
+    const int i0 = blockIdx.y * 128, j0 = blockIdx.x * 64;
+    for (int e = threadIdx.x; e < 128 * 64; e += 256) {
+        const int i = tall ? e % 128 : e / 64, j = tall ? e / 128 : e % 64;
+        float v = 0.0f;
+        if (i0 + i < n && j0 + j < m) v = (float)((double)(tall ? orth_load<T, false>(io, b, j0 + j, i0 + i) : orth_load<T, false>(io, b, i0 + i, j0 + j)) * inv);
+        __half h[LIMBS];
+        ot_split<LIMBS>(v, h);
+#pragma unroll
+        for (int l = 0; l < LIMBS; ++l) *reinterpret_cast<__half*>(&s_tile[l][ot_at(i, j)]) = h[l];
+    }
+    __syncthreads();
+    uint8_t* to = x + (int64_t)b * LIMBS * limb_bytes + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * OT_TILE;
+#pragma unroll
+    for (int l = 0; l < LIMBS; ++l)
+        for (int e = threadIdx.x; e < OT_TILE / 16; e += 256)
+            *reinterpret_cast<uint4*>(to + l * limb_bytes + e * 16) = *reinterpret_cast<const uint4*>(&s_tile[l][e * 16]);
+}
+
+// ---- the products -----------------------------------------------------------------------------------------------------
+struct OtGemm {
+    const uint8_t* a;    // left operand's tiles [batch][limbs][rows / 128][chunks]
+    const uint8_t* b;    // right operand's tiles
+    uint8_t* out;        // the result's tiles
+    int64_t a_limb, b_limb, out_limb;  // bytes of a limb
+    int chunks;          // K / 64
+    int row_tiles;       // of the result, 128 CTAS each
+    int col_tiles;       // of the result, 128 CTAS each; the result's rows (apply: and b's) hold 2 CTAS col_tiles tiles
+    float ca, cb, cc;    // square: a I + b A + c A A
+};
+
+template <int LIMBS>
+struct OtShape {
+    static constexpr int STAGE = LIMBS * 2 * OT_TILE;
+    static constexpr int STAGES = LIMBS == 2 ? 3 : 6;
+    static constexpr int SMEM = STAGE * STAGES + 1024;
+    // chunks of 64 whose products share an accumulator
+    static constexpr int DRAIN = LIMBS == 2 ? 4 : 1 << 30;
+};
+
+// CTAS = 1: a block computes 128 x 128.  CTAS = 2: a cluster of two blocks computes 256 x 256 with cta_group::2 MMAs: each block holds 128 rows
+// of the left operand, 128 columns of the right one and 128 x 256 accumulators; the even block issues the MMAs.
+// Warps 0-7 read the accumulators (warp w: lanes 32 (w % 4) .. of them, columns 64 CTAS (w / 4) ..), warp 8 copies, warp 9 issues the MMAs.
+template <int KIND, int LIMBS, int CTAS, typename T>
+__global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
+    using S = OtShape<LIMBS>;
+    constexpr int TN = 128 * CTAS, COLS = 64 * CTAS;  // accumulator columns of a block, of a thread
+    constexpr bool SYM = KIND == OT_GRAM || KIND == OT_SQUARE;
+    extern __shared__ uint8_t s_raw[];
+    __shared__ __align__(8) unsigned long long s_full[S::STAGES], s_peer[S::STAGES], s_empty[S::STAGES], s_acc_full[2], s_acc_empty[2];
+    __shared__ unsigned s_tmem;
+    __shared__ int s_failed;
+    uint8_t* s_dyn = s_raw + ((1024u - (ot_smem(s_raw) & 1023u)) & 1023u);
+    const unsigned ring = ot_smem(s_dyn);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, batch = blockIdx.z;
+    const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, tile = blockIdx.x / CTAS;
+    int ti, tj;
+    if (SYM) {  // tiles on and below the diagonal, row by row
+        ti = (int)((sqrtf(8.0f * (float)tile + 1.0f) - 1.0f) * 0.5f);
+        while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
+        while (ti * (ti + 1) / 2 > tile) --ti;
+        tj = tile - ti * (ti + 1) / 2;
+    } else {
+        ti = tile % g.row_tiles;
+        tj = tile / g.row_tiles;
+    }
+    const bool same = SYM && ti == tj;              // one operand serves as both
+    const int row_tile = ti * CTAS + rank;          // this block's rows, in 128s
+    const int width = 2 * CTAS * g.col_tiles;       // tiles in a row of the result
+    if (tid == 0) {
+        for (int s = 0; s < S::STAGES; ++s) {
+            ot_bar_init(ot_smem(&s_full[s]), 1);
+            ot_bar_init(ot_smem(&s_peer[s]), 1);
+            ot_bar_init(ot_smem(&s_empty[s]), 1);
+        }
+        for (int q = 0; q < 2; ++q) {
+            ot_bar_init(ot_smem(&s_acc_full[q]), 1);
+            ot_bar_init(ot_smem(&s_acc_empty[q]), 8 * CTAS);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        s_failed = 0;
+    }
+    if (warp == 9) {
+        if (CTAS == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ot_smem(&s_tmem)), "r"(2 * TN) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ot_smem(&s_tmem)), "r"(2 * TN) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (CTAS == 2) ot_cluster_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = s_tmem;
+    const int chunks = g.chunks, rounds = (chunks + S::DRAIN - 1) / S::DRAIN;
+    float acc[COLS];
+
+    if (warp == 8) {
+        if (lane == 0) {
+            const uint8_t* a = g.a + (int64_t)batch * LIMBS * g.a_limb + (int64_t)row_tile * chunks * OT_TILE;
+            const uint8_t* b = g.b + (int64_t)batch * LIMBS * g.b_limb;
+            const int col_tile = tj * CTAS + rank;  // this block's columns of the right operand
+            bool ok = true;
+            int k = 0;
+            for (; k < chunks; ++k) {
+                const int s = k % S::STAGES;
+                if (k >= S::STAGES && !ot_wait(ot_smem(&s_empty[s]), (unsigned)((k / S::STAGES - 1) & 1))) {
+                    ok = false;
+                    break;
+                }
+                const unsigned bar = ot_smem(&s_full[s]), to = ring + s * S::STAGE;
+                ot_expect(bar, same ? LIMBS * OT_TILE : 2 * LIMBS * OT_TILE);
+#pragma unroll
+                for (int l = 0; l < LIMBS; ++l) {
+                    ot_copy(to + l * OT_TILE, a + l * g.a_limb + (int64_t)k * OT_TILE, OT_TILE, bar);
+                    if (same) continue;
+                    const unsigned tb = to + (LIMBS + l) * OT_TILE;
+                    if (SYM) {
+                        ot_copy(tb, b + l * g.b_limb + ((int64_t)col_tile * chunks + k) * OT_TILE, OT_TILE, bar);
+                    } else {  // rows 64 k .. 64 k + 63 of two column tiles
+                        const uint8_t* p = b + l * g.b_limb + ((int64_t)(k >> 1) * width + 2 * col_tile) * OT_TILE + (k & 1) * (OT_TILE / 2);
+                        ot_copy(tb, p, OT_TILE / 2, bar);
+                        ot_copy(tb + OT_TILE / 2, p + OT_TILE, OT_TILE / 2, bar);
+                    }
+                }
+            }
+            if (!ok) {  // the copies in flight land before the block ends
+                atomicExch(&s_failed, 1);
+                for (int q = k < S::STAGES ? 0 : k - S::STAGES; q < k; ++q) ot_wait(ot_smem(&s_full[q % S::STAGES]), (unsigned)((q / S::STAGES) & 1));
+            }
+        }
+    } else if (warp == 9) {
+        if (lane == 0 && rank == 0) {
+            // fp32 accumulator (1 at bit 4), fp16 operands, N / 8 at bit 17, M / 16 at bit 24; apply: the right operand is N-major (bit 16)
+            constexpr unsigned IDESC = (1u << 4) | (SYM ? 0u : 1u << 16) | ((unsigned)(TN / 8) << 17) | ((unsigned)(8 * CTAS) << 24);
+            bool ok = true;
+            for (int r = 0, k = 0; r < rounds && ok; ++r) {
+                const unsigned d = tmem + (unsigned)((r & 1) * TN);
+                if (r >= 2) ok = ot_wait_cluster(ot_smem(&s_acc_empty[r & 1]), (unsigned)((r / 2 - 1) & 1));
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int q0 = k; ok && k < chunks && k < q0 + S::DRAIN; ++k) {
+                    const int s = k % S::STAGES;
+                    const unsigned parity = (unsigned)((k / S::STAGES) & 1);
+                    ok = ot_wait(ot_smem(&s_full[s]), parity) && (CTAS == 1 || ot_wait_cluster(ot_smem(&s_peer[s]), parity));
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const unsigned at = ring + s * S::STAGE, bt = same ? at : at + LIMBS * OT_TILE;
+#pragma unroll
+                    for (int q = 0; q < (LIMBS == 2 ? 3 : 1); ++q) {
+                        const unsigned la = at + (q == 2 ? OT_TILE : 0), lb = bt + (q == 1 ? OT_TILE : 0);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            // K-major: 32 bytes along the row, 8-row groups 1024 bytes apart.  N-major: 16 rows of 128 bytes, 8-row groups
+                            // 1024 bytes apart, the next 64 columns 8 KB further
+                            const unsigned long long da = ot_desc(la + 32 * j, 16, 1024);
+                            const unsigned long long db = SYM ? ot_desc(lb + 32 * j, 16, 1024) : ot_desc(lb + 2048 * j, OT_TILE / 2, 1024);
+                            ot_mma<CTAS>(d, da, db, IDESC, (k > q0 || q > 0 || j > 0) ? 1u : 0u);
+                        }
+                    }
+                    ot_commit<CTAS>(ot_smem(&s_empty[s]));
+                }
+                ot_commit<CTAS>(ot_smem(&s_acc_full[r & 1]));
+            }
+            if (!ok) atomicExch(&s_failed, 1);
+        } else if (lane == 0) {
+            // the odd block: tells the even one that its operands are there
+            for (int k = 0; k < chunks; ++k) {
+                const int s = k % S::STAGES;
+                if (!ot_wait(ot_smem(&s_full[s]), (unsigned)((k / S::STAGES) & 1))) {
+                    atomicExch(&s_failed, 1);
+                    break;
+                }
+                ot_arrive_at(ot_smem(&s_peer[s]), 0);
+            }
+        }
+    } else {
+        const unsigned taddr = tmem + ((unsigned)((warp & 3) * 32) << 16) + (unsigned)((warp >> 2) * COLS);
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) acc[c] = 0.0f;
+        for (int r = 0; r < rounds; ++r) {
+            const bool ok = ot_wait(ot_smem(&s_acc_full[r & 1]), (unsigned)((r / 2) & 1));
+            if (!__all_sync(0xffffffffu, ok)) {
+                if (lane == 0) atomicExch(&s_failed, 1);
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int c0 = 0; c0 < COLS; c0 += 32) {
+                unsigned v[32];
+                ot_read32(taddr + (unsigned)((r & 1) * TN + c0), v);
+#pragma unroll
+                for (int c = 0; c < 32; ++c) acc[c0 + c] += __uint_as_float(v[c]);
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                if (CTAS == 2) ot_arrive_at(ot_smem(&s_acc_empty[r & 1]), 0);
+                else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ot_smem(&s_acc_empty[r & 1])) : "memory");
+            }
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (CTAS == 2) ot_cluster_sync();  // the other block's MMAs are done with this block's memory, and no signal is under way
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 9) {
+        if (CTAS == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TN) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TN) : "memory");
+    }
+    if (warp >= 8) return;
+
+    // Epilogue by two groups of 128 threads, a row each, in rounds of 64 columns through the group's part of shared memory.
+    const float poison = s_failed ? __int_as_float(0x7fc00000) : 0.0f;
+    const int group = warp >> 2, row = tid & 127;
+    uint8_t* direct = s_dyn + group * (2 * LIMBS * OT_TILE);      // [limb] tile
+    uint8_t* mirror = direct + LIMBS * OT_TILE;                   // [limb][column half] half a tile: 64 rows
+    float* flat = reinterpret_cast<float*>(s_dyn + group * 40960);  // OT_LAST: [128][65]
+#pragma unroll
+    for (int h = 0; h < CTAS; ++h) {
+        const int col_tile = tj * 2 * CTAS + group * CTAS + h;    // the round's columns, in 64s
+        if (h) asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+        if (KIND == OT_LAST) {
+#pragma unroll
+            for (int c = 0; c < 64; ++c) flat[row * 65 + c] = acc[64 * h + c] * OT_UNSCALE + poison;
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+            const bool tall = io.rows > io.cols;
+            const int n = tall ? io.cols : io.rows, m = tall ? io.rows : io.cols;
+            // 128 (64) neighbours in memory at a time
+            for (int e = 0; e < 64; ++e) {
+                const int r = tall ? row : 2 * e + (row >> 6), c = tall ? e : row & 63, i = row_tile * 128 + r, j = col_tile * 64 + c;
+                if (i >= n || j >= m) continue;
+                if (tall) orth_store<T>(io, batch, j, i, flat[r * 65 + c]); else orth_store<T>(io, batch, i, j, flat[r * 65 + c]);
+            }
+        } else {
+            const uint8_t* old = KIND == OT_SQUARE ? g.a + (int64_t)batch * LIMBS * g.a_limb + ((int64_t)row_tile * chunks + col_tile) * OT_TILE : nullptr;
+#pragma unroll
+            for (int c0 = 0; c0 < 64; c0 += 8) {
+                float x[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) x[c] = acc[64 * h + c0 + c] * OT_UNSCALE + poison;
+                if (KIND == OT_SQUARE) {
+                    float a[8];
+#pragma unroll
+                    for (int l = 0; l < LIMBS; ++l) {
+                        float t[8];
+                        op_load<__half, 8>(reinterpret_cast<const __half*>(old + l * g.a_limb + ot_at(row, c0)), t);
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) a[c] = l ? a[c] + t[c] : t[c];
+                    }
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        x[c] = fmaf(g.cc, x[c], fmaf(g.cb / OT_SCALE, a[c], row_tile * 128 + row == col_tile * 64 + c0 + c ? g.ca : 0.0f));
+                }
+                OpVec<__half, 8> piece[LIMBS];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    __half s[LIMBS];
+                    ot_split<LIMBS>(x[c] * OT_SCALE, s);
+#pragma unroll
+                    for (int l = 0; l < LIMBS; ++l) {
+                        piece[l].v[c] = s[l];
+                        if (SYM && !same) *reinterpret_cast<__half*>(mirror + (l * 2 + (row >> 6)) * (OT_TILE / 2) + ot_at(c0 + c, row & 63)) = s[l];
+                    }
+                }
+#pragma unroll
+                for (int l = 0; l < LIMBS; ++l) *reinterpret_cast<OpVec<__half, 8>*>(direct + l * OT_TILE + ot_at(row, c0)) = piece[l];
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+            if (row == 0) {
+                uint8_t* o = g.out + (int64_t)batch * LIMBS * g.out_limb;
+#pragma unroll
+                for (int l = 0; l < LIMBS; ++l) {
+                    ot_store(o + l * g.out_limb + ((int64_t)row_tile * width + col_tile) * OT_TILE, ot_smem(direct + l * OT_TILE), OT_TILE);
+                    if (SYM && !same) {
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+                            ot_store(o + l * g.out_limb + ((int64_t)(col_tile >> 1) * width + 2 * row_tile + q) * OT_TILE + (col_tile & 1) * (OT_TILE / 2),
+                                     ot_smem(mirror + (l * 2 + q) * (OT_TILE / 2)), OT_TILE / 2);
+                    }
+                }
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+            }
+        }
+    }
+}
+
+struct OtPlan {
+    int ctas, n_pad, m_pad;
+    int64_t x_limb, a_limb;                  // bytes of a limb
+    int64_t x0, x1, a, q, total;             // offsets in the workspace
+};
+OtPlan ot_plan(int batch, int rows, int cols, int limbs) {
+    const int64_t n = rows < cols ? rows : cols, m = rows < cols ? cols : rows;
+    OtPlan p;
+    // pairs of blocks where their larger tiles still fill the chip
+    const int64_t big = (n + 255) / 256;
+    p.ctas = batch * big * (big + 1) / 2 >= 64 ? 2 : 1;
+    const int64_t pad = 128 * p.ctas;
+    p.n_pad = (int)((n + pad - 1) / pad * pad);
+    p.m_pad = (int)((m + pad - 1) / pad * pad);
+    p.x_limb = (int64_t)p.n_pad * p.m_pad * 2;
+    p.a_limb = (int64_t)p.n_pad * p.n_pad * 2;
+    p.x0 = ((int64_t)batch * OT_NORM_BLOCKS * 8 + 127) / 128 * 128;
+    p.x1 = p.x0 + p.x_limb * limbs * batch;
+    p.a = p.x1 + p.x_limb * limbs * batch;
+    p.q = p.a + p.a_limb * limbs * batch;
+    p.total = p.q + p.a_limb * limbs * batch;
+    return p;
+}
+
+template <int KIND, int LIMBS, int CTAS, typename T>
+void ot_gemm(cudaStream_t s, const OtGemm& g, const OrthIo& io) {
+    using S = OtShape<LIMBS>;
+    cudaFuncSetAttribute(k_orth_gemm<KIND, LIMBS, CTAS, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    const int tiles = KIND == OT_GRAM || KIND == OT_SQUARE ? g.row_tiles * (g.row_tiles + 1) / 2 : g.row_tiles * g.col_tiles;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * CTAS), 1, (unsigned)io.batch);
+    cfg.blockDim = dim3(320);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CTAS;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, k_orth_gemm<KIND, LIMBS, CTAS, T>, g, io);
+}
+
+template <typename T, int LIMBS, int CTAS>
+void ot_steps(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, uint8_t* work, const OtPlan& p) {
+    uint8_t *x = work + p.x0, *y = work + p.x1, *a = work + p.a, *q = work + p.q;
+    const int rt = p.n_pad / (128 * CTAS), ct = p.m_pad / (128 * CTAS);
+    for (int k = 0; k < poly.steps; ++k) {
+        ot_gemm<OT_GRAM, LIMBS, CTAS, float>(s, {x, x, a, p.x_limb, p.x_limb, p.a_limb, p.m_pad / 64, rt, rt, 0.f, 0.f, 0.f}, io);
+        ot_gemm<OT_SQUARE, LIMBS, CTAS, float>(s, {a, a, q, p.a_limb, p.a_limb, p.a_limb, p.n_pad / 64, rt, rt, poly.a, poly.b, poly.c}, io);
+        const OtGemm g = {q, x, y, p.a_limb, p.x_limb, p.x_limb, p.n_pad / 64, rt, ct, 0.f, 0.f, 0.f};
+        if (k + 1 < poly.steps) ot_gemm<OT_APPLY, LIMBS, CTAS, float>(s, g, io); else ot_gemm<OT_LAST, LIMBS, CTAS, T>(s, g, io);
+        uint8_t* z = x;
+        x = y;
+        y = z;
+    }
+}
+
+template <typename T, int LIMBS>
+void ot_run(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, uint8_t* work) {
+    const OtPlan p = ot_plan(io.batch, io.rows, io.cols, LIMBS);
+    double* partial = reinterpret_cast<double*>(work);
+    const int blocks = io.rows < OT_NORM_BLOCKS ? io.rows : OT_NORM_BLOCKS;
+    k_orth_norm<T><<<dim3((unsigned)blocks, (unsigned)io.batch), 512, 0, s>>>(io, partial);
+    k_orth_pack<T, LIMBS><<<dim3((unsigned)(p.m_pad / 64), (unsigned)(p.n_pad / 128), (unsigned)io.batch), 256, 0, s>>>(io, poly.eps, partial, blocks, work + p.x0, p.x_limb);
+    if (p.ctas == 2) ot_steps<T, LIMBS, 2>(s, io, poly, work, p); else ot_steps<T, LIMBS, 1>(s, io, poly, work, p);
+}
+
+}  // namespace
+
+int64_t orth_tc_workspace(int batch, int rows, int cols, int limbs) { return ot_plan(batch, rows, cols, limbs).total; }
+
+void launch_orth_tc(cudaStream_t s, const OrthIo& io, const OrthPoly& p, int type, int limbs, void* work) {
+    uint8_t* w = static_cast<uint8_t*>(work);
+    if (type == TB_TYPE_F32) ot_run<float, 2>(s, io, p, w);
+    else if (type == TB_TYPE_F16) ot_run<__half, 2>(s, io, p, w);
+    else if (limbs == 2) ot_run<__nv_bfloat16, 2>(s, io, p, w);
+    else ot_run<__nv_bfloat16, 1>(s, io, p, w);
+}

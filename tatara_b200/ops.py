@@ -1,4 +1,5 @@
-"""Operators on torch CUDA tensors for trainers with learned buckets: layer norm, routing with a balance loss.
+"""Operators on torch CUDA tensors for trainers with learned buckets: layer norm, routing with a balance loss, Newton-Schulz
+orthogonalisation and the Muon step.
 
 Thin wrappers over the entry points of libtatara_b200.so that work on the caller's device tensors: they check the arguments, take
 outputs and workspaces from torch's allocator and enqueue on torch's current stream of the tensors' device.  Nothing is
@@ -167,3 +168,70 @@ def route_backward(logits: torch.Tensor, routing: Routing, dgate: Optional[torch
         _call("tb_route_backward", logits.data_ptr(), stride, _TYPES[logits.dtype], rows, experts, k, renormalise, m, ix, g, dg, c, n, dl, out.data_ptr(),
               experts, stream)
     return out
+
+
+# ---- orthogonalisation ------------------------------------------------------------------------------------------------
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # of the quintic step: singular values end between 0.7 and 1.2
+
+
+def _matrices(t: torch.Tensor, name: str) -> Tuple[int, int, int, int, int]:
+    """Checks a [rows, cols] or [batch, rows, cols] tensor with adjacent columns; (batch, rows, cols, batch stride, row stride)."""
+    _need(isinstance(t, torch.Tensor) and t.is_cuda, "%s must be a CUDA tensor" % name)
+    _need(t.dtype in _TYPES, "%s must be float32, float16 or bfloat16 (got %s)" % (name, t.dtype))
+    _need(t.dim() in (2, 3), "%s must have two or three dimensions (got %d)" % (name, t.dim()))
+    rows, cols = t.shape[-2:]
+    batch = t.shape[0] if t.dim() == 3 else 1
+    _need(rows >= 1 and cols >= 1, "%s has no elements in a matrix" % name)
+    stride, step = t.stride()[-2:]
+    _need(cols == 1 or step == 1, "%s must have adjacent columns" % name)
+    stride = stride if rows > 1 else cols
+    _need(stride >= cols, "rows of %s overlap" % name)
+    return batch, rows, cols, t.stride(0) if batch > 1 else 0, stride
+
+
+def orthogonalise(x: torch.Tensor, *, steps: int = 5, coefficients: Tuple[float, float, float] = COEFFICIENTS, eps: float = 1e-7,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of x [rows, cols] or of every matrix of x [batch, rows, cols].
+
+    X = x / (|x| + eps), then `steps` times X = (a I + b A + c A^2) X with A = X X^T over the shorter side: singular values that are not
+    tiny end near 1, the singular vectors stay.  `out` may be x.
+    """
+    batch, rows, cols, xb, xs = _matrices(x, "x")
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    _need(out is None or (isinstance(out, torch.Tensor) and out.shape == x.shape and out.dtype == x.dtype and out.device == x.device), "out must match x")
+    _, _, _, yb, ys = _matrices(y, "out")
+    _need(len(coefficients) == 3, "three coefficients are needed")
+    kind = _TYPES[x.dtype]
+    with _On(x) as stream:
+        size = L.load().tb_orthogonalise_workspace(kind, batch, rows, cols)
+        work = torch.empty(size, dtype=torch.uint8, device=x.device) if size > 0 else None
+        _call("tb_orthogonalise", x.data_ptr(), xb, xs, kind, batch, rows, cols, steps, (C.c_float * 3)(*coefficients), eps, y.data_ptr(), yb, ys,
+              None if work is None else work.data_ptr(), max(size, 0), stream)
+    return y
+
+
+def muon_step(weight: torch.Tensor, momentum: torch.Tensor, grad: torch.Tensor, *, lr: float, beta: float = 0.95, nesterov: bool = True,
+              weight_decay: float = 0.0, scale: Optional[float] = None, clip: float = float("inf"), steps: int = 5,
+              coefficients: Tuple[float, float, float] = COEFFICIENTS, eps: float = 1e-7, weight_out: Optional[torch.Tensor] = None,
+              momentum_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """One Muon step of weight [rows, cols] or [batch, rows, cols] (float32, contiguous); returns (weight, momentum).
+
+    m' = beta m + grad, u = grad + beta m' (`nesterov`) or m', w' = clamp(w (1 - lr weight_decay) - lr scale orthogonalise(u), -clip, clip).
+    In place unless `weight_out` / `momentum_out` are given; `scale` defaults to sqrt(max(1, rows / cols)).  grad may have any type.
+    """
+    batch, rows, cols, _, _ = _matrices(weight, "weight")
+    shape = tuple(weight.shape)
+    w, m = _vector(weight, "weight", weight, shape), _vector(momentum, "momentum", weight, shape)
+    _need(isinstance(grad, torch.Tensor) and grad.dtype in _TYPES, "grad must be a float32, float16 or bfloat16 tensor")
+    g = _vector(grad, "grad", weight, shape, grad.dtype)
+    weight_out, momentum_out = weight if weight_out is None else weight_out, momentum if momentum_out is None else momentum_out
+    wo, mo = _vector(weight_out, "weight_out", weight, shape), _vector(momentum_out, "momentum_out", weight, shape)
+    if scale is None:
+        scale = max(1.0, rows / cols) ** 0.5
+    _need(len(coefficients) == 3, "three coefficients are needed")
+    cfg = L.Muon(C.sizeof(L.Muon), steps, nesterov, *coefficients, eps, lr, beta, weight_decay, scale, clip)
+    with _On(weight) as stream:
+        size = L.load().tb_muon_step_workspace(batch, rows, cols)
+        work = torch.empty(size, dtype=torch.uint8, device=weight.device) if size > 0 else None
+        _call("tb_muon_step", C.byref(cfg), w, m, g, _TYPES[grad.dtype], batch, rows, cols, wo, mo, None if work is None else work.data_ptr(), max(size, 0), stream)
+    return weight_out, momentum_out

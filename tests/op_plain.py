@@ -68,3 +68,29 @@ def route_objective(x, index, counts, n, k, renormalise, live, dgate, dlosses):
     n1 = max(n, 1)
     balance = x.shape[1] / (n1 * k) * (counts.double() * p.sum(0) / n1).sum()
     return (gate * dgate * ok).sum() + dlosses[0] * balance + dlosses[1] * (lse ** 2).sum() / n1
+
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalise(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+    """The definition, matrix by matrix."""
+    x = x.double()
+    if x.dim() == 2:
+        return orthogonalise(x[None], steps, coefficients, eps)[0]
+    tall = x.shape[1] > x.shape[2]
+    if tall:
+        x = x.transpose(1, 2)
+    x = x / (x.square().sum((1, 2), keepdim=True).sqrt() + eps)
+    a, b, c = coefficients
+    for _ in range(steps):
+        g = x @ x.transpose(1, 2)
+        x = a * x + (b * g + c * g @ g) @ x
+    return x.transpose(1, 2) if tall else x
+
+
+def muon_step(w, m, g, lr, beta, nesterov, weight_decay, scale, clip, steps=5):
+    w, m, g = w.double(), m.double(), g.double()
+    m = beta * m + g
+    o = orthogonalise(g + beta * m if nesterov else m, steps)
+    return (w * (1 - lr * weight_decay) - lr * scale * o).clamp(-clip, clip), m
