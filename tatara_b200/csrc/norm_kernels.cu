@@ -29,12 +29,28 @@ __device__ __forceinline__ float norm_row_sum(float v, float* buf, int warp_in_r
     return v;
 }
 
+// VEC columns of a weight or bias, in 16-byte accesses (one element at a time they cost four to eight times the L1 wavefronts of the row
+// itself: 24 -> 8 us for 10000 rows of 1000 fp16)
+template <int VEC>
+__device__ __forceinline__ void norm_columns(const float* __restrict__ p, int col, float none, float (&to)[VEC]) {
+    constexpr int STEP = VEC < 4 ? VEC : 4;
+#pragma unroll
+    for (int i = 0; i < VEC; i += STEP) {
+        float t[STEP];
+#pragma unroll
+        for (int k = 0; k < STEP; ++k) t[k] = none;
+        if (p) op_load<float, STEP>(p + col + i, t);
+#pragma unroll
+        for (int k = 0; k < STEP; ++k) to[i + k] = t[k];
+    }
+}
+
 // W warps per row, VEC adjacent columns per access, CH accesses per thread: a thread holds columns (c * 32 W + t) * VEC + i
 template <typename T, int W, int VEC, int CH>
-__global__ void __launch_bounds__(W == 1 ? 256 : W * 32)
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32)
 k_norm_forward(const T* __restrict__ x, int64_t x_stride, const float* __restrict__ weight, const float* __restrict__ bias, float eps,
                int64_t rows, int n, T* __restrict__ y, int64_t y_stride, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-    constexpr int RB = W == 1 ? 8 : 1;  // rows per block
+    constexpr int RB = W == 1 ? 4 : 1;  // rows per block
     __shared__ float s_sum[2][W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = W == 1 ? lane : threadIdx.x;
     const int64_t row = (int64_t)blockIdx.x * RB + (W == 1 ? warp : 0);
@@ -79,10 +95,8 @@ k_norm_forward(const T* __restrict__ x, int64_t x_stride, const float* __restric
         const int col = (c * 32 * W + t) * VEC;
         if (col >= n) continue;
         float w[VEC], b[VEC], o[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) w[i] = weight ? weight[col + i] : 1.0f;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) b[i] = bias ? bias[col + i] : 0.0f;
+        norm_columns<VEC>(weight, col, 1.0f, w);
+        norm_columns<VEC>(bias, col, 0.0f, b);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[i] = fmaf((v[c][i] - mean) * rstd, w[i], b[i]);
         op_store<T, VEC>(yr + col, o);
@@ -115,98 +129,125 @@ k_norm_forward_long(const T* __restrict__ x, int64_t x_stride, const float* __re
         yr[c] = op_round<T>(fmaf((op_float(xr[c]) - mean) * rstd, weight ? weight[c] : 1.0f, bias ? bias[c] : 0.0f));
 }
 
-// Backward: a block of W warps per row (W = 1: four rows side by side, a warp each) walks the rows block, block + grid, .. and keeps its
-// columns' weight and bias gradients in registers; partial: [2][blocks][n].
-template <typename T, int W, int VEC, int CH>
-__global__ void __launch_bounds__(W == 1 ? 128 : W * 32)
-k_norm_backward(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x, int64_t x_stride, const float* __restrict__ mean,
-                const float* __restrict__ rstd, const float* __restrict__ weight, int64_t rows, int n, T* __restrict__ dx, int64_t dx_stride,
+// Blocks of the backward pass that one SM holds: 24 warps of 80 registers.  fp16, 16384 x 768: 20.4 us; 30 warps of 64 (some spilled) 24.6, four rows
+// at a time in 96 registers 26.0, the next rows fetched ahead in 175 registers 34.
+constexpr int norm_backward_per_sm(int warps) {
+    const int w = warps == 1 ? 4 : warps;
+    return 24 / w < 1 ? 1 : 24 / w;
+}
+
+// Backward: a block of W warps per row (W = 1: four rows side by side, a warp each) takes R rows at a time, which shares one barrier, walks
+// down the rows and keeps its columns' weight and bias gradients in registers; partial: [2][blocks (W = 1: four times)][n].
+// fp32, 65536 x 1536: 175 us, 6.9 TB/s.
+template <typename T, int W, int VEC, int CH, int R>
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, norm_backward_per_sm(W))
+k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, const float* __restrict__ mean,
+                const float* __restrict__ rstd, const float* __restrict__ weight, int64_t rows, int n, T* dx, int64_t dx_stride,
                 float* __restrict__ partial) {
     constexpr int RB = W == 1 ? 4 : 1;
-    __shared__ float s_sum[4][W];
+    __shared__ float s_sum[2][2 * R][W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = W == 1 ? lane : threadIdx.x;
     float w[CH][VEC], aw[CH][VEC], ab[CH][VEC];
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int c = 0; c < CH; ++c) {
+        const int col = (c * 32 * W + t) * VEC;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int col = (c * 32 * W + t) * VEC + i;
-            w[c][i] = weight && col < n ? weight[col] : 1.0f;
-            aw[c][i] = ab[c][i] = 0.0f;
-        }
+        for (int i = 0; i < VEC; ++i) w[c][i] = aw[c][i] = ab[c][i] = 0.0f;
+        if (col < n) norm_columns<VEC>(weight, col, 1.0f, w[c]);
+    }
     const float inv_n = 1.0f / (float)n;
     int turn = 0;
-    for (int64_t row = (int64_t)blockIdx.x * RB + (W == 1 ? warp : 0); row < rows; row += (int64_t)gridDim.x * RB, turn ^= 2) {
-        const T *xr = x + row * x_stride, *gr = dy + row * dy_stride;
-        float xv[CH][VEC], gv[CH][VEC];
+    for (int64_t first = ((int64_t)blockIdx.x * RB + (W == 1 ? warp : 0)) * R; first < rows; first += (int64_t)gridDim.x * RB * R, turn ^= 1) {
+        OpRaw<T, VEC> xv[R][CH], gv[R][CH];
+        float mu[R], r[R], s1[R], s2[R];
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int col = (c * 32 * W + t) * VEC;
-            if (col < n) {
-                op_load<T, VEC>(xr + col, xv[c]);
-                op_load<T, VEC>(gr + col, gv[c]);
+        for (int q = 0; q < R; ++q) {
+            const bool in = first + q < rows;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int col = (c * 32 * W + t) * VEC;
+                if (in && col < n) {
+                    xv[q][c].load(x + (first + q) * x_stride + col);
+                    gv[q][c].load(dy + (first + q) * dy_stride + col);
+                } else {
+                    xv[q][c].zero();
+                    gv[q][c].zero();
+                }
             }
+            mu[q] = in ? mean[first + q] : 0.0f;
+            r[q] = in ? rstd[first + q] : 0.0f;
         }
-        const float mu = mean[row], r = rstd[row];
-        float s1 = 0.0f, s2 = 0.0f;
+        // columns and rows that do not exist are zeros throughout: dy is, and so is whatever it is multiplied with
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            if ((c * 32 * W + t) * VEC < n) {
+        for (int q = 0; q < R; ++q) {
+            s1[q] = s2[q] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    const float xh = (xv[c][i] - mu) * r, g = gv[c][i];
+                    const float xh = (xv[q][c].get(i) - mu[q]) * r[q], g = gv[q][c].get(i), gw = g * w[c][i];
                     aw[c][i] = fmaf(g, xh, aw[c][i]);
                     ab[c][i] += g;
-                    xv[c][i] = xh;
-                    gv[c][i] = g * w[c][i];
-                    s1 += gv[c][i];
-                    s2 = fmaf(gv[c][i], xh, s2);
+                    s1[q] += gw;
+                    s2[q] = fmaf(gw, xh, s2[q]);
+                }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int q = 0; q < R; ++q) {
+                s1[q] += __shfl_xor_sync(0xffffffffu, s1[q], o);
+                s2[q] += __shfl_xor_sync(0xffffffffu, s2[q], o);
+            }
+        if (W > 1) {
+            // a warp that is a round ahead writes the other set
+            if (lane == 0)
+#pragma unroll
+                for (int q = 0; q < R; ++q) {
+                    s_sum[turn][2 * q][warp] = s1[q];
+                    s_sum[turn][2 * q + 1][warp] = s2[q];
+                }
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < R; ++q) {
+                s1[q] = s_sum[turn][2 * q][0];
+                s2[q] = s_sum[turn][2 * q + 1][0];
+#pragma unroll
+                for (int k = 1; k < W; ++k) {
+                    s1[q] += s_sum[turn][2 * q][k];
+                    s2[q] += s_sum[turn][2 * q + 1][k];
                 }
             }
         }
-        // two barriers' worth of buffers: a warp that is a row ahead writes the other pair
-        s1 = op_group_sum<32>(s1);
-        s2 = op_group_sum<32>(s2);
-        if (W > 1) {
-            if (lane == 0) {
-                s_sum[turn][warp] = s1;
-                s_sum[turn + 1][warp] = s2;
-            }
-            __syncthreads();
-            s1 = s_sum[turn][0];
-            s2 = s_sum[turn + 1][0];
 #pragma unroll
-            for (int k = 1; k < W; ++k) {
-                s1 += s_sum[turn][k];
-                s2 += s_sum[turn + 1][k];
-            }
-        }
-        const float m1 = s1 * inv_n, m2 = s2 * inv_n;
-        T* dr = dx + row * dx_stride;
+        for (int q = 0; q < R; ++q) {
+            const float m1 = s1[q] * inv_n, m2 = s2[q] * inv_n;
+            if (first + q < rows)
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int col = (c * 32 * W + t) * VEC;
-            if (col < n) {
-                float o[VEC];
+                for (int c = 0; c < CH; ++c) {
+                    const int col = (c * 32 * W + t) * VEC;
+                    if (col < n) {
+                        float o[VEC];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) o[i] = r * (gv[c][i] - m1 - xv[c][i] * m2);
-                op_store<T, VEC>(dr + col, o);
-            }
+                        for (int i = 0; i < VEC; ++i) {
+                            const float xh = (xv[q][c].get(i) - mu[q]) * r[q];
+                            o[i] = r[q] * (gv[q][c].get(i) * w[c][i] - m1 - xh * m2);
+                        }
+                        op_store<T, VEC>(dx + (first + q) * dx_stride + col, o);
+                    }
+                }
         }
     }
     if (!partial) return;
-    // W = 1: the four warps' sums are added in order, through the rows of the partials themselves (four per block)
     const int64_t prow = W == 1 ? (int64_t)blockIdx.x * RB + warp : blockIdx.x, prows = (int64_t)gridDim.x * RB;
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int col = (c * 32 * W + t) * VEC + i;
-            if (col < n) {
-                partial[prow * n + col] = aw[c][i];
-                partial[(prows + prow) * n + col] = ab[c][i];
-            }
+    for (int c = 0; c < CH; ++c) {
+        const int col = (c * 32 * W + t) * VEC;
+        if (col < n) {  // n is a multiple of VEC
+            op_store<float, VEC>(partial + prow * n + col, aw[c]);
+            op_store<float, VEC>(partial + (prows + prow) * n + col, ab[c]);
         }
+    }
 }
 
 // rows longer than NORM_REG_N_BACK: dx by a block per row, then the columns' sums by threads that walk down stripes of rows
@@ -248,43 +289,60 @@ k_norm_columns_long(const T* __restrict__ dy, int64_t dy_stride, const T* __rest
     partial[(int64_t)(gridDim.y + blockIdx.y) * n + col] = ab;
 }
 
-// dweight and dbias from the blocks' rows: 32 columns per block, warp w adds the rows w, w + 32, .., then the warps in order
+// dweight and dbias from the blocks' rows: eight columns (a 32-byte sector) per block; thread group r of 128 adds the rows r, r + 128, .., the four
+// groups of a warp are added in halves, then the warps in halves.
 __global__ void __launch_bounds__(1024) k_norm_columns_final(const float* __restrict__ partial, int prows, int n, float* __restrict__ dweight,
                                                               float* __restrict__ dbias) {
-    __shared__ float s_sum[32][33];
+    __shared__ float s_sum[32][9];
     float* out = blockIdx.y ? dbias : dweight;
     if (!out) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = threadIdx.x & 7, col = blockIdx.x * 8 + c;
     const float* p = partial + (int64_t)blockIdx.y * prows * n;
     float v = 0.0f;
     if (col < n)
-#pragma unroll 4
-        for (int r = warp; r < prows; r += 32) v += p[(int64_t)r * n + col];
-    s_sum[warp][lane] = v;
-    __syncthreads();
-    if (warp == 0 && col < n) {
-        v = s_sum[0][lane];
+        for (int r0 = threadIdx.x >> 3; r0 < prows; r0 += 128 * 8) {
+            float t[8];
 #pragma unroll
-        for (int w = 1; w < 32; ++w) v += s_sum[w][lane];
-        out[col] = v;
-    }
+            for (int i = 0; i < 8; ++i) t[i] = r0 + 128 * i < prows ? p[(int64_t)(r0 + 128 * i) * n + col] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v += t[i];
+        }
+    v += __shfl_xor_sync(0xffffffffu, v, 8);
+    v += __shfl_xor_sync(0xffffffffu, v, 16);
+    if (lane < 8) s_sum[warp][c] = v;
+    __syncthreads();
+    if (warp >= 8) return;
+    v = op_group_sum<32>(s_sum[lane][warp]);
+    if (lane == 0 && blockIdx.x * 8 + warp < n) out[blockIdx.x * 8 + warp] = v;
 }
 
-// Blocks of the backward pass.  More than a few rows per block, or the blocks' rows of gradients cost as much as the rows themselves;
-// at most what runs at once.
+// Shape of the backward pass: warps per row and columns per thread.  Eight columns a thread (two rows at a time) up to 4096 columns, sixteen
+// (one row) up to 8192.
+struct NormShape {
+    int warps, columns;
+};
+NormShape norm_backward_shape(int n) {
+    const int w8[] = {1, 2, 3, 4, 6, 8, 12, 16};
+    for (int w : w8)
+        if (n <= w * 256) return {w, 8};
+    return {16, 16};
+}
+// Blocks: at most what runs at once, and 16 rows or more for each, or the blocks' rows of gradients cost as much
+// as the rows themselves.
 int norm_backward_blocks(int64_t rows, int n) {
     if (n > NORM_REG_N_BACK) return (int)(rows < 64 ? (rows < 1 ? 1 : rows) : 64);
-    const int64_t per = n <= 512 ? 4 : 1, most = (int64_t)sm_count() * (n <= 2048 ? 4 : 2);
-    const int64_t want = (rows + 8 * per - 1) / (8 * per);
+    const int w = norm_backward_shape(n).warps;
+    const int64_t per = w == 1 ? 4 * 16 : 16, most = (int64_t)sm_count() * norm_backward_per_sm(w);
+    const int64_t want = (rows + per - 1) / per;
     return (int)(want < 1 ? 1 : want < most ? want : most);
 }
-int norm_partial_rows(int64_t rows, int n) { return norm_backward_blocks(rows, n) * (n <= 512 ? 4 : 1); }
+int norm_partial_rows(int64_t rows, int n) { return norm_backward_blocks(rows, n) * (n <= 256 ? 4 : 1); }
 
 template <typename T, int VEC, int W, int CH>
 void norm_forward_go(cudaStream_t s, const void* x, int64_t xs, const float* w, const float* b, float eps, int64_t rows, int n, void* y, int64_t ys,
                      float* mean, float* rstd) {
-    const int64_t blocks = W == 1 ? (rows + 7) / 8 : rows;
-    k_norm_forward<T, W, VEC, CH><<<(unsigned)blocks, W == 1 ? 256 : W * 32, 0, s>>>((const T*)x, xs, w, b, eps, rows, n, (T*)y, ys, mean, rstd);
+    const int64_t blocks = W == 1 ? (rows + 3) / 4 : rows;
+    k_norm_forward<T, W, VEC, CH><<<(unsigned)blocks, W == 1 ? 128 : W * 32, 0, s>>>((const T*)x, xs, w, b, eps, rows, n, (T*)y, ys, mean, rstd);
 }
 // A warp per row up to 2048 columns (no barrier in a row), eight warps above.
 template <typename T, int VEC>
@@ -301,15 +359,25 @@ void norm_forward_pick(cudaStream_t s, const void* x, int64_t xs, const float* w
 template <typename T, int VEC>
 void norm_backward_pick(cudaStream_t s, const void* dy, int64_t dys, const void* x, int64_t xs, const float* mean, const float* rstd, const float* w,
                         int64_t rows, int n, void* dx, int64_t dxs, float* partial, int blocks) {
-    // W warps x K columns per lane
-#define GO(W, K)                                                                                                                              \
-    if (n <= (W) * (K) * 32) {                                                                                                                \
-        k_norm_backward<T, W, VEC, ((K) + VEC - 1) / VEC><<<(unsigned)blocks, W == 1 ? 128 : W * 32, 0, s>>>(                                  \
-            (const T*)dy, dys, (const T*)x, xs, mean, rstd, w, rows, n, (T*)dx, dxs, partial);                                                \
-        return;                                                                                                                               \
-    }
-    GO(1, 8) GO(1, 16) GO(4, 8) GO(4, 16) GO(8, 16) GO(16, 16)
+    if (n <= NORM_REG_N_BACK) {
+        const NormShape shape = norm_backward_shape(n);
+#define GO(W, K, R)                                                                                                                           \
+    k_norm_backward<T, W, VEC, (K) / VEC, R><<<(unsigned)blocks, W == 1 ? 128 : W * 32, 0, s>>>((const T*)dy, dys, (const T*)x, xs, mean, rstd, \
+                                                                                               w, rows, n, (T*)dx, dxs, partial)
+        switch (shape.warps) {
+            case 1: GO(1, 8, 2); break;
+            case 2: GO(2, 8, 2); break;
+            case 3: GO(3, 8, 2); break;
+            case 4: GO(4, 8, 2); break;
+            case 6: GO(6, 8, 2); break;
+            case 8: GO(8, 8, 2); break;
+            case 12: GO(12, 8, 2); break;
+            default:
+                if (shape.columns == 8) GO(16, 8, 2); else GO(16, 16, 1);
+        }
 #undef GO
+        return;
+    }
     k_norm_backward_long<T><<<(unsigned)rows, 1024, 0, s>>>((const T*)dy, dys, (const T*)x, xs, mean, rstd, w, n, (T*)dx, dxs);
     if (partial)
         k_norm_columns_long<T><<<dim3((unsigned)ceil_div(n, 256), (unsigned)blocks), 256, 0, s>>>((const T*)dy, dys, (const T*)x, xs, mean, rstd, rows, n, partial);
@@ -332,9 +400,9 @@ extern "C" int tb_layer_norm_forward(const void* d_x, int64_t x_stride, const fl
     if (rows == 0) return TB_OK;
     if (!d_x || !d_y) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_x or d_y is NULL");
     if (rows > 1 && (x_stride < n || y_stride < n)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "row strides must be at least n");
-    if (((uintptr_t)d_x | (uintptr_t)d_y) % size) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_x and d_y must be aligned to their elements");
+    if (((uintptr_t)d_x | (uintptr_t)d_y) % size || ((uintptr_t)d_weight | (uintptr_t)d_bias) & 3) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool wide = n % (16 / size) == 0 && norm_aligned(d_x, x_stride, size) && norm_aligned(d_y, y_stride, size);
+    const bool wide = n % (16 / size) == 0 && norm_aligned(d_x, x_stride, size) && norm_aligned(d_y, y_stride, size) && (((uintptr_t)d_weight | (uintptr_t)d_bias) & 15) == 0;
 #define ARGS s, d_x, x_stride, d_weight, d_bias, eps, rows, n, d_y, y_stride, d_mean, d_rstd
     if (type == TB_TYPE_F32) wide ? norm_forward_pick<float, 4>(ARGS) : norm_forward_pick<float, 1>(ARGS);
     else if (type == TB_TYPE_F16) wide ? norm_forward_pick<__half, 8>(ARGS) : norm_forward_pick<__half, 1>(ARGS);
@@ -357,9 +425,9 @@ extern "C" int tb_layer_norm_backward(const void* d_dy, int64_t dy_stride, const
     if (rows < 0 || rows > NORM_MAX_ROWS || n < 1) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "rows must be in [0, 2^31) and n positive");
     if (rows > 0 && (!d_dy || !d_x || !d_mean || !d_rstd || !d_dx)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "a device pointer is NULL");
     if (rows > 1 && (dy_stride < n || x_stride < n || dx_stride < n)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "row strides must be at least n");
-    if (((uintptr_t)d_dy | (uintptr_t)d_x | (uintptr_t)d_dx) % size) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "rows must be aligned to their elements");
+    if (((uintptr_t)d_dy | (uintptr_t)d_x | (uintptr_t)d_dx) % size || ((uintptr_t)d_weight & 3)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "rows must be aligned to their elements");
     const bool columns = d_dweight || d_dbias;
-    if (columns && (!d_work || work_bytes < tb_layer_norm_backward_workspace(rows, n) || ((uintptr_t)d_work & 3)))
+    if (columns && (!d_work || work_bytes < tb_layer_norm_backward_workspace(rows, n) || ((uintptr_t)d_work & 31)))
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "the workspace must be aligned and hold %lld bytes (got %lld)",
                          (long long)tb_layer_norm_backward_workspace(rows, n), (long long)work_bytes);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -370,12 +438,12 @@ extern "C" int tb_layer_norm_backward(const void* d_dy, int64_t dy_stride, const
         if (d_dbias) cudaMemsetAsync(d_dbias, 0, (size_t)n * sizeof(float), s);
         return op_launched(err, err_len);
     }
-    const bool wide = n % (16 / size) == 0 && norm_aligned(d_dy, dy_stride, size) && norm_aligned(d_x, x_stride, size) && norm_aligned(d_dx, dx_stride, size);
+    const bool wide = n % (16 / size) == 0 && norm_aligned(d_dy, dy_stride, size) && norm_aligned(d_x, x_stride, size) && norm_aligned(d_dx, dx_stride, size) && ((uintptr_t)d_weight & 15) == 0;
 #define ARGS s, d_dy, dy_stride, d_x, x_stride, d_mean, d_rstd, d_weight, rows, n, d_dx, dx_stride, partial, blocks
     if (type == TB_TYPE_F32) wide ? norm_backward_pick<float, 4>(ARGS) : norm_backward_pick<float, 1>(ARGS);
     else if (type == TB_TYPE_F16) wide ? norm_backward_pick<__half, 8>(ARGS) : norm_backward_pick<__half, 1>(ARGS);
     else wide ? norm_backward_pick<__nv_bfloat16, 8>(ARGS) : norm_backward_pick<__nv_bfloat16, 1>(ARGS);
 #undef ARGS
-    if (columns) k_norm_columns_final<<<dim3((unsigned)ceil_div(n, 32), 2), 1024, 0, s>>>(partial, norm_partial_rows(rows, n), n, d_dweight, d_dbias);
+    if (columns) k_norm_columns_final<<<dim3((unsigned)ceil_div(n, 8), 2), 1024, 0, s>>>(partial, norm_partial_rows(rows, n), n, d_dweight, d_dbias);
     return op_launched(err, err_len);
 }

@@ -37,6 +37,34 @@ static __device__ __forceinline__ void op_store(T* p, const float (&from)[N]) {
     *reinterpret_cast<OpVec<T, N>*>(p) = u;
 }
 
+// N adjacent elements as they lie in memory, two 16-bit ones to a register (as an array of __half they would take one each)
+template <typename T, int N>
+struct OpRaw {
+    static constexpr int WORDS = N * sizeof(T) >= 4 ? N * sizeof(T) / 4 : 1;
+    unsigned w[WORDS];
+    __device__ __forceinline__ void load(const T* p) {
+        if (N * sizeof(T) == 16) {
+            const uint4 u = *reinterpret_cast<const uint4*>(p);
+            w[0] = u.x, w[1 % WORDS] = u.y, w[2 % WORDS] = u.z, w[3 % WORDS] = u.w;
+        } else if (sizeof(T) == 2) {
+            w[0] = *reinterpret_cast<const unsigned short*>(p);
+        } else {
+            w[0] = *reinterpret_cast<const unsigned*>(p);
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ float get(int i) const;
+};
+template <typename T> static __device__ __forceinline__ float op_word(unsigned w, int half);
+template <> __device__ __forceinline__ float op_word<float>(unsigned w, int) { return __uint_as_float(w); }
+template <> __device__ __forceinline__ float op_word<__half>(unsigned w, int half) { return __half2float(__ushort_as_half((unsigned short)(half ? w >> 16 : w))); }
+template <> __device__ __forceinline__ float op_word<__nv_bfloat16>(unsigned w, int half) { return __uint_as_float(half ? w & 0xffff0000u : w << 16); }
+template <typename T, int N>
+__device__ __forceinline__ float OpRaw<T, N>::get(int i) const { return sizeof(T) == 4 ? op_word<T>(w[i % WORDS], 0) : op_word<T>(w[i / 2], i & 1); }
+
 // sum over aligned groups of G lanes, the same bits in every lane (halves are added in a fixed order)
 template <int G>
 static __device__ __forceinline__ float op_group_sum(float v) {

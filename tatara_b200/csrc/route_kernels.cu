@@ -9,80 +9,135 @@
 //   backward   h_e = dB E c_e / (N k) / N,  dl = p (h - sum(p h)) + dZ 2 lse / N p + the gates' part: renormalised
 //              g_j (dg_j - sum(g dg)) at the chosen, else p_cj dg_j at the chosen - p sum(g dg)
 //
-// A group of G lanes owns a row and keeps it in registers, V logits per lane; every logit is read once.  The choice compares order-preserving
-// integer keys of the logits as they are, so it does not depend on how the softmax rounds.  Bound by memory for wide rows of
+// A group of G lanes owns a row and keeps it in registers, V logits per lane; every logit is read once.  The choice compares integer words
+// made of the logits' bits as they are and the expert, so it does not depend on how the softmax rounds.  Bound by memory for wide rows of
 // many experts and by latency for the handful of experts of a net.  Sums: fp32 chains over a group's rows, then the groups of a
 // block in order, then the blocks in order in 64 bits (second kernel): results repeat bit for bit.
 #include "op_common.cuh"
-
-#include <float.h>
 
 namespace {
 
 #define ROUTE_THREADS 512
 #define ROUTE_MAX_K 16
 #define ROUTE_MAX_E 1024
-#define KEY_NEG_INF 0x007fffffu
 
-// unsigned keys in the order of the floats; both zeros alike; a NaN is larger than any number
-__device__ __forceinline__ unsigned route_key(float v) {
-    if (v != v) return 0xffffffffu;
-    const unsigned u = __float_as_uint(v + 0.0f);
-    return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
-}
-__device__ __forceinline__ float route_unkey(unsigned k) {
-    if (k == 0xffffffffu) return __int_as_float(0x7fc00000);
-    return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
-}
-
-template <int G>
-__device__ __forceinline__ unsigned group_max(unsigned v) {
-    if (G == 32) return __reduce_max_sync(0xffffffffu, v);
+// A logit and its expert as one unsigned word that orders like (logit, -expert): the order-preserving key of the logit's bits above the
+// expert's complement.  16-bit logits make 32-bit words, 32-bit ones 64-bit words.  Both zeros are alike, a NaN is larger than any number; words are
+// distinct, so the k-th largest is one comparison, ties included.
+template <typename T> struct RouteWord;
+template <> struct RouteWord<float> {
+    using W = unsigned long long;
+    static constexpr W NONE = ((W)0x007fffffu << 32) | 0xffffffffu;  // of -inf: words above it can be chosen
+    static __device__ __forceinline__ W make(float x, int e) {
+        const unsigned u = __float_as_uint(x + 0.0f);
+        const unsigned key = x != x ? 0xffffffffu : u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+        return ((W)key << 32) | (unsigned)~e;
+    }
+    static __device__ __forceinline__ int expert(W w) { return (int)~(unsigned)w; }
+    static __device__ __forceinline__ float logit(W w) {
+        const unsigned k = (unsigned)(w >> 32);
+        return k == 0xffffffffu ? __int_as_float(0x7fc00000) : __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
+    }
+    template <int G>
+    static __device__ __forceinline__ W group_max(W w) {
+        if (G == 32) {
+            const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(w >> 32));
+            const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned)(w >> 32) == hi ? (unsigned)w : 0u);
+            return ((W)hi << 32) | lo;
+        }
 #pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
-template <int G>
-__device__ __forceinline__ int group_min(int v) {
-    if (G == 32) return __reduce_min_sync(0xffffffffu, v);
+        for (int o = G / 2; o > 0; o >>= 1) w = max(w, __shfl_xor_sync(0xffffffffu, w, o));
+        return w;
+    }
+};
+template <typename T, unsigned NEG_INF>
+struct RouteWord16 {
+    using W = unsigned;
+    static constexpr W NONE = (NEG_INF << 16) | 0xffffu;
+    static __device__ __forceinline__ W make(T x, int e) {
+        unsigned u = *reinterpret_cast<const unsigned short*>(&x);
+        const float v = op_float(x);
+        u = v == 0.0f ? 0u : u;
+        const unsigned key = v != v ? 0xffffu : (u >> 15) ? u ^ 0xffffu : u ^ 0x8000u;
+        return (key << 16) | (0xffffu - (unsigned)e);
+    }
+    static __device__ __forceinline__ int expert(W w) { return (int)(0xffffu - (w & 0xffffu)); }
+    static __device__ __forceinline__ float logit(W w) {
+        const unsigned k = w >> 16;
+        const unsigned short u = (unsigned short)(k ^ ((k >> 15) ? 0x8000u : 0xffffu));
+        return k == 0xffffu ? __int_as_float(0x7fc00000) : op_float(*reinterpret_cast<const T*>(&u));
+    }
+    template <int G>
+    static __device__ __forceinline__ W group_max(W w) {
+        if (G == 32) return __reduce_max_sync(0xffffffffu, w);
 #pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) v = min(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
+        for (int o = G / 2; o > 0; o >>= 1) w = max(w, __shfl_xor_sync(0xffffffffu, w, o));
+        return w;
+    }
+};
+template <> struct RouteWord<__half> : RouteWord16<__half, 0x03ffu> {};
+template <> struct RouteWord<__nv_bfloat16> : RouteWord16<__nv_bfloat16, 0x007fu> {};
 
 // the expert of a lane's v-th logit
 template <int G, int VEC>
 __device__ __forceinline__ int route_expert(int v, int lane) { return (v / VEC) * G * VEC + lane * VEC + v % VEC; }
 
+template <typename T> __device__ __forceinline__ T route_never();
+template <> __device__ __forceinline__ float route_never<float>() { return -INFINITY; }
+template <> __device__ __forceinline__ __half route_never<__half>() { return __ushort_as_half(0xfc00); }
+template <> __device__ __forceinline__ __nv_bfloat16 route_never<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
+
+// a lane's logits, -inf where there are none
 template <typename T, int G, int V, int VEC>
-__device__ __forceinline__ void route_load(const T* row, int experts, int lane, float (&l)[V]) {
+__device__ __forceinline__ void route_load(const T* row, bool in, int experts, int lane, OpVec<T, VEC> (&l)[V / VEC]) {
 #pragma unroll
     for (int c = 0; c < V / VEC; ++c) {
         const int e = c * G * VEC + lane * VEC;
-        float t[VEC];
-        if (e < experts) {
-            op_load<T, VEC>(row + e, t);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) l[c * VEC + i] = t[i];
+        if (in && e < experts) {
+            l[c] = *reinterpret_cast<const OpVec<T, VEC>*>(row + e);
         } else {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) l[c * VEC + i] = -INFINITY;
+            for (int i = 0; i < VEC; ++i) l[c].v[i] = route_never<T>();
         }
     }
 }
 
-// The sums of a launch: counts, rows and probability sums of every block.  part_p [blocks][E] floats, part_c [blocks][E + 1] ints (the last
-// is the block's rows), part_z [blocks] floats.
+// descending, by Batcher's odd-even merges
+template <typename W, int N>
+__device__ __forceinline__ void route_sort(W (&w)[N]) {
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < N && (i + j) / (p * 2) == (i + j + k) / (p * 2)) {
+                        const W a = w[i + j], b = w[i + j + k];
+                        w[i + j] = max(a, b);
+                        w[i + j + k] = min(a, b);
+                    }
+}
+
+// The sums of a launch: counts, rows and probability sums of every block.  p [blocks][E], c [blocks][E + 1] (the last is the block's
+// rows), z [blocks]; balance [ceil(E / 32)] and ticket belong to the second kernel.
 struct RouteParts {
+    double* balance;
     float* p;
     float* z;
     int* c;
+    int* ticket;
 };
 
-template <typename T, int G, int V, int VEC>
+// SORTED: a lane sorts its logits once and gives the largest away in every round, which pays from three choices on (16-bit logits, 256 experts, k = 8:
+// 1040 instructions per row when every round looks at all of them).
+template <typename T, int G, int V, int VEC, bool SORTED>
 __global__ void __launch_bounds__(ROUTE_THREADS)
 k_route_forward(const T* __restrict__ logits, int64_t stride, const uint8_t* __restrict__ mask, int64_t rows, int experts, int k, int renormalise,
                 int* __restrict__ index, float* __restrict__ gate, RouteParts part) {
+    using R = RouteWord<T>;
+    using W = typename R::W;
     constexpr int GROUPS = ROUTE_THREADS / G, SLOTS = ROUTE_MAX_K > G ? ROUTE_MAX_K / G : 1;
     extern __shared__ int s_dyn[];
     int* s_count = s_dyn;                                       // [experts + 1]
@@ -90,6 +145,7 @@ k_route_forward(const T* __restrict__ logits, int64_t stride, const uint8_t* __r
     __shared__ float s_z[ROUTE_THREADS / 32];
     const int lane = threadIdx.x % G, group = threadIdx.x / G, wl = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int e = threadIdx.x; e <= experts; e += ROUTE_THREADS) s_count[e] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *part.ticket = 0;
     __syncthreads();
     float sum_p[V], sum_z = 0.0f;
 #pragma unroll
@@ -101,71 +157,63 @@ k_route_forward(const T* __restrict__ logits, int64_t stride, const uint8_t* __r
         const int64_t row = base + group % (32 / G);
         const bool exists = row < rows;
         const bool in = exists && (!mask || mask[row]);
-        float l[V];
-        if (in) {
-            route_load<T, G, V, VEC>(logits + row * stride, experts, lane, l);
-        } else {
+        OpVec<T, VEC> raw[V / VEC];
+        route_load<T, G, V, VEC>(logits + row * stride, in, experts, lane, raw);
+        W w[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) l[v] = -INFINITY;
-        }
-        unsigned key[V];
+        for (int v = 0; v < V; ++v) w[v] = R::make(raw[v / VEC].v[v % VEC], route_expert<G, VEC>(v, lane));
+        if (SORTED) route_sort<W, V>(w);
+        W mine[SLOTS];
 #pragma unroll
-        for (int v = 0; v < V; ++v) key[v] = route_key(l[v]);
-        unsigned top = 0;
-        float top_l = 0.0f, chosen_sum = 0.0f, total = 0.0f;
-        int mine[SLOTS];
-        float mine_g[SLOTS];
-#pragma unroll
-        for (int s = 0; s < SLOTS; ++s) {
-            mine[s] = -1;
-            mine_g[s] = 0.0f;
-        }
-        bool live = false;
+        for (int s = 0; s < SLOTS; ++s) mine[s] = 0;
+        W top = 0;
         for (int j = 0; j < k; ++j) {
-            unsigned best = 0;
-            int at = INT32_MAX;
+            W best = w[0];
+            if (!SORTED)
 #pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (key[v] > best) {
-                    best = key[v];
-                    at = route_expert<G, VEC>(v, lane);
-                }
-            const unsigned m = group_max<G>(best);
-            if (j == 0) {
-                top = m;
-                live = m > KEY_NEG_INF;
-                top_l = live ? route_unkey(top) : 0.0f;
+                for (int v = 1; v < V; ++v) best = max(best, w[v]);
+            const W m = R::template group_max<G>(best);
+            if (j == 0) top = m;
+            if (SORTED) {
+                if (best == m) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    l[v] = live ? expf(l[v] - top_l) : 0.0f;
-                    total += l[v];
+                    for (int v = 0; v + 1 < V; ++v) w[v] = w[v + 1];
+                    w[V - 1] = 0;
                 }
-                total = op_group_sum<G>(total);
-            }
-            const bool ok = m > KEY_NEG_INF;
-            const int e = group_min<G>(best == m ? at : INT32_MAX);
-            const float g = ok ? expf(route_unkey(m) - top_l) : 0.0f;
-            chosen_sum += g;
-            if (ok) {
+            } else {
 #pragma unroll
                 for (int v = 0; v < V; ++v)
-                    if (route_expert<G, VEC>(v, lane) == e) key[v] = 0;
+                    if (w[v] == m) w[v] = 0;
             }
 #pragma unroll
             for (int s = 0; s < SLOTS; ++s)
-                if (ok && j == s * G + lane) {
-                    mine[s] = e;
-                    mine_g[s] = g;
-                }
+                if (j == s * G + lane) mine[s] = m;
         }
-        const float norm = renormalise ? chosen_sum : total;
+        const bool live = top > R::NONE;
+        const float top_l = live ? R::logit(top) : 0.0f;
+        float l[V], total = 0.0f, chosen = 0.0f, g[SLOTS];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            l[v] = live ? expf(op_float(raw[v / VEC].v[v % VEC]) - top_l) : 0.0f;
+            total += l[v];
+        }
+        total = op_group_sum<G>(total);
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) {
+            g[s] = mine[s] > R::NONE ? expf(R::logit(mine[s]) - top_l) : 0.0f;
+            chosen += g[s];
+        }
+        chosen = op_group_sum<G>(chosen);
+        const float norm = renormalise ? chosen : total;
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
             const int j = s * G + lane;
             if (exists && j < k) {
-                index[row * k + j] = mine[s];
-                gate[row * k + j] = mine[s] >= 0 ? mine_g[s] / norm : 0.0f;
-                if (mine[s] >= 0) atomicAdd(&s_count[mine[s]], 1);
+                const bool ok = mine[s] > R::NONE;
+                const int e = ok ? R::expert(mine[s]) : -1;
+                index[row * k + j] = e;
+                gate[row * k + j] = ok ? g[s] / norm : 0.0f;
+                if (ok) atomicAdd(&s_count[e], 1);
             }
         }
         if (live) {
@@ -203,68 +251,76 @@ k_route_forward(const T* __restrict__ logits, int64_t stride, const uint8_t* __r
     }
     if (threadIdx.x == 0) {
         float t = s_z[0];
+#pragma unroll
         for (int w = 1; w < ROUTE_THREADS / 32; ++w) t += s_z[w];
         part.z[blockIdx.x] = t;
     }
 }
 
-// The blocks' sums: one block; S = 1024 / width threads per expert add every S-th block, then those in order, in 64 bits.
-__global__ void __launch_bounds__(1024) k_route_final(RouteParts part, int blocks, int experts, int width, int k, int* __restrict__ counts,
-                                                       int* __restrict__ rows_out, float* __restrict__ prob_mean, float* __restrict__ losses) {
-    __shared__ double s_p[1024];
-    __shared__ int s_c[1024];
-    __shared__ int s_rows;
-    const int e = threadIdx.x % width, slice = threadIdx.x / width, slices = 1024 / width;
+// The blocks' sums, 32 experts per block of 32 warps: lane l of warp w adds expert l of the blocks w, w + 32, .., then warp l adds those of expert l
+// in halves, all in 64 bits.  The last block to finish adds up the balance loss of the others, in order.
+__global__ void __launch_bounds__(1024) k_route_final(RouteParts part, int blocks, int experts, int k, int* __restrict__ counts, int* __restrict__ rows_out,
+                                                       float* __restrict__ prob_mean, float* __restrict__ losses) {
+    __shared__ double s_p[32][33], s_z[32], s_b[32];
+    __shared__ int s_c[32][33], s_n[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e0 = blockIdx.x * 32;
     double p = 0.0, z = 0.0;
     int c = 0, n = 0;
-    if (e < experts)
-#pragma unroll 4
-        for (int b = slice; b < blocks; b += slices) {
-            p += (double)part.p[(int64_t)b * experts + e];
-            c += part.c[(int64_t)b * (experts + 1) + e];
-        }
-    s_p[threadIdx.x] = p;
-    s_c[threadIdx.x] = c;
-    if (threadIdx.x == 0) s_rows = 0;
-    __syncthreads();
-    if (slice == 0)
-        for (int s = 1; s < slices; ++s) {
-            p += s_p[s * width + e];
-            c += s_c[s * width + e];
+    if (e0 + lane < experts)
+#pragma unroll 8
+        for (int b = warp; b < blocks; b += 32) {
+            p += (double)part.p[(int64_t)b * experts + e0 + lane];
+            c += part.c[(int64_t)b * (experts + 1) + e0 + lane];
         }
     for (int b = threadIdx.x; b < blocks; b += 1024) {
         z += (double)part.z[b];
         n += part.c[(int64_t)b * (experts + 1) + experts];
     }
-    if (n) atomicAdd(&s_rows, n);
-    __syncthreads();
-    const int rows = s_rows;
-    const double inv = 1.0 / (double)(rows > 0 ? rows : 1);
-    const bool owner = slice == 0 && e < experts;
-    if (owner) {
-        counts[e] = c;
-        prob_mean[e] = (float)(p * inv);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) {
+        s_z[warp] = z;
+        s_n[warp] = n;
     }
-    // both losses by a tree over the threads
-    s_p[threadIdx.x] = owner ? p * inv * (double)c : 0.0;
+    s_p[warp][lane] = p;
+    s_c[warp][lane] = c;
     __syncthreads();
-    for (int o = 512; o > 0; o >>= 1) {
-        if (threadIdx.x < o) s_p[threadIdx.x] += s_p[threadIdx.x + o];
-        __syncthreads();
+    p = s_p[lane][warp];
+    c = __reduce_add_sync(0xffffffffu, s_c[lane][warp]);
+    n = __reduce_add_sync(0xffffffffu, s_n[lane]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) p += __shfl_xor_sync(0xffffffffu, p, o);
+    const double inv = 1.0 / (double)(n > 0 ? n : 1);
+    if (lane == 0) {
+        const bool owner = e0 + warp < experts;
+        s_b[warp] = owner ? p * inv * (double)c : 0.0;
+        if (owner) {
+            counts[e0 + warp] = c;
+            prob_mean[e0 + warp] = (float)(p * inv);
+        }
     }
-    const double balance = s_p[0] * (double)experts * inv / (double)k;
     __syncthreads();
-    s_p[threadIdx.x] = z;
-    __syncthreads();
-    for (int o = 512; o > 0; o >>= 1) {
-        if (threadIdx.x < o) s_p[threadIdx.x] += s_p[threadIdx.x + o];
-        __syncthreads();
+    if (warp != 0) return;
+    double balance = s_b[lane];
+    z = s_z[lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        balance += __shfl_xor_sync(0xffffffffu, balance, o);
+        z += __shfl_xor_sync(0xffffffffu, z, o);
     }
-    if (threadIdx.x == 0) {
-        losses[0] = (float)balance;
-        losses[1] = (float)(s_p[0] * inv);
-        *rows_out = rows;
+    if (lane != 0) return;
+    if (gridDim.x > 1) {
+        part.balance[blockIdx.x] = balance;
+        __threadfence();
+        if (atomicAdd(part.ticket, 1) != (int)gridDim.x - 1) return;
+        __threadfence();
+        balance = 0.0;
+        for (unsigned b = 0; b < gridDim.x; ++b) balance += *static_cast<volatile double*>(part.balance + b);
     }
+    losses[0] = (float)(balance * (double)experts * inv / (double)k);
+    losses[1] = (float)(z * inv);
+    *rows_out = n;
 }
 
 template <typename T, int G, int V, int VEC>
@@ -273,7 +329,11 @@ k_route_backward(const T* __restrict__ logits, int64_t stride, const uint8_t* __
                  const int* __restrict__ index, const float* __restrict__ gate, const float* __restrict__ dgate, const int* __restrict__ counts,
                  const int* __restrict__ n_rows, const float* __restrict__ dlosses, T* __restrict__ dlogits, int64_t dstride) {
     constexpr int GROUPS = 256 / G, SLOTS = ROUTE_MAX_K > G ? ROUTE_MAX_K / G : 1;
+    // the gates' part of a group's row: zero but while the chosen experts' lanes pass it to the lanes that hold those logits
+    __shared__ __align__(16) float s_add[GROUPS][G * V];
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
+#pragma unroll
+    for (int v = 0; v < V; ++v) s_add[group][v * G + lane] = 0.0f;
     const float n = (float)max(*n_rows, 1);
     const float db = dlosses ? dlosses[0] : 0.0f, dz = dlosses ? dlosses[1] : 0.0f;
     const float hk = db * (float)experts / (n * (float)k) / n, zk = 2.0f * dz / n;
@@ -283,18 +343,14 @@ k_route_backward(const T* __restrict__ logits, int64_t stride, const uint8_t* __
         const int e = route_expert<G, VEC>(v, lane);
         h[v] = e < experts ? hk * (float)counts[e] : 0.0f;
     }
+    __syncwarp();
     const int64_t first = (int64_t)blockIdx.x * GROUPS + (threadIdx.x / 32) * (32 / G);
     for (int64_t base = first; base < rows; base += (int64_t)gridDim.x * GROUPS) {
         const int64_t row = base + group % (32 / G);
         const bool exists = row < rows;
         const bool in = exists && (!mask || mask[row]);
-        float l[V];
-        if (in) {
-            route_load<T, G, V, VEC>(logits + row * stride, experts, lane, l);
-        } else {
-#pragma unroll
-            for (int v = 0; v < V; ++v) l[v] = -INFINITY;
-        }
+        OpVec<T, VEC> raw[V / VEC];
+        route_load<T, G, V, VEC>(logits + row * stride, in, experts, lane, raw);
         int at[SLOTS];
         float ga[SLOTS], dg[SLOTS], dot = 0.0f;
 #pragma unroll
@@ -302,54 +358,61 @@ k_route_backward(const T* __restrict__ logits, int64_t stride, const uint8_t* __
             const int j = s * G + lane;
             const bool mine = in && j < k;
             at[s] = mine ? index[row * k + j] : -1;
-            const bool ok = at[s] >= 0;
+            const bool ok = at[s] >= 0 && at[s] < experts;
             ga[s] = ok ? gate[row * k + j] : 0.0f;
             dg[s] = ok && dgate ? dgate[row * k + j] : 0.0f;
             dot = fmaf(ga[s], dg[s], dot);
+            if (!ok) at[s] = -1;
         }
         dot = op_group_sum<G>(dot);
-        unsigned best = 0;
 #pragma unroll
-        for (int v = 0; v < V; ++v) best = max(best, route_key(l[v]));
-        best = group_max<G>(best);
-        const bool live = best > KEY_NEG_INF;
-        const float top_l = live ? route_unkey(best) : 0.0f;
-        float total = 0.0f, ph = 0.0f;
+        for (int s = 0; s < SLOTS; ++s)
+            if (at[s] >= 0) s_add[group][at[s]] = ga[s] * (renormalise ? dg[s] - dot : dg[s]);
+        float l[V], top = -INFINITY, total = 0.0f, ph = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            l[v] = live ? expf(l[v] - top_l) : 0.0f;
+            l[v] = op_float(raw[v / VEC].v[v % VEC]);
+            top = fmaxf(top, l[v]);  // leaves a NaN out, which the sums then bring in
+        }
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        bool live = top > -INFINITY;
+        const float top_l = live ? top : 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            l[v] = expf(l[v] - top_l);
             total += l[v];
             ph = fmaf(l[v], h[v], ph);
         }
         total = op_group_sum<G>(total);
+        live = live || total != total;  // NaN beside -inf alone
         total = live ? total : 1.0f;
-        ph = op_group_sum<G>(ph) / total;
-        const float shift = zk * (top_l + logf(total)) - ph - (renormalise ? 0.0f : dot), inv = 1.0f / total;
-#pragma unroll
-        for (int v = 0; v < V; ++v) l[v] = l[v] * inv * (h[v] + shift);
-#pragma unroll
-        for (int s = 0; s < SLOTS; ++s) {
-            const float add = ga[s] * (renormalise ? dg[s] - dot : dg[s]);
-            for (int j = 0; j < G && s * G + j < k; ++j) {
-                const int e = __shfl_sync(0xffffffffu, at[s], j, G);
-                const float a = __shfl_sync(0xffffffffu, add, j, G);
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (route_expert<G, VEC>(v, lane) == e) l[v] += a;
-            }
-        }
-        if (!exists) continue;
+        const float inv = 1.0f / total;
+        ph = op_group_sum<G>(ph) * inv;
+        const float shift = zk * (top_l + logf(total)) - ph - (renormalise ? 0.0f : dot);
+        __syncwarp();
         T* out = dlogits + row * dstride;
 #pragma unroll
         for (int c = 0; c < V / VEC; ++c) {
             const int e = c * G * VEC + lane * VEC;
-            if (e < experts) {
-                float t[VEC];
+            float add[VEC], t[VEC];
+            constexpr int STEP = VEC < 4 ? VEC : 4;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) t[i] = live ? l[c * VEC + i] : 0.0f;
-                op_store<T, VEC>(out + e, t);
+            for (int i = 0; i < VEC; i += STEP) {
+                float q[STEP];
+                op_load<float, STEP>(&s_add[group][e + i], q);
+#pragma unroll
+                for (int r = 0; r < STEP; ++r) add[i + r] = q[r];
             }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) t[i] = live ? fmaf(l[c * VEC + i] * inv, h[c * VEC + i] + shift, add[i]) : 0.0f;
+            if (exists && e < experts) op_store<T, VEC>(out + e, t);
         }
+        __syncwarp();
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s)
+            if (at[s] >= 0) s_add[group][at[s]] = 0.0f;
+        __syncwarp();
     }
 }
 
@@ -364,6 +427,7 @@ int route_forward_blocks(int64_t rows, int experts) {
     const int64_t groups = ROUTE_THREADS / route_group(experts), want = (rows + groups - 1) / groups, most = 2 * (int64_t)sm_count();
     return (int)(want < 1 ? 1 : want < most ? want : most);
 }
+int64_t route_balance_bytes(int experts) { return (int64_t)((experts + 31) / 32) * 8; }
 size_t route_smem(int experts) { return (size_t)(experts + 1 + ROUTE_THREADS / 32 * experts) * 4; }
 
 template <typename T>
@@ -375,7 +439,9 @@ void route_forward_go(cudaStream_t s, const void* logits, int64_t stride, const 
 #define GO(G, V)                                                                                                                                \
     do {                                                                                                                                        \
         constexpr int VW = W < (V) ? W : (V);                                                                                                   \
-        auto kern = wide ? k_route_forward<T, G, V, VW> : k_route_forward<T, G, V, 1>;                                                          \
+        constexpr bool S = (V) <= 8;                                                                                                            \
+        auto kern = wide ? (S && k > 2 ? k_route_forward<T, G, V, VW, S> : k_route_forward<T, G, V, VW, false>)                                 \
+                         : (S && k > 2 ? k_route_forward<T, G, V, 1, S> : k_route_forward<T, G, V, 1, false>);                                  \
         if (smem > 40000) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);                                   \
         kern<<<blocks, ROUTE_THREADS, smem, s>>>((const T*)logits, stride, mask, rows, experts, k, renormalise, index, gate, part);             \
     } while (0)
@@ -421,7 +487,7 @@ int route_check(int type, int64_t rows, int experts, int k, const void* logits, 
 
 extern "C" int64_t tb_route_forward_workspace(int64_t rows, int experts) {
     if (rows < 0 || experts < 1 || experts > ROUTE_MAX_E) return TB_ERR_INVALID_ARGUMENT;
-    return (int64_t)route_forward_blocks(rows, experts) * (2 * experts + 2) * 4;
+    return route_balance_bytes(experts) + ((int64_t)route_forward_blocks(rows, experts) * (2 * experts + 2) + 1) * 4;
 }
 
 extern "C" int tb_route_forward(const void* d_logits, int64_t stride, int type, int64_t rows, int experts, int k, int renormalise, const uint8_t* d_mask,
@@ -433,23 +499,23 @@ extern "C" int tb_route_forward(const void* d_logits, int64_t stride, int type, 
     if ((rows > 0 && (!d_index || !d_gate)) || !d_counts || !d_rows || !d_prob_mean || !d_losses)
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "an output pointer is NULL");
     const int64_t need = tb_route_forward_workspace(rows, experts);
-    if (!d_work || work_bytes < need || ((uintptr_t)d_work & 3))
+    if (!d_work || work_bytes < need || ((uintptr_t)d_work & 7))
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "the workspace must be aligned and hold %lld bytes (got %lld)", (long long)need, (long long)work_bytes);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int blocks = route_forward_blocks(rows, experts);
     RouteParts part;
-    part.p = static_cast<float*>(d_work);
+    part.balance = static_cast<double*>(d_work);
+    part.p = reinterpret_cast<float*>(static_cast<uint8_t*>(d_work) + route_balance_bytes(experts));
     part.c = reinterpret_cast<int*>(part.p + (size_t)blocks * experts);
     part.z = reinterpret_cast<float*>(part.c + (size_t)blocks * (experts + 1));
+    part.ticket = reinterpret_cast<int*>(part.z + blocks);
     const bool wide = route_wide(d_logits, stride, experts, op_type_size(type));
 #define ARGS s, d_logits, stride, d_mask, rows, experts, k, renormalise, d_index, d_gate, part, wide
     if (type == TB_TYPE_F32) route_forward_go<float>(ARGS);
     else if (type == TB_TYPE_F16) route_forward_go<__half>(ARGS);
     else route_forward_go<__nv_bfloat16>(ARGS);
 #undef ARGS
-    int width = 1;
-    while (width < experts) width *= 2;
-    k_route_final<<<1, 1024, 0, s>>>(part, blocks, experts, width, k, d_counts, d_rows, d_prob_mean, d_losses);
+    k_route_final<<<(unsigned)((experts + 31) / 32), 1024, 0, s>>>(part, blocks, experts, k, d_counts, d_rows, d_prob_mean, d_losses);
     return op_launched(err, err_len);
 }
 

@@ -9,6 +9,7 @@ package does not.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -26,48 +27,69 @@ def _need(ok: bool, what: str) -> None:
 
 def _rows(t: torch.Tensor, name: str) -> int:
     """Checks a [rows, n] tensor of a supported type with adjacent columns and returns its row stride."""
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, "%s must be a CUDA tensor" % name)
-    _need(t.dtype in _TYPES, "%s must be float32, float16 or bfloat16 (got %s)" % (name, t.dtype))
-    _need(t.dim() == 2, "%s must have two dimensions (got %d)" % (name, t.dim()))
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise TrainerError("%s must be a CUDA tensor" % name)
+    if t.dtype not in _TYPES:
+        raise TrainerError("%s must be float32, float16 or bfloat16 (got %s)" % (name, t.dtype))
+    if t.dim() != 2:
+        raise TrainerError("%s must have two dimensions (got %d)" % (name, t.dim()))
     rows, n = t.shape
     stride, step = t.stride()
-    _need(n <= 1 or step == 1, "%s must have adjacent columns" % name)
-    _need(rows <= 1 or stride >= n, "rows of %s overlap" % name)
-    return stride if rows > 1 else max(stride, n)
+    if n > 1 and step != 1:
+        raise TrainerError("%s must have adjacent columns" % name)
+    if rows <= 1:
+        return n
+    if stride < n:
+        raise TrainerError("rows of %s overlap" % name)
+    return stride
 
 
 def _vector(t: Optional[torch.Tensor], name: str, like: torch.Tensor, shape: Tuple[int, ...], dtype=torch.float32) -> Optional[int]:
     """Checks a contiguous tensor beside `like` and returns its address (None for None)."""
     if t is None:
         return None
-    _need(isinstance(t, torch.Tensor) and t.device == like.device, "%s must be on %s" % (name, like.device))
-    _need(t.dtype == dtype and t.shape == shape and t.is_contiguous(), "%s must be a contiguous %s tensor of shape %s" % (name, dtype, tuple(shape)))
+    if not (isinstance(t, torch.Tensor) and t.device == like.device):
+        raise TrainerError("%s must be on %s" % (name, like.device))
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise TrainerError("%s must be a contiguous %s tensor of shape %s" % (name, dtype, tuple(shape)))
     return t.data_ptr()
 
 
-class _On:
-    """Makes a tensor's device current where it is not."""
-    __slots__ = ("was", "index")
-
-    def __init__(self, t: torch.Tensor):
-        self.index = t.device.index
-
-    def __enter__(self):
-        self.was = torch.cuda.current_device()
-        if self.was != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.was != self.index:
-            torch.cuda.set_device(self.was)
+# torch.cuda.current_stream() builds an object in 3 us; the handle alone costs 0.1
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_local = threading.local()
 
 
-def _call(name: str, *args) -> None:
-    err = C.create_string_buffer(256)
-    rc = getattr(L.load(), name)(*args, err, 256)
-    if rc != L.TB_OK:
-        raise TrainerError("%s failed (%d): %s" % (name, rc, err.value.decode("utf-8", "replace")))
+def _call(name: str, like: torch.Tensor, *args) -> None:
+    """Calls an entry point with the tensors' device current, on torch's current stream of it."""
+    index = like.device.index
+    was = torch.cuda.current_device()
+    if was != index:
+        torch.cuda.set_device(index)
+    try:
+        err = getattr(_local, "err", None)
+        if err is None:
+            err = _local.err = C.create_string_buffer(256)
+        rc = getattr(L.load(), name)(*args, _raw_stream(index), err, 256)
+        if rc != L.TB_OK:
+            raise TrainerError("%s failed (%d): %s" % (name, rc, err.value.decode("utf-8", "replace")))
+    finally:
+        if was != index:
+            torch.cuda.set_device(was)
+
+
+def _work(name: str, like: torch.Tensor, *args) -> Tuple[Optional[torch.Tensor], int]:
+    """A workspace of the size that an entry point asks for, and the size (sizes that it refuses are left to the call itself)."""
+    index = like.device.index
+    was = torch.cuda.current_device()
+    if was != index:
+        torch.cuda.set_device(index)
+    try:
+        size = getattr(L.load(), name)(*args)
+    finally:
+        if was != index:
+            torch.cuda.set_device(was)
+    return (like.new_empty(size, dtype=torch.uint8), size) if size > 0 else (None, 0)
 
 
 # ---- layer norm -------------------------------------------------------------------------------------------------------
@@ -80,13 +102,13 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
     """
     xs = _rows(x, "x")
     rows, n = x.shape
-    y = torch.empty((rows, n), dtype=x.dtype, device=x.device) if out is None else out
+    y = x.new_empty((rows, n)) if out is None else out
     ys = n if out is None else _rows(out, "out")
     _need(out is None or (out.shape == x.shape and out.dtype == x.dtype and out.device == x.device), "out must match x")
     w, b = _vector(weight, "weight", x, (n,)), _vector(bias, "bias", x, (n,))
-    mean, rstd = torch.empty(rows, dtype=torch.float32, device=x.device), torch.empty(rows, dtype=torch.float32, device=x.device)
-    with _On(x) as stream:
-        _call("tb_layer_norm_forward", x.data_ptr(), xs, w, b, eps, _TYPES[x.dtype], rows, n, y.data_ptr(), ys, mean.data_ptr(), rstd.data_ptr(), stream)
+    mean = x.new_empty(rows, dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    _call("tb_layer_norm_forward", x, x.data_ptr(), xs, w, b, eps, _TYPES[x.dtype], rows, n, y.data_ptr(), ys, mean.data_ptr(), rstd.data_ptr())
     return y, mean, rstd
 
 
@@ -97,17 +119,15 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     rows, n = x.shape
     _need(dy.shape == x.shape and dy.dtype == x.dtype and dy.device == x.device, "dy must match x")
     m, r, w = _vector(mean, "mean", x, (rows,)), _vector(rstd, "rstd", x, (rows,)), _vector(weight, "weight", x, (n,))
-    dx = torch.empty((rows, n), dtype=x.dtype, device=x.device) if out is None else out
+    dx = x.new_empty((rows, n)) if out is None else out
     ds = n if out is None else _rows(out, "out")
     _need(out is None or (out.shape == x.shape and out.dtype == x.dtype and out.device == x.device), "out must match x")
-    d = torch.empty((2, n), dtype=torch.float32, device=x.device)
-    with _On(x) as stream:
-        size = L.load().tb_layer_norm_backward_workspace(rows, n)
-        work = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)
-        p = d.data_ptr()
-        _call("tb_layer_norm_backward", dy.data_ptr(), gs, x.data_ptr(), xs, m, r, w, _TYPES[x.dtype], rows, n, dx.data_ptr(), ds, p, p + 4 * n,
-              work.data_ptr(), size, stream)
-    return dx, d[0], d[1]
+    dweight = x.new_empty(n, dtype=torch.float32)
+    dbias = torch.empty_like(dweight)
+    work, size = _work("tb_layer_norm_backward_workspace", x, rows, n)
+    _call("tb_layer_norm_backward", x, dy.data_ptr(), gs, x.data_ptr(), xs, m, r, w, _TYPES[x.dtype], rows, n, dx.data_ptr(), ds, dweight.data_ptr(),
+          dbias.data_ptr(), None if work is None else work.data_ptr(), size)
+    return dx, dweight, dbias
 
 
 # ---- routing ----------------------------------------------------------------------------------------------------------
@@ -136,18 +156,15 @@ def route_forward(logits: torch.Tensor, k: int, *, renormalise: bool = True, mas
     """
     stride = _rows(logits, "logits")
     rows, experts = logits.shape
-    dev = logits.device
     m = _mask(mask, logits, rows)
     _need(1 <= k, "k must be positive")
-    index, gate = torch.empty((rows, k), dtype=torch.int32, device=dev), torch.empty((rows, k), dtype=torch.float32, device=dev)
-    whole, real = torch.empty(experts + 1, dtype=torch.int32, device=dev), torch.empty(experts + 2, dtype=torch.float32, device=dev)
-    with _On(logits) as stream:
-        size = L.load().tb_route_forward_workspace(rows, experts)
-        work = torch.empty(max(size, 1), dtype=torch.uint8, device=dev)
-        c, p = whole.data_ptr(), real.data_ptr()
-        _call("tb_route_forward", logits.data_ptr(), stride, _TYPES[logits.dtype], rows, experts, k, renormalise, m, index.data_ptr(), gate.data_ptr(), c,
-              c + 4 * experts, p, p + 4 * experts, work.data_ptr(), size, stream)
-    return Routing(index, gate, whole[:experts], whole[experts:], real[:experts], real[experts:])
+    index, gate = logits.new_empty((rows, k), dtype=torch.int32), logits.new_empty((rows, k), dtype=torch.float32)
+    counts, n = logits.new_empty(experts, dtype=torch.int32), logits.new_empty(1, dtype=torch.int32)
+    mean, losses = logits.new_empty(experts, dtype=torch.float32), logits.new_empty(2, dtype=torch.float32)
+    work, size = _work("tb_route_forward_workspace", logits, rows, experts)
+    _call("tb_route_forward", logits, logits.data_ptr(), stride, _TYPES[logits.dtype], rows, experts, k, renormalise, m, index.data_ptr(), gate.data_ptr(),
+          counts.data_ptr(), n.data_ptr(), mean.data_ptr(), losses.data_ptr(), None if work is None else work.data_ptr(), size)
+    return Routing(index, gate, counts, n, mean, losses)
 
 
 def route_backward(logits: torch.Tensor, routing: Routing, dgate: Optional[torch.Tensor] = None, dlosses: Optional[torch.Tensor] = None, *,
@@ -163,10 +180,9 @@ def route_backward(logits: torch.Tensor, routing: Routing, dgate: Optional[torch
     g, dg = _vector(routing.gate, "routing.gate", logits, (rows, k)), _vector(dgate, "dgate", logits, (rows, k))
     c, n = _vector(routing.counts, "routing.counts", logits, (experts,), torch.int32), _vector(routing.rows, "routing.rows", logits, (1,), torch.int32)
     dl = _vector(dlosses, "dlosses", logits, (2,))
-    out = torch.empty((rows, experts), dtype=logits.dtype, device=logits.device)
-    with _On(logits) as stream:
-        _call("tb_route_backward", logits.data_ptr(), stride, _TYPES[logits.dtype], rows, experts, k, renormalise, m, ix, g, dg, c, n, dl, out.data_ptr(),
-              experts, stream)
+    out = logits.new_empty((rows, experts))
+    _call("tb_route_backward", logits, logits.data_ptr(), stride, _TYPES[logits.dtype], rows, experts, k, renormalise, m, ix, g, dg, c, n, dl, out.data_ptr(),
+          experts)
     return out
 
 
@@ -197,16 +213,14 @@ def orthogonalise(x: torch.Tensor, *, steps: int = 5, coefficients: Tuple[float,
     tiny end near 1, the singular vectors stay.  `out` may be x.
     """
     batch, rows, cols, xb, xs = _matrices(x, "x")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    y = x.new_empty(x.shape) if out is None else out
     _need(out is None or (isinstance(out, torch.Tensor) and out.shape == x.shape and out.dtype == x.dtype and out.device == x.device), "out must match x")
     _, _, _, yb, ys = _matrices(y, "out")
     _need(len(coefficients) == 3, "three coefficients are needed")
     kind = _TYPES[x.dtype]
-    with _On(x) as stream:
-        size = L.load().tb_orthogonalise_workspace(kind, batch, rows, cols)
-        work = torch.empty(size, dtype=torch.uint8, device=x.device) if size > 0 else None
-        _call("tb_orthogonalise", x.data_ptr(), xb, xs, kind, batch, rows, cols, steps, (C.c_float * 3)(*coefficients), eps, y.data_ptr(), yb, ys,
-              None if work is None else work.data_ptr(), max(size, 0), stream)
+    work, size = _work("tb_orthogonalise_workspace", x, kind, batch, rows, cols)
+    _call("tb_orthogonalise", x, x.data_ptr(), xb, xs, kind, batch, rows, cols, steps, (C.c_float * 3)(*coefficients), eps, y.data_ptr(), yb, ys,
+          None if work is None else work.data_ptr(), size)
     return y
 
 
@@ -230,8 +244,6 @@ def muon_step(weight: torch.Tensor, momentum: torch.Tensor, grad: torch.Tensor, 
         scale = max(1.0, rows / cols) ** 0.5
     _need(len(coefficients) == 3, "three coefficients are needed")
     cfg = L.Muon(C.sizeof(L.Muon), steps, nesterov, *coefficients, eps, lr, beta, weight_decay, scale, clip)
-    with _On(weight) as stream:
-        size = L.load().tb_muon_step_workspace(batch, rows, cols)
-        work = torch.empty(size, dtype=torch.uint8, device=weight.device) if size > 0 else None
-        _call("tb_muon_step", C.byref(cfg), w, m, g, _TYPES[grad.dtype], batch, rows, cols, wo, mo, None if work is None else work.data_ptr(), max(size, 0), stream)
+    work, size = _work("tb_muon_step_workspace", weight, batch, rows, cols)
+    _call("tb_muon_step", weight, C.byref(cfg), w, m, g, _TYPES[grad.dtype], batch, rows, cols, wo, mo, None if work is None else work.data_ptr(), size)
     return weight_out, momentum_out
