@@ -39,14 +39,15 @@ static __device__ __forceinline__ float orth_load(const OrthIo& io, int b, int64
     }
     return io.nesterov ? fmaf(io.beta, m, g) : m;
 }
+// x is element (r, c) of the result, w that of the old weights (Muon)
 template <typename T>
-static __device__ __forceinline__ void orth_store(const OrthIo& io, int b, int64_t r, int64_t c, float x) {
+static __device__ __forceinline__ void orth_store(const OrthIo& io, int b, int64_t r, int64_t c, float w, float x) {
     const int64_t at = b * io.out_batch + r * io.out_stride + c;
     if (!io.m) {
         static_cast<T*>(io.out)[at] = op_round<T>(x);
         return;
     }
-    float w = fmaf(-io.step, x, io.w[at] * io.w_mul);
+    w = fmaf(-io.step, x, w * io.w_mul);
     w = w < -io.clip ? -io.clip : w;  // comparisons keep a NaN
     w = w > io.clip ? io.clip : w;
     static_cast<float*>(io.out)[at] = w;

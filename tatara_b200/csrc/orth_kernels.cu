@@ -9,173 +9,209 @@
 // singular value 1e-3 of the largest would lose 1e-2 of itself with fp32 sums, here nothing is lost.  What bounds it is latency: a cluster
 // of CTAs shares the long side of a matrix, every CTA adds up the CTAs' Gram matrices (distributed shared memory, in order) and
 // runs the steps by itself, which costs less than telling the others.  All matrices are polynomials of one symmetric matrix, so they are
-// symmetric and commute: half of every product is computed.  A fixed order everywhere: results repeat bit for bit.
+// symmetric and commute: half of every product is computed.  The products are the tensor cores' 64-bit ones (8 x 8 x 4 per warp): a step of
+// 32 x 32 matrices waits for a chain of four of them where thread-wise sums wait for sixteen additions and four times the shared-memory
+// reads.  A fixed order everywhere: results repeat bit for bit.
 #include "orth.cuh"
 
 #include <cooperative_groups.h>
+
+#include <atomic>
 
 namespace cg = cooperative_groups;
 
 namespace {
 
-#define SMALL_THREADS 256
-#define SMALL_CHUNK 4096  // doubles of a chunk of columns in shared memory
+#define SMALL_THREADS 320
+#define SMALL_WARPS 10
+#define SMALL_CLUSTER 16   // most CTAs that share a matrix
+#define SMALL_SMEM 229376  // 224 KB
+#define SMALL_BATCH 8      // elements a thread has on their way at once
 
-// TS x TS entries of a symmetric product per thread; pitch: of the matrices' rows
-template <int TS>
-__device__ __forceinline__ void small_product(const double* __restrict__ x, const double* __restrict__ y, double* __restrict__ out, int np, int pitch, int ti, int tj,
-                                              double scale, double ident, const double* __restrict__ add, double add_scale) {
-    double acc[TS][TS];
+// rows of 64-bit matrices start 4 doubles apart modulo 16: the 4 x 8 operands below touch every bank once
+__host__ __device__ constexpr int small_pitch(int np) { return (np + 11) / 16 * 16 + 4; }
+
+// C (8 x 8) += A (8 x 4) B (4 x 8) in 64 bits; lane l holds A[l / 4][l % 4], B[l % 4][l / 4], C[l / 4][2 (l % 4) + {0, 1}]
+__device__ __forceinline__ void small_mma(double (&c)[2], double a, double b) {
+    asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};" : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
+}
+
+// the lower triangle's block of a linear index: t = bi (bi + 1) / 2 + bj
+__device__ __forceinline__ void small_block(int t, int& bi, int& bj) {
+    bi = 0;
+    while ((bi + 1) * (bi + 2) / 2 <= t) ++bi;
+    bj = t - bi * (bi + 1) / 2;
+}
+
+// Block (bi, bj) of out = x y or, with LINEAR, scale x y + linear x + ident I, by one warp, and its mirror image: the matrices are symmetric and
+// commute.  Two chains; what does not depend on them is ready when they are (a 64-bit addition takes as long as a quarter of the chain).
+template <bool LINEAR>
+__device__ __forceinline__ void small_product(const double* __restrict__ x, const double* __restrict__ y, double* __restrict__ out, int np, int pitch, int block, int lane,
+                                              double scale, double linear, double ident) {
+    const int bi = block >> 8, bj = block & 255, i = bi * 8 + (lane >> 2), j = bj * 8 + 2 * (lane & 3);
+    const double *a = x + (lane & 3) * pitch + i, *b = y + (lane & 3) * pitch + bj * 8 + (lane >> 2);
+    double c[2][2] = {{0.0, 0.0}, {0.0, 0.0}}, rest[2] = {0.0, 0.0};
+    if (LINEAR)
 #pragma unroll
-    for (int r = 0; r < TS; ++r)
-#pragma unroll
-        for (int c = 0; c < TS; ++c) acc[r][c] = 0.0;
-    if (ti >= 0) {
+        for (int q = 0; q < 2; ++q) rest[q] = fma(linear, x[i * pitch + j + q], i == j + q ? ident : 0.0);
 #pragma unroll 4
-        for (int k = 0; k < np; ++k) {
-            double a[TS], b[TS];
+    for (int k = 0; k < np; k += 8, a += 8 * pitch, b += 8 * pitch) {
+        small_mma(c[0], a[0], b[0]);
+        small_mma(c[1], a[4 * pitch], b[4 * pitch]);
+    }
 #pragma unroll
-            for (int r = 0; r < TS; ++r) a[r] = x[k * pitch + ti * TS + r];
+    for (int q = 0; q < 2; ++q) {
+        const double v = LINEAR ? fma(scale, c[0][q], fma(scale, c[1][q], rest[q])) : c[0][q] + c[1][q];
+        if (i >= j + q) {
+            out[i * pitch + j + q] = v;
+            out[(j + q) * pitch + i] = v;
+        }
+    }
+}
+
+// columns [j0, j0 + jc) of a matrix into xs[j][pitch] (64 bits); rows n .. np - 1 and columns jc .. jp - 1 are zero.  Neighbours in memory go to
+// neighbouring threads; all loads of a batch are issued before the first is used (one at a time this was half of the kernel).
+template <typename T, bool FIRST>
+__device__ __forceinline__ void small_fill(const OrthIo& io, int b, int n, int np, bool tall, int64_t j0, int jc, int jp, double* xs, int pitch) {
+    const int total = np * jp, inner = tall ? np : jp;
+    const unsigned magic = (unsigned)((0x100000000ull + inner - 1) / inner);  // e / inner = e * magic >> 32 for e * inner < 2^32
+    for (int e0 = threadIdx.x; e0 < total; e0 += SMALL_THREADS * SMALL_BATCH) {
+        float g[SMALL_BATCH], m[SMALL_BATCH];
+        int64_t at[SMALL_BATCH];
+        int to[SMALL_BATCH];
 #pragma unroll
-            for (int c = 0; c < TS; ++c) b[c] = y[k * pitch + tj * TS + c];
-#pragma unroll
-            for (int r = 0; r < TS; ++r)
-#pragma unroll
-                for (int c = 0; c < TS; ++c) acc[r][c] = fma(a[r], b[c], acc[r][c]);
+        for (int u = 0; u < SMALL_BATCH; ++u) {
+            const int e = e0 + u * SMALL_THREADS;
+            const int hi = (int)__umulhi((unsigned)e, magic), lo = e - hi * inner;
+            const int i = tall ? lo : hi, j = tall ? hi : lo;
+            to[u] = e < total ? j * pitch + i : -1;
+            at[u] = -1;
+            g[u] = m[u] = 0.0f;
+            if (e < total && i < n && j < jc) {
+                const int64_t r = tall ? j0 + j : i, c = tall ? i : j0 + j;
+                g[u] = op_float(static_cast<const T*>(io.g)[b * io.g_batch + r * io.g_stride + c]);
+                if (io.m) {
+                    at[u] = ((int64_t)b * io.rows + r) * io.cols + c;
+                    m[u] = FIRST ? io.m[at[u]] : io.m_out[at[u]];
+                }
+            }
         }
 #pragma unroll
-        for (int r = 0; r < TS; ++r)
-#pragma unroll
-            for (int c = 0; c < TS; ++c) {
-                const int i = ti * TS + r, j = tj * TS + c;
-                double v = acc[r][c] * scale;
-                if (add) v = fma(add_scale, add[i * pitch + j], v);
-                if (i == j) v += ident;
-                out[i * pitch + j] = v;
-                out[j * pitch + i] = v;
+        for (int u = 0; u < SMALL_BATCH; ++u) {
+            float v = g[u];
+            if (at[u] >= 0) {
+                if (FIRST) {
+                    m[u] = fmaf(io.beta, m[u], g[u]);
+                    io.m_out[at[u]] = m[u];
+                }
+                v = io.nesterov ? fmaf(io.beta, m[u], g[u]) : m[u];
             }
+            if (to[u] >= 0) xs[to[u]] = (double)v;
+        }
     }
 }
 
-// the lower triangle's tile of a linear index: t = ti (ti + 1) / 2 + tj
-__device__ __forceinline__ void small_tile(int t, int& ti, int& tj) {
-    ti = 0;
-    while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
-    tj = t - ti * (ti + 1) / 2;
-}
-
-// columns [j0, j0 + jc) of a matrix into xs[j][pitch] (64 bits); rows n .. np - 1 are zero
-template <typename T, bool FIRST>
-__device__ __forceinline__ void small_fill(const OrthIo& io, int b, int n, int np, bool tall, int64_t j0, int jc, double* xs, int pitch) {
-    for (int e = threadIdx.x; e < np * jc; e += SMALL_THREADS) {
-        // neighbours in memory go to neighbouring threads
-        const int i = tall ? e % np : e / jc, j = tall ? e / np : e % jc;
-        double v = 0.0;
-        if (i < n) v = (double)(tall ? orth_load<T, FIRST>(io, b, j0 + j, i) : orth_load<T, FIRST>(io, b, i, j0 + j));
-        xs[j * pitch + i] = v;
-    }
-}
-
-// TS: side of a thread's part of the n x n products
-template <typename T, int TS>
-__global__ void __launch_bounds__(SMALL_THREADS) k_orth_small(OrthIo io, OrthPoly poly) {
+// jc_max: columns of a chunk in shared memory, a multiple of 8
+template <typename T>
+__global__ void __launch_bounds__(SMALL_THREADS) k_orth_small(OrthIo io, OrthPoly poly, int jc_max) {
     extern __shared__ double s_mem[];
     cg::cluster_group cluster = cg::this_cluster();
-    const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.y, tid = threadIdx.x;
+    const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const bool tall = io.rows > io.cols;
     const int n = tall ? io.cols : io.rows;
     const int64_t m = tall ? io.rows : io.cols;
-    const int np = (n + 3) / 4 * 4, pitch = np + 2;  // rows of matrices start two banks apart
-    const int xp = np + 1;                           // pitch of the columns' chunk
-    const int jc_max = SMALL_CHUNK / np;
-    double* s_x = s_mem;                            // [jc_max][xp], also the partial sums
-    double* s_own = s_x + SMALL_CHUNK + jc_max;     // this CTA's Gram matrix, read by the others
-    double* s_a = s_own + np * pitch;
-    double* s_q = s_a + np * pitch;
-    double* s_p = s_q + np * pitch;
-    double* s_t = s_p + np * pitch;
+    const int np = (n + 7) / 8 * 8, pitch = small_pitch(np), size = np * pitch, side = np / 8, blocks = side * (side + 1) / 2;
+    double* s_x = s_mem;                     // [jc_max][pitch]
+    double* s_own = s_x + jc_max * pitch;    // this CTA's Gram matrix by blocks [blocks][64], read by the others
+    double* s_a = s_own + size;
+    double* s_q = s_a + size;
+    double* s_p = s_q + size;
+    double* s_t = s_p + size;
+    double* s_part = s_q;                    // partial sums of the Gram matrix
     const int64_t per = (m + cs - 1) / cs, begin = min(m, per * rank), end = min(m, begin + per);
 
-    // Gram matrix of this CTA's columns: 4 x 4 entries per thread, the columns of a chunk dealt to `groups` threads per tile
-    const int tiles4 = (np / 4) * (np / 4 + 1) / 2, groups = min(SMALL_THREADS / tiles4, 32);
-    const int t4 = tid % tiles4, kg = tid / tiles4;
-    int gi, gj;
-    small_tile(t4, gi, gj);
-    double acc[4][4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[r][c] = 0.0;
-    for (int64_t j0 = begin; j0 < end; j0 += jc_max) {
-        const int jc = (int)min((int64_t)jc_max, end - j0);
-        __syncthreads();
-        small_fill<T, true>(io, b, n, np, tall, j0, jc, s_x, xp);
-        __syncthreads();
-        if (kg < groups)
-            for (int j = kg; j < jc; j += groups) {
-                double x[4], y[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = s_x[j * xp + gi * 4 + r];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) y[c] = s_x[j * xp + gj * 4 + c];
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) acc[r][c] = fma(x[r], y[c], acc[r][c]);
-            }
+    __shared__ int s_block[36];  // (bi, bj) of the lower triangle's blocks
+    if (tid < blocks) {
+        int bi, bj;
+        small_block(tid, bi, bj);
+        s_block[tid] = bi << 8 | bj;
     }
-    __syncthreads();
-    if (kg < groups)
+    // Gram matrix of this CTA's columns: a warp per block, or a few per block that share the columns
+    const int splits = blocks < SMALL_WARPS ? SMALL_WARPS / blocks : 1, units = blocks * splits;
+    double gram[4][2];  // of the units warp, warp + 10, ..
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s_x[(e * groups + kg) * tiles4 + t4] = acc[e / 4][e % 4];
-    __syncthreads();
-    for (int e = tid; e < 16 * tiles4; e += SMALL_THREADS) {
-        const int t = e % tiles4, q = e / tiles4;
-        double v = 0.0;
-        for (int k = 0; k < groups; ++k) v += s_x[(q * groups + k) * tiles4 + t];
-        int ti, tj;
-        small_tile(t, ti, tj);
-        const int i = ti * 4 + q / 4, j = tj * 4 + q % 4;
-        s_own[i * pitch + j] = v;
-        s_own[j * pitch + i] = v;
+    for (int u = 0; u < 4; ++u) gram[u][0] = gram[u][1] = 0.0;
+    for (int64_t j0 = begin; j0 < end; j0 += jc_max) {
+        const int jc = (int)min((int64_t)jc_max, end - j0), jp = (jc + 7) / 8 * 8;
+        __syncthreads();
+        small_fill<T, true>(io, b, n, np, tall, j0, jc, jp, s_x, pitch);
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int unit = warp + u * SMALL_WARPS;
+            if (unit >= units) break;
+            const int bi = s_block[unit % blocks] >> 8, bj = s_block[unit % blocks] & 255;
+            const double *x = s_x + (lane & 3) * pitch + bi * 8 + (lane >> 2), *y = s_x + (lane & 3) * pitch + bj * 8 + (lane >> 2);
+#pragma unroll 4
+            for (int j = unit / blocks * 4; j < jp; j += 4 * splits) small_mma(gram[u], x[j * pitch], y[j * pitch]);
+        }
+    }
+    double* gram_to = splits > 1 ? s_part : s_own;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int unit = warp + u * SMALL_WARPS;
+        if (unit < units) *reinterpret_cast<double2*>(gram_to + unit * 64 + lane * 2) = make_double2(gram[u][0], gram[u][1]);
+    }
+    if (splits > 1) {
+        __syncthreads();
+        for (int e = tid; e < blocks * 64; e += SMALL_THREADS) {
+            double v = s_part[e];
+            for (int k = 1; k < splits; ++k) v += s_part[k * blocks * 64 + e];
+            s_own[e] = v;
+        }
     }
     cluster.sync();
-    for (int e = tid; e < np * np; e += SMALL_THREADS) {
-        const int at = (e / np) * pitch + e % np;
-        double v = 0.0;
-        for (int r = 0; r < cs; ++r) v += cluster.map_shared_rank(s_own, r)[at];
-        s_a[at] = v;
+    // every CTA adds up its share of the entries over the CTAs, in order, and hands the sums to all
+    for (int e = blocks * 32 * rank / cs + tid; e < blocks * 32 * (rank + 1) / cs; e += SMALL_THREADS) {
+        double2 part[SMALL_CLUSTER], v = make_double2(0.0, 0.0);
+#pragma unroll
+        for (int r = 0; r < SMALL_CLUSTER; ++r) part[r] = r < cs ? reinterpret_cast<const double2*>(cluster.map_shared_rank(s_own, r))[e] : make_double2(0.0, 0.0);
+#pragma unroll
+        for (int r = 0; r < SMALL_CLUSTER; ++r) {
+            v.x += part[r].x;
+            v.y += part[r].y;
+        }
+        for (int r = 0; r < cs; ++r) reinterpret_cast<double2*>(cluster.map_shared_rank(s_t, r))[e] = v;
     }
-    cluster.sync();  // nobody leaves, or reads on, while another reads its part
-    __shared__ double s_inv;
-    if (tid == 0) {
-        double trace = 0.0;
-        for (int i = 0; i < n; ++i) trace += s_a[i * pitch + i];
-        s_inv = 1.0 / (sqrt(trace) + (double)poly.eps);
+    cluster.sync();  // from here on no CTA touches another's memory
+    double trace = 0.0;
+    for (int i = lane; i < np; i += 32) {
+        const int bi = i >> 3;
+        trace += s_t[(bi * (bi + 1) / 2 + bi) * 64 + (i & 7) * 9];
     }
-    __syncthreads();
-    const double inv = s_inv;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) trace += __shfl_xor_sync(0xffffffffu, trace, o);
     // a matrix of zeros with eps 0: 0 / 0, as the definition says
-    for (int e = tid; e < np * np; e += SMALL_THREADS) {
-        const int at = (e / np) * pitch + e % np;
-        s_a[at] = s_a[at] * inv * inv;
+    const double inv = 1.0 / (sqrt(trace) + (double)poly.eps);
+    for (int e = tid; e < blocks * 64; e += SMALL_THREADS) {
+        const int i = (s_block[e >> 6] >> 8) * 8 + ((e & 63) >> 3), j = (s_block[e >> 6] & 255) * 8 + (e & 7);
+        const double v = s_t[e] * inv * inv;
+        if (i >= j) s_a[i * pitch + j] = s_a[j * pitch + i] = v;
     }
     __syncthreads();
 
-    const int tiles = (np / TS) * (np / TS + 1) / 2;
-    int ti = -1, tj = 0;
-    if (tid < tiles) small_tile(tid, ti, tj);
     for (int s = 0; s < poly.steps; ++s) {
         const bool last = s + 1 == poly.steps;
-        small_product<TS>(s_a, s_a, s_q, np, pitch, ti, tj, poly.c, poly.a, s_a, poly.b);  // Q
+        for (int t = warp; t < blocks; t += SMALL_WARPS) small_product<true>(s_a, s_a, s_q, np, pitch, s_block[t], lane, poly.c, poly.b, poly.a);  // Q
         __syncthreads();
-        // P = Q P (P = Q in the first step) and, unless it is the last, A = (Q A) Q
-        if (s == 0) {
-            for (int e = tid; e < np * pitch; e += SMALL_THREADS) s_p[e] = s_q[e];
-        } else {
-            small_product<TS>(s_q, s_p, s_own, np, pitch, ti, tj, 1.0, 0.0, nullptr, 0.0);
+        // unless it is the last step, A = (Q A) Q; P = Q P (P = Q in the first step)
+        const int first = last ? blocks : 0, total = s == 0 ? blocks : 2 * blocks;
+        for (int t = first + warp; t < total; t += SMALL_WARPS) {
+            if (t < blocks) small_product<false>(s_q, s_a, s_t, np, pitch, s_block[t], lane, 0.0, 0.0, 0.0);
+            else small_product<false>(s_q, s_p, s_own, np, pitch, s_block[t - blocks], lane, 0.0, 0.0, 0.0);
         }
-        if (!last) small_product<TS>(s_q, s_a, s_t, np, pitch, ti, tj, 1.0, 0.0, nullptr, 0.0);
+        if (s == 0)
+            for (int e = tid; e < size; e += SMALL_THREADS) s_p[e] = s_q[e];
         __syncthreads();
         if (s > 0) {
             double* z = s_p;
@@ -183,57 +219,80 @@ __global__ void __launch_bounds__(SMALL_THREADS) k_orth_small(OrthIo io, OrthPol
             s_own = z;
         }
         if (!last) {
-            small_product<TS>(s_t, s_q, s_a, np, pitch, ti, tj, 1.0, 0.0, nullptr, 0.0);
+            for (int t = warp; t < blocks; t += SMALL_WARPS) small_product<false>(s_t, s_q, s_a, np, pitch, s_block[t], lane, 0.0, 0.0, 0.0);
             __syncthreads();
         }
     }
 
-    // out = P U / (|U| + eps): 4 rows and 4 columns (a quarter of the chunk apart) per thread
-    const int row_tiles = np / 4;
+    // out = P U / (|U| + eps), 8 rows x 8 columns per warp
     for (int64_t j0 = begin; j0 < end; j0 += jc_max) {
-        const int jc = (int)min((int64_t)jc_max, end - j0), quarter = (jc + 3) / 4;
-        __syncthreads();
-        small_fill<T, false>(io, b, n, np, tall, j0, jc, s_x, xp);
-        __syncthreads();
-        for (int t = tid; t < row_tiles * quarter; t += SMALL_THREADS) {
-            const int it = tall ? t % row_tiles : t / quarter, jt = tall ? t / row_tiles : t % quarter;
-            double o[4][4];
+        const int jc = (int)min((int64_t)jc_max, end - j0), jp = (jc + 7) / 8 * 8;
+        if (end - begin > jc_max) {  // else they are still there
+            __syncthreads();
+            small_fill<T, false>(io, b, n, np, tall, j0, jc, jp, s_x, pitch);
+            __syncthreads();
+        }
+        for (int t = warp; t < side * (jp / 8); t += SMALL_WARPS) {
+            const int bi = t % side, bj = t / side, i = bi * 8 + (lane >> 2), j = bj * 8 + 2 * (lane & 3);
+            float w[2];
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) o[r][c] = 0.0;
-            for (int k = 0; k < n; ++k) {
-                double p[4], x[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) p[r] = s_p[k * pitch + it * 4 + r];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) x[c] = s_x[min(jt + c * quarter, jc - 1) * xp + k];
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) o[r][c] = fma(p[r], x[c], o[r][c]);
+            for (int q = 0; q < 2; ++q)
+                w[q] = io.m && i < n && j + q < jc ? io.w[b * io.out_batch + (tall ? (j0 + j + q) * io.out_stride + i : i * io.out_stride + j0 + j + q)] : 0.0f;
+            const double *p = s_p + (lane & 3) * pitch + bi * 8 + (lane >> 2), *x = s_x + (bj * 8 + (lane >> 2)) * pitch + (lane & 3);
+            double c[2][2] = {{0.0, 0.0}, {0.0, 0.0}};
+#pragma unroll 4
+            for (int k = 0; k < np; k += 8) {
+                small_mma(c[0], p[k * pitch], x[k]);
+                small_mma(c[1], p[(k + 4) * pitch], x[k + 4]);
             }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int j = jt + c * quarter;
-                if (j >= jc) continue;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = it * 4 + r;
-                    if (i >= n) continue;
-                    const float v = (float)(o[r][c] * inv);
-                    if (tall) orth_store<T>(io, b, j0 + j, i, v); else orth_store<T>(io, b, i, j0 + j, v);
-                }
-            }
+            for (int q = 0; q < 2; ++q)
+                if (i < n && j + q < jc) orth_store<T>(io, b, tall ? j0 + j + q : i, tall ? i : j0 + j + q, w[q], (float)((c[0][q] + c[1][q]) * inv));
         }
     }
 }
 
-template <typename T, int TS>
-void orth_small_go(cudaStream_t s, const OrthIo& io, const OrthPoly& p, int cs) {
-    const int n = io.rows < io.cols ? io.rows : io.cols, np = (n + 3) / 4 * 4;
-    const size_t smem = (size_t)(SMALL_CHUNK + SMALL_CHUNK / np + 5 * np * (np + 2)) * sizeof(double);
-    cudaFuncSetAttribute(k_orth_small<T, TS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+// Whether the current device runs clusters of sixteen (which are not portable) at the largest shared memory: asked once per device.
+template <typename T>
+bool small_cluster_fits() {
+    static std::atomic<signed char> known[64];  // 0 not asked, 1 yes, -1 no
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    signed char k = known[dev].load();
+    if (!k) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(SMALL_CLUSTER);
+        cfg.blockDim = dim3(SMALL_THREADS);
+        cfg.dynamicSmemBytes = SMALL_SMEM;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = SMALL_CLUSTER;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        int fit = 0;
+        const bool ok = cudaFuncSetAttribute(k_orth_small<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMALL_SMEM) == cudaSuccess &&
+                        cudaFuncSetAttribute(k_orth_small<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                        cudaOccupancyMaxActiveClusters(&fit, k_orth_small<T>, &cfg) == cudaSuccess && fit >= 1;
+        if (!ok) cudaGetLastError();
+        known[dev].store(k = ok ? 1 : -1);
+    }
+    return k > 0;
+}
+
+template <typename T>
+void orth_small_go(cudaStream_t s, const OrthIo& io, const OrthPoly& p) {
+    const int n = io.rows < io.cols ? io.rows : io.cols, m = io.rows < io.cols ? io.cols : io.rows, np = (n + 7) / 8 * 8, pitch = small_pitch(np);
+    // 32 columns or more per CTA, and no more CTAs than the chip holds at once (sixteen for eight: n = 32, m = 1024 in 16 us for 20)
+    int cs = 1;
+    const int most = small_cluster_fits<T>() ? SMALL_CLUSTER : 8;
+    while (cs < most && cs * 32 < m && (int64_t)io.batch * 2 * cs <= sm_count()) cs *= 2;
+    // a CTA's columns stay in shared memory where they fit beside the matrices; the partial sums take 640 doubles of the matrices
+    const int matrices = np * pitch * 2 + (np * pitch * 3 > 640 ? np * pitch * 3 : 640), room = (SMALL_SMEM / 8 - matrices) / pitch / 8 * 8;
+    const int64_t per = ((int64_t)m + cs - 1) / cs;
+    const int jc_max = per < room ? (int)((per + 7) / 8 * 8) : room;
+    const size_t smem = (size_t)(jc_max * pitch + matrices) * sizeof(double);
+    cudaFuncSetAttribute(k_orth_small<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMALL_SMEM);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)cs, (unsigned)io.batch);
     cfg.blockDim = dim3(SMALL_THREADS);
@@ -245,16 +304,7 @@ void orth_small_go(cudaStream_t s, const OrthIo& io, const OrthPoly& p, int cs) 
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, k_orth_small<T, TS>, io, p);
-}
-template <typename T>
-void orth_small_pick(cudaStream_t s, const OrthIo& io, const OrthPoly& p) {
-    const int n = io.rows < io.cols ? io.rows : io.cols, m = io.rows < io.cols ? io.cols : io.rows;
-    int cs = 1;  // about 64 columns or more per CTA
-    while (cs < 8 && cs * 64 < m) cs *= 2;
-    if (n <= 16) orth_small_go<T, 1>(s, io, p, cs);
-    else if (n <= 32) orth_small_go<T, 2>(s, io, p, cs);
-    else orth_small_go<T, 4>(s, io, p, cs);
+    cudaLaunchKernelEx(&cfg, k_orth_small<T>, io, p, jc_max);
 }
 
 // The limbs hold numbers up to 32 (orth_tc.cu); fp16 inputs' results are rounded to 11 bits, bf16's to 8: one limb of 11 bits is
@@ -310,9 +360,9 @@ int orth_run(const OrthIo& io, const OrthPoly& p, int type, int limbs, void* wor
 }  // namespace
 
 void launch_orth_small(cudaStream_t s, const OrthIo& io, const OrthPoly& p, int type) {
-    if (type == TB_TYPE_F32) orth_small_pick<float>(s, io, p);
-    else if (type == TB_TYPE_F16) orth_small_pick<__half>(s, io, p);
-    else orth_small_pick<__nv_bfloat16>(s, io, p);
+    if (type == TB_TYPE_F32) orth_small_go<float>(s, io, p);
+    else if (type == TB_TYPE_F16) orth_small_go<__half>(s, io, p);
+    else orth_small_go<__nv_bfloat16>(s, io, p);
 }
 
 extern "C" int64_t tb_orthogonalise_workspace(int type, int batch, int rows, int cols) {

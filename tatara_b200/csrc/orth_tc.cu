@@ -386,11 +386,19 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
             asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
             const bool tall = io.rows > io.cols;
             const int n = tall ? io.cols : io.rows, m = tall ? io.rows : io.cols;
-            // 128 (64) neighbours in memory at a time
-            for (int e = 0; e < 64; ++e) {
-                const int r = tall ? row : 2 * e + (row >> 6), c = tall ? e : row & 63, i = row_tile * 128 + r, j = col_tile * 64 + c;
-                if (i >= n || j >= m) continue;
-                if (tall) orth_store<T>(io, batch, j, i, flat[r * 65 + c]); else orth_store<T>(io, batch, i, j, flat[r * 65 + c]);
+            // 128 (64) neighbours in memory at a time, eight of a thread's old weights on their way
+            for (int e0 = 0; e0 < 64; e0 += 8) {
+                float w[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int e = e0 + u, i = row_tile * 128 + (tall ? row : 2 * e + (row >> 6)), j = col_tile * 64 + (tall ? e : row & 63);
+                    w[u] = io.m && i < n && j < m ? io.w[batch * io.out_batch + (tall ? j * io.out_stride + i : i * io.out_stride + j)] : 0.0f;
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int e = e0 + u, r = tall ? row : 2 * e + (row >> 6), c = tall ? e : row & 63, i = row_tile * 128 + r, j = col_tile * 64 + c;
+                    if (i < n && j < m) orth_store<T>(io, batch, tall ? j : i, tall ? i : j, w[u], flat[r * 65 + c]);
+                }
             }
         } else {
             const uint8_t* old = KIND == OT_SQUARE ? g.a + (int64_t)batch * LIMBS * g.a_limb + ((int64_t)row_tile * chunks + col_tile) * OT_TILE : nullptr;
