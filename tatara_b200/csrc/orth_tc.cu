@@ -27,7 +27,7 @@ namespace {
 #define OT_SCALE 2048.0f
 #define OT_UNSCALE (1.0f / (2048.0f * 2048.0f))
 #define OT_WAIT_LIMIT (1 << 20)
-#define OT_NORM_BLOCKS 64       // partial sums of squares per matrix
+#define OT_NORM_BLOCKS 512      // most partial sums of squares per matrix
 enum { OT_GRAM = 0, OT_SQUARE = 1, OT_APPLY = 2, OT_LAST = 3 };
 
 __device__ __forceinline__ unsigned ot_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -50,7 +50,11 @@ __device__ __forceinline__ void ot_expect(unsigned bar, unsigned bytes) {
 __device__ __forceinline__ void ot_copy(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-// the same where blocks of the cluster arrive
+// Launches of a call overlap (programmatic dependent launch): a kernel may start before the one ahead of it has finished, and waits for it before
+// it touches global memory.
+__device__ __forceinline__ void ot_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void ot_next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// ot_wait where blocks of the cluster arrive
 __device__ __forceinline__ bool ot_wait_cluster(unsigned bar, unsigned parity) {
     for (int i = 0; i < OT_WAIT_LIMIT; ++i) {
         unsigned ok;
@@ -75,6 +79,12 @@ __device__ __forceinline__ void ot_cluster_sync() {
 }
 __device__ __forceinline__ void ot_store(void* dst, unsigned src, unsigned bytes) {
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+// true in one lane of a whole warp, always the same one
+__device__ __forceinline__ bool ot_elect() {
+    unsigned one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
 }
 template <int CTAS>
 __device__ __forceinline__ void ot_mma(unsigned d, unsigned long long da, unsigned long long db, unsigned idesc, unsigned accumulate) {
@@ -120,59 +130,149 @@ __device__ __forceinline__ void ot_split(float x, __half (&h)[LIMBS]) {
 __device__ __forceinline__ int ot_at(int row, int col) { return row * 128 + ((((col >> 3) ^ row) & 7) << 4) + (col & 7) * 2; }
 
 // ---- the norm and the tiles of the first X ----------------------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(512) k_orth_norm(OrthIo io, double* __restrict__ partial) {
-    __shared__ double s_sum[16];
+// N adjacent elements of u at (r, c), the momentum's update included in the FIRST pass; the loads of the gradient and of the momentum are
+// separate from what follows them so that a caller can issue several
+template <typename T, int N>
+struct OtPiece {
+    OpRaw<T, N> g;
+    float m[N];
+    int64_t at;
+    __device__ __forceinline__ void load(const OrthIo& io, const float* momentum, int b, int64_t r, int64_t c) {
+        g.load(static_cast<const T*>(io.g) + b * io.g_batch + r * io.g_stride + c);
+        if (io.m) {
+            at = ((int64_t)b * io.rows + r) * io.cols + c;
+            constexpr int STEP = N < 4 ? N : 4;
+#pragma unroll
+            for (int i = 0; i < N; i += STEP) {
+                float t[STEP];
+                op_load<float, STEP>(momentum + at + i, t);
+#pragma unroll
+                for (int k = 0; k < STEP; ++k) m[i + k] = t[k];
+            }
+        }
+    }
+    template <bool FIRST>
+    __device__ __forceinline__ void finish(const OrthIo& io, float (&u)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = g.get(i);
+        if (!io.m) return;
+        if (FIRST) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) m[i] = fmaf(io.beta, m[i], u[i]);
+            constexpr int STEP = N < 4 ? N : 4;
+#pragma unroll
+            for (int i = 0; i < N; i += STEP) {
+                float t[STEP];
+#pragma unroll
+                for (int k = 0; k < STEP; ++k) t[k] = m[i + k];
+                op_store<float, STEP>(io.m_out + at + i, t);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = io.nesterov ? fmaf(io.beta, m[i], u[i]) : m[i];
+    }
+};
+
+// Sum of squares (64 bits) of a matrix cut into segments of `len` elements (a row, or 4096 of a matrix without gaps), dealt to the blocks; every
+// thread has 16 elements on their way.  64 blocks with one element each took 270 us for 4096 x 4096, 8 times this.
+template <typename T, int N>
+__global__ void __launch_bounds__(256) k_orth_norm(OrthIo io, int64_t segments, int64_t len, int64_t total, double* __restrict__ partial) {
+    __shared__ double s_sum[8];
     const int b = blockIdx.y;
     double sum = 0.0;
-    for (int r = blockIdx.x; r < io.rows; r += gridDim.x)
-        for (int c = threadIdx.x; c < io.cols; c += 512) {
-            const double u = (double)orth_load<T, true>(io, b, r, c);
-            sum = fma(u, u, sum);
+    for (int64_t seg = blockIdx.x; seg < segments; seg += gridDim.x) {
+        const int64_t r = total ? 0 : seg, c0 = total ? seg * len : 0, end = total ? min(total, c0 + len) : len;
+        for (int64_t c = c0 + threadIdx.x * N; c < end; c += 256 * 16) {
+            OtPiece<T, N> piece[16 / N];
+#pragma unroll
+            for (int q = 0; q < 16 / N; ++q)
+                if (c + q * 256 * N < end) piece[q].load(io, io.m, b, r, c + q * 256 * N);
+#pragma unroll
+            for (int q = 0; q < 16 / N; ++q)
+                if (c + q * 256 * N < end) {
+                    float u[N];
+                    piece[q].template finish<true>(io, u);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) sum = fma((double)u[i], (double)u[i], sum);
+                }
         }
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) sum += s_sum[w];
+        for (int w = 1; w < 8; ++w) sum += s_sum[w];
         partial[b * OT_NORM_BLOCKS + blockIdx.x] = sum;
     }
+    ot_next_may_start();
 }
 
-// one tile per block: X0 = u / (|u| + eps), n x m with n <= m, zeros beyond both
-template <typename T, int LIMBS>
+// One tile per block: X0 = u / (|u| + eps), n x m with n <= m, zeros beyond both.  A thread makes 16-byte pieces of the tile: of N adjacent elements each
+// where rows of u are rows of X, of eight rows of u where they are columns (TALL), through shared memory then.
+template <typename T, int LIMBS, int N, bool TALL>
 __global__ void __launch_bounds__(256) k_orth_pack(OrthIo io, float eps, const double* __restrict__ partial, int n_partial, uint8_t* __restrict__ x, int64_t limb_bytes) {
-    __shared__ __align__(128) uint8_t s_tile[LIMBS][OT_TILE];
-    __shared__ double s_inv;
+    __shared__ __align__(128) uint8_t s_tile[TALL ? LIMBS : 1][TALL ? OT_TILE : 16];
+    __shared__ double s_part[8];
     const int b = blockIdx.z;
-    const bool tall = io.rows > io.cols;
-    const int n = tall ? io.cols : io.rows, m = tall ? io.rows : io.cols;
-    if (threadIdx.x < 32) {
-        double v = 0.0;
-        for (int i = threadIdx.x; i < n_partial; i += 32) v += partial[b * OT_NORM_BLOCKS + i];
+    const int n = TALL ? io.cols : io.rows, m = TALL ? io.rows : io.cols;
+    ot_wait_for_previous();
+    ot_next_may_start();
+    double v = 0.0;
+    for (int i = threadIdx.x; i < n_partial; i += 256) v += partial[b * OT_NORM_BLOCKS + i];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (threadIdx.x == 0) s_inv = (double)OT_SCALE / (sqrt(v) + (double)eps);
-    }
-    __syncthreads();
-    const double inv = s_inv;
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = v;
     const int i0 = blockIdx.y * 128, j0 = blockIdx.x * 64;
-    for (int e = threadIdx.x; e < 128 * 64; e += 256) {
-        const int i = tall ? e % 128 : e / 64, j = tall ? e / 128 : e % 64;
-        float v = 0.0f;
-        if (i0 + i < n && j0 + j < m) v = (float)((double)(tall ? orth_load<T, false>(io, b, j0 + j, i0 + i) : orth_load<T, false>(io, b, i0 + i, j0 + j)) * inv);
-        __half h[LIMBS];
-        ot_split<LIMBS>(v, h);
-#pragma unroll
-        for (int l = 0; l < LIMBS; ++l) *reinterpret_cast<__half*>(&s_tile[l][ot_at(i, j)]) = h[l];
-    }
-    __syncthreads();
     uint8_t* to = x + (int64_t)b * LIMBS * limb_bytes + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * OT_TILE;
+    constexpr int P = 8 / N;  // accesses of a piece
+    double inv = 0.0;
+#pragma unroll 1
+    for (int e = threadIdx.x; e < 128 * 8; e += 256) {
+        const int i = TALL ? e % 128 : e / 8, j = TALL ? e / 128 * 8 : e % 8 * 8;
+        OtPiece<T, N> piece[P];
 #pragma unroll
-    for (int l = 0; l < LIMBS; ++l)
-        for (int e = threadIdx.x; e < OT_TILE / 16; e += 256)
-            *reinterpret_cast<uint4*>(to + l * limb_bytes + e * 16) = *reinterpret_cast<const uint4*>(&s_tile[l][e * 16]);
+        for (int q = 0; q < P; ++q) {
+            const bool in = i0 + i < n && j0 + j + q * N < m;
+            if (in) piece[q].load(io, io.m_out, b, TALL ? j0 + j + q : i0 + i, TALL ? i0 + i : j0 + j + q * N);
+        }
+        if (e == threadIdx.x) {
+            __syncthreads();
+            v = s_part[0];
+#pragma unroll
+            for (int w = 1; w < 8; ++w) v += s_part[w];
+            inv = (double)OT_SCALE / (sqrt(v) + (double)eps);
+        }
+        OpVec<__half, 8> out[LIMBS];
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+            float u[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) u[k] = 0.0f;
+            if (i0 + i < n && j0 + j + q * N < m) {
+                piece[q].template finish<false>(io, u);
+#pragma unroll
+                for (int k = 0; k < N; ++k) u[k] = (float)((double)u[k] * inv);
+            }
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                __half h[LIMBS];
+                ot_split<LIMBS>(u[k], h);
+#pragma unroll
+                for (int l = 0; l < LIMBS; ++l) out[l].v[q * N + k] = h[l];
+            }
+        }
+#pragma unroll
+        for (int l = 0; l < LIMBS; ++l)
+            *reinterpret_cast<OpVec<__half, 8>*>((TALL ? &s_tile[l][0] : to + l * limb_bytes) + ot_at(i, j)) = out[l];
+    }
+    if (TALL) {
+        __syncthreads();
+#pragma unroll
+        for (int l = 0; l < LIMBS; ++l)
+            for (int e = threadIdx.x; e < OT_TILE / 16; e += 256)
+                *reinterpret_cast<uint4*>(to + l * limb_bytes + e * 16) = *reinterpret_cast<const uint4*>(&s_tile[l][e * 16]);
+    }
 }
 
 // ---- the products -----------------------------------------------------------------------------------------------------
@@ -210,7 +310,8 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
     __shared__ int s_failed;
     uint8_t* s_dyn = s_raw + ((1024u - (ot_smem(s_raw) & 1023u)) & 1023u);
     const unsigned ring = ot_smem(s_dyn);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, batch = blockIdx.z;
+    // the warp's number is the same in its lanes, and the compiler has to know it: what the MMAs take lives in uniform registers then
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, batch = blockIdx.z;
     const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, tile = blockIdx.x / CTAS;
     int ti, tj;
     if (SYM) {  // tiles on and below the diagonal, row by row
@@ -251,88 +352,107 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
     __syncthreads();
     if (CTAS == 2) ot_cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    ot_wait_for_previous();
+    ot_next_may_start();
     const unsigned tmem = s_tmem;
     const int chunks = g.chunks, rounds = (chunks + S::DRAIN - 1) / S::DRAIN;
     float acc[COLS];
 
     if (warp == 8) {
-        if (lane == 0) {
-            const uint8_t* a = g.a + (int64_t)batch * LIMBS * g.a_limb + (int64_t)row_tile * chunks * OT_TILE;
-            const uint8_t* b = g.b + (int64_t)batch * LIMBS * g.b_limb;
-            const int col_tile = tj * CTAS + rank;  // this block's columns of the right operand
-            bool ok = true;
-            int k = 0;
-            for (; k < chunks; ++k) {
-                const int s = k % S::STAGES;
-                if (k >= S::STAGES && !ot_wait(ot_smem(&s_empty[s]), (unsigned)((k / S::STAGES - 1) & 1))) {
-                    ok = false;
-                    break;
-                }
-                const unsigned bar = ot_smem(&s_full[s]), to = ring + s * S::STAGE;
-                ot_expect(bar, same ? LIMBS * OT_TILE : 2 * LIMBS * OT_TILE);
+        const int col_tile = tj * CTAS + rank;  // this block's columns of the right operand
+        const uint8_t* a = g.a + (int64_t)batch * LIMBS * g.a_limb + (int64_t)row_tile * chunks * OT_TILE;
+        // SYM: the tiles of a row, one after the other; else two half tiles (64 rows) at a time, the next rows' half in the same tiles or a row of tiles on
+        const uint8_t* b = g.b + (int64_t)batch * LIMBS * g.b_limb + (SYM ? (int64_t)col_tile * chunks : (int64_t)2 * col_tile) * OT_TILE;
+        const int64_t b_odd = SYM ? OT_TILE : OT_TILE / 2, b_even = SYM ? OT_TILE : (int64_t)width * OT_TILE - OT_TILE / 2;
+        const unsigned bytes = same ? LIMBS * OT_TILE : 2 * LIMBS * OT_TILE;
+        bool ok = true;
+        int k = 0;
+        unsigned s = 0, parity = 1;  // a barrier that nothing has arrived at yet passes for the phase before its first
+        for (; k < chunks; ++k) {
+            const unsigned bar = ot_smem(&s_full[0]) + 8 * s, to = ring + s * S::STAGE;
+            ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_empty[0]) + 8 * s, parity));
+            if (!ok) break;
+            if (lane == 0) {
+                ot_expect(bar, bytes);
 #pragma unroll
                 for (int l = 0; l < LIMBS; ++l) {
-                    ot_copy(to + l * OT_TILE, a + l * g.a_limb + (int64_t)k * OT_TILE, OT_TILE, bar);
+                    ot_copy(to + l * OT_TILE, a + l * g.a_limb, OT_TILE, bar);
                     if (same) continue;
                     const unsigned tb = to + (LIMBS + l) * OT_TILE;
-                    if (SYM) {
-                        ot_copy(tb, b + l * g.b_limb + ((int64_t)col_tile * chunks + k) * OT_TILE, OT_TILE, bar);
-                    } else {  // rows 64 k .. 64 k + 63 of two column tiles
-                        const uint8_t* p = b + l * g.b_limb + ((int64_t)(k >> 1) * width + 2 * col_tile) * OT_TILE + (k & 1) * (OT_TILE / 2);
-                        ot_copy(tb, p, OT_TILE / 2, bar);
-                        ot_copy(tb + OT_TILE / 2, p + OT_TILE, OT_TILE / 2, bar);
-                    }
+                    ot_copy(tb, b + l * g.b_limb, SYM ? OT_TILE : OT_TILE / 2, bar);
+                    if (!SYM) ot_copy(tb + OT_TILE / 2, b + l * g.b_limb + OT_TILE, OT_TILE / 2, bar);
                 }
             }
-            if (!ok) {  // the copies in flight land before the block ends
-                atomicExch(&s_failed, 1);
-                for (int q = k < S::STAGES ? 0 : k - S::STAGES; q < k; ++q) ot_wait(ot_smem(&s_full[q % S::STAGES]), (unsigned)((q / S::STAGES) & 1));
+            __syncwarp();
+            a += OT_TILE;
+            b += k & 1 ? b_even : b_odd;
+            if (++s == S::STAGES) {
+                s = 0;
+                parity ^= 1;
             }
+        }
+        if (!ok) {  // the copies in flight land before the block ends
+            if (lane == 0) atomicExch(&s_failed, 1);
+            for (int q = k < S::STAGES ? 0 : k - S::STAGES; q < k; ++q) ot_wait(ot_smem(&s_full[q % S::STAGES]), (unsigned)((q / S::STAGES) & 1));
         }
     } else if (warp == 9) {
-        if (lane == 0 && rank == 0) {
+        unsigned s = 0, parity = 0;
+        bool ok = true;
+        if (rank == 0) {
             // fp32 accumulator (1 at bit 4), fp16 operands, N / 8 at bit 17, M / 16 at bit 24; apply: the right operand is N-major (bit 16)
             constexpr unsigned IDESC = (1u << 4) | (SYM ? 0u : 1u << 16) | ((unsigned)(TN / 8) << 17) | ((unsigned)(8 * CTAS) << 24);
-            bool ok = true;
-            for (int r = 0, k = 0; r < rounds && ok; ++r) {
+            // descriptors of the first stage; steps along K and to other stages are added in units of 16 bytes.  K-major: 32 bytes along the
+            // row, 8-row groups 1024 bytes apart.  N-major: 16 rows of 128 bytes, 8-row groups 1024 bytes apart, the next 64 columns 8 KB further
+            const unsigned long long da0 = ot_desc(ring, 16, 1024);
+            const unsigned long long db0 = SYM ? ot_desc(same ? ring : ring + LIMBS * OT_TILE, 16, 1024) : ot_desc(ring + LIMBS * OT_TILE, OT_TILE / 2, 1024);
+            constexpr unsigned STEP_A = 2, STEP_B = SYM ? 2 : 128;
+            const bool leader = ot_elect();
+            int k = 0;
+            for (int r = 0; r < rounds && ok; ++r) {
                 const unsigned d = tmem + (unsigned)((r & 1) * TN);
-                if (r >= 2) ok = ot_wait_cluster(ot_smem(&s_acc_empty[r & 1]), (unsigned)((r / 2 - 1) & 1));
+                if (r >= 2) ok = __all_sync(0xffffffffu, ot_wait_cluster(ot_smem(&s_acc_empty[r & 1]), (unsigned)((r / 2 - 1) & 1)));
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int q0 = k; ok && k < chunks && k < q0 + S::DRAIN; ++k) {
-                    const int s = k % S::STAGES;
-                    const unsigned parity = (unsigned)((k / S::STAGES) & 1);
-                    ok = ot_wait(ot_smem(&s_full[s]), parity) && (CTAS == 1 || ot_wait_cluster(ot_smem(&s_peer[s]), parity));
+                const int last = min(chunks, k + S::DRAIN);
+                unsigned accumulate = 0;
+                for (; ok && k < last; ++k) {
+                    ok = ot_wait(ot_smem(&s_full[0]) + 8 * s, parity);
+                    if (CTAS == 2) ok = ok && ot_wait_cluster(ot_smem(&s_peer[0]) + 8 * s, parity);
+                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const unsigned at = ring + s * S::STAGE, bt = same ? at : at + LIMBS * OT_TILE;
+                    if (leader) {
+                        const unsigned long long da = da0 + s * (S::STAGE / 16), db = db0 + s * (S::STAGE / 16);
 #pragma unroll
-                    for (int q = 0; q < (LIMBS == 2 ? 3 : 1); ++q) {
-                        const unsigned la = at + (q == 2 ? OT_TILE : 0), lb = bt + (q == 1 ? OT_TILE : 0);
+                        for (int q = 0; q < (LIMBS == 2 ? 3 : 1); ++q)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            // K-major: 32 bytes along the row, 8-row groups 1024 bytes apart.  N-major: 16 rows of 128 bytes, 8-row groups
-                            // 1024 bytes apart, the next 64 columns 8 KB further
-                            const unsigned long long da = ot_desc(la + 32 * j, 16, 1024);
-                            const unsigned long long db = SYM ? ot_desc(lb + 32 * j, 16, 1024) : ot_desc(lb + 2048 * j, OT_TILE / 2, 1024);
-                            ot_mma<CTAS>(d, da, db, IDESC, (k > q0 || q > 0 || j > 0) ? 1u : 0u);
-                        }
+                            for (int j = 0; j < 4; ++j)
+                                ot_mma<CTAS>(d, da + (q == 2 ? OT_TILE / 16 : 0) + STEP_A * j, db + (q == 1 ? OT_TILE / 16 : 0) + STEP_B * j, IDESC,
+                                             q > 0 || j > 0 ? 1u : accumulate);
+                        ot_commit<CTAS>(ot_smem(&s_empty[0]) + 8 * s);
                     }
-                    ot_commit<CTAS>(ot_smem(&s_empty[s]));
+                    __syncwarp();
+                    accumulate = 1;
+                    if (++s == S::STAGES) {
+                        s = 0;
+                        parity ^= 1;
+                    }
                 }
-                ot_commit<CTAS>(ot_smem(&s_acc_full[r & 1]));
+                if (leader) ot_commit<CTAS>(ot_smem(&s_acc_full[r & 1]));
+                __syncwarp();
             }
-            if (!ok) atomicExch(&s_failed, 1);
-        } else if (lane == 0) {
+        } else {
             // the odd block: tells the even one that its operands are there
-            for (int k = 0; k < chunks; ++k) {
-                const int s = k % S::STAGES;
-                if (!ot_wait(ot_smem(&s_full[s]), (unsigned)((k / S::STAGES) & 1))) {
-                    atomicExch(&s_failed, 1);
-                    break;
+            for (int k = 0; k < chunks && ok; ++k) {
+                ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_full[0]) + 8 * s, parity));
+                if (ok && lane == 0) ot_arrive_at(ot_smem(&s_peer[0]) + 8 * s, 0);
+                __syncwarp();
+                if (++s == S::STAGES) {
+                    s = 0;
+                    parity ^= 1;
                 }
-                ot_arrive_at(ot_smem(&s_peer[s]), 0);
             }
         }
+        if (!ok && lane == 0) atomicExch(&s_failed, 1);
     } else {
         const unsigned taddr = tmem + ((unsigned)((warp & 3) * 32) << 16) + (unsigned)((warp >> 2) * COLS);
 #pragma unroll
@@ -460,12 +580,19 @@ struct OtPlan {
     int64_t x_limb, a_limb;                  // bytes of a limb
     int64_t x0, x1, a, q, total;             // offsets in the workspace
 };
+// Waves of tiles times the cycles of a tile, over the three products of a step: a chunk of K takes as long as its copies (64 bytes per
+// cycle and SM) or its MMAs (4096 multiply-adds per cycle and SM, single blocks' slowed by what they read from shared memory), whichever is longer, a
+// tile some 6000 cycles besides (launch, first copies, epilogue).
+int64_t ot_cost(int64_t batch, int64_t n, int64_t m, int limbs, int ctas) {
+    const int64_t tile = 128 * ctas, nt = (n + tile - 1) / tile, mt = (m + tile - 1) / tile, slots = sm_count() / ctas;
+    const int64_t chunk = limbs == 1 ? 512 : ctas == 1 ? 1024 : 1536, sym = batch * nt * (nt + 1) / 2, all = batch * nt * mt;
+    const int64_t sym_waves = (sym + slots - 1) / slots, all_waves = (all + slots - 1) / slots, kn = nt * tile / 64, km = mt * tile / 64;
+    return sym_waves * (km * chunk + 6000) + sym_waves * (kn * chunk + 6000) + all_waves * (kn * chunk + 6000);
+}
 OtPlan ot_plan(int batch, int rows, int cols, int limbs) {
     const int64_t n = rows < cols ? rows : cols, m = rows < cols ? cols : rows;
     OtPlan p;
-    // pairs of blocks where their larger tiles still fill the chip
-    const int64_t big = (n + 255) / 256;
-    p.ctas = batch * big * (big + 1) / 2 >= 64 ? 2 : 1;
+    p.ctas = ot_cost(batch, n, m, limbs, 2) < ot_cost(batch, n, m, limbs, 1) ? 2 : 1;
     const int64_t pad = 128 * p.ctas;
     p.n_pad = (int)((n + pad - 1) / pad * pad);
     p.m_pad = (int)((m + pad - 1) / pad * pad);
@@ -489,12 +616,14 @@ void ot_gemm(cudaStream_t s, const OtGemm& g, const OrthIo& io) {
     cfg.blockDim = dim3(320);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = CTAS;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     cudaLaunchKernelEx(&cfg, k_orth_gemm<KIND, LIMBS, CTAS, T>, g, io);
 }
 
@@ -513,13 +642,37 @@ void ot_steps(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, uint8_t* w
     }
 }
 
+// the norm and the tiles of X0; N: adjacent elements per access
+template <typename T, int LIMBS, int N>
+void ot_begin(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, const OtPlan& p, double* partial, uint8_t* x) {
+    const bool gaps = io.g_stride != io.cols;
+    const int64_t total = gaps ? 0 : (int64_t)io.rows * io.cols, len = gaps ? io.cols : 4096, segments = gaps ? io.rows : (total + 4095) / 4096;
+    int64_t most = 8 * (int64_t)sm_count() / io.batch;
+    most = most < 1 ? 1 : most < OT_NORM_BLOCKS ? most : OT_NORM_BLOCKS;
+    const int blocks = (int)(segments < most ? segments : most);
+    k_orth_norm<T, N><<<dim3((unsigned)blocks, (unsigned)io.batch), 256, 0, s>>>(io, segments, len, total, partial);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.m_pad / 64), (unsigned)(p.n_pad / 128), (unsigned)io.batch);
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const double* sums = partial;
+    if (io.rows > io.cols) cudaLaunchKernelEx(&cfg, k_orth_pack<T, LIMBS, 1, true>, io, poly.eps, sums, blocks, x, p.x_limb);
+    else cudaLaunchKernelEx(&cfg, k_orth_pack<T, LIMBS, N, false>, io, poly.eps, sums, blocks, x, p.x_limb);
+}
+
 template <typename T, int LIMBS>
 void ot_run(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, uint8_t* work) {
     const OtPlan p = ot_plan(io.batch, io.rows, io.cols, LIMBS);
     double* partial = reinterpret_cast<double*>(work);
-    const int blocks = io.rows < OT_NORM_BLOCKS ? io.rows : OT_NORM_BLOCKS;
-    k_orth_norm<T><<<dim3((unsigned)blocks, (unsigned)io.batch), 512, 0, s>>>(io, partial);
-    k_orth_pack<T, LIMBS><<<dim3((unsigned)(p.m_pad / 64), (unsigned)(p.n_pad / 128), (unsigned)io.batch), 256, 0, s>>>(io, poly.eps, partial, blocks, work + p.x0, p.x_limb);
+    // 16 bytes at a time where all rows start on such a boundary
+    constexpr int W = 16 / (int)sizeof(T);
+    const bool wide = io.cols % W == 0 && ((uintptr_t)io.g & 15) == 0 && io.g_stride % W == 0 && io.g_batch % W == 0 && (((uintptr_t)io.m | (uintptr_t)io.m_out) & 15) == 0;
+    if (wide) ot_begin<T, LIMBS, W>(s, io, poly, p, partial, work + p.x0); else ot_begin<T, LIMBS, 1>(s, io, poly, p, partial, work + p.x0);
     if (p.ctas == 2) ot_steps<T, LIMBS, 2>(s, io, poly, work, p); else ot_steps<T, LIMBS, 1>(s, io, poly, work, p);
 }
 
