@@ -27,8 +27,9 @@ namespace {
 #define OT_SCALE 2048.0f
 #define OT_UNSCALE (1.0f / (2048.0f * 2048.0f))
 #define OT_WAIT_LIMIT (1 << 20)
+#define OT_PARTS 8             // most parts of a Gram product
 #define OT_NORM_BLOCKS 512      // most partial sums of squares per matrix
-enum { OT_GRAM = 0, OT_SQUARE = 1, OT_APPLY = 2, OT_LAST = 3 };
+enum { OT_GRAM = 0, OT_SQUARE = 1, OT_APPLY = 2, OT_LAST = 3, OT_GRAM_PART = 4 };
 
 __device__ __forceinline__ unsigned ot_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void ot_bar_init(unsigned bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
@@ -54,23 +55,12 @@ __device__ __forceinline__ void ot_copy(unsigned dst, const void* src, unsigned 
 // it touches global memory.
 __device__ __forceinline__ void ot_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void ot_next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-// ot_wait where blocks of the cluster arrive
-__device__ __forceinline__ bool ot_wait_cluster(unsigned bar, unsigned parity) {
-    for (int i = 0; i < OT_WAIT_LIMIT; ++i) {
-        unsigned ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (ok) return true;
-    }
-    return false;
-}
-// arrives at the same barrier of block `rank` of the cluster
+// Arrives at the same barrier of block `rank` of the cluster.  What it announces are operands that copies have brought (their bytes were counted
+// before this thread arrives) or accumulators that have been read; no store of this thread's.  A release at cluster scope waits for the copies in
+// flight as well: it made a chunk of 256 x 256 tiles of one limb take 1250 cycles instead of 500.
 __device__ __forceinline__ void ot_arrive_at(unsigned bar, unsigned rank) {
     asm volatile(
-        "{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %0, %1;\n\tmbarrier.arrive.release.cluster.shared::cluster.b64 _, [at];\n\t}" ::"r"(bar), "r"(rank)
+        "{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %0, %1;\n\tmbarrier.arrive.shared::cluster.b64 _, [at];\n\t}" ::"r"(bar), "r"(rank)
         : "memory");
 }
 __device__ __forceinline__ void ot_cluster_sync() {
@@ -277,14 +267,16 @@ __global__ void __launch_bounds__(256) k_orth_pack(OrthIo io, float eps, const d
 
 // ---- the products -----------------------------------------------------------------------------------------------------
 struct OtGemm {
-    const uint8_t* a;    // left operand's tiles [batch][limbs][rows / 128][chunks]
-    const uint8_t* b;    // right operand's tiles
-    uint8_t* out;        // the result's tiles
+    const uint8_t* a;    // left operand's tiles [batch][limbs][rows / 128][a_width]
+    const uint8_t* b;    // right operand's tiles [batch][limbs][rows / 128][b_width]
+    uint8_t* out;        // the result's tiles [batch][limbs][rows / 128][out_width]
     int64_t a_limb, b_limb, out_limb;  // bytes of a limb
-    int chunks;          // K / 64
+    int a_width, b_width, out_width;
+    int chunks;          // of K, 64 each: what lies beyond them in the tiles is never read as K, whatever it holds
     int row_tiles;       // of the result, 128 CTAS each
-    int col_tiles;       // of the result, 128 CTAS each; the result's rows (apply: and b's) hold 2 CTAS col_tiles tiles
+    int col_tiles;
     float ca, cb, cc;    // square: a I + b A + c A A
+    float* part;         // Gram in gridDim.y parts of K: the parts' sums [batch][tile][part][32 column quads][128 rows][4]
 };
 
 template <int LIMBS>
@@ -303,7 +295,7 @@ template <int KIND, int LIMBS, int CTAS, typename T>
 __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
     using S = OtShape<LIMBS>;
     constexpr int TN = 128 * CTAS, COLS = 64 * CTAS;  // accumulator columns of a block, of a thread
-    constexpr bool SYM = KIND == OT_GRAM || KIND == OT_SQUARE;
+    constexpr bool SYM = KIND == OT_GRAM || KIND == OT_SQUARE || KIND == OT_GRAM_PART;
     extern __shared__ uint8_t s_raw[];
     __shared__ __align__(8) unsigned long long s_full[S::STAGES], s_peer[S::STAGES], s_empty[S::STAGES], s_acc_full[2], s_acc_empty[2];
     __shared__ unsigned s_tmem;
@@ -325,7 +317,6 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
     }
     const bool same = SYM && ti == tj;              // one operand serves as both
     const int row_tile = ti * CTAS + rank;          // this block's rows, in 128s
-    const int width = 2 * CTAS * g.col_tiles;       // tiles in a row of the result
     if (tid == 0) {
         for (int s = 0; s < S::STAGES; ++s) {
             ot_bar_init(ot_smem(&s_full[s]), 1);
@@ -355,15 +346,17 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
     ot_wait_for_previous();
     ot_next_may_start();
     const unsigned tmem = s_tmem;
-    const int chunks = g.chunks, rounds = (chunks + S::DRAIN - 1) / S::DRAIN;
+    const int chunk0 = KIND == OT_GRAM_PART ? (int)((int64_t)g.chunks * blockIdx.y / gridDim.y) : 0;
+    const int chunks = KIND == OT_GRAM_PART ? (int)((int64_t)g.chunks * (blockIdx.y + 1) / gridDim.y) - chunk0 : g.chunks;
+    const int rounds = (chunks + S::DRAIN - 1) / S::DRAIN;
     float acc[COLS];
 
     if (warp == 8) {
         const int col_tile = tj * CTAS + rank;  // this block's columns of the right operand
-        const uint8_t* a = g.a + (int64_t)batch * LIMBS * g.a_limb + (int64_t)row_tile * chunks * OT_TILE;
+        const uint8_t* a = g.a + (int64_t)batch * LIMBS * g.a_limb + ((int64_t)row_tile * g.a_width + chunk0) * OT_TILE;
         // SYM: the tiles of a row, one after the other; else two half tiles (64 rows) at a time, the next rows' half in the same tiles or a row of tiles on
-        const uint8_t* b = g.b + (int64_t)batch * LIMBS * g.b_limb + (SYM ? (int64_t)col_tile * chunks : (int64_t)2 * col_tile) * OT_TILE;
-        const int64_t b_odd = SYM ? OT_TILE : OT_TILE / 2, b_even = SYM ? OT_TILE : (int64_t)width * OT_TILE - OT_TILE / 2;
+        const uint8_t* b = g.b + (int64_t)batch * LIMBS * g.b_limb + (SYM ? (int64_t)col_tile * g.b_width + chunk0 : (int64_t)2 * col_tile) * OT_TILE;
+        const int64_t b_odd = SYM ? OT_TILE : OT_TILE / 2, b_even = SYM ? OT_TILE : (int64_t)g.b_width * OT_TILE - OT_TILE / 2;
         const unsigned bytes = same ? LIMBS * OT_TILE : 2 * LIMBS * OT_TILE;
         bool ok = true;
         int k = 0;
@@ -410,13 +403,13 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
             int k = 0;
             for (int r = 0; r < rounds && ok; ++r) {
                 const unsigned d = tmem + (unsigned)((r & 1) * TN);
-                if (r >= 2) ok = __all_sync(0xffffffffu, ot_wait_cluster(ot_smem(&s_acc_empty[r & 1]), (unsigned)((r / 2 - 1) & 1)));
+                if (r >= 2) ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_acc_empty[r & 1]), (unsigned)((r / 2 - 1) & 1)));
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const int last = min(chunks, k + S::DRAIN);
                 unsigned accumulate = 0;
                 for (; ok && k < last; ++k) {
                     ok = ot_wait(ot_smem(&s_full[0]) + 8 * s, parity);
-                    if (CTAS == 2) ok = ok && ot_wait_cluster(ot_smem(&s_peer[0]) + 8 * s, parity);
+                    if (CTAS == 2) ok = ok && ot_wait(ot_smem(&s_peer[0]) + 8 * s, parity);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -490,16 +483,26 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
     }
     if (warp >= 8) return;
 
+    if (KIND == OT_GRAM_PART) {
+        const float poison = s_failed ? __int_as_float(0x7fc00000) : 0.0f;
+        float4* to = reinterpret_cast<float4*>(g.part) + (((int64_t)batch * gridDim.x + blockIdx.x) * gridDim.y + blockIdx.y) * 4096 + (tid & 127);
+#pragma unroll
+        for (int c = 0; c < COLS; c += 4) to[((warp >> 2) * COLS + c) / 4 * 128] = make_float4(acc[c] + poison, acc[c + 1] + poison, acc[c + 2] + poison, acc[c + 3] + poison);
+        return;
+    }
     // Epilogue by two groups of 128 threads, a row each, in rounds of 64 columns through the group's part of shared memory.
     const float poison = s_failed ? __int_as_float(0x7fc00000) : 0.0f;
     const int group = warp >> 2, row = tid & 127;
-    uint8_t* direct = s_dyn + group * (2 * LIMBS * OT_TILE);      // [limb] tile
-    uint8_t* mirror = direct + LIMBS * OT_TILE;                   // [limb][column half] half a tile: 64 rows
+    // a round's images: [limb] tile, and mirrored [limb][column half] half a tile of 64 rows; every round has its own where the ring has room
+    constexpr int IMAGES = (SYM ? 2 : 1) * LIMBS * OT_TILE;
+    constexpr bool APART = 2 * CTAS * IMAGES <= S::STAGE * S::STAGES;
     float* flat = reinterpret_cast<float*>(s_dyn + group * 40960);  // OT_LAST: [128][65]
 #pragma unroll
     for (int h = 0; h < CTAS; ++h) {
         const int col_tile = tj * 2 * CTAS + group * CTAS + h;    // the round's columns, in 64s
-        if (h) asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+        uint8_t* direct = s_dyn + (group + (APART ? 2 * h : 0)) * IMAGES;
+        uint8_t* mirror = direct + LIMBS * OT_TILE;
+        if (h && (!APART || KIND == OT_LAST)) asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
         if (KIND == OT_LAST) {
 #pragma unroll
             for (int c = 0; c < 64; ++c) flat[row * 65 + c] = acc[64 * h + c] * OT_UNSCALE + poison;
@@ -521,7 +524,7 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                 }
             }
         } else {
-            const uint8_t* old = KIND == OT_SQUARE ? g.a + (int64_t)batch * LIMBS * g.a_limb + ((int64_t)row_tile * chunks + col_tile) * OT_TILE : nullptr;
+            const uint8_t* old = KIND == OT_SQUARE ? g.a + (int64_t)batch * LIMBS * g.a_limb + ((int64_t)row_tile * g.a_width + col_tile) * OT_TILE : nullptr;
 #pragma unroll
             for (int c0 = 0; c0 < 64; c0 += 8) {
                 float x[8];
@@ -560,59 +563,110 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                 uint8_t* o = g.out + (int64_t)batch * LIMBS * g.out_limb;
 #pragma unroll
                 for (int l = 0; l < LIMBS; ++l) {
-                    ot_store(o + l * g.out_limb + ((int64_t)row_tile * width + col_tile) * OT_TILE, ot_smem(direct + l * OT_TILE), OT_TILE);
+                    ot_store(o + l * g.out_limb + ((int64_t)row_tile * g.out_width + col_tile) * OT_TILE, ot_smem(direct + l * OT_TILE), OT_TILE);
                     if (SYM && !same) {
 #pragma unroll
                         for (int q = 0; q < 2; ++q)
-                            ot_store(o + l * g.out_limb + ((int64_t)(col_tile >> 1) * width + 2 * row_tile + q) * OT_TILE + (col_tile & 1) * (OT_TILE / 2),
+                            ot_store(o + l * g.out_limb + ((int64_t)(col_tile >> 1) * g.out_width + 2 * row_tile + q) * OT_TILE + (col_tile & 1) * (OT_TILE / 2),
                                      ot_smem(mirror + (l * 2 + q) * (OT_TILE / 2)), OT_TILE / 2);
                     }
                 }
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+                // the images must be read before they are written again, or the block ends
+                if (!APART || h + 1 == CTAS) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             }
         }
     }
 }
 
+// The parts of a Gram matrix, added in order, as tiles: eight columns of a tile per block.
+template <int LIMBS>
+__global__ void __launch_bounds__(256) k_orth_join(const float* __restrict__ part, int parts, uint8_t* __restrict__ out, int64_t limb_bytes, int width) {
+    const int tile = blockIdx.x >> 4, batch = blockIdx.z, tiles = gridDim.x >> 4;
+    int ti = 0;
+    while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
+    const int tj = tile - ti * (ti + 1) / 2, row = threadIdx.x & 127, quad = (blockIdx.x & 15) * 2 + (threadIdx.x >> 7), col = quad * 4;
+    ot_wait_for_previous();
+    ot_next_may_start();
+    const float4* p = reinterpret_cast<const float4*>(part) + ((int64_t)batch * tiles + tile) * parts * 4096 + quad * 128 + row;
+    float4 t[OT_PARTS];
+#pragma unroll
+    for (int q = 0; q < OT_PARTS; ++q) t[q] = q < parts ? p[(int64_t)q * 4096] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float x[4] = {t[0].x, t[0].y, t[0].z, t[0].w};
+#pragma unroll
+    for (int q = 1; q < OT_PARTS; ++q) {
+        x[0] += t[q].x;
+        x[1] += t[q].y;
+        x[2] += t[q].z;
+        x[3] += t[q].w;
+    }
+    uint8_t* o = out + (int64_t)batch * LIMBS * limb_bytes;
+    OpVec<__half, 4> piece[LIMBS];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        __half s[LIMBS];
+        ot_split<LIMBS>(x[c] * (OT_UNSCALE * OT_SCALE), s);
+#pragma unroll
+        for (int l = 0; l < LIMBS; ++l) {
+            piece[l].v[c] = s[l];
+            if (ti != tj) *reinterpret_cast<__half*>(o + l * limb_bytes + ((int64_t)tj * width + 2 * ti + (row >> 6)) * OT_TILE + ot_at(col + c, row & 63)) = s[l];
+        }
+    }
+#pragma unroll
+    for (int l = 0; l < LIMBS; ++l)
+        *reinterpret_cast<OpVec<__half, 4>*>(o + l * limb_bytes + ((int64_t)ti * width + 2 * tj + (col >> 6)) * OT_TILE + ot_at(row, col & 63)) = piece[l];
+}
+
 struct OtPlan {
-    int ctas, n_pad, m_pad;
+    int sym_ctas, all_ctas;                  // blocks per tile of the symmetric products and of Q X
+    int parts;                               // of K in the Gram product
+    int n, m, n_pad, m_pad;
     int64_t x_limb, a_limb;                  // bytes of a limb
-    int64_t x0, x1, a, q, total;             // offsets in the workspace
+    int64_t x0, x1, a, q, part, total;       // offsets in the workspace
 };
-// Waves of tiles times the cycles of a tile, over the three products of a step: a chunk of K takes as long as its copies (64 bytes per
-// cycle and SM) or its MMAs (4096 multiply-adds per cycle and SM, single blocks' slowed by what they read from shared memory), whichever is longer, a
-// tile some 6000 cycles besides (launch, first copies, epilogue).
-int64_t ot_cost(int64_t batch, int64_t n, int64_t m, int limbs, int ctas) {
-    const int64_t tile = 128 * ctas, nt = (n + tile - 1) / tile, mt = (m + tile - 1) / tile, slots = sm_count() / ctas;
-    const int64_t chunk = limbs == 1 ? 512 : ctas == 1 ? 1024 : 1536, sym = batch * nt * (nt + 1) / 2, all = batch * nt * mt;
-    const int64_t sym_waves = (sym + slots - 1) / slots, all_waves = (all + slots - 1) / slots, kn = nt * tile / 64, km = mt * tile / 64;
-    return sym_waves * (km * chunk + 6000) + sym_waves * (kn * chunk + 6000) + all_waves * (kn * chunk + 6000);
+// Cycles of a product by the waves of its tiles: a chunk of K in a 128 x 128 tile of one block, a 256 x 256 tile of two, with one limb or two, and
+// a tile's fixed part (launch, first copies, epilogue), as measured at n = 777, m = 1000 and 4096 x 4096.
+int64_t ot_cost(int64_t tiles, int64_t chunks, int limbs, int ctas) {
+    const int64_t slots = sm_count() / ctas, waves = (tiles + slots - 1) / slots;
+    return waves * (ctas == 1 ? chunks * (limbs == 1 ? 390 : 990) + 9000 : chunks * (limbs == 1 ? 450 : 1520) + (limbs == 1 ? 13000 : 18000));
 }
 OtPlan ot_plan(int batch, int rows, int cols, int limbs) {
-    const int64_t n = rows < cols ? rows : cols, m = rows < cols ? cols : rows;
     OtPlan p;
-    p.ctas = ot_cost(batch, n, m, limbs, 2) < ot_cost(batch, n, m, limbs, 1) ? 2 : 1;
-    const int64_t pad = 128 * p.ctas;
-    p.n_pad = (int)((n + pad - 1) / pad * pad);
-    p.m_pad = (int)((m + pad - 1) / pad * pad);
+    p.n = rows < cols ? rows : cols;
+    p.m = rows < cols ? cols : rows;
+    const int64_t n1 = (p.n + 127) / 128, n2 = (p.n + 255) / 256, m1 = (p.m + 127) / 128, m2 = (p.m + 255) / 256, kn = (p.n + 63) / 64, km = (p.m + 63) / 64;
+    const int64_t s1 = batch * n1 * (n1 + 1) / 2, s2 = batch * n2 * (n2 + 1) / 2;
+    p.sym_ctas = ot_cost(s2, kn, limbs, 2) + ot_cost(s2, km, limbs, 2) < ot_cost(s1, kn, limbs, 1) + ot_cost(s1, km, limbs, 1) ? 2 : 1;
+    p.all_ctas = ot_cost(batch * n2 * m2, kn, limbs, 2) < ot_cost(batch * n1 * m1, kn, limbs, 1) ? 2 : 1;
+    // few tiles with a long K are cut into parts where that saves more than the launch that joins them
+    p.parts = 1;
+    if (p.sym_ctas == 1) {
+        int64_t q = sm_count() / s1;
+        q = q < OT_PARTS ? q : OT_PARTS;
+        q = q < km / 4 ? q : km / 4;
+        if (q > 1 && (km - km / q) * (limbs == 1 ? 390 : 990) > 9000) p.parts = (int)q;
+    }
+    const int pad = 128 * (p.sym_ctas > p.all_ctas ? p.sym_ctas : p.all_ctas);
+    p.n_pad = (p.n + pad - 1) / pad * pad;
+    p.m_pad = (int)(((int64_t)p.m + pad - 1) / pad * pad);
     p.x_limb = (int64_t)p.n_pad * p.m_pad * 2;
     p.a_limb = (int64_t)p.n_pad * p.n_pad * 2;
     p.x0 = ((int64_t)batch * OT_NORM_BLOCKS * 8 + 127) / 128 * 128;
     p.x1 = p.x0 + p.x_limb * limbs * batch;
     p.a = p.x1 + p.x_limb * limbs * batch;
     p.q = p.a + p.a_limb * limbs * batch;
-    p.total = p.q + p.a_limb * limbs * batch;
+    p.part = p.q + p.a_limb * limbs * batch;
+    p.total = p.part + (p.parts > 1 ? s1 * p.parts * 65536 : 0);
     return p;
 }
 
 template <int KIND, int LIMBS, int CTAS, typename T>
-void ot_gemm(cudaStream_t s, const OtGemm& g, const OrthIo& io) {
+void ot_gemm(cudaStream_t s, const OtGemm& g, const OrthIo& io, int parts = 1) {
     using S = OtShape<LIMBS>;
     cudaFuncSetAttribute(k_orth_gemm<KIND, LIMBS, CTAS, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-    const int tiles = KIND == OT_GRAM || KIND == OT_SQUARE ? g.row_tiles * (g.row_tiles + 1) / 2 : g.row_tiles * g.col_tiles;
+    const int tiles = KIND == OT_APPLY || KIND == OT_LAST ? g.row_tiles * g.col_tiles : g.row_tiles * (g.row_tiles + 1) / 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * CTAS), 1, (unsigned)io.batch);
+    cfg.gridDim = dim3((unsigned)(tiles * CTAS), (unsigned)parts, (unsigned)io.batch);
     cfg.blockDim = dim3(320);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = s;
@@ -627,15 +681,40 @@ void ot_gemm(cudaStream_t s, const OtGemm& g, const OrthIo& io) {
     cudaLaunchKernelEx(&cfg, k_orth_gemm<KIND, LIMBS, CTAS, T>, g, io);
 }
 
-template <typename T, int LIMBS, int CTAS>
+template <typename T, int LIMBS>
 void ot_steps(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, uint8_t* work, const OtPlan& p) {
     uint8_t *x = work + p.x0, *y = work + p.x1, *a = work + p.a, *q = work + p.q;
-    const int rt = p.n_pad / (128 * CTAS), ct = p.m_pad / (128 * CTAS);
+    const int wn = p.n_pad / 64, wm = p.m_pad / 64, kn = (p.n + 63) / 64, km = (p.m + 63) / 64;
+    const int st = (p.n + 128 * p.sym_ctas - 1) / (128 * p.sym_ctas), rt = (p.n + 128 * p.all_ctas - 1) / (128 * p.all_ctas), ct = (p.m + 128 * p.all_ctas - 1) / (128 * p.all_ctas);
+    float* part = reinterpret_cast<float*>(work + p.part);
     for (int k = 0; k < poly.steps; ++k) {
-        ot_gemm<OT_GRAM, LIMBS, CTAS, float>(s, {x, x, a, p.x_limb, p.x_limb, p.a_limb, p.m_pad / 64, rt, rt, 0.f, 0.f, 0.f}, io);
-        ot_gemm<OT_SQUARE, LIMBS, CTAS, float>(s, {a, a, q, p.a_limb, p.a_limb, p.a_limb, p.n_pad / 64, rt, rt, poly.a, poly.b, poly.c}, io);
-        const OtGemm g = {q, x, y, p.a_limb, p.x_limb, p.x_limb, p.n_pad / 64, rt, ct, 0.f, 0.f, 0.f};
-        if (k + 1 < poly.steps) ot_gemm<OT_APPLY, LIMBS, CTAS, float>(s, g, io); else ot_gemm<OT_LAST, LIMBS, CTAS, T>(s, g, io);
+        const OtGemm gram = {x, x, a, p.x_limb, p.x_limb, p.a_limb, wm, wm, wn, km, st, st, 0.f, 0.f, 0.f, part};
+        const OtGemm square = {a, a, q, p.a_limb, p.a_limb, p.a_limb, wn, wn, wn, kn, st, st, poly.a, poly.b, poly.c, nullptr};
+        const OtGemm apply = {q, x, y, p.a_limb, p.x_limb, p.x_limb, wn, wm, wm, kn, rt, ct, 0.f, 0.f, 0.f, nullptr};
+        if (p.parts > 1) {
+            ot_gemm<OT_GRAM_PART, LIMBS, 1, float>(s, gram, io, p.parts);
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)(st * (st + 1) / 2 * 16), 1, (unsigned)io.batch);
+            cfg.blockDim = dim3(256);
+            cfg.stream = s;
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            at[0].val.programmaticStreamSerializationAllowed = 1;
+            cfg.attrs = at;
+            cfg.numAttrs = 1;
+            const float* sums = part;
+            cudaLaunchKernelEx(&cfg, k_orth_join<LIMBS>, sums, p.parts, a, p.a_limb, wn);
+        } else if (p.sym_ctas == 2) {
+            ot_gemm<OT_GRAM, LIMBS, 2, float>(s, gram, io);
+        } else {
+            ot_gemm<OT_GRAM, LIMBS, 1, float>(s, gram, io);
+        }
+        if (p.sym_ctas == 2) ot_gemm<OT_SQUARE, LIMBS, 2, float>(s, square, io); else ot_gemm<OT_SQUARE, LIMBS, 1, float>(s, square, io);
+        if (k + 1 < poly.steps) {
+            if (p.all_ctas == 2) ot_gemm<OT_APPLY, LIMBS, 2, float>(s, apply, io); else ot_gemm<OT_APPLY, LIMBS, 1, float>(s, apply, io);
+        } else {
+            if (p.all_ctas == 2) ot_gemm<OT_LAST, LIMBS, 2, T>(s, apply, io); else ot_gemm<OT_LAST, LIMBS, 1, T>(s, apply, io);
+        }
         uint8_t* z = x;
         x = y;
         y = z;
@@ -673,7 +752,7 @@ void ot_run(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, uint8_t* wor
     constexpr int W = 16 / (int)sizeof(T);
     const bool wide = io.cols % W == 0 && ((uintptr_t)io.g & 15) == 0 && io.g_stride % W == 0 && io.g_batch % W == 0 && (((uintptr_t)io.m | (uintptr_t)io.m_out) & 15) == 0;
     if (wide) ot_begin<T, LIMBS, W>(s, io, poly, p, partial, work + p.x0); else ot_begin<T, LIMBS, 1>(s, io, poly, p, partial, work + p.x0);
-    if (p.ctas == 2) ot_steps<T, LIMBS, 2>(s, io, poly, work, p); else ot_steps<T, LIMBS, 1>(s, io, poly, work, p);
+    ot_steps<T, LIMBS>(s, io, poly, work, p);
 }
 
 }  // namespace
