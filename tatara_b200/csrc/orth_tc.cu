@@ -21,6 +21,8 @@
 // Every wait is bounded; where one runs out the block's results become NaN, and so the output.
 #include "orth.cuh"
 
+#include <atomic>
+
 namespace {
 
 #define OT_TILE 16384           // bytes of a tile of 128 x 64 fp16
@@ -66,9 +68,6 @@ __device__ __forceinline__ void ot_arrive_at(unsigned bar, unsigned rank) {
 __device__ __forceinline__ void ot_cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void ot_store(void* dst, unsigned src, unsigned bytes) {
-    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
 }
 // true in one lane of a whole warp, always the same one
 __device__ __forceinline__ bool ot_elect() {
@@ -288,10 +287,69 @@ struct OtShape {
     static constexpr int DRAIN = LIMBS == 2 ? 4 : 1 << 30;
 };
 
+// a tile's place: of a symmetric result those on and below the diagonal, row by row
+struct OtTile {
+    int batch, i, j;
+};
+template <bool SYM>
+__device__ __forceinline__ OtTile ot_tile(const OtGemm& g, int t, int tiles) {
+    OtTile p;
+    p.batch = t / tiles;
+    t -= p.batch * tiles;
+    if (SYM) {
+        p.i = (int)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
+        while ((p.i + 1) * (p.i + 2) / 2 <= t) ++p.i;
+        while (p.i * (p.i + 1) / 2 > t) --p.i;
+        p.j = t - p.i * (p.i + 1) / 2;
+    } else {
+        p.i = t % g.row_tiles;
+        p.j = t / g.row_tiles;
+    }
+    return p;
+}
+
+__device__ __forceinline__ void ot_store_shared(uint8_t* p, __half v) {
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(ot_smem(p)), "h"(__half_as_ushort(v)) : "memory");
+}
+__device__ __forceinline__ void ot_put(void* dst, unsigned src, unsigned bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+
+// 16 fp16 numbers of a row as they lie in a tile: two 16-byte pieces, which have changed places in odd rows
+struct OtSector {
+    unsigned w[8];
+    __device__ __forceinline__ void load(const uint8_t* p) {
+        const uint4 a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(p + 16);
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+    }
+    __device__ __forceinline__ void exchange(int swap) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned a = w[i], b = w[i + 4];
+            w[i] = swap ? b : a;
+            w[i + 4] = swap ? a : b;
+        }
+    }
+    __device__ __forceinline__ float get(int i) const { return op_word<__half>(w[i >> 1], i & 1); }
+    // into a tile's image in shared memory, the first piece at that place of the row and the second at its neighbour
+    __device__ __forceinline__ void store_shared(uint8_t* row, int place) const {
+        const unsigned p = ot_smem(row);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p + (place << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p + ((place ^ 1) << 4)), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+    }
+    __device__ __forceinline__ void store(uint8_t* p) const {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+    }
+};
+
 // CTAS = 1: a block computes 128 x 128.  CTAS = 2: a cluster of two blocks computes 256 x 256 with cta_group::2 MMAs: each block holds 128 rows
 // of the left operand, 128 columns of the right one and 128 x 256 accumulators; the even block issues the MMAs.
 // Warps 0-7 read the accumulators (warp w: lanes 32 (w % 4) .. of them, columns 64 CTAS (w / 4) ..), warp 8 copies, warp 9 issues the MMAs.
-template <int KIND, int LIMBS, int CTAS, typename T>
+// MULTI: a block (pair) takes the tiles t, t + blocks, ..; while the eight warps store a tile from their registers, the next one's copies and MMAs are
+// under way.  Those stores go straight to memory in whole 32-byte sectors (one instruction per lane; a tile's 16-byte pieces swap places inside their
+// sector in odd rows), the mirrored tile's in 64 bytes per warp.  4096 x 4096 in bf16: 1406 us with a block per tile, 1200 so.  Where all tiles run at once
+// they leave through shared memory, 5 % sooner, and both in one kernel would cost the small products 15 % (a launch runs through its code once).
+template <int KIND, int LIMBS, int CTAS, bool MULTI, typename T>
 __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
     using S = OtShape<LIMBS>;
     constexpr int TN = 128 * CTAS, COLS = 64 * CTAS;  // accumulator columns of a block, of a thread
@@ -303,20 +361,10 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
     uint8_t* s_dyn = s_raw + ((1024u - (ot_smem(s_raw) & 1023u)) & 1023u);
     const unsigned ring = ot_smem(s_dyn);
     // the warp's number is the same in its lanes, and the compiler has to know it: what the MMAs take lives in uniform registers then
-    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, batch = blockIdx.z;
-    const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, tile = blockIdx.x / CTAS;
-    int ti, tj;
-    if (SYM) {  // tiles on and below the diagonal, row by row
-        ti = (int)((sqrtf(8.0f * (float)tile + 1.0f) - 1.0f) * 0.5f);
-        while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
-        while (ti * (ti + 1) / 2 > tile) --ti;
-        tj = tile - ti * (ti + 1) / 2;
-    } else {
-        ti = tile % g.row_tiles;
-        tj = tile / g.row_tiles;
-    }
-    const bool same = SYM && ti == tj;              // one operand serves as both
-    const int row_tile = ti * CTAS + rank;          // this block's rows, in 128s
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
+    const int tiles = SYM ? g.row_tiles * (g.row_tiles + 1) / 2 : g.row_tiles * g.col_tiles, total = tiles * io.batch;
+    const OtTile only = ot_tile<SYM>(g, first, tiles);  // of a block with one tile: known before the launch ahead is done
     if (tid == 0) {
         for (int s = 0; s < S::STAGES; ++s) {
             ot_bar_init(ot_smem(&s_full[s]), 1);
@@ -349,126 +397,278 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
     const int chunk0 = KIND == OT_GRAM_PART ? (int)((int64_t)g.chunks * blockIdx.y / gridDim.y) : 0;
     const int chunks = KIND == OT_GRAM_PART ? (int)((int64_t)g.chunks * (blockIdx.y + 1) / gridDim.y) - chunk0 : g.chunks;
     const int rounds = (chunks + S::DRAIN - 1) / S::DRAIN;
-    float acc[COLS];
+    bool ok = true;
 
     if (warp == 8) {
-        const int col_tile = tj * CTAS + rank;  // this block's columns of the right operand
-        const uint8_t* a = g.a + (int64_t)batch * LIMBS * g.a_limb + ((int64_t)row_tile * g.a_width + chunk0) * OT_TILE;
-        // SYM: the tiles of a row, one after the other; else two half tiles (64 rows) at a time, the next rows' half in the same tiles or a row of tiles on
-        const uint8_t* b = g.b + (int64_t)batch * LIMBS * g.b_limb + (SYM ? (int64_t)col_tile * g.b_width + chunk0 : (int64_t)2 * col_tile) * OT_TILE;
-        const int64_t b_odd = SYM ? OT_TILE : OT_TILE / 2, b_even = SYM ? OT_TILE : (int64_t)g.b_width * OT_TILE - OT_TILE / 2;
-        const unsigned bytes = same ? LIMBS * OT_TILE : 2 * LIMBS * OT_TILE;
-        bool ok = true;
-        int k = 0;
+        asm volatile("fence.proxy.async;" ::: "memory");  // bulk copies read what the launch ahead has stored
         unsigned s = 0, parity = 1;  // a barrier that nothing has arrived at yet passes for the phase before its first
-        for (; k < chunks; ++k) {
-            const unsigned bar = ot_smem(&s_full[0]) + 8 * s, to = ring + s * S::STAGE;
-            ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_empty[0]) + 8 * s, parity));
-            if (!ok) break;
-            if (lane == 0) {
-                ot_expect(bar, bytes);
+        int64_t count = 0;           // chunks issued
+        for (int t = first; ok && t < total; t += MULTI ? step : total) {
+            const OtTile at = MULTI ? ot_tile<SYM>(g, t, tiles) : only;
+            const bool same = SYM && at.i == at.j;
+            const int col_tile = at.j * CTAS + rank;  // this block's columns of the right operand, in 128s
+            const uint8_t* a = g.a + (int64_t)at.batch * LIMBS * g.a_limb + ((int64_t)(at.i * CTAS + rank) * g.a_width + chunk0) * OT_TILE;
+            // SYM: the tiles of a row, one after the other; else two half tiles (64 rows) at a time, the next rows' half in the same tiles or a row of tiles on
+            const uint8_t* b = g.b + (int64_t)at.batch * LIMBS * g.b_limb + (SYM ? (int64_t)col_tile * g.b_width + chunk0 : (int64_t)2 * col_tile) * OT_TILE;
+            const int64_t b_odd = SYM ? OT_TILE : OT_TILE / 2, b_even = SYM ? OT_TILE : (int64_t)g.b_width * OT_TILE - OT_TILE / 2;
+            const unsigned bytes = same ? LIMBS * OT_TILE : 2 * LIMBS * OT_TILE;
+            for (int k = 0; k < chunks; ++k, ++count) {
+                const unsigned bar = ot_smem(&s_full[0]) + 8 * s, to = ring + s * S::STAGE;
+                ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_empty[0]) + 8 * s, parity));
+                if (!ok) break;
+                if (lane == 0) {
+                    ot_expect(bar, bytes);
 #pragma unroll
-                for (int l = 0; l < LIMBS; ++l) {
-                    ot_copy(to + l * OT_TILE, a + l * g.a_limb, OT_TILE, bar);
-                    if (same) continue;
-                    const unsigned tb = to + (LIMBS + l) * OT_TILE;
-                    ot_copy(tb, b + l * g.b_limb, SYM ? OT_TILE : OT_TILE / 2, bar);
-                    if (!SYM) ot_copy(tb + OT_TILE / 2, b + l * g.b_limb + OT_TILE, OT_TILE / 2, bar);
-                }
-            }
-            __syncwarp();
-            a += OT_TILE;
-            b += k & 1 ? b_even : b_odd;
-            if (++s == S::STAGES) {
-                s = 0;
-                parity ^= 1;
-            }
-        }
-        if (!ok) {  // the copies in flight land before the block ends
-            if (lane == 0) atomicExch(&s_failed, 1);
-            for (int q = k < S::STAGES ? 0 : k - S::STAGES; q < k; ++q) ot_wait(ot_smem(&s_full[q % S::STAGES]), (unsigned)((q / S::STAGES) & 1));
-        }
-    } else if (warp == 9) {
-        unsigned s = 0, parity = 0;
-        bool ok = true;
-        if (rank == 0) {
-            // fp32 accumulator (1 at bit 4), fp16 operands, N / 8 at bit 17, M / 16 at bit 24; apply: the right operand is N-major (bit 16)
-            constexpr unsigned IDESC = (1u << 4) | (SYM ? 0u : 1u << 16) | ((unsigned)(TN / 8) << 17) | ((unsigned)(8 * CTAS) << 24);
-            // descriptors of the first stage; steps along K and to other stages are added in units of 16 bytes.  K-major: 32 bytes along the
-            // row, 8-row groups 1024 bytes apart.  N-major: 16 rows of 128 bytes, 8-row groups 1024 bytes apart, the next 64 columns 8 KB further
-            const unsigned long long da0 = ot_desc(ring, 16, 1024);
-            const unsigned long long db0 = SYM ? ot_desc(same ? ring : ring + LIMBS * OT_TILE, 16, 1024) : ot_desc(ring + LIMBS * OT_TILE, OT_TILE / 2, 1024);
-            constexpr unsigned STEP_A = 2, STEP_B = SYM ? 2 : 128;
-            const bool leader = ot_elect();
-            int k = 0;
-            for (int r = 0; r < rounds && ok; ++r) {
-                const unsigned d = tmem + (unsigned)((r & 1) * TN);
-                if (r >= 2) ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_acc_empty[r & 1]), (unsigned)((r / 2 - 1) & 1)));
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const int last = min(chunks, k + S::DRAIN);
-                unsigned accumulate = 0;
-                for (; ok && k < last; ++k) {
-                    ok = ot_wait(ot_smem(&s_full[0]) + 8 * s, parity);
-                    if (CTAS == 2) ok = ok && ot_wait(ot_smem(&s_peer[0]) + 8 * s, parity);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (leader) {
-                        const unsigned long long da = da0 + s * (S::STAGE / 16), db = db0 + s * (S::STAGE / 16);
-#pragma unroll
-                        for (int q = 0; q < (LIMBS == 2 ? 3 : 1); ++q)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                ot_mma<CTAS>(d, da + (q == 2 ? OT_TILE / 16 : 0) + STEP_A * j, db + (q == 1 ? OT_TILE / 16 : 0) + STEP_B * j, IDESC,
-                                             q > 0 || j > 0 ? 1u : accumulate);
-                        ot_commit<CTAS>(ot_smem(&s_empty[0]) + 8 * s);
-                    }
-                    __syncwarp();
-                    accumulate = 1;
-                    if (++s == S::STAGES) {
-                        s = 0;
-                        parity ^= 1;
+                    for (int l = 0; l < LIMBS; ++l) {
+                        ot_copy(to + l * OT_TILE, a + l * g.a_limb, OT_TILE, bar);
+                        if (same) continue;
+                        const unsigned tb = to + (LIMBS + l) * OT_TILE;
+                        ot_copy(tb, b + l * g.b_limb, SYM ? OT_TILE : OT_TILE / 2, bar);
+                        if (!SYM) ot_copy(tb + OT_TILE / 2, b + l * g.b_limb + OT_TILE, OT_TILE / 2, bar);
                     }
                 }
-                if (leader) ot_commit<CTAS>(ot_smem(&s_acc_full[r & 1]));
                 __syncwarp();
-            }
-        } else {
-            // the odd block: tells the even one that its operands are there
-            for (int k = 0; k < chunks && ok; ++k) {
-                ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_full[0]) + 8 * s, parity));
-                if (ok && lane == 0) ot_arrive_at(ot_smem(&s_peer[0]) + 8 * s, 0);
-                __syncwarp();
+                a += OT_TILE;
+                b += k & 1 ? b_even : b_odd;
                 if (++s == S::STAGES) {
                     s = 0;
                     parity ^= 1;
                 }
             }
         }
+        if (!ok) {  // the copies in flight land before the block ends
+            if (lane == 0) atomicExch(&s_failed, 1);
+            for (int64_t q = count < S::STAGES ? 0 : count - S::STAGES; q < count; ++q) ot_wait(ot_smem(&s_full[q % S::STAGES]), (unsigned)((q / S::STAGES) & 1));
+        }
+    } else if (warp == 9) {
+        unsigned s = 0, parity = 0;
+        if (rank == 0) {
+            // fp32 accumulator (1 at bit 4), fp16 operands, N / 8 at bit 17, M / 16 at bit 24; apply: the right operand is N-major (bit 16)
+            constexpr unsigned IDESC = (1u << 4) | (SYM ? 0u : 1u << 16) | ((unsigned)(TN / 8) << 17) | ((unsigned)(8 * CTAS) << 24);
+            // descriptors of the first stage; steps along K and to other stages are added in units of 16 bytes.  K-major: 32 bytes along the
+            // row, 8-row groups 1024 bytes apart.  N-major: 16 rows of 128 bytes, 8-row groups 1024 bytes apart, the next 64 columns 8 KB further
+            const unsigned long long da0 = ot_desc(ring, 16, 1024);
+            constexpr unsigned STEP_A = 2, STEP_B = SYM ? 2 : 128;
+            const bool leader = ot_elect();
+            unsigned buffer = 0, drained = 1;  // the accumulator, and the parity of its being empty
+            for (int t = first; ok && t < total; t += MULTI ? step : total) {
+                const OtTile at = MULTI ? ot_tile<SYM>(g, t, tiles) : only;
+                const unsigned b_at = SYM && at.i == at.j ? ring : ring + LIMBS * OT_TILE;
+                const unsigned long long db0 = SYM ? ot_desc(b_at, 16, 1024) : ot_desc(b_at, OT_TILE / 2, 1024);
+                int k = 0;
+                for (int r = 0; r < rounds && ok; ++r) {
+                    const unsigned d = tmem + buffer * TN;
+                    ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_acc_empty[0]) + 8 * buffer, drained));
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const int last = min(chunks, k + S::DRAIN);
+                    unsigned accumulate = 0;
+                    for (; ok && k < last; ++k) {
+                        ok = ot_wait(ot_smem(&s_full[0]) + 8 * s, parity);
+                        if (CTAS == 2) ok = ok && ot_wait(ot_smem(&s_peer[0]) + 8 * s, parity);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (leader) {
+                            const unsigned long long da = da0 + s * (S::STAGE / 16), db = db0 + s * (S::STAGE / 16);
+#pragma unroll
+                            for (int q = 0; q < (LIMBS == 2 ? 3 : 1); ++q)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+                                    ot_mma<CTAS>(d, da + (q == 2 ? OT_TILE / 16 : 0) + STEP_A * j, db + (q == 1 ? OT_TILE / 16 : 0) + STEP_B * j, IDESC,
+                                                 q > 0 || j > 0 ? 1u : accumulate);
+                            ot_commit<CTAS>(ot_smem(&s_empty[0]) + 8 * s);
+                        }
+                        __syncwarp();
+                        accumulate = 1;
+                        if (++s == S::STAGES) {
+                            s = 0;
+                            parity ^= 1;
+                        }
+                    }
+                    if (leader) ot_commit<CTAS>(ot_smem(&s_acc_full[0]) + 8 * buffer);
+                    __syncwarp();
+                    drained ^= buffer;
+                    buffer ^= 1;
+                }
+            }
+        } else {
+            // the odd block: tells the even one that its operands are there
+            for (int t = first; ok && t < total; t += MULTI ? step : total)
+                for (int k = 0; k < chunks && ok; ++k) {
+                    ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_full[0]) + 8 * s, parity));
+                    if (ok && lane == 0) ot_arrive_at(ot_smem(&s_peer[0]) + 8 * s, 0);
+                    __syncwarp();
+                    if (++s == S::STAGES) {
+                        s = 0;
+                        parity ^= 1;
+                    }
+                }
+        }
         if (!ok && lane == 0) atomicExch(&s_failed, 1);
     } else {
         const unsigned taddr = tmem + ((unsigned)((warp & 3) * 32) << 16) + (unsigned)((warp >> 2) * COLS);
+        const int group = warp >> 2, row = tid & 127;
+        unsigned buffer = 0, filled = 0;
+        for (int t = first; t < total; t += MULTI ? step : total) {
+            const OtTile at = MULTI ? ot_tile<SYM>(g, t, tiles) : only;
+            float acc[COLS];
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) acc[c] = 0.0f;
-        for (int r = 0; r < rounds; ++r) {
-            const bool ok = ot_wait(ot_smem(&s_acc_full[r & 1]), (unsigned)((r / 2) & 1));
-            if (!__all_sync(0xffffffffu, ok)) {
-                if (lane == 0) atomicExch(&s_failed, 1);
-                break;
+            for (int c = 0; c < COLS; ++c) acc[c] = 0.0f;
+            for (int r = 0; r < rounds && ok; ++r) {
+                ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_acc_full[0]) + 8 * buffer, filled));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int c0 = 0; c0 < COLS; c0 += 32) {
+                    unsigned v[32];
+                    ot_read32(taddr + buffer * TN + c0, v);
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) acc[c0 + c] += __uint_as_float(v[c]);
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    if (CTAS == 2) ot_arrive_at(ot_smem(&s_acc_empty[0]) + 8 * buffer, 0);
+                    else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ot_smem(&s_acc_empty[0]) + 8 * buffer) : "memory");
+                }
+                filled ^= buffer;
+                buffer ^= 1;
             }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (!ok && lane == 0) atomicExch(&s_failed, 1);
+            const float poison = !ok || *static_cast<volatile int*>(&s_failed) ? __int_as_float(0x7fc00000) : 0.0f;
+
+            if (KIND == OT_GRAM_PART) {
+                float4* to = reinterpret_cast<float4*>(g.part) + ((int64_t)t * gridDim.y + blockIdx.y) * 4096 + row;
 #pragma unroll
-            for (int c0 = 0; c0 < COLS; c0 += 32) {
-                unsigned v[32];
-                ot_read32(taddr + (unsigned)((r & 1) * TN + c0), v);
+                for (int c = 0; c < COLS; c += 4) to[(group * COLS + c) / 4 * 128] = make_float4(acc[c] + poison, acc[c + 1] + poison, acc[c + 2] + poison, acc[c + 3] + poison);
+            } else if (KIND == OT_LAST) {
+                // by rounds of 64 columns through shared memory (a block has one tile, its ring is free by now)
+                float* flat = reinterpret_cast<float*>(s_dyn + group * 40960);  // [128][65]
+                const bool tall = io.rows > io.cols;
+                const int n = tall ? io.cols : io.rows, m = tall ? io.rows : io.cols;
 #pragma unroll
-                for (int c = 0; c < 32; ++c) acc[c0 + c] += __uint_as_float(v[c]);
-            }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-                if (CTAS == 2) ot_arrive_at(ot_smem(&s_acc_empty[r & 1]), 0);
-                else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ot_smem(&s_acc_empty[r & 1])) : "memory");
+                for (int h = 0; h < CTAS; ++h) {
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) flat[row * 65 + c] = acc[64 * h + c] * OT_UNSCALE + poison;
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+                    const int i0 = (at.i * CTAS + rank) * 128, j0 = (at.j * 2 * CTAS + group * CTAS + h) * 64;
+                    // 128 (64) neighbours in memory at a time, eight of a thread's old weights on their way
+                    for (int e0 = 0; e0 < 64; e0 += 8) {
+                        float w[8];
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            const int e = e0 + u, i = i0 + (tall ? row : 2 * e + (row >> 6)), j = j0 + (tall ? e : row & 63);
+                            w[u] = io.m && i < n && j < m ? io.w[at.batch * io.out_batch + (tall ? j * io.out_stride + i : i * io.out_stride + j)] : 0.0f;
+                        }
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            const int e = e0 + u, r = tall ? row : 2 * e + (row >> 6), c = tall ? e : row & 63, i = i0 + r, j = j0 + c;
+                            if (i < n && j < m) orth_store<T>(io, at.batch, tall ? j : i, tall ? i : j, w[u], flat[r * 65 + c]);
+                        }
+                    }
+                }
+            } else {
+                const bool same = SYM && at.i == at.j;
+                const int row_tile = at.i * CTAS + rank;
+                uint8_t* out = g.out + (int64_t)at.batch * LIMBS * g.out_limb;
+                // Nothing follows a block's only tile, so its ring is free for images of the result's tiles, which go out as bulk copies.  An image:
+                // [limb] tile, then mirrored [limb][column half] half a tile of 64 rows; every round has its own where the ring has room.
+                constexpr bool staged = !MULTI;
+                constexpr int IMAGES = (SYM ? 2 : 1) * LIMBS * OT_TILE;
+                constexpr bool APART = 2 * CTAS * IMAGES <= S::STAGE * S::STAGES;
+                const int swap = row & 1;  // of a sector's two pieces
+#pragma unroll
+                for (int h = 0; h < CTAS; ++h) {
+                    const int col_tile = at.j * 2 * CTAS + group * CTAS + h;  // the round's columns, in 64s
+                    const int64_t to_direct = ((int64_t)row_tile * g.out_width + col_tile) * OT_TILE;
+                    const int64_t to_mirror = ((int64_t)(col_tile >> 1) * g.out_width + 2 * row_tile) * OT_TILE + (col_tile & 1) * (OT_TILE / 2);
+                    uint8_t* image = s_dyn + (group + (APART ? 2 * h : 0)) * IMAGES;
+                    uint8_t* direct = staged ? image + row * 128 : out + to_direct + row * 128;
+                    const int64_t direct_limb = staged ? OT_TILE : g.out_limb;
+                    uint8_t* mirror = staged ? image + LIMBS * OT_TILE + (row >> 6) * (OT_TILE / 2) + (row & 7) * 2 : out + to_mirror + (row >> 6) * OT_TILE + (row & 7) * 2;
+                    const uint8_t* old = g.a + (int64_t)at.batch * LIMBS * g.a_limb + ((int64_t)row_tile * g.a_width + col_tile) * OT_TILE + row * 128;
+                    const int ident = row_tile * 128 + row - col_tile * 64;  // the diagonal's column
+                    if (h && staged && !APART) asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+                    OtSector before[LIMBS];
+                    if (KIND == OT_SQUARE)
+#pragma unroll
+                        for (int l = 0; l < LIMBS; ++l) before[l].load(old + l * g.a_limb + ((row & 6) << 4));
+#pragma unroll
+                    for (int c0 = 0; c0 < 64; c0 += 16) {
+                        float x[16];
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) x[c] = acc[64 * h + c0 + c] * OT_UNSCALE + poison;
+                        if (KIND == OT_SQUARE) {
+                            float a[16];
+#pragma unroll
+                            for (int l = 0; l < LIMBS; ++l) before[l].exchange(swap);
+#pragma unroll
+                            for (int l = 0; l < LIMBS; ++l)
+#pragma unroll
+                                for (int c = 0; c < 16; ++c) {
+                                    const float v = before[l].get(c);
+                                    a[c] = l ? a[c] + v : v;
+                                }
+                            if (c0 < 48)
+#pragma unroll
+                                for (int l = 0; l < LIMBS; ++l) before[l].load(old + l * g.a_limb + ((((c0 + 16) >> 3) ^ (row & 6)) << 4));
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) x[c] = fmaf(g.cc, x[c], fmaf(g.cb / OT_SCALE, a[c], ident == c0 + c ? g.ca : 0.0f));
+                        }
+                        OtSector piece[LIMBS];
+#pragma unroll
+                        for (int c = 0; c < 16; c += 2) {
+                            __half u[LIMBS], v[LIMBS];
+                            ot_split<LIMBS>(x[c] * OT_SCALE, u);
+                            ot_split<LIMBS>(x[c + 1] * OT_SCALE, v);
+#pragma unroll
+                            for (int l = 0; l < LIMBS; ++l) {
+                                const __half2 pair = __halves2half2(u[l], v[l]);
+                                piece[l].w[c / 2] = *reinterpret_cast<const unsigned*>(&pair);
+                                if (SYM && !same) {
+                                    uint8_t* to = mirror + (staged ? l * OT_TILE : l * g.out_limb) + (c0 + c) * 128;
+                                    const int slot = (row & 63) >> 3;
+                                    if (staged) {  // not left to the compiler: a generic store costs as much as a global one
+                                        ot_store_shared(to + (((slot ^ (c0 + c)) & 7) << 4), u[l]);
+                                        ot_store_shared(to + 128 + (((slot ^ (c0 + c + 1)) & 7) << 4), v[l]);
+                                    } else {
+                                        *reinterpret_cast<__half*>(to + (((slot ^ (c0 + c)) & 7) << 4)) = u[l];
+                                        *reinterpret_cast<__half*>(to + 128 + (((slot ^ (c0 + c + 1)) & 7) << 4)) = v[l];
+                                    }
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int l = 0; l < LIMBS; ++l) {
+                            uint8_t* to = direct + l * direct_limb;
+                            if (staged) {
+                                piece[l].store_shared(to, (c0 >> 3) ^ (row & 7));
+                            } else {
+                                piece[l].exchange(swap);
+                                piece[l].store(to + (((c0 >> 3) ^ (row & 6)) << 4));
+                            }
+                        }
+                    }
+                    if (staged) {
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+                        if (row == 0) {
+#pragma unroll
+                            for (int l = 0; l < LIMBS; ++l) {
+                                ot_put(out + l * g.out_limb + to_direct, ot_smem(image + l * OT_TILE), OT_TILE);
+                                if (SYM && !same) {
+#pragma unroll
+                                    for (int q = 0; q < 2; ++q)
+                                        ot_put(out + l * g.out_limb + to_mirror + q * OT_TILE, ot_smem(image + (LIMBS + l) * OT_TILE + q * (OT_TILE / 2)), OT_TILE / 2);
+                                }
+                            }
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                            // the images must be read before they are written again, or the block ends
+                            if (!APART || h + 1 == CTAS) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        }
+                    }
+                }
             }
         }
     }
@@ -480,102 +680,6 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
     if (warp == 9) {
         if (CTAS == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TN) : "memory");
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TN) : "memory");
-    }
-    if (warp >= 8) return;
-
-    if (KIND == OT_GRAM_PART) {
-        const float poison = s_failed ? __int_as_float(0x7fc00000) : 0.0f;
-        float4* to = reinterpret_cast<float4*>(g.part) + (((int64_t)batch * gridDim.x + blockIdx.x) * gridDim.y + blockIdx.y) * 4096 + (tid & 127);
-#pragma unroll
-        for (int c = 0; c < COLS; c += 4) to[((warp >> 2) * COLS + c) / 4 * 128] = make_float4(acc[c] + poison, acc[c + 1] + poison, acc[c + 2] + poison, acc[c + 3] + poison);
-        return;
-    }
-    // Epilogue by two groups of 128 threads, a row each, in rounds of 64 columns through the group's part of shared memory.
-    const float poison = s_failed ? __int_as_float(0x7fc00000) : 0.0f;
-    const int group = warp >> 2, row = tid & 127;
-    // a round's images: [limb] tile, and mirrored [limb][column half] half a tile of 64 rows; every round has its own where the ring has room
-    constexpr int IMAGES = (SYM ? 2 : 1) * LIMBS * OT_TILE;
-    constexpr bool APART = 2 * CTAS * IMAGES <= S::STAGE * S::STAGES;
-    float* flat = reinterpret_cast<float*>(s_dyn + group * 40960);  // OT_LAST: [128][65]
-#pragma unroll
-    for (int h = 0; h < CTAS; ++h) {
-        const int col_tile = tj * 2 * CTAS + group * CTAS + h;    // the round's columns, in 64s
-        uint8_t* direct = s_dyn + (group + (APART ? 2 * h : 0)) * IMAGES;
-        uint8_t* mirror = direct + LIMBS * OT_TILE;
-        if (h && (!APART || KIND == OT_LAST)) asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
-        if (KIND == OT_LAST) {
-#pragma unroll
-            for (int c = 0; c < 64; ++c) flat[row * 65 + c] = acc[64 * h + c] * OT_UNSCALE + poison;
-            asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
-            const bool tall = io.rows > io.cols;
-            const int n = tall ? io.cols : io.rows, m = tall ? io.rows : io.cols;
-            // 128 (64) neighbours in memory at a time, eight of a thread's old weights on their way
-            for (int e0 = 0; e0 < 64; e0 += 8) {
-                float w[8];
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int e = e0 + u, i = row_tile * 128 + (tall ? row : 2 * e + (row >> 6)), j = col_tile * 64 + (tall ? e : row & 63);
-                    w[u] = io.m && i < n && j < m ? io.w[batch * io.out_batch + (tall ? j * io.out_stride + i : i * io.out_stride + j)] : 0.0f;
-                }
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int e = e0 + u, r = tall ? row : 2 * e + (row >> 6), c = tall ? e : row & 63, i = row_tile * 128 + r, j = col_tile * 64 + c;
-                    if (i < n && j < m) orth_store<T>(io, batch, tall ? j : i, tall ? i : j, w[u], flat[r * 65 + c]);
-                }
-            }
-        } else {
-            const uint8_t* old = KIND == OT_SQUARE ? g.a + (int64_t)batch * LIMBS * g.a_limb + ((int64_t)row_tile * g.a_width + col_tile) * OT_TILE : nullptr;
-#pragma unroll
-            for (int c0 = 0; c0 < 64; c0 += 8) {
-                float x[8];
-#pragma unroll
-                for (int c = 0; c < 8; ++c) x[c] = acc[64 * h + c0 + c] * OT_UNSCALE + poison;
-                if (KIND == OT_SQUARE) {
-                    float a[8];
-#pragma unroll
-                    for (int l = 0; l < LIMBS; ++l) {
-                        float t[8];
-                        op_load<__half, 8>(reinterpret_cast<const __half*>(old + l * g.a_limb + ot_at(row, c0)), t);
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) a[c] = l ? a[c] + t[c] : t[c];
-                    }
-#pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        x[c] = fmaf(g.cc, x[c], fmaf(g.cb / OT_SCALE, a[c], row_tile * 128 + row == col_tile * 64 + c0 + c ? g.ca : 0.0f));
-                }
-                OpVec<__half, 8> piece[LIMBS];
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    __half s[LIMBS];
-                    ot_split<LIMBS>(x[c] * OT_SCALE, s);
-#pragma unroll
-                    for (int l = 0; l < LIMBS; ++l) {
-                        piece[l].v[c] = s[l];
-                        if (SYM && !same) *reinterpret_cast<__half*>(mirror + (l * 2 + (row >> 6)) * (OT_TILE / 2) + ot_at(c0 + c, row & 63)) = s[l];
-                    }
-                }
-#pragma unroll
-                for (int l = 0; l < LIMBS; ++l) *reinterpret_cast<OpVec<__half, 8>*>(direct + l * OT_TILE + ot_at(row, c0)) = piece[l];
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
-            if (row == 0) {
-                uint8_t* o = g.out + (int64_t)batch * LIMBS * g.out_limb;
-#pragma unroll
-                for (int l = 0; l < LIMBS; ++l) {
-                    ot_store(o + l * g.out_limb + ((int64_t)row_tile * g.out_width + col_tile) * OT_TILE, ot_smem(direct + l * OT_TILE), OT_TILE);
-                    if (SYM && !same) {
-#pragma unroll
-                        for (int q = 0; q < 2; ++q)
-                            ot_store(o + l * g.out_limb + ((int64_t)(col_tile >> 1) * g.out_width + 2 * row_tile + q) * OT_TILE + (col_tile & 1) * (OT_TILE / 2),
-                                     ot_smem(mirror + (l * 2 + q) * (OT_TILE / 2)), OT_TILE / 2);
-                    }
-                }
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                // the images must be read before they are written again, or the block ends
-                if (!APART || h + 1 == CTAS) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            }
-        }
     }
 }
 
@@ -660,25 +764,38 @@ OtPlan ot_plan(int batch, int rows, int cols, int limbs) {
     return p;
 }
 
-template <int KIND, int LIMBS, int CTAS, typename T>
-void ot_gemm(cudaStream_t s, const OtGemm& g, const OrthIo& io, int parts = 1) {
+template <int KIND, int LIMBS, int CTAS, bool MULTI, typename T>
+void ot_launch(cudaStream_t s, const OtGemm& g, const OrthIo& io, int64_t blocks, int parts) {
     using S = OtShape<LIMBS>;
-    cudaFuncSetAttribute(k_orth_gemm<KIND, LIMBS, CTAS, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-    const int tiles = KIND == OT_APPLY || KIND == OT_LAST ? g.row_tiles * g.col_tiles : g.row_tiles * (g.row_tiles + 1) / 2;
+    auto kern = k_orth_gemm<KIND, LIMBS, CTAS, MULTI, T>;
+    static std::atomic<uint64_t> known{0};  // devices on which the kernel may take that much shared memory
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !(known.load(std::memory_order_relaxed) >> dev & 1)) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) == cudaSuccess && dev >= 0 && dev < 64) known.fetch_or(1ull << dev);
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * CTAS), (unsigned)parts, (unsigned)io.batch);
+    cfg.gridDim = dim3((unsigned)(blocks * CTAS), (unsigned)parts);
     cfg.blockDim = dim3(320);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = s;
     cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = CTAS;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = CTAS;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 2;
-    cudaLaunchKernelEx(&cfg, k_orth_gemm<KIND, LIMBS, CTAS, T>, g, io);
+    cfg.numAttrs = CTAS == 2 ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kern, g, io);
+}
+template <int KIND, int LIMBS, int CTAS, typename T>
+void ot_gemm(cudaStream_t s, const OtGemm& g, const OrthIo& io, int parts = 1) {
+    const int64_t tiles = KIND == OT_APPLY || KIND == OT_LAST ? (int64_t)g.row_tiles * g.col_tiles : (int64_t)g.row_tiles * (g.row_tiles + 1) / 2;
+    const int64_t all = tiles * io.batch, slots = sm_count() / CTAS;
+    if constexpr (KIND != OT_LAST && KIND != OT_GRAM_PART)
+        if (all > slots) return ot_launch<KIND, LIMBS, CTAS, true, T>(s, g, io, slots, parts);
+    ot_launch<KIND, LIMBS, CTAS, false, T>(s, g, io, all, parts);
 }
 
 template <typename T, int LIMBS>
