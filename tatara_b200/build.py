@@ -4,6 +4,8 @@
 
 nvcc cross-compiles without a GPU.  The library links the CUDA runtime statically and has no other
 link-time dependency (NCCL is opened at run time only when world_size > 1).
+
+Where torch is installed, the binding of the operators on torch tensors (_ops.so, csrc/torch_ops.cpp, plain C++) is built too.
 """
 from __future__ import annotations
 
@@ -11,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -68,5 +71,32 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB_PATH
 
 
+OPS_PATH = os.path.join(HERE, "_ops.so")
+
+
+def build_ops(force: bool = False) -> str | None:
+    """Builds the torch binding beside the library it calls; None where torch is not installed."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    root = os.path.dirname(torch.__file__)
+    src, libs = os.path.join(CSRC, "torch_ops.cpp"), os.path.join(root, "lib")
+    stamp = os.path.join(OBJ_DIR, "torch_version")  # the binding belongs to one torch
+    same = os.path.exists(stamp) and open(stamp).read() == torch.__version__
+    if force or not same or _stale(OPS_PATH, [src, HEADERS[-1]]):
+        cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
+               "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               "-I" + os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include"), src, "-o", OPS_PATH, "-L" + libs, "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu",
+               "-ltorch", "-lc10_cuda", "-lc10", "-L" + HERE, "-l:libtatara_b200.so", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + libs]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("g++ failed: %s\n%s" % (" ".join(cmd), r.stderr))
+        with open(stamp, "w") as f:
+            f.write(torch.__version__)
+    return OPS_PATH
+
+
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="-v" in sys.argv))
+    print(build_ops(force="--force" in sys.argv) or "torch is not installed: no _ops.so")

@@ -137,7 +137,7 @@ constexpr int norm_backward_per_sm(int warps) {
 }
 
 // Backward: a block of W warps per row (W = 1: four rows side by side, a warp each) takes R rows at a time, which shares one barrier, walks
-// down the rows and keeps its columns' weight and bias gradients in registers; partial: [2][blocks (W = 1: four times)][n].
+// down the rows and keeps its columns' weight and bias gradients in registers; partial: [2][blocks][n].
 // fp32, 65536 x 1536: 175 us, 6.9 TB/s.
 template <typename T, int W, int VEC, int CH, int R>
 __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, norm_backward_per_sm(W))
@@ -157,6 +157,7 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
     }
     const float inv_n = 1.0f / (float)n;
     int turn = 0;
+    op_next_may_start();
     for (int64_t first = ((int64_t)blockIdx.x * RB + (W == 1 ? warp : 0)) * R; first < rows; first += (int64_t)gridDim.x * RB * R, turn ^= 1) {
         OpRaw<T, VEC> xv[R][CH], gv[R][CH];
         float mu[R], r[R], s1[R], s2[R];
@@ -239,13 +240,34 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
         }
     }
     if (!partial) return;
-    const int64_t prow = W == 1 ? (int64_t)blockIdx.x * RB + warp : blockIdx.x, prows = (int64_t)gridDim.x * RB;
+    if (W == 1) {  // the four warps' sums, in order
+        __shared__ float s_acc[3][2][32 * CH * VEC];
+        if (warp > 0)
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    s_acc[warp - 1][0][(c * VEC + i) * 32 + lane] = aw[c][i];
+                    s_acc[warp - 1][1][(c * VEC + i) * 32 + lane] = ab[c][i];
+                }
+        __syncthreads();
+        if (warp > 0) return;
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    aw[c][i] += s_acc[q][0][(c * VEC + i) * 32 + lane];
+                    ab[c][i] += s_acc[q][1][(c * VEC + i) * 32 + lane];
+                }
+    }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int col = (c * 32 * W + t) * VEC;
         if (col < n) {  // n is a multiple of VEC
-            op_store<float, VEC>(partial + prow * n + col, aw[c]);
-            op_store<float, VEC>(partial + (prows + prow) * n + col, ab[c]);
+            op_store<float, VEC>(partial + (int64_t)blockIdx.x * n + col, aw[c]);
+            op_store<float, VEC>(partial + ((int64_t)gridDim.x + blockIdx.x) * n + col, ab[c]);
         }
     }
 }
@@ -287,6 +309,7 @@ k_norm_columns_long(const T* __restrict__ dy, int64_t dy_stride, const T* __rest
     }
     partial[(int64_t)blockIdx.y * n + col] = aw;
     partial[(int64_t)(gridDim.y + blockIdx.y) * n + col] = ab;
+    op_next_may_start();
 }
 
 // dweight and dbias from the blocks' rows: eight columns (a 32-byte sector) per block; thread group r of 128 adds the rows r, r + 128, .., the four
@@ -295,10 +318,11 @@ __global__ void __launch_bounds__(1024) k_norm_columns_final(const float* __rest
                                                               float* __restrict__ dbias) {
     __shared__ float s_sum[32][9];
     float* out = blockIdx.y ? dbias : dweight;
-    if (!out) return;
+    if (!out) return;  // of the same block all
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = threadIdx.x & 7, col = blockIdx.x * 8 + c;
     const float* p = partial + (int64_t)blockIdx.y * prows * n;
     float v = 0.0f;
+    op_wait_for_previous();
     if (col < n)
         for (int r0 = threadIdx.x >> 3; r0 < prows; r0 += 128 * 8) {
             float t[8];
@@ -327,16 +351,16 @@ NormShape norm_backward_shape(int n) {
         if (n <= w * 256) return {w, 8};
     return {16, 16};
 }
-// Blocks: at most what runs at once, and 16 rows or more for each, or the blocks' rows of gradients cost as much
-// as the rows themselves.
+// Blocks: at most what runs at once; 16 rows (W = 1: 64) or more for each, or the blocks' rows of gradients cost as much as the rows themselves, but
+// one per SM as far as the rows go (256 rows of 256: 4 blocks took 12 us).
 int norm_backward_blocks(int64_t rows, int n) {
     if (n > NORM_REG_N_BACK) return (int)(rows < 64 ? (rows < 1 ? 1 : rows) : 64);
     const int w = norm_backward_shape(n).warps;
-    const int64_t per = w == 1 ? 4 * 16 : 16, most = (int64_t)sm_count() * norm_backward_per_sm(w);
-    const int64_t want = (rows + per - 1) / per;
-    return (int)(want < 1 ? 1 : want < most ? want : most);
+    const int64_t turn = w == 1 ? 8 : 2, sms = sm_count(), most = sms * norm_backward_per_sm(w);
+    const int64_t turns = (rows + turn - 1) / turn, want = (turns + 7) / 8;
+    const int64_t few = turns < sms ? turns : sms, blocks = want < few ? few : want < most ? want : most;
+    return (int)(blocks < 1 ? 1 : blocks);
 }
-int norm_partial_rows(int64_t rows, int n) { return norm_backward_blocks(rows, n) * (n <= 256 ? 4 : 1); }
 
 template <typename T, int VEC, int W, int CH>
 void norm_forward_go(cudaStream_t s, const void* x, int64_t xs, const float* w, const float* b, float eps, int64_t rows, int n, void* y, int64_t ys,
@@ -413,7 +437,7 @@ extern "C" int tb_layer_norm_forward(const void* d_x, int64_t x_stride, const fl
 
 extern "C" int64_t tb_layer_norm_backward_workspace(int64_t rows, int n) {
     if (rows < 0 || rows > NORM_MAX_ROWS || n < 1) return TB_ERR_INVALID_ARGUMENT;
-    return (int64_t)norm_partial_rows(rows, n) * 2 * n * (int64_t)sizeof(float);
+    return (int64_t)norm_backward_blocks(rows, n) * 2 * n * (int64_t)sizeof(float);
 }
 
 extern "C" int tb_layer_norm_backward(const void* d_dy, int64_t dy_stride, const void* d_x, int64_t x_stride, const float* d_mean, const float* d_rstd,
@@ -444,6 +468,6 @@ extern "C" int tb_layer_norm_backward(const void* d_dy, int64_t dy_stride, const
     else if (type == TB_TYPE_F16) wide ? norm_backward_pick<__half, 8>(ARGS) : norm_backward_pick<__half, 1>(ARGS);
     else wide ? norm_backward_pick<__nv_bfloat16, 8>(ARGS) : norm_backward_pick<__nv_bfloat16, 1>(ARGS);
 #undef ARGS
-    if (columns) k_norm_columns_final<<<dim3((unsigned)ceil_div(n, 8), 2), 1024, 0, s>>>(partial, norm_partial_rows(rows, n), n, d_dweight, d_dbias);
+    if (columns) op_launch_next(s, dim3((unsigned)ceil_div(n, 8), 2), dim3(1024), 0, k_norm_columns_final, partial, blocks, n, d_dweight, d_dbias);
     return op_launched(err, err_len);
 }

@@ -73,6 +73,25 @@ static __device__ __forceinline__ float op_group_sum(float v) {
     return v;
 }
 
+// Launches of one call overlap (programmatic dependent launch): a kernel may start before the one ahead of it has finished, and waits for it
+// before it touches what that one writes or reads.
+static __device__ __forceinline__ void op_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+static __device__ __forceinline__ void op_next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... P, typename... A>
+static inline void op_launch_next(cudaStream_t s, dim3 grid, dim3 block, size_t smem, void (*kernel)(P...), A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 static inline int op_type_size(int type) { return type == TB_TYPE_F32 ? 4 : type == TB_TYPE_F16 || type == TB_TYPE_BF16 ? 2 : 0; }
 
 #if defined(__GNUC__)

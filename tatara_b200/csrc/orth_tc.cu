@@ -53,10 +53,6 @@ __device__ __forceinline__ void ot_expect(unsigned bar, unsigned bytes) {
 __device__ __forceinline__ void ot_copy(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-// Launches of a call overlap (programmatic dependent launch): a kernel may start before the one ahead of it has finished, and waits for it before
-// it touches global memory.
-__device__ __forceinline__ void ot_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void ot_next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // Arrives at the same barrier of block `rank` of the cluster.  What it announces are operands that copies have brought (their bytes were counted
 // before this thread arrives) or accumulators that have been read; no store of this thread's.  A release at cluster scope waits for the copies in
 // flight as well: it made a chunk of 256 x 256 tiles of one limb take 1250 cycles instead of 500.
@@ -194,7 +190,7 @@ __global__ void __launch_bounds__(256) k_orth_norm(OrthIo io, int64_t segments, 
         for (int w = 1; w < 8; ++w) sum += s_sum[w];
         partial[b * OT_NORM_BLOCKS + blockIdx.x] = sum;
     }
-    ot_next_may_start();
+    op_next_may_start();
 }
 
 // One tile per block: X0 = u / (|u| + eps), n x m with n <= m, zeros beyond both.  A thread makes 16-byte pieces of the tile: of N adjacent elements each
@@ -205,8 +201,8 @@ __global__ void __launch_bounds__(256) k_orth_pack(OrthIo io, float eps, const d
     __shared__ double s_part[8];
     const int b = blockIdx.z;
     const int n = TALL ? io.cols : io.rows, m = TALL ? io.rows : io.cols;
-    ot_wait_for_previous();
-    ot_next_may_start();
+    op_wait_for_previous();
+    op_next_may_start();
     double v = 0.0;
     for (int i = threadIdx.x; i < n_partial; i += 256) v += partial[b * OT_NORM_BLOCKS + i];
 #pragma unroll
@@ -391,8 +387,8 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
     __syncthreads();
     if (CTAS == 2) ot_cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    ot_wait_for_previous();
-    ot_next_may_start();
+    op_wait_for_previous();
+    op_next_may_start();
     const unsigned tmem = s_tmem;
     const int chunk0 = KIND == OT_GRAM_PART ? (int)((int64_t)g.chunks * blockIdx.y / gridDim.y) : 0;
     const int chunks = KIND == OT_GRAM_PART ? (int)((int64_t)g.chunks * (blockIdx.y + 1) / gridDim.y) - chunk0 : g.chunks;
@@ -690,8 +686,8 @@ __global__ void __launch_bounds__(256) k_orth_join(const float* __restrict__ par
     int ti = 0;
     while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
     const int tj = tile - ti * (ti + 1) / 2, row = threadIdx.x & 127, quad = (blockIdx.x & 15) * 2 + (threadIdx.x >> 7), col = quad * 4;
-    ot_wait_for_previous();
-    ot_next_may_start();
+    op_wait_for_previous();
+    op_next_may_start();
     const float4* p = reinterpret_cast<const float4*>(part) + ((int64_t)batch * tiles + tile) * parts * 4096 + quad * 128 + row;
     float4 t[OT_PARTS];
 #pragma unroll
@@ -810,17 +806,7 @@ void ot_steps(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, uint8_t* w
         const OtGemm apply = {q, x, y, p.a_limb, p.x_limb, p.x_limb, wn, wm, wm, kn, rt, ct, 0.f, 0.f, 0.f, nullptr};
         if (p.parts > 1) {
             ot_gemm<OT_GRAM_PART, LIMBS, 1, float>(s, gram, io, p.parts);
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3((unsigned)(st * (st + 1) / 2 * 16), 1, (unsigned)io.batch);
-            cfg.blockDim = dim3(256);
-            cfg.stream = s;
-            cudaLaunchAttribute at[1];
-            at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-            at[0].val.programmaticStreamSerializationAllowed = 1;
-            cfg.attrs = at;
-            cfg.numAttrs = 1;
-            const float* sums = part;
-            cudaLaunchKernelEx(&cfg, k_orth_join<LIMBS>, sums, p.parts, a, p.a_limb, wn);
+            op_launch_next(s, dim3((unsigned)(st * (st + 1) / 2 * 16), 1, (unsigned)io.batch), dim3(256), 0, k_orth_join<LIMBS>, part, p.parts, a, p.a_limb, wn);
         } else if (p.sym_ctas == 2) {
             ot_gemm<OT_GRAM, LIMBS, 2, float>(s, gram, io);
         } else {
@@ -847,18 +833,9 @@ void ot_begin(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, const OtPl
     most = most < 1 ? 1 : most < OT_NORM_BLOCKS ? most : OT_NORM_BLOCKS;
     const int blocks = (int)(segments < most ? segments : most);
     k_orth_norm<T, N><<<dim3((unsigned)blocks, (unsigned)io.batch), 256, 0, s>>>(io, segments, len, total, partial);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(p.m_pad / 64), (unsigned)(p.n_pad / 128), (unsigned)io.batch);
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    const double* sums = partial;
-    if (io.rows > io.cols) cudaLaunchKernelEx(&cfg, k_orth_pack<T, LIMBS, 1, true>, io, poly.eps, sums, blocks, x, p.x_limb);
-    else cudaLaunchKernelEx(&cfg, k_orth_pack<T, LIMBS, N, false>, io, poly.eps, sums, blocks, x, p.x_limb);
+    const dim3 grid((unsigned)(p.m_pad / 64), (unsigned)(p.n_pad / 128), (unsigned)io.batch);
+    if (io.rows > io.cols) op_launch_next(s, grid, dim3(256), 0, k_orth_pack<T, LIMBS, 1, true>, io, poly.eps, partial, blocks, x, p.x_limb);
+    else op_launch_next(s, grid, dim3(256), 0, k_orth_pack<T, LIMBS, N, false>, io, poly.eps, partial, blocks, x, p.x_limb);
 }
 
 template <typename T, int LIMBS>

@@ -146,6 +146,7 @@ k_route_forward(const T* __restrict__ logits, int64_t stride, const uint8_t* __r
     const int lane = threadIdx.x % G, group = threadIdx.x / G, wl = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int e = threadIdx.x; e <= experts; e += ROUTE_THREADS) s_count[e] = 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) *part.ticket = 0;
+    op_next_may_start();
     __syncthreads();
     float sum_p[V], sum_z = 0.0f;
 #pragma unroll
@@ -266,6 +267,7 @@ __global__ void __launch_bounds__(1024) k_route_final(RouteParts part, int block
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e0 = blockIdx.x * 32;
     double p = 0.0, z = 0.0;
     int c = 0, n = 0;
+    op_wait_for_previous();
     if (e0 + lane < experts)
 #pragma unroll 8
         for (int b = warp; b < blocks; b += 32) {
@@ -515,7 +517,7 @@ extern "C" int tb_route_forward(const void* d_logits, int64_t stride, int type, 
     else if (type == TB_TYPE_F16) route_forward_go<__half>(ARGS);
     else route_forward_go<__nv_bfloat16>(ARGS);
 #undef ARGS
-    k_route_final<<<(unsigned)((experts + 31) / 32), 1024, 0, s>>>(part, blocks, experts, k, d_counts, d_rows, d_prob_mean, d_losses);
+    op_launch_next(s, dim3((unsigned)((experts + 31) / 32)), dim3(1024), 0, k_route_final, part, blocks, experts, k, d_counts, d_rows, d_prob_mean, d_losses);
     return op_launched(err, err_len);
 }
 
