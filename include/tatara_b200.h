@@ -299,7 +299,7 @@ int tb_orthogonalise(const void* d_x, int64_t x_batch, int64_t x_stride, int typ
 
 /* The Muon step of a batch of weight matrices, all contiguous [batch, rows, cols]: m' = beta m + g; u = nesterov ? g + beta m' : m';
  * w' = clamp(w (1 - lr weight_decay) - lr scale orthogonalise(u), -clip, clip).  w, m and their results are fp32 (each result may be its
- * input's memory), g any type. */
+ * input's memory and must not overlap any other tensor), g any type. */
 typedef struct tb_muon {
     int32_t struct_size; /* sizeof(tb_muon) of the caller */
     int32_t steps, nesterov;

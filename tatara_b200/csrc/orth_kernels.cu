@@ -414,6 +414,13 @@ extern "C" int tb_muon_step(const tb_muon* cfg, const float* d_w, const float* d
     if (!d_w || !d_m || !d_g || !d_w_out || !d_m_out) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "a device pointer is NULL");
     if (((uintptr_t)d_w | (uintptr_t)d_m | (uintptr_t)d_w_out | (uintptr_t)d_m_out) & 3 || (uintptr_t)d_g % op_type_size(g_type))
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
+    // a result may be its input's memory and must not touch any other tensor's
+    const uintptr_t count = (uintptr_t)batch * rows * cols;
+    const auto apart = [](const void* a, uintptr_t a_bytes, const void* b, uintptr_t b_bytes) { return (uintptr_t)a + a_bytes <= (uintptr_t)b || (uintptr_t)b + b_bytes <= (uintptr_t)a; };
+    const uintptr_t f = count * 4, gb = count * op_type_size(g_type);
+    if ((d_w_out != d_w && !apart(d_w_out, f, d_w, f)) || (d_m_out != d_m && !apart(d_m_out, f, d_m, f)) || !apart(d_w_out, f, d_m_out, f) || !apart(d_w_out, f, d_m, f) ||
+        !apart(d_m_out, f, d_w, f) || !apart(d_g, gb, d_w_out, f) || !apart(d_g, gb, d_m_out, f))
+        return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "a result overlaps another tensor");
     OrthIo io = {};
     io.g = d_g;
     io.g_batch = io.out_batch = (int64_t)rows * cols;

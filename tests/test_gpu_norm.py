@@ -136,6 +136,22 @@ def test_gradient_against_differences(rows, n):
         assert abs(float((grad.double() * d).sum()) - want) <= tol
 
 
+def test_offsets_beyond_32_bits():
+    rows, n = 1_100_000, 2048
+    x = torch.empty(rows, n, dtype=torch.float16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1))
+    tail, keep = x[-5:].clone(), x[:5].clone()
+    want = ops().layer_norm_forward(tail, eps=EPS)
+    y, mean, rstd = ops().layer_norm_forward(x, eps=EPS, out=x)
+    assert torch.equal(y[-5:], want[0]) and torch.equal(mean[-5:], want[1])
+    assert torch.equal(y[:5], ops().layer_norm_forward(keep, eps=EPS)[0])
+    dx, dw, db = ops().layer_norm_backward(y, y, torch.zeros_like(mean), torch.ones_like(rstd), out=y)
+    t = want[0].float()
+    ref = norm_backward(want[0], want[0], torch.zeros(5, device="cuda"), torch.ones(5, device="cuda"), None)
+    assert (dx[-5:].double() - ref[0]).abs().max() <= 2.0 ** -10 * float(t.abs().max())   # one rounding of a value that cancels
+    # sums of 1.1e6 squares of unit variance: chains of a few thousand per block, then 600 blocks
+    assert (dw / rows - 1).abs().max() <= 0.01
+
+
 def test_another_stream():
     x = make(5000, 768, torch.float32, 11)
     torch.cuda.synchronize()

@@ -151,17 +151,32 @@ def test_another_stream():
     assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("rows,cols", [(8, 40), (70, 130)])
+def test_matrices_far_apart(rows, cols):
+    """Offsets beyond 32 bits."""
+    far = (1 << 31) + 64
+    wide = torch.zeros(far + rows * cols, dtype=torch.bfloat16, device="cuda")
+    x = wide.as_strided((2, rows, cols), (far, cols, 1))
+    x.copy_(make(2, rows, cols, 9, torch.bfloat16))
+    want = ops().orthogonalise(x.contiguous())
+    assert torch.equal(ops().orthogonalise(x), want)
+    assert torch.equal(ops().orthogonalise(x, out=x), want) and (wide[rows * cols:far] == 0).all()
+
+
 def test_refusals():
     o = ops()
     x = make(2, 70, 80, 0)
     w = x.clone()
+    both = torch.zeros(3, 70, 80, device="cuda")
     for bad in (lambda: o.orthogonalise(x.double()), lambda: o.orthogonalise(x.cpu()), lambda: o.orthogonalise(x[0, 0]), lambda: o.orthogonalise(x.transpose(1, 2)),
                 lambda: o.orthogonalise(x, steps=0), lambda: o.orthogonalise(x, steps=33), lambda: o.orthogonalise(x, eps=-1.0), lambda: o.orthogonalise(x, coefficients=(8.0, 0.0, 0.0)),
                 lambda: o.orthogonalise(x, coefficients=(1.0, 2.0)), lambda: o.orthogonalise(x, coefficients=(math.nan, 0.0, 0.0)), lambda: o.orthogonalise(x, out=x.half()),
                 lambda: o.orthogonalise(x, out=x[0]), lambda: o.orthogonalise(x[:, :0]), lambda: o.orthogonalise(x[:1].expand(2, 70, 80)),
                 lambda: o.muon_step(w, x[:1], x, lr=0.1), lambda: o.muon_step(w, w, x.double(), lr=0.1), lambda: o.muon_step(w.half(), w, x, lr=0.1),
                 lambda: o.muon_step(w, w, x.cpu(), lr=0.1), lambda: o.muon_step(w, w, x, lr=0.1, clip=0.0), lambda: o.muon_step(w, w, x, lr=0.1, clip=math.nan),
-                lambda: o.muon_step(w.transpose(1, 2), w, x, lr=0.1)):
+                lambda: o.muon_step(w.transpose(1, 2), w, x, lr=0.1), lambda: o.muon_step(w, w, x, lr=0.1), lambda: o.muon_step(w, x, x, lr=0.1),
+                lambda: o.muon_step(both[:2], x, w, lr=0.1, weight_out=both[1:]), lambda: o.muon_step(both[0], both[1], both[2], lr=0.1, momentum_out=both[2]),
+                lambda: o.muon_step(both[0], both[1], both[2], lr=0.1, weight_out=both[1])):
         with pytest.raises(tb.TrainerError):
             bad()
     lib = tb.load_library()

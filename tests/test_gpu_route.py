@@ -182,6 +182,14 @@ def test_either_gradient_alone_and_strides():
     assert all(torch.equal(p, q) for p, q in zip(r, again))
 
 
+def test_offsets_beyond_32_bits():
+    far = (1 << 30) + 16
+    wide = torch.zeros(3 * far, dtype=torch.float16, device="cuda")
+    x = wide.as_strided((3, 12), (far, 1))
+    x.copy_(make(3, 12, torch.float16, 4))
+    check(x, 2, True, None, ops().route_forward(x, 2))
+
+
 def test_uint8_mask_and_another_stream():
     x = make(3000, 9, torch.float32, 8)
     mask = torch.rand(3000, device="cuda") > 0.5
