@@ -29,6 +29,19 @@ __device__ __forceinline__ float norm_row_sum(float v, float* buf, int warp_in_r
     return v;
 }
 
+// the same of R rows of a warp (R = 1 with several warps per row), in place
+template <int W, int R>
+__device__ __forceinline__ void norm_rows_sum(float (&v)[R], float* buf, int warp_in_row, int lane) {
+    if (W > 1) {
+        v[0] = norm_row_sum<W>(v[0], buf, warp_in_row, lane);
+        return;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int q = 0; q < R; ++q) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
+}
+
 // VEC columns of a weight or bias, in 16-byte accesses (one element at a time they cost four to eight times the L1 wavefronts of the row
 // itself: 24 -> 8 us for 10000 rows of 1000 fp16)
 template <int VEC>
@@ -45,61 +58,73 @@ __device__ __forceinline__ void norm_columns(const float* __restrict__ p, int co
     }
 }
 
-// W warps per row, VEC adjacent columns per access, CH accesses per thread: a thread holds columns (c * 32 W + t) * VEC + i
-template <typename T, int W, int VEC, int CH>
+// W warps per row, VEC adjacent columns per access, CH accesses per thread: a thread holds columns (c * 32 W + t) * VEC + i.  A warp of its own (W = 1) takes R
+// rows at once, which share its reads of weight and bias.
+template <typename T, int W, int VEC, int CH, int R>
 __global__ void __launch_bounds__(W == 1 ? 128 : W * 32)
-k_norm_forward(const T* __restrict__ x, int64_t x_stride, const float* __restrict__ weight, const float* __restrict__ bias, float eps,
-               int64_t rows, int n, T* __restrict__ y, int64_t y_stride, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-    constexpr int RB = W == 1 ? 4 : 1;  // rows per block
+k_norm_forward(const T* x, int64_t x_stride, const float* __restrict__ weight, const float* __restrict__ bias, float eps,
+               int64_t rows, int n, T* y, int64_t y_stride, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+    constexpr int RB = W == 1 ? 4 * R : 1;  // rows per block
     __shared__ float s_sum[2][W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = W == 1 ? lane : threadIdx.x;
-    const int64_t row = (int64_t)blockIdx.x * RB + (W == 1 ? warp : 0);
+    const int64_t row = (int64_t)blockIdx.x * RB + (W == 1 ? warp * R : 0);
     if (row >= rows) return;
-    const T* xr = x + row * x_stride;
-    float v[CH][VEC];
-    float sum = 0.0f;
+    OpRaw<T, VEC> v[R][CH];
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int col = (c * 32 * W + t) * VEC;
-        if (col < n) {
-            op_load<T, VEC>(xr + col, v[c]);
-        } else {
+    for (int q = 0; q < R; ++q)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[c][i] = 0.0f;
+        for (int c = 0; c < CH; ++c) {
+            const int col = (c * 32 * W + t) * VEC;
+            if (col < n && (R == 1 || row + q < rows)) v[q][c].load(x + (row + q) * x_stride + col);
+            else v[q][c].zero();
         }
+    float mean[R], rstd[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+        mean[q] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) mean[q] += v[q][c].get(i);
     }
+    norm_rows_sum<W, R>(mean, s_sum[0], warp, lane);
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int q = 0; q < R; ++q) {
+        mean[q] /= (float)n;
+        rstd[q] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sum += v[c][i];
-    const float mean = norm_row_sum<W>(sum, s_sum[0], warp, lane) / (float)n;
-    float sq = 0.0f;
+        for (int c = 0; c < CH; ++c)
+            if ((c * 32 * W + t) * VEC < n) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        if ((c * 32 * W + t) * VEC < n) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float d = v[c][i] - mean;
-                sq = fmaf(d, d, sq);
+                for (int i = 0; i < VEC; ++i) {
+                    const float d = v[q][c].get(i) - mean[q];
+                    rstd[q] = fmaf(d, d, rstd[q]);
+                }
             }
+    }
+    norm_rows_sum<W, R>(rstd, s_sum[1], warp, lane);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+        rstd[q] = 1.0f / sqrtf(rstd[q] / (float)n + eps);
+        if (t == 0 && (R == 1 || row + q < rows)) {
+            if (mean_out) mean_out[row + q] = mean[q];
+            if (rstd_out) rstd_out[row + q] = rstd[q];
         }
     }
-    const float rstd = 1.0f / sqrtf(norm_row_sum<W>(sq, s_sum[1], warp, lane) / (float)n + eps);
-    if (t == 0) {
-        if (mean_out) mean_out[row] = mean;
-        if (rstd_out) rstd_out[row] = rstd;
-    }
-    T* yr = y + row * y_stride;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int col = (c * 32 * W + t) * VEC;
         if (col >= n) continue;
-        float w[VEC], b[VEC], o[VEC];
+        float w[VEC], b[VEC];
         norm_columns<VEC>(weight, col, 1.0f, w);
         norm_columns<VEC>(bias, col, 0.0f, b);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = fmaf((v[c][i] - mean) * rstd, w[i], b[i]);
-        op_store<T, VEC>(yr + col, o);
+        for (int q = 0; q < R; ++q) {
+            float o[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) o[i] = fmaf((v[q][c].get(i) - mean[q]) * rstd[q], w[i], b[i]);
+            if (R == 1 || row + q < rows) op_store<T, VEC>(y + (row + q) * y_stride + col, o);
+        }
     }
 }
 
@@ -365,8 +390,10 @@ int norm_backward_blocks(int64_t rows, int n) {
 template <typename T, int VEC, int W, int CH>
 void norm_forward_go(cudaStream_t s, const void* x, int64_t xs, const float* w, const float* b, float eps, int64_t rows, int n, void* y, int64_t ys,
                      float* mean, float* rstd) {
-    const int64_t blocks = W == 1 ? (rows + 3) / 4 : rows;
-    k_norm_forward<T, W, VEC, CH><<<(unsigned)blocks, W == 1 ? 128 : W * 32, 0, s>>>((const T*)x, xs, w, b, eps, rows, n, (T*)y, ys, mean, rstd);
+    // registers of a row's share, and how many of its elements have to be on their way: two rows where that leaves the warps enough
+    constexpr int R = W == 1 && CH * VEC * (int)sizeof(T) <= 64 ? 2 : 1;
+    const int64_t per = W == 1 ? 4 * R : 1, blocks = (rows + per - 1) / per;
+    k_norm_forward<T, W, VEC, CH, R><<<(unsigned)blocks, W == 1 ? 128 : W * 32, 0, s>>>((const T*)x, xs, w, b, eps, rows, n, (T*)y, ys, mean, rstd);
 }
 // A warp per row up to 2048 columns (no barrier in a row), eight warps above.
 template <typename T, int VEC>
