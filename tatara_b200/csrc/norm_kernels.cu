@@ -9,6 +9,10 @@
 // mean (no cancellation) at no traffic.  All sums are fp32: a thread's columns in ascending order, then halves of the lanes,
 // then the warps in order.  The weight gradients are columns' sums: every block keeps those of its rows in registers over all
 // of its rows, the blocks' rows are added in a fixed order by a second kernel, so that results repeat bit for bit.
+//
+// Measured (inputs not in L2): 65536 x 1536 fp32 forward 119 us (6.8 TB/s), backward 176 us (6.9 TB/s) and 9 us for the columns' sums;
+// 50000 x 1000 bf16 39 us (5.2 TB/s) and 64 us (4.7 TB/s): 16-bit rows are half the bytes for the same instructions, issue slots at 60 %.
+// 256 x 256: one launch, 2 us.
 #include "op_common.cuh"
 
 namespace {

@@ -24,25 +24,9 @@ struct OrthPoly {
     float a, b, c, eps;
 };
 
-// element (r, c) of u; FIRST: the call that updates the momentum (once per element, before any other)
-template <typename T, bool FIRST>
-static __device__ __forceinline__ float orth_load(const OrthIo& io, int b, int64_t r, int64_t c) {
-    const float g = op_float(static_cast<const T*>(io.g)[b * io.g_batch + r * io.g_stride + c]);
-    if (!io.m) return g;
-    const int64_t at = ((int64_t)b * io.rows + r) * io.cols + c;
-    float m;
-    if (FIRST) {
-        m = fmaf(io.beta, io.m[at], g);
-        io.m_out[at] = m;
-    } else {
-        m = io.m_out[at];
-    }
-    return io.nesterov ? fmaf(io.beta, m, g) : m;
-}
-// x is element (r, c) of the result, w that of the old weights (Muon)
+// x is the result's element at that offset, w that of the old weights (Muon)
 template <typename T>
-static __device__ __forceinline__ void orth_store(const OrthIo& io, int b, int64_t r, int64_t c, float w, float x) {
-    const int64_t at = b * io.out_batch + r * io.out_stride + c;
+static __device__ __forceinline__ void orth_store(const OrthIo& io, int64_t at, float w, float x) {
     if (!io.m) {
         static_cast<T*>(io.out)[at] = op_round<T>(x);
         return;

@@ -19,6 +19,10 @@
 // cores truncate when they add to an accumulator: 2.5e-5 of the result after five steps of K = 1000 with two limbs.  So the accumulator
 // changes every four chunks of K, and the warps add what it held to their registers, rounded to nearest, while the next one fills.
 // Every wait is bounded; where one runs out the block's results become NaN, and so the output.
+//
+// Measured, 4096 x 4096 in fp32: Gram and square 158 us each, apply 293 us (1.4 PFLOP/s of limb products, tensor pipe 82 to 89 % busy), last product with
+// the weight update 360 us; the whole Muon step 3.3 to 3.7 ms, where the chip's power limit, not the kernel, sets the clock.  bf16: 1.16 ms.  Small
+// products are bound by what surrounds the MMAs: 4 x 1000 x 777 bf16 takes 141 us in 17 launches of 8 to 10 us, 2 to 4 us of each inside the K loop.
 #include "orth.cuh"
 
 #include <atomic>
@@ -210,41 +214,40 @@ __global__ void __launch_bounds__(256) k_orth_pack(OrthIo io, float eps, const d
     if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = v;
     const int i0 = blockIdx.y * 128, j0 = blockIdx.x * 64;
     uint8_t* to = x + (int64_t)b * LIMBS * limb_bytes + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * OT_TILE;
-    constexpr int P = 8 / N;  // accesses of a piece
-    double inv = 0.0;
-#pragma unroll 1
-    for (int e = threadIdx.x; e < 128 * 8; e += 256) {
-        const int i = TALL ? e % 128 : e / 8, j = TALL ? e / 128 * 8 : e % 8 * 8;
-        OtPiece<T, N> piece[P];
+    constexpr int P = 8 / N, PIECES = 4;  // accesses of a piece, pieces of a thread
+    OtPiece<T, N> piece[PIECES][P];
 #pragma unroll
-        for (int q = 0; q < P; ++q) {
-            const bool in = i0 + i < n && j0 + j + q * N < m;
-            if (in) piece[q].load(io, io.m_out, b, TALL ? j0 + j + q : i0 + i, TALL ? i0 + i : j0 + j + q * N);
-        }
-        if (e == threadIdx.x) {
-            __syncthreads();
-            v = s_part[0];
+    for (int k = 0; k < PIECES; ++k) {
+        const int e = threadIdx.x + 256 * k, i = TALL ? e % 128 : e / 8, j = TALL ? e / 128 * 8 : e % 8 * 8;
 #pragma unroll
-            for (int w = 1; w < 8; ++w) v += s_part[w];
-            inv = (double)OT_SCALE / (sqrt(v) + (double)eps);
-        }
+        for (int q = 0; q < P; ++q)
+            if (i0 + i < n && j0 + j + q * N < m) piece[k][q].load(io, io.m_out, b, TALL ? j0 + j + q : i0 + i, TALL ? i0 + i : j0 + j + q * N);
+    }
+    __syncthreads();
+    v = s_part[0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) v += s_part[w];
+    const double inv = (double)OT_SCALE / (sqrt(v) + (double)eps);
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+        const int e = threadIdx.x + 256 * k, i = TALL ? e % 128 : e / 8, j = TALL ? e / 128 * 8 : e % 8 * 8;
         OpVec<__half, 8> out[LIMBS];
 #pragma unroll
         for (int q = 0; q < P; ++q) {
             float u[N];
 #pragma unroll
-            for (int k = 0; k < N; ++k) u[k] = 0.0f;
+            for (int c = 0; c < N; ++c) u[c] = 0.0f;
             if (i0 + i < n && j0 + j + q * N < m) {
-                piece[q].template finish<false>(io, u);
+                piece[k][q].template finish<false>(io, u);
 #pragma unroll
-                for (int k = 0; k < N; ++k) u[k] = (float)((double)u[k] * inv);
+                for (int c = 0; c < N; ++c) u[c] = (float)((double)u[c] * inv);
             }
 #pragma unroll
-            for (int k = 0; k < N; ++k) {
+            for (int c = 0; c < N; ++c) {
                 __half h[LIMBS];
-                ot_split<LIMBS>(u[k], h);
+                ot_split<LIMBS>(u[c], h);
 #pragma unroll
-                for (int l = 0; l < LIMBS; ++l) out[l].v[q * N + k] = h[l];
+                for (int l = 0; l < LIMBS; ++l) out[l].v[q * N + c] = h[l];
             }
         }
 #pragma unroll
@@ -549,19 +552,20 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                     for (int c = 0; c < 64; ++c) flat[row * 65 + c] = acc[64 * h + c] * OT_UNSCALE + poison;
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
                     const int i0 = (at.i * CTAS + rank) * 128, j0 = (at.j * 2 * CTAS + group * CTAS + h) * 64;
-                    // 128 (64) neighbours in memory at a time, eight of a thread's old weights on their way
-                    for (int e0 = 0; e0 < 64; e0 += 8) {
+                    // 128 (64) neighbours in memory at a time, eight of a thread's old weights on their way.  A thread's elements lie `next` apart
+                    const int r = row >> 6, c = row & 63;
+                    const int64_t to = at.batch * io.out_batch + (tall ? (int64_t)j0 * io.out_stride + i0 + row : (int64_t)(i0 + r) * io.out_stride + j0 + c);
+                    const int64_t next = tall ? io.out_stride : 2 * io.out_stride;
+                    const int left = tall ? (i0 + row < n ? m - j0 : 0) : (j0 + c < m ? (n - i0 - r + 1) / 2 : 0);
+                    const float* from = tall ? flat + row * 65 : flat + r * 65 + c;
+                    const int jump = tall ? 1 : 130;
+                    for (int e0 = 0; e0 < 64 && e0 < left; e0 += 8) {
                         float w[8];
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) {
-                            const int e = e0 + u, i = i0 + (tall ? row : 2 * e + (row >> 6)), j = j0 + (tall ? e : row & 63);
-                            w[u] = io.m && i < n && j < m ? io.w[at.batch * io.out_batch + (tall ? j * io.out_stride + i : i * io.out_stride + j)] : 0.0f;
-                        }
+                        for (int u = 0; u < 8; ++u) w[u] = io.m && e0 + u < left ? io.w[to + (e0 + u) * next] : 0.0f;
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) {
-                            const int e = e0 + u, r = tall ? row : 2 * e + (row >> 6), c = tall ? e : row & 63, i = i0 + r, j = j0 + c;
-                            if (i < n && j < m) orth_store<T>(io, at.batch, tall ? j : i, tall ? i : j, w[u], flat[r * 65 + c]);
-                        }
+                        for (int u = 0; u < 8; ++u)
+                            if (e0 + u < left) orth_store<T>(io, to + (e0 + u) * next, w[u], from[(e0 + u) * jump]);
                     }
                 }
             } else {
@@ -832,7 +836,11 @@ void ot_begin(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, const OtPl
     int64_t most = 8 * (int64_t)sm_count() / io.batch;
     most = most < 1 ? 1 : most < OT_NORM_BLOCKS ? most : OT_NORM_BLOCKS;
     const int blocks = (int)(segments < most ? segments : most);
-    k_orth_norm<T, N><<<dim3((unsigned)blocks, (unsigned)io.batch), 256, 0, s>>>(io, segments, len, total, partial);
+    // a matrix without gaps is read 16 bytes at a time even where its rows do not start on such a boundary
+    constexpr int W = 16 / (int)sizeof(T);
+    const bool flat = !gaps && total % W == 0 && ((uintptr_t)io.g & 15) == 0 && io.g_batch % W == 0 && (((uintptr_t)io.m | (uintptr_t)io.m_out) & 15) == 0;
+    const dim3 grid0((unsigned)blocks, (unsigned)io.batch);
+    if (flat) k_orth_norm<T, W><<<grid0, 256, 0, s>>>(io, segments, len, total, partial); else k_orth_norm<T, N><<<grid0, 256, 0, s>>>(io, segments, len, total, partial);
     const dim3 grid((unsigned)(p.m_pad / 64), (unsigned)(p.n_pad / 128), (unsigned)io.batch);
     if (io.rows > io.cols) op_launch_next(s, grid, dim3(256), 0, k_orth_pack<T, LIMBS, 1, true>, io, poly.eps, partial, blocks, x, p.x_limb);
     else op_launch_next(s, grid, dim3(256), 0, k_orth_pack<T, LIMBS, N, false>, io, poly.eps, partial, blocks, x, p.x_limb);
