@@ -16,8 +16,9 @@
 // a I is part of Q, so that no product has to add its own input.
 //
 // One thread issues the bulk copies into a ring of stages, one the MMAs, eight warps read the accumulators from tensor memory.  The tensor
-// cores truncate when they add to an accumulator: 2.5e-5 of the result after five steps of K = 1000 with two limbs.  So the accumulator
-// changes every four chunks of K, and the warps add what it held to their registers, rounded to nearest, while the next one fills.
+// cores truncate when they add to an accumulator: with two limbs that left 2.5e-5 of the result after five steps of K = 1000, 1.4e-5 with a new accumulator
+// every 256 columns of K.  So it changes with every chunk of 64, which adds the small products first and the four large ones last, and the
+// warps add what it held to their registers, rounded to nearest, while the next one fills.
 // Every wait is bounded; where one runs out the block's results become NaN, and so the output.
 //
 // Measured, 4096 x 4096 in fp32: Gram and square 158 us each, apply 293 us (1.4 PFLOP/s of limb products, tensor pipe 82 to 89 % busy), last product with
@@ -282,8 +283,8 @@ struct OtShape {
     static constexpr int STAGE = LIMBS * 2 * OT_TILE;
     static constexpr int STAGES = LIMBS == 2 ? 3 : 6;
     static constexpr int SMEM = STAGE * STAGES + 1024;
-    // chunks of 64 whose products share an accumulator
-    static constexpr int DRAIN = LIMBS == 2 ? 4 : 1 << 30;
+    // chunks of 64 whose products share an accumulator (two limbs: four instead of one are 4 to 9 % faster and three times as far off)
+    static constexpr int DRAIN = LIMBS == 2 ? 1 : 1 << 30;
 };
 
 // a tile's place: of a symmetric result those on and below the diagonal, row by row
@@ -470,10 +471,10 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                         if (leader) {
                             const unsigned long long da = da0 + s * (S::STAGE / 16), db = db0 + s * (S::STAGE / 16);
 #pragma unroll
-                            for (int q = 0; q < (LIMBS == 2 ? 3 : 1); ++q)
+                            for (int q = 0; q < (LIMBS == 2 ? 3 : 1); ++q)  // high low, low high, high high: the large terms last
 #pragma unroll
                                 for (int j = 0; j < 4; ++j)
-                                    ot_mma<CTAS>(d, da + (q == 2 ? OT_TILE / 16 : 0) + STEP_A * j, db + (q == 1 ? OT_TILE / 16 : 0) + STEP_B * j, IDESC,
+                                    ot_mma<CTAS>(d, da + (LIMBS == 2 && q == 1 ? OT_TILE / 16 : 0) + STEP_A * j, db + (LIMBS == 2 && q == 0 ? OT_TILE / 16 : 0) + STEP_B * j, IDESC,
                                                  q > 0 || j > 0 ? 1u : accumulate);
                             ot_commit<CTAS>(ot_smem(&s_empty[0]) + 8 * s);
                         }
