@@ -33,15 +33,15 @@ __device__ __forceinline__ float norm_row_sum(float v, float* buf, int warp_in_r
     return v;
 }
 
-// the same of R rows of a warp (R = 1 with several warps per row), in place
-template <int W, int R>
+// the same of R rows of L lanes (R = 1 with several warps per row), in place
+template <int W, int L, int R>
 __device__ __forceinline__ void norm_rows_sum(float (&v)[R], float* buf, int warp_in_row, int lane) {
     if (W > 1) {
         v[0] = norm_row_sum<W>(v[0], buf, warp_in_row, lane);
         return;
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
+    for (int o = L / 2; o > 0; o >>= 1)
 #pragma unroll
         for (int q = 0; q < R; ++q) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
 }
@@ -62,24 +62,25 @@ __device__ __forceinline__ void norm_columns(const float* __restrict__ p, int co
     }
 }
 
-// W warps per row, VEC adjacent columns per access, CH accesses per thread: a thread holds columns (c * 32 W + t) * VEC + i.  A warp of its own (W = 1) takes R
-// rows at once, which share its reads of weight and bias.
-template <typename T, int W, int VEC, int CH, int R>
+// W warps per row, VEC adjacent columns per access, CH accesses per thread: a thread holds columns (c * LANES + t) * VEC + i.  With W = 1 a row has L lanes
+// (8 for rows of up to 64 columns, or most lanes of a warp idle: 33615 x 9 fp32), which take R rows at once: those share the reads of weight and bias.
+template <typename T, int W, int L, int VEC, int CH, int R>
 __global__ void __launch_bounds__(W == 1 ? 128 : W * 32)
 k_norm_forward(const T* x, int64_t x_stride, const float* __restrict__ weight, const float* __restrict__ bias, float eps,
                int64_t rows, int n, T* y, int64_t y_stride, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-    constexpr int RB = W == 1 ? 4 * R : 1;  // rows per block
+    constexpr int LANES = W == 1 ? L : 32 * W, SUBS = W == 1 ? 32 / L : 1, RB = W == 1 ? 4 * SUBS * R : 1;  // rows per block
     __shared__ float s_sum[2][W];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = W == 1 ? lane : threadIdx.x;
-    const int64_t row = (int64_t)blockIdx.x * RB + (W == 1 ? warp * R : 0);
-    if (row >= rows) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = W == 1 ? lane % L : threadIdx.x;
+    const int64_t row = (int64_t)blockIdx.x * RB + (W == 1 ? (warp * SUBS + lane / L) * R : 0);
+    if (L == 32 && row >= rows) return;  // by whole warps; lanes that share a warp stay for its sums
+    constexpr bool ALL = R == 1 && L == 32;
     OpRaw<T, VEC> v[R][CH];
 #pragma unroll
     for (int q = 0; q < R; ++q)
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int col = (c * 32 * W + t) * VEC;
-            if (col < n && (R == 1 || row + q < rows)) v[q][c].load(x + (row + q) * x_stride + col);
+            const int col = (c * LANES + t) * VEC;
+            if (col < n && (ALL || row + q < rows)) v[q][c].load(x + (row + q) * x_stride + col);
             else v[q][c].zero();
         }
     float mean[R], rstd[R];
@@ -91,14 +92,14 @@ k_norm_forward(const T* x, int64_t x_stride, const float* __restrict__ weight, c
 #pragma unroll
             for (int i = 0; i < VEC; ++i) mean[q] += v[q][c].get(i);
     }
-    norm_rows_sum<W, R>(mean, s_sum[0], warp, lane);
+    norm_rows_sum<W, L, R>(mean, s_sum[0], warp, lane);
 #pragma unroll
     for (int q = 0; q < R; ++q) {
         mean[q] /= (float)n;
         rstd[q] = 0.0f;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
-            if ((c * 32 * W + t) * VEC < n) {
+            if ((c * LANES + t) * VEC < n) {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
                     const float d = v[q][c].get(i) - mean[q];
@@ -106,18 +107,18 @@ k_norm_forward(const T* x, int64_t x_stride, const float* __restrict__ weight, c
                 }
             }
     }
-    norm_rows_sum<W, R>(rstd, s_sum[1], warp, lane);
+    norm_rows_sum<W, L, R>(rstd, s_sum[1], warp, lane);
 #pragma unroll
     for (int q = 0; q < R; ++q) {
         rstd[q] = 1.0f / sqrtf(rstd[q] / (float)n + eps);
-        if (t == 0 && (R == 1 || row + q < rows)) {
+        if (t == 0 && (ALL || row + q < rows)) {
             if (mean_out) mean_out[row + q] = mean[q];
             if (rstd_out) rstd_out[row + q] = rstd[q];
         }
     }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int col = (c * 32 * W + t) * VEC;
+        const int col = (c * LANES + t) * VEC;
         if (col >= n) continue;
         float w[VEC], b[VEC];
         norm_columns<VEC>(weight, col, 1.0f, w);
@@ -127,7 +128,7 @@ k_norm_forward(const T* x, int64_t x_stride, const float* __restrict__ weight, c
             float o[VEC];
 #pragma unroll
             for (int i = 0; i < VEC; ++i) o[i] = fmaf((v[q][c].get(i) - mean[q]) * rstd[q], w[i], b[i]);
-            if (R == 1 || row + q < rows) op_store<T, VEC>(y + (row + q) * y_stride + col, o);
+            if (ALL || row + q < rows) op_store<T, VEC>(y + (row + q) * y_stride + col, o);
         }
     }
 }
@@ -165,21 +166,21 @@ constexpr int norm_backward_per_sm(int warps) {
     return 24 / w < 1 ? 1 : 24 / w;
 }
 
-// Backward: a block of W warps per row (W = 1: four rows side by side, a warp each) takes R rows at a time, which shares one barrier, walks
+// Backward: a block of W warps per row (W = 1: rows side by side, L lanes each) takes R rows at a time, which shares one barrier, walks
 // down the rows and keeps its columns' weight and bias gradients in registers; partial: [2][blocks][n].
 // fp32, 65536 x 1536: 175 us, 6.9 TB/s.
-template <typename T, int W, int VEC, int CH, int R>
+template <typename T, int W, int L, int VEC, int CH, int R>
 __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, norm_backward_per_sm(W))
 k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, const float* __restrict__ mean,
                 const float* __restrict__ rstd, const float* __restrict__ weight, int64_t rows, int n, T* dx, int64_t dx_stride,
                 float* __restrict__ partial) {
-    constexpr int RB = W == 1 ? 4 : 1;
+    constexpr int LANES = W == 1 ? L : 32 * W, SUBS = W == 1 ? 32 / L : 1, RB = W == 1 ? 4 * SUBS : 1;
     __shared__ float s_sum[2][2 * R][W];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = W == 1 ? lane : threadIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = W == 1 ? lane % L : threadIdx.x;
     float w[CH][VEC], aw[CH][VEC], ab[CH][VEC];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int col = (c * 32 * W + t) * VEC;
+        const int col = (c * LANES + t) * VEC;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) w[c][i] = aw[c][i] = ab[c][i] = 0.0f;
         if (col < n) norm_columns<VEC>(weight, col, 1.0f, w[c]);
@@ -187,7 +188,9 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
     const float inv_n = 1.0f / (float)n;
     int turn = 0;
     op_next_may_start();
-    for (int64_t first = ((int64_t)blockIdx.x * RB + (W == 1 ? warp : 0)) * R; first < rows; first += (int64_t)gridDim.x * RB * R, turn ^= 1) {
+    // the lanes of a warp take the same number of turns
+    for (int64_t turn0 = ((int64_t)blockIdx.x * RB + (W == 1 ? warp * SUBS : 0)) * R; turn0 < rows; turn0 += (int64_t)gridDim.x * RB * R, turn ^= 1) {
+        const int64_t first = turn0 + (SUBS > 1 ? lane / L * R : 0);
         OpRaw<T, VEC> xv[R][CH], gv[R][CH];
         float mu[R], r[R], s1[R], s2[R];
 #pragma unroll
@@ -195,7 +198,7 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
             const bool in = first + q < rows;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                const int col = (c * 32 * W + t) * VEC;
+                const int col = (c * LANES + t) * VEC;
                 if (in && col < n) {
                     xv[q][c].load(x + (first + q) * x_stride + col);
                     gv[q][c].load(dy + (first + q) * dy_stride + col);
@@ -223,7 +226,7 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
                 }
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
+        for (int o = L / 2; o > 0; o >>= 1)
 #pragma unroll
             for (int q = 0; q < R; ++q) {
                 s1[q] += __shfl_xor_sync(0xffffffffu, s1[q], o);
@@ -255,7 +258,7 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
             if (first + q < rows)
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
-                    const int col = (c * 32 * W + t) * VEC;
+                    const int col = (c * LANES + t) * VEC;
                     if (col < n) {
                         float o[VEC];
 #pragma unroll
@@ -269,6 +272,16 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
         }
     }
     if (!partial) return;
+    if (SUBS > 1)  // the rows of a warp, in halves
+#pragma unroll
+        for (int o = 16; o >= L; o >>= 1)
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    aw[c][i] += __shfl_xor_sync(0xffffffffu, aw[c][i], o);
+                    ab[c][i] += __shfl_xor_sync(0xffffffffu, ab[c][i], o);
+                }
     if (W == 1) {  // the four warps' sums, in order
         __shared__ float s_acc[3][2][32 * CH * VEC];
         if (warp > 0)
@@ -293,8 +306,8 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
     }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int col = (c * 32 * W + t) * VEC;
-        if (col < n) {  // n is a multiple of VEC
+        const int col = (c * LANES + t) * VEC;
+        if (col < n && (SUBS == 1 || lane < L)) {  // n is a multiple of VEC
             op_store<float, VEC>(partial + (int64_t)blockIdx.x * n + col, aw[c]);
             op_store<float, VEC>(partial + ((int64_t)gridDim.x + blockIdx.x) * n + col, ab[c]);
         }
@@ -380,33 +393,33 @@ NormShape norm_backward_shape(int n) {
         if (n <= w * 256) return {w, 8};
     return {16, 16};
 }
-// Blocks: at most what runs at once; 16 rows (W = 1: 64) or more for each, or the blocks' rows of gradients cost as much as the rows themselves, but
+// Blocks: at most what runs at once; 16 rows or more for each, or the blocks' rows of gradients cost as much as the rows themselves, but
 // one per SM as far as the rows go (256 rows of 256: 4 blocks took 12 us).
 int norm_backward_blocks(int64_t rows, int n) {
     if (n > NORM_REG_N_BACK) return (int)(rows < 64 ? (rows < 1 ? 1 : rows) : 64);
     const int w = norm_backward_shape(n).warps;
-    const int64_t turn = w == 1 ? 8 : 2, sms = sm_count(), most = sms * norm_backward_per_sm(w);
-    const int64_t turns = (rows + turn - 1) / turn, want = (turns + 7) / 8;
+    const int64_t turn = n <= 64 ? 32 : w == 1 ? 8 : 2, sms = sm_count(), most = sms * norm_backward_per_sm(w);
+    const int64_t turns = (rows + turn - 1) / turn, least = (16 + turn - 1) / turn, want = (turns + least - 1) / least;
     const int64_t few = turns < sms ? turns : sms, blocks = want < few ? few : want < most ? want : most;
     return (int)(blocks < 1 ? 1 : blocks);
 }
 
-template <typename T, int VEC, int W, int CH>
+template <typename T, int VEC, int W, int L, int CH>
 void norm_forward_go(cudaStream_t s, const void* x, int64_t xs, const float* w, const float* b, float eps, int64_t rows, int n, void* y, int64_t ys,
                      float* mean, float* rstd) {
     // registers of a row's share, and how many of its elements have to be on their way: two rows where that leaves the warps enough
     constexpr int R = W == 1 && CH * VEC * (int)sizeof(T) <= 64 ? 2 : 1;
-    const int64_t per = W == 1 ? 4 * R : 1, blocks = (rows + per - 1) / per;
-    k_norm_forward<T, W, VEC, CH, R><<<(unsigned)blocks, W == 1 ? 128 : W * 32, 0, s>>>((const T*)x, xs, w, b, eps, rows, n, (T*)y, ys, mean, rstd);
+    const int64_t per = W == 1 ? 128 / L * R : 1, blocks = (rows + per - 1) / per;
+    k_norm_forward<T, W, L, VEC, CH, R><<<(unsigned)blocks, W == 1 ? 128 : W * 32, 0, s>>>((const T*)x, xs, w, b, eps, rows, n, (T*)y, ys, mean, rstd);
 }
-// A warp per row up to 2048 columns (no barrier in a row), eight warps above.
+// Eight lanes per row up to 64 columns, a warp up to 2048 (no barrier in a row), eight warps above.
 template <typename T, int VEC>
 void norm_forward_pick(cudaStream_t s, const void* x, int64_t xs, const float* w, const float* b, float eps, int64_t rows, int n, void* y, int64_t ys,
                        float* mean, float* rstd) {
-#define GO(W, K) \
-    if (n <= (W) * (K) * 32) return norm_forward_go<T, VEC, W, ((K) + VEC - 1) / VEC>(s, x, xs, w, b, eps, rows, n, y, ys, mean, rstd)
-    GO(1, 8); GO(1, 16); GO(1, 24); GO(1, 32); GO(1, 48); GO(1, 64);
-    GO(8, 16); GO(8, 32); GO(16, 32);
+#define GO(W, L, K) \
+    if (n <= (W) * (K) * (L)) return norm_forward_go<T, VEC, W, L, ((K) + VEC - 1) / VEC>(s, x, xs, w, b, eps, rows, n, y, ys, mean, rstd)
+    GO(1, 8, 8); GO(1, 32, 8); GO(1, 32, 16); GO(1, 32, 24); GO(1, 32, 32); GO(1, 32, 48); GO(1, 32, 64);
+    GO(8, 32, 16); GO(8, 32, 32); GO(16, 32, 32);
 #undef GO
     k_norm_forward_long<T><<<(unsigned)rows, 1024, 0, s>>>((const T*)x, xs, w, b, eps, n, (T*)y, ys, mean, rstd);
 }
@@ -416,19 +429,21 @@ void norm_backward_pick(cudaStream_t s, const void* dy, int64_t dys, const void*
                         int64_t rows, int n, void* dx, int64_t dxs, float* partial, int blocks) {
     if (n <= NORM_REG_N_BACK) {
         const NormShape shape = norm_backward_shape(n);
-#define GO(W, K, R)                                                                                                                           \
-    k_norm_backward<T, W, VEC, (K) / VEC, R><<<(unsigned)blocks, W == 1 ? 128 : W * 32, 0, s>>>((const T*)dy, dys, (const T*)x, xs, mean, rstd, \
+#define GO(W, L, K, R)                                                                                                                        \
+    k_norm_backward<T, W, L, VEC, (K) / VEC, R><<<(unsigned)blocks, W == 1 ? 128 : W * 32, 0, s>>>((const T*)dy, dys, (const T*)x, xs, mean, rstd, \
                                                                                                w, rows, n, (T*)dx, dxs, partial)
         switch (shape.warps) {
-            case 1: GO(1, 8, 2); break;
-            case 2: GO(2, 8, 2); break;
-            case 3: GO(3, 8, 2); break;
-            case 4: GO(4, 8, 2); break;
-            case 6: GO(6, 8, 2); break;
-            case 8: GO(8, 8, 2); break;
-            case 12: GO(12, 8, 2); break;
+            case 1:
+                if (n <= 64) GO(1, 8, 8, 2); else GO(1, 32, 8, 2);
+                break;
+            case 2: GO(2, 32, 8, 2); break;
+            case 3: GO(3, 32, 8, 2); break;
+            case 4: GO(4, 32, 8, 2); break;
+            case 6: GO(6, 32, 8, 2); break;
+            case 8: GO(8, 32, 8, 2); break;
+            case 12: GO(12, 32, 8, 2); break;
             default:
-                if (shape.columns == 8) GO(16, 8, 2); else GO(16, 16, 1);
+                if (shape.columns == 8) GO(16, 32, 8, 2); else GO(16, 32, 16, 1);
         }
 #undef GO
         return;
