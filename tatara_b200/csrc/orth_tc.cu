@@ -535,12 +535,15 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                 buffer ^= 1;
             }
             if (!ok && lane == 0) atomicExch(&s_failed, 1);
-            const float poison = !ok || *static_cast<volatile int*>(&s_failed) ? __int_as_float(0x7fc00000) : 0.0f;
+            if (!ok || *static_cast<volatile int*>(&s_failed)) {
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) acc[c] = __int_as_float(0x7fc00000);
+            }
 
             if (KIND == OT_GRAM_PART) {
                 float4* to = reinterpret_cast<float4*>(g.part) + ((int64_t)t * gridDim.y + blockIdx.y) * 4096 + row;
 #pragma unroll
-                for (int c = 0; c < COLS; c += 4) to[(group * COLS + c) / 4 * 128] = make_float4(acc[c] + poison, acc[c + 1] + poison, acc[c + 2] + poison, acc[c + 3] + poison);
+                for (int c = 0; c < COLS; c += 4) to[(group * COLS + c) / 4 * 128] = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
             } else if (KIND == OT_LAST) {
                 // by rounds of 64 columns through shared memory (a block has one tile, its ring is free by now)
                 float* flat = reinterpret_cast<float*>(s_dyn + group * 40960);  // [128][65]
@@ -550,7 +553,7 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                 for (int h = 0; h < CTAS; ++h) {
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) flat[row * 65 + c] = acc[64 * h + c] * OT_UNSCALE + poison;
+                    for (int c = 0; c < 64; ++c) flat[row * 65 + c] = acc[64 * h + c] * OT_UNSCALE;
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
                     const int i0 = (at.i * CTAS + rank) * 128, j0 = (at.j * 2 * CTAS + group * CTAS + h) * 64;
                     // 128 (64) neighbours in memory at a time, eight of a thread's old weights on their way.  A thread's elements lie `next` apart
@@ -579,6 +582,7 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                 constexpr int IMAGES = (SYM ? 2 : 1) * LIMBS * OT_TILE;
                 constexpr bool APART = 2 * CTAS * IMAGES <= S::STAGE * S::STAGES;
                 const int swap = row & 1;  // of a sector's two pieces
+                const float square = g.cc * (OT_UNSCALE * OT_SCALE);
 #pragma unroll
                 for (int h = 0; h < CTAS; ++h) {
                     const int col_tile = at.j * 2 * CTAS + group * CTAS + h;  // the round's columns, in 64s
@@ -591,51 +595,48 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                     const uint8_t* old = g.a + (int64_t)at.batch * LIMBS * g.a_limb + ((int64_t)row_tile * g.a_width + col_tile) * OT_TILE + row * 128;
                     const int ident = row_tile * 128 + row - col_tile * 64;  // the diagonal's column
                     if (h && staged && !APART) asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
-                    OtSector before[LIMBS];
+                    OtSector before[LIMBS];  // square: A, a sector ahead
                     if (KIND == OT_SQUARE)
 #pragma unroll
                         for (int l = 0; l < LIMBS; ++l) before[l].load(old + l * g.a_limb + ((row & 6) << 4));
 #pragma unroll
                     for (int c0 = 0; c0 < 64; c0 += 16) {
-                        float x[16];
+                        float x[16];  // scaled as it is stored
 #pragma unroll
-                        for (int c = 0; c < 16; ++c) x[c] = acc[64 * h + c0 + c] * OT_UNSCALE + poison;
+                        for (int c = 0; c < 16; ++c) x[c] = acc[64 * h + c0 + c] * (KIND == OT_SQUARE ? square : OT_UNSCALE * OT_SCALE);
                         if (KIND == OT_SQUARE) {
-                            float a[16];
 #pragma unroll
-                            for (int l = 0; l < LIMBS; ++l) before[l].exchange(swap);
+                            for (int l = LIMBS - 1; l >= 0; --l) {
+                                before[l].exchange(swap);
 #pragma unroll
-                            for (int l = 0; l < LIMBS; ++l)
+                                for (int c = 0; c < 16; ++c) x[c] = fmaf(g.cb, before[l].get(c), x[c]);
+                                if (c0 < 48) before[l].load(old + l * g.a_limb + ((((c0 + 16) >> 3) ^ (row & 6)) << 4));
+                            }
+                            if (same)  // the diagonal passes through these tiles alone
 #pragma unroll
-                                for (int c = 0; c < 16; ++c) {
-                                    const float v = before[l].get(c);
-                                    a[c] = l ? a[c] + v : v;
-                                }
-                            if (c0 < 48)
-#pragma unroll
-                                for (int l = 0; l < LIMBS; ++l) before[l].load(old + l * g.a_limb + ((((c0 + 16) >> 3) ^ (row & 6)) << 4));
-#pragma unroll
-                            for (int c = 0; c < 16; ++c) x[c] = fmaf(g.cc, x[c], fmaf(g.cb / OT_SCALE, a[c], ident == c0 + c ? g.ca : 0.0f));
+                                for (int c = 0; c < 16; ++c) x[c] += ident == c0 + c ? g.ca * OT_SCALE : 0.0f;
                         }
                         OtSector piece[LIMBS];
 #pragma unroll
                         for (int c = 0; c < 16; c += 2) {
-                            __half u[LIMBS], v[LIMBS];
-                            ot_split<LIMBS>(x[c] * OT_SCALE, u);
-                            ot_split<LIMBS>(x[c + 1] * OT_SCALE, v);
+                            __half2 pair[LIMBS];
+                            pair[0] = __floats2half2_rn(x[c], x[c + 1]);
+                            if (LIMBS == 2) {
+                                const float2 high = __half22float2(pair[0]);
+                                pair[LIMBS - 1] = __floats2half2_rn(x[c] - high.x, x[c + 1] - high.y);
+                            }
 #pragma unroll
                             for (int l = 0; l < LIMBS; ++l) {
-                                const __half2 pair = __halves2half2(u[l], v[l]);
-                                piece[l].w[c / 2] = *reinterpret_cast<const unsigned*>(&pair);
+                                piece[l].w[c / 2] = *reinterpret_cast<const unsigned*>(&pair[l]);
                                 if (SYM && !same) {
                                     uint8_t* to = mirror + (staged ? l * OT_TILE : l * g.out_limb) + (c0 + c) * 128;
                                     const int slot = (row & 63) >> 3;
                                     if (staged) {  // not left to the compiler: a generic store costs as much as a global one
-                                        ot_store_shared(to + (((slot ^ (c0 + c)) & 7) << 4), u[l]);
-                                        ot_store_shared(to + 128 + (((slot ^ (c0 + c + 1)) & 7) << 4), v[l]);
+                                        ot_store_shared(to + (((slot ^ (c0 + c)) & 7) << 4), __low2half(pair[l]));
+                                        ot_store_shared(to + 128 + (((slot ^ (c0 + c + 1)) & 7) << 4), __high2half(pair[l]));
                                     } else {
-                                        *reinterpret_cast<__half*>(to + (((slot ^ (c0 + c)) & 7) << 4)) = u[l];
-                                        *reinterpret_cast<__half*>(to + 128 + (((slot ^ (c0 + c + 1)) & 7) << 4)) = v[l];
+                                        *reinterpret_cast<__half*>(to + (((slot ^ (c0 + c)) & 7) << 4)) = __low2half(pair[l]);
+                                        *reinterpret_cast<__half*>(to + 128 + (((slot ^ (c0 + c + 1)) & 7) << 4)) = __high2half(pair[l]);
                                     }
                                 }
                             }
