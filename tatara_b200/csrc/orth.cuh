@@ -24,6 +24,12 @@ struct OrthPoly {
     float a, b, c, eps;
 };
 
+// the new weight: w the old one, x the orthogonalised update
+static __device__ __forceinline__ float orth_update(const OrthIo& io, float w, float x) {
+    w = fmaf(-io.step, x, w * io.w_mul);
+    w = w < -io.clip ? -io.clip : w;  // comparisons keep a NaN
+    return w > io.clip ? io.clip : w;
+}
 // x is the result's element at that offset, w that of the old weights (Muon)
 template <typename T>
 static __device__ __forceinline__ void orth_store(const OrthIo& io, int64_t at, float w, float x) {
@@ -31,10 +37,7 @@ static __device__ __forceinline__ void orth_store(const OrthIo& io, int64_t at, 
         static_cast<T*>(io.out)[at] = op_round<T>(x);
         return;
     }
-    w = fmaf(-io.step, x, w * io.w_mul);
-    w = w < -io.clip ? -io.clip : w;  // comparisons keep a NaN
-    w = w > io.clip ? io.clip : w;
-    static_cast<float*>(io.out)[at] = w;
+    static_cast<float*>(io.out)[at] = orth_update(io, w, x);
 }
 
 // orth_kernels.cu: n <= ORTH_SMALL_N

@@ -544,8 +544,41 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                 float4* to = reinterpret_cast<float4*>(g.part) + ((int64_t)t * gridDim.y + blockIdx.y) * 4096 + row;
 #pragma unroll
                 for (int c = 0; c < COLS; c += 4) to[(group * COLS + c) / 4 * 128] = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+            } else if (KIND == OT_LAST && MULTI) {
+                // rows on 16-byte boundaries go out straight from the registers, eight elements at a time
+                const int i = (at.i * CTAS + rank) * 128 + row, j0 = (at.j * 2 + group) * COLS;
+                const int64_t to = at.batch * io.out_batch + i * io.out_stride + j0;
+                if (i < io.rows)
+#pragma unroll
+                    for (int c0 = 0; c0 < COLS; c0 += 8) {
+                        if (j0 + c0 >= io.cols) break;  // a multiple of eight
+                        float x[8];
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) x[c] = acc[c0 + c] * OT_UNSCALE;
+                        if (io.m) {
+                            float w[2][4];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) op_load<float, 4>(io.w + to + c0 + 4 * h, w[h]);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                float q[4];
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) q[c] = orth_update(io, w[h][c], x[4 * h + c]);
+                                op_store<float, 4>(static_cast<float*>(io.out) + to + c0 + 4 * h, q);
+                            }
+                        } else {
+                            constexpr int STEP = 16 / (int)sizeof(T);
+#pragma unroll
+                            for (int h = 0; h < 8; h += STEP) {
+                                float q[STEP];
+#pragma unroll
+                                for (int c = 0; c < STEP; ++c) q[c] = x[h + c];
+                                op_store<T, STEP>(static_cast<T*>(io.out) + to + c0 + h, q);
+                            }
+                        }
+                    }
             } else if (KIND == OT_LAST) {
-                // by rounds of 64 columns through shared memory (a block has one tile, its ring is free by now)
+                // rows that start anywhere, or are columns: by rounds of 64 columns through shared memory (a block has one tile, its ring is free by now)
                 float* flat = reinterpret_cast<float*>(s_dyn + group * 40960);  // [128][65]
                 const bool tall = io.rows > io.cols;
                 const int n = tall ? io.cols : io.rows, m = tall ? io.rows : io.cols;
@@ -795,8 +828,12 @@ template <int KIND, int LIMBS, int CTAS, typename T>
 void ot_gemm(cudaStream_t s, const OtGemm& g, const OrthIo& io, int parts = 1) {
     const int64_t tiles = KIND == OT_APPLY || KIND == OT_LAST ? (int64_t)g.row_tiles * g.col_tiles : (int64_t)g.row_tiles * (g.row_tiles + 1) / 2;
     const int64_t all = tiles * io.batch, slots = sm_count() / CTAS;
-    if constexpr (KIND != OT_LAST && KIND != OT_GRAM_PART)
+    if constexpr (KIND == OT_LAST) {  // MULTI: the result can be stored straight from the registers
+        const bool aligned = io.cols % 8 == 0 && io.out_stride % 8 == 0 && io.out_batch % 8 == 0 && (((uintptr_t)io.out | (uintptr_t)io.w) & 15) == 0;
+        if (io.rows <= io.cols && aligned) return ot_launch<KIND, LIMBS, CTAS, true, T>(s, g, io, all > slots ? slots : all, parts);
+    } else if constexpr (KIND != OT_GRAM_PART) {
         if (all > slots) return ot_launch<KIND, LIMBS, CTAS, true, T>(s, g, io, slots, parts);
+    }
     ot_launch<KIND, LIMBS, CTAS, false, T>(s, g, io, all, parts);
 }
 
