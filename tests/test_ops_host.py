@@ -1,0 +1,128 @@
+"""The operators' entry points without a GPU: refused arguments come back as codes and texts before anything is launched, accepted ones as
+"no device" where there is none; workspace sizes; the torch binding refuses host tensors."""
+import ctypes as C
+import math
+
+import pytest
+
+import tatara_b200 as tb
+from tatara_b200 import _lib as L
+
+INVALID, NO_DEVICE = -1, -6
+P = 0x10000  # an address that is never read: arguments are refused, or the launch fails, before it could be
+
+
+def lib():
+    return tb.load_library()
+
+
+def err():
+    return C.create_string_buffer(200)
+
+
+def no_gpu():
+    return lib().tb_device_count() <= 0
+
+
+def muon(**kw):
+    v = dict(struct_size=C.sizeof(L.Muon), steps=5, nesterov=1, a=3.4445, b=-4.775, c=2.0315, eps=1e-7, lr=0.1, beta=0.9, weight_decay=0.0, scale=1.0, clip=math.inf)
+    v.update(kw)
+    return L.Muon(**v)
+
+
+COEF = (C.c_float * 3)(3.4445, -4.775, 2.0315)
+
+
+def test_layer_norm_arguments():
+    f = lambda x=P, xs=8, w=None, b=None, eps=1e-5, t=0, rows=4, n=8, y=P, ys=8: lib().tb_layer_norm_forward(x, xs, w, b, eps, t, rows, n, y, ys, None, None, None, e, 200)  # noqa: E731
+    for kw, text in ((dict(x=None), b"NULL"), (dict(y=None), b"NULL"), (dict(xs=7), b"stride"), (dict(ys=7), b"stride"), (dict(t=3), b"type"), (dict(t=-1), b"type"),
+                     (dict(rows=-1), b"rows"), (dict(rows=1 << 31), b"rows"), (dict(n=0), b"n positive"), (dict(eps=-1.0), b"eps"), (dict(eps=math.nan), b"eps"),
+                     (dict(x=P + 2), b"aligned"), (dict(w=P + 2), b"aligned"), (dict(x=P + 1, t=1), b"aligned")):
+        e = err()
+        assert f(**kw) == INVALID and text in e.value, (kw, e.value)
+    e = err()
+    assert f(rows=0, x=None, y=None) == 0 and e.value == b""   # nothing to do
+    g = lambda wb, **kw: lib().tb_layer_norm_backward(kw.get("dy", P), 8, P, 8, P, kw.get("rstd", P), None, 0, 4, 8, P, 8, kw.get("dw", P), P, kw.get("work", P), wb, None, e, 200)  # noqa: E731
+    need = lib().tb_layer_norm_backward_workspace(4, 8)
+    assert need > 0
+    for call in (lambda: g(need - 1), lambda: g(need, work=None), lambda: g(need, work=P + 4), lambda: g(need, dy=None), lambda: g(need, rstd=None)):
+        e = err()
+        assert call() == INVALID and e.value
+    assert lib().tb_layer_norm_forward(None, 8, None, None, 1e-5, 0, 4, 8, P, 8, None, None, None, None, 0) == INVALID   # no text wanted
+
+
+def test_route_arguments():
+    need = lib().tb_route_forward_workspace(100, 9)
+    assert need > 0 and lib().tb_route_forward_workspace(0, 1) > 0
+    f = lambda x=P, s=9, t=0, rows=100, e_=9, k=2, ix=P, work=P, wb=need: lib().tb_route_forward(x, s, t, rows, e_, k, 1, None, ix, P, P, P, P, P, work, wb, None, e, 200)  # noqa: E731
+    for kw, text in ((dict(x=None), b"NULL"), (dict(ix=None), b"NULL"), (dict(s=8), b"stride"), (dict(t=9), b"type"), (dict(e_=0), b"experts"), (dict(e_=1025, s=1025), b"experts"),
+                     (dict(k=0), b"k must"), (dict(k=10), b"k must"), (dict(k=17, e_=64, s=64), b"k must"), (dict(rows=-1), b"rows"), (dict(rows=1 << 31), b"rows"),
+                     (dict(wb=need - 1), b"workspace"), (dict(work=None), b"workspace"), (dict(x=P + 1), b"aligned")):
+        e = err()
+        assert f(**kw) == INVALID and text in e.value, (kw, e.value)
+    for bad in ((-1, 9), (5, 0), (5, 1025)):
+        assert lib().tb_route_forward_workspace(*bad) == INVALID
+    e = err()
+    assert lib().tb_route_backward(P, 9, 0, 100, 9, 2, 1, None, None, P, P, P, P, P, P, 9, None, e, 200) == INVALID
+    assert lib().tb_route_backward(P, 9, 0, 100, 9, 2, 1, None, P, P, P, P, P, P, P, 8, None, e, 200) == INVALID
+    assert lib().tb_route_backward(None, 9, 0, 0, 9, 2, 1, None, None, None, None, None, None, None, None, 9, None, e, 200) == 0
+
+
+def test_orthogonalise_arguments():
+    need = lib().tb_orthogonalise_workspace(0, 2, 100, 200)
+    assert need > 0 and need % 128 == 0 and lib().tb_orthogonalise_workspace(0, 9, 16, 1536) == 0   # short sides of up to 64 need none
+    assert lib().tb_orthogonalise_workspace(2, 2, 100, 200) < need                                  # one limb, not two
+    f = lambda x=P, xb=20000, xs=200, t=0, b=2, r=100, c=200, steps=5, co=COEF, eps=1e-7, out=P, ob=20000, os=200, work=P, wb=need: lib().tb_orthogonalise(  # noqa: E731
+        x, xb, xs, t, b, r, c, steps, co, eps, out, ob, os, work, wb, None, e, 200)
+    bad = lambda *v: (C.c_float * 3)(*v)  # noqa: E731
+    for kw, text in ((dict(x=None), b"NULL"), (dict(out=None), b"NULL"), (dict(xs=199), b"strides"), (dict(os=199), b"strides"), (dict(xb=19999), b"overlap"), (dict(ob=19999), b"overlap"),
+                     (dict(t=5), b"type"), (dict(b=-1), b"batch"), (dict(b=65536), b"batch"), (dict(r=0), b"positive"), (dict(steps=0), b"steps"), (dict(steps=33), b"steps"),
+                     (dict(co=None), b"coefficients"), (dict(co=bad(8, 0, 0)), b"coefficients"), (dict(co=bad(math.nan, 0, 0)), b"coefficients"), (dict(co=bad(1, 40, 0)), b"coefficients"),
+                     (dict(eps=-1.0), b"eps"), (dict(work=None), b"workspace"), (dict(wb=need - 1), b"workspace"), (dict(work=P + 64), b"workspace"), (dict(x=P + 2), b"aligned")):
+        e = err()
+        assert f(**kw) == INVALID and text in e.value, (kw, e.value)
+    for v in ((9, 1, 1, 1), (0, -1, 1, 1), (0, 1, 0, 1), (0, 1, 1, 0)):
+        assert lib().tb_orthogonalise_workspace(*v) == INVALID
+    e = err()
+    assert f(b=0, x=None, out=None) == 0
+
+
+def test_coefficients_that_keep_the_range_are_accepted():
+    # the quintic of the defaults over many steps, a convergent quintic, the cubic: what stops these calls is the missing workspace, not the coefficients
+    e = err()
+    for c in ((3.4445, -4.775, 2.0315), (1.875, -1.25, 0.375), (1.5, -0.5, 0.0), (1.0, 0.0, 0.0)):
+        assert lib().tb_orthogonalise(P, 20000, 200, 0, 2, 100, 200, 32, (C.c_float * 3)(*c), 1e-7, P, 20000, 200, None, 0, None, e, 200) == INVALID
+        assert b"workspace" in e.value, (c, e.value)
+
+
+def test_muon_arguments():
+    need = lib().tb_muon_step_workspace(2, 100, 200)
+    size = 4 * 2 * 100 * 200
+    w, m, g = P, P + size, P + 2 * size
+    work = P + (1 << 30)
+    f = lambda cfg=None, w=w, m=m, g=g, t=0, wo=w, mo=m, wb=need: lib().tb_muon_step(C.byref(cfg or muon()), w, m, g, t, 2, 100, 200, wo, mo, work, wb, None, e, 200)  # noqa: E731
+    for kw, text in ((dict(cfg=muon(struct_size=8)), b"size"), (dict(cfg=muon(steps=0)), b"steps"), (dict(cfg=muon(clip=0.0)), b"clip"), (dict(cfg=muon(clip=math.nan)), b"clip"),
+                     (dict(cfg=muon(eps=-1.0)), b"eps"), (dict(w=None), b"NULL"), (dict(m=None), b"NULL"), (dict(g=None), b"NULL"), (dict(wo=None), b"NULL"), (dict(t=4), b"type"),
+                     (dict(wo=m), b"overlaps"), (dict(mo=w), b"overlaps"), (dict(wo=g), b"overlaps"), (dict(mo=g), b"overlaps"), (dict(wo=w + 4), b"overlaps"), (dict(g=m), b"overlaps"),
+                     (dict(w=w + 2), b"aligned"), (dict(wb=need - 1), b"workspace")):
+        e = err()
+        assert f(**kw) == INVALID and text in e.value, (kw, e.value)
+    e = err()
+    assert lib().tb_muon_step(None, w, m, g, 0, 2, 100, 200, w, m, work, need, None, e, 200) == INVALID
+
+
+@pytest.mark.skipif("not no_gpu()", reason="a device is present")
+def test_no_device_is_an_error_and_not_a_crash():
+    e = err()
+    assert lib().tb_layer_norm_forward(P, 8, None, None, 1e-5, 0, 4, 8, P, 8, None, None, None, e, 200) == NO_DEVICE and e.value
+    assert lib().tb_orthogonalise(P, 0, 8, 0, 1, 8, 8, 5, COEF, 1e-7, P, 0, 8, None, 0, None, e, 200) == NO_DEVICE and e.value
+
+
+def test_torch_binding_refuses_host_tensors():
+    torch = pytest.importorskip("torch")
+    from tatara_b200 import ops
+    x = torch.zeros(4, 8)
+    for bad in (lambda: ops.layer_norm_forward(x), lambda: ops.layer_norm_forward(None), lambda: ops.route_forward(x, 2), lambda: ops.orthogonalise(x),
+                lambda: ops.muon_step(x, x, x, lr=0.1), lambda: ops.layer_norm_backward(x, x, x, x)):
+        with pytest.raises(tb.TrainerError, match="CUDA tensor"):
+            bad()
