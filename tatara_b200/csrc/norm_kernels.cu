@@ -46,6 +46,32 @@ __device__ __forceinline__ void norm_rows_sum(float (&v)[R], float* buf, int war
         for (int q = 0; q < R; ++q) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
 }
 
+// the sums of R rows over the W warps of a block, in place; buf is not written again before the next barrier but one
+template <int W, int R>
+__device__ __forceinline__ void norm_block_sums(float (&v)[R], float (*buf)[R], int warp, int lane) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int q = 0; q < R; ++q) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
+    if (lane == 0)
+#pragma unroll
+        for (int q = 0; q < R; ++q) buf[warp][q] = v[q];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < R; ++q) v[q] = buf[0][q];
+#pragma unroll
+    for (int k = 1; k < W; ++k)
+#pragma unroll
+        for (int q = 0; q < R; ++q) v[q] += buf[k][q];
+}
+
+// Blocks of the kernels that walk down the rows which one SM holds: 24 warps of 80 registers.  Backward, fp16, 16384 x 768: 20.4 us; 30 warps of 64 (some
+// spilled) 24.6, four rows at a time in 96 registers 26.0, the next rows fetched ahead in 175 registers 34.
+constexpr int norm_per_sm(int warps, int all = 24) {
+    const int w = warps == 1 ? 4 : warps;
+    return all / w < 1 ? 1 : all / w;
+}
+
 // VEC columns of a weight or bias, in 16-byte accesses (one element at a time they cost four to eight times the L1 wavefronts of the row
 // itself: 24 -> 8 us for 10000 rows of 1000 fp16)
 template <int VEC>
@@ -63,7 +89,7 @@ __device__ __forceinline__ void norm_columns(const float* __restrict__ p, int co
 }
 
 // W warps per row, VEC adjacent columns per access, CH accesses per thread: a thread holds columns (c * LANES + t) * VEC + i.  With W = 1 a row has L lanes
-// (8 for rows of up to 64 columns, or most lanes of a warp idle: 33615 x 9 fp32), which take R rows at once: those share the reads of weight and bias.
+// (8 or 16 for rows of up to 64 or 128 columns, or most lanes of a warp idle), which take R rows at once: those share the reads of weight and bias.
 template <typename T, int W, int L, int VEC, int CH, int R>
 __global__ void __launch_bounds__(W == 1 ? 128 : W * 32)
 k_norm_forward(const T* x, int64_t x_stride, const float* __restrict__ weight, const float* __restrict__ bias, float eps,
@@ -133,6 +159,78 @@ k_norm_forward(const T* x, int64_t x_stride, const float* __restrict__ weight, c
     }
 }
 
+// ---- rows that start anywhere: a thread's columns are single ones -----------------------------------------------------------
+// How many of a thread's places are inside the row for every thread: W warps are the fewest that hold it with eight columns a thread, and sixteen with
+// sixteen columns hold 4097 or more.
+__host__ __device__ constexpr int norm_full(int warps, int vec, int places) { return vec * places == 16 ? places / 2 : places * (warps - 1) / warps; }
+
+// Forward for rows over 256 columns that start anywhere: a block walks down the rows with its columns' weight and bias in registers, R rows at a time.
+// 35954 x 1175: 64 us in fp32 (5.2 TB/s), 55 in bf16; with a warp per row, which reads weight and bias for every row and checks every column, 105 and 127.
+// Two adjacent 16-bit columns per thread, one access where the row starts on a 4-byte boundary: 108 (the branch keeps the loads apart).
+template <typename T, int W, int CH, int R>
+__global__ void __launch_bounds__(W * 32, norm_per_sm(W, 32))
+k_norm_forward_down(const T* x, int64_t x_stride, const float* __restrict__ weight, const float* __restrict__ bias, float eps, int64_t rows, int n, T* y,
+                    int64_t y_stride, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+    constexpr int LANES = 32 * W, FULL = norm_full(W, 1, CH);
+    __shared__ float s_sum[2][2][W][R];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = threadIdx.x;
+    float w[CH], b[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int col = c * LANES + t;
+        w[c] = weight && col < n ? weight[col] : 1.0f;
+        b[c] = bias && col < n ? bias[col] : 0.0f;
+    }
+    int turn = 0;
+    for (int64_t first = (int64_t)blockIdx.x * R; first < rows; first += (int64_t)gridDim.x * R, turn ^= 1) {
+        OpRaw<T, 1> v[R][CH];
+        float mean[R], rstd[R];
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            const T* xr = x + (first + q) * x_stride;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int col = c * LANES + t;
+                v[q][c].zero();
+                if (first + q < rows && (c < FULL || col < n)) v[q][c].load(xr + col);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            mean[q] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) mean[q] += v[q][c].get(0);
+        }
+        norm_block_sums<W, R>(mean, s_sum[turn][0], warp, lane);
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            mean[q] /= (float)n;
+            rstd[q] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const float d = v[q][c].get(0) - mean[q];
+                if (c < FULL || c * LANES + t < n) rstd[q] = fmaf(d, d, rstd[q]);
+            }
+        }
+        norm_block_sums<W, R>(rstd, s_sum[turn][1], warp, lane);
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            rstd[q] = 1.0f / sqrtf(rstd[q] / (float)n + eps);
+            if (first + q >= rows) continue;
+            if (t == 0) {
+                if (mean_out) mean_out[first + q] = mean[q];
+                if (rstd_out) rstd_out[first + q] = rstd[q];
+            }
+            T* yr = y + (first + q) * y_stride;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int col = c * LANES + t;
+                if (c < FULL || col < n) yr[col] = op_round<T>(fmaf((v[q][c].get(0) - mean[q]) * rstd[q], w[c], b[c]));
+            }
+        }
+    }
+}
+
 // rows longer than NORM_REG_N: a block per row, three passes over it
 template <typename T>
 __global__ void __launch_bounds__(1024)
@@ -159,21 +257,15 @@ k_norm_forward_long(const T* __restrict__ x, int64_t x_stride, const float* __re
         yr[c] = op_round<T>(fmaf((op_float(xr[c]) - mean) * rstd, weight ? weight[c] : 1.0f, bias ? bias[c] : 0.0f));
 }
 
-// Blocks of the backward pass that one SM holds: 24 warps of 80 registers.  fp16, 16384 x 768: 20.4 us; 30 warps of 64 (some spilled) 24.6, four rows
-// at a time in 96 registers 26.0, the next rows fetched ahead in 175 registers 34.
-constexpr int norm_backward_per_sm(int warps) {
-    const int w = warps == 1 ? 4 : warps;
-    return 24 / w < 1 ? 1 : 24 / w;
-}
-
 // Backward: a block of W warps per row (W = 1: rows side by side, L lanes each) takes R rows at a time, which shares one barrier, walks
 // down the rows and keeps its columns' weight and bias gradients in registers; partial: [2][blocks][n].
 // fp32, 65536 x 1536: 175 us, 6.9 TB/s.
 template <typename T, int W, int L, int VEC, int CH, int R>
-__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, norm_backward_per_sm(W))
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, norm_per_sm(W))
 k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, const float* __restrict__ mean,
                 const float* __restrict__ rstd, const float* __restrict__ weight, int64_t rows, int n, T* dx, int64_t dx_stride,
                 float* __restrict__ partial) {
+    constexpr int FULL = norm_full(W, VEC, CH);
     constexpr int LANES = W == 1 ? L : 32 * W, SUBS = W == 1 ? 32 / L : 1, RB = W == 1 ? 4 * SUBS : 1;
     __shared__ float s_sum[2][2 * R][W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = W == 1 ? lane % L : threadIdx.x;
@@ -199,12 +291,11 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int col = (c * LANES + t) * VEC;
-                if (in && col < n) {
+                xv[q][c].zero();
+                gv[q][c].zero();
+                if (in && (c < FULL || col < n)) {
                     xv[q][c].load(x + (first + q) * x_stride + col);
                     gv[q][c].load(dy + (first + q) * dy_stride + col);
-                } else {
-                    xv[q][c].zero();
-                    gv[q][c].zero();
                 }
             }
             mu[q] = in ? mean[first + q] : 0.0f;
@@ -259,7 +350,7 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
                     const int col = (c * LANES + t) * VEC;
-                    if (col < n) {
+                    if (c < FULL || col < n) {
                         float o[VEC];
 #pragma unroll
                         for (int i = 0; i < VEC; ++i) {
@@ -382,75 +473,106 @@ __global__ void __launch_bounds__(1024) k_norm_columns_final(const float* __rest
     if (lane == 0 && blockIdx.x * 8 + warp < n) out[blockIdx.x * 8 + warp] = v;
 }
 
-// Shape of the backward pass: warps per row and columns per thread.  Eight columns a thread (two rows at a time) up to 4096 columns, sixteen
-// (one row) up to 8192.
-struct NormShape {
-    int warps, columns;
-};
-NormShape norm_backward_shape(int n) {
-    const int w8[] = {1, 2, 3, 4, 6, 8, 12, 16};
-    for (int w : w8)
-        if (n <= w * 256) return {w, 8};
-    return {16, 16};
+// Warps per row of the kernels that walk down the rows: the fewest that hold it with eight columns a thread (up to 4096 columns, two rows at a time),
+// sixteen with sixteen columns (one row) up to 8192.
+int norm_warps(int n) { return n <= 4096 ? (n + 255) / 256 : 16; }
+template <int FROM, typename F>
+void norm_with_warps(int w, F&& f) {  // f(std::integral_constant<int, W>)
+    if constexpr (FROM <= 16) {
+        if (w == FROM) f(std::integral_constant<int, FROM>());
+        else norm_with_warps<FROM + 1>(w, f);
+    }
 }
 // Blocks: at most what runs at once; 16 rows or more for each, or the blocks' rows of gradients cost as much as the rows themselves, but
 // one per SM as far as the rows go (256 rows of 256: 4 blocks took 12 us).
 int norm_backward_blocks(int64_t rows, int n) {
     if (n > NORM_REG_N_BACK) return (int)(rows < 64 ? (rows < 1 ? 1 : rows) : 64);
-    const int w = norm_backward_shape(n).warps;
-    const int64_t turn = n <= 64 ? 32 : w == 1 ? 8 : 2, sms = sm_count(), most = sms * norm_backward_per_sm(w);
+    const int w = norm_warps(n);
+    const int64_t turn = n <= 64 ? 32 : n <= 128 ? 16 : w == 1 ? 8 : 2, sms = sm_count(), most = sms * norm_per_sm(w);
     const int64_t turns = (rows + turn - 1) / turn, least = (16 + turn - 1) / turn, want = (turns + least - 1) / least;
     const int64_t few = turns < sms ? turns : sms, blocks = want < few ? few : want < most ? want : most;
     return (int)(blocks < 1 ? 1 : blocks);
 }
 
+struct NormForward {
+    cudaStream_t s;
+    const void* x;
+    int64_t xs;
+    const float *w, *b;
+    float eps;
+    int64_t rows;
+    int n;
+    void* y;
+    int64_t ys;
+    float *mean, *rstd;
+};
 template <typename T, int VEC, int W, int L, int CH>
-void norm_forward_go(cudaStream_t s, const void* x, int64_t xs, const float* w, const float* b, float eps, int64_t rows, int n, void* y, int64_t ys,
-                     float* mean, float* rstd) {
+void norm_forward_go(const NormForward& a) {
     // registers of a row's share, and how many of its elements have to be on their way: two rows where that leaves the warps enough
     constexpr int R = W == 1 && CH * VEC * (int)sizeof(T) <= 64 ? 2 : 1;
-    const int64_t per = W == 1 ? 128 / L * R : 1, blocks = (rows + per - 1) / per;
-    k_norm_forward<T, W, L, VEC, CH, R><<<(unsigned)blocks, W == 1 ? 128 : W * 32, 0, s>>>((const T*)x, xs, w, b, eps, rows, n, (T*)y, ys, mean, rstd);
+    const int64_t per = W == 1 ? 128 / L * R : 1, blocks = (a.rows + per - 1) / per;
+    k_norm_forward<T, W, L, VEC, CH, R><<<(unsigned)blocks, W == 1 ? 128 : W * 32, 0, a.s>>>((const T*)a.x, a.xs, a.w, a.b, a.eps, a.rows, a.n, (T*)a.y, a.ys, a.mean, a.rstd);
 }
-// Eight lanes per row up to 64 columns, a warp up to 2048 (no barrier in a row), eight warps above.
+template <typename T, int W, int CH, int R>
+void norm_forward_down(const NormForward& a) {
+    const int64_t want = (a.rows + R - 1) / R, most = (int64_t)sm_count() * norm_per_sm(W, 32);
+    k_norm_forward_down<T, W, CH, R><<<(unsigned)(want < most ? want : most), W * 32, 0, a.s>>>((const T*)a.x, a.xs, a.w, a.b, a.eps, a.rows, a.n, (T*)a.y, a.ys, a.mean, a.rstd);
+}
+// Rows on 16-byte boundaries: 8, 16 or 32 lanes per row up to 64, 128 and 256 columns (200000 x 128 bf16 with 32 lanes 45 us, with 16 28.7), a warp up to
+// 2048 columns of fp32 and 3072 of 16 bits (no barrier in a row; 30000 x 2560 bf16 72 us, with eight warps 94; 20000 x 4096 93 and 84), eight warps above.
+// A block that walks down the rows with weight and bias in registers needs a barrier per sum: 40000 x 2048 fp16 88 us, a warp per row 72.
 template <typename T, int VEC>
-void norm_forward_pick(cudaStream_t s, const void* x, int64_t xs, const float* w, const float* b, float eps, int64_t rows, int n, void* y, int64_t ys,
-                       float* mean, float* rstd) {
+void norm_forward_pick(const NormForward& a) {
 #define GO(W, L, K) \
-    if (n <= (W) * (K) * (L)) return norm_forward_go<T, VEC, W, L, ((K) + VEC - 1) / VEC>(s, x, xs, w, b, eps, rows, n, y, ys, mean, rstd)
-    GO(1, 8, 8); GO(1, 32, 8); GO(1, 32, 16); GO(1, 32, 24); GO(1, 32, 32); GO(1, 32, 48); GO(1, 32, 64);
-    GO(8, 32, 16); GO(8, 32, 32); GO(16, 32, 32);
+    if (a.n <= (W) * (K) * (L)) return norm_forward_go<T, VEC, W, L, ((K) + VEC - 1) / VEC>(a)
+    GO(1, 8, 8); GO(1, 16, 8); GO(1, 32, 8);
+    if constexpr (VEC > 1) {
+        if constexpr (VEC == 4) GO(1, 32, 12);
+        GO(1, 32, 16); GO(1, 32, 24); GO(1, 32, 32); GO(1, 32, 40); GO(1, 32, 48); GO(1, 32, 56); GO(1, 32, 64);
+        if constexpr (VEC == 8) { GO(1, 32, 80); GO(1, 32, 96); }
+        GO(8, 32, 16); GO(8, 32, 32); GO(16, 32, 32);
+    } else {
+        if (a.n <= 4096) return norm_with_warps<2>(norm_warps(a.n), [&](auto w) { norm_forward_down<T, decltype(w)::value, 8, 2>(a); });
+        if (a.n <= NORM_REG_N_BACK) return norm_forward_down<T, 16, 16, 1>(a);
+    }
 #undef GO
-    k_norm_forward_long<T><<<(unsigned)rows, 1024, 0, s>>>((const T*)x, xs, w, b, eps, n, (T*)y, ys, mean, rstd);
+    k_norm_forward_long<T><<<(unsigned)a.rows, 1024, 0, a.s>>>((const T*)a.x, a.xs, a.w, a.b, a.eps, a.n, (T*)a.y, a.ys, a.mean, a.rstd);
 }
 
+struct NormBackward {
+    cudaStream_t s;
+    const void* dy;
+    int64_t dys;
+    const void* x;
+    int64_t xs;
+    const float *mean, *rstd, *w;
+    int64_t rows;
+    int n;
+    void* dx;
+    int64_t dxs;
+    float* partial;
+    int blocks;
+};
+template <typename T, int VEC, int W, int L, int CH, int R>
+void norm_backward_go(const NormBackward& a) {
+    k_norm_backward<T, W, L, VEC, CH / VEC, R><<<(unsigned)a.blocks, W == 1 ? 128 : W * 32, 0, a.s>>>((const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.w, a.rows, a.n,
+                                                                                                      (T*)a.dx, a.dxs, a.partial);
+}
 template <typename T, int VEC>
-void norm_backward_pick(cudaStream_t s, const void* dy, int64_t dys, const void* x, int64_t xs, const float* mean, const float* rstd, const float* w,
-                        int64_t rows, int n, void* dx, int64_t dxs, float* partial, int blocks) {
-    if (n <= NORM_REG_N_BACK) {
-        const NormShape shape = norm_backward_shape(n);
-#define GO(W, L, K, R)                                                                                                                        \
-    k_norm_backward<T, W, L, VEC, (K) / VEC, R><<<(unsigned)blocks, W == 1 ? 128 : W * 32, 0, s>>>((const T*)dy, dys, (const T*)x, xs, mean, rstd, \
-                                                                                               w, rows, n, (T*)dx, dxs, partial)
-        switch (shape.warps) {
-            case 1:
-                if (n <= 64) GO(1, 8, 8, 2); else GO(1, 32, 8, 2);
-                break;
-            case 2: GO(2, 32, 8, 2); break;
-            case 3: GO(3, 32, 8, 2); break;
-            case 4: GO(4, 32, 8, 2); break;
-            case 6: GO(6, 32, 8, 2); break;
-            case 8: GO(8, 32, 8, 2); break;
-            case 12: GO(12, 32, 8, 2); break;
-            default:
-                if (shape.columns == 8) GO(16, 32, 8, 2); else GO(16, 32, 16, 1);
-        }
-#undef GO
-        return;
+void norm_backward_pick(const NormBackward& a) {
+    if (a.n > NORM_REG_N_BACK) {
+        k_norm_backward_long<T><<<(unsigned)a.rows, 1024, 0, a.s>>>((const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.w, a.n, (T*)a.dx, a.dxs);
+        if (a.partial)
+            k_norm_columns_long<T><<<dim3((unsigned)ceil_div(a.n, 256), (unsigned)a.blocks), 256, 0, a.s>>>((const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.rows, a.n, a.partial);
+    } else if (a.n <= 64) {
+        norm_backward_go<T, VEC, 1, 8, 8, 2>(a);
+    } else if (a.n <= 128) {
+        norm_backward_go<T, VEC, 1, 16, 8, 2>(a);
+    } else if (a.n > 4096) {
+        norm_backward_go<T, VEC, 16, 32, 16, 1>(a);
+    } else {
+        norm_with_warps<1>(norm_warps(a.n), [&](auto w) { norm_backward_go<T, VEC, decltype(w)::value, 32, 8, 2>(a); });
     }
-    k_norm_backward_long<T><<<(unsigned)rows, 1024, 0, s>>>((const T*)dy, dys, (const T*)x, xs, mean, rstd, w, n, (T*)dx, dxs);
-    if (partial)
-        k_norm_columns_long<T><<<dim3((unsigned)ceil_div(n, 256), (unsigned)blocks), 256, 0, s>>>((const T*)dy, dys, (const T*)x, xs, mean, rstd, rows, n, partial);
 }
 
 bool norm_aligned(const void* p, int64_t stride, int size) { return ((uintptr_t)p & 15) == 0 && (stride * size) % 16 == 0; }
@@ -473,11 +595,10 @@ extern "C" int tb_layer_norm_forward(const void* d_x, int64_t x_stride, const fl
     if (((uintptr_t)d_x | (uintptr_t)d_y) % size || ((uintptr_t)d_weight | (uintptr_t)d_bias) & 3) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = n % (16 / size) == 0 && norm_aligned(d_x, x_stride, size) && norm_aligned(d_y, y_stride, size) && (((uintptr_t)d_weight | (uintptr_t)d_bias) & 15) == 0;
-#define ARGS s, d_x, x_stride, d_weight, d_bias, eps, rows, n, d_y, y_stride, d_mean, d_rstd
-    if (type == TB_TYPE_F32) wide ? norm_forward_pick<float, 4>(ARGS) : norm_forward_pick<float, 1>(ARGS);
-    else if (type == TB_TYPE_F16) wide ? norm_forward_pick<__half, 8>(ARGS) : norm_forward_pick<__half, 1>(ARGS);
-    else wide ? norm_forward_pick<__nv_bfloat16, 8>(ARGS) : norm_forward_pick<__nv_bfloat16, 1>(ARGS);
-#undef ARGS
+    const NormForward a = {s, d_x, x_stride, d_weight, d_bias, eps, rows, n, d_y, y_stride, d_mean, d_rstd};
+    if (type == TB_TYPE_F32) wide ? norm_forward_pick<float, 4>(a) : norm_forward_pick<float, 1>(a);
+    else if (type == TB_TYPE_F16) wide ? norm_forward_pick<__half, 8>(a) : norm_forward_pick<__half, 1>(a);
+    else wide ? norm_forward_pick<__nv_bfloat16, 8>(a) : norm_forward_pick<__nv_bfloat16, 1>(a);
     return op_launched(err, err_len);
 }
 
@@ -509,11 +630,10 @@ extern "C" int tb_layer_norm_backward(const void* d_dy, int64_t dy_stride, const
         return op_launched(err, err_len);
     }
     const bool wide = n % (16 / size) == 0 && norm_aligned(d_dy, dy_stride, size) && norm_aligned(d_x, x_stride, size) && norm_aligned(d_dx, dx_stride, size) && ((uintptr_t)d_weight & 15) == 0;
-#define ARGS s, d_dy, dy_stride, d_x, x_stride, d_mean, d_rstd, d_weight, rows, n, d_dx, dx_stride, partial, blocks
-    if (type == TB_TYPE_F32) wide ? norm_backward_pick<float, 4>(ARGS) : norm_backward_pick<float, 1>(ARGS);
-    else if (type == TB_TYPE_F16) wide ? norm_backward_pick<__half, 8>(ARGS) : norm_backward_pick<__half, 1>(ARGS);
-    else wide ? norm_backward_pick<__nv_bfloat16, 8>(ARGS) : norm_backward_pick<__nv_bfloat16, 1>(ARGS);
-#undef ARGS
+    const NormBackward a = {s, d_dy, dy_stride, d_x, x_stride, d_mean, d_rstd, d_weight, rows, n, d_dx, dx_stride, partial, blocks};
+    if (type == TB_TYPE_F32) wide ? norm_backward_pick<float, 4>(a) : norm_backward_pick<float, 1>(a);
+    else if (type == TB_TYPE_F16) wide ? norm_backward_pick<__half, 8>(a) : norm_backward_pick<__half, 1>(a);
+    else wide ? norm_backward_pick<__nv_bfloat16, 8>(a) : norm_backward_pick<__nv_bfloat16, 1>(a);
     if (columns) op_launch_next(s, dim3((unsigned)ceil_div(n, 8), 2), dim3(1024), 0, k_norm_columns_final, partial, blocks, n, d_dweight, d_dbias);
     return op_launched(err, err_len);
 }

@@ -46,7 +46,7 @@ struct OpRaw {
         if (N * sizeof(T) == 16) {
             const uint4 u = *reinterpret_cast<const uint4*>(p);
             w[0] = u.x, w[1 % WORDS] = u.y, w[2 % WORDS] = u.z, w[3 % WORDS] = u.w;
-        } else if (sizeof(T) == 2) {
+        } else if (N * sizeof(T) == 2) {
             w[0] = *reinterpret_cast<const unsigned short*>(p);
         } else {
             w[0] = *reinterpret_cast<const unsigned*>(p);
