@@ -21,9 +21,9 @@
 // warps add what it held to their registers, rounded to nearest, while the next one fills.
 // Every wait is bounded; where one runs out the block's results become NaN, and so the output.
 //
-// Measured, 4096 x 4096 in fp32: Gram and square 158 us each, apply 293 us (1.4 PFLOP/s of limb products, tensor pipe 82 to 89 % busy), last product with
-// the weight update 360 us; the whole Muon step 3.3 to 3.7 ms, where the chip's power limit, not the kernel, sets the clock.  bf16: 1.16 ms.  Small
-// products are bound by what surrounds the MMAs: 4 x 1000 x 777 bf16 takes 141 us in 17 launches of 8 to 10 us, 2 to 4 us of each inside the K loop.
+// Measured, 4096 x 4096 in fp32: Gram 156 us, square 166, apply 287 (1.4 PFLOP/s of limb products, tensor pipe 78 to 92 % busy), last product with
+// the weight update 324; the whole Muon step 3.3 to 3.8 ms, where the chip's power limit, not the kernel, sets the clock.  bf16: 1.15 ms.  Small
+// products are bound by what surrounds the MMAs: 4 x 1000 x 777 bf16 takes 137 us in 17 launches of 8 to 10 us, 2 to 4 us of each inside the K loop.
 #include "orth.cuh"
 
 #include <atomic>
@@ -272,7 +272,7 @@ struct OtGemm {
     int64_t a_limb, b_limb, out_limb;  // bytes of a limb
     int a_width, b_width, out_width;
     int chunks;          // of K, 64 each: what lies beyond them in the tiles is never read as K, whatever it holds
-    int row_tiles;       // of the result, 128 CTAS each
+    int row_tiles;       // of the result
     int col_tiles;
     float ca, cb, cc;    // square: a I + b A + c A A
     float* part;         // Gram in gridDim.y parts of K: the parts' sums [batch][tile][part][32 column quads][128 rows][4]
@@ -291,12 +291,20 @@ struct OtShape {
 struct OtTile {
     int batch, i, j;
 };
-template <bool SYM>
+// W: columns of a tile, in 64s.  A tile of 64 or 128 columns has 128 rows, one of 256 has 256
+template <int W>
+__host__ __device__ constexpr int ot_sym_tiles(int row_tiles) { return W == 1 ? row_tiles * (row_tiles + 1) : row_tiles * (row_tiles + 1) / 2; }
+template <bool SYM, int W>
 __device__ __forceinline__ OtTile ot_tile(const OtGemm& g, int t, int tiles) {
     OtTile p;
     p.batch = t / tiles;
     t -= p.batch * tiles;
-    if (SYM) {
+    if (SYM && W == 1) {
+        p.i = (int)((sqrtf(4.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
+        while ((p.i + 1) * (p.i + 2) <= t) ++p.i;
+        while (p.i * (p.i + 1) > t) --p.i;
+        p.j = t - p.i * (p.i + 1);
+    } else if (SYM) {
         p.i = (int)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
         while ((p.i + 1) * (p.i + 2) / 2 <= t) ++p.i;
         while (p.i * (p.i + 1) / 2 > t) --p.i;
@@ -342,17 +350,22 @@ struct OtSector {
     }
 };
 
-// CTAS = 1: a block computes 128 x 128.  CTAS = 2: a cluster of two blocks computes 256 x 256 with cta_group::2 MMAs: each block holds 128 rows
-// of the left operand, 128 columns of the right one and 128 x 256 accumulators; the even block issues the MMAs.
-// Warps 0-7 read the accumulators (warp w: lanes 32 (w % 4) .. of them, columns 64 CTAS (w / 4) ..), warp 8 copies, warp 9 issues the MMAs.
+// W, a tile's columns in 64s.  W = 4: a cluster of two blocks computes 256 x 256 with cta_group::2 MMAs: each block holds 128 rows of the left
+// operand, 128 columns of the right one and 128 x 256 accumulators; the even block issues the MMAs.  W = 2 and 1: a block computes 128 x 128 or
+// 128 x 64.  Where all tiles run at once, half of a tile is half of its MMAs and of its epilogue: 359 x 785 170 us with 128 x 128 tiles, 127 with
+// 128 x 64 (fp32; bf16 90 and 74), 65 x 65 92 and 68 us.
+// Warps 0-7 read the accumulators (warp w: lanes 32 (w % 4) .. of them, columns 32 W (w / 4) ..), warp 8 copies, warp 9 issues the MMAs.
 // MULTI: a block (pair) takes the tiles t, t + blocks, ..; while the eight warps store a tile from their registers, the next one's copies and MMAs are
 // under way.  Those stores go straight to memory in whole 32-byte sectors (one instruction per lane; a tile's 16-byte pieces swap places inside their
 // sector in odd rows), the mirrored tile's in 64 bytes per warp.  4096 x 4096 in bf16: 1406 us with a block per tile, 1200 so.  Where all tiles run at once
 // they leave through shared memory, 5 % sooner, and both in one kernel would cost the small products 15 % (a launch runs through its code once).
-template <int KIND, int LIMBS, int CTAS, bool MULTI, typename T>
+template <int KIND, int LIMBS, int W, bool MULTI, typename T>
 __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
     using S = OtShape<LIMBS>;
-    constexpr int TN = 128 * CTAS, COLS = 64 * CTAS;  // accumulator columns of a block, of a thread
+    constexpr int CTAS = W == 4 ? 2 : 1;
+    constexpr int TN = 64 * W, COLS = 32 * W;  // accumulator columns of a block, of a thread
+    constexpr int HALF = OT_TILE / 2;          // 64 rows of a tile
+    constexpr int RC = W == 1 ? 32 : 64;       // columns of a thread that leave at a time
     constexpr bool SYM = KIND == OT_GRAM || KIND == OT_SQUARE || KIND == OT_GRAM_PART;
     extern __shared__ uint8_t s_raw[];
     __shared__ __align__(8) unsigned long long s_full[S::STAGES], s_peer[S::STAGES], s_empty[S::STAGES], s_acc_full[2], s_acc_empty[2];
@@ -363,8 +376,8 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
     // the warp's number is the same in its lanes, and the compiler has to know it: what the MMAs take lives in uniform registers then
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
-    const int tiles = SYM ? g.row_tiles * (g.row_tiles + 1) / 2 : g.row_tiles * g.col_tiles, total = tiles * io.batch;
-    const OtTile only = ot_tile<SYM>(g, first, tiles);  // of a block with one tile: known before the launch ahead is done
+    const int tiles = SYM ? ot_sym_tiles<W>(g.row_tiles) : g.row_tiles * g.col_tiles, total = tiles * io.batch;
+    const OtTile only = ot_tile<SYM, W>(g, first, tiles);  // of a block with one tile: known before the launch ahead is done
     if (tid == 0) {
         for (int s = 0; s < S::STAGES; ++s) {
             ot_bar_init(ot_smem(&s_full[s]), 1);
@@ -404,14 +417,15 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
         unsigned s = 0, parity = 1;  // a barrier that nothing has arrived at yet passes for the phase before its first
         int64_t count = 0;           // chunks issued
         for (int t = first; ok && t < total; t += MULTI ? step : total) {
-            const OtTile at = MULTI ? ot_tile<SYM>(g, t, tiles) : only;
-            const bool same = SYM && at.i == at.j;
-            const int col_tile = at.j * CTAS + rank;  // this block's columns of the right operand, in 128s
+            const OtTile at = MULTI ? ot_tile<SYM, W>(g, t, tiles) : only;
+            const bool same = SYM && at.i == (W == 1 ? at.j >> 1 : at.j);
+            const int col_tile = at.j * CTAS + rank;  // this block's columns of the right operand, in 128s (W = 1: 64s)
             const uint8_t* a = g.a + (int64_t)at.batch * LIMBS * g.a_limb + ((int64_t)(at.i * CTAS + rank) * g.a_width + chunk0) * OT_TILE;
             // SYM: the tiles of a row, one after the other; else two half tiles (64 rows) at a time, the next rows' half in the same tiles or a row of tiles on
-            const uint8_t* b = g.b + (int64_t)at.batch * LIMBS * g.b_limb + (SYM ? (int64_t)col_tile * g.b_width + chunk0 : (int64_t)2 * col_tile) * OT_TILE;
-            const int64_t b_odd = SYM ? OT_TILE : OT_TILE / 2, b_even = SYM ? OT_TILE : (int64_t)g.b_width * OT_TILE - OT_TILE / 2;
-            const unsigned bytes = same ? LIMBS * OT_TILE : 2 * LIMBS * OT_TILE;
+            const uint8_t* b = g.b + (int64_t)at.batch * LIMBS * g.b_limb + (W == 1 ? (SYM ? ((int64_t)(col_tile >> 1) * g.b_width + chunk0) * OT_TILE + (col_tile & 1) * HALF : (int64_t)col_tile * OT_TILE)
+                                                                                : (SYM ? (int64_t)col_tile * g.b_width + chunk0 : (int64_t)2 * col_tile) * OT_TILE);
+            const int64_t b_odd = SYM ? OT_TILE : HALF, b_even = SYM ? OT_TILE : (int64_t)g.b_width * OT_TILE - HALF;
+            const unsigned bytes = LIMBS * (same ? OT_TILE : W == 1 ? OT_TILE + HALF : 2 * OT_TILE);
             for (int k = 0; k < chunks; ++k, ++count) {
                 const unsigned bar = ot_smem(&s_full[0]) + 8 * s, to = ring + s * S::STAGE;
                 ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_empty[0]) + 8 * s, parity));
@@ -423,8 +437,8 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                         ot_copy(to + l * OT_TILE, a + l * g.a_limb, OT_TILE, bar);
                         if (same) continue;
                         const unsigned tb = to + (LIMBS + l) * OT_TILE;
-                        ot_copy(tb, b + l * g.b_limb, SYM ? OT_TILE : OT_TILE / 2, bar);
-                        if (!SYM) ot_copy(tb + OT_TILE / 2, b + l * g.b_limb + OT_TILE, OT_TILE / 2, bar);
+                        ot_copy(tb, b + l * g.b_limb, SYM && W > 1 ? OT_TILE : HALF, bar);
+                        if (!SYM && W > 1) ot_copy(tb + HALF, b + l * g.b_limb + OT_TILE, HALF, bar);
                     }
                 }
                 __syncwarp();
@@ -452,9 +466,10 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
             const bool leader = ot_elect();
             unsigned buffer = 0, drained = 1;  // the accumulator, and the parity of its being empty
             for (int t = first; ok && t < total; t += MULTI ? step : total) {
-                const OtTile at = MULTI ? ot_tile<SYM>(g, t, tiles) : only;
-                const unsigned b_at = SYM && at.i == at.j ? ring : ring + LIMBS * OT_TILE;
-                const unsigned long long db0 = SYM ? ot_desc(b_at, 16, 1024) : ot_desc(b_at, OT_TILE / 2, 1024);
+                const OtTile at = MULTI ? ot_tile<SYM, W>(g, t, tiles) : only;
+                const bool same = SYM && at.i == (W == 1 ? at.j >> 1 : at.j);
+                const unsigned b_at = same ? ring + (W == 1 ? (at.j & 1) * HALF : 0) : ring + LIMBS * OT_TILE;
+                const unsigned long long db0 = SYM ? ot_desc(b_at, 16, 1024) : ot_desc(b_at, HALF, 1024);
                 int k = 0;
                 for (int r = 0; r < rounds && ok; ++r) {
                     const unsigned d = tmem + buffer * TN;
@@ -510,7 +525,7 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
         const int group = warp >> 2, row = tid & 127;
         unsigned buffer = 0, filled = 0;
         for (int t = first; t < total; t += MULTI ? step : total) {
-            const OtTile at = MULTI ? ot_tile<SYM>(g, t, tiles) : only;
+            const OtTile at = MULTI ? ot_tile<SYM, W>(g, t, tiles) : only;
             float acc[COLS];
 #pragma unroll
             for (int c = 0; c < COLS; ++c) acc[c] = 0.0f;
@@ -541,9 +556,10 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
             }
 
             if (KIND == OT_GRAM_PART) {
-                float4* to = reinterpret_cast<float4*>(g.part) + ((int64_t)t * gridDim.y + blockIdx.y) * 4096 + row;
+                const int whole = W == 1 ? t / tiles * (tiles / 2) + at.i * (at.i + 1) / 2 + (at.j >> 1) : t, from = W == 1 ? (at.j & 1) * 64 : 0;  // of the 128 x 128 tiles
+                float4* to = reinterpret_cast<float4*>(g.part) + ((int64_t)whole * gridDim.y + blockIdx.y) * 4096 + row;
 #pragma unroll
-                for (int c = 0; c < COLS; c += 4) to[(group * COLS + c) / 4 * 128] = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+                for (int c = 0; c < COLS; c += 4) to[(from + group * COLS + c) / 4 * 128] = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
             } else if (KIND == OT_LAST && MULTI) {
                 // rows on 16-byte boundaries go out straight from the registers, eight elements at a time
                 const int i = (at.i * CTAS + rank) * 128 + row, j0 = (at.j * 2 + group) * COLS;
@@ -578,7 +594,7 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                         }
                     }
             } else if (KIND == OT_LAST) {
-                // rows that start anywhere, or are columns: by rounds of 64 columns through shared memory (a block has one tile, its ring is free by now)
+                // rows that start anywhere, or are columns: by rounds of 64 (W = 1: 32) columns through shared memory (a block has one tile, its ring is free by now)
                 float* flat = reinterpret_cast<float*>(s_dyn + group * 40960);  // [128][65]
                 const bool tall = io.rows > io.cols;
                 const int n = tall ? io.cols : io.rows, m = tall ? io.rows : io.cols;
@@ -586,17 +602,18 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                 for (int h = 0; h < CTAS; ++h) {
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) flat[row * 65 + c] = acc[64 * h + c] * OT_UNSCALE;
+                    for (int c = 0; c < RC; ++c) flat[row * 65 + c] = acc[RC * h + c] * OT_UNSCALE;
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
-                    const int i0 = (at.i * CTAS + rank) * 128, j0 = (at.j * 2 * CTAS + group * CTAS + h) * 64;
-                    // 128 (64) neighbours in memory at a time, eight of a thread's old weights on their way.  A thread's elements lie `next` apart
-                    const int r = row >> 6, c = row & 63;
+                    const int i0 = (at.i * CTAS + rank) * 128, j0 = W == 1 ? at.j * 64 + group * 32 : (at.j * 2 * CTAS + group * CTAS + h) * 64;
+                    // 128 (64, 32) neighbours in memory at a time, eight of a thread's old weights on their way.  A thread's elements lie `next` apart
+                    constexpr int AT_ONCE = 128 / RC;
+                    const int r = row / RC, c = row % RC;
                     const int64_t to = at.batch * io.out_batch + (tall ? (int64_t)j0 * io.out_stride + i0 + row : (int64_t)(i0 + r) * io.out_stride + j0 + c);
-                    const int64_t next = tall ? io.out_stride : 2 * io.out_stride;
-                    const int left = tall ? (i0 + row < n ? m - j0 : 0) : (j0 + c < m ? (n - i0 - r + 1) / 2 : 0);
+                    const int64_t next = tall ? io.out_stride : AT_ONCE * io.out_stride;
+                    const int left = tall ? (i0 + row < n ? m - j0 : 0) : (j0 + c < m ? (n - i0 - r + AT_ONCE - 1) / AT_ONCE : 0);
                     const float* from = tall ? flat + row * 65 : flat + r * 65 + c;
-                    const int jump = tall ? 1 : 130;
-                    for (int e0 = 0; e0 < 64 && e0 < left; e0 += 8) {
+                    const int jump = tall ? 1 : 65 * AT_ONCE;
+                    for (int e0 = 0; e0 < RC && e0 < left; e0 += 8) {
                         float w[8];
 #pragma unroll
                         for (int u = 0; u < 8; ++u) w[u] = io.m && e0 + u < left ? io.w[to + (e0 + u) * next] : 0.0f;
@@ -606,7 +623,7 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                     }
                 }
             } else {
-                const bool same = SYM && at.i == at.j;
+                const bool same = SYM && at.i == (W == 1 ? at.j >> 1 : at.j);
                 const int row_tile = at.i * CTAS + rank;
                 uint8_t* out = g.out + (int64_t)at.batch * LIMBS * g.out_limb;
                 // Nothing follows a block's only tile, so its ring is free for images of the result's tiles, which go out as bulk copies.  An image:
@@ -618,32 +635,33 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                 const float square = g.cc * (OT_UNSCALE * OT_SCALE);
 #pragma unroll
                 for (int h = 0; h < CTAS; ++h) {
-                    const int col_tile = at.j * 2 * CTAS + group * CTAS + h;  // the round's columns, in 64s
+                    const int col_tile = W == 1 ? at.j : at.j * 2 * CTAS + group * CTAS + h;  // the round's columns, in 64s
+                    const int base = W == 1 ? group * 32 : 0;                               // W = 1: both groups have half of the same ones
                     const int64_t to_direct = ((int64_t)row_tile * g.out_width + col_tile) * OT_TILE;
                     const int64_t to_mirror = ((int64_t)(col_tile >> 1) * g.out_width + 2 * row_tile) * OT_TILE + (col_tile & 1) * (OT_TILE / 2);
-                    uint8_t* image = s_dyn + (group + (APART ? 2 * h : 0)) * IMAGES;
+                    uint8_t* image = s_dyn + (W == 1 ? 0 : group + (APART ? 2 * h : 0)) * IMAGES;
                     uint8_t* direct = staged ? image + row * 128 : out + to_direct + row * 128;
                     const int64_t direct_limb = staged ? OT_TILE : g.out_limb;
                     uint8_t* mirror = staged ? image + LIMBS * OT_TILE + (row >> 6) * (OT_TILE / 2) + (row & 7) * 2 : out + to_mirror + (row >> 6) * OT_TILE + (row & 7) * 2;
                     const uint8_t* old = g.a + (int64_t)at.batch * LIMBS * g.a_limb + ((int64_t)row_tile * g.a_width + col_tile) * OT_TILE + row * 128;
-                    const int ident = row_tile * 128 + row - col_tile * 64;  // the diagonal's column
+                    const int ident = row_tile * 128 + row - col_tile * 64 - base;  // the diagonal's column
                     if (h && staged && !APART) asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
                     OtSector before[LIMBS];  // square: A, a sector ahead
                     if (KIND == OT_SQUARE)
 #pragma unroll
-                        for (int l = 0; l < LIMBS; ++l) before[l].load(old + l * g.a_limb + ((row & 6) << 4));
+                        for (int l = 0; l < LIMBS; ++l) before[l].load(old + l * g.a_limb + (((base >> 3) ^ (row & 6)) << 4));
 #pragma unroll
-                    for (int c0 = 0; c0 < 64; c0 += 16) {
+                    for (int c0 = 0; c0 < RC; c0 += 16) {
                         float x[16];  // scaled as it is stored
 #pragma unroll
-                        for (int c = 0; c < 16; ++c) x[c] = acc[64 * h + c0 + c] * (KIND == OT_SQUARE ? square : OT_UNSCALE * OT_SCALE);
+                        for (int c = 0; c < 16; ++c) x[c] = acc[RC * h + c0 + c] * (KIND == OT_SQUARE ? square : OT_UNSCALE * OT_SCALE);
                         if (KIND == OT_SQUARE) {
 #pragma unroll
                             for (int l = LIMBS - 1; l >= 0; --l) {
                                 before[l].exchange(swap);
 #pragma unroll
                                 for (int c = 0; c < 16; ++c) x[c] = fmaf(g.cb, before[l].get(c), x[c]);
-                                if (c0 < 48) before[l].load(old + l * g.a_limb + ((((c0 + 16) >> 3) ^ (row & 6)) << 4));
+                                if (c0 + 16 < RC) before[l].load(old + l * g.a_limb + ((((base + c0 + 16) >> 3) ^ (row & 6)) << 4));
                             }
                             if (same)  // the diagonal passes through these tiles alone
 #pragma unroll
@@ -662,7 +680,7 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                             for (int l = 0; l < LIMBS; ++l) {
                                 piece[l].w[c / 2] = *reinterpret_cast<const unsigned*>(&pair[l]);
                                 if (SYM && !same) {
-                                    uint8_t* to = mirror + (staged ? l * OT_TILE : l * g.out_limb) + (c0 + c) * 128;
+                                    uint8_t* to = mirror + (staged ? l * OT_TILE : l * g.out_limb) + (base + c0 + c) * 128;
                                     const int slot = (row & 63) >> 3;
                                     if (staged) {  // not left to the compiler: a generic store costs as much as a global one
                                         ot_store_shared(to + (((slot ^ (c0 + c)) & 7) << 4), __low2half(pair[l]));
@@ -678,17 +696,18 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                         for (int l = 0; l < LIMBS; ++l) {
                             uint8_t* to = direct + l * direct_limb;
                             if (staged) {
-                                piece[l].store_shared(to, (c0 >> 3) ^ (row & 7));
+                                piece[l].store_shared(to, ((base + c0) >> 3) ^ (row & 7));
                             } else {
                                 piece[l].exchange(swap);
-                                piece[l].store(to + (((c0 >> 3) ^ (row & 6)) << 4));
+                                piece[l].store(to + ((((base + c0) >> 3) ^ (row & 6)) << 4));
                             }
                         }
                     }
                     if (staged) {
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
-                        if (row == 0) {
+                        if (W == 1) asm volatile("bar.sync 1, 256;" ::: "memory");
+                        else asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+                        if (W == 1 ? tid == 0 : row == 0) {
 #pragma unroll
                             for (int l = 0; l < LIMBS; ++l) {
                                 ot_put(out + l * g.out_limb + to_direct, ot_smem(image + l * OT_TILE), OT_TILE);
@@ -757,35 +776,41 @@ __global__ void __launch_bounds__(256) k_orth_join(const float* __restrict__ par
 }
 
 struct OtPlan {
-    int sym_ctas, all_ctas;                  // blocks per tile of the symmetric products and of Q X
+    int sym, all;                            // columns of a tile of the symmetric products and of Q X, in 64s
     int parts;                               // of K in the Gram product
     int n, m, n_pad, m_pad;
     int64_t x_limb, a_limb;                  // bytes of a limb
     int64_t x0, x1, a, q, part, total;       // offsets in the workspace
 };
-// Cycles of a product by the waves of its tiles: a chunk of K in a 128 x 128 tile of one block, a 256 x 256 tile of two, with one limb or two, and
-// a tile's fixed part (launch, first copies, epilogue), as measured at n = 777, m = 1000 and 4096 x 4096.
-int64_t ot_cost(int64_t tiles, int64_t chunks, int limbs, int ctas) {
-    const int64_t slots = sm_count() / ctas, waves = (tiles + slots - 1) / slots;
-    return waves * (ctas == 1 ? chunks * (limbs == 1 ? 390 : 990) + 9000 : chunks * (limbs == 1 ? 450 : 1520) + (limbs == 1 ? 13000 : 18000));
+// Cycles of a product by the waves of its tiles: a chunk of K in a tile of 64, 128 (one block) or 256 (two) columns, with one limb or two, and
+// a tile's fixed part (launch, first copies, epilogue), as measured at n = 777, m = 1000 and 4096 x 4096 and, for 64 columns, n = 359, m = 785.
+int64_t ot_chunk(int limbs, int w) { return limbs == 1 ? (w == 1 ? 350 : w == 2 ? 390 : 450) : w == 1 ? 600 : w == 2 ? 990 : 1520; }
+int64_t ot_cost(int64_t tiles, int64_t chunks, int limbs, int w) {
+    const int64_t slots = sm_count() / (w == 4 ? 2 : 1), waves = (tiles + slots - 1) / slots;
+    return waves * (chunks * ot_chunk(limbs, w) + (w == 1 ? 8000 : w == 2 ? 9000 : limbs == 1 ? 13000 : 18000));
 }
 OtPlan ot_plan(int batch, int rows, int cols, int limbs) {
     OtPlan p;
     p.n = rows < cols ? rows : cols;
     p.m = rows < cols ? cols : rows;
     const int64_t n1 = (p.n + 127) / 128, n2 = (p.n + 255) / 256, m1 = (p.m + 127) / 128, m2 = (p.m + 255) / 256, kn = (p.n + 63) / 64, km = (p.m + 63) / 64;
-    const int64_t s1 = batch * n1 * (n1 + 1) / 2, s2 = batch * n2 * (n2 + 1) / 2;
-    p.sym_ctas = ot_cost(s2, kn, limbs, 2) + ot_cost(s2, km, limbs, 2) < ot_cost(s1, kn, limbs, 1) + ot_cost(s1, km, limbs, 1) ? 2 : 1;
-    p.all_ctas = ot_cost(batch * n2 * m2, kn, limbs, 2) < ot_cost(batch * n1 * m1, kn, limbs, 1) ? 2 : 1;
+    int64_t best = 0, sym_best = 0;
+    for (int w = 1; w <= 4; w *= 2) {
+        const int64_t sym = batch * (w == 4 ? n2 * (n2 + 1) / 2 : n1 * (n1 + 1) / (w == 1 ? 1 : 2)), all = batch * (w == 4 ? n2 * m2 : w == 2 ? n1 * m1 : 2 * n1 * m1);
+        const int64_t cs = ot_cost(sym, kn, limbs, w) + ot_cost(sym, km, limbs, w), ca = ot_cost(all, kn, limbs, w);
+        if ((w > 1 || sym <= sm_count()) && (sym_best == 0 || cs < sym_best)) sym_best = cs, p.sym = w;
+        if ((w > 1 || all <= sm_count()) && (best == 0 || ca < best)) best = ca, p.all = w;
+    }
     // few tiles with a long K are cut into parts where that saves more than the launch that joins them
     p.parts = 1;
-    if (p.sym_ctas == 1) {
-        int64_t q = sm_count() / s1;
+    const int64_t s1 = batch * n1 * (n1 + 1) / 2;
+    if (p.sym < 4) {
+        int64_t q = sm_count() / (s1 * (p.sym == 1 ? 2 : 1));
         q = q < OT_PARTS ? q : OT_PARTS;
         q = q < km / 4 ? q : km / 4;
-        if (q > 1 && (km - km / q) * (limbs == 1 ? 390 : 990) > 9000) p.parts = (int)q;
+        if (q > 1 && (km - km / q) * ot_chunk(limbs, p.sym) > 9000) p.parts = (int)q;
     }
-    const int pad = 128 * (p.sym_ctas > p.all_ctas ? p.sym_ctas : p.all_ctas);
+    const int pad = p.sym == 4 || p.all == 4 ? 256 : 128;
     p.n_pad = (p.n + pad - 1) / pad * pad;
     p.m_pad = (int)(((int64_t)p.m + pad - 1) / pad * pad);
     p.x_limb = (int64_t)p.n_pad * p.m_pad * 2;
@@ -799,10 +824,11 @@ OtPlan ot_plan(int batch, int rows, int cols, int limbs) {
     return p;
 }
 
-template <int KIND, int LIMBS, int CTAS, bool MULTI, typename T>
+template <int KIND, int LIMBS, int W, bool MULTI, typename T>
 void ot_launch(cudaStream_t s, const OtGemm& g, const OrthIo& io, int64_t blocks, int parts) {
     using S = OtShape<LIMBS>;
-    auto kern = k_orth_gemm<KIND, LIMBS, CTAS, MULTI, T>;
+    constexpr int CTAS = W == 4 ? 2 : 1;
+    auto kern = k_orth_gemm<KIND, LIMBS, W, MULTI, T>;
     static std::atomic<uint64_t> known{0};  // devices on which the kernel may take that much shared memory
     int dev = 0;
     cudaGetDevice(&dev);
@@ -824,43 +850,45 @@ void ot_launch(cudaStream_t s, const OtGemm& g, const OrthIo& io, int64_t blocks
     cfg.numAttrs = CTAS == 2 ? 2 : 1;
     cudaLaunchKernelEx(&cfg, kern, g, io);
 }
-template <int KIND, int LIMBS, int CTAS, typename T>
-void ot_gemm(cudaStream_t s, const OtGemm& g, const OrthIo& io, int parts = 1) {
-    const int64_t tiles = KIND == OT_APPLY || KIND == OT_LAST ? (int64_t)g.row_tiles * g.col_tiles : (int64_t)g.row_tiles * (g.row_tiles + 1) / 2;
-    const int64_t all = tiles * io.batch, slots = sm_count() / CTAS;
+template <int KIND, int LIMBS, int W, typename T>
+void ot_gemm_of(cudaStream_t s, const OtGemm& g, const OrthIo& io, int parts) {
+    const int64_t tiles = KIND == OT_APPLY || KIND == OT_LAST ? (int64_t)g.row_tiles * g.col_tiles : ot_sym_tiles<W>(g.row_tiles);
+    const int64_t all = tiles * io.batch, slots = sm_count() / (W == 4 ? 2 : 1);
     if constexpr (KIND == OT_LAST) {  // MULTI: the result can be stored straight from the registers
         const bool aligned = io.cols % 8 == 0 && io.out_stride % 8 == 0 && io.out_batch % 8 == 0 && (((uintptr_t)io.out | (uintptr_t)io.w) & 15) == 0;
-        if (io.rows <= io.cols && aligned) return ot_launch<KIND, LIMBS, CTAS, true, T>(s, g, io, all > slots ? slots : all, parts);
-    } else if constexpr (KIND != OT_GRAM_PART) {
-        if (all > slots) return ot_launch<KIND, LIMBS, CTAS, true, T>(s, g, io, slots, parts);
+        if (io.rows <= io.cols && aligned) return ot_launch<KIND, LIMBS, W, true, T>(s, g, io, all > slots ? slots : all, parts);
+    } else if constexpr (KIND != OT_GRAM_PART && W > 1) {  // tiles of 64 columns are taken where all run at once
+        if (all > slots) return ot_launch<KIND, LIMBS, W, true, T>(s, g, io, slots, parts);
     }
-    ot_launch<KIND, LIMBS, CTAS, false, T>(s, g, io, all, parts);
+    ot_launch<KIND, LIMBS, W, false, T>(s, g, io, all, parts);
+}
+template <int KIND, int LIMBS, typename T>
+void ot_gemm(cudaStream_t s, const OtGemm& g, const OrthIo& io, int w, int parts = 1) {
+    if (w == 1) ot_gemm_of<KIND, LIMBS, 1, T>(s, g, io, parts);
+    else if (w == 2) ot_gemm_of<KIND, LIMBS, 2, T>(s, g, io, parts);
+    else if constexpr (KIND != OT_GRAM_PART) ot_gemm_of<KIND, LIMBS, 4, T>(s, g, io, parts);
 }
 
 template <typename T, int LIMBS>
 void ot_steps(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, uint8_t* work, const OtPlan& p) {
     uint8_t *x = work + p.x0, *y = work + p.x1, *a = work + p.a, *q = work + p.q;
     const int wn = p.n_pad / 64, wm = p.m_pad / 64, kn = (p.n + 63) / 64, km = (p.m + 63) / 64;
-    const int st = (p.n + 128 * p.sym_ctas - 1) / (128 * p.sym_ctas), rt = (p.n + 128 * p.all_ctas - 1) / (128 * p.all_ctas), ct = (p.m + 128 * p.all_ctas - 1) / (128 * p.all_ctas);
+    const int sym_rows = p.sym == 4 ? 256 : 128, all_rows = p.all == 4 ? 256 : 128;
+    const int st = (p.n + sym_rows - 1) / sym_rows, rt = (p.n + all_rows - 1) / all_rows, ct = (p.m + all_rows - 1) / all_rows * (p.all == 1 ? 2 : 1);
     float* part = reinterpret_cast<float*>(work + p.part);
     for (int k = 0; k < poly.steps; ++k) {
         const OtGemm gram = {x, x, a, p.x_limb, p.x_limb, p.a_limb, wm, wm, wn, km, st, st, 0.f, 0.f, 0.f, part};
         const OtGemm square = {a, a, q, p.a_limb, p.a_limb, p.a_limb, wn, wn, wn, kn, st, st, poly.a, poly.b, poly.c, nullptr};
         const OtGemm apply = {q, x, y, p.a_limb, p.x_limb, p.x_limb, wn, wm, wm, kn, rt, ct, 0.f, 0.f, 0.f, nullptr};
         if (p.parts > 1) {
-            ot_gemm<OT_GRAM_PART, LIMBS, 1, float>(s, gram, io, p.parts);
+            ot_gemm<OT_GRAM_PART, LIMBS, float>(s, gram, io, p.sym, p.parts);
             op_launch_next(s, dim3((unsigned)(st * (st + 1) / 2 * 16), 1, (unsigned)io.batch), dim3(256), 0, k_orth_join<LIMBS>, part, p.parts, a, p.a_limb, wn);
-        } else if (p.sym_ctas == 2) {
-            ot_gemm<OT_GRAM, LIMBS, 2, float>(s, gram, io);
         } else {
-            ot_gemm<OT_GRAM, LIMBS, 1, float>(s, gram, io);
+            ot_gemm<OT_GRAM, LIMBS, float>(s, gram, io, p.sym);
         }
-        if (p.sym_ctas == 2) ot_gemm<OT_SQUARE, LIMBS, 2, float>(s, square, io); else ot_gemm<OT_SQUARE, LIMBS, 1, float>(s, square, io);
-        if (k + 1 < poly.steps) {
-            if (p.all_ctas == 2) ot_gemm<OT_APPLY, LIMBS, 2, float>(s, apply, io); else ot_gemm<OT_APPLY, LIMBS, 1, float>(s, apply, io);
-        } else {
-            if (p.all_ctas == 2) ot_gemm<OT_LAST, LIMBS, 2, T>(s, apply, io); else ot_gemm<OT_LAST, LIMBS, 1, T>(s, apply, io);
-        }
+        ot_gemm<OT_SQUARE, LIMBS, float>(s, square, io, p.sym);
+        if (k + 1 < poly.steps) ot_gemm<OT_APPLY, LIMBS, float>(s, apply, io, p.all);
+        else ot_gemm<OT_LAST, LIMBS, T>(s, apply, io, p.all);
         uint8_t* z = x;
         x = y;
         y = z;
