@@ -234,8 +234,8 @@ k_norm_forward_down(const T* x, int64_t x_stride, const float* __restrict__ weig
 // rows longer than NORM_REG_N: a block per row, three passes over it
 template <typename T>
 __global__ void __launch_bounds__(1024)
-k_norm_forward_long(const T* __restrict__ x, int64_t x_stride, const float* __restrict__ weight, const float* __restrict__ bias, float eps, int n,
-                    T* __restrict__ y, int64_t y_stride, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+k_norm_forward_long(const T* x, int64_t x_stride, const float* __restrict__ weight, const float* __restrict__ bias, float eps, int n,
+                    T* y, int64_t y_stride, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
     __shared__ float s_sum[2][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = blockIdx.x;
@@ -408,8 +408,8 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
 // rows longer than NORM_REG_N_BACK: dx by a block per row, then the columns' sums by threads that walk down stripes of rows
 template <typename T>
 __global__ void __launch_bounds__(1024)
-k_norm_backward_long(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x, int64_t x_stride, const float* __restrict__ mean,
-                     const float* __restrict__ rstd, const float* __restrict__ weight, int n, T* __restrict__ dx, int64_t dx_stride) {
+k_norm_backward_long(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, const float* __restrict__ mean,
+                     const float* __restrict__ rstd, const float* __restrict__ weight, int n, T* dx, int64_t dx_stride) {
     __shared__ float s_sum[2][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = blockIdx.x;
@@ -442,7 +442,6 @@ k_norm_columns_long(const T* __restrict__ dy, int64_t dy_stride, const T* __rest
     }
     partial[(int64_t)blockIdx.y * n + col] = aw;
     partial[(int64_t)(gridDim.y + blockIdx.y) * n + col] = ab;
-    op_next_may_start();
 }
 
 // dweight and dbias from the blocks' rows: eight columns (a 32-byte sector) per block; thread group r of 128 adds the rows r, r + 128, .., the four
@@ -561,9 +560,10 @@ void norm_backward_go(const NormBackward& a) {
 template <typename T, int VEC>
 void norm_backward_pick(const NormBackward& a) {
     if (a.n > NORM_REG_N_BACK) {
-        k_norm_backward_long<T><<<(unsigned)a.rows, 1024, 0, a.s>>>((const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.w, a.n, (T*)a.dx, a.dxs);
+        // the columns first: dx may be dy's or x's memory
         if (a.partial)
             k_norm_columns_long<T><<<dim3((unsigned)ceil_div(a.n, 256), (unsigned)a.blocks), 256, 0, a.s>>>((const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.rows, a.n, a.partial);
+        k_norm_backward_long<T><<<(unsigned)a.rows, 1024, 0, a.s>>>((const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.w, a.n, (T*)a.dx, a.dxs);
     } else if (a.n <= 64) {
         norm_backward_go<T, VEC, 1, 8, 8, 2>(a);
     } else if (a.n <= 128) {
@@ -593,6 +593,7 @@ extern "C" int tb_layer_norm_forward(const void* d_x, int64_t x_stride, const fl
     if (!d_x || !d_y) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_x or d_y is NULL");
     if (rows > 1 && (x_stride < n || y_stride < n)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "row strides must be at least n");
     if (((uintptr_t)d_x | (uintptr_t)d_y) % size || ((uintptr_t)d_weight | (uintptr_t)d_bias) & 3) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
+    if (!op_apart(d_x, 0, x_stride, d_y, 0, y_stride, 1, rows, n, size)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_y overlaps d_x in part");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = n % (16 / size) == 0 && norm_aligned(d_x, x_stride, size) && norm_aligned(d_y, y_stride, size) && (((uintptr_t)d_weight | (uintptr_t)d_bias) & 15) == 0;
     const NormForward a = {s, d_x, x_stride, d_weight, d_bias, eps, rows, n, d_y, y_stride, d_mean, d_rstd};
@@ -617,6 +618,8 @@ extern "C" int tb_layer_norm_backward(const void* d_dy, int64_t dy_stride, const
     if (rows > 0 && (!d_dy || !d_x || !d_mean || !d_rstd || !d_dx)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "a device pointer is NULL");
     if (rows > 1 && (dy_stride < n || x_stride < n || dx_stride < n)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "row strides must be at least n");
     if (((uintptr_t)d_dy | (uintptr_t)d_x | (uintptr_t)d_dx) % size || ((uintptr_t)d_weight & 3)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "rows must be aligned to their elements");
+    if (rows > 0 && (!op_apart(d_dy, 0, dy_stride, d_dx, 0, dx_stride, 1, rows, n, size) || !op_apart(d_x, 0, x_stride, d_dx, 0, dx_stride, 1, rows, n, size)))
+        return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_dx overlaps d_dy or d_x in part");
     const bool columns = d_dweight || d_dbias;
     if (columns && (!d_work || work_bytes < tb_layer_norm_backward_workspace(rows, n) || ((uintptr_t)d_work & 31)))
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "the workspace must be aligned and hold %lld bytes (got %lld)",

@@ -94,6 +94,23 @@ static inline void op_launch_next(cudaStream_t s, dim3 grid, dim3 block, size_t 
 
 static inline int op_type_size(int type) { return type == TB_TYPE_F32 ? 4 : type == TB_TYPE_F16 || type == TB_TYPE_BF16 ? 2 : 0; }
 
+// Whether a result may be written while an input of the same shape is read: both are the same memory, element by element, or have no element in
+// common.  (Rows are taken in any order and a row is read before it is written, so anything between gives results that depend on the order.)
+static inline bool op_apart(const void* in, int64_t in_batch, int64_t in_stride, const void* out, int64_t out_batch, int64_t out_stride, int64_t batch, int64_t rows, int64_t n, int size) {
+    if (rows == 1) in_stride = out_stride = batch > 1 ? 0 : n;
+    if (batch == 1) in_batch = out_batch = 0;
+    const auto bytes = [=](int64_t b, int64_t r) { return (uintptr_t)((batch - 1) * b + (rows - 1) * r + n) * size; };
+    const uintptr_t a = (uintptr_t)in, b = (uintptr_t)out;
+    if (a + bytes(in_batch, in_stride) <= b || b + bytes(out_batch, out_stride) <= a) return true;
+    if (in_stride != out_stride || in_batch != out_batch) return false;
+    if (a == b) return true;
+    // the same pitch: other columns of the same rows
+    const int64_t pitch = rows == 1 ? in_batch : in_stride, d = (int64_t)(b - a);
+    if (pitch == 0 || in_batch % pitch || d % size) return false;
+    const int64_t at = ((d / size) % pitch + pitch) % pitch;
+    return at >= n && pitch - at >= n;
+}
+
 #if defined(__GNUC__)
 __attribute__((format(printf, 4, 5)))
 #endif

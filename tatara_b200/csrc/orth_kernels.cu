@@ -386,6 +386,7 @@ extern "C" int tb_orthogonalise(const void* d_x, int64_t x_batch, int64_t x_stri
     if (rows > 1 && (x_stride < cols || out_stride < cols)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "row strides must be at least cols");
     if (batch > 1 && (x_batch < (rows - 1) * x_stride + cols || out_batch < (rows - 1) * out_stride + cols))
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "matrices of the batch overlap");
+    if (!op_apart(d_x, x_batch, x_stride, d_out, out_batch, out_stride, batch, rows, cols, op_type_size(type))) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_out overlaps d_x in part");
     OrthIo io = {};
     io.g = d_x;
     io.g_batch = x_batch;

@@ -556,7 +556,8 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
             }
 
             if (KIND == OT_GRAM_PART) {
-                const int whole = W == 1 ? t / tiles * (tiles / 2) + at.i * (at.i + 1) / 2 + (at.j >> 1) : t, from = W == 1 ? (at.j & 1) * 64 : 0;  // of the 128 x 128 tiles
+                static_assert(KIND != OT_GRAM_PART || W == 1, "parts are of tiles of 64 columns");
+                const int whole = at.batch * (tiles / 2) + at.i * (at.i + 1) / 2 + (at.j >> 1), from = (at.j & 1) * 64;  // in the 128 x 128 tiles
                 float4* to = reinterpret_cast<float4*>(g.part) + ((int64_t)whole * gridDim.y + blockIdx.y) * 4096 + row;
 #pragma unroll
                 for (int c = 0; c < COLS; c += 4) to[(from + group * COLS + c) / 4 * 128] = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
@@ -804,11 +805,11 @@ OtPlan ot_plan(int batch, int rows, int cols, int limbs) {
     // few tiles with a long K are cut into parts where that saves more than the launch that joins them
     p.parts = 1;
     const int64_t s1 = batch * n1 * (n1 + 1) / 2;
-    if (p.sym < 4) {
-        int64_t q = sm_count() / (s1 * (p.sym == 1 ? 2 : 1));
+    if (p.sym == 1) {  // room for another part of 128 x 128 tiles is room for tiles of half the size
+        int64_t q = sm_count() / (2 * s1);
         q = q < OT_PARTS ? q : OT_PARTS;
         q = q < km / 4 ? q : km / 4;
-        if (q > 1 && (km - km / q) * ot_chunk(limbs, p.sym) > 9000) p.parts = (int)q;
+        if (q > 1 && (km - km / q) * ot_chunk(limbs, 1) > 9000) p.parts = (int)q;
     }
     const int pad = p.sym == 4 || p.all == 4 ? 256 : 128;
     p.n_pad = (p.n + pad - 1) / pad * pad;
@@ -864,9 +865,10 @@ void ot_gemm_of(cudaStream_t s, const OtGemm& g, const OrthIo& io, int parts) {
 }
 template <int KIND, int LIMBS, typename T>
 void ot_gemm(cudaStream_t s, const OtGemm& g, const OrthIo& io, int w, int parts = 1) {
-    if (w == 1) ot_gemm_of<KIND, LIMBS, 1, T>(s, g, io, parts);
+    if constexpr (KIND == OT_GRAM_PART) return ot_gemm_of<KIND, LIMBS, 1, T>(s, g, io, parts);
+    else if (w == 1) ot_gemm_of<KIND, LIMBS, 1, T>(s, g, io, parts);
     else if (w == 2) ot_gemm_of<KIND, LIMBS, 2, T>(s, g, io, parts);
-    else if constexpr (KIND != OT_GRAM_PART) ot_gemm_of<KIND, LIMBS, 4, T>(s, g, io, parts);
+    else ot_gemm_of<KIND, LIMBS, 4, T>(s, g, io, parts);
 }
 
 template <typename T, int LIMBS>

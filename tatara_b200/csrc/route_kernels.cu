@@ -481,7 +481,7 @@ int route_check(int type, int64_t rows, int experts, int k, const void* logits, 
     if (!size) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "type must be TB_TYPE_F32, TB_TYPE_F16 or TB_TYPE_BF16 (got %d)", type);
     if (experts < 1 || experts > ROUTE_MAX_E) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "experts must be in [1, %d] (got %d)", ROUTE_MAX_E, experts);
     if (k < 1 || k > experts || k > ROUTE_MAX_K) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "k must be in [1, min(experts, %d)] (got %d)", ROUTE_MAX_K, k);
-    if (rows < 0 || rows * k > INT32_MAX) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "rows must not be negative and rows * k below 2^31");
+    if (rows < 0 || rows > INT32_MAX || rows * k > INT32_MAX) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "rows must not be negative and rows * k below 2^31");
     if (rows > 0 && !logits) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_logits is NULL");
     if (rows > 1 && stride < experts) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "the row stride must be at least experts");
     if ((uintptr_t)logits % size) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_logits must be aligned to its elements");
@@ -534,6 +534,7 @@ extern "C" int tb_route_backward(const void* d_logits, int64_t stride, int type,
     if (!d_index || !d_gate || !d_counts || !d_rows || !d_dlogits) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "a device pointer is NULL");
     if (rows > 1 && dstride < experts) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "the row stride must be at least experts");
     if ((uintptr_t)d_dlogits % op_type_size(type)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_dlogits must be aligned to its elements");
+    if (!op_apart(d_logits, 0, stride, d_dlogits, 0, dstride, 1, rows, experts, op_type_size(type))) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_dlogits overlaps d_logits in part");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = route_wide(d_logits, stride, experts, op_type_size(type)) && route_wide(d_dlogits, dstride, experts, op_type_size(type));
 #define ARGS s, d_logits, stride, d_mask, rows, experts, k, renormalise, d_index, d_gate, d_dgate, d_counts, d_rows, d_dlosses, d_dlogits, dstride, wide

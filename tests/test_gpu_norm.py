@@ -116,6 +116,50 @@ def test_no_rows():
     assert y.shape == dx.shape == (0, 40) and (dw == 0).all() and (db == 0).all()
 
 
+@pytest.mark.parametrize("n", [100, 1000, 1001, 5000, 9001, 20000])
+def test_in_place_at_every_length(n):
+    x, dy = make(40, n, torch.float32, 31), make(40, n, torch.float32, 32)
+    w = 1 + 0.2 * torch.randn(n, device="cuda")
+    y, mean, rstd = ops().layer_norm_forward(x, w, eps=EPS)
+    want = ops().layer_norm_backward(dy, x, mean, rstd, w)
+    z = x.clone()
+    assert torch.equal(ops().layer_norm_forward(z, w, eps=EPS, out=z)[0], y)
+    for same in ("dy", "x"):
+        t = {"dy": dy.clone(), "x": x.clone()}
+        got = ops().layer_norm_backward(t["dy"], t["x"], mean, rstd, w, out=t[same])
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), same
+
+
+def test_outputs_beside_and_over_the_inputs():
+    n = 24
+    wide = make(50, 2 * n + 3, torch.float32, 33)
+    x, dy = wide[:, :n].clone(), make(50, n, torch.float32, 34)
+    y, mean, rstd = ops().layer_norm_forward(wide[:, :n], eps=EPS)   # strides decide the order of a row's sum
+    assert torch.equal(ops().layer_norm_forward(wide[:, :n], eps=EPS, out=wide[:, n:2 * n])[0], y)   # other columns of the same rows
+    rows = torch.cat([x, x])
+    assert torch.equal(ops().layer_norm_forward(rows[::2], eps=EPS, out=rows[1::2])[0], ops().layer_norm_forward(torch.cat([x, x])[::2].clone(), eps=EPS)[0])
+    with pytest.raises(tb.TrainerError, match="overlaps"):
+        ops().layer_norm_forward(wide[:, :n], eps=EPS, out=wide[:, 1:n + 1])
+    with pytest.raises(tb.TrainerError, match="overlaps"):
+        ops().layer_norm_backward(dy, wide[:, :n], mean, rstd, out=wide[:, 1:n + 1])
+    with pytest.raises(tb.TrainerError, match="overlaps"):
+        ops().layer_norm_forward(rows[:50], eps=EPS, out=rows[1:51])
+    with pytest.raises(tb.TrainerError, match="overlaps"):
+        ops().layer_norm_backward(rows[:50], x, mean, rstd, out=rows[1:51])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [127, 128, 129, 255, 257, 511, 769, 1175, 2561, 3071, 3073, 4095, 4097, 8191])
+def test_columns_around_the_kernels_bounds(n, dtype):
+    rows = 37
+    for offset in (0, 1):
+        x, dy = make(rows, n, dtype, n, True, offset), make(rows, n, dtype, n + 1, False, offset)
+        w, b = 1 + 0.2 * torch.randn(n, device="cuda"), torch.randn(n, device="cuda")
+        got = ops().layer_norm_forward(x, w, b, eps=EPS)
+        check_forward(x, w, b, got)
+        check_backward(dy, x, got[1], got[2], w, ops().layer_norm_backward(dy, x, got[1], got[2], w))
+
+
 @pytest.mark.parametrize("rows,n", [(6, 33), (4, 512)])
 def test_gradient_against_differences(rows, n):
     x, dy = make(rows, n, torch.float32, 21), make(rows, n, torch.float32, 22)

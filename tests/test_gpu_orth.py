@@ -163,6 +163,30 @@ def test_matrices_far_apart(rows, cols):
     assert torch.equal(ops().orthogonalise(x, out=x), want) and (wide[rows * cols:far] == 0).all()
 
 
+@pytest.mark.parametrize("rows,cols", [(12, 40), (70, 90)])
+def test_outputs_that_overlap_the_input_in_part(rows, cols):
+    x = make(3, rows, cols, 5)
+    flat = torch.cat([x.flatten(), torch.zeros(rows * cols, device="cuda")])
+    want = ops().orthogonalise(x)
+    with pytest.raises(tb.TrainerError, match="overlaps"):
+        ops().orthogonalise(flat[:x.numel()].view_as(x), out=flat[rows * cols:].view_as(x))
+    wide = torch.zeros(3, rows, 2 * cols, device="cuda")
+    wide[:, :, :cols] = x
+    with pytest.raises(tb.TrainerError, match="overlaps"):
+        ops().orthogonalise(wide[:, :, :cols], out=wide[:, :, 3:3 + cols])
+    # other columns of the same rows
+    assert torch.equal(ops().orthogonalise(wide[:, :, :cols], out=wide[:, :, cols:]), ops().orthogonalise(wide[:, :, :cols]))
+    assert float((wide[:, :, cols:] - want).abs().max()) <= 1e-4
+
+
+# tiles of 64, 128 and 256 columns, K in parts and whole, several matrices; every layout of the result
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch,rows,cols", [(1, 130, 4096), (2, 130, 1500), (1, 359, 785), (1, 785, 360), (3, 500, 304), (7, 66, 128), (1, 1024, 1024), (20, 65, 129), (1, 1500, 1100)])
+def test_orthogonalise_in_every_tile_shape(batch, rows, cols, dtype):
+    x = make(batch, rows, cols, batch + rows + cols, dtype)
+    assert far(ops().orthogonalise(x), orthogonalise(x)) <= tolerance(dtype, rows, cols)
+
+
 def test_refusals():
     o = ops()
     x = make(2, 70, 80, 0)

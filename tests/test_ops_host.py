@@ -51,6 +51,29 @@ def test_layer_norm_arguments():
     assert lib().tb_layer_norm_forward(None, 8, None, None, 1e-5, 0, 4, 8, P, 8, None, None, None, None, 0) == INVALID   # no text wanted
 
 
+def test_results_that_overlap_an_input_in_part():
+    f = lambda x, xs, y, ys, rows=4: lib().tb_layer_norm_forward(x, xs, None, None, 1e-5, 0, rows, 8, y, ys, None, None, None, e, 200)  # noqa: E731
+    for x, xs, y, ys in ((P, 8, P + 4, 8), (P, 8, P + 32, 8), (P + 96, 8, P, 8), (P, 16, P + 28, 16), (P, 16, P + 36, 16), (P, 8, P, 16), (P, 16, P + 32, 8)):
+        e = err()
+        assert f(x, xs, y, ys) == INVALID and b"overlaps" in e.value, (x, xs, y, ys)
+    if no_gpu():  # the same memory, memory that follows, other columns of the same rows, rows in between
+        for x, xs, y, ys in ((P, 8, P, 8), (P, 8, P + 128, 8), (P + 128, 8, P, 8), (P, 16, P + 32, 16), (P + 32, 16, P, 16), (P, 24, P + 40, 24), (P, 9, P + 4 * 35, 16)):
+            e = err()
+            assert f(x, xs, y, ys) == NO_DEVICE, (x, xs, y, ys, e.value)
+        assert f(P, 8, P, 16, rows=1) == NO_DEVICE
+    need = lib().tb_layer_norm_backward_workspace(4, 8)
+    g = lambda dy, x, dx: lib().tb_layer_norm_backward(dy, 8, x, 8, P, P, None, 0, 4, 8, dx, 8, None, None, P, need, None, e, 200)  # noqa: E731
+    for args in ((P, P + 4096, P + 4), (P + 4096, P, P + 64)):
+        e = err()
+        assert g(*args) == INVALID and b"overlaps" in e.value
+    e = err()
+    assert lib().tb_route_backward(P, 9, 0, 100, 9, 2, 1, None, P, P, P, P, P, P, P + 4, 9, None, e, 200) == INVALID and b"overlaps" in e.value
+    h = lambda x, xb, out, ob, b=2: lib().tb_orthogonalise(x, xb, 8, 0, b, 4, 8, 5, COEF, 1e-7, out, ob, 8, None, 0, None, e, 200)  # noqa: E731
+    for args in ((P, 32, P + 4, 32), (P, 32, P + 128, 32), (P, 32, P, 64)):
+        e = err()
+        assert h(*args) == INVALID and b"overlaps" in e.value, args
+
+
 def test_route_arguments():
     need = lib().tb_route_forward_workspace(100, 9)
     assert need > 0 and lib().tb_route_forward_workspace(0, 1) > 0
