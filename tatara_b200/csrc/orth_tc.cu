@@ -116,33 +116,40 @@ __device__ __forceinline__ void ot_split(float x, __half (&h)[LIMBS]) {
     h[0] = __float2half_rn(x);
     if (LIMBS == 2) h[LIMBS - 1] = __float2half_rn(x - __half2float(h[0]));
 }
+// ... of two neighbours, as they lie in a tile
+template <int LIMBS>
+__device__ __forceinline__ void ot_split(float x, float y, __half2 (&h)[LIMBS]) {
+    h[0] = __floats2half2_rn(x, y);
+    if (LIMBS == 2) {
+        const float2 high = __half22float2(h[0]);
+        h[LIMBS - 1] = __floats2half2_rn(x - high.x, y - high.y);
+    }
+}
 // byte offset of element (row, col) in a 128 x 64 tile
 __device__ __forceinline__ int ot_at(int row, int col) { return row * 128 + ((((col >> 3) ^ row) & 7) << 4) + (col & 7) * 2; }
 
 // ---- the norm and the tiles of the first X ----------------------------------------------------------------------------
-// N adjacent elements of u at (r, c), the momentum's update included in the FIRST pass; the loads of the gradient and of the momentum are
+// N adjacent elements of u, the momentum's update included in the FIRST pass; the loads of the gradient and of the momentum (NULL: none) are
 // separate from what follows them so that a caller can issue several
 template <typename T, int N>
 struct OtPiece {
     OpRaw<T, N> g;
     float m[N];
-    int64_t at;
-    __device__ __forceinline__ void load(const OrthIo& io, const float* momentum, int b, int64_t r, int64_t c) {
-        g.load(static_cast<const T*>(io.g) + b * io.g_batch + r * io.g_stride + c);
-        if (io.m) {
-            at = ((int64_t)b * io.rows + r) * io.cols + c;
+    __device__ __forceinline__ void load(const T* from, const float* momentum) {
+        g.load(from);
+        if (momentum) {
             constexpr int STEP = N < 4 ? N : 4;
 #pragma unroll
             for (int i = 0; i < N; i += STEP) {
                 float t[STEP];
-                op_load<float, STEP>(momentum + at + i, t);
+                op_load<float, STEP>(momentum + i, t);
 #pragma unroll
                 for (int k = 0; k < STEP; ++k) m[i + k] = t[k];
             }
         }
     }
     template <bool FIRST>
-    __device__ __forceinline__ void finish(const OrthIo& io, float (&u)[N]) {
+    __device__ __forceinline__ void finish(const OrthIo& io, float (&u)[N], float* momentum = nullptr) {
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = g.get(i);
         if (!io.m) return;
@@ -155,7 +162,7 @@ struct OtPiece {
                 float t[STEP];
 #pragma unroll
                 for (int k = 0; k < STEP; ++k) t[k] = m[i + k];
-                op_store<float, STEP>(io.m_out + at + i, t);
+                op_store<float, STEP>(momentum + i, t);
             }
         }
 #pragma unroll
@@ -172,16 +179,19 @@ __global__ void __launch_bounds__(256) k_orth_norm(OrthIo io, int64_t segments, 
     double sum = 0.0;
     for (int64_t seg = blockIdx.x; seg < segments; seg += gridDim.x) {
         const int64_t r = total ? 0 : seg, c0 = total ? seg * len : 0, end = total ? min(total, c0 + len) : len;
+        const T* g = static_cast<const T*>(io.g) + b * io.g_batch + r * io.g_stride;
+        const int64_t at = ((int64_t)b * io.rows + r) * io.cols;
+        const float* m = io.m ? io.m + at : nullptr;
         for (int64_t c = c0 + threadIdx.x * N; c < end; c += 256 * 16) {
             OtPiece<T, N> piece[16 / N];
 #pragma unroll
             for (int q = 0; q < 16 / N; ++q)
-                if (c + q * 256 * N < end) piece[q].load(io, io.m, b, r, c + q * 256 * N);
+                if (c + q * 256 * N < end) piece[q].load(g + c + q * 256 * N, m ? m + c + q * 256 * N : nullptr);
 #pragma unroll
             for (int q = 0; q < 16 / N; ++q)
                 if (c + q * 256 * N < end) {
                     float u[N];
-                    piece[q].template finish<true>(io, u);
+                    piece[q].template finish<true>(io, u, io.m_out + at + c + q * 256 * N);
 #pragma unroll
                     for (int i = 0; i < N; ++i) sum = fma((double)u[i], (double)u[i], sum);
                 }
@@ -217,43 +227,57 @@ __global__ void __launch_bounds__(256) k_orth_pack(OrthIo io, float eps, const d
     uint8_t* to = x + (int64_t)b * LIMBS * limb_bytes + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * OT_TILE;
     constexpr int P = 8 / N, PIECES = 4;  // accesses of a piece, pieces of a thread
     OtPiece<T, N> piece[PIECES][P];
+    // piece k: rows 32 k below the first one's, or columns 16 k beside
+    const int i = TALL ? threadIdx.x & 127 : threadIdx.x >> 3, j = TALL ? threadIdx.x >> 7 << 3 : (threadIdx.x & 7) << 3;
+    const int64_t r = TALL ? j0 + j : i0 + i, c = TALL ? i0 + i : j0 + j;
+    const T* g = static_cast<const T*>(io.g) + b * io.g_batch + r * io.g_stride + c;
+    const float* mo = io.m ? io.m_out + ((int64_t)b * io.rows + r) * io.cols + c : nullptr;
+    const int left = TALL ? (i0 + i < n ? m - j0 - j : 0) : m - j0 - j;  // columns of X from the first element on
 #pragma unroll
-    for (int k = 0; k < PIECES; ++k) {
-        const int e = threadIdx.x + 256 * k, i = TALL ? e % 128 : e / 8, j = TALL ? e / 128 * 8 : e % 8 * 8;
+    for (int k = 0; k < PIECES; ++k)
 #pragma unroll
-        for (int q = 0; q < P; ++q)
-            if (i0 + i < n && j0 + j + q * N < m) piece[k][q].load(io, io.m_out, b, TALL ? j0 + j + q : i0 + i, TALL ? i0 + i : j0 + j + q * N);
-    }
+        for (int q = 0; q < P; ++q) {
+            const bool in = TALL ? 16 * k + q < left : i0 + i + 32 * k < n && q * N < left;
+            if (in) piece[k][q].load(g, mo);
+            if (TALL) {  // one row of u after the other
+                const int64_t step = q < 7 ? 1 : 9;
+                g += step * io.g_stride;
+                if (mo) mo += step * io.cols;
+            } else {
+                const bool next = q == P - 1;
+                g += next ? 32 * io.g_stride - (P - 1) * N : N;
+                if (mo) mo += next ? 32 * (int64_t)io.cols - (P - 1) * N : N;
+            }
+        }
     __syncthreads();
     v = s_part[0];
 #pragma unroll
     for (int w = 1; w < 8; ++w) v += s_part[w];
-    const double inv = (double)OT_SCALE / (sqrt(v) + (double)eps);
+    const float inv = (float)((double)OT_SCALE / (sqrt(v) + (double)eps));  // one more rounding of 2^-24
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
-        const int e = threadIdx.x + 256 * k, i = TALL ? e % 128 : e / 8, j = TALL ? e / 128 * 8 : e % 8 * 8;
-        OpVec<__half, 8> out[LIMBS];
+        float u[8];
 #pragma unroll
         for (int q = 0; q < P; ++q) {
-            float u[N];
+            float t[N];
 #pragma unroll
-            for (int c = 0; c < N; ++c) u[c] = 0.0f;
-            if (i0 + i < n && j0 + j + q * N < m) {
-                piece[k][q].template finish<false>(io, u);
+            for (int e = 0; e < N; ++e) t[e] = 0.0f;
+            if (TALL ? 16 * k + q < left : i0 + i + 32 * k < n && q * N < left) piece[k][q].template finish<false>(io, t);
 #pragma unroll
-                for (int c = 0; c < N; ++c) u[c] = (float)((double)u[c] * inv);
-            }
+            for (int e = 0; e < N; ++e) u[q * N + e] = t[e] * inv;
+        }
+        unsigned out[LIMBS][4];
 #pragma unroll
-            for (int c = 0; c < N; ++c) {
-                __half h[LIMBS];
-                ot_split<LIMBS>(u[c], h);
+        for (int e = 0; e < 4; ++e) {
+            __half2 h[LIMBS];
+            ot_split<LIMBS>(u[2 * e], u[2 * e + 1], h);
 #pragma unroll
-                for (int l = 0; l < LIMBS; ++l) out[l].v[q * N + c] = h[l];
-            }
+            for (int l = 0; l < LIMBS; ++l) out[l][e] = *reinterpret_cast<const unsigned*>(&h[l]);
         }
 #pragma unroll
         for (int l = 0; l < LIMBS; ++l)
-            *reinterpret_cast<OpVec<__half, 8>*>((TALL ? &s_tile[l][0] : to + l * limb_bytes) + ot_at(i, j)) = out[l];
+            *reinterpret_cast<uint4*>((TALL ? &s_tile[l][0] : to + l * limb_bytes) + ot_at(TALL ? i : i + 32 * k, TALL ? j + 16 * k : j)) =
+                make_uint4(out[l][0], out[l][1], out[l][2], out[l][3]);
     }
     if (TALL) {
         __syncthreads();
@@ -561,6 +585,21 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                 float4* to = reinterpret_cast<float4*>(g.part) + ((int64_t)whole * gridDim.y + blockIdx.y) * 4096 + row;
 #pragma unroll
                 for (int c = 0; c < COLS; c += 4) to[(from + group * COLS + c) / 4 * 128] = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+            } else if (KIND == OT_LAST && MULTI && io.rows > io.cols) {
+                // rows of X are columns of the result: a warp's lanes are neighbours there.  Eight old weights on their way
+                const int i = (at.i * CTAS + rank) * 128 + row, j0 = (at.j * 2 + group) * COLS, left = io.rows - j0;
+                int64_t to = at.batch * io.out_batch + j0 * io.out_stride + i;
+                if (i < io.cols)
+#pragma unroll
+                    for (int c0 = 0; c0 < COLS; c0 += 8, to += 8 * io.out_stride) {
+                        if (c0 >= left) break;
+                        float w[8];
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) w[c] = io.m && c0 + c < left ? io.w[to + c * io.out_stride] : 0.0f;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            if (c0 + c < left) orth_store<T>(io, to + c * io.out_stride, w[c], acc[c0 + c] * OT_UNSCALE);
+                    }
             } else if (KIND == OT_LAST && MULTI) {
                 // rows on 16-byte boundaries go out straight from the registers, eight elements at a time
                 const int i = (at.i * CTAS + rank) * 128 + row, j0 = (at.j * 2 + group) * COLS;
@@ -595,10 +634,8 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                         }
                     }
             } else if (KIND == OT_LAST) {
-                // rows that start anywhere, or are columns: by rounds of 64 (W = 1: 32) columns through shared memory (a block has one tile, its ring is free by now)
+                // rows that start anywhere: by rounds of 64 (W = 1: 32) columns through shared memory (a block has one tile, its ring is free by now)
                 float* flat = reinterpret_cast<float*>(s_dyn + group * 40960);  // [128][65]
-                const bool tall = io.rows > io.cols;
-                const int n = tall ? io.cols : io.rows, m = tall ? io.rows : io.cols;
 #pragma unroll
                 for (int h = 0; h < CTAS; ++h) {
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
@@ -606,21 +643,19 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                     for (int c = 0; c < RC; ++c) flat[row * 65 + c] = acc[RC * h + c] * OT_UNSCALE;
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
                     const int i0 = (at.i * CTAS + rank) * 128, j0 = W == 1 ? at.j * 64 + group * 32 : (at.j * 2 * CTAS + group * CTAS + h) * 64;
-                    // 128 (64, 32) neighbours in memory at a time, eight of a thread's old weights on their way.  A thread's elements lie `next` apart
+                    // 64 (32) neighbours of two (four) rows at a time, eight of a thread's old weights on their way
                     constexpr int AT_ONCE = 128 / RC;
                     const int r = row / RC, c = row % RC;
-                    const int64_t to = at.batch * io.out_batch + (tall ? (int64_t)j0 * io.out_stride + i0 + row : (int64_t)(i0 + r) * io.out_stride + j0 + c);
-                    const int64_t next = tall ? io.out_stride : AT_ONCE * io.out_stride;
-                    const int left = tall ? (i0 + row < n ? m - j0 : 0) : (j0 + c < m ? (n - i0 - r + AT_ONCE - 1) / AT_ONCE : 0);
-                    const float* from = tall ? flat + row * 65 : flat + r * 65 + c;
-                    const int jump = tall ? 1 : 65 * AT_ONCE;
+                    const int64_t to = at.batch * io.out_batch + (i0 + r) * io.out_stride + j0 + c, next = AT_ONCE * io.out_stride;
+                    const int left = j0 + c < io.cols ? (io.rows - i0 - r + AT_ONCE - 1) / AT_ONCE : 0;
+                    const float* from = flat + r * 65 + c;
                     for (int e0 = 0; e0 < RC && e0 < left; e0 += 8) {
                         float w[8];
 #pragma unroll
                         for (int u = 0; u < 8; ++u) w[u] = io.m && e0 + u < left ? io.w[to + (e0 + u) * next] : 0.0f;
 #pragma unroll
                         for (int u = 0; u < 8; ++u)
-                            if (e0 + u < left) orth_store<T>(io, to + (e0 + u) * next, w[u], from[(e0 + u) * jump]);
+                            if (e0 + u < left) orth_store<T>(io, to + (e0 + u) * next, w[u], from[(e0 + u) * 65 * AT_ONCE]);
                     }
                 }
             } else {
@@ -672,11 +707,7 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
 #pragma unroll
                         for (int c = 0; c < 16; c += 2) {
                             __half2 pair[LIMBS];
-                            pair[0] = __floats2half2_rn(x[c], x[c + 1]);
-                            if (LIMBS == 2) {
-                                const float2 high = __half22float2(pair[0]);
-                                pair[LIMBS - 1] = __floats2half2_rn(x[c] - high.x, x[c + 1] - high.y);
-                            }
+                            ot_split<LIMBS>(x[c], x[c + 1], pair);
 #pragma unroll
                             for (int l = 0; l < LIMBS; ++l) {
                                 piece[l].w[c / 2] = *reinterpret_cast<const unsigned*>(&pair[l]);
@@ -857,7 +888,7 @@ void ot_gemm_of(cudaStream_t s, const OtGemm& g, const OrthIo& io, int parts) {
     const int64_t all = tiles * io.batch, slots = sm_count() / (W == 4 ? 2 : 1);
     if constexpr (KIND == OT_LAST) {  // MULTI: the result can be stored straight from the registers
         const bool aligned = io.cols % 8 == 0 && io.out_stride % 8 == 0 && io.out_batch % 8 == 0 && (((uintptr_t)io.out | (uintptr_t)io.w) & 15) == 0;
-        if (io.rows <= io.cols && aligned) return ot_launch<KIND, LIMBS, W, true, T>(s, g, io, all > slots ? slots : all, parts);
+        if (io.rows > io.cols || aligned) return ot_launch<KIND, LIMBS, W, true, T>(s, g, io, all > slots ? slots : all, parts);
     } else if constexpr (KIND != OT_GRAM_PART && W > 1) {  // tiles of 64 columns are taken where all run at once
         if (all > slots) return ot_launch<KIND, LIMBS, W, true, T>(s, g, io, slots, parts);
     }
