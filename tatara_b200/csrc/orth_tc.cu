@@ -129,15 +129,15 @@ __device__ __forceinline__ void ot_split(float x, float y, __half2 (&h)[LIMBS]) 
 __device__ __forceinline__ int ot_at(int row, int col) { return row * 128 + ((((col >> 3) ^ row) & 7) << 4) + (col & 7) * 2; }
 
 // ---- the norm and the tiles of the first X ----------------------------------------------------------------------------
-// N adjacent elements of u, the momentum's update included in the FIRST pass; the loads of the gradient and of the momentum (NULL: none) are
-// separate from what follows them so that a caller can issue several
-template <typename T, int N>
+// N adjacent elements of u, with MUON the momentum's update included in the FIRST pass; the loads of the gradient and of the momentum are separate from
+// what follows them so that a caller can issue several (a branch on the momentum in front of every load kept them apart and made a third of the instructions)
+template <typename T, int N, bool MUON>
 struct OtPiece {
     OpRaw<T, N> g;
-    float m[N];
+    float m[MUON ? N : 1];
     __device__ __forceinline__ void load(const T* from, const float* momentum) {
         g.load(from);
-        if (momentum) {
+        if constexpr (MUON) {
             constexpr int STEP = N < 4 ? N : 4;
 #pragma unroll
             for (int i = 0; i < N; i += STEP) {
@@ -152,27 +152,28 @@ struct OtPiece {
     __device__ __forceinline__ void finish(const OrthIo& io, float (&u)[N], float* momentum = nullptr) {
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = g.get(i);
-        if (!io.m) return;
-        if (FIRST) {
+        if constexpr (MUON) {
+            if (FIRST) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) m[i] = fmaf(io.beta, m[i], u[i]);
-            constexpr int STEP = N < 4 ? N : 4;
+                for (int i = 0; i < N; ++i) m[i] = fmaf(io.beta, m[i], u[i]);
+                constexpr int STEP = N < 4 ? N : 4;
 #pragma unroll
-            for (int i = 0; i < N; i += STEP) {
-                float t[STEP];
+                for (int i = 0; i < N; i += STEP) {
+                    float t[STEP];
 #pragma unroll
-                for (int k = 0; k < STEP; ++k) t[k] = m[i + k];
-                op_store<float, STEP>(momentum + i, t);
+                    for (int k = 0; k < STEP; ++k) t[k] = m[i + k];
+                    op_store<float, STEP>(momentum + i, t);
+                }
             }
-        }
 #pragma unroll
-        for (int i = 0; i < N; ++i) u[i] = io.nesterov ? fmaf(io.beta, m[i], u[i]) : m[i];
+            for (int i = 0; i < N; ++i) u[i] = io.nesterov ? fmaf(io.beta, m[i], u[i]) : m[i];
+        }
     }
 };
 
 // Sum of squares (64 bits) of a matrix cut into segments of `len` elements (a row, or 4096 of a matrix without gaps), dealt to the blocks; every
 // thread has 16 elements on their way.  64 blocks with one element each took 270 us for 4096 x 4096, 8 times this.
-template <typename T, int N>
+template <typename T, int N, bool MUON>
 __global__ void __launch_bounds__(256) k_orth_norm(OrthIo io, int64_t segments, int64_t len, int64_t total, double* __restrict__ partial) {
     __shared__ double s_sum[8];
     const int b = blockIdx.y;
@@ -181,17 +182,17 @@ __global__ void __launch_bounds__(256) k_orth_norm(OrthIo io, int64_t segments, 
         const int64_t r = total ? 0 : seg, c0 = total ? seg * len : 0, end = total ? min(total, c0 + len) : len;
         const T* g = static_cast<const T*>(io.g) + b * io.g_batch + r * io.g_stride;
         const int64_t at = ((int64_t)b * io.rows + r) * io.cols;
-        const float* m = io.m ? io.m + at : nullptr;
+        const float* m = MUON ? io.m + at : nullptr;
         for (int64_t c = c0 + threadIdx.x * N; c < end; c += 256 * 16) {
-            OtPiece<T, N> piece[16 / N];
+            OtPiece<T, N, MUON> piece[16 / N];
 #pragma unroll
             for (int q = 0; q < 16 / N; ++q)
-                if (c + q * 256 * N < end) piece[q].load(g + c + q * 256 * N, m ? m + c + q * 256 * N : nullptr);
+                if (c + q * 256 * N < end) piece[q].load(g + c + q * 256 * N, MUON ? m + c + q * 256 * N : nullptr);
 #pragma unroll
             for (int q = 0; q < 16 / N; ++q)
                 if (c + q * 256 * N < end) {
                     float u[N];
-                    piece[q].template finish<true>(io, u, io.m_out + at + c + q * 256 * N);
+                    piece[q].template finish<true>(io, u, MUON ? io.m_out + at + c + q * 256 * N : nullptr);
 #pragma unroll
                     for (int i = 0; i < N; ++i) sum = fma((double)u[i], (double)u[i], sum);
                 }
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(256) k_orth_norm(OrthIo io, int64_t segments, 
 
 // One tile per block: X0 = u / (|u| + eps), n x m with n <= m, zeros beyond both.  A thread makes 16-byte pieces of the tile: of N adjacent elements each
 // where rows of u are rows of X, of eight rows of u where they are columns (TALL), through shared memory then.
-template <typename T, int LIMBS, int N, bool TALL>
+template <typename T, int LIMBS, int N, bool TALL, bool MUON>
 __global__ void __launch_bounds__(256) k_orth_pack(OrthIo io, float eps, const double* __restrict__ partial, int n_partial, uint8_t* __restrict__ x, int64_t limb_bytes) {
     __shared__ __align__(128) uint8_t s_tile[TALL ? LIMBS : 1][TALL ? OT_TILE : 16];
     __shared__ double s_part[8];
@@ -226,12 +227,12 @@ __global__ void __launch_bounds__(256) k_orth_pack(OrthIo io, float eps, const d
     const int i0 = blockIdx.y * 128, j0 = blockIdx.x * 64;
     uint8_t* to = x + (int64_t)b * LIMBS * limb_bytes + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * OT_TILE;
     constexpr int P = 8 / N, PIECES = 4;  // accesses of a piece, pieces of a thread
-    OtPiece<T, N> piece[PIECES][P];
+    OtPiece<T, N, MUON> piece[PIECES][P];
     // piece k: rows 32 k below the first one's, or columns 16 k beside
     const int i = TALL ? threadIdx.x & 127 : threadIdx.x >> 3, j = TALL ? threadIdx.x >> 7 << 3 : (threadIdx.x & 7) << 3;
     const int64_t r = TALL ? j0 + j : i0 + i, c = TALL ? i0 + i : j0 + j;
     const T* g = static_cast<const T*>(io.g) + b * io.g_batch + r * io.g_stride + c;
-    const float* mo = io.m ? io.m_out + ((int64_t)b * io.rows + r) * io.cols + c : nullptr;
+    const float* mo = MUON ? io.m_out + ((int64_t)b * io.rows + r) * io.cols + c : nullptr;
     const int left = TALL ? (i0 + i < n ? m - j0 - j : 0) : m - j0 - j;  // columns of X from the first element on
 #pragma unroll
     for (int k = 0; k < PIECES; ++k)
@@ -242,11 +243,11 @@ __global__ void __launch_bounds__(256) k_orth_pack(OrthIo io, float eps, const d
             if (TALL) {  // one row of u after the other
                 const int64_t step = q < 7 ? 1 : 9;
                 g += step * io.g_stride;
-                if (mo) mo += step * io.cols;
+                if (MUON) mo += step * io.cols;
             } else {
                 const bool next = q == P - 1;
                 g += next ? 32 * io.g_stride - (P - 1) * N : N;
-                if (mo) mo += next ? 32 * (int64_t)io.cols - (P - 1) * N : N;
+                if (MUON) mo += next ? 32 * (int64_t)io.cols - (P - 1) * N : N;
             }
         }
     __syncthreads();
@@ -593,12 +594,19 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
 #pragma unroll
                     for (int c0 = 0; c0 < COLS; c0 += 8, to += 8 * io.out_stride) {
                         if (c0 >= left) break;
+                        if (!io.m) {
+                            T* out = static_cast<T*>(io.out) + to;
+#pragma unroll
+                            for (int c = 0; c < 8; ++c, out += io.out_stride)
+                                if (c0 + c < left) *out = op_round<T>(acc[c0 + c] * OT_UNSCALE);
+                            continue;
+                        }
                         float w[8];
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) w[c] = io.m && c0 + c < left ? io.w[to + c * io.out_stride] : 0.0f;
+                        for (int c = 0; c < 8; ++c) w[c] = c0 + c < left ? io.w[to + c * io.out_stride] : 0.0f;
 #pragma unroll
                         for (int c = 0; c < 8; ++c)
-                            if (c0 + c < left) orth_store<T>(io, to + c * io.out_stride, w[c], acc[c0 + c] * OT_UNSCALE);
+                            if (c0 + c < left) static_cast<float*>(io.out)[to + c * io.out_stride] = orth_update(io, w[c], acc[c0 + c] * OT_UNSCALE);
                     }
             } else if (KIND == OT_LAST && MULTI) {
                 // rows on 16-byte boundaries go out straight from the registers, eight elements at a time
@@ -929,8 +937,8 @@ void ot_steps(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, uint8_t* w
 }
 
 // the norm and the tiles of X0; N: adjacent elements per access
-template <typename T, int LIMBS, int N>
-void ot_begin(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, const OtPlan& p, double* partial, uint8_t* x) {
+template <typename T, int LIMBS, int N, bool MUON>
+void ot_begin_of(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, const OtPlan& p, double* partial, uint8_t* x) {
     const bool gaps = io.g_stride != io.cols;
     const int64_t total = gaps ? 0 : (int64_t)io.rows * io.cols, len = gaps ? io.cols : 4096, segments = gaps ? io.rows : (total + 4095) / 4096;
     int64_t most = 8 * (int64_t)sm_count() / io.batch;
@@ -940,10 +948,17 @@ void ot_begin(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, const OtPl
     constexpr int W = 16 / (int)sizeof(T);
     const bool flat = !gaps && total % W == 0 && ((uintptr_t)io.g & 15) == 0 && io.g_batch % W == 0 && (((uintptr_t)io.m | (uintptr_t)io.m_out) & 15) == 0;
     const dim3 grid0((unsigned)blocks, (unsigned)io.batch);
-    if (flat) k_orth_norm<T, W><<<grid0, 256, 0, s>>>(io, segments, len, total, partial); else k_orth_norm<T, N><<<grid0, 256, 0, s>>>(io, segments, len, total, partial);
+    if (flat) k_orth_norm<T, W, MUON><<<grid0, 256, 0, s>>>(io, segments, len, total, partial); else k_orth_norm<T, N, MUON><<<grid0, 256, 0, s>>>(io, segments, len, total, partial);
     const dim3 grid((unsigned)(p.m_pad / 64), (unsigned)(p.n_pad / 128), (unsigned)io.batch);
-    if (io.rows > io.cols) op_launch_next(s, grid, dim3(256), 0, k_orth_pack<T, LIMBS, 1, true>, io, poly.eps, partial, blocks, x, p.x_limb);
-    else op_launch_next(s, grid, dim3(256), 0, k_orth_pack<T, LIMBS, N, false>, io, poly.eps, partial, blocks, x, p.x_limb);
+    if (io.rows > io.cols) op_launch_next(s, grid, dim3(256), 0, k_orth_pack<T, LIMBS, 1, true, MUON>, io, poly.eps, partial, blocks, x, p.x_limb);
+    else op_launch_next(s, grid, dim3(256), 0, k_orth_pack<T, LIMBS, N, false, MUON>, io, poly.eps, partial, blocks, x, p.x_limb);
+}
+
+template <typename T, int LIMBS, int N>
+void ot_begin(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, const OtPlan& p, double* partial, uint8_t* x) {
+    if constexpr (LIMBS == 2)  // Muon's update always has two
+        if (io.m) return ot_begin_of<T, LIMBS, N, true>(s, io, poly, p, partial, x);
+    ot_begin_of<T, LIMBS, N, false>(s, io, poly, p, partial, x);
 }
 
 template <typename T, int LIMBS>
