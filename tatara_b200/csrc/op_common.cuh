@@ -40,12 +40,16 @@ static __device__ __forceinline__ void op_store(T* p, const float (&from)[N]) {
 // N adjacent elements as they lie in memory, two 16-bit ones to a register (as an array of __half they would take one each)
 template <typename T, int N>
 struct OpRaw {
+    static_assert(N * sizeof(T) == 2 || N * sizeof(T) == 4 || N * sizeof(T) == 8 || N * sizeof(T) == 16, "one access");
     static constexpr int WORDS = N * sizeof(T) >= 4 ? N * sizeof(T) / 4 : 1;
     unsigned w[WORDS];
     __device__ __forceinline__ void load(const T* p) {
         if (N * sizeof(T) == 16) {
             const uint4 u = *reinterpret_cast<const uint4*>(p);
             w[0] = u.x, w[1 % WORDS] = u.y, w[2 % WORDS] = u.z, w[3 % WORDS] = u.w;
+        } else if (N * sizeof(T) == 8) {
+            const uint2 u = *reinterpret_cast<const uint2*>(p);
+            w[0] = u.x, w[1 % WORDS] = u.y;
         } else if (N * sizeof(T) == 2) {
             w[0] = *reinterpret_cast<const unsigned short*>(p);
         } else {

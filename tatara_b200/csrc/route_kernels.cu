@@ -31,7 +31,9 @@ template <typename T> struct RouteWord;
 template <> struct RouteWord<float> {
     using W = unsigned long long;
     static constexpr W NONE = ((W)0x007fffffu << 32) | 0xffffffffu;  // of -inf: words above it can be chosen
-    static __device__ __forceinline__ W make(float x, int e) {
+    template <int N>
+    static __device__ __forceinline__ W make(const OpRaw<float, N>& l, int i, int e) {
+        const float x = l.get(i);
         const unsigned u = __float_as_uint(x + 0.0f);
         const unsigned key = x != x ? 0xffffffffu : u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
         return ((W)key << 32) | (unsigned)~e;
@@ -53,16 +55,30 @@ template <> struct RouteWord<float> {
         return w;
     }
 };
+template <typename T> struct RoutePair;
+template <> struct RoutePair<__half> {
+    using P = __half2;
+    static __device__ __forceinline__ P zeros() { return __float2half2_rn(0.0f); }
+};
+template <> struct RoutePair<__nv_bfloat16> {
+    using P = __nv_bfloat162;
+    static __device__ __forceinline__ P zeros() { return __float2bfloat162_rn(0.0f); }
+};
 template <typename T, unsigned NEG_INF>
 struct RouteWord16 {
     using W = unsigned;
     static constexpr W NONE = (NEG_INF << 16) | 0xffffu;
-    static __device__ __forceinline__ W make(T x, int e) {
-        unsigned u = *reinterpret_cast<const unsigned short*>(&x);
-        const float v = op_float(x);
-        u = v == 0.0f ? 0u : u;
-        const unsigned key = v != v ? 0xffffu : (u >> 15) ? u ^ 0xffffu : u ^ 0x8000u;
-        return (key << 16) | (0xffffu - (unsigned)e);
+    // Two logits' keys at once: x + 0 makes both zeros alike and every NaN 0x7fff, whose key is the largest.
+    static __device__ __forceinline__ unsigned keys(unsigned pair) {
+        using P = typename RoutePair<T>::P;
+        const P sum = __hadd2(*reinterpret_cast<const P*>(&pair), RoutePair<T>::zeros());
+        const unsigned u = *reinterpret_cast<const unsigned*>(&sum);
+        return u ^ ((u >> 15 & 0x00010001u) * 0x7fffu + 0x80008000u);
+    }
+    template <int N>
+    static __device__ __forceinline__ W make(const OpRaw<T, N>& l, int i, int e) {
+        const unsigned k = keys(l.w[i / 2]);
+        return (i & 1 ? k & 0xffff0000u : k << 16) | (0xffffu - (unsigned)e);
     }
     static __device__ __forceinline__ int expert(W w) { return (int)(0xffffu - (w & 0xffffu)); }
     static __device__ __forceinline__ float logit(W w) {
@@ -85,24 +101,32 @@ template <> struct RouteWord<__nv_bfloat16> : RouteWord16<__nv_bfloat16, 0x007fu
 template <int G, int VEC>
 __device__ __forceinline__ int route_expert(int v, int lane) { return (v / VEC) * G * VEC + lane * VEC + v % VEC; }
 
-template <typename T> __device__ __forceinline__ T route_never();
-template <> __device__ __forceinline__ float route_never<float>() { return -INFINITY; }
-template <> __device__ __forceinline__ __half route_never<__half>() { return __ushort_as_half(0xfc00); }
-template <> __device__ __forceinline__ __nv_bfloat16 route_never<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
+// -inf in every element of a register
+template <typename T> __device__ __forceinline__ unsigned route_never();
+template <> __device__ __forceinline__ unsigned route_never<float>() { return 0xff800000u; }
+template <> __device__ __forceinline__ unsigned route_never<__half>() { return 0xfc00fc00u; }
+template <> __device__ __forceinline__ unsigned route_never<__nv_bfloat16>() { return 0xff80ff80u; }
 
 // a lane's logits, -inf where there are none
 template <typename T, int G, int V, int VEC>
-__device__ __forceinline__ void route_load(const T* row, bool in, int experts, int lane, OpVec<T, VEC> (&l)[V / VEC]) {
+__device__ __forceinline__ void route_load(const T* row, bool in, int experts, int lane, OpRaw<T, VEC> (&l)[V / VEC]) {
 #pragma unroll
     for (int c = 0; c < V / VEC; ++c) {
         const int e = c * G * VEC + lane * VEC;
         if (in && e < experts) {
-            l[c] = *reinterpret_cast<const OpVec<T, VEC>*>(row + e);
+            l[c].load(row + e);
         } else {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) l[c].v[i] = route_never<T>();
+            for (int i = 0; i < OpRaw<T, VEC>::WORDS; ++i) l[c].w[i] = route_never<T>();
         }
     }
+}
+
+// exp(x - top) of a whole row, as a power of two: the product's rounding costs |x - top| 2^-24 of a probability, so 1e-6 of one of e^-16; exp(-inf) is 0
+__device__ __forceinline__ float route_exp(float x, float top) {
+    float y = (x - top) * 1.44269504f;
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y));
+    return y;
 }
 
 // descending, by Batcher's odd-even merges
@@ -161,11 +185,11 @@ k_route_forward(const T* __restrict__ logits, int64_t stride, const uint8_t* __r
         const int64_t row = base + group % (32 / G);
         const bool exists = row < rows;
         const bool in = exists && (!mask || mask[row]);
-        OpVec<T, VEC> raw[V / VEC];
+        OpRaw<T, VEC> raw[V / VEC];
         route_load<T, G, V, VEC>(logits + row * stride, in, experts, lane, raw);
         W w[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) w[v] = R::make(raw[v / VEC].v[v % VEC], route_expert<G, VEC>(v, lane));
+        for (int v = 0; v < V; ++v) w[v] = R::make(raw[v / VEC], v % VEC, route_expert<G, VEC>(v, lane));
         if (SORTED) route_sort<W, V>(w);
         W mine[SLOTS];
 #pragma unroll
@@ -198,7 +222,7 @@ k_route_forward(const T* __restrict__ logits, int64_t stride, const uint8_t* __r
         float l[V], total = 0.0f, chosen = 0.0f, g[SLOTS];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            l[v] = live ? expf(op_float(raw[v / VEC].v[v % VEC]) - top_l) : 0.0f;
+            l[v] = route_exp(raw[v / VEC].get(v % VEC), top_l);  // a row that is not live has nothing but -inf
             total += l[v];
         }
         total = op_group_sum<G>(total);
@@ -354,7 +378,7 @@ k_route_backward(const T* __restrict__ logits, int64_t stride, const uint8_t* __
         const int64_t row = base + group % (32 / G);
         const bool exists = row < rows;
         const bool in = exists && (!mask || mask[row]);
-        OpVec<T, VEC> raw[V / VEC];
+        OpRaw<T, VEC> raw[V / VEC];
         route_load<T, G, V, VEC>(logits + row * stride, in, experts, lane, raw);
         int at[SLOTS];
         float ga[SLOTS], dg[SLOTS], dot = 0.0f;
@@ -376,7 +400,7 @@ k_route_backward(const T* __restrict__ logits, int64_t stride, const uint8_t* __
         float l[V], top = -INFINITY, total = 0.0f, ph = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            l[v] = op_float(raw[v / VEC].v[v % VEC]);
+            l[v] = raw[v / VEC].get(v % VEC);
             top = fmaxf(top, l[v]);  // leaves a NaN out, which the sums then bring in
         }
 #pragma unroll
@@ -385,7 +409,7 @@ k_route_backward(const T* __restrict__ logits, int64_t stride, const uint8_t* __
         const float top_l = live ? top : 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            l[v] = expf(l[v] - top_l);
+            l[v] = route_exp(l[v], top_l);
             total += l[v];
             ph = fmaf(l[v], h[v], ph);
         }
