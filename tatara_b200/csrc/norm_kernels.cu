@@ -67,10 +67,9 @@ __device__ __forceinline__ void norm_block_sums(float (&v)[R], float (*buf)[R], 
 
 // Blocks of the kernels that walk down the rows which one SM holds: 24 warps of 80 registers.  Backward, fp16, 16384 x 768: 20.4 us; 30 warps of 64 (some
 // spilled) 24.6, four rows at a time in 96 registers 26.0, the next rows fetched ahead in 175 registers 34.
-constexpr int norm_per_sm(int warps, int all = 24) {
-    const int w = warps == 1 ? 4 : warps;
-    return all / w < 1 ? 1 : all / w;
-}
+constexpr int norm_per_sm(int warps, int all = 24) { return all / warps < 1 ? 1 : all / warps; }
+// ... backward.  Four warps with a row each hold more of their own: 16 warps of 128 registers (200000 x 256 fp16: 71 us, with 24 warps 89)
+constexpr int norm_per_sm_back(int warps) { return warps == 1 ? 4 : norm_per_sm(warps); }
 
 // VEC columns of a weight or bias, in 16-byte accesses (one element at a time they cost four to eight times the L1 wavefronts of the row
 // itself: 24 -> 8 us for 10000 rows of 1000 fp16)
@@ -258,14 +257,18 @@ k_norm_forward_long(const T* x, int64_t x_stride, const float* __restrict__ weig
 }
 
 // Backward: a block of W warps per row (W = 1: rows side by side, L lanes each) takes R rows at a time, which shares one barrier, walks
-// down the rows and keeps its columns' weight and bias gradients in registers; partial: [2][blocks][n].
+// down the rows and keeps its columns' weight and bias gradients in registers; part_w, part_b: [blocks][n] (of a single block the gradients themselves),
+// or both NULL.
 // fp32, 65536 x 1536: 175 us, 6.9 TB/s.
 template <typename T, int W, int L, int VEC, int CH, int R>
-__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, norm_per_sm(W))
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, norm_per_sm_back(W))
 k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, const float* __restrict__ mean,
                 const float* __restrict__ rstd, const float* __restrict__ weight, int64_t rows, int n, T* dx, int64_t dx_stride,
-                float* __restrict__ partial) {
+                float* __restrict__ part_w, float* __restrict__ part_b) {
     constexpr int FULL = norm_full(W, VEC, CH);
+    // What is not there is read from the last row and columns and then set to zero, so that no branch keeps the loads apart: 16-bit rows of several warps
+    // (16384 x 768 29.5 us, 27.6 so) and single columns of a warp (100000 x 201 120 us, 56 so).  fp32 and the others lose 0 to 20 %.
+    constexpr bool CLAMP = sizeof(T) == 2 && (W > 1 ? VEC > 1 && W < 16 : VEC == 1 && L == 32);
     constexpr int LANES = W == 1 ? L : 32 * W, SUBS = W == 1 ? 32 / L : 1, RB = W == 1 ? 4 * SUBS : 1;
     __shared__ float s_sum[2][2 * R][W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = W == 1 ? lane % L : threadIdx.x;
@@ -291,9 +294,18 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int col = (c * LANES + t) * VEC;
-                xv[q][c].zero();
-                gv[q][c].zero();
-                if (in && (c < FULL || col < n)) {
+                const bool there = in && (c < FULL || col < n);
+                if (CLAMP) {
+                    const int64_t row = in ? first + q : rows - 1;
+                    const int from = c < FULL ? col : min(col, n - VEC);
+                    xv[q][c].load(x + row * x_stride + from);
+                    gv[q][c].load(dy + row * dy_stride + from);
+                }
+                if (!CLAMP || !there) {
+                    xv[q][c].zero();
+                    gv[q][c].zero();
+                }
+                if (!CLAMP && there) {
                     xv[q][c].load(x + (first + q) * x_stride + col);
                     gv[q][c].load(dy + (first + q) * dy_stride + col);
                 }
@@ -362,7 +374,7 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
                 }
         }
     }
-    if (!partial) return;
+    if (!part_w) return;
     if (SUBS > 1)  // the rows of a warp, in halves
 #pragma unroll
         for (int o = 16; o >= L; o >>= 1)
@@ -399,8 +411,8 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
     for (int c = 0; c < CH; ++c) {
         const int col = (c * LANES + t) * VEC;
         if (col < n && (SUBS == 1 || lane < L)) {  // n is a multiple of VEC
-            op_store<float, VEC>(partial + (int64_t)blockIdx.x * n + col, aw[c]);
-            op_store<float, VEC>(partial + ((int64_t)gridDim.x + blockIdx.x) * n + col, ab[c]);
+            op_store<float, VEC>(part_w + (int64_t)blockIdx.x * n + col, aw[c]);
+            op_store<float, VEC>(part_b + (int64_t)blockIdx.x * n + col, ab[c]);
         }
     }
 }
@@ -431,7 +443,7 @@ k_norm_backward_long(const T* dy, int64_t dy_stride, const T* x, int64_t x_strid
 template <typename T>
 __global__ void __launch_bounds__(256)
 k_norm_columns_long(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x, int64_t x_stride, const float* __restrict__ mean,
-                    const float* __restrict__ rstd, int64_t rows, int n, float* __restrict__ partial) {
+                    const float* __restrict__ rstd, int64_t rows, int n, float* __restrict__ part_w, float* __restrict__ part_b) {
     const int col = blockIdx.x * 256 + threadIdx.x;
     if (col >= n) return;
     float aw = 0.0f, ab = 0.0f;
@@ -440,8 +452,8 @@ k_norm_columns_long(const T* __restrict__ dy, int64_t dy_stride, const T* __rest
         aw = fmaf(g, (op_float(x[row * x_stride + col]) - mean[row]) * rstd[row], aw);
         ab += g;
     }
-    partial[(int64_t)blockIdx.y * n + col] = aw;
-    partial[(int64_t)(gridDim.y + blockIdx.y) * n + col] = ab;
+    part_w[(int64_t)blockIdx.y * n + col] = aw;
+    part_b[(int64_t)blockIdx.y * n + col] = ab;
 }
 
 // dweight and dbias from the blocks' rows: eight columns (a 32-byte sector) per block; thread group r of 128 adds the rows r, r + 128, .., the four
@@ -487,10 +499,11 @@ void norm_with_warps(int w, F&& f) {  // f(std::integral_constant<int, W>)
 int norm_backward_blocks(int64_t rows, int n) {
     if (n > NORM_REG_N_BACK) return (int)(rows < 64 ? (rows < 1 ? 1 : rows) : 64);
     const int w = norm_warps(n);
-    const int64_t turn = n <= 64 ? 32 : n <= 128 ? 16 : w == 1 ? 8 : 2, sms = sm_count(), most = sms * norm_per_sm(w);
+    const int64_t turn = n <= 64 ? 32 : n <= 128 ? 16 : w == 1 ? 8 : 2, sms = sm_count(), most = sms * norm_per_sm_back(w);
     const int64_t turns = (rows + turn - 1) / turn, least = (16 + turn - 1) / turn, want = (turns + least - 1) / least;
+    if (turns <= 2) return 1;  // no second launch then
     const int64_t few = turns < sms ? turns : sms, blocks = want < few ? few : want < most ? want : most;
-    return (int)(blocks < 1 ? 1 : blocks);
+    return (int)blocks;
 }
 
 struct NormForward {
@@ -549,20 +562,21 @@ struct NormBackward {
     int n;
     void* dx;
     int64_t dxs;
-    float* partial;
+    float *part_w, *part_b;
     int blocks;
 };
 template <typename T, int VEC, int W, int L, int CH, int R>
 void norm_backward_go(const NormBackward& a) {
     k_norm_backward<T, W, L, VEC, CH / VEC, R><<<(unsigned)a.blocks, W == 1 ? 128 : W * 32, 0, a.s>>>((const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.w, a.rows, a.n,
-                                                                                                      (T*)a.dx, a.dxs, a.partial);
+                                                                                                      (T*)a.dx, a.dxs, a.part_w, a.part_b);
 }
 template <typename T, int VEC>
 void norm_backward_pick(const NormBackward& a) {
     if (a.n > NORM_REG_N_BACK) {
         // the columns first: dx may be dy's or x's memory
-        if (a.partial)
-            k_norm_columns_long<T><<<dim3((unsigned)ceil_div(a.n, 256), (unsigned)a.blocks), 256, 0, a.s>>>((const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.rows, a.n, a.partial);
+        if (a.part_w)
+            k_norm_columns_long<T><<<dim3((unsigned)ceil_div(a.n, 256), (unsigned)a.blocks), 256, 0, a.s>>>((const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.rows, a.n, a.part_w,
+                                                                                                             a.part_b);
         k_norm_backward_long<T><<<(unsigned)a.rows, 1024, 0, a.s>>>((const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.w, a.n, (T*)a.dx, a.dxs);
     } else if (a.n <= 64) {
         norm_backward_go<T, VEC, 1, 8, 8, 2>(a);
@@ -633,10 +647,13 @@ extern "C" int tb_layer_norm_backward(const void* d_dy, int64_t dy_stride, const
         return op_launched(err, err_len);
     }
     const bool wide = n % (16 / size) == 0 && norm_aligned(d_dy, dy_stride, size) && norm_aligned(d_x, x_stride, size) && norm_aligned(d_dx, dx_stride, size) && ((uintptr_t)d_weight & 15) == 0;
-    const NormBackward a = {s, d_dy, dy_stride, d_x, x_stride, d_mean, d_rstd, d_weight, rows, n, d_dx, dx_stride, partial, blocks};
+    // a single block writes the gradients themselves (its stores are as wide as 32 bytes)
+    const bool direct = blocks == 1 && d_dweight && d_dbias && (((uintptr_t)d_dweight | (uintptr_t)d_dbias) & 31) == 0;
+    const NormBackward a = {s, d_dy, dy_stride, d_x, x_stride, d_mean, d_rstd, d_weight, rows, n, d_dx, dx_stride, direct ? d_dweight : partial,
+                            direct ? d_dbias : partial ? partial + (int64_t)blocks * n : nullptr, blocks};
     if (type == TB_TYPE_F32) wide ? norm_backward_pick<float, 4>(a) : norm_backward_pick<float, 1>(a);
     else if (type == TB_TYPE_F16) wide ? norm_backward_pick<__half, 8>(a) : norm_backward_pick<__half, 1>(a);
     else wide ? norm_backward_pick<__nv_bfloat16, 8>(a) : norm_backward_pick<__nv_bfloat16, 1>(a);
-    if (columns) op_launch_next(s, dim3((unsigned)ceil_div(n, 8), 2), dim3(1024), 0, k_norm_columns_final, partial, blocks, n, d_dweight, d_dbias);
+    if (columns && !direct) op_launch_next(s, dim3((unsigned)ceil_div(n, 8), 2), dim3(1024), 0, k_norm_columns_final, partial, blocks, n, d_dweight, d_dbias);
     return op_launched(err, err_len);
 }

@@ -3,6 +3,8 @@
 Tolerances count roundings of fp32 (u = 2^-24).  A row's sum runs through at most n / 32 + 1 terms of a thread and ten more
 additions, so L = n / 32 + 11 bounds its relative error in u; a column's sum through at most `rows` + 40 terms.
 """
+import ctypes as C
+
 import pytest
 
 import tatara_b200 as tb
@@ -227,3 +229,25 @@ def test_refusals():
     assert lib.tb_layer_norm_forward(p, 7, None, None, 1e-5, 0, 4, 8, p, 8, None, None, None, None, 0) == -1
     assert lib.tb_layer_norm_forward(p, 8, None, None, 1e-5, 3, 4, 8, p, 8, None, None, None, None, 0) == -1
     assert lib.tb_layer_norm_backward_workspace(-1, 8) == -1 and lib.tb_layer_norm_backward_workspace(4, 0) == -1
+
+
+@pytest.mark.parametrize("rows,n", [(1, 9), (5, 19), (32, 64), (33, 64), (64, 40), (65, 40), (2, 100), (9, 200), (17, 200), (4, 1000), (5, 1001), (2, 5000), (1, 9000), (2, 9000)])
+def test_gradients_of_few_rows(rows, n):
+    x, dy = make(rows, n, torch.float32, rows + n), make(rows, n, torch.float32, rows + n + 7)
+    w = 1 + 0.2 * torch.randn(n, device="cuda")
+    _, mean, rstd = ops().layer_norm_forward(x, w, eps=EPS)
+    got = ops().layer_norm_backward(dy, x, mean, rstd, w)
+    check_backward(dy, x, mean, rstd, w, got)
+    # either gradient alone, and gradients that do not start on a wide boundary
+    lib, need = tb.load_library(), tb.load_library().tb_layer_norm_backward_workspace(rows, n)
+    work, err = torch.empty(need, dtype=torch.uint8, device="cuda"), C.create_string_buffer(200)
+    for use_w, use_b, off in ((True, False, 0), (False, True, 0), (False, False, 0), (True, True, 1)):
+        dx, dw, db = torch.empty_like(x), torch.full((n + 1,), 7.0, device="cuda"), torch.full((n + 1,), 7.0, device="cuda")
+        rc = lib.tb_layer_norm_backward(dy.data_ptr(), n, x.data_ptr(), n, mean.data_ptr(), rstd.data_ptr(), w.data_ptr(), 0, rows, n, dx.data_ptr(), n,
+                                        dw[off:].data_ptr() if use_w else None, db[off:].data_ptr() if use_b else None, work.data_ptr(), need,
+                                        torch.cuda.current_stream().cuda_stream, err, 200)
+        assert rc == 0, err.value
+        assert torch.equal(dx, got[0])
+        for t, used, want in ((dw, use_w, got[1]), (db, use_b, got[2])):
+            assert torch.equal(t[off:off + n], want) if used else (t == 7).all()
+            assert (t[:off] == 7).all() and (t[off + n:] == 7).all()
