@@ -256,17 +256,17 @@ int tb_ft_backward_static_scratch(const float* d_dft, const int32_t* d_indices, 
  * allocated and nothing is kept between calls, so calls on different streams may overlap as long as each has its own workspace.
  * A failed call returns a code, writes the reason to err (may be NULL) and launches nothing when an argument is refused.
  * Workspaces: tb_*_workspace returns the bytes a call of these sizes needs on the current device (negative: invalid sizes).
- * Row strides count elements; they may exceed the row (columns of a wider buffer).  Sums are fp32 in a fixed order
+ * Row strides count elements; they may exceed the row (columns of a wider buffer).  A result may be the memory of an input of its shape
+ * element by element (same address and strides) or have no element in common with it; one that overlaps an input in part is refused.  Sums are fp32 in a fixed order
  * (repeated calls agree bit for bit), results are rounded once to the tensors' type. */
 enum { TB_TYPE_F32 = 0, TB_TYPE_F16 = 1, TB_TYPE_BF16 = 2 };
 
 /* y = (x - mean) * rstd * weight + bias per row of n; weight, bias (fp32 [n]) may be NULL (1 and 0), mean, rstd (fp32 [rows], kept
- * for the backward pass) may be NULL.  x and y have the same type; y may be x. */
+ * for the backward pass) may be NULL.  x and y have the same type. */
 int tb_layer_norm_forward(const void* d_x, int64_t x_stride, const float* d_weight, const float* d_bias, float eps, int type, int64_t rows,
                           int n, void* d_y, int64_t y_stride, float* d_mean, float* d_rstd, void* stream, char* err, size_t err_len);
 int64_t tb_layer_norm_backward_workspace(int64_t rows, int n);
-/* dx, and dweight, dbias (fp32 [n], written, not added to; either may be NULL, both NULL need no workspace).  dx may be dy or x when
- * the strides are the same. */
+/* dx, and dweight, dbias (fp32 [n], written, not added to; either may be NULL, both NULL need no workspace).  dx may be dy or x. */
 int tb_layer_norm_backward(const void* d_dy, int64_t dy_stride, const void* d_x, int64_t x_stride, const float* d_mean, const float* d_rstd,
                            const float* d_weight, int type, int64_t rows, int n, void* d_dx, int64_t dx_stride, float* d_dweight,
                            float* d_dbias, void* d_work, int64_t work_bytes, void* stream, char* err, size_t err_len);
@@ -282,14 +282,14 @@ int tb_route_forward(const void* d_logits, int64_t stride, int type, int64_t row
                      int32_t* d_index, float* d_gate, int32_t* d_counts, int32_t* d_rows, float* d_prob_mean, float* d_losses, void* d_work,
                      int64_t work_bytes, void* stream, char* err, size_t err_len);
 /* The logits' gradient from dgate [rows, k] and dlosses [2] (the gradients of the gates and of the two losses; either may be NULL: zero) and
- * what the forward call wrote; the choice and the counts are constants.  Rows that take no part get zeros. */
+ * what the forward call wrote; the choice and the counts are constants.  Rows that take no part get zeros.  dlogits may be the logits. */
 int tb_route_backward(const void* d_logits, int64_t stride, int type, int64_t rows, int experts, int k, int renormalise, const uint8_t* d_mask,
                       const int32_t* d_index, const float* d_gate, const float* d_dgate, const int32_t* d_counts, const int32_t* d_rows,
                       const float* d_dlosses, void* d_dlogits, int64_t dstride, void* stream, char* err, size_t err_len);
 
 /* Newton-Schulz orthogonalisation of every matrix of a batch: X = x / (|x| + eps) (Frobenius norm), then `steps` (1 .. 32) times
  * X = (a I + b A + c A^2) X with A = X X^T taken over the shorter side; coefficients = {a, b, c} on the HOST.  x and out have the same
- * type and may be the same memory; x_batch and out_batch are the strides between matrices.  Coefficients for which a singular value of at most 1
+ * type; x_batch and out_batch are the strides between matrices.  Coefficients for which a singular value of at most 1
  * could grow beyond 4 (or |a| + |b| s^2 + |c| s^4 beyond 31) are refused.  fp32 and fp16: products of 22-bit operands (64-bit where the shorter
  * side is at most 64); bf16: 11-bit operands; fp32 sums.  A matrix with an infinity or a NaN comes out NaN. */
 int64_t tb_orthogonalise_workspace(int type, int batch, int rows, int cols);

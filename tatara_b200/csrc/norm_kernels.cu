@@ -10,9 +10,9 @@
 // then the warps in order.  The weight gradients are columns' sums: every block keeps those of its rows in registers over all
 // of its rows, the blocks' rows are added in a fixed order by a second kernel, so that results repeat bit for bit.
 //
-// Measured (inputs not in L2): 65536 x 1536 fp32 forward 119 us (6.8 TB/s), backward 176 us (6.9 TB/s) and 9 us for the columns' sums;
-// 50000 x 1000 bf16 39 us (5.2 TB/s) and 64 us (4.7 TB/s): 16-bit rows are half the bytes for the same instructions, issue slots at 60 %.
-// 256 x 256: one launch, 2 us.
+// Measured (inputs not in L2): 65536 x 1536 fp32 forward 120 us (6.7 TB/s), backward 177 us (6.8 TB/s) and 9 us for the columns' sums;
+// 40000 x 2048 fp16 72 us (4.6 TB/s) and 114 us (4.3 TB/s): 16-bit rows are half the bytes for the same instructions, issue slots at 60 %.
+// Rows that start anywhere, 35954 x 1175: fp32 64 us (5.2 TB/s) and 93 us (5.4 TB/s), bf16 55 and 87.  256 x 256: one launch, 2 us.
 #include "op_common.cuh"
 
 namespace {
@@ -259,7 +259,7 @@ k_norm_forward_long(const T* x, int64_t x_stride, const float* __restrict__ weig
 // Backward: a block of W warps per row (W = 1: rows side by side, L lanes each) takes R rows at a time, which shares one barrier, walks
 // down the rows and keeps its columns' weight and bias gradients in registers; part_w, part_b: [blocks][n] (of a single block the gradients themselves),
 // or both NULL.
-// fp32, 65536 x 1536: 175 us, 6.9 TB/s.
+// fp32, 65536 x 1536: 177 us, 6.8 TB/s.
 template <typename T, int W, int L, int VEC, int CH, int R>
 __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, norm_per_sm_back(W))
 k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, const float* __restrict__ mean,

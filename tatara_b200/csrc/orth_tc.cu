@@ -21,9 +21,9 @@
 // warps add what it held to their registers, rounded to nearest, while the next one fills.
 // Every wait is bounded; where one runs out the block's results become NaN, and so the output.
 //
-// Measured, 4096 x 4096 in fp32: Gram 156 us, square 166, apply 287 (1.4 PFLOP/s of limb products, tensor pipe 78 to 92 % busy), last product with
-// the weight update 324; the whole Muon step 3.3 to 3.8 ms, where the chip's power limit, not the kernel, sets the clock.  bf16: 1.15 ms.  Small
-// products are bound by what surrounds the MMAs: 4 x 1000 x 777 bf16 takes 137 us in 17 launches of 8 to 10 us, 2 to 4 us of each inside the K loop.
+// Measured, 4096 x 4096 in fp32: Gram 159 us, square 168, apply 293 (1.4 PFLOP/s of limb products, tensor pipe 78 to 92 % busy), last product with
+// the weight update 334; the whole Muon step 3.3 to 3.8 ms, where the chip's power limit, not the kernel, sets the clock.  bf16: 1.15 ms.  Small
+// products are bound by what surrounds the MMAs: 4 x 1000 x 777 bf16 takes 124 us in 17 launches of 7 to 9 us, 3 to 4 us of each inside the K loop.
 #include "orth.cuh"
 
 #include <atomic>

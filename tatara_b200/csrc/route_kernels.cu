@@ -13,8 +13,8 @@
 // made of the logits' bits as they are and the expert, so it does not depend on how the softmax rounds.  Sums: fp32 chains over a group's
 // rows, then the groups of a block in order, then the blocks in order in 64 bits (second kernel): results repeat bit for bit.
 //
-// What bounds it are issue slots for many experts (615 instructions per row of 256 bf16 logits and eight choices, slots at 75 %: 35 us for 40000
-// rows, whose bytes would take 3.5; their gradient 24 us at 355 instructions per row) and latency for the handful of a net (65536 x 9 fp32, one choice:
+// What bounds it are issue slots for many experts (490 instructions per row of 256 bf16 logits and eight choices, slots at 73 %: 29 us for 40000
+// rows, whose bytes would take 3.5; their gradient 17 us at 290 instructions per row) and latency for the handful of a net (65536 x 9 fp32, one choice:
 // 10 us with both launches, the gradient 5.5).
 #include "op_common.cuh"
 
