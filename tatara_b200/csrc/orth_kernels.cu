@@ -24,8 +24,6 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-#define SMALL_THREADS 320
-#define SMALL_WARPS 10
 #define SMALL_CLUSTER 16   // most CTAs that share a matrix
 #define SMALL_SMEM 229376  // 224 KB
 #define SMALL_BATCH 8      // elements a thread has on their way at once
@@ -73,17 +71,17 @@ __device__ __forceinline__ void small_product(const double* __restrict__ x, cons
 
 // columns [j0, j0 + jc) of a matrix into xs[j][pitch] (64 bits); rows n .. np - 1 and columns jc .. jp - 1 are zero.  Neighbours in memory go to
 // neighbouring threads; all loads of a batch are issued before the first is used (one at a time this was half of the kernel).
-template <typename T, bool FIRST>
+template <typename T, bool FIRST, int THREADS>
 __device__ __forceinline__ void small_fill(const OrthIo& io, int b, int n, int np, bool tall, int64_t j0, int jc, int jp, double* xs, int pitch) {
     const int total = np * jp, inner = tall ? np : jp;
     const unsigned magic = (unsigned)((0x100000000ull + inner - 1) / inner);  // e / inner = e * magic >> 32 for e * inner < 2^32
-    for (int e0 = threadIdx.x; e0 < total; e0 += SMALL_THREADS * SMALL_BATCH) {
+    for (int e0 = threadIdx.x; e0 < total; e0 += THREADS * SMALL_BATCH) {
         float g[SMALL_BATCH], m[SMALL_BATCH];
         int64_t at[SMALL_BATCH];
         int to[SMALL_BATCH];
 #pragma unroll
         for (int u = 0; u < SMALL_BATCH; ++u) {
-            const int e = e0 + u * SMALL_THREADS;
+            const int e = e0 + u * THREADS;
             const int hi = (int)__umulhi((unsigned)e, magic), lo = e - hi * inner;
             const int i = tall ? lo : hi, j = tall ? hi : lo;
             to[u] = e < total ? j * pitch + i : -1;
@@ -114,8 +112,9 @@ __device__ __forceinline__ void small_fill(const OrthIo& io, int b, int n, int n
 }
 
 // jc_max: columns of a chunk in shared memory, a multiple of 8
-template <typename T>
-__global__ void __launch_bounds__(SMALL_THREADS) k_orth_small(OrthIo io, OrthPoly poly, int jc_max) {
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) k_orth_small(OrthIo io, OrthPoly poly, int jc_max) {
+    constexpr int THREADS = 32 * WARPS;
     extern __shared__ double s_mem[];
     cg::cluster_group cluster = cg::this_cluster();
     const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -139,18 +138,19 @@ __global__ void __launch_bounds__(SMALL_THREADS) k_orth_small(OrthIo io, OrthPol
         s_block[tid] = bi << 8 | bj;
     }
     // Gram matrix of this CTA's columns: a warp per block, or a few per block that share the columns
-    const int splits = blocks < SMALL_WARPS ? SMALL_WARPS / blocks : 1, units = blocks * splits;
-    double gram[4][2];  // of the units warp, warp + 10, ..
+    const int splits = blocks < WARPS ? max(1, min(WARPS / blocks, jc_max / 8)) : 1, units = blocks * splits;
+    constexpr int UNITS = 36 / WARPS + 1;  // of a warp: warp, warp + WARPS, ..
+    double gram[UNITS][2];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) gram[u][0] = gram[u][1] = 0.0;
+    for (int u = 0; u < UNITS; ++u) gram[u][0] = gram[u][1] = 0.0;
     for (int64_t j0 = begin; j0 < end; j0 += jc_max) {
         const int jc = (int)min((int64_t)jc_max, end - j0), jp = (jc + 7) / 8 * 8;
-        __syncthreads();
-        small_fill<T, true>(io, b, n, np, tall, j0, jc, jp, s_x, pitch);
+        if (j0 > begin) __syncthreads();
+        small_fill<T, true, THREADS>(io, b, n, np, tall, j0, jc, jp, s_x, pitch);
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int unit = warp + u * SMALL_WARPS;
+        for (int u = 0; u < UNITS; ++u) {
+            const int unit = warp + u * WARPS;
             if (unit >= units) break;
             const int bi = s_block[unit % blocks] >> 8, bj = s_block[unit % blocks] & 255;
             const double *x = s_x + (lane & 3) * pitch + bi * 8 + (lane >> 2), *y = s_x + (lane & 3) * pitch + bj * 8 + (lane >> 2);
@@ -160,21 +160,23 @@ __global__ void __launch_bounds__(SMALL_THREADS) k_orth_small(OrthIo io, OrthPol
     }
     double* gram_to = splits > 1 ? s_part : s_own;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int unit = warp + u * SMALL_WARPS;
+    for (int u = 0; u < UNITS; ++u) {
+        const int unit = warp + u * WARPS;
         if (unit < units) *reinterpret_cast<double2*>(gram_to + unit * 64 + lane * 2) = make_double2(gram[u][0], gram[u][1]);
     }
     if (splits > 1) {
         __syncthreads();
-        for (int e = tid; e < blocks * 64; e += SMALL_THREADS) {
-            double v = s_part[e];
-            for (int k = 1; k < splits; ++k) v += s_part[k * blocks * 64 + e];
+        for (int e = tid; e < blocks * 64; e += THREADS) {
+            double v = 0.0;
+#pragma unroll
+            for (int k = 0; k < WARPS; ++k)
+                if (k < splits) v += s_part[k * blocks * 64 + e];
             s_own[e] = v;
         }
     }
     cluster.sync();
     // every CTA adds up its share of the entries over the CTAs, in order, and hands the sums to all
-    for (int e = blocks * 32 * rank / cs + tid; e < blocks * 32 * (rank + 1) / cs; e += SMALL_THREADS) {
+    for (int e = blocks * 32 * rank / cs + tid; e < blocks * 32 * (rank + 1) / cs; e += THREADS) {
         double2 part[SMALL_CLUSTER], v = make_double2(0.0, 0.0);
 #pragma unroll
         for (int r = 0; r < SMALL_CLUSTER; ++r) part[r] = r < cs ? reinterpret_cast<const double2*>(cluster.map_shared_rank(s_own, r))[e] : make_double2(0.0, 0.0);
@@ -195,7 +197,7 @@ __global__ void __launch_bounds__(SMALL_THREADS) k_orth_small(OrthIo io, OrthPol
     for (int o = 16; o > 0; o >>= 1) trace += __shfl_xor_sync(0xffffffffu, trace, o);
     // a matrix of zeros with eps 0: 0 / 0, as the definition says
     const double inv = 1.0 / (sqrt(trace) + (double)poly.eps);
-    for (int e = tid; e < blocks * 64; e += SMALL_THREADS) {
+    for (int e = tid; e < blocks * 64; e += THREADS) {
         const int i = (s_block[e >> 6] >> 8) * 8 + ((e & 63) >> 3), j = (s_block[e >> 6] & 255) * 8 + (e & 7);
         const double v = s_t[e] * inv * inv;
         if (i >= j) s_a[i * pitch + j] = s_a[j * pitch + i] = v;
@@ -204,16 +206,16 @@ __global__ void __launch_bounds__(SMALL_THREADS) k_orth_small(OrthIo io, OrthPol
 
     for (int s = 0; s < poly.steps; ++s) {
         const bool last = s + 1 == poly.steps;
-        for (int t = warp; t < blocks; t += SMALL_WARPS) small_product<true>(s_a, s_a, s_q, np, pitch, s_block[t], lane, poly.c, poly.b, poly.a);  // Q
+        for (int t = warp; t < blocks; t += WARPS) small_product<true>(s_a, s_a, s_q, np, pitch, s_block[t], lane, poly.c, poly.b, poly.a);  // Q
         __syncthreads();
         // unless it is the last step, A = (Q A) Q; P = Q P (P = Q in the first step)
         const int first = last ? blocks : 0, total = s == 0 ? blocks : 2 * blocks;
-        for (int t = first + warp; t < total; t += SMALL_WARPS) {
+        for (int t = first + warp; t < total; t += WARPS) {
             if (t < blocks) small_product<false>(s_q, s_a, s_t, np, pitch, s_block[t], lane, 0.0, 0.0, 0.0);
             else small_product<false>(s_q, s_p, s_own, np, pitch, s_block[t - blocks], lane, 0.0, 0.0, 0.0);
         }
         if (s == 0)
-            for (int e = tid; e < size; e += SMALL_THREADS) s_p[e] = s_q[e];
+            for (int e = tid; e < size; e += THREADS) s_p[e] = s_q[e];
         __syncthreads();
         if (s > 0) {
             double* z = s_p;
@@ -221,7 +223,7 @@ __global__ void __launch_bounds__(SMALL_THREADS) k_orth_small(OrthIo io, OrthPol
             s_own = z;
         }
         if (!last) {
-            for (int t = warp; t < blocks; t += SMALL_WARPS) small_product<false>(s_t, s_q, s_a, np, pitch, s_block[t], lane, 0.0, 0.0, 0.0);
+            for (int t = warp; t < blocks; t += WARPS) small_product<false>(s_t, s_q, s_a, np, pitch, s_block[t], lane, 0.0, 0.0, 0.0);
             __syncthreads();
         }
     }
@@ -231,10 +233,10 @@ __global__ void __launch_bounds__(SMALL_THREADS) k_orth_small(OrthIo io, OrthPol
         const int jc = (int)min((int64_t)jc_max, end - j0), jp = (jc + 7) / 8 * 8;
         if (end - begin > jc_max) {  // else they are still there
             __syncthreads();
-            small_fill<T, false>(io, b, n, np, tall, j0, jc, jp, s_x, pitch);
+            small_fill<T, false, THREADS>(io, b, n, np, tall, j0, jc, jp, s_x, pitch);
             __syncthreads();
         }
-        for (int t = warp; t < side * (jp / 8); t += SMALL_WARPS) {
+        for (int t = warp; t < side * (jp / 8); t += WARPS) {
             const int bi = t % side, bj = t / side, i = bi * 8 + (lane >> 2), j = bj * 8 + 2 * (lane & 3);
             const int64_t at = b * io.out_batch + (tall ? (j0 + j) * io.out_stride + i : i * io.out_stride + j0 + j), next = tall ? io.out_stride : 1;
             float w[2];
@@ -254,17 +256,17 @@ __global__ void __launch_bounds__(SMALL_THREADS) k_orth_small(OrthIo io, OrthPol
     }
 }
 
-// Whether the current device runs clusters of sixteen (which are not portable) at the largest shared memory: asked once per device.
-template <typename T>
-bool small_cluster_fits() {
-    static std::atomic<signed char> known[64];  // 0 not asked, 1 yes, -1 no
+// How many clusters of sixteen (which are not portable) the current device runs at once at the largest shared memory: asked once per device.
+template <typename T, int WARPS>
+int small_clusters() {
+    static std::atomic<int> known[64];  // 0 not asked, else one more
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
-    signed char k = known[dev].load();
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    int k = known[dev].load();
     if (!k) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(SMALL_CLUSTER);
-        cfg.blockDim = dim3(SMALL_THREADS);
+        cfg.blockDim = dim3(32 * WARPS);
         cfg.dynamicSmemBytes = SMALL_SMEM;
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeClusterDimension;
@@ -273,31 +275,33 @@ bool small_cluster_fits() {
         cfg.attrs = at;
         cfg.numAttrs = 1;
         int fit = 0;
-        const bool ok = cudaFuncSetAttribute(k_orth_small<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMALL_SMEM) == cudaSuccess &&
-                        cudaFuncSetAttribute(k_orth_small<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
-                        cudaOccupancyMaxActiveClusters(&fit, k_orth_small<T>, &cfg) == cudaSuccess && fit >= 1;
+        const bool ok = cudaFuncSetAttribute(k_orth_small<T, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMALL_SMEM) == cudaSuccess &&
+                        cudaFuncSetAttribute(k_orth_small<T, WARPS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                        cudaOccupancyMaxActiveClusters(&fit, k_orth_small<T, WARPS>, &cfg) == cudaSuccess && fit >= 1;
         if (!ok) cudaGetLastError();
-        known[dev].store(k = ok ? 1 : -1);
+        known[dev].store(k = (ok ? fit : 0) + 1);
     }
-    return k > 0;
+    return k - 1;
 }
 
-template <typename T>
-void orth_small_go(cudaStream_t s, const OrthIo& io, const OrthPoly& p) {
-    const int n = io.rows < io.cols ? io.rows : io.cols, m = io.rows < io.cols ? io.cols : io.rows, np = (n + 7) / 8 * 8, pitch = small_pitch(np);
-    // 32 columns or more per CTA, and no more CTAs than the chip holds at once (sixteen for eight: n = 32, m = 1024 in 16 us for 20)
+// CTAs per matrix: 32 columns or more for each, and no more than the chip holds at once (sixteen for eight: n = 32, m = 1024 in 16 us for 20); most: of a cluster
+int small_ctas(const OrthIo& io, int64_t m, int most) {
     int cs = 1;
-    const int most = small_cluster_fits<T>() ? SMALL_CLUSTER : 8;
     while (cs < most && cs * 32 < m && (int64_t)io.batch * 2 * cs <= sm_count()) cs *= 2;
-    // a CTA's columns stay in shared memory where they fit beside the matrices; the partial sums take 640 doubles of the matrices
-    const int matrices = np * pitch * 2 + (np * pitch * 3 > 640 ? np * pitch * 3 : 640), room = (SMALL_SMEM / 8 - matrices) / pitch / 8 * 8;
-    const int64_t per = ((int64_t)m + cs - 1) / cs;
+    return cs;
+}
+template <typename T, int WARPS>
+void small_launch(cudaStream_t s, const OrthIo& io, const OrthPoly& p, int n, int64_t m, int cs) {
+    // a CTA's columns stay in shared memory where they fit beside the matrices; the partial sums take 64 doubles per warp of the matrices
+    const int np = (n + 7) / 8 * 8, pitch = small_pitch(np), three = np * pitch * 3, part = 64 * WARPS;
+    const int matrices = np * pitch * 2 + (three > part ? three : part), room = (SMALL_SMEM / 8 - matrices) / pitch / 8 * 8;
+    const int64_t per = (m + cs - 1) / cs;
     const int jc_max = per < room ? (int)((per + 7) / 8 * 8) : room;
     const size_t smem = (size_t)(jc_max * pitch + matrices) * sizeof(double);
-    cudaFuncSetAttribute(k_orth_small<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMALL_SMEM);
+    cudaFuncSetAttribute(k_orth_small<T, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMALL_SMEM);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)cs, (unsigned)io.batch);
-    cfg.blockDim = dim3(SMALL_THREADS);
+    cfg.blockDim = dim3(32 * WARPS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
@@ -306,7 +310,17 @@ void orth_small_go(cudaStream_t s, const OrthIo& io, const OrthPoly& p) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, k_orth_small<T>, io, p, jc_max);
+    cudaLaunchKernelEx(&cfg, k_orth_small<T, WARPS>, io, p, jc_max);
+}
+// Sixteen warps where the products or the loads keep them busy (64 x 512: 44 us, with ten 50, eight 47; 15 of 19 x 2200: 18, 20, 21), else eight: fewer to wait
+// for at a barrier, and two CTAs per SM (9 of 16 x 1536: 12.5 us, with sixteen 21.6: the ninth cluster has to wait).
+template <typename T>
+void orth_small_go(cudaStream_t s, const OrthIo& io, const OrthPoly& p) {
+    const int n = io.rows < io.cols ? io.rows : io.cols;
+    const int64_t m = io.rows < io.cols ? io.cols : io.rows;
+    const int few = small_ctas(io, m, small_clusters<T, 8>() > 0 ? SMALL_CLUSTER : 8);
+    if (n <= 24 && (m + few - 1) / few <= 128) return small_launch<T, 8>(s, io, p, n, m, few);
+    small_launch<T, 16>(s, io, p, n, m, small_ctas(io, m, io.batch <= small_clusters<T, 16>() ? SMALL_CLUSTER : 8));
 }
 
 // The limbs hold numbers up to 32 (orth_tc.cu); fp16 inputs' results are rounded to 11 bits, bf16's to 8: one limb of 11 bits is
