@@ -12,8 +12,8 @@
 // symmetric and commute: half of every product is computed.  The products are the tensor cores' 64-bit ones (8 x 8 x 4 per warp): a step of
 // 32 x 32 matrices waits for a chain of four of them where thread-wise sums wait for sixteen additions and four times the shared-memory
 // reads.  A fixed order everywhere: results repeat bit for bit.
-// Measured: 9 matrices of 16 x 1536 12.5 us (the loads 2.4, the steps 4), the Muon step of 1024 x 32 16.7 us (the steps 8: 64-bit products at 32
-// multiply-adds per cycle and SM), 64 x 2048 69 us.
+// Measured: 9 matrices of 16 x 1536 12.4 us (the loads 2.4, the steps 4), the Muon step of 1024 x 32 16.0 us (the steps 7), 64 x 512 43.6 us (the steps 36:
+// 64-bit products at 40 of the 64 multiply-adds per cycle and SM).
 #include "orth.cuh"
 
 #include <cooperative_groups.h>
@@ -174,7 +174,8 @@ __global__ void __launch_bounds__(32 * WARPS) k_orth_small(OrthIo io, OrthPoly p
             s_own[e] = v;
         }
     }
-    cluster.sync();
+    if (cs > 1) cluster.sync();
+    else __syncthreads();
     // every CTA adds up its share of the entries over the CTAs, in order, and hands the sums to all
     for (int e = blocks * 32 * rank / cs + tid; e < blocks * 32 * (rank + 1) / cs; e += THREADS) {
         double2 part[SMALL_CLUSTER], v = make_double2(0.0, 0.0);
@@ -187,7 +188,8 @@ __global__ void __launch_bounds__(32 * WARPS) k_orth_small(OrthIo io, OrthPoly p
         }
         for (int r = 0; r < cs; ++r) reinterpret_cast<double2*>(cluster.map_shared_rank(s_t, r))[e] = v;
     }
-    cluster.sync();  // from here on no CTA touches another's memory
+    if (cs > 1) cluster.sync();  // from here on no CTA touches another's memory
+    else __syncthreads();
     double trace = 0.0;
     for (int i = lane; i < np; i += 32) {
         const int bi = i >> 3;
@@ -312,14 +314,14 @@ void small_launch(cudaStream_t s, const OrthIo& io, const OrthPoly& p, int n, in
     cfg.numAttrs = 1;
     cudaLaunchKernelEx(&cfg, k_orth_small<T, WARPS>, io, p, jc_max);
 }
-// Sixteen warps where the products or the loads keep them busy (64 x 512: 44 us, with ten 50, eight 47; 15 of 19 x 2200: 18, 20, 21), else eight: fewer to wait
-// for at a barrier, and two CTAs per SM (9 of 16 x 1536: 12.5 us, with sixteen 21.6: the ninth cluster has to wait).
+// Sixteen warps where the products or the loads keep them busy (64 x 512: 44 us, with ten 50, eight 47; 15 of 19 x 2200: 18, 20, 21; 9 of 24 x 1536: 16.0, with eight 17.5), else eight, whose columns
+// are one batch of loads: fewer to wait for at a barrier (16 x 64: 9.1 us, 10.1), and two CTAs per SM (9 of 16 x 1536: 12.5 us, with sixteen 21.6: the ninth cluster has to wait).
 template <typename T>
 void orth_small_go(cudaStream_t s, const OrthIo& io, const OrthPoly& p) {
     const int n = io.rows < io.cols ? io.rows : io.cols;
     const int64_t m = io.rows < io.cols ? io.cols : io.rows;
     const int few = small_ctas(io, m, small_clusters<T, 8>() > 0 ? SMALL_CLUSTER : 8);
-    if (n <= 24 && (m + few - 1) / few <= 128) return small_launch<T, 8>(s, io, p, n, m, few);
+    if (n <= 24 && (n + 7) / 8 * 8 * ((m + few - 1) / few) <= 256 * SMALL_BATCH) return small_launch<T, 8>(s, io, p, n, m, few);
     small_launch<T, 16>(s, io, p, n, m, small_ctas(io, m, io.batch <= small_clusters<T, 16>() ? SMALL_CLUSTER : 8));
 }
 
