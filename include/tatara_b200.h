@@ -254,6 +254,7 @@ int tb_ft_backward_static_scratch(const float* d_dft, const int32_t* d_indices, 
  * front of a gate, the choice of a bucket (expert) per row with a balance loss, and the matrix optimizer of hidden weights.  ALL tensor pointers are DEVICE memory of the
  * current device, owned by the caller; the work is enqueued on `stream` (a cudaStream_t, NULL = default stream) and not synchronised; nothing is
  * allocated and nothing is kept between calls, so calls on different streams may overlap as long as each has its own workspace.
+ * A call's kernels may be started while the kernel ahead of them on the stream is ending; they wait for its end before they touch memory.
  * A failed call returns a code, writes the reason to err (may be NULL) and launches nothing when an argument is refused.
  * Workspaces: tb_*_workspace returns the bytes a call of these sizes needs on the current device (negative: invalid sizes).
  * Row strides count elements; they may exceed the row (columns of a wider buffer).  A result may be the memory of an input of its shape

@@ -97,9 +97,11 @@ k_norm_forward(const T* x, int64_t x_stride, const float* __restrict__ weight, c
     __shared__ float s_sum[2][W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = W == 1 ? lane % L : threadIdx.x;
     const int64_t row = (int64_t)blockIdx.x * RB + (W == 1 ? (warp * SUBS + lane / L) * R : 0);
+    op_next_may_start();
     if (L == 32 && row >= rows) return;  // by whole warps; lanes that share a warp stay for its sums
     constexpr bool ALL = R == 1 && L == 32;
     OpRaw<T, VEC> v[R][CH];
+    op_wait_for_previous();
 #pragma unroll
     for (int q = 0; q < R; ++q)
 #pragma unroll
@@ -174,6 +176,8 @@ k_norm_forward_down(const T* x, int64_t x_stride, const float* __restrict__ weig
     __shared__ float s_sum[2][2][W][R];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = threadIdx.x;
     float w[CH], b[CH];
+    op_next_may_start();
+    op_wait_for_previous();
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int col = c * LANES + t;
@@ -240,6 +244,8 @@ k_norm_forward_long(const T* x, int64_t x_stride, const float* __restrict__ weig
     const int64_t row = blockIdx.x;
     const T* xr = x + row * x_stride;
     float sum = 0.0f, sq = 0.0f;
+    op_next_may_start();
+    op_wait_for_previous();
     for (int c = threadIdx.x; c < n; c += 1024) sum += op_float(xr[c]);
     const float mean = norm_row_sum<32>(sum, s_sum[0], warp, lane) / (float)n;
     for (int c = threadIdx.x; c < n; c += 1024) {
@@ -273,6 +279,8 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
     __shared__ float s_sum[2][2 * R][W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = W == 1 ? lane % L : threadIdx.x;
     float w[CH][VEC], aw[CH][VEC], ab[CH][VEC];
+    op_next_may_start();
+    op_wait_for_previous();
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int col = (c * LANES + t) * VEC;
@@ -282,7 +290,6 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
     }
     const float inv_n = 1.0f / (float)n;
     int turn = 0;
-    op_next_may_start();
     // the lanes of a warp take the same number of turns
     for (int64_t turn0 = ((int64_t)blockIdx.x * RB + (W == 1 ? warp * SUBS : 0)) * R; turn0 < rows; turn0 += (int64_t)gridDim.x * RB * R, turn ^= 1) {
         const int64_t first = turn0 + (SUBS > 1 ? lane / L * R : 0);
@@ -426,6 +433,8 @@ k_norm_backward_long(const T* dy, int64_t dy_stride, const T* x, int64_t x_strid
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = blockIdx.x;
     const T *xr = x + row * x_stride, *gr = dy + row * dy_stride;
+    op_next_may_start();
+    op_wait_for_previous();
     const float mu = mean[row], r = rstd[row];
     float s1 = 0.0f, s2 = 0.0f;
     for (int c = threadIdx.x; c < n; c += 1024) {
@@ -445,6 +454,8 @@ __global__ void __launch_bounds__(256)
 k_norm_columns_long(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x, int64_t x_stride, const float* __restrict__ mean,
                     const float* __restrict__ rstd, int64_t rows, int n, float* __restrict__ part_w, float* __restrict__ part_b) {
     const int col = blockIdx.x * 256 + threadIdx.x;
+    op_next_may_start();
+    op_wait_for_previous();
     if (col >= n) return;
     float aw = 0.0f, ab = 0.0f;
     for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
@@ -462,6 +473,7 @@ __global__ void __launch_bounds__(1024) k_norm_columns_final(const float* __rest
                                                               float* __restrict__ dbias) {
     __shared__ float s_sum[32][9];
     float* out = blockIdx.y ? dbias : dweight;
+    op_next_may_start();
     if (!out) return;  // of the same block all
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = threadIdx.x & 7, col = blockIdx.x * 8 + c;
     const float* p = partial + (int64_t)blockIdx.y * prows * n;
@@ -523,12 +535,12 @@ void norm_forward_go(const NormForward& a) {
     // registers of a row's share, and how many of its elements have to be on their way: two rows where that leaves the warps enough
     constexpr int R = W == 1 && CH * VEC * (int)sizeof(T) <= 64 ? 2 : 1;
     const int64_t per = W == 1 ? 128 / L * R : 1, blocks = (a.rows + per - 1) / per;
-    k_norm_forward<T, W, L, VEC, CH, R><<<(unsigned)blocks, W == 1 ? 128 : W * 32, 0, a.s>>>((const T*)a.x, a.xs, a.w, a.b, a.eps, a.rows, a.n, (T*)a.y, a.ys, a.mean, a.rstd);
+    op_launch_next(a.s, dim3((unsigned)blocks), dim3(W == 1 ? 128 : W * 32), 0, k_norm_forward<T, W, L, VEC, CH, R>, (const T*)a.x, a.xs, a.w, a.b, a.eps, a.rows, a.n, (T*)a.y, a.ys, a.mean, a.rstd);
 }
 template <typename T, int W, int CH, int R>
 void norm_forward_down(const NormForward& a) {
     const int64_t want = (a.rows + R - 1) / R, most = (int64_t)sm_count() * norm_per_sm(W, 32);
-    k_norm_forward_down<T, W, CH, R><<<(unsigned)(want < most ? want : most), W * 32, 0, a.s>>>((const T*)a.x, a.xs, a.w, a.b, a.eps, a.rows, a.n, (T*)a.y, a.ys, a.mean, a.rstd);
+    op_launch_next(a.s, dim3((unsigned)(want < most ? want : most)), dim3(W * 32), 0, k_norm_forward_down<T, W, CH, R>, (const T*)a.x, a.xs, a.w, a.b, a.eps, a.rows, a.n, (T*)a.y, a.ys, a.mean, a.rstd);
 }
 // Rows on 16-byte boundaries: 8, 16 or 32 lanes per row up to 64, 128 and 256 columns (200000 x 128 bf16 with 32 lanes 45 us, with 16 28.7), a warp up to
 // 2048 columns of fp32 and 3072 of 16 bits (no barrier in a row; 30000 x 2560 bf16 72 us, with eight warps 94; 20000 x 4096 93 and 84), eight warps above.
@@ -548,7 +560,7 @@ void norm_forward_pick(const NormForward& a) {
         if (a.n <= NORM_REG_N_BACK) return norm_forward_down<T, 16, 16, 1>(a);
     }
 #undef GO
-    k_norm_forward_long<T><<<(unsigned)a.rows, 1024, 0, a.s>>>((const T*)a.x, a.xs, a.w, a.b, a.eps, a.n, (T*)a.y, a.ys, a.mean, a.rstd);
+    op_launch_next(a.s, dim3((unsigned)a.rows), dim3(1024), 0, k_norm_forward_long<T>, (const T*)a.x, a.xs, a.w, a.b, a.eps, a.n, (T*)a.y, a.ys, a.mean, a.rstd);
 }
 
 struct NormBackward {
@@ -567,7 +579,7 @@ struct NormBackward {
 };
 template <typename T, int VEC, int W, int L, int CH, int R>
 void norm_backward_go(const NormBackward& a) {
-    k_norm_backward<T, W, L, VEC, CH / VEC, R><<<(unsigned)a.blocks, W == 1 ? 128 : W * 32, 0, a.s>>>((const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.w, a.rows, a.n,
+    op_launch_next(a.s, dim3((unsigned)a.blocks), dim3(W == 1 ? 128 : W * 32), 0, k_norm_backward<T, W, L, VEC, CH / VEC, R>, (const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.w, a.rows, a.n,
                                                                                                       (T*)a.dx, a.dxs, a.part_w, a.part_b);
 }
 template <typename T, int VEC>
@@ -575,9 +587,9 @@ void norm_backward_pick(const NormBackward& a) {
     if (a.n > NORM_REG_N_BACK) {
         // the columns first: dx may be dy's or x's memory
         if (a.part_w)
-            k_norm_columns_long<T><<<dim3((unsigned)ceil_div(a.n, 256), (unsigned)a.blocks), 256, 0, a.s>>>((const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.rows, a.n, a.part_w,
+            op_launch_next(a.s, dim3((unsigned)ceil_div(a.n, 256), (unsigned)a.blocks), dim3(256), 0, k_norm_columns_long<T>, (const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.rows, a.n, a.part_w,
                                                                                                              a.part_b);
-        k_norm_backward_long<T><<<(unsigned)a.rows, 1024, 0, a.s>>>((const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.w, a.n, (T*)a.dx, a.dxs);
+        op_launch_next(a.s, dim3((unsigned)a.rows), dim3(1024), 0, k_norm_backward_long<T>, (const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.w, a.n, (T*)a.dx, a.dxs);
     } else if (a.n <= 64) {
         norm_backward_go<T, VEC, 1, 8, 8, 2>(a);
     } else if (a.n <= 128) {

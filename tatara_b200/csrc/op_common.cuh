@@ -77,8 +77,8 @@ static __device__ __forceinline__ float op_group_sum(float v) {
     return v;
 }
 
-// Launches of one call overlap (programmatic dependent launch): a kernel may start before the one ahead of it has finished, and waits for it
-// before it touches what that one writes or reads.
+// Launches overlap, those of one call and those of calls that follow one another on a stream (programmatic dependent launch): every kernel may start before
+// the one ahead of it has finished, and waits for it to end before it touches global memory.  That one has waited for those ahead of itself in the same way.
 static __device__ __forceinline__ void op_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 static __device__ __forceinline__ void op_next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 template <typename... P, typename... A>

@@ -131,6 +131,8 @@ __global__ void __launch_bounds__(32 * WARPS) k_orth_small(OrthIo io, OrthPoly p
     double* s_part = s_q;                    // partial sums of the Gram matrix
     const int64_t per = (m + cs - 1) / cs, begin = min(m, per * rank), end = min(m, begin + per);
 
+    op_next_may_start();
+    op_wait_for_previous();
     __shared__ int s_block[36];  // (bi, bj) of the lower triangle's blocks
     if (tid < blocks) {
         int bi, bj;
@@ -306,12 +308,14 @@ void small_launch(cudaStream_t s, const OrthIo& io, const OrthPoly& p, int n, in
     cfg.blockDim = dim3(32 * WARPS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned)cs;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     cudaLaunchKernelEx(&cfg, k_orth_small<T, WARPS>, io, p, jc_max);
 }
 // Sixteen warps where the products or the loads keep them busy (64 x 512: 44 us, with ten 50, eight 47; 15 of 19 x 2200: 18, 20, 21; 9 of 24 x 1536: 16.0, with eight 17.5), else eight, whose columns

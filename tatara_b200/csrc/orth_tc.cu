@@ -178,6 +178,8 @@ __global__ void __launch_bounds__(256) k_orth_norm(OrthIo io, int64_t segments, 
     __shared__ double s_sum[8];
     const int b = blockIdx.y;
     double sum = 0.0;
+    op_next_may_start();
+    op_wait_for_previous();
     for (int64_t seg = blockIdx.x; seg < segments; seg += gridDim.x) {
         const int64_t r = total ? 0 : seg, c0 = total ? seg * len : 0, end = total ? min(total, c0 + len) : len;
         const T* g = static_cast<const T*>(io.g) + b * io.g_batch + r * io.g_stride;
@@ -206,7 +208,6 @@ __global__ void __launch_bounds__(256) k_orth_norm(OrthIo io, int64_t segments, 
         for (int w = 1; w < 8; ++w) sum += s_sum[w];
         partial[b * OT_NORM_BLOCKS + blockIdx.x] = sum;
     }
-    op_next_may_start();
 }
 
 // One tile per block: X0 = u / (|u| + eps), n x m with n <= m, zeros beyond both.  A thread makes 16-byte pieces of the tile: of N adjacent elements each
@@ -948,7 +949,7 @@ void ot_begin_of(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, const O
     constexpr int W = 16 / (int)sizeof(T);
     const bool flat = !gaps && total % W == 0 && ((uintptr_t)io.g & 15) == 0 && io.g_batch % W == 0 && (((uintptr_t)io.m | (uintptr_t)io.m_out) & 15) == 0;
     const dim3 grid0((unsigned)blocks, (unsigned)io.batch);
-    if (flat) k_orth_norm<T, W, MUON><<<grid0, 256, 0, s>>>(io, segments, len, total, partial); else k_orth_norm<T, N, MUON><<<grid0, 256, 0, s>>>(io, segments, len, total, partial);
+    op_launch_next(s, grid0, dim3(256), 0, flat ? k_orth_norm<T, W, MUON> : k_orth_norm<T, N, MUON>, io, segments, len, total, partial);
     const dim3 grid((unsigned)(p.m_pad / 64), (unsigned)(p.n_pad / 128), (unsigned)io.batch);
     if (io.rows > io.cols) op_launch_next(s, grid, dim3(256), 0, k_orth_pack<T, LIMBS, 1, true, MUON>, io, poly.eps, partial, blocks, x, p.x_limb);
     else op_launch_next(s, grid, dim3(256), 0, k_orth_pack<T, LIMBS, N, false, MUON>, io, poly.eps, partial, blocks, x, p.x_limb);

@@ -172,8 +172,9 @@ k_route_forward(const T* __restrict__ logits, int64_t stride, const uint8_t* __r
     __shared__ float s_z[ROUTE_THREADS / 32];
     const int lane = threadIdx.x % G, group = threadIdx.x / G, wl = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int e = threadIdx.x; e <= experts; e += ROUTE_THREADS) s_count[e] = 0;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *part.ticket = 0;
     op_next_may_start();
+    op_wait_for_previous();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *part.ticket = 0;
     __syncthreads();
     float sum_p[V], sum_z = 0.0f;
 #pragma unroll
@@ -294,6 +295,7 @@ __global__ void __launch_bounds__(1024) k_route_final(RouteParts part, int block
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e0 = blockIdx.x * 32;
     double p = 0.0, z = 0.0;
     int c = 0, n = 0;
+    op_next_may_start();
     op_wait_for_previous();
     if (e0 + lane < experts)
 #pragma unroll 8
@@ -363,6 +365,8 @@ k_route_backward(const T* __restrict__ logits, int64_t stride, const uint8_t* __
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
 #pragma unroll
     for (int v = 0; v < V; ++v) s_add[group][v * G + lane] = 0.0f;
+    op_next_may_start();
+    op_wait_for_previous();
     const float n = (float)max(*n_rows, 1);
     const float db = dlosses ? dlosses[0] : 0.0f, dz = dlosses ? dlosses[1] : 0.0f;
     const float hk = db * (float)experts / (n * (float)k) / n, zk = 2.0f * dz / n;
@@ -472,7 +476,7 @@ void route_forward_go(cudaStream_t s, const void* logits, int64_t stride, const 
         auto kern = wide ? (S && k > 2 ? k_route_forward<T, G, V, VW, S> : k_route_forward<T, G, V, VW, false>)                                 \
                          : (S && k > 2 ? k_route_forward<T, G, V, 1, S> : k_route_forward<T, G, V, 1, false>);                                  \
         if (smem > 40000) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);                                   \
-        kern<<<blocks, ROUTE_THREADS, smem, s>>>((const T*)logits, stride, mask, rows, experts, k, renormalise, index, gate, part);             \
+        op_launch_next(s, dim3((unsigned)blocks), dim3(ROUTE_THREADS), smem, kern, (const T*)logits, stride, mask, rows, experts, k, renormalise, index, gate, part);             \
     } while (0)
     ROUTE_SHAPES(GO)
 #undef GO
@@ -488,7 +492,7 @@ void route_backward_go(cudaStream_t s, const void* logits, int64_t stride, const
     do {                                                                                                                                      \
         constexpr int VW = W < (V) ? W : (V);                                                                                                 \
         auto kern = wide ? k_route_backward<T, G, V, VW> : k_route_backward<T, G, V, 1>;                                                      \
-        kern<<<blocks, 256, 0, s>>>((const T*)logits, stride, mask, rows, experts, k, renormalise, index, gate, dgate, counts, n_rows, dlosses, \
+        op_launch_next(s, dim3((unsigned)blocks), dim3(256), 0, kern, (const T*)logits, stride, mask, rows, experts, k, renormalise, index, gate, dgate, counts, n_rows, dlosses, \
                                     (T*)dlogits, dstride);                                                                                    \
     } while (0)
     ROUTE_SHAPES(GO)

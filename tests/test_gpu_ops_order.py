@@ -1,0 +1,84 @@
+"""Calls that follow one another on a stream overlap at their ends; what one writes, the next one reads.  The same chains with the device idle between the calls,
+on another stream and in a graph give the same bits."""
+import pytest
+
+import tatara_b200 as tb  # noqa: F401
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def ops():
+    from tatara_b200 import ops as o
+    return o
+
+
+def state(rows, n, experts, side, seed):
+    g = torch.Generator("cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    return dict(x=r(rows, n), gate=0.05 * r(experts, n), m=torch.zeros(experts, n, device="cuda"), w=r(side, n), wm=torch.zeros(side, n, device="cuda"), scale=1 + 0.1 * r(n), k=2)
+
+
+def chain(s, turns, between=lambda: None):
+    """Every call reads what the one before it has written, in place where it can; workspaces and outputs are freed and given out again along the way."""
+    for _ in range(turns):
+        y, mean, rstd = ops().layer_norm_forward(s["x"], s["scale"])
+        between()
+        logits = y @ s["gate"].t()
+        r = ops().route_forward(logits, s["k"])
+        between()
+        d = ops().route_backward(logits, r, r.gate, r.losses)
+        between()
+        dx, dw, _ = ops().layer_norm_backward(d @ s["gate"], s["x"], mean, rstd, s["scale"])
+        between()
+        ops().layer_norm_forward(dx, out=dx)
+        between()
+        ops().muon_step(s["gate"], s["m"], d.t() @ y, lr=0.01)
+        between()
+        ops().orthogonalise(s["w"], out=s["w"])
+        between()
+        ops().muon_step(s["w"], s["wm"], s["w"] * dw, lr=0.05)
+        between()
+        ops().layer_norm_forward(s["w"], out=s["w"])
+        between()
+        s["x"].add_(dx, alpha=0.1)
+    return s
+
+
+SHAPES = [(4000, 40, 9, 6), (300, 256, 16, 100), (5000, 1001, 33, 70), (64, 9000, 8, 3)]
+
+
+@pytest.mark.parametrize("rows,n,experts,side", SHAPES)
+def test_calls_in_a_row(rows, n, experts, side):
+    want = chain(state(rows, n, experts, side, 1), 12, torch.cuda.synchronize)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = chain(state(rows, n, experts, side, 1), 12)
+        assert all(torch.equal(got[k], want[k]) for k in ("x", "gate", "m", "w", "wm")) and got["x"].isfinite().all()
+
+
+@pytest.mark.parametrize("rows,n,experts,side", SHAPES[:2])
+def test_calls_in_a_row_on_another_stream_and_in_a_graph(rows, n, experts, side):
+    want = chain(state(rows, n, experts, side, 2), 4, torch.cuda.synchronize)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    s = state(rows, n, experts, side, 2)
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        chain(s, 4)
+    stream.synchronize()
+    assert all(torch.equal(s[k], want[k]) for k in ("x", "gate", "m", "w", "wm"))
+    s = state(rows, n, experts, side, 2)
+    keep = {k: v.clone() for k, v in s.items() if torch.is_tensor(v)}
+    with torch.cuda.stream(stream):
+        chain(s, 1)                      # whatever is set up once, before the capture
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            chain(s, 1)
+        for k, v in keep.items():
+            s[k].copy_(v)
+        for _ in range(4):
+            graph.replay()
+    stream.synchronize()
+    assert all(torch.equal(s[k], want[k]) for k in ("x", "gate", "m", "w", "wm"))
