@@ -302,7 +302,7 @@ void small_launch(cudaStream_t s, const OrthIo& io, const OrthPoly& p, int n, in
     const int64_t per = (m + cs - 1) / cs;
     const int jc_max = per < room ? (int)((per + 7) / 8 * 8) : room;
     const size_t smem = (size_t)(jc_max * pitch + matrices) * sizeof(double);
-    cudaFuncSetAttribute(k_orth_small<T, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMALL_SMEM);
+    if (!small_clusters<T, WARPS>()) cudaFuncSetAttribute(k_orth_small<T, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMALL_SMEM);  // else it is set
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)cs, (unsigned)io.batch);
     cfg.blockDim = dim3(32 * WARPS);

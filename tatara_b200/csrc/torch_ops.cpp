@@ -91,6 +91,23 @@ void* vector_of(PyObject* o, const char* name, const at::Tensor& like, at::IntAr
     return t.data_ptr();
 }
 at::Tensor make(const at::Tensor& like, at::IntArrayRef shape, at::ScalarType type) { return at::detail::empty_cuda(shape, type, like.device(), std::nullopt); }
+// Small results of one call from one allocation (one each costs 0.5 us): places of 128 bytes' alignment, and the tensors there.
+struct Shared {
+    int64_t bytes = 0;
+    at::Tensor base;
+    int64_t place(int64_t elements) {  // 32-bit ones
+        const int64_t at = bytes;
+        bytes += (elements * 4 + 127) / 128 * 128;
+        return at;
+    }
+    void allocate(const at::Tensor& like) { base = make(like, {bytes}, at::kByte); }
+    at::Tensor tensor(int64_t at, at::IntArrayRef shape, at::ScalarType type) const {
+        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(type));
+        t.unsafeGetTensorImpl()->set_storage_offset(at / 4);
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+        return t;
+    }
+};
 // `out`, which has to match `like`, or a new tensor
 at::Tensor output(PyObject* out, const at::Tensor& like) {
     if (out == Py_None) return make(like, like.sizes(), like.scalar_type());
@@ -167,7 +184,11 @@ PyObject* layer_norm_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const float* b = static_cast<float*>(vector_of(a[2], "bias", x, {n}));
     const double eps = number(a[3], "eps");
     const On on(x);
-    const at::Tensor y = output(a[4], x), mean = make(x, {rows}, at::kFloat), rstd = make(x, {rows}, at::kFloat);
+    const at::Tensor y = output(a[4], x);
+    Shared both;
+    const int64_t mean_at = both.place(rows), rstd_at = both.place(rows);
+    both.allocate(x);
+    const at::Tensor mean = both.tensor(mean_at, {rows}, at::kFloat), rstd = both.tensor(rstd_at, {rows}, at::kFloat);
     char err[256];
     check(tb_layer_norm_forward(x.data_ptr(), xs, w, b, (float)eps, type_of(x), rows, side(n, "n"), y.data_ptr(), rows_of(y, "out"), mean.data_ptr<float>(),
                                 rstd.data_ptr<float>(), on.stream, err, sizeof err),
@@ -187,7 +208,11 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) 
     const float* r = static_cast<float*>(vector_of(a[3], "rstd", x, {rows}, at::kFloat, true));
     const float* w = static_cast<float*>(vector_of(a[4], "weight", x, {n}));
     const On on(x);
-    const at::Tensor dx = output(a[5], x), dweight = make(x, {n}, at::kFloat), dbias = make(x, {n}, at::kFloat);
+    const at::Tensor dx = output(a[5], x);
+    Shared both;
+    const int64_t w_at = both.place(n), b_at = both.place(n);
+    both.allocate(x);
+    const at::Tensor dweight = both.tensor(w_at, {n}, at::kFloat), dbias = both.tensor(b_at, {n}, at::kFloat);
     const Work work(x, tb_layer_norm_backward_workspace(rows, side(n, "n")));
     char err[256];
     check(tb_layer_norm_backward(dy.data_ptr(), gs, x.data_ptr(), xs, m, r, w, type_of(x), rows, (int)n, dx.data_ptr(), rows_of(dx, "out"),
@@ -212,8 +237,12 @@ PyObject* route_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (k < 1) refuse("k must be positive (got %d)", k);
     const uint8_t* mask = mask_of(a[3], x);
     const On on(x);
-    const at::Tensor index = make(x, {rows, k}, at::kInt), gate = make(x, {rows, k}, at::kFloat), counts = make(x, {experts}, at::kInt), n = make(x, {1}, at::kInt),
-                     mean = make(x, {experts}, at::kFloat), losses = make(x, {2}, at::kFloat);
+    const at::Tensor index = make(x, {rows, k}, at::kInt), gate = make(x, {rows, k}, at::kFloat);
+    Shared few;
+    const int64_t counts_at = few.place(experts), n_at = few.place(1), mean_at = few.place(experts), losses_at = few.place(2);
+    few.allocate(x);
+    const at::Tensor counts = few.tensor(counts_at, {experts}, at::kInt), n = few.tensor(n_at, {1}, at::kInt), mean = few.tensor(mean_at, {experts}, at::kFloat),
+                     losses = few.tensor(losses_at, {2}, at::kFloat);
     const Work work(x, tb_route_forward_workspace(rows, side(experts, "experts")));
     char err[256];
     check(tb_route_forward(x.data_ptr(), stride, type_of(x), rows, (int)experts, k, truth(a[2]), mask, index.data_ptr<int>(), gate.data_ptr<float>(),

@@ -82,3 +82,24 @@ def test_calls_in_a_row_on_another_stream_and_in_a_graph(rows, n, experts, side)
             graph.replay()
     stream.synchronize()
     assert all(torch.equal(s[k], want[k]) for k in ("x", "gate", "m", "w", "wm"))
+
+
+def test_results_of_one_call_are_tensors_of_their_own():
+    x = torch.randn(37, 19, device="cuda")
+    y, mean, rstd = ops().layer_norm_forward(x)
+    dx, dw, db = ops().layer_norm_backward(y, x, mean, rstd)
+    r = ops().route_forward(x, 3)
+    for group in ((mean, rstd), (dw, db), (r.counts, r.rows, r.prob_mean, r.losses)):
+        keep = [t.clone() for t in group]
+        for i, t in enumerate(group):
+            assert t.is_contiguous() and not t.requires_grad and t.data_ptr() % 128 == 0 and t.device == x.device
+            t.fill_(7)   # touches no other result
+            for j, u in enumerate(group):
+                assert j == i or torch.equal(u, keep[j])
+            t.copy_(keep[i])
+            assert torch.equal((t * 2).cpu(), (keep[i] * 2).cpu()) and torch.equal(t.view(-1)[:1], keep[i][:1])
+    assert r.rows.dtype == r.counts.dtype == torch.int32 and r.losses.dtype == torch.float32 and r.losses.shape == (2,)
+    # a leaf of its own, as any new tensor
+    leaf = dw.requires_grad_()
+    (leaf * leaf).sum().backward()
+    assert torch.equal(leaf.grad, 2 * dw.detach()) and not db.requires_grad
