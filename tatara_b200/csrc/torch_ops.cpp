@@ -1,7 +1,8 @@
 // The operators on torch tensors: checks of the arguments, outputs and workspaces from torch's allocator, torch's current stream, and the entry
 // points of include/tatara_b200.h.  tatara_b200/ops.py documents the functions and calls these.
 //
-// In Python the checks, allocations and the foreign call cost 13 to 24 us of a call, several times what the kernels of a small problem take; here 3 to 6.
+// In Python the checks, allocations and the foreign call cost 13 to 24 us of a call, several times what the kernels of a small problem take; here 2 to 5 beside
+// the launches.
 // Every function takes all of its arguments by position; None stands for a tensor that is not given.  Wrong arguments raise
 // tatara_b200.TrainerError, what torch raises (memory) stays as it is.
 #include <torch/csrc/Exceptions.h>

@@ -4,8 +4,8 @@ orthogonalisation and the Muon step.
 The functions check their arguments, take outputs and workspaces from torch's allocator and enqueue kernels of libtatara_b200.so on torch's current
 stream of the tensors' device (csrc/torch_ops.cpp).  Nothing is synchronised and nothing is kept between calls.  Wrong arguments raise
 `TrainerError`.  Small results of one call (mean and rstd; dweight and dbias; a routing's counts, rows, prob_mean and losses) are parts of one
-allocation: clone what is to outlive the others by long.  Gradients are what the *_backward functions return; torch's automatic differentiation does not see these calls.  This module needs
-torch; the rest of the package does not.
+allocation: clone what is to outlive the others by long.  Gradients are what the *_backward functions return; torch's automatic differentiation
+does not see these calls.  This module needs torch; the rest of the package does not.
 """
 from __future__ import annotations
 
