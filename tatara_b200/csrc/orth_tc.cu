@@ -19,7 +19,8 @@
 // cores truncate when they add to an accumulator: with two limbs that left 2.5e-5 of the result after five steps of K = 1000, 1.4e-5 with a new accumulator
 // every 256 columns of K.  So it changes with every chunk of 64, which adds the small products first and the four large ones last, and the
 // warps add what it held to their registers, rounded to nearest, while the next one fills.
-// Every wait is bounded; where one runs out the block's results become NaN, and so the output.
+// Every wait is bounded.  An accumulator is announced only when all of its MMAs were issued on operands that have arrived; a warp that waits in vain for one
+// takes NaN for it, and stores those once the copies and MMAs that were under way are done: what a block stores is right or NaN.
 //
 // Measured, 4096 x 4096 in fp32: Gram 159 us, square 168, apply 293 (1.4 PFLOP/s of limb products, tensor pipe 78 to 92 % busy), last product with
 // the weight update 334; the whole Muon step 3.3 to 3.8 ms, where the chip's power limit, not the kernel, sets the clock.  bf16: 1.15 ms.  Small
@@ -33,15 +34,21 @@ namespace {
 #define OT_TILE 16384           // bytes of a tile of 128 x 64 fp16
 #define OT_SCALE 2048.0f
 #define OT_UNSCALE (1.0f / (2048.0f * 2048.0f))
-#define OT_WAIT_LIMIT (1 << 20)
 #define OT_PARTS 8             // most parts of a Gram product
 #define OT_NORM_BLOCKS 512      // most partial sums of squares per matrix
 enum { OT_GRAM = 0, OT_SQUARE = 1, OT_APPLY = 2, OT_LAST = 3, OT_GRAM_PART = 4 };
+// Who waits: the warp that copies, the one that issues the MMAs, the odd block's that tells it of its operands, those that read the accumulators; and any of
+// them, in the end, for what is under way.
+enum { OT_COPIES = 0, OT_PRODUCTS = 1, OT_RELAY = 2, OT_SUMS = 3, OT_END = 4 };
+#ifndef OT_WAIT_LIMIT  // tries before a wait gives up; the last one outlasts the others
+#define OT_WAIT_LIMIT(role) ((role) == OT_END ? 1 << 22 : 1 << 20)
+#endif
 
 __device__ __forceinline__ unsigned ot_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void ot_bar_init(unsigned bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+template <int ROLE>
 __device__ __forceinline__ bool ot_wait(unsigned bar, unsigned parity) {
-    for (int i = 0; i < OT_WAIT_LIMIT; ++i) {
+    for (int i = 0; i < OT_WAIT_LIMIT(ROLE); ++i) {
         unsigned ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -395,8 +402,8 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
     constexpr bool SYM = KIND == OT_GRAM || KIND == OT_SQUARE || KIND == OT_GRAM_PART;
     extern __shared__ uint8_t s_raw[];
     __shared__ __align__(8) unsigned long long s_full[S::STAGES], s_peer[S::STAGES], s_empty[S::STAGES], s_acc_full[2], s_acc_empty[2];
+    __shared__ __align__(8) unsigned long long s_quiet;  // this block's copies have landed and the pair's MMAs are done
     __shared__ unsigned s_tmem;
-    __shared__ int s_failed;
     uint8_t* s_dyn = s_raw + ((1024u - (ot_smem(s_raw) & 1023u)) & 1023u);
     const unsigned ring = ot_smem(s_dyn);
     // the warp's number is the same in its lanes, and the compiler has to know it: what the MMAs take lives in uniform registers then
@@ -414,8 +421,8 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
             ot_bar_init(ot_smem(&s_acc_full[q]), 1);
             ot_bar_init(ot_smem(&s_acc_empty[q]), 8 * CTAS);
         }
+        ot_bar_init(ot_smem(&s_quiet), 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        s_failed = 0;
     }
     if (warp == 9) {
         if (CTAS == 2) {
@@ -454,7 +461,7 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
             const unsigned bytes = LIMBS * (same ? OT_TILE : W == 1 ? OT_TILE + HALF : 2 * OT_TILE);
             for (int k = 0; k < chunks; ++k, ++count) {
                 const unsigned bar = ot_smem(&s_full[0]) + 8 * s, to = ring + s * S::STAGE;
-                ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_empty[0]) + 8 * s, parity));
+                ok = __all_sync(0xffffffffu, ot_wait<OT_COPIES>(ot_smem(&s_empty[0]) + 8 * s, parity));
                 if (!ok) break;
                 if (lane == 0) {
                     ot_expect(bar, bytes);
@@ -476,10 +483,9 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                 }
             }
         }
-        if (!ok) {  // the copies in flight land before the block ends
-            if (lane == 0) atomicExch(&s_failed, 1);
-            for (int64_t q = count < S::STAGES ? 0 : count - S::STAGES; q < count; ++q) ot_wait(ot_smem(&s_full[q % S::STAGES]), (unsigned)((q / S::STAGES) & 1));
-        }
+        // whoever gave up: the copies land before the block ends
+        for (int64_t q = count < S::STAGES ? 0 : count - S::STAGES; q < count; ++q) ot_wait<OT_END>(ot_smem(&s_full[q % S::STAGES]), (unsigned)((q / S::STAGES) & 1));
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ot_smem(&s_quiet)) : "memory");
     } else if (warp == 9) {
         unsigned s = 0, parity = 0;
         if (rank == 0) {
@@ -499,13 +505,13 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                 int k = 0;
                 for (int r = 0; r < rounds && ok; ++r) {
                     const unsigned d = tmem + buffer * TN;
-                    ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_acc_empty[0]) + 8 * buffer, drained));
+                    ok = __all_sync(0xffffffffu, ot_wait<OT_PRODUCTS>(ot_smem(&s_acc_empty[0]) + 8 * buffer, drained));
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const int last = min(chunks, k + S::DRAIN);
                     unsigned accumulate = 0;
                     for (; ok && k < last; ++k) {
-                        ok = ot_wait(ot_smem(&s_full[0]) + 8 * s, parity);
-                        if (CTAS == 2) ok = ok && ot_wait(ot_smem(&s_peer[0]) + 8 * s, parity);
+                        ok = ot_wait<OT_PRODUCTS>(ot_smem(&s_full[0]) + 8 * s, parity);
+                        if (CTAS == 2) ok = ok && ot_wait<OT_PRODUCTS>(ot_smem(&s_peer[0]) + 8 * s, parity);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -526,17 +532,18 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                             parity ^= 1;
                         }
                     }
-                    if (leader) ot_commit<CTAS>(ot_smem(&s_acc_full[0]) + 8 * buffer);
+                    if (leader && ok) ot_commit<CTAS>(ot_smem(&s_acc_full[0]) + 8 * buffer);
                     __syncwarp();
                     drained ^= buffer;
                     buffer ^= 1;
                 }
             }
+            if (leader) ot_commit<CTAS>(ot_smem(&s_quiet));
         } else {
             // the odd block: tells the even one that its operands are there
             for (int t = first; ok && t < total; t += MULTI ? step : total)
                 for (int k = 0; k < chunks && ok; ++k) {
-                    ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_full[0]) + 8 * s, parity));
+                    ok = __all_sync(0xffffffffu, ot_wait<OT_RELAY>(ot_smem(&s_full[0]) + 8 * s, parity));
                     if (ok && lane == 0) ot_arrive_at(ot_smem(&s_peer[0]) + 8 * s, 0);
                     __syncwarp();
                     if (++s == S::STAGES) {
@@ -545,7 +552,7 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                     }
                 }
         }
-        if (!ok && lane == 0) atomicExch(&s_failed, 1);
+        ot_wait<OT_END>(ot_smem(&s_quiet), 0);
     } else {
         const unsigned taddr = tmem + ((unsigned)((warp & 3) * 32) << 16) + (unsigned)((warp >> 2) * COLS);
         const int group = warp >> 2, row = tid & 127;
@@ -556,7 +563,7 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
 #pragma unroll
             for (int c = 0; c < COLS; ++c) acc[c] = 0.0f;
             for (int r = 0; r < rounds && ok; ++r) {
-                ok = __all_sync(0xffffffffu, ot_wait(ot_smem(&s_acc_full[0]) + 8 * buffer, filled));
+                ok = __all_sync(0xffffffffu, ot_wait<OT_SUMS>(ot_smem(&s_acc_full[0]) + 8 * buffer, filled));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
@@ -575,8 +582,8 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                 filled ^= buffer;
                 buffer ^= 1;
             }
-            if (!ok && lane == 0) atomicExch(&s_failed, 1);
-            if (!ok || *static_cast<volatile int*>(&s_failed)) {
+            if (!ok) {
+                ot_wait<OT_END>(ot_smem(&s_quiet), 0);  // what is stored may pass through the ring
 #pragma unroll
                 for (int c = 0; c < COLS; ++c) acc[c] = __int_as_float(0x7fc00000);
             }
