@@ -234,7 +234,7 @@ k_norm_forward_down(const T* x, int64_t x_stride, const float* __restrict__ weig
     }
 }
 
-// rows longer than NORM_REG_N: a block per row, three passes over it
+// rows longer than NORM_REG_N: a block per row, three passes over it.  Columns of long rows are unsigned: the last step goes beyond 2^31.
 template <typename T>
 __global__ void __launch_bounds__(1024)
 k_norm_forward_long(const T* x, int64_t x_stride, const float* __restrict__ weight, const float* __restrict__ bias, float eps, int n,
@@ -246,9 +246,9 @@ k_norm_forward_long(const T* x, int64_t x_stride, const float* __restrict__ weig
     float sum = 0.0f, sq = 0.0f;
     op_next_may_start();
     op_wait_for_previous();
-    for (int c = threadIdx.x; c < n; c += 1024) sum += op_float(xr[c]);
+    for (unsigned c = threadIdx.x; c < (unsigned)n; c += 1024) sum += op_float(xr[c]);
     const float mean = norm_row_sum<32>(sum, s_sum[0], warp, lane) / (float)n;
-    for (int c = threadIdx.x; c < n; c += 1024) {
+    for (unsigned c = threadIdx.x; c < (unsigned)n; c += 1024) {
         const float d = op_float(xr[c]) - mean;
         sq = fmaf(d, d, sq);
     }
@@ -258,7 +258,7 @@ k_norm_forward_long(const T* x, int64_t x_stride, const float* __restrict__ weig
         if (rstd_out) rstd_out[row] = rstd;
     }
     T* yr = y + row * y_stride;
-    for (int c = threadIdx.x; c < n; c += 1024)
+    for (unsigned c = threadIdx.x; c < (unsigned)n; c += 1024)
         yr[c] = op_round<T>(fmaf((op_float(xr[c]) - mean) * rstd, weight ? weight[c] : 1.0f, bias ? bias[c] : 0.0f));
 }
 
@@ -437,14 +437,14 @@ k_norm_backward_long(const T* dy, int64_t dy_stride, const T* x, int64_t x_strid
     op_wait_for_previous();
     const float mu = mean[row], r = rstd[row];
     float s1 = 0.0f, s2 = 0.0f;
-    for (int c = threadIdx.x; c < n; c += 1024) {
+    for (unsigned c = threadIdx.x; c < (unsigned)n; c += 1024) {
         const float xh = (op_float(xr[c]) - mu) * r, t = op_float(gr[c]) * (weight ? weight[c] : 1.0f);
         s1 += t;
         s2 = fmaf(t, xh, s2);
     }
     const float m1 = norm_row_sum<32>(s1, s_sum[0], warp, lane) / (float)n, m2 = norm_row_sum<32>(s2, s_sum[1], warp, lane) / (float)n;
     T* dr = dx + row * dx_stride;
-    for (int c = threadIdx.x; c < n; c += 1024) {
+    for (unsigned c = threadIdx.x; c < (unsigned)n; c += 1024) {
         const float xh = (op_float(xr[c]) - mu) * r, t = op_float(gr[c]) * (weight ? weight[c] : 1.0f);
         dr[c] = op_round<T>(r * (t - m1 - xh * m2));
     }
@@ -453,10 +453,10 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 k_norm_columns_long(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x, int64_t x_stride, const float* __restrict__ mean,
                     const float* __restrict__ rstd, int64_t rows, int n, float* __restrict__ part_w, float* __restrict__ part_b) {
-    const int col = blockIdx.x * 256 + threadIdx.x;
+    const unsigned col = blockIdx.x * 256 + threadIdx.x;
     op_next_may_start();
     op_wait_for_previous();
-    if (col >= n) return;
+    if (col >= (unsigned)n) return;
     float aw = 0.0f, ab = 0.0f;
     for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
         const float g = op_float(dy[row * dy_stride + col]);
@@ -475,11 +475,12 @@ __global__ void __launch_bounds__(1024) k_norm_columns_final(const float* __rest
     float* out = blockIdx.y ? dbias : dweight;
     op_next_may_start();
     if (!out) return;  // of the same block all
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = threadIdx.x & 7, col = blockIdx.x * 8 + c;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = threadIdx.x & 7;
+    const unsigned col = blockIdx.x * 8 + c;
     const float* p = partial + (int64_t)blockIdx.y * prows * n;
     float v = 0.0f;
     op_wait_for_previous();
-    if (col < n)
+    if (col < (unsigned)n)
         for (int r0 = threadIdx.x >> 3; r0 < prows; r0 += 128 * 8) {
             float t[8];
 #pragma unroll
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(1024) k_norm_columns_final(const float* __rest
     __syncthreads();
     if (warp >= 8) return;
     v = op_group_sum<32>(s_sum[lane][warp]);
-    if (lane == 0 && blockIdx.x * 8 + warp < n) out[blockIdx.x * 8 + warp] = v;
+    if (lane == 0 && blockIdx.x * 8 + warp < (unsigned)n) out[blockIdx.x * 8 + warp] = v;
 }
 
 // Warps per row of the kernels that walk down the rows: the fewest that hold it with eight columns a thread (up to 4096 columns, two rows at a time),
@@ -587,7 +588,7 @@ void norm_backward_pick(const NormBackward& a) {
     if (a.n > NORM_REG_N_BACK) {
         // the columns first: dx may be dy's or x's memory
         if (a.part_w)
-            op_launch_next(a.s, dim3((unsigned)ceil_div(a.n, 256), (unsigned)a.blocks), dim3(256), 0, k_norm_columns_long<T>, (const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.rows, a.n, a.part_w,
+            op_launch_next(a.s, dim3((unsigned)ceil_div64(a.n, 256), (unsigned)a.blocks), dim3(256), 0, k_norm_columns_long<T>, (const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.rows, a.n, a.part_w,
                                                                                                              a.part_b);
         op_launch_next(a.s, dim3((unsigned)a.rows), dim3(1024), 0, k_norm_backward_long<T>, (const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.w, a.n, (T*)a.dx, a.dxs);
     } else if (a.n <= 64) {
@@ -666,6 +667,6 @@ extern "C" int tb_layer_norm_backward(const void* d_dy, int64_t dy_stride, const
     if (type == TB_TYPE_F32) wide ? norm_backward_pick<float, 4>(a) : norm_backward_pick<float, 1>(a);
     else if (type == TB_TYPE_F16) wide ? norm_backward_pick<__half, 8>(a) : norm_backward_pick<__half, 1>(a);
     else wide ? norm_backward_pick<__nv_bfloat16, 8>(a) : norm_backward_pick<__nv_bfloat16, 1>(a);
-    if (columns && !direct) op_launch_next(s, dim3((unsigned)ceil_div(n, 8), 2), dim3(1024), 0, k_norm_columns_final, partial, blocks, n, d_dweight, d_dbias);
+    if (columns && !direct) op_launch_next(s, dim3((unsigned)ceil_div64(n, 8), 2), dim3(1024), 0, k_norm_columns_final, partial, blocks, n, d_dweight, d_dbias);
     return op_launched(err, err_len);
 }

@@ -4,6 +4,7 @@ Tolerances count roundings of fp32 (u = 2^-24).  A row's sum runs through at mos
 additions, so L = n / 32 + 11 bounds its relative error in u; a column's sum through at most `rows` + 40 terms.
 """
 import ctypes as C
+import math
 
 import pytest
 
@@ -251,3 +252,26 @@ def test_gradients_of_few_rows(rows, n):
         for t, used, want in ((dw, use_w, got[1]), (db, use_b, got[2])):
             assert torch.equal(t[off:off + n], want) if used else (t == 7).all()
             assert (t[:off] == 7).all() and (t[off + n:] == 7).all()
+
+
+def test_rows_of_two_to_the_31():
+    """The longest rows that are taken, 2^31 - 5 columns, in numbers that leave nothing to round: columns of 1 and -1 in turn."""
+    n = 2 ** 31 - 5
+    if torch.cuda.mem_get_info()[0] < 130 << 30:
+        pytest.skip("needs 130 GB of free device memory")
+    half = lambda *s: torch.empty(*s, dtype=torch.float16, device="cuda")  # noqa: E731
+    x, dy = half(2, n), half(2, n)
+    x[:, 0::2], x[:, 1::2] = 1, -1
+    x[1].neg_()
+    y, mean, rstd = ops().layer_norm_forward(x, eps=EPS)   # mean 1 / n, deviation 1: rounded to 11 bits the row itself
+    assert torch.equal(y, x) and mean.abs().max() <= 1e-8 and (rstd - 1 / math.sqrt(1 + EPS)).abs().max() <= 1e-6
+    dy[0], dy[1] = x[0], 1
+    del mean, rstd
+    mean, rstd = torch.zeros(2, device="cuda"), torch.tensor([0.5, 1.0], device="cuda")
+    dx, dw, db = ops().layer_norm_backward(dy, x, mean, rstd, out=y)
+    # row 0: t = x, xh = x / 2, so dx = (x - x / 4) / 2; row 1: t = 1 and xh of mean zero, so nothing is left
+    assert (dx[0, 0::2] == 0.375).all() and (dx[0, 1::2] == -0.375).all() and dx[1].abs().max() <= 1e-6
+    assert (dw[0::2] == -0.5).all() and (dw[1::2] == 1.5).all()
+    assert (db[0::2] == 2).all() and (db[1::2] == 0).all()
+    del x, dy, y, dx, dw, db
+    torch.cuda.empty_cache()
