@@ -354,11 +354,12 @@ __global__ void __launch_bounds__(1024) k_route_final(RouteParts part, int block
     *rows_out = n;
 }
 
+// dlogits may be the logits: a group reads its row before it writes it
 template <typename T, int G, int V, int VEC>
 __global__ void __launch_bounds__(256)
-k_route_backward(const T* __restrict__ logits, int64_t stride, const uint8_t* __restrict__ mask, int64_t rows, int experts, int k, int renormalise,
+k_route_backward(const T* logits, int64_t stride, const uint8_t* __restrict__ mask, int64_t rows, int experts, int k, int renormalise,
                  const int* __restrict__ index, const float* __restrict__ gate, const float* __restrict__ dgate, const int* __restrict__ counts,
-                 const int* __restrict__ n_rows, const float* __restrict__ dlosses, T* __restrict__ dlogits, int64_t dstride) {
+                 const int* __restrict__ n_rows, const float* __restrict__ dlosses, T* dlogits, int64_t dstride) {
     constexpr int GROUPS = 256 / G, SLOTS = ROUTE_MAX_K > G ? ROUTE_MAX_K / G : 1;
     // the gates' part of a group's row: zero but while the chosen experts' lanes pass it to the lanes that hold those logits
     __shared__ __align__(16) float s_add[GROUPS][G * V];

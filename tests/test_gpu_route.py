@@ -218,3 +218,21 @@ def test_refusals():
     p = x.data_ptr()
     assert lib.tb_route_forward(p, 8, 0, 4, 8, 2, 1, None, p, p, p, p, p, p, p, 0, None, None, 0) == -1
     assert lib.tb_route_forward_workspace(4, 0) == -1 and lib.tb_route_forward_workspace(-1, 8) == -1
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,experts,k,offset", [(20001, 9, 2, 0), (20001, 12, 4, 0), (9001, 48, 8, 0), (9001, 47, 8, 1), (5003, 128, 4, 0), (5003, 256, 8, 0), (3001, 255, 8, 3), (777, 1024, 16, 0)])
+def test_gradient_over_the_logits(rows, experts, k, offset, dtype):
+    """dlogits in the logits' memory, through the C entry point: the bits of a result of its own."""
+    wide = torch.full((rows, experts + offset), 3.0, dtype=dtype, device="cuda")
+    x = wide[:, offset:]
+    x.copy_(make(rows, experts, dtype, 3, forbidden=0.1))
+    mask = torch.rand(rows, device="cuda") > 0.2
+    r = ops().route_forward(x, k, mask=mask)
+    dgate, dl = torch.randn(rows, k, device="cuda"), torch.tensor([0.7, 0.3], device="cuda")
+    want = ops().route_backward(x, r, dgate, dl, mask=mask)
+    kind = TYPES.index(dtype)
+    rc = tb.load_library().tb_route_backward(x.data_ptr(), x.stride(0), kind, rows, experts, k, 1, mask.data_ptr(), r.index.data_ptr(), r.gate.data_ptr(), dgate.data_ptr(),
+                                             r.counts.data_ptr(), r.rows.data_ptr(), dl.data_ptr(), x.data_ptr(), x.stride(0), torch.cuda.current_stream().cuda_stream, None, 0)
+    assert rc == 0
+    assert torch.equal(x, want) and (wide[:, :offset] == 3).all()
