@@ -357,9 +357,16 @@ bool orth_bounded(const OrthPoly& p) {
     return true;
 }
 
+// More elements than any device holds are refused, before the sizes of what is derived from them could wrap.
+#define ORTH_MAX_ELEMENTS (1LL << 40)
+bool orth_sizes(int batch, int rows, int cols) {
+    return batch >= 0 && batch <= 65535 && rows >= 1 && cols >= 1 && (int64_t)rows * cols <= ORTH_MAX_ELEMENTS / (batch > 0 ? batch : 1);
+}
+
 int orth_check(int type, int batch, int rows, int cols, const OrthPoly& p, char* err, size_t err_len) {
     if (!op_type_size(type)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "type must be TB_TYPE_F32, TB_TYPE_F16 or TB_TYPE_BF16 (got %d)", type);
-    if (batch < 0 || batch > 65535 || rows < 1 || cols < 1) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "batch must be in [0, 65535], rows and cols positive");
+    if (!orth_sizes(batch, rows, cols))
+        return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "batch must be in [0, 65535], rows and cols positive, and batch * rows * cols at most 2^40");
     if (p.steps < 1 || p.steps > 32) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "steps must be in [1, 32] (got %d)", p.steps);
     if (!(p.eps >= 0.0f)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "eps must not be negative");
     if (!orth_bounded(p)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "with these coefficients singular values could grow beyond 4, or the factors beyond 31");
@@ -388,7 +395,7 @@ void launch_orth_small(cudaStream_t s, const OrthIo& io, const OrthPoly& p, int 
 }
 
 extern "C" int64_t tb_orthogonalise_workspace(int type, int batch, int rows, int cols) {
-    if (!op_type_size(type) || batch < 0 || batch > 65535 || rows < 1 || cols < 1) return TB_ERR_INVALID_ARGUMENT;
+    if (!op_type_size(type) || !orth_sizes(batch, rows, cols)) return TB_ERR_INVALID_ARGUMENT;
     return orth_workspace(orth_limbs(type), batch, rows, cols);
 }
 
@@ -421,7 +428,7 @@ extern "C" int tb_orthogonalise(const void* d_x, int64_t x_batch, int64_t x_stri
 }
 
 extern "C" int64_t tb_muon_step_workspace(int batch, int rows, int cols) {
-    if (batch < 0 || batch > 65535 || rows < 1 || cols < 1) return TB_ERR_INVALID_ARGUMENT;
+    if (!orth_sizes(batch, rows, cols)) return TB_ERR_INVALID_ARGUMENT;
     return orth_workspace(2, batch, rows, cols);
 }
 

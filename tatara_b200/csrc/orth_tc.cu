@@ -826,7 +826,8 @@ __global__ void __launch_bounds__(256) k_orth_join(const float* __restrict__ par
 struct OtPlan {
     int sym, all;                            // columns of a tile of the symmetric products and of Q X, in 64s
     int parts;                               // of K in the Gram product
-    int n, m, n_pad, m_pad;
+    int n, m;
+    int64_t n_pad, m_pad;
     int64_t x_limb, a_limb;                  // bytes of a limb
     int64_t x0, x1, a, q, part, total;       // offsets in the workspace
 };
@@ -841,7 +842,8 @@ OtPlan ot_plan(int batch, int rows, int cols, int limbs) {
     OtPlan p;
     p.n = rows < cols ? rows : cols;
     p.m = rows < cols ? cols : rows;
-    const int64_t n1 = (p.n + 127) / 128, n2 = (p.n + 255) / 256, m1 = (p.m + 127) / 128, m2 = (p.m + 255) / 256, kn = (p.n + 63) / 64, km = (p.m + 63) / 64;
+    const int64_t n = p.n, m = p.m;  // m + 255 may be beyond 2^31
+    const int64_t n1 = (n + 127) / 128, n2 = (n + 255) / 256, m1 = (m + 127) / 128, m2 = (m + 255) / 256, kn = (n + 63) / 64, km = (m + 63) / 64;
     int64_t best = 0, sym_best = 0;
     for (int w = 1; w <= 4; w *= 2) {
         const int64_t sym = batch * (w == 4 ? n2 * (n2 + 1) / 2 : n1 * (n1 + 1) / (w == 1 ? 1 : 2)), all = batch * (w == 4 ? n2 * m2 : w == 2 ? n1 * m1 : 2 * n1 * m1);
@@ -859,10 +861,10 @@ OtPlan ot_plan(int batch, int rows, int cols, int limbs) {
         if (q > 1 && (km - km / q) * ot_chunk(limbs, 1) > 9000) p.parts = (int)q;
     }
     const int pad = p.sym == 4 || p.all == 4 ? 256 : 128;
-    p.n_pad = (p.n + pad - 1) / pad * pad;
-    p.m_pad = (int)(((int64_t)p.m + pad - 1) / pad * pad);
-    p.x_limb = (int64_t)p.n_pad * p.m_pad * 2;
-    p.a_limb = (int64_t)p.n_pad * p.n_pad * 2;
+    p.n_pad = (n + pad - 1) / pad * pad;
+    p.m_pad = (m + pad - 1) / pad * pad;
+    p.x_limb = p.n_pad * p.m_pad * 2;
+    p.a_limb = p.n_pad * p.n_pad * 2;
     p.x0 = ((int64_t)batch * OT_NORM_BLOCKS * 8 + 127) / 128 * 128;
     p.x1 = p.x0 + p.x_limb * limbs * batch;
     p.a = p.x1 + p.x_limb * limbs * batch;
@@ -921,9 +923,9 @@ void ot_gemm(cudaStream_t s, const OtGemm& g, const OrthIo& io, int w, int parts
 template <typename T, int LIMBS>
 void ot_steps(cudaStream_t s, const OrthIo& io, const OrthPoly& poly, uint8_t* work, const OtPlan& p) {
     uint8_t *x = work + p.x0, *y = work + p.x1, *a = work + p.a, *q = work + p.q;
-    const int wn = p.n_pad / 64, wm = p.m_pad / 64, kn = (p.n + 63) / 64, km = (p.m + 63) / 64;
+    const int wn = (int)(p.n_pad / 64), wm = (int)(p.m_pad / 64), kn = (int)ceil_div64(p.n, 64), km = (int)ceil_div64(p.m, 64);
     const int sym_rows = p.sym == 4 ? 256 : 128, all_rows = p.all == 4 ? 256 : 128;
-    const int st = (p.n + sym_rows - 1) / sym_rows, rt = (p.n + all_rows - 1) / all_rows, ct = (p.m + all_rows - 1) / all_rows * (p.all == 1 ? 2 : 1);
+    const int st = (int)ceil_div64(p.n, sym_rows), rt = (int)ceil_div64(p.n, all_rows), ct = (int)ceil_div64(p.m, all_rows) * (p.all == 1 ? 2 : 1);
     float* part = reinterpret_cast<float*>(work + p.part);
     for (int k = 0; k < poly.steps; ++k) {
         const OtGemm gram = {x, x, a, p.x_limb, p.x_limb, p.a_limb, wm, wm, wn, km, st, st, 0.f, 0.f, 0.f, part};

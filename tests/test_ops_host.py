@@ -149,3 +149,21 @@ def test_torch_binding_refuses_host_tensors():
                 lambda: ops.muon_step(x, x, x, lr=0.1), lambda: ops.layer_norm_backward(x, x, x, x)):
         with pytest.raises(tb.TrainerError, match="CUDA tensor"):
             bad()
+
+
+@pytest.mark.parametrize("type_,limbs", [(0, 2), (1, 2), (2, 1)])
+def test_workspaces_of_the_longest_matrices(type_, limbs):
+    """What is derived from sides near 2^31 does not wrap: two X of padded tiles, A and Q at least."""
+    most = 2 ** 31 - 1
+    for rows, cols in ((65, most), (most, 65), (65, most - 255), (500, most), (2 ** 20, 2 ** 20)):
+        n, m = min(rows, cols), max(rows, cols)
+        need = lib().tb_orthogonalise_workspace(type_, 1, rows, cols)
+        assert need >= 2 * 2 * limbs * (n * m + n * n), (rows, cols)
+        assert need <= 2 * 2 * limbs * ((n + 255) * (m + 255) + (n + 255) ** 2) + 8 * 65536 * 128 + 8192
+        e = err()
+        assert lib().tb_orthogonalise(P, 0, cols, type_, 1, rows, cols, 5, COEF, 1e-7, P, 0, cols, P, need - 1, None, e, 200) == INVALID and b"workspace" in e.value
+    assert lib().tb_orthogonalise_workspace(type_, 1, 64, most) == 0
+    for batch, rows, cols in ((1, most, most), (2, 2 ** 20, 2 ** 20), (65535, 2 ** 20, 64), (1, 2 ** 20 + 1, 2 ** 20)):
+        assert lib().tb_orthogonalise_workspace(type_, batch, rows, cols) == INVALID and lib().tb_muon_step_workspace(batch, rows, cols) == INVALID
+        e = err()
+        assert lib().tb_orthogonalise(P, rows * cols, cols, type_, batch, rows, cols, 5, COEF, 1e-7, P, rows * cols, cols, P, 1 << 62, None, e, 200) == INVALID and b"2^40" in e.value
