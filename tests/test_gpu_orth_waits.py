@@ -51,8 +51,9 @@ def waits(tmp_path_factory):
         pytest.skip("nvcc is not installed")
     at = tmp_path_factory.mktemp("waits")
     (at / "waits.cu").write_text(SOURCE)
-    lib = str(at / "waits.so")
-    r = subprocess.run([nvcc] + build.NVCC_FLAGS + ["-I", os.path.join(ROOT, "tatara_b200", "csrc"), "-shared", str(at / "waits.cu"), "-o", lib], capture_output=True, text=True)
+    lib = str(at / "waits.so")  # bound to its own functions: the package's library has the same ones in the global scope
+    r = subprocess.run([nvcc] + build.NVCC_FLAGS + ["-I", os.path.join(ROOT, "tatara_b200", "csrc"), "-shared", "-Xlinker", "-Bsymbolic", str(at / "waits.cu"), "-o", lib],
+                       capture_output=True, text=True)
     assert r.returncode == 0, r.stderr[-2000:]
     lib = C.CDLL(lib)
     lib.waits_workspace.restype = C.c_longlong
