@@ -619,7 +619,7 @@ extern "C" int tb_layer_norm_forward(const void* d_x, int64_t x_stride, const fl
     if (rows == 0) return TB_OK;
     if (!d_x || !d_y) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_x or d_y is NULL");
     if (rows > 1 && (x_stride < n || y_stride < n)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "row strides must be at least n");
-    if (((uintptr_t)d_x | (uintptr_t)d_y) % size || ((uintptr_t)d_weight | (uintptr_t)d_bias) & 3) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
+    if (((uintptr_t)d_x | (uintptr_t)d_y) % size || ((uintptr_t)d_weight | (uintptr_t)d_bias | (uintptr_t)d_mean | (uintptr_t)d_rstd) & 3) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
     if (!op_apart(d_x, 0, x_stride, d_y, 0, y_stride, 1, rows, n, size)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_y overlaps d_x in part");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = n % (16 / size) == 0 && norm_aligned(d_x, x_stride, size) && norm_aligned(d_y, y_stride, size) && (((uintptr_t)d_weight | (uintptr_t)d_bias) & 15) == 0;
@@ -644,7 +644,9 @@ extern "C" int tb_layer_norm_backward(const void* d_dy, int64_t dy_stride, const
     if (rows < 0 || rows > NORM_MAX_ROWS || n < 1) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "rows must be in [0, 2^31) and n positive");
     if (rows > 0 && (!d_dy || !d_x || !d_mean || !d_rstd || !d_dx)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "a device pointer is NULL");
     if (rows > 1 && (dy_stride < n || x_stride < n || dx_stride < n)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "row strides must be at least n");
-    if (((uintptr_t)d_dy | (uintptr_t)d_x | (uintptr_t)d_dx) % size || ((uintptr_t)d_weight & 3)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "rows must be aligned to their elements");
+    if (((uintptr_t)d_dy | (uintptr_t)d_x | (uintptr_t)d_dx) % size ||
+        ((uintptr_t)d_weight | (uintptr_t)d_mean | (uintptr_t)d_rstd | (uintptr_t)d_dweight | (uintptr_t)d_dbias) & 3)
+        return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
     if (rows > 0 && (!op_apart(d_dy, 0, dy_stride, d_dx, 0, dx_stride, 1, rows, n, size) || !op_apart(d_x, 0, x_stride, d_dx, 0, dx_stride, 1, rows, n, size)))
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_dx overlaps d_dy or d_x in part");
     const bool columns = d_dweight || d_dbias;

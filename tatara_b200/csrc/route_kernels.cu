@@ -532,6 +532,8 @@ extern "C" int tb_route_forward(const void* d_logits, int64_t stride, int type, 
     if (rc != TB_OK) return rc;
     if ((rows > 0 && (!d_index || !d_gate)) || !d_counts || !d_rows || !d_prob_mean || !d_losses)
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "an output pointer is NULL");
+    if (((uintptr_t)d_index | (uintptr_t)d_gate | (uintptr_t)d_counts | (uintptr_t)d_rows | (uintptr_t)d_prob_mean | (uintptr_t)d_losses) & 3)
+        return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "outputs must be aligned to their elements");
     const int64_t need = tb_route_forward_workspace(rows, experts);
     if (!d_work || work_bytes < need || ((uintptr_t)d_work & 7))
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "the workspace must be aligned and hold %lld bytes (got %lld)", (long long)need, (long long)work_bytes);
@@ -562,7 +564,9 @@ extern "C" int tb_route_backward(const void* d_logits, int64_t stride, int type,
     if (rows == 0) return TB_OK;
     if (!d_index || !d_gate || !d_counts || !d_rows || !d_dlogits) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "a device pointer is NULL");
     if (rows > 1 && dstride < experts) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "the row stride must be at least experts");
-    if ((uintptr_t)d_dlogits % op_type_size(type)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_dlogits must be aligned to its elements");
+    if ((uintptr_t)d_dlogits % op_type_size(type) ||
+        ((uintptr_t)d_index | (uintptr_t)d_gate | (uintptr_t)d_dgate | (uintptr_t)d_counts | (uintptr_t)d_rows | (uintptr_t)d_dlosses) & 3)
+        return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
     if (!op_apart(d_logits, 0, stride, d_dlogits, 0, dstride, 1, rows, experts, op_type_size(type))) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_dlogits overlaps d_logits in part");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = route_wide(d_logits, stride, experts, op_type_size(type)) && route_wide(d_dlogits, dstride, experts, op_type_size(type));

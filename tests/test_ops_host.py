@@ -167,3 +167,29 @@ def test_workspaces_of_the_longest_matrices(type_, limbs):
         assert lib().tb_orthogonalise_workspace(type_, batch, rows, cols) == INVALID and lib().tb_muon_step_workspace(batch, rows, cols) == INVALID
         e = err()
         assert lib().tb_orthogonalise(P, rows * cols, cols, type_, batch, rows, cols, 5, COEF, 1e-7, P, rows * cols, cols, P, 1 << 62, None, e, 200) == INVALID and b"2^40" in e.value
+
+
+def test_every_tensor_has_to_be_aligned_to_its_elements():
+    """A vector at an odd address would be a misaligned access on the device."""
+    at = lambda i: P + 4096 * i  # noqa: E731
+    for bad in ("mean", "rstd"):
+        for step in (1, 2):
+            v = {"mean": at(2), "rstd": at(3)}
+            v[bad] += step
+            e = err()
+            assert lib().tb_layer_norm_forward(at(0), 8, None, None, 1e-5, 1, 4, 8, at(1), 8, v["mean"], v["rstd"], None, e, 200) == INVALID and b"aligned" in e.value, (bad, e.value)
+    need = lib().tb_layer_norm_backward_workspace(4, 8)
+    for bad in ("mean", "rstd", "weight", "dweight", "dbias"):
+        v = {"mean": at(2), "rstd": at(3), "weight": at(4), "dweight": at(5), "dbias": at(6)}
+        v[bad] += 2
+        e = err()
+        assert lib().tb_layer_norm_backward(at(0), 8, at(1), 8, v["mean"], v["rstd"], v["weight"], 1, 4, 8, at(7), 8, v["dweight"], v["dbias"], at(8), need, None, e, 200) == INVALID
+        assert b"aligned" in e.value, bad
+    need = lib().tb_route_forward_workspace(100, 9)
+    for i in range(6):
+        v = [at(1 + j) + (2 if j == i else 0) for j in range(6)]
+        e = err()
+        assert lib().tb_route_forward(at(0), 9, 0, 100, 9, 2, 1, None, *v, at(9), need, None, e, 200) == INVALID and b"aligned" in e.value, i
+        e = err()
+        index, gate, dgate, counts, n, dlosses = v
+        assert lib().tb_route_backward(at(0), 9, 0, 100, 9, 2, 1, None, index, gate, dgate, counts, n, dlosses, at(9), 9, None, e, 200) == INVALID and b"aligned" in e.value, i
