@@ -257,8 +257,9 @@ int tb_ft_backward_static_scratch(const float* d_dft, const int32_t* d_indices, 
  * A call's kernels may be started while the kernel ahead of them on the stream is ending; they wait for its end before they touch memory.
  * A failed call returns a code, writes the reason to err (may be NULL) and launches nothing when an argument is refused.
  * Workspaces: tb_*_workspace returns the bytes a call of these sizes needs on the current device (negative: invalid sizes).
- * Row strides count elements; they may exceed the row (columns of a wider buffer).  A result may be the memory of an input of its shape
- * element by element (same address and strides) or have no element in common with it; one that overlaps an input in part is refused.  Sums are fp32 in a fixed order
+ * Row strides count elements; they may exceed the row (columns of a wider buffer).  Where a function says so, a result may be the memory of an
+ * input element by element (same address and strides): y that of x, dx of dy or x, dlogits of the logits, an orthogonalised matrix of its input, the Muon step's of what they replace.
+ * Any other element in common with an input or another result is refused.  Sums are fp32 in a fixed order
  * (repeated calls agree bit for bit), results are rounded once to the tensors' type. */
 enum { TB_TYPE_F32 = 0, TB_TYPE_F16 = 1, TB_TYPE_BF16 = 2 };
 

@@ -621,6 +621,10 @@ extern "C" int tb_layer_norm_forward(const void* d_x, int64_t x_stride, const fl
     if (rows > 1 && (x_stride < n || y_stride < n)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "row strides must be at least n");
     if (((uintptr_t)d_x | (uintptr_t)d_y) % size || ((uintptr_t)d_weight | (uintptr_t)d_bias | (uintptr_t)d_mean | (uintptr_t)d_rstd) & 3) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
     if (!op_apart(d_x, 0, x_stride, d_y, 0, y_stride, 1, rows, n, size)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_y overlaps d_x in part");
+    const OpRows xr = {d_x, x_stride * size, rows, (int64_t)n * size}, yr = {d_y, y_stride * size, rows, (int64_t)n * size};
+    const OpRows wv = op_vector(d_weight, n), bv = op_vector(d_bias, n), mv = op_vector(d_mean, rows), rv = op_vector(d_rstd, rows);
+    if (op_meets(yr, {wv, bv, mv, rv}) || op_meets(xr, {mv, rv}) || op_meets(wv, {mv, rv}) || op_meets(bv, {mv, rv}) || op_meets(mv, {rv}))
+        return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "a result overlaps another tensor");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = n % (16 / size) == 0 && norm_aligned(d_x, x_stride, size) && norm_aligned(d_y, y_stride, size) && (((uintptr_t)d_weight | (uintptr_t)d_bias) & 15) == 0;
     const NormForward a = {s, d_x, x_stride, d_weight, d_bias, eps, rows, n, d_y, y_stride, d_mean, d_rstd};
@@ -653,6 +657,11 @@ extern "C" int tb_layer_norm_backward(const void* d_dy, int64_t dy_stride, const
     if (columns && (!d_work || work_bytes < tb_layer_norm_backward_workspace(rows, n) || ((uintptr_t)d_work & 31)))
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "the workspace must be aligned and hold %lld bytes (got %lld)",
                          (long long)tb_layer_norm_backward_workspace(rows, n), (long long)work_bytes);
+    const OpRows wv = op_vector(d_weight, n), mv = op_vector(d_mean, rows), rv = op_vector(d_rstd, rows), dwv = op_vector(d_dweight, n), dbv = op_vector(d_dbias, n);
+    const OpRows gr = {d_dy, dy_stride * size, rows, (int64_t)n * size}, xr = {d_x, x_stride * size, rows, (int64_t)n * size}, dr = {d_dx, dx_stride * size, rows, (int64_t)n * size};
+    if (op_meets(dwv, {dbv}) || (rows > 0 && (op_meets(dr, {wv, mv, rv, dwv, dbv}) || op_meets(gr, {dwv, dbv}) || op_meets(xr, {dwv, dbv}) || op_meets(wv, {dwv, dbv}) ||
+                                              op_meets(mv, {dwv, dbv}) || op_meets(rv, {dwv, dbv}))))
+        return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "a result overlaps another tensor");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     float* partial = columns ? static_cast<float*>(d_work) : nullptr;
     const int blocks = norm_backward_blocks(rows, n);

@@ -10,6 +10,8 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <initializer_list>
+
 static __device__ __forceinline__ float op_float(float v) { return v; }
 static __device__ __forceinline__ float op_float(__half v) { return __half2float(v); }
 static __device__ __forceinline__ float op_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -113,6 +115,23 @@ static inline bool op_apart(const void* in, int64_t in_batch, int64_t in_stride,
     if (pitch == 0 || in_batch % pitch || d % size) return false;
     const int64_t at = ((d / size) % pitch + pitch) % pitch;
     return at >= n && pitch - at >= n;
+}
+
+// Rows in memory; a vector is a single one, and one that is not given is NULL.
+struct OpRows {
+    const void* p;
+    int64_t stride, rows, bytes;  // stride and the length of a row in bytes
+};
+static inline OpRows op_vector(const void* p, int64_t count, int size = 4) { return {p, 0, 1, count * size}; }
+// Whether rows have a byte in common with one of the vectors: the first row that ends behind a vector's begin, where it begins before the vector's end.
+static inline bool op_meets(const OpRows& a, std::initializer_list<OpRows> vectors) {
+    for (const OpRows& v : vectors) {
+        if (!a.p || !v.p || v.bytes < 1) continue;
+        const uintptr_t at = (uintptr_t)a.p, begin = (uintptr_t)v.p, bytes = (uintptr_t)a.bytes;
+        const uintptr_t first = begin < at + bytes ? 0 : a.rows > 1 ? (begin - at - bytes) / (uintptr_t)a.stride + 1 : 1;
+        if (first < (uintptr_t)a.rows && at + first * (uintptr_t)a.stride < begin + (uintptr_t)v.bytes) return true;
+    }
+    return false;
 }
 
 #if defined(__GNUC__)

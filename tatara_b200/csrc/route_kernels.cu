@@ -537,6 +537,12 @@ extern "C" int tb_route_forward(const void* d_logits, int64_t stride, int type, 
     const int64_t need = tb_route_forward_workspace(rows, experts);
     if (!d_work || work_bytes < need || ((uintptr_t)d_work & 7))
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "the workspace must be aligned and hold %lld bytes (got %lld)", (long long)need, (long long)work_bytes);
+    const int size = op_type_size(type);
+    const OpRows xr = {d_logits, stride * size, rows, (int64_t)experts * size}, mask = op_vector(d_mask, rows, 1), ix = op_vector(d_index, rows * k), ga = op_vector(d_gate, rows * k),
+                 co = op_vector(d_counts, experts), nr = op_vector(d_rows, 1), pm = op_vector(d_prob_mean, experts), lo = op_vector(d_losses, 2);
+    if (op_meets(xr, {ix, ga, co, nr, pm, lo}) || op_meets(mask, {ix, ga, co, nr, pm, lo}) || op_meets(ix, {ga, co, nr, pm, lo}) || op_meets(ga, {co, nr, pm, lo}) ||
+        op_meets(co, {nr, pm, lo}) || op_meets(nr, {pm, lo}) || op_meets(pm, {lo}))
+        return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "a result overlaps another tensor");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int blocks = route_forward_blocks(rows, experts);
     RouteParts part;
@@ -545,7 +551,7 @@ extern "C" int tb_route_forward(const void* d_logits, int64_t stride, int type, 
     part.c = reinterpret_cast<int*>(part.p + (size_t)blocks * experts);
     part.z = reinterpret_cast<float*>(part.c + (size_t)blocks * (experts + 1));
     part.ticket = reinterpret_cast<int*>(part.z + blocks);
-    const bool wide = route_wide(d_logits, stride, experts, op_type_size(type));
+    const bool wide = route_wide(d_logits, stride, experts, size);
 #define ARGS s, d_logits, stride, d_mask, rows, experts, k, renormalise, d_index, d_gate, part, wide
     if (type == TB_TYPE_F32) route_forward_go<float>(ARGS);
     else if (type == TB_TYPE_F16) route_forward_go<__half>(ARGS);
@@ -568,6 +574,10 @@ extern "C" int tb_route_backward(const void* d_logits, int64_t stride, int type,
         ((uintptr_t)d_index | (uintptr_t)d_gate | (uintptr_t)d_dgate | (uintptr_t)d_counts | (uintptr_t)d_rows | (uintptr_t)d_dlosses) & 3)
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");
     if (!op_apart(d_logits, 0, stride, d_dlogits, 0, dstride, 1, rows, experts, op_type_size(type))) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_dlogits overlaps d_logits in part");
+    if (op_meets({d_dlogits, dstride * op_type_size(type), rows, (int64_t)experts * op_type_size(type)},
+                 {op_vector(d_mask, rows, 1), op_vector(d_index, rows * k), op_vector(d_gate, rows * k), op_vector(d_dgate, rows * k), op_vector(d_counts, experts), op_vector(d_rows, 1),
+                  op_vector(d_dlosses, 2)}))
+        return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_dlogits overlaps another tensor");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = route_wide(d_logits, stride, experts, op_type_size(type)) && route_wide(d_dlogits, dstride, experts, op_type_size(type));
 #define ARGS s, d_logits, stride, d_mask, rows, experts, k, renormalise, d_index, d_gate, d_dgate, d_counts, d_rows, d_dlosses, d_dlogits, dstride, wide

@@ -193,3 +193,66 @@ def test_every_tensor_has_to_be_aligned_to_its_elements():
         e = err()
         index, gate, dgate, counts, n, dlosses = v
         assert lib().tb_route_backward(at(0), 9, 0, 100, 9, 2, 1, None, index, gate, dgate, counts, n, dlosses, at(9), 9, None, e, 200) == INVALID and b"aligned" in e.value, i
+
+
+def test_results_that_overlap_vectors():
+    """mean over the weight, dx over rstd, ..: refused as far as an element is shared, and no further."""
+    at = lambda i: P + 65536 * i  # noqa: E731
+    rows, n = 4, 8
+    fine = NO_DEVICE
+
+    def forward(stride=n, **kw):
+        v = dict(x=at(0), y=at(1), w=at(2), b=at(3), mean=at(4), rstd=at(5))
+        v.update(kw)
+        e = err()
+        return lib().tb_layer_norm_forward(v["x"], stride, v["w"], v["b"], 1e-5, 0, rows, n, v["y"], stride, v["mean"], v["rstd"], None, e, 200), e.value
+
+    last = 4 * (rows * n - 1)
+    for kw in (dict(w=at(1)), dict(b=at(1) + last), dict(mean=at(1) + last), dict(rstd=at(0)), dict(mean=at(2) + 28), dict(rstd=at(3)), dict(mean=at(5) - 12), dict(w=at(1) - 28)):
+        rc, text = forward(**kw)
+        assert rc == INVALID and b"overlaps" in text, kw
+    need = lib().tb_layer_norm_backward_workspace(rows, n)
+
+    def backward(stride=n, **kw):
+        v = dict(dy=at(0), x=at(1), dx=at(2), mean=at(3), rstd=at(4), w=at(5), dw=at(6), db=at(7))
+        v.update(kw)
+        e = err()
+        return lib().tb_layer_norm_backward(v["dy"], stride, v["x"], stride, v["mean"], v["rstd"], v["w"], 0, rows, n, v["dx"], stride, v["dw"], v["db"], at(8), need, None, e, 200), e.value
+
+    for kw in (dict(w=at(2)), dict(mean=at(2) + last), dict(rstd=at(2)), dict(dw=at(2)), dict(db=at(2) + last), dict(dw=at(0)), dict(db=at(1)), dict(dw=at(5)), dict(db=at(3) + 12), dict(dw=at(4)),
+               dict(db=at(6) + 28)):
+        rc, text = backward(**kw)
+        assert rc == INVALID and b"overlaps" in text, kw
+    routes = lib().tb_route_forward_workspace(100, 9)
+    names = ("index", "gate", "counts", "n", "mean", "losses")
+
+    def route(**kw):
+        v = dict(x=at(0), mask=at(1), **{q: at(2 + i) for i, q in enumerate(names)})
+        v.update(kw)
+        e = err()
+        return lib().tb_route_forward(v["x"], 9, 0, 100, 9, 2, 1, v["mask"], *[v[q] for q in names], at(9), routes, None, e, 200), e.value
+
+    ends = {"x": (0, 3596), "mask": (1, 96), "index": (2, 796), "gate": (3, 796), "counts": (4, 32), "n": (5, 0), "mean": (6, 32), "losses": (7, 4)}
+    for a in names:
+        for b, (i, end) in ends.items():
+            if a != b:
+                rc, text = route(**{a: at(i) + end})
+                assert rc == INVALID and b"overlaps" in text, (a, b)
+
+    def route_back(**kw):
+        v = dict(mask=at(1), index=at(2), gate=at(3), counts=at(4), n=at(5), dgate=at(6), dlosses=at(7), d=at(8))
+        v.update(kw)
+        e = err()
+        return lib().tb_route_backward(at(0), 9, 0, 100, 9, 2, 1, v["mask"], v["index"], v["gate"], v["dgate"], v["counts"], v["n"], v["dlosses"], v["d"], 9, None, e, 200), e.value
+
+    for q in ("mask", "index", "gate", "counts", "n", "dgate", "dlosses"):
+        for off in (0, 3596):
+            rc, text = route_back(**{q: at(8) + off})
+            assert rc == INVALID and b"overlaps" in text, (q, off)
+    if no_gpu():  # side by side, and in the gaps between the rows of a wider buffer
+        gap = dict(stride=3 * n)
+        assert forward()[0] == backward()[0] == route()[0] == route_back()[0] == fine
+        assert forward(w=at(1) + 4 * rows * n, mean=at(1) - 16, b=at(1) - 48)[0] == fine
+        assert forward(w=at(1) + 32, b=at(1) + 96 + 64, mean=at(0) + 32, rstd=at(0) + 48, **gap)[0] == fine
+        assert backward(w=at(2) + 32, dw=at(0) + 64, db=at(1) + 96 + 32, mean=at(2) + 192 + 80, **gap)[0] == fine
+        assert forward(y=at(0))[0] == backward(dx=at(0))[0] == backward(dx=at(1))[0] == route_back(d=at(0))[0] == fine
