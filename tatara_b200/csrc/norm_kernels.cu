@@ -666,8 +666,8 @@ extern "C" int tb_layer_norm_backward(const void* d_dy, int64_t dy_stride, const
     float* partial = columns ? static_cast<float*>(d_work) : nullptr;
     const int blocks = norm_backward_blocks(rows, n);
     if (rows == 0) {
-        if (d_dweight) cudaMemsetAsync(d_dweight, 0, (size_t)n * sizeof(float), s);
-        if (d_dbias) cudaMemsetAsync(d_dbias, 0, (size_t)n * sizeof(float), s);
+        if (d_dweight) op_note(cudaMemsetAsync(d_dweight, 0, (size_t)n * sizeof(float), s));
+        if (d_dbias) op_note(cudaMemsetAsync(d_dbias, 0, (size_t)n * sizeof(float), s));
         return op_launched(err, err_len);
     }
     const bool wide = n % (16 / size) == 0 && norm_aligned(d_dy, dy_stride, size) && norm_aligned(d_x, x_stride, size) && norm_aligned(d_dx, dx_stride, size) && ((uintptr_t)d_weight & 15) == 0;

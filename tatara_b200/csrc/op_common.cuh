@@ -79,6 +79,14 @@ static __device__ __forceinline__ float op_group_sum(float v) {
     return v;
 }
 
+// The first error of a call's launches, taken from what they return: the thread's last error may be one that somebody else has left, and stays as it is.
+inline thread_local cudaError_t op_first_error = cudaSuccess;
+static inline void op_note(cudaError_t e) {
+    if (e == cudaSuccess) return;
+    cudaGetLastError();  // ours, reported by op_launched
+    if (op_first_error == cudaSuccess) op_first_error = e;
+}
+
 // Launches overlap, those of one call and those of calls that follow one another on a stream (programmatic dependent launch): every kernel may start before
 // the one ahead of it has finished, and waits for it to end before it touches global memory.  That one has waited for those ahead of itself in the same way.
 static __device__ __forceinline__ void op_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -95,7 +103,7 @@ static inline void op_launch_next(cudaStream_t s, dim3 grid, dim3 block, size_t 
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    op_note(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
 }
 
 static inline int op_type_size(int type) { return type == TB_TYPE_F32 ? 4 : type == TB_TYPE_F16 || type == TB_TYPE_BF16 ? 2 : 0; }
@@ -147,7 +155,8 @@ static inline int op_report(char* err, size_t err_len, int code, const char* fmt
     return code;
 }
 static inline int op_launched(char* err, size_t err_len) {
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = op_first_error;
+    op_first_error = cudaSuccess;
     if (e == cudaSuccess) return TB_OK;
     return op_report(err, err_len, e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver ? TB_ERR_NO_DEVICE : TB_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
 }

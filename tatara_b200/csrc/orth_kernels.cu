@@ -302,7 +302,7 @@ void small_launch(cudaStream_t s, const OrthIo& io, const OrthPoly& p, int n, in
     const int64_t per = (m + cs - 1) / cs;
     const int jc_max = per < room ? (int)((per + 7) / 8 * 8) : room;
     const size_t smem = (size_t)(jc_max * pitch + matrices) * sizeof(double);
-    if (!small_clusters<T, WARPS>()) cudaFuncSetAttribute(k_orth_small<T, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMALL_SMEM);  // else it is set
+    if (!small_clusters<T, WARPS>()) op_note(cudaFuncSetAttribute(k_orth_small<T, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMALL_SMEM));  // else it is set
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)cs, (unsigned)io.batch);
     cfg.blockDim = dim3(32 * WARPS);
@@ -316,7 +316,7 @@ void small_launch(cudaStream_t s, const OrthIo& io, const OrthPoly& p, int n, in
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    cudaLaunchKernelEx(&cfg, k_orth_small<T, WARPS>, io, p, jc_max);
+    op_note(cudaLaunchKernelEx(&cfg, k_orth_small<T, WARPS>, io, p, jc_max));
 }
 // Sixteen warps where the products or the loads keep them busy (64 x 512: 44 us, with ten 50, eight 47; 15 of 19 x 2200: 18, 20, 21; 9 of 24 x 1536: 16.0, with eight 17.5), else eight, whose columns
 // are one batch of loads: fewer to wait for at a barrier (16 x 64: 9.1 us, 10.1), and two CTAs per SM (9 of 16 x 1536: 12.5 us, with sixteen 21.6: the ninth cluster has to wait).

@@ -883,7 +883,9 @@ void ot_launch(cudaStream_t s, const OtGemm& g, const OrthIo& io, int64_t blocks
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !(known.load(std::memory_order_relaxed) >> dev & 1)) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) == cudaSuccess && dev >= 0 && dev < 64) known.fetch_or(1ull << dev);
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        if (e == cudaSuccess && dev >= 0 && dev < 64) known.fetch_or(1ull << dev);
+        op_note(e);
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(blocks * CTAS), (unsigned)parts);
@@ -898,7 +900,7 @@ void ot_launch(cudaStream_t s, const OtGemm& g, const OrthIo& io, int64_t blocks
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = CTAS == 2 ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, kern, g, io);
+    op_note(cudaLaunchKernelEx(&cfg, kern, g, io));
 }
 template <int KIND, int LIMBS, int W, typename T>
 void ot_gemm_of(cudaStream_t s, const OtGemm& g, const OrthIo& io, int parts) {

@@ -476,7 +476,7 @@ void route_forward_go(cudaStream_t s, const void* logits, int64_t stride, const 
         constexpr bool S = (V) <= 8;                                                                                                            \
         auto kern = wide ? (S && k > 2 ? k_route_forward<T, G, V, VW, S> : k_route_forward<T, G, V, VW, false>)                                 \
                          : (S && k > 2 ? k_route_forward<T, G, V, 1, S> : k_route_forward<T, G, V, 1, false>);                                  \
-        if (smem > 40000) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);                                   \
+        if (smem > 40000) op_note(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));                          \
         op_launch_next(s, dim3((unsigned)blocks), dim3(ROUTE_THREADS), smem, kern, (const T*)logits, stride, mask, rows, experts, k, renormalise, index, gate, part);             \
     } while (0)
     ROUTE_SHAPES(GO)

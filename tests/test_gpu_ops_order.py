@@ -103,3 +103,16 @@ def test_results_of_one_call_are_tensors_of_their_own():
     leaf = dw.requires_grad_()
     (leaf * leaf).sum().backward()
     assert torch.equal(leaf.grad, 2 * dw.detach()) and not db.requires_grad
+
+
+def test_an_error_that_an_earlier_call_left_is_not_this_call_s():
+    """A call of another part of the library that failed (no such device) leaves its error on the thread; the operators' launches did not fail."""
+    import ctypes as C
+    lib = tb.load_library()
+    x = torch.randn(70, 90, device="cuda")
+    want = [ops().layer_norm_forward(x)[0], ops().route_forward(x, 2).gate, ops().orthogonalise(x), ops().orthogonalise(x[:40])]
+    zero, result = (C.c_int32 * 8)(), tb._lib.MicrobenchResult()
+    for call, w in ((lambda: ops().layer_norm_forward(x)[0], want[0]), (lambda: ops().route_forward(x, 2).gate, want[1]), (lambda: ops().orthogonalise(x), want[2]),
+                    (lambda: ops().orthogonalise(x[:40]), want[3])):
+        assert lib.tb_ft_microbench(99, zero, zero, 1, 128, 4, 0, 8, 1, 0, C.byref(result)) != 0
+        assert torch.equal(call(), w)
