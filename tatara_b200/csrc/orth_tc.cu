@@ -1,9 +1,11 @@
 // Newton-Schulz steps of matrices with a short side above 64: products on the 5th-generation tensor cores.
 //
-// Operands are fp16 "limbs" of numbers scaled by 2^11: one limb holds 11 bits of a number, two hold 22 (the second is the first one's
-// rounding error).  With two limbs a product is three products of limbs (high high, high low, low high; low low is below 2^-22)
-// into one fp32 accumulator, which keeps the steps at fp32 accuracy at a third of the fp16 rate; fp32 on the CUDA cores has a thirtieth.
-// With one limb the roundings (2^-12 of an element, a few times over) stay below those of a bf16 result (2^-9).  Numbers up to 32
+// Operands are fp16 "limbs" of numbers scaled by 2^11: one limb holds 11 bits of a number, two hold 22 (the second is the first one's rounding error, times
+// 2^11 once more, so that it leaves the range of fp16 no sooner than the first).  That is so from 2^-25 on, the matrix's norm being 1; below, one limb is off by at
+// most 2^-36 and two by 2^-47.  With two limbs a product is three products of limbs (high low, low high, high high; low low is below 2^-22) into one
+// fp32 accumulator, which the first high product scales back by 2^-11: the steps keep fp32 accuracy, for blocks and rows far below the norm too, at a third of
+// the fp16 rate; fp32 on the CUDA cores has a thirtieth.  (The second limb at the first one's scale left the range sooner: a block of 1e-5 of another came
+// out 2e-4 off, now 2e-7.)  With one limb the roundings (2^-12 of an element, a few times over) stay below those of a bf16 result (2^-9).  Numbers up to 32
 // fit; the entry points refuse coefficients that could leave that range.
 //
 // All matrices live in the workspace as 16 KB tiles of 128 rows x 64 columns, stored as the tensor cores want them in shared memory
@@ -34,6 +36,8 @@ namespace {
 #define OT_TILE 16384           // bytes of a tile of 128 x 64 fp16
 #define OT_SCALE 2048.0f
 #define OT_UNSCALE (1.0f / (2048.0f * 2048.0f))
+#define OT_LOW_BITS 11          // of the second limb's further scale
+#define OT_LOW ((float)(1 << OT_LOW_BITS))
 #define OT_PARTS 8             // most parts of a Gram product
 #define OT_NORM_BLOCKS 512      // most partial sums of squares per matrix
 enum { OT_GRAM = 0, OT_SQUARE = 1, OT_APPLY = 2, OT_LAST = 3, OT_GRAM_PART = 4 };
@@ -83,15 +87,16 @@ __device__ __forceinline__ bool ot_elect() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
     return one != 0;
 }
-template <int CTAS>
+// d = a b + d 2^-DOWN, or a b alone
+template <int CTAS, int DOWN>
 __device__ __forceinline__ void ot_mma(unsigned d, unsigned long long da, unsigned long long db, unsigned idesc, unsigned accumulate) {
     if (CTAS == 2)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(da), "l"(db),
-                     "r"(idesc), "r"(accumulate)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p, %5;\n\t}" ::"r"(d), "l"(da), "l"(db),
+                     "r"(idesc), "r"(accumulate), "n"(DOWN)
                      : "memory");
     else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(da), "l"(db),
-                     "r"(idesc), "r"(accumulate)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, %5;\n\t}" ::"r"(d), "l"(da), "l"(db),
+                     "r"(idesc), "r"(accumulate), "n"(DOWN)
                      : "memory");
 }
 // arrives at the barrier (of both blocks) when the MMAs issued so far are done
@@ -117,11 +122,11 @@ __device__ __forceinline__ unsigned long long ot_desc(unsigned addr, unsigned lb
     return (unsigned long long)((addr & 0x3FFFFu) >> 4) | ((unsigned long long)(lbo >> 4) << 16) | ((unsigned long long)(sbo >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// limbs of x: hi + lo = x to 22 bits
+// limbs of x: hi + lo / OT_LOW = x to 22 bits
 template <int LIMBS>
 __device__ __forceinline__ void ot_split(float x, __half (&h)[LIMBS]) {
     h[0] = __float2half_rn(x);
-    if (LIMBS == 2) h[LIMBS - 1] = __float2half_rn(x - __half2float(h[0]));
+    if (LIMBS == 2) h[LIMBS - 1] = __float2half_rn((x - __half2float(h[0])) * OT_LOW);
 }
 // ... of two neighbours, as they lie in a tile
 template <int LIMBS>
@@ -129,7 +134,7 @@ __device__ __forceinline__ void ot_split(float x, float y, __half2 (&h)[LIMBS]) 
     h[0] = __floats2half2_rn(x, y);
     if (LIMBS == 2) {
         const float2 high = __half22float2(h[0]);
-        h[LIMBS - 1] = __floats2half2_rn(x - high.x, y - high.y);
+        h[LIMBS - 1] = __floats2half2_rn((x - high.x) * OT_LOW, (y - high.y) * OT_LOW);
     }
 }
 // byte offset of element (row, col) in a 128 x 64 tile
@@ -316,7 +321,8 @@ struct OtShape {
     static constexpr int STAGE = LIMBS * 2 * OT_TILE;
     static constexpr int STAGES = LIMBS == 2 ? 3 : 6;
     static constexpr int SMEM = STAGE * STAGES + 1024;
-    // chunks of 64 whose products share an accumulator (two limbs: four instead of one are 4 to 9 % faster and three times as far off)
+    // chunks of 64 whose products share an accumulator (two limbs: four instead of one are 4 to 9 % faster and three times as far off, and a chunk's small products
+    // have to be the first in what is scaled after them)
     static constexpr int DRAIN = LIMBS == 2 ? 1 : 1 << 30;
 };
 
@@ -520,9 +526,12 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
 #pragma unroll
                             for (int q = 0; q < (LIMBS == 2 ? 3 : 1); ++q)  // high low, low high, high high: the large terms last
 #pragma unroll
-                                for (int j = 0; j < 4; ++j)
-                                    ot_mma<CTAS>(d, da + (LIMBS == 2 && q == 1 ? OT_TILE / 16 : 0) + STEP_A * j, db + (LIMBS == 2 && q == 0 ? OT_TILE / 16 : 0) + STEP_B * j, IDESC,
-                                                 q > 0 || j > 0 ? 1u : accumulate);
+                                for (int j = 0; j < 4; ++j) {
+                                    const unsigned long long a = da + (LIMBS == 2 && q == 1 ? OT_TILE / 16 : 0) + STEP_A * j, b = db + (LIMBS == 2 && q == 0 ? OT_TILE / 16 : 0) + STEP_B * j;
+                                    const unsigned more = q > 0 || j > 0 ? 1u : accumulate;
+                                    if (q == 2 && j == 0) ot_mma<CTAS, OT_LOW_BITS>(d, a, b, IDESC, more);
+                                    else ot_mma<CTAS, 0>(d, a, b, IDESC, more);
+                                }
                             ot_commit<CTAS>(ot_smem(&s_empty[0]) + 8 * s);
                         }
                         __syncwarp();
@@ -712,7 +721,7 @@ __global__ void __launch_bounds__(320, 1) k_orth_gemm(OtGemm g, OrthIo io) {
                             for (int l = LIMBS - 1; l >= 0; --l) {
                                 before[l].exchange(swap);
 #pragma unroll
-                                for (int c = 0; c < 16; ++c) x[c] = fmaf(g.cb, before[l].get(c), x[c]);
+                                for (int c = 0; c < 16; ++c) x[c] = fmaf(l ? g.cb / OT_LOW : g.cb, before[l].get(c), x[c]);
                                 if (c0 + 16 < RC) before[l].load(old + l * g.a_limb + ((((base + c0 + 16) >> 3) ^ (row & 6)) << 4));
                             }
                             if (same)  // the diagonal passes through these tiles alone

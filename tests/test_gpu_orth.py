@@ -211,3 +211,23 @@ def test_refusals():
     assert lib.tb_orthogonalise_workspace(0, 1, 0, 5) == -1 and lib.tb_orthogonalise_workspace(7, 1, 5, 5) == -1 and lib.tb_muon_step_workspace(-1, 5, 5) == -1
     assert lib.tb_orthogonalise(None, 0, 80, 0, 0, 70, 80, 5, c, 1e-7, None, 0, 80, None, 0, None, None, 0) == 0        # an empty batch
     assert lib.tb_muon_step(None, p, p, p, 0, 2, 70, 80, p, p, None, 0, None, None, 0) == -1
+
+
+# Blocks far below the others keep their digits: nothing of one block's rounding reaches another, so each is as near as a whole matrix is.  (Entries of
+# the last block are about 1e-8 of the norm: two limbs are off by at most 2^-47 of it there, which is less than 2^-20 of such an entry.)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(200, 200), (60, 230), (230, 70), (600, 800), (1100, 1000)])
+def test_blocks_of_different_scale(rows, cols, dtype):
+    scales = (1.0, 0.03, 1e-2) if dtype == torch.float16 else (1.0, 1e-3, 1e-5)  # results of fp16 stay in the range of their type
+    x = torch.zeros(3 * rows, 3 * cols, device="cuda")
+    blocks = [(slice(i * rows, (i + 1) * rows), slice(i * cols, (i + 1) * cols)) for i in range(3)]
+    for i, b in enumerate(blocks):
+        x[b] = make(1, rows, cols, 7 + i)[0] * (scales[i] * 30)
+    x = x.to(dtype)
+    got, want = ops().orthogonalise(x), orthogonalise(x)
+    for b in blocks:
+        assert far(got[b], want[b]) <= tolerance(dtype, 3 * rows, 3 * cols), far(got[b], want[b])
+    out = torch.ones(3 * rows, 3 * cols, dtype=torch.bool, device="cuda")
+    for b in blocks:
+        out[b] = False
+    assert (got[out] == 0).all()
