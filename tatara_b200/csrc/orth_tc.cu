@@ -267,7 +267,9 @@ __global__ void __launch_bounds__(256) k_orth_pack(OrthIo io, float eps, const d
     v = s_part[0];
 #pragma unroll
     for (int w = 1; w < 8; ++w) v += s_part[w];
-    const float inv = (float)((double)OT_SCALE / (sqrt(v) + (double)eps));  // one more rounding of 2^-24
+    // 2^11 / (|u| + eps), one more rounding of 2^-24; beyond fp32's range for norms near its ends, so in two factors, the first a power of two
+    const double scale = (double)OT_SCALE / (sqrt(v) + (double)eps);
+    const float inv0 = scale > 0x1p100 ? 0x1p64f : scale < 0x1p-100 ? 0x1p-64f : 1.0f, inv = (float)(scale / (double)inv0);
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
         float u[8];
@@ -278,7 +280,7 @@ __global__ void __launch_bounds__(256) k_orth_pack(OrthIo io, float eps, const d
             for (int e = 0; e < N; ++e) t[e] = 0.0f;
             if (TALL ? 16 * k + q < left : i0 + i + 32 * k < n && q * N < left) piece[k][q].template finish<false>(io, t);
 #pragma unroll
-            for (int e = 0; e < N; ++e) u[q * N + e] = t[e] * inv;
+            for (int e = 0; e < N; ++e) u[q * N + e] = t[e] * inv0 * inv;
         }
         unsigned out[LIMBS][4];
 #pragma unroll

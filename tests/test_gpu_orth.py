@@ -231,3 +231,16 @@ def test_blocks_of_different_scale(rows, cols, dtype):
     for b in blocks:
         out[b] = False
     assert (got[out] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols", [(16, 200), (120, 256), (256, 120), (301, 97)])
+def test_norms_at_the_ends_of_the_range(rows, cols, dtype):
+    """eps = 0: what the norm divides is the type's smallest and largest numbers, and its reciprocal beyond them."""
+    for size in (2.0 ** -136, 2.0 ** -125, 2.0 ** -110, 2.0 ** 110, 2.0 ** 126):
+        x = (make(2, rows, cols, 4, torch.float32).clamp_(-1, 1).double() * size).to(dtype)
+        got = ops().orthogonalise(x, eps=0.0)
+        if (x == 0).all():  # below the type's smallest number: 0 / 0
+            assert got.isnan().all()
+        else:
+            assert far(got, orthogonalise(x, eps=0.0)) <= tolerance(dtype, rows, cols), size
