@@ -73,7 +73,7 @@ extern "C" int tb_ft_microbench(int device, const int32_t* indices, const int32_
     sc.lr = 1e-3f; sc.step_size = 1.f; sc.decay = 0.01f; sc.beta1 = 0.9f; sc.beta2 = 0.999f; sc.eps = 1e-8f;
     sc.min_w = -32767.0f / 127.0f; sc.max_w = 32767.0f / 127.0f;  // the i16 range at QA = 127 (bins/nnue_train/src/arch.rs:122-131)
     sc.alpha = 0.5f; sc.denom = 1; sc.lerp = 0;
-#define MB(call) do { cudaError_t e_ = (call); if (e_ != cudaSuccess) { fprintf(stderr, "tb_ft_microbench: %s: %s\n", #call, cudaGetErrorString(e_)); rc = e_ == cudaErrorMemoryAllocation ? TB_ERR_OUT_OF_MEMORY : TB_ERR_CUDA; goto done; } } while (0)
+#define MB(call) do { cudaError_t e_ = (call); if (e_ != cudaSuccess) { cudaGetLastError(); fprintf(stderr, "tb_ft_microbench: %s: %s\n", #call, cudaGetErrorString(e_)); rc = e_ == cudaErrorMemoryAllocation ? TB_ERR_OUT_OF_MEMORY : TB_ERR_CUDA; goto done; } } while (0)
     MB(cudaSetDevice(device));
     MB(cudaMalloc(&d_table, N * F * 4)); MB(cudaMalloc(&d_x, B * F * 4)); MB(cudaMalloc(&d_grad, N * F * 4));
     MB(cudaMalloc(&d_m, N * F * 4)); MB(cudaMalloc(&d_v, N * F * 4));

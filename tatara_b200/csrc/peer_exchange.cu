@@ -120,6 +120,7 @@ struct PeerExchange {
     do {                                                                                           \
         cudaError_t e_ = (call);                                                                   \
         if (e_ != cudaSuccess) {                                                                   \
+            cudaGetLastError();                                                                    \
             if (err) *err = std::string(#call) + ": " + cudaGetErrorString(e_);                    \
             return -1;                                                                             \
         }                                                                                          \

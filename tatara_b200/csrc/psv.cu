@@ -520,7 +520,7 @@ extern "C" int tb_psv_extract(int device, int feature_set, const uint8_t* psv, i
     if (!fs_spec(feature_set, &spec) || n < 0) return TB_ERR_INVALID_ARGUMENT;
     if (n == 0) return TB_OK;
     if (!psv || !stm_indices || !nstm_indices || !nnz || !score || !wdl) return TB_ERR_INVALID_ARGUMENT;
-    if (cudaSetDevice(device) != cudaSuccess) return TB_ERR_NO_DEVICE;
+    if (cudaSetDevice(device) != cudaSuccess) { cudaGetLastError(); return TB_ERR_NO_DEVICE; }
     ExtractCtx* c = extract_take(device);
     if (!c) return TB_ERR_CUDA;
     const size_t A = (size_t)spec.max_active;
@@ -604,6 +604,7 @@ extern "C" int tb_psv_extract(int device, int feature_set, const uint8_t* psv, i
         cudaStreamSynchronize(c->s[0]);
         cudaStreamSynchronize(c->s[1]);
         extract_free(c);
+        cudaGetLastError();
         return TB_ERR_CUDA;
     }
     extract_give_back(c);

@@ -244,7 +244,8 @@ int fail(tb_trainer* t, int code, const char* fmt, ...) {
     return code;
 }
 
-#define CU(t, call) do { cudaError_t e_ = (call); if (e_ != cudaSuccess) return fail(t, e_ == cudaErrorMemoryAllocation ? TB_ERR_OUT_OF_MEMORY : TB_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_)); } while (0)
+// A reported error does not stay on the thread: the checks after launches (cudaGetLastError) would take it for theirs.
+#define CU(t, call) do { cudaError_t e_ = (call); if (e_ != cudaSuccess) return cudaGetLastError(), fail(t, e_ == cudaErrorMemoryAllocation ? TB_ERR_OUT_OF_MEMORY : TB_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_)); } while (0)
 
 template <typename T>
 cudaError_t dalloc(T** p, size_t n) {
@@ -264,6 +265,7 @@ int nccl_host_allgather(void* ctx, const void* send, void* recv, size_t bytes) {
         cudaMemcpy(recv, dr, bytes * t->cfg.world_size, cudaMemcpyDeviceToHost) == cudaSuccess)
         rc = 0;
     cudaFree(ds); cudaFree(dr);
+    if (rc) cudaGetLastError();
     return rc;
 }
 
@@ -1663,7 +1665,7 @@ int tb_device_count(void) {
 const char* tb_version(void) { return "tatara_b200 0.1 (sm_100a)"; }
 
 // ---- FT kernels alone -------------------------------------------------------------------------------------
-#define CUX(call) do { cudaError_t e_ = (call); if (e_ != cudaSuccess) { rc = fail(nullptr, TB_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_)); goto done; } } while (0)
+#define CUX(call) do { cudaError_t e_ = (call); if (e_ != cudaSuccess) { cudaGetLastError(); rc = fail(nullptr, TB_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_)); goto done; } } while (0)
 
 int tb_ft_forward_bench(int device, const float* table, const int32_t* indices, const int32_t* nnz, int batch, int ft_out,
                         int ft_in, int max_active, int iters, float* out, float* ms_per_iter) {
