@@ -116,6 +116,12 @@ at::Tensor output(PyObject* out, const at::Tensor& like) {
     if (t.sizes() != like.sizes() || t.scalar_type() != like.scalar_type() || t.device() != like.device()) refuse("out must match the input");
     return t;
 }
+// A caller's tensor has been written: what automatic differentiation has saved of it is no longer there, as after any operation in place.
+void written(PyObject* o) {
+    if (o == Py_None) return;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 double number(PyObject* o, const char* name) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) {
@@ -194,6 +200,7 @@ PyObject* layer_norm_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     check(tb_layer_norm_forward(x.data_ptr(), xs, w, b, (float)eps, type_of(x), rows, side(n, "n"), y.data_ptr(), rows_of(y, "out"), mean.data_ptr<float>(),
                                 rstd.data_ptr<float>(), on.stream, err, sizeof err),
           "tb_layer_norm_forward", err);
+    written(a[4]);
     return tuple_of({y, mean, rstd});
     BODY_END
 }
@@ -219,6 +226,7 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) 
     check(tb_layer_norm_backward(dy.data_ptr(), gs, x.data_ptr(), xs, m, r, w, type_of(x), rows, (int)n, dx.data_ptr(), rows_of(dx, "out"),
                                  dweight.data_ptr<float>(), dbias.data_ptr<float>(), work.at(), work.bytes, on.stream, err, sizeof err),
           "tb_layer_norm_backward", err);
+    written(a[5]);
     return tuple_of({dx, dweight, dbias});
     BODY_END
 }
@@ -332,6 +340,7 @@ PyObject* orthogonalise(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     check(tb_orthogonalise(x.data_ptr(), m.batch_stride, m.stride, type_of(x), m.batch, m.rows, m.cols, steps, c, (float)eps, y.data_ptr(), o.batch_stride, o.stride,
                            work.at(), work.bytes, on.stream, err, sizeof err),
           "tb_orthogonalise", err);
+    written(a[4]);
     return THPVariable_Wrap(y);
     BODY_END
 }
@@ -369,6 +378,8 @@ PyObject* muon_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     char err[256];
     check(tb_muon_step(&cfg, weight, momentum, grad, type_of(g), m.batch, m.rows, m.cols, weight_out, momentum_out, work.at(), work.bytes, on.stream, err, sizeof err),
           "tb_muon_step", err);
+    written(wo);
+    written(mo);
     return PyTuple_Pack(2, wo, mo);
     BODY_END
 }

@@ -5,7 +5,7 @@ The functions check their arguments, take outputs and workspaces from torch's al
 stream of the tensors' device (csrc/torch_ops.cpp).  Nothing is synchronised and nothing is kept between calls.  Wrong arguments raise
 `TrainerError`.  Small results of one call (mean and rstd; dweight and dbias; a routing's counts, rows, prob_mean and losses) are parts of one
 allocation: clone what is to outlive the others by long.  Gradients are what the *_backward functions return; torch's automatic differentiation
-does not see these calls.  This module needs torch; the rest of the package does not.
+does not see these calls, but it refuses to use what it saved of a tensor that one of them has written since (`out`, or a Muon step's weight and momentum).  This module needs torch; the rest of the package does not.
 """
 from __future__ import annotations
 

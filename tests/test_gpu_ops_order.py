@@ -116,3 +116,41 @@ def test_an_error_that_an_earlier_call_left_is_not_this_call_s():
                     (lambda: ops().orthogonalise(x[:40]), want[3])):
         assert lib.tb_ft_microbench(99, zero, zero, 1, 128, 4, 0, 8, 1, 0, C.byref(result)) != 0
         assert torch.equal(call(), w)
+
+
+def writes():
+    """A call, the tensors it writes and those it only reads."""
+    r = lambda *s: torch.randn(*s, device="cuda")  # noqa: E731
+    x, dy, v, one = r(6, 40), r(6, 40), torch.zeros(6, device="cuda"), torch.ones(6, device="cuda")
+    w, m, g, w2, m2 = r(12, 40), r(12, 40), r(12, 40), r(12, 40), r(12, 40)
+    yield lambda: ops().layer_norm_forward(x, out=x), [x], []
+    yield lambda: ops().layer_norm_forward(x, out=dy), [dy], [x]
+    yield lambda: ops().layer_norm_backward(dy, x, v, one, out=dy), [dy], [x, v, one]
+    yield lambda: ops().orthogonalise(g, out=g), [g], []
+    yield lambda: ops().orthogonalise(g[:3], out=w2[4:7]), [w2], [g]  # a view's memory is its base's
+    yield lambda: ops().muon_step(w, m, g, lr=0.1), [w, m], [g]
+    yield lambda: ops().muon_step(w, m, g, lr=0.1, weight_out=w2, momentum_out=m2), [w2, m2], [w, m, g]
+    yield lambda: ops().muon_step(w, m, g, lr=0.1, weight_out=w2), [w2, m], [w, g]
+    yield lambda: (ops().layer_norm_forward(x, one.new_ones(40)), ops().layer_norm_backward(dy, x, v, one), ops().orthogonalise(x), ops().route_forward(x, 2)), [], [x, dy, v, one]
+
+
+def test_tensors_that_were_written_are_known_to_be():
+    for call, written, read in writes():
+        before = [t._version for t in written + read]
+        call()
+        after = [t._version for t in written + read]
+        assert all(b > a for a, b in zip(before, after[:len(written)])) and before[len(written):] == after[len(written):]
+    # a gradient through values that a step has replaced since is refused, not computed from the new ones
+    w = torch.randn(20, 30, device="cuda", requires_grad=True)
+    value = (w * w).sum()
+    ops().muon_step(w, torch.zeros(20, 30, device="cuda"), torch.randn(20, 30, device="cuda"), lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        value.backward()
+    with torch.inference_mode():  # tensors without such a count
+        x = torch.randn(6, 40, device="cuda")
+        want = ops().layer_norm_forward(x.clone())[0]
+        assert torch.equal(ops().layer_norm_forward(x, out=x)[0], want)
+    x = torch.ones(3, 8, device="cuda")
+    with pytest.raises(tb.TrainerError):
+        ops().layer_norm_forward(x, eps=-1.0, out=x)
+    assert x._version == torch.ones(3, 8, device="cuda")._version  # nothing was written
