@@ -139,7 +139,14 @@ int whole(PyObject* o, const char* name) {
     if (v < INT32_MIN || v > INT32_MAX) refuse("%s is out of range (got %lld)", name, v);
     return (int)v;
 }
-bool truth(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+bool truth(PyObject* o, const char* name) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) {
+        PyErr_Clear();
+        refuse("%s must be a truth value", name);
+    }
+    return v == 1;
+}
 int side(int64_t v, const char* name) {
     if (v > INT32_MAX) refuse("%s is out of range (got %lld)", name, (long long)v);
     return (int)v;
@@ -244,6 +251,7 @@ PyObject* route_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const int64_t stride = rows_of(x, "logits"), rows = x.size(0), experts = x.size(1);
     const int k = whole(a[1], "k");
     if (k < 1) refuse("k must be positive (got %d)", k);
+    const bool renormalise = truth(a[2], "renormalise");
     const uint8_t* mask = mask_of(a[3], x);
     const On on(x);
     const at::Tensor index = make(x, {rows, k}, at::kInt), gate = make(x, {rows, k}, at::kFloat);
@@ -254,7 +262,7 @@ PyObject* route_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                      losses = few.tensor(losses_at, {2}, at::kFloat);
     const Work work(x, tb_route_forward_workspace(rows, side(experts, "experts")));
     char err[256];
-    check(tb_route_forward(x.data_ptr(), stride, type_of(x), rows, (int)experts, k, truth(a[2]), mask, index.data_ptr<int>(), gate.data_ptr<float>(),
+    check(tb_route_forward(x.data_ptr(), stride, type_of(x), rows, (int)experts, k, renormalise, mask, index.data_ptr<int>(), gate.data_ptr<float>(),
                            counts.data_ptr<int>(), n.data_ptr<int>(), mean.data_ptr<float>(), losses.data_ptr<float>(), work.at(), work.bytes, on.stream, err, sizeof err),
           "tb_route_forward", err);
     return tuple_of({index, gate, counts, n, mean, losses});
@@ -276,11 +284,12 @@ PyObject* route_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const int32_t* n = static_cast<int32_t*>(vector_of(a[4], "routing.rows", x, {1}, at::kInt, true));
     const float* dgate = static_cast<float*>(vector_of(a[5], "dgate", x, {rows, k}));
     const float* dlosses = static_cast<float*>(vector_of(a[6], "dlosses", x, {2}));
+    const bool renormalise = truth(a[7], "renormalise");
     const uint8_t* mask = mask_of(a[8], x);
     const On on(x);
     const at::Tensor out = make(x, x.sizes(), x.scalar_type());
     char err[256];
-    check(tb_route_backward(x.data_ptr(), stride, type_of(x), rows, side(experts, "experts"), side(k, "k"), truth(a[7]), mask, index, gate, dgate, counts, n, dlosses,
+    check(tb_route_backward(x.data_ptr(), stride, type_of(x), rows, side(experts, "experts"), side(k, "k"), renormalise, mask, index, gate, dgate, counts, n, dlosses,
                             out.data_ptr(), experts, on.stream, err, sizeof err),
           "tb_route_backward", err);
     return THPVariable_Wrap(out);
@@ -363,7 +372,7 @@ PyObject* muon_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     tb_muon cfg;
     cfg.struct_size = (int32_t)sizeof cfg;
     cfg.steps = whole(a[5], "steps");
-    cfg.nesterov = truth(a[6]);
+    cfg.nesterov = truth(a[6], "nesterov");
     cfg.a = c[0];
     cfg.b = c[1];
     cfg.c = c[2];

@@ -154,3 +154,13 @@ def test_tensors_that_were_written_are_known_to_be():
     with pytest.raises(tb.TrainerError):
         ops().layer_norm_forward(x, eps=-1.0, out=x)
     assert x._version == torch.ones(3, 8, device="cuda")._version  # nothing was written
+
+
+def test_arguments_without_a_truth_value():
+    x, w = torch.randn(6, 9, device="cuda"), torch.randn(6, 9, device="cuda")
+    r, neither = ops().route_forward(x, 2), torch.ones(2)
+    for bad in (lambda: ops().route_forward(x, 2, renormalise=neither), lambda: ops().route_backward(x, r, renormalise=neither),
+                lambda: ops().muon_step(w, torch.zeros_like(w), x, lr=0.1, nesterov=neither)):
+        with pytest.raises(tb.TrainerError, match="truth value"):
+            bad()
+    assert torch.equal(ops().route_forward(x, 2, renormalise=torch.tensor(True)).gate, r.gate)
