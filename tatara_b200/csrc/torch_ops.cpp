@@ -58,10 +58,15 @@ std::string shape_text(at::IntArrayRef s) {
     for (size_t i = 0; i < s.size(); ++i) t += (i ? ", " : "") + std::to_string(s[i]);
     return t + ")";
 }
+// a tensor whose memory does not hold its values: a negated view, or zeros without memory
+void in_memory(const at::Tensor& t, const char* name) {
+    if (t.is_neg() || t._is_zerotensor()) refuse("%s must hold its values in memory (resolve_neg, clone)", name);
+}
 const at::Tensor& cuda_tensor(PyObject* o, const char* name) {
     if (!THPVariable_Check(o)) refuse("%s must be a CUDA tensor", name);
     const at::Tensor& t = THPVariable_Unpack(o);
     if (!t.is_cuda() || t.layout() != at::kStrided) refuse("%s must be a CUDA tensor", name);
+    in_memory(t, name);
     return t;
 }
 const at::Tensor& typed(PyObject* o, const char* name) {
@@ -87,6 +92,7 @@ void* vector_of(PyObject* o, const char* name, const at::Tensor& like, at::IntAr
     if (!THPVariable_Check(o)) refuse("%s must be a tensor on %s", name, like.device().str().c_str());
     const at::Tensor& t = THPVariable_Unpack(o);
     if (t.device() != like.device()) refuse("%s must be on %s", name, like.device().str().c_str());
+    in_memory(t, name);
     if (t.scalar_type() != type || t.sizes() != shape || !t.is_contiguous())
         refuse("%s must be a contiguous %s tensor of shape %s", name, c10::toString(type), shape_text(shape).c_str());
     return t.data_ptr();

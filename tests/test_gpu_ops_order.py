@@ -164,3 +164,13 @@ def test_arguments_without_a_truth_value():
         with pytest.raises(tb.TrainerError, match="truth value"):
             bad()
     assert torch.equal(ops().route_forward(x, 2, renormalise=torch.tensor(True)).gate, r.gate)
+
+
+def test_tensors_whose_memory_does_not_hold_their_values():
+    x, v = torch.randn(6, 9, device="cuda"), torch.randn(9, device="cuda")
+    for t, u in ((torch._neg_view(x), torch._neg_view(v)), (torch._efficientzerotensor((6, 9), device="cuda"), torch._efficientzerotensor((9,), device="cuda"))):
+        for bad in (lambda: ops().layer_norm_forward(t), lambda: ops().layer_norm_forward(x, u), lambda: ops().layer_norm_forward(x, out=t), lambda: ops().route_forward(t, 2),
+                    lambda: ops().orthogonalise(t), lambda: ops().muon_step(x, torch.zeros_like(x), t, lr=0.1)):
+            with pytest.raises(tb.TrainerError, match="in memory"):
+                bad()
+    assert torch.equal(ops().orthogonalise(torch._neg_view(x).resolve_neg()), ops().orthogonalise(-x))
