@@ -244,3 +244,41 @@ def test_norms_at_the_ends_of_the_range(rows, cols, dtype):
             assert got.isnan().all()
         else:
             assert far(got, orthogonalise(x, eps=0.0)) <= tolerance(dtype, rows, cols), size
+
+
+# Products of tiles of 256 columns by pairs of blocks that take several tiles each (all three kinds at 4096 x 4096, and in 16 bits from 3072 on), results that
+# are stored straight from registers (rows on 16-byte boundaries, or tall) and through shared memory.  fp32 sums of K terms: the tolerance's 1.1e-5 is of K = 1000 and
+# grows with its root.
+LARGEST = [(1, 4096, 4096), (1, 3072, 3200), (1, 3200, 3072), (1, 2600, 4096), (1, 3073, 3001), (1, 4097, 4100), (6, 1024, 1024)]
+
+
+def large_tolerance(dtype, rows, cols):
+    return 17 * UNIT[dtype] + 1.1e-5 * math.sqrt(max(1.0, max(rows, cols) / 1000)) + HALF[dtype]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch,rows,cols", LARGEST)
+def test_largest(batch, rows, cols, dtype):
+    x = make(batch, rows, cols, rows + 2 * cols, dtype)
+    assert far(ops().orthogonalise(x), orthogonalise(x)) <= large_tolerance(dtype, rows, cols)
+
+
+@pytest.mark.parametrize("g_type", TYPES)
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("batch,rows,cols", [(1, 4096, 4096), (1, 3200, 3072), (1, 2600, 2700), (2, 136, 304), (2, 304, 136), (4, 72, 1000), (1, 100, 2048), (3, 520, 520), (12, 200, 264)])
+def test_muon_step_of_every_layout(batch, rows, cols, nesterov, g_type):
+    """Rows on 16-byte boundaries with gradients of every type, tall ones, one and several tiles per block."""
+    w, m = 0.05 * torch.randn(batch, rows, cols, device="cuda"), make(batch, rows, cols, 1)
+    g = make(batch, rows, cols, 2, g_type)
+    args = dict(lr=0.05, beta=0.9, nesterov=nesterov, weight_decay=0.1, scale=1.5, clip=0.12)
+    want_w, want_m = muon_step(w, m, g, **args)
+    w2, m2 = ops().muon_step(w, m, g, weight_out=torch.empty_like(w), momentum_out=torch.empty_like(m), **args)
+    assert ((m2.double() - want_m).abs() <= 2.0 ** -23 * (0.9 * m.double().abs() + g.double().abs())).all()
+    size = 0.05 * 1.5 * math.sqrt(batch * min(rows, cols)) * 1.2
+    off = float((w2.double() - want_w).norm())
+    assert off <= 3 * 2.0 ** -24 * float(w.double().norm()) + size * (large_tolerance(torch.float32, rows, cols) + 100 * 2.0 ** -23), off
+    # every weight by itself: an update's element is off by no more than the whole update's root mean square times 1e-3
+    each = 1e-3 * 0.05 * 1.5 / math.sqrt(max(rows, cols)) + 2.0 ** -22 * w.double().abs()
+    assert ((w2.double() - want_w).abs() <= each).all()
+    w3, m3 = ops().muon_step(w, m, g, **args)
+    assert torch.equal(w3, w2) and torch.equal(m3, m2)
