@@ -236,3 +236,41 @@ def test_gradient_over_the_logits(rows, experts, k, offset, dtype):
                                              r.counts.data_ptr(), r.rows.data_ptr(), dl.data_ptr(), x.data_ptr(), x.stride(0), torch.cuda.current_stream().cuda_stream, None, 0)
     assert rc == 0
     assert torch.equal(x, want) and (wide[:, :offset] == 3).all()
+
+
+@pytest.mark.parametrize("dtype,bits", [(torch.float16, (0x7e00, 0xfe00, 0x7c01, 0xffff)), (torch.bfloat16, (0x7fc0, 0xffc0, 0x7f81, 0xffff))])
+@pytest.mark.parametrize("experts,k", [(9, 2), (9, 1), (48, 8), (256, 8), (300, 4)])
+def test_values_that_are_not_numbers_in_16_bits(experts, k, dtype, bits):
+    """A NaN of either sign, quiet or not, is the largest; two of them tie, and +inf comes behind them."""
+    x = make(40, experts, dtype, 3)
+    raw = x.view(torch.int16)
+    for row, pattern in enumerate(bits):
+        raw[row, 5] = pattern - (1 << 16) if pattern >= 1 << 15 else pattern
+    x[4, 7], x[4, 2] = math.nan, math.nan
+    x[5, 6], x[5, 8] = math.inf, math.nan
+    x[6, 3] = math.inf
+    x[7] = -math.inf
+    x[7, 1] = math.nan
+    r = ops().route_forward(x, k)
+    assert r.index[:8, 0].tolist() == [5, 5, 5, 5, 2, 8, 3, 1]
+    if k > 1:
+        assert r.index[4, 1] == 7 and r.index[5, 1] == 6 and r.index[7, 1] == -1
+    assert r.gate[:6, 0].isnan().all() and r.gate[7, 0].isnan() and r.losses.isnan().all()
+    keep = list(range(8, 40))
+    want = route_forward(x[keep], k, True)
+    assert torch.equal(r.index[keep].cpu(), want["index"])
+    # the gradient: NaN in those rows, the others as without them
+    dgate, dl = torch.randn(40, k, device="cuda"), torch.tensor([0.0, 0.0], device="cuda")
+    d = ops().route_backward(x, r, dgate, dl)
+    mask = torch.zeros(40, dtype=torch.bool, device="cuda")
+    mask[8:] = True
+    clean = ops().route_backward(x, ops().route_forward(x, k, mask=mask), dgate, dl, mask=mask)
+    assert d[:8].isnan().any(1).all() and torch.equal(d[8:], clean[8:]) and (clean[:8] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_order_of_the_smallest_numbers_in_16_bits(dtype):
+    """Subnormal logits are told apart, of either sign."""
+    bits = torch.tensor([[0x0001, 0x0003, 0x8001, 0x0002, 0x8002, 0x0000, 0x8000, 0x0010]], dtype=torch.int32)
+    x = bits.to(torch.int16).view(dtype).cuda()
+    assert ops().route_forward(x, 8).index.tolist() == [[7, 1, 3, 0, 5, 6, 2, 4]]
