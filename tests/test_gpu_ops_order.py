@@ -174,3 +174,31 @@ def test_tensors_whose_memory_does_not_hold_their_values():
             with pytest.raises(tb.TrainerError, match="in memory"):
                 bad()
     assert torch.equal(ops().orthogonalise(torch._neg_view(x).resolve_neg()), ops().orthogonalise(-x))
+
+
+def test_two_threads_with_a_stream_each():
+    """Chains on two streams at once, fed by two threads: the bits of each by itself."""
+    import threading
+    shapes = [(4000, 40, 9, 6), (300, 256, 16, 100)]
+    want = [chain(state(*s, 3 + i), 20) for i, s in enumerate(shapes)]
+    got = [state(*s, 3 + i) for i, s in enumerate(shapes)]
+    streams = [torch.cuda.Stream() for _ in shapes]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(streams[i]):
+                chain(got[i], 20)
+            streams[i].synchronize()
+        except Exception as e:  # shown by the assertion below
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for g, w in zip(got, want):
+        assert all(torch.equal(g[k], w[k]) for k in ("x", "gate", "m", "w", "wm"))
