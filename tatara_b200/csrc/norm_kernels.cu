@@ -234,8 +234,9 @@ k_norm_forward_down(const T* x, int64_t x_stride, const float* __restrict__ weig
     }
 }
 
-// rows longer than NORM_REG_N: a block per row, three passes over it.  Columns of long rows are unsigned: the last step goes beyond 2^31.
-template <typename T>
+// rows longer than NORM_REG_N: a block per row, three passes over it.  C counts columns: int, or int64_t where the last step would go beyond 2^31 (64-bit columns
+// cost the fp16 gradient of 2000 x 12288 10 %)
+template <typename T, typename C>
 __global__ void __launch_bounds__(1024)
 k_norm_forward_long(const T* x, int64_t x_stride, const float* __restrict__ weight, const float* __restrict__ bias, float eps, int n,
                     T* y, int64_t y_stride, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
@@ -246,9 +247,9 @@ k_norm_forward_long(const T* x, int64_t x_stride, const float* __restrict__ weig
     float sum = 0.0f, sq = 0.0f;
     op_next_may_start();
     op_wait_for_previous();
-    for (unsigned c = threadIdx.x; c < (unsigned)n; c += 1024) sum += op_float(xr[c]);
+    for (C c = threadIdx.x; c < n; c += 1024) sum += op_float(xr[c]);
     const float mean = norm_row_sum<32>(sum, s_sum[0], warp, lane) / (float)n;
-    for (unsigned c = threadIdx.x; c < (unsigned)n; c += 1024) {
+    for (C c = threadIdx.x; c < n; c += 1024) {
         const float d = op_float(xr[c]) - mean;
         sq = fmaf(d, d, sq);
     }
@@ -258,7 +259,7 @@ k_norm_forward_long(const T* x, int64_t x_stride, const float* __restrict__ weig
         if (rstd_out) rstd_out[row] = rstd;
     }
     T* yr = y + row * y_stride;
-    for (unsigned c = threadIdx.x; c < (unsigned)n; c += 1024)
+    for (C c = threadIdx.x; c < n; c += 1024)
         yr[c] = op_round<T>(fmaf((op_float(xr[c]) - mean) * rstd, weight ? weight[c] : 1.0f, bias ? bias[c] : 0.0f));
 }
 
@@ -425,7 +426,7 @@ k_norm_backward(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, co
 }
 
 // rows longer than NORM_REG_N_BACK: dx by a block per row, then the columns' sums by threads that walk down stripes of rows
-template <typename T>
+template <typename T, typename C>
 __global__ void __launch_bounds__(1024)
 k_norm_backward_long(const T* dy, int64_t dy_stride, const T* x, int64_t x_stride, const float* __restrict__ mean,
                      const float* __restrict__ rstd, const float* __restrict__ weight, int n, T* dx, int64_t dx_stride) {
@@ -437,14 +438,14 @@ k_norm_backward_long(const T* dy, int64_t dy_stride, const T* x, int64_t x_strid
     op_wait_for_previous();
     const float mu = mean[row], r = rstd[row];
     float s1 = 0.0f, s2 = 0.0f;
-    for (unsigned c = threadIdx.x; c < (unsigned)n; c += 1024) {
+    for (C c = threadIdx.x; c < n; c += 1024) {
         const float xh = (op_float(xr[c]) - mu) * r, t = op_float(gr[c]) * (weight ? weight[c] : 1.0f);
         s1 += t;
         s2 = fmaf(t, xh, s2);
     }
     const float m1 = norm_row_sum<32>(s1, s_sum[0], warp, lane) / (float)n, m2 = norm_row_sum<32>(s2, s_sum[1], warp, lane) / (float)n;
     T* dr = dx + row * dx_stride;
-    for (unsigned c = threadIdx.x; c < (unsigned)n; c += 1024) {
+    for (C c = threadIdx.x; c < n; c += 1024) {
         const float xh = (op_float(xr[c]) - mu) * r, t = op_float(gr[c]) * (weight ? weight[c] : 1.0f);
         dr[c] = op_round<T>(r * (t - m1 - xh * m2));
     }
@@ -453,10 +454,11 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 k_norm_columns_long(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x, int64_t x_stride, const float* __restrict__ mean,
                     const float* __restrict__ rstd, int64_t rows, int n, float* __restrict__ part_w, float* __restrict__ part_b) {
-    const unsigned col = blockIdx.x * 256 + threadIdx.x;
+    const unsigned at = blockIdx.x * 256 + threadIdx.x;  // may be beyond 2^31
     op_next_may_start();
     op_wait_for_previous();
-    if (col >= (unsigned)n) return;
+    if (at >= (unsigned)n) return;
+    const int col = (int)at;
     float aw = 0.0f, ab = 0.0f;
     for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
         const float g = op_float(dy[row * dy_stride + col]);
@@ -519,6 +521,9 @@ int norm_backward_blocks(int64_t rows, int n) {
     return (int)blocks;
 }
 
+// whether int counts a long row's columns, one step of 1024 beyond the last included
+bool norm_counts(int n) { return n <= INT32_MAX - 1023; }
+
 struct NormForward {
     cudaStream_t s;
     const void* x;
@@ -561,7 +566,7 @@ void norm_forward_pick(const NormForward& a) {
         if (a.n <= NORM_REG_N_BACK) return norm_forward_down<T, 16, 16, 1>(a);
     }
 #undef GO
-    op_launch_next(a.s, dim3((unsigned)a.rows), dim3(1024), 0, k_norm_forward_long<T>, (const T*)a.x, a.xs, a.w, a.b, a.eps, a.n, (T*)a.y, a.ys, a.mean, a.rstd);
+    op_launch_next(a.s, dim3((unsigned)a.rows), dim3(1024), 0, norm_counts(a.n) ? k_norm_forward_long<T, int> : k_norm_forward_long<T, int64_t>, (const T*)a.x, a.xs, a.w, a.b, a.eps, a.n, (T*)a.y, a.ys, a.mean, a.rstd);
 }
 
 struct NormBackward {
@@ -590,7 +595,7 @@ void norm_backward_pick(const NormBackward& a) {
         if (a.part_w)
             op_launch_next(a.s, dim3((unsigned)ceil_div64(a.n, 256), (unsigned)a.blocks), dim3(256), 0, k_norm_columns_long<T>, (const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.rows, a.n, a.part_w,
                                                                                                              a.part_b);
-        op_launch_next(a.s, dim3((unsigned)a.rows), dim3(1024), 0, k_norm_backward_long<T>, (const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.w, a.n, (T*)a.dx, a.dxs);
+        op_launch_next(a.s, dim3((unsigned)a.rows), dim3(1024), 0, norm_counts(a.n) ? k_norm_backward_long<T, int> : k_norm_backward_long<T, int64_t>, (const T*)a.dy, a.dys, (const T*)a.x, a.xs, a.mean, a.rstd, a.w, a.n, (T*)a.dx, a.dxs);
     } else if (a.n <= 64) {
         norm_backward_go<T, VEC, 1, 8, 8, 2>(a);
     } else if (a.n <= 128) {
