@@ -292,8 +292,9 @@ int tb_route_backward(const void* d_logits, int64_t stride, int type, int64_t ro
 /* Newton-Schulz orthogonalisation of every matrix of a batch: X = x / (|x| + eps) (Frobenius norm), then `steps` (1 .. 32) times
  * X = (a I + b A + c A^2) X with A = X X^T taken over the shorter side; coefficients = {a, b, c} on the HOST.  x and out have the same
  * type; x_batch and out_batch are the strides between matrices.  Coefficients for which a singular value of at most 1
- * could grow beyond 4 (or |a| + |b| s^2 + |c| s^4 beyond 31) are refused.  fp32 and fp16: products of 22-bit operands (64-bit where the shorter
- * side is at most 64); bf16: 11-bit operands; fp32 sums.  A matrix with an infinity or a NaN comes out NaN. */
+ * could grow beyond 4 (or |a| + |b| s^2 + |c| s^4 beyond 31) are refused.  64-bit throughout where the shorter side is at most 64.  Above: fp32 and fp16
+ * are products of 22-bit operands (elements below 2^-25 of the norm to 2^-47 of it), bf16 of 11-bit ones (2^-36; 1e-3 of the result beside its own rounding: give
+ * fp32 for more), with fp32 sums.  A matrix with an infinity or a NaN comes out NaN. */
 int64_t tb_orthogonalise_workspace(int type, int batch, int rows, int cols);
 int tb_orthogonalise(const void* d_x, int64_t x_batch, int64_t x_stride, int type, int batch, int rows, int cols, int steps,
                      const float* coefficients, float eps, void* d_out, int64_t out_batch, int64_t out_stride, void* d_work,

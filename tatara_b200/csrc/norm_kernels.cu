@@ -10,9 +10,9 @@
 // then the warps in order.  The weight gradients are columns' sums: every block keeps those of its rows in registers over all
 // of its rows, the blocks' rows are added in a fixed order by a second kernel, so that results repeat bit for bit.
 //
-// Measured (inputs not in L2): 65536 x 1536 fp32 forward 120 us (6.7 TB/s), backward 177 us (6.8 TB/s) and 9 us for the columns' sums;
-// 40000 x 2048 fp16 72 us (4.6 TB/s) and 114 us (4.3 TB/s): 16-bit rows are half the bytes for the same instructions, issue slots at 60 %.
-// Rows that start anywhere, 35954 x 1175: fp32 64 us (5.2 TB/s) and 93 us (5.4 TB/s), bf16 55 and 87.  256 x 256: one launch, 2 us.
+// Measured (inputs not in L2): 65536 x 1536 fp32 forward 122 us (6.6 TB/s), backward 176 us (6.9 TB/s) and 9 us for the columns' sums; whole calls in a row,
+// columns' sums included: 40000 x 2048 fp16 66 us (4.9 TB/s) and 107 us (4.6 TB/s): 16-bit rows are half the bytes for the same instructions, issue slots at 60 %.
+// Rows that start anywhere, 35954 x 1175: fp32 63 us (5.4 TB/s) and 86 us (5.9 TB/s), bf16 55 and 83 (the gradient's first kernel 76).  256 x 256: one launch, 2 us.
 #include "op_common.cuh"
 
 namespace {

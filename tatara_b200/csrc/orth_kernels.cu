@@ -12,7 +12,7 @@
 // symmetric and commute: half of every product is computed.  The products are the tensor cores' 64-bit ones (8 x 8 x 4 per warp): a step of
 // 32 x 32 matrices waits for a chain of four of them where thread-wise sums wait for sixteen additions and four times the shared-memory
 // reads.  A fixed order everywhere: results repeat bit for bit.
-// Measured: 9 matrices of 16 x 1536 12.4 us (the loads 2.4, the steps 4), the Muon step of 1024 x 32 16.0 us (the steps 7), 64 x 512 43.6 us (the steps 36:
+// Measured: 9 matrices of 16 x 1536 11.9 us (the loads 2.4, the steps 4), the Muon step of 1024 x 32 15.6 us (the steps 7), 64 x 512 43.7 us (the steps 36:
 // 64-bit products at 40 of the 64 multiply-adds per cycle and SM).
 #include "orth.cuh"
 

@@ -5,7 +5,8 @@
 // most 2^-36 and two by 2^-47.  With two limbs a product is three products of limbs (high low, low high, high high; low low is below 2^-22) into one
 // fp32 accumulator, which the first high product scales back by 2^-11: the steps keep fp32 accuracy, for blocks and rows far below the norm too, at a third of
 // the fp16 rate; fp32 on the CUDA cores has a thirtieth.  (The second limb at the first one's scale left the range sooner: a block of 1e-5 of another came
-// out 2e-4 off, now 2e-7.)  With one limb the roundings (2^-12 of an element, a few times over) stay below those of a bf16 result (2^-9).  Numbers up to 32
+// out 2e-4 off, now 2e-7.)  With one limb the roundings (2^-12 of an element, a few times over: 1.0e-3 to 1.3e-3 of a result) stay below those of a bf16
+// result (2^-9 of an element, 1.7e-3), at a third of the products: half of the time of two limbs at 4 x 1000 x 777, a third at 4096 x 4096.  Numbers up to 32
 // fit; the entry points refuse coefficients that could leave that range.
 //
 // All matrices live in the workspace as 16 KB tiles of 128 rows x 64 columns, stored as the tensor cores want them in shared memory
@@ -24,9 +25,9 @@
 // Every wait is bounded.  An accumulator is announced only when all of its MMAs were issued on operands that have arrived; a warp that waits in vain for one
 // takes NaN for it, and stores those once the copies and MMAs that were under way are done: what a block stores is right or NaN.
 //
-// Measured, 4096 x 4096 in fp32: Gram 159 us, square 168, apply 293 (1.4 PFLOP/s of limb products, tensor pipe 78 to 92 % busy), last product with
-// the weight update 334; the whole Muon step 3.3 to 3.8 ms, where the chip's power limit, not the kernel, sets the clock.  bf16: 1.15 ms.  Small
-// products are bound by what surrounds the MMAs: 4 x 1000 x 777 bf16 takes 124 us in 17 launches of 7 to 9 us, 3 to 4 us of each inside the K loop.
+// Measured, 4096 x 4096 in fp32: Gram 155 us, square 172, apply 290 (1.4 PFLOP/s of limb products, tensor pipe 76 to 92 % busy), last product with
+// the weight update 331; the whole Muon step 3.7 to 3.85 ms, where the chip's power limit, not the kernel, sets the clock.  bf16: 1.25 ms.  Small
+// products are bound by what surrounds the MMAs: 4 x 1000 x 777 bf16 takes 131 us in 17 launches of 7 to 9 us, 3 to 4 us of each inside the K loop.
 #include "orth.cuh"
 
 #include <atomic>

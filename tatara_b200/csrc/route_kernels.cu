@@ -14,8 +14,8 @@
 // rows, then the groups of a block in order, then the blocks in order in 64 bits (second kernel): results repeat bit for bit.
 //
 // What bounds it are issue slots for many experts (490 instructions per row of 256 bf16 logits and eight choices, slots at 73 %: 29 us for 40000
-// rows, whose bytes would take 3.5; their gradient 17 us at 290 instructions per row) and latency for the handful of a net (65536 x 9 fp32, one choice:
-// 10 us with both launches, the gradient 5.5).
+// rows, whose bytes would take 3.5; their gradient 20 us at 290 instructions per row) and latency for the handful of a net (65536 x 9 fp32, one choice:
+// 10 us with both launches, the gradient 5.3).
 #include "op_common.cuh"
 
 namespace {

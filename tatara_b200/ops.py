@@ -80,7 +80,8 @@ def orthogonalise(x: torch.Tensor, *, steps: int = 5, coefficients: Tuple[float,
     """Newton-Schulz orthogonalisation of x [rows, cols] or of every matrix of x [batch, rows, cols].
 
     X = x / (|x| + eps), then `steps` times X = (a I + b A + c A^2) X with A = X X^T over the shorter side: singular values that are not
-    tiny end near 1, the singular vectors stay.  `out` may be x.
+    tiny end near 1, the singular vectors stay.  `out` may be x.  With a shorter side above 64, float32 and float16 matrices are multiplied from 22-bit operands,
+    bfloat16 ones from 11-bit operands at half to a third of the time: 1e-3 of the result beside its own rounding of 1.7e-3.  Give float32 for more.
     """
     return _ops.orthogonalise(x, steps, coefficients, eps, out)
 
