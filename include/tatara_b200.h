@@ -251,7 +251,8 @@ int tb_ft_backward_static_scratch(const float* d_dft, const int32_t* d_indices, 
 
 /* ---- operators on the caller's device tensors ----------------------------------------------
  * No counterpart in the reference.  What a trainer with learned buckets needs beside the step: normalised rows in
- * front of a gate, the choice of a bucket (expert) per row with a balance loss, and the matrix optimizer of hidden weights.  ALL tensor pointers are DEVICE memory of the
+ * front of a gate, the choice of a bucket (expert) per row with a balance loss, the rows sorted by expert and back, rows of a table by token with the table's gradient, and the
+ * matrix optimizer of hidden weights.  ALL tensor pointers are DEVICE memory of the
  * current device, owned by the caller; the work is enqueued on `stream` (a cudaStream_t, NULL = default stream) and not synchronised; nothing is
  * allocated and nothing is kept between calls, so calls on different streams may overlap as long as each has its own workspace.
  * A call's kernels may be started while the kernel ahead of them on the stream is ending; they wait for its end before they touch memory.
@@ -312,6 +313,54 @@ typedef struct tb_muon {
 int64_t tb_muon_step_workspace(int batch, int rows, int cols);
 int tb_muon_step(const tb_muon* cfg, const float* d_w, const float* d_m, const void* d_g, int g_type, int batch, int rows, int cols,
                  float* d_w_out, float* d_m_out, void* d_work, int64_t work_bytes, void* stream, char* err, size_t err_len);
+
+/* Root-mean-square norm on a residual stream: h = x + residual, y = h * rstd * weight per row of n, rstd = 1 / sqrt(mean(h^2) + eps).  The norm is that of the fp32 sum;
+ * d_h receives the sum rounded to the tensors' type, for the next layer and the backward pass.  residual may be NULL (h is x; d_h must be NULL then), weight (fp32 [n]), d_h and d_rstd
+ * (fp32 [rows], kept for the backward pass) may be NULL.  All rows have the same type.  y and h may each be the memory of x or of the residual (not the same one). */
+int tb_rms_norm_forward(const void* d_x, int64_t x_stride, const void* d_residual, int64_t residual_stride, const float* d_weight, float eps, int type,
+                        int64_t rows, int n, void* d_y, int64_t y_stride, void* d_h, int64_t h_stride, float* d_rstd, void* stream, char* err, size_t err_len);
+/* The same with y in 8 bits: q [rows, n] (e4m3 bytes) and scale [rows, ceil(n / group)] (fp32, contiguous) with y ~ q * scale; group: 32, 64, 128 columns, or n (a scale
+ * per row).  scale = max(largest |y| of the group / 448, 2^-126), q = y / scale rounded to nearest.  A group with an infinity or a NaN has q NaN throughout.  q overlaps no other
+ * tensor; h may be the memory of x or of the residual. */
+int tb_rms_norm_quantised(const void* d_x, int64_t x_stride, const void* d_residual, int64_t residual_stride, const float* d_weight, float eps, int type,
+                          int64_t rows, int n, int group, void* d_q, int64_t q_stride, float* d_scale, void* d_h, int64_t h_stride, float* d_rstd, void* stream,
+                          char* err, size_t err_len);
+int64_t tb_rms_norm_backward_workspace(int64_t rows, int n);
+/* dx (the gradient of x and of the residual alike) from dy, h and rstd, plus dresidual, the gradient that arrives at h from elsewhere (may be NULL), and dweight (fp32 [n], written, not
+ * added to; NULL: not wanted, and no workspace).  dx may be the memory of dy, h or dresidual. */
+int tb_rms_norm_backward(const void* d_dy, int64_t dy_stride, const void* d_h, int64_t h_stride, const float* d_rstd, const float* d_weight,
+                         const void* d_dresidual, int64_t dresidual_stride, int type, int64_t rows, int n, void* d_dx, int64_t dx_stride, float* d_dweight,
+                         void* d_work, int64_t work_bytes, void* stream, char* err, size_t err_len);
+
+/* Rows to their experts and back.  index [rows, k] holds the experts of every row (as tb_route_forward writes it: 1 <= k <= 16, experts <= 1024; anything outside
+ * [0, experts) is no choice).  tb_expert_order sorts the choices by expert, within one by row and then choice: expert e has the places [offsets[e], offsets[e + 1]), a multiple of
+ * `align` of them; position [rows, k] is the place of every choice (-1: none), source [slots] the choice r * k + j of every place, -1 at the places that align or missing choices
+ * leave over.  slots is what tb_expert_slots returns (negative: invalid sizes), enough for any choice; offsets [experts + 1] ends at the last place in use. */
+int64_t tb_expert_slots(int64_t rows, int k, int experts, int align);
+int64_t tb_expert_order_workspace(int64_t rows, int k, int experts);
+int tb_expert_order(const int32_t* d_index, int64_t rows, int k, int experts, int align, int32_t* d_position, int32_t* d_source, int64_t slots,
+                    int32_t* d_offsets, void* d_work, int64_t work_bytes, void* stream, char* err, size_t err_len);
+/* out [slots, n]: x[r] at the places of its choices, zeros at places without a choice.  position and source as tb_expert_order wrote them (a place outside [0, slots) is skipped); n <= 2^30
+ * here and below.  The results of these three overlap no other tensor, the gaps between rows of a wider buffer included. */
+int tb_dispatch_forward(const void* d_x, int64_t x_stride, int type, int64_t rows, int n, int k, const int32_t* d_position, const int32_t* d_source,
+                        int64_t slots, void* d_out, int64_t out_stride, void* stream, char* err, size_t err_len);
+/* out[r] = sum over j of gate[r, j] * y[position[r, j]]; a choice without a place adds nothing, whatever its gate.  gate (fp32 [rows, k]) NULL: 1, which makes this the gradient
+ * of tb_dispatch_forward. */
+int tb_combine_forward(const void* d_y, int64_t y_stride, int type, int64_t slots, int64_t rows, int n, int k, const int32_t* d_position, const float* d_gate,
+                       void* d_out, int64_t out_stride, void* stream, char* err, size_t err_len);
+/* dy [slots, n] (zeros at places without a choice) and dgate [rows, k] (0 without a place) of tb_combine_forward from the gradient dout [rows, n] of its result. */
+int tb_combine_backward(const void* d_dout, int64_t dout_stride, const void* d_y, int64_t y_stride, int type, int64_t slots, int64_t rows, int n, int k,
+                        const int32_t* d_position, const int32_t* d_source, const float* d_gate, void* d_dy, int64_t dy_stride, float* d_dgate, void* stream,
+                        char* err, size_t err_len);
+
+/* out [count, n] = scale * table[token]; tokens are 32- or 64-bit whole numbers (token_bytes 4 or 8), one outside [0, rows) has a row of zeros.  out and table have the same type;
+ * results overlap no other tensor, gaps included. */
+int tb_embedding_forward(const void* d_tokens, int token_bytes, int64_t count, const void* d_table, int64_t table_stride, int type, int64_t rows, int n, float scale,
+                         void* d_out, int64_t out_stride, void* stream, char* err, size_t err_len);
+int64_t tb_embedding_backward_workspace(int64_t count, int64_t rows, int n);
+/* dtable [rows, n] = scale * the sum of dy over the tokens of every row, written (not added to), zeros where there are none; of type dtable_type: that of dy, or TB_TYPE_F32. */
+int tb_embedding_backward(const void* d_dy, int64_t dy_stride, int type, const void* d_tokens, int token_bytes, int64_t count, int64_t rows, int n, float scale,
+                          void* d_dtable, int64_t dtable_stride, int dtable_type, void* d_work, int64_t work_bytes, void* stream, char* err, size_t err_len);
 
 /* ---- inputs: PackedSfenValue records -> step inputs, on the device ---------------------
  * Decodes 40-byte records (crates/shogi-format/src/packed_sfen.rs:387-448) and extracts the active

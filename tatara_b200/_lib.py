@@ -111,6 +111,19 @@ SIGNATURES = {
     "tb_orthogonalise": (C.c_int, [vp, i64, i64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(f), f, vp, i64, i64, vp, i64, vp, C.c_char_p, C.c_size_t]),
     "tb_muon_step_workspace": (i64, [C.c_int, C.c_int, C.c_int]),
     "tb_muon_step": (C.c_int, [C.POINTER(Muon), vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp, i64, vp, C.c_char_p, C.c_size_t]),
+    "tb_rms_norm_forward": (C.c_int, [vp, i64, vp, i64, vp, f, C.c_int, i64, C.c_int, vp, i64, vp, i64, vp, vp, C.c_char_p, C.c_size_t]),
+    "tb_rms_norm_quantised": (C.c_int, [vp, i64, vp, i64, vp, f, C.c_int, i64, C.c_int, C.c_int, vp, i64, vp, vp, i64, vp, vp, C.c_char_p, C.c_size_t]),
+    "tb_rms_norm_backward_workspace": (i64, [i64, C.c_int]),
+    "tb_rms_norm_backward": (C.c_int, [vp, i64, vp, i64, vp, vp, vp, i64, C.c_int, i64, C.c_int, vp, i64, vp, vp, i64, vp, C.c_char_p, C.c_size_t]),
+    "tb_expert_slots": (i64, [i64, C.c_int, C.c_int, C.c_int]),
+    "tb_expert_order_workspace": (i64, [i64, C.c_int, C.c_int]),
+    "tb_expert_order": (C.c_int, [vp, i64, C.c_int, C.c_int, C.c_int, vp, vp, i64, vp, vp, i64, vp, C.c_char_p, C.c_size_t]),
+    "tb_dispatch_forward": (C.c_int, [vp, i64, C.c_int, i64, C.c_int, C.c_int, vp, vp, i64, vp, i64, vp, C.c_char_p, C.c_size_t]),
+    "tb_combine_forward": (C.c_int, [vp, i64, C.c_int, i64, i64, C.c_int, C.c_int, vp, vp, vp, i64, vp, C.c_char_p, C.c_size_t]),
+    "tb_combine_backward": (C.c_int, [vp, i64, vp, i64, C.c_int, i64, i64, C.c_int, C.c_int, vp, vp, vp, vp, i64, vp, vp, C.c_char_p, C.c_size_t]),
+    "tb_embedding_forward": (C.c_int, [vp, C.c_int, i64, vp, i64, C.c_int, i64, C.c_int, f, vp, i64, vp, C.c_char_p, C.c_size_t]),
+    "tb_embedding_backward_workspace": (i64, [i64, i64, C.c_int]),
+    "tb_embedding_backward": (C.c_int, [vp, i64, C.c_int, vp, C.c_int, i64, i64, C.c_int, f, vp, i64, C.c_int, vp, i64, vp, C.c_char_p, C.c_size_t]),
     "tb_nccl_unique_id": (C.c_int, [vp]),
     "tb_device_count": (C.c_int, []),
     "tb_version": (C.c_char_p, []),

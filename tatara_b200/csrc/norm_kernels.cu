@@ -13,79 +13,18 @@
 // Measured (inputs not in L2): 65536 x 1536 fp32 forward 122 us (6.6 TB/s), backward 176 us (6.9 TB/s) and 9 us for the columns' sums; whole calls in a row,
 // columns' sums included: 40000 x 2048 fp16 66 us (4.9 TB/s) and 107 us (4.6 TB/s): 16-bit rows are half the bytes for the same instructions, issue slots at 60 %.
 // Rows that start anywhere, 35954 x 1175: fp32 63 us (5.4 TB/s) and 86 us (5.9 TB/s), bf16 55 and 83 (the gradient's first kernel 76).  256 x 256: one launch, 2 us.
-#include "op_common.cuh"
+#include "norm.cuh"
 
 namespace {
 
 #define NORM_REG_N 16384     // longest row that the forward pass keeps in registers
 #define NORM_REG_N_BACK 8192 // ... the backward pass, with two rows and three rows of columns' values
 
-// sum over the W warps of a row, the same bits in every thread; buf: a row's own [W] floats, not reused before the next barrier
-template <int W>
-__device__ __forceinline__ float norm_row_sum(float v, float* buf, int warp_in_row, int lane) {
-    v = op_group_sum<32>(v);
-    if (W == 1) return v;
-    if (lane == 0) buf[warp_in_row] = v;
-    __syncthreads();
-    v = buf[0];
-#pragma unroll
-    for (int w = 1; w < W; ++w) v += buf[w];
-    return v;
-}
-
-// the same of R rows of L lanes (R = 1 with several warps per row), in place
-template <int W, int L, int R>
-__device__ __forceinline__ void norm_rows_sum(float (&v)[R], float* buf, int warp_in_row, int lane) {
-    if (W > 1) {
-        v[0] = norm_row_sum<W>(v[0], buf, warp_in_row, lane);
-        return;
-    }
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1)
-#pragma unroll
-        for (int q = 0; q < R; ++q) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
-}
-
-// the sums of R rows over the W warps of a block, in place; buf is not written again before the next barrier but one
-template <int W, int R>
-__device__ __forceinline__ void norm_block_sums(float (&v)[R], float (*buf)[R], int warp, int lane) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-        for (int q = 0; q < R; ++q) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
-    if (lane == 0)
-#pragma unroll
-        for (int q = 0; q < R; ++q) buf[warp][q] = v[q];
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < R; ++q) v[q] = buf[0][q];
-#pragma unroll
-    for (int k = 1; k < W; ++k)
-#pragma unroll
-        for (int q = 0; q < R; ++q) v[q] += buf[k][q];
-}
-
 // Blocks of the kernels that walk down the rows which one SM holds: 24 warps of 80 registers.  Backward, fp16, 16384 x 768: 20.4 us; 30 warps of 64 (some
 // spilled) 24.6, four rows at a time in 96 registers 26.0, the next rows fetched ahead in 175 registers 34.
 constexpr int norm_per_sm(int warps, int all = 24) { return all / warps < 1 ? 1 : all / warps; }
 // ... backward.  Four warps with a row each hold more of their own: 16 warps of 128 registers (200000 x 256 fp16: 71 us, with 24 warps 89)
 constexpr int norm_per_sm_back(int warps) { return warps == 1 ? 4 : norm_per_sm(warps); }
-
-// VEC columns of a weight or bias, in 16-byte accesses (one element at a time they cost four to eight times the L1 wavefronts of the row
-// itself: 24 -> 8 us for 10000 rows of 1000 fp16)
-template <int VEC>
-__device__ __forceinline__ void norm_columns(const float* __restrict__ p, int col, float none, float (&to)[VEC]) {
-    constexpr int STEP = VEC < 4 ? VEC : 4;
-#pragma unroll
-    for (int i = 0; i < VEC; i += STEP) {
-        float t[STEP];
-#pragma unroll
-        for (int k = 0; k < STEP; ++k) t[k] = none;
-        if (p) op_load<float, STEP>(p + col + i, t);
-#pragma unroll
-        for (int k = 0; k < STEP; ++k) to[i + k] = t[k];
-    }
-}
 
 // W warps per row, VEC adjacent columns per access, CH accesses per thread: a thread holds columns (c * LANES + t) * VEC + i.  With W = 1 a row has L lanes
 // (8 or 16 for rows of up to 64 or 128 columns, or most lanes of a warp idle), which take R rows at once: those share the reads of weight and bias.
@@ -161,10 +100,6 @@ k_norm_forward(const T* x, int64_t x_stride, const float* __restrict__ weight, c
 }
 
 // ---- rows that start anywhere: a thread's columns are single ones -----------------------------------------------------------
-// How many of a thread's places are inside the row for every thread: W warps are the fewest that hold it with eight columns a thread, and sixteen with
-// sixteen columns hold 4097 or more.
-__host__ __device__ constexpr int norm_full(int warps, int vec, int places) { return vec * places == 16 ? places / 2 : places * (warps - 1) / warps; }
-
 // Forward for rows over 256 columns that start anywhere: a block walks down the rows with its columns' weight and bias in registers, R rows at a time.
 // 35954 x 1175: 64 us in fp32 (5.2 TB/s), 55 in bf16; with a warp per row, which reads weight and bias for every row and checks every column, 105 and 127.
 // Two adjacent 16-bit columns per thread, one access where the row starts on a 4-byte boundary: 108 (the branch keeps the loads apart).
@@ -469,46 +404,6 @@ k_norm_columns_long(const T* __restrict__ dy, int64_t dy_stride, const T* __rest
     part_b[(int64_t)blockIdx.y * n + col] = ab;
 }
 
-// dweight and dbias from the blocks' rows: eight columns (a 32-byte sector) per block; thread group r of 128 adds the rows r, r + 128, .., the four
-// groups of a warp are added in halves, then the warps in halves.
-__global__ void __launch_bounds__(1024) k_norm_columns_final(const float* __restrict__ partial, int prows, int n, float* __restrict__ dweight,
-                                                              float* __restrict__ dbias) {
-    __shared__ float s_sum[32][9];
-    float* out = blockIdx.y ? dbias : dweight;
-    op_next_may_start();
-    if (!out) return;  // of the same block all
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = threadIdx.x & 7;
-    const unsigned col = blockIdx.x * 8 + c;
-    const float* p = partial + (int64_t)blockIdx.y * prows * n;
-    float v = 0.0f;
-    op_wait_for_previous();
-    if (col < (unsigned)n)
-        for (int r0 = threadIdx.x >> 3; r0 < prows; r0 += 128 * 8) {
-            float t[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) t[i] = r0 + 128 * i < prows ? p[(int64_t)(r0 + 128 * i) * n + col] : 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v += t[i];
-        }
-    v += __shfl_xor_sync(0xffffffffu, v, 8);
-    v += __shfl_xor_sync(0xffffffffu, v, 16);
-    if (lane < 8) s_sum[warp][c] = v;
-    __syncthreads();
-    if (warp >= 8) return;
-    v = op_group_sum<32>(s_sum[lane][warp]);
-    if (lane == 0 && blockIdx.x * 8 + warp < (unsigned)n) out[blockIdx.x * 8 + warp] = v;
-}
-
-// Warps per row of the kernels that walk down the rows: the fewest that hold it with eight columns a thread (up to 4096 columns, two rows at a time),
-// sixteen with sixteen columns (one row) up to 8192.
-int norm_warps(int n) { return n <= 4096 ? (n + 255) / 256 : 16; }
-template <int FROM, typename F>
-void norm_with_warps(int w, F&& f) {  // f(std::integral_constant<int, W>)
-    if constexpr (FROM <= 16) {
-        if (w == FROM) f(std::integral_constant<int, FROM>());
-        else norm_with_warps<FROM + 1>(w, f);
-    }
-}
 // Blocks: at most what runs at once; 16 rows or more for each, or the blocks' rows of gradients cost as much as the rows themselves, but
 // one per SM as far as the rows go (256 rows of 256: 4 blocks took 12 us).
 int norm_backward_blocks(int64_t rows, int n) {
@@ -606,8 +501,6 @@ void norm_backward_pick(const NormBackward& a) {
         norm_with_warps<1>(norm_warps(a.n), [&](auto w) { norm_backward_go<T, VEC, decltype(w)::value, 32, 8, 2>(a); });
     }
 }
-
-bool norm_aligned(const void* p, int64_t stride, int size) { return ((uintptr_t)p & 15) == 0 && (stride * size) % 16 == 0; }
 
 }  // namespace
 

@@ -12,6 +12,9 @@
 
 #include <initializer_list>
 
+#define OP_MAX_ENTRIES (INT32_MAX - 1023)  // of operators that count entries in int: one step of a block beyond the last
+#define OP_MAX_COLUMNS (1 << 30)  // of operators whose columns are counted in tiles: the end of the last one is within int
+
 static __device__ __forceinline__ float op_float(float v) { return v; }
 static __device__ __forceinline__ float op_float(__half v) { return __half2float(v); }
 static __device__ __forceinline__ float op_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -139,6 +142,14 @@ static inline bool op_meets(const OpRows& a, std::initializer_list<OpRows> vecto
         const uintptr_t first = begin < at + bytes ? 0 : a.rows > 1 ? (begin - at - bytes) / (uintptr_t)a.stride + 1 : 1;
         if (first < (uintptr_t)a.rows && at + first * (uintptr_t)a.stride < begin + (uintptr_t)v.bytes) return true;
     }
+    return false;
+}
+
+// Whether rows, gaps between them included, have a byte in common with one of the others, gaps included: for tensors of different shapes.
+static inline bool op_extents_meet(const OpRows& a, std::initializer_list<OpRows> others) {
+    const auto end = [](const OpRows& r) { return (uintptr_t)r.p + (uintptr_t)(r.rows - 1) * (uintptr_t)r.stride + (uintptr_t)r.bytes; };
+    for (const OpRows& o : others)
+        if (a.p && o.p && a.rows > 0 && o.rows > 0 && a.bytes > 0 && o.bytes > 0 && (uintptr_t)a.p < end(o) && (uintptr_t)o.p < end(a)) return true;
     return false;
 }
 

@@ -16,6 +16,7 @@
 #include <math.h>
 #include <stdarg.h>
 #include <string>
+#include <vector>
 
 #include "../../include/tatara_b200.h"
 
@@ -399,6 +400,254 @@ PyObject* muon_step(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     BODY_END
 }
 
+// `out`, which has to match `like`, or a new tensor of its shape
+at::Tensor output_named(PyObject* out, const at::Tensor& like, const char* name) {
+    if (out == Py_None) return make(like, like.sizes(), like.scalar_type());
+    const at::Tensor& t = cuda_tensor(out, name);
+    if (t.sizes() != like.sizes() || t.scalar_type() != like.scalar_type() || t.device() != like.device()) refuse("%s must match x", name);
+    return t;
+}
+// a [rows, n] tensor of another one's shape, type and device; an undefined one for None
+at::Tensor matching(PyObject* o, const at::Tensor& like, const char* name) {
+    if (o == Py_None) return at::Tensor();
+    const at::Tensor& t = typed(o, name);
+    if (t.sizes() != like.sizes() || t.scalar_type() != like.scalar_type() || t.device() != like.device()) refuse("%s must match the other rows", name);
+    return t;
+}
+const void* address(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// x, weight, residual, eps, out, residual_out; and with group (None: a scale per row) in the place of out: 8 bits
+PyObject* rms_norm(PyObject* const* a, bool eight) {
+    const at::Tensor& x = typed(a[0], "x");
+    const int64_t xs = rows_of(x, "x"), rows = x.size(0);
+    const int n = side(x.size(1), "n");
+    const float* w = static_cast<float*>(vector_of(a[1], "weight", x, {n}));
+    const at::Tensor r = matching(a[2], x, "residual");
+    const int64_t rs = r.defined() ? rows_of(r, "residual") : 0;
+    const float eps = (float)number(a[3], "eps");
+    if (!r.defined() && a[5] != Py_None) refuse("residual_out needs a residual");
+    const int group = !eight ? 0 : a[4] == Py_None ? n : whole(a[4], "group");
+    if (eight && group != 32 && group != 64 && group != 128 && group != n) refuse("group must be 32, 64, 128 or the number of columns (got %d)", group);
+    const On on(x);
+    const at::Tensor h = r.defined() ? output_named(a[5], x, "residual_out") : at::Tensor();
+    const int64_t hs = h.defined() ? rows_of(h, "residual_out") : 0;
+    const at::Tensor y = eight ? make(x, x.sizes(), at::kFloat8_e4m3fn) : output(a[4], x), rstd = make(x, {rows}, at::kFloat);
+    const int64_t ys = rows_of(y, "out");
+    char err[256];
+    if (eight) {
+        const at::Tensor scale = make(x, {rows, n < 1 ? 0 : (n + (int64_t)group - 1) / group}, at::kFloat);
+        check(tb_rms_norm_quantised(x.data_ptr(), xs, address(r), rs, w, eps, type_of(x), rows, n, group, y.data_ptr(), ys, scale.data_ptr<float>(), const_cast<void*>(address(h)), hs,
+                                    rstd.data_ptr<float>(), on.stream, err, sizeof err),
+              "tb_rms_norm_quantised", err);
+        if (r.defined()) written(a[5]);
+        return tuple_of({y, scale, h.defined() ? h : x, rstd});
+    }
+    check(tb_rms_norm_forward(x.data_ptr(), xs, address(r), rs, w, eps, type_of(x), rows, n, y.data_ptr(), ys, const_cast<void*>(address(h)), hs, rstd.data_ptr<float>(), on.stream, err, sizeof err),
+          "tb_rms_norm_forward", err);
+    written(a[4]);
+    if (r.defined()) written(a[5]);
+    return tuple_of({y, h.defined() ? h : x, rstd});
+}
+PyObject* rms_norm_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    BODY_BEGIN
+    arguments(n_args, 6);
+    return rms_norm(a, false);
+    BODY_END
+}
+PyObject* rms_norm_quantised(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    BODY_BEGIN
+    arguments(n_args, 6);
+    return rms_norm(a, true);
+    BODY_END
+}
+
+// dy, h, rstd, weight, dresidual, out
+PyObject* rms_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    BODY_BEGIN
+    arguments(n_args, 6);
+    const at::Tensor &h = typed(a[1], "h"), dy = matching(a[0], h, "dy");
+    if (!dy.defined()) refuse("dy must be a CUDA tensor");
+    const int64_t hs = rows_of(h, "h"), gs = rows_of(dy, "dy"), rows = h.size(0);
+    const int n = side(h.size(1), "n");
+    const float* r = static_cast<float*>(vector_of(a[2], "rstd", h, {rows}, at::kFloat, true));
+    const float* w = static_cast<float*>(vector_of(a[3], "weight", h, {n}));
+    const at::Tensor dres = matching(a[4], h, "dresidual");
+    const int64_t ds = dres.defined() ? rows_of(dres, "dresidual") : 0;
+    const On on(h);
+    const at::Tensor dx = output(a[5], h), dweight = make(h, {n}, at::kFloat);
+    const Work work(h, tb_rms_norm_backward_workspace(rows, n));
+    char err[256];
+    check(tb_rms_norm_backward(dy.data_ptr(), gs, h.data_ptr(), hs, r, w, address(dres), ds, type_of(h), rows, n, dx.data_ptr(), rows_of(dx, "out"), dweight.data_ptr<float>(), work.at(), work.bytes,
+                               on.stream, err, sizeof err),
+          "tb_rms_norm_backward", err);
+    written(a[5]);
+    return tuple_of({dx, dweight});
+    BODY_END
+}
+
+// index, experts, align
+PyObject* expert_order(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    BODY_BEGIN
+    arguments(n_args, 3);
+    const at::Tensor& ix = cuda_tensor(a[0], "index");
+    if (ix.dim() != 2) refuse("index must have two dimensions (got %d)", (int)ix.dim());
+    const int64_t rows = ix.size(0);
+    const int k = side(ix.size(1), "k");
+    const int32_t* index = static_cast<int32_t*>(vector_of(a[0], "index", ix, {rows, k}, at::kInt, true));
+    const int experts = whole(a[1], "experts"), align = whole(a[2], "align");
+    const int64_t slots = tb_expert_slots(rows, k, experts, align);
+    const On on(ix);
+    const int64_t room = slots > 0 ? slots : 0;  // invalid sizes are refused below
+    const at::Tensor position = make(ix, {rows, k}, at::kInt), source = make(ix, {room}, at::kInt), offsets = make(ix, {experts > 0 ? experts + (int64_t)1 : 1}, at::kInt);
+    const Work work(ix, tb_expert_order_workspace(rows, k, experts));
+    char err[256];
+    check(tb_expert_order(index, rows, k, experts, align, position.data_ptr<int>(), source.data_ptr<int>(), room, offsets.data_ptr<int>(), work.at(), work.bytes, on.stream, err, sizeof err),
+          "tb_expert_order", err);
+    return tuple_of({position, source, offsets});
+    BODY_END
+}
+
+struct Places {
+    const int32_t *position, *source;
+    int64_t rows, slots;
+    int k;
+};
+// order.position and order.source beside `like`
+Places places_of(PyObject* position, PyObject* source, const at::Tensor& like) {
+    Places p;
+    const at::Tensor &po = cuda_tensor(position, "order.position"), &so = cuda_tensor(source, "order.source");
+    if (po.dim() != 2 || so.dim() != 1) refuse("order.position must have two dimensions and order.source one");
+    p.rows = po.size(0);
+    p.k = side(po.size(1), "k");
+    p.slots = so.size(0);
+    p.position = static_cast<int32_t*>(vector_of(position, "order.position", like, {p.rows, p.k}, at::kInt, true));
+    p.source = static_cast<int32_t*>(vector_of(source, "order.source", like, {p.slots}, at::kInt, true));
+    return p;
+}
+void as_many(const at::Tensor& t, const char* name, int64_t rows, const char* what) {
+    if (t.size(0) != rows) refuse("%s must have %lld rows, as the order has %s (got %lld)", name, (long long)rows, what, (long long)t.size(0));
+}
+
+// x, position, source
+PyObject* dispatch_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    BODY_BEGIN
+    arguments(n_args, 3);
+    const at::Tensor& x = typed(a[0], "x");
+    const int64_t xs = rows_of(x, "x");
+    const Places p = places_of(a[1], a[2], x);
+    as_many(x, "x", p.rows, "rows");
+    const int n = side(x.size(1), "n");
+    const On on(x);
+    const at::Tensor out = make(x, {p.slots, n}, x.scalar_type());
+    char err[256];
+    check(tb_dispatch_forward(x.data_ptr(), xs, type_of(x), p.rows, n, p.k, p.position, p.source, p.slots, out.data_ptr(), n, on.stream, err, sizeof err), "tb_dispatch_forward", err);
+    return THPVariable_Wrap(out);
+    BODY_END
+}
+
+// y, position, source, gate (None: 1)
+PyObject* combine_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    BODY_BEGIN
+    arguments(n_args, 4);
+    const at::Tensor& y = typed(a[0], "y");
+    const int64_t ys = rows_of(y, "y");
+    const Places p = places_of(a[1], a[2], y);
+    as_many(y, "y", p.slots, "places");
+    const int n = side(y.size(1), "n");
+    const float* gate = static_cast<float*>(vector_of(a[3], "gate", y, {p.rows, p.k}));
+    const On on(y);
+    const at::Tensor out = make(y, {p.rows, n}, y.scalar_type());
+    char err[256];
+    check(tb_combine_forward(y.data_ptr(), ys, type_of(y), p.slots, p.rows, n, p.k, p.position, gate, out.data_ptr(), n, on.stream, err, sizeof err), "tb_combine_forward", err);
+    return THPVariable_Wrap(out);
+    BODY_END
+}
+
+// dout, y, position, source, gate
+PyObject* combine_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    BODY_BEGIN
+    arguments(n_args, 5);
+    const at::Tensor &y = typed(a[1], "y"), &dout = typed(a[0], "dout");
+    const int64_t ys = rows_of(y, "y"), ds = rows_of(dout, "dout");
+    const Places p = places_of(a[2], a[3], y);
+    as_many(y, "y", p.slots, "places");
+    as_many(dout, "dout", p.rows, "rows");
+    if (dout.size(1) != y.size(1) || dout.scalar_type() != y.scalar_type() || dout.device() != y.device()) refuse("dout must match y");
+    const int n = side(y.size(1), "n");
+    const float* gate = static_cast<float*>(vector_of(a[4], "gate", y, {p.rows, p.k}, at::kFloat, true));
+    const On on(y);
+    const at::Tensor dy = make(y, {p.slots, n}, y.scalar_type()), dgate = make(y, {p.rows, p.k}, at::kFloat);
+    char err[256];
+    check(tb_combine_backward(dout.data_ptr(), ds, y.data_ptr(), ys, type_of(y), p.slots, p.rows, n, p.k, p.position, p.source, gate, dy.data_ptr(), n, dgate.data_ptr<float>(), on.stream, err, sizeof err),
+          "tb_combine_backward", err);
+    return tuple_of({dy, dgate});
+    BODY_END
+}
+
+// contiguous tokens of any shape beside `like`
+const at::Tensor& tokens_of(PyObject* o, const at::Tensor& like) {
+    const at::Tensor& t = cuda_tensor(o, "tokens");
+    if (t.device() != like.device()) refuse("tokens must be on %s", like.device().str().c_str());
+    if ((t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) || !t.is_contiguous()) refuse("tokens must be a contiguous int32 or int64 tensor");
+    return t;
+}
+
+// tokens, table, scale, out
+PyObject* embedding_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    BODY_BEGIN
+    arguments(n_args, 4);
+    const at::Tensor& table = typed(a[1], "table");
+    const int64_t ts = rows_of(table, "table"), rows = table.size(0);
+    const int n = side(table.size(1), "n");
+    const at::Tensor& tokens = tokens_of(a[0], table);
+    const double scale = number(a[2], "scale");
+    const On on(table);
+    std::vector<int64_t> shape = tokens.sizes().vec();
+    shape.push_back(n);
+    at::Tensor out;
+    int64_t os = n;
+    if (a[3] == Py_None) {
+        out = make(table, shape, table.scalar_type());
+    } else {
+        out = cuda_tensor(a[3], "out");
+        if (out.sizes() != at::IntArrayRef(shape) || out.scalar_type() != table.scalar_type() || out.device() != table.device()) refuse("out must be a tensor like table of shape %s", shape_text(shape).c_str());
+        if (out.dim() == 2) os = rows_of(out, "out");
+        else if (!out.is_contiguous()) refuse("out must be contiguous, or have two dimensions");
+    }
+    char err[256];
+    check(tb_embedding_forward(tokens.data_ptr(), (int)tokens.element_size(), tokens.numel(), table.data_ptr(), ts, type_of(table), rows, n, (float)scale, out.data_ptr(), os, on.stream, err, sizeof err),
+          "tb_embedding_forward", err);
+    written(a[3]);
+    return THPVariable_Wrap(out);
+    BODY_END
+}
+
+// dy, tokens, rows, scale, whether dtable is float32
+PyObject* embedding_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    BODY_BEGIN
+    arguments(n_args, 5);
+    const at::Tensor& dy = typed(a[0], "dy");
+    const at::Tensor& tokens = tokens_of(a[1], dy);
+    if (dy.dim() != tokens.dim() + 1 || dy.sizes().slice(0, tokens.dim()) != tokens.sizes()) refuse("dy must have a row for each token: the shape of tokens and one more dimension");
+    const int n = side(dy.size(-1), "n");
+    int64_t gs = n;
+    if (dy.dim() == 2) gs = rows_of(dy, "dy");
+    else if (!dy.is_contiguous()) refuse("dy must be contiguous, or have two dimensions");
+    const int64_t rows = whole(a[2], "rows");
+    const double scale = number(a[3], "scale");
+    const bool single = truth(a[4], "float32");
+    if (rows < 1) refuse("rows must be positive (got %lld)", (long long)rows);
+    const On on(dy);
+    const at::Tensor dtable = make(dy, {rows, n}, single ? at::kFloat : dy.scalar_type());
+    const Work work(dy, tb_embedding_backward_workspace(tokens.numel(), rows, n));
+    char err[256];
+    check(tb_embedding_backward(dy.data_ptr(), gs, type_of(dy), tokens.data_ptr(), (int)tokens.element_size(), tokens.numel(), rows, n, (float)scale, dtable.data_ptr(), n, type_of(dtable), work.at(),
+                                work.bytes, on.stream, err, sizeof err),
+          "tb_embedding_backward", err);
+    return THPVariable_Wrap(dtable);
+    BODY_END
+}
+
 PyObject* set_error(PyObject*, PyObject* type) {
     Py_INCREF(type);
     Py_XDECREF(g_error);
@@ -408,6 +657,8 @@ PyObject* set_error(PyObject*, PyObject* type) {
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {FAST(layer_norm_forward), FAST(layer_norm_backward), FAST(route_forward), FAST(route_backward), FAST(orthogonalise), FAST(muon_step),
+                           FAST(rms_norm_forward), FAST(rms_norm_quantised), FAST(rms_norm_backward), FAST(expert_order), FAST(dispatch_forward), FAST(combine_forward),
+                           FAST(combine_backward), FAST(embedding_forward), FAST(embedding_backward),
                            {"set_error", set_error, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_ops", "the operators on torch tensors", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,5 +1,5 @@
-"""Operators on torch CUDA tensors for trainers with learned buckets: layer norm, routing with a balance loss, Newton-Schulz
-orthogonalisation and the Muon step.
+"""Operators on torch CUDA tensors for trainers with learned buckets: layer norm, root-mean-square norm on a residual stream, routing with a balance loss, rows sorted
+by expert and back, rows of a table by token, Newton-Schulz orthogonalisation and the Muon step.
 
 The functions check their arguments, take outputs and workspaces from torch's allocator and enqueue kernels of libtatara_b200.so on torch's current
 stream of the tensors' device (csrc/torch_ops.cpp).  Nothing is synchronised and nothing is kept between calls.  Wrong arguments raise
@@ -69,6 +69,91 @@ def route_backward(logits: torch.Tensor, routing: Routing, dgate: Optional[torch
     """The logits' gradient from the gradients of the gates (float32 [rows, k]) and of the two losses (float32 [2]); the choice and the counts
     are constants.  `renormalise` and `mask` as in the `route_forward` call that gave `routing`."""
     return _ops.route_backward(logits, routing.index, routing.gate, routing.counts, routing.rows, dgate, dlosses, renormalise, mask)
+
+
+# ---- root-mean-square norm ----------------------------------------------------------------------------------------------
+def rms_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                     out: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, h, rstd): h = x + residual and y = h * rstd * weight for every row of x [rows, n]; rstd = 1 / sqrt(mean(h^2) + eps).
+
+    x, residual, y and h are of one type (float32, float16 or bfloat16) with any row strides, weight float32 [n].  y is the norm of the 32-bit sum, h the sum
+    rounded to the type (x itself without a residual): the residual of the next layer.  h and rstd (float32 [rows]) are what `rms_norm_backward` takes.  `out` and
+    `residual_out` may be x or residual, not both the same.  Without `eps`, a row of zeros is NaN.
+    """
+    return _ops.rms_norm_forward(x, weight, residual, eps, out, residual_out)
+
+
+def rms_norm_quantised(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                       group: Optional[int] = None, residual_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(q, scale, h, rstd): `rms_norm_forward` with y ~ q * scale in 8 bits.
+
+    q is float8_e4m3fn [rows, n], scale float32 [rows, ceil(n / group)]: the largest |y| of a row's group of 32, 64, 128 or (None) all columns over 448, at least
+    2^-126.  The backward pass is `rms_norm_backward`, as if y had not been rounded.  A group that holds an infinity or a NaN is NaN throughout.
+    """
+    return _ops.rms_norm_quantised(x, weight, residual, eps, group, residual_out)
+
+
+def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, weight: Optional[torch.Tensor] = None, *, dresidual: Optional[torch.Tensor] = None,
+                      out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(dx, dweight) of `rms_norm_forward` from the gradients dy of y and `dresidual` of h (what later layers send back along the residual stream).  dx [rows, n] is the
+    gradient of x and of the residual alike, dweight float32 [n].  `out` may be dy, h or dresidual."""
+    return _ops.rms_norm_backward(dy, h, rstd, weight, dresidual, out)
+
+
+# ---- rows by expert -----------------------------------------------------------------------------------------------------
+class Order(NamedTuple):
+    """Where the choices of a router go when they are sorted by expert."""
+    position: torch.Tensor  # int32 [rows, k]: the place of every choice, -1 where there is none
+    source: torch.Tensor    # int32 [places]: the choice r * k + j of every place, -1 where there is none
+    offsets: torch.Tensor   # int32 [experts + 1]: expert e has the places offsets[e] to offsets[e + 1]
+
+
+def expert_order(index: torch.Tensor, experts: int, *, align: int = 1) -> Order:
+    """The choices index [rows, k] (int32, as in a `Routing`) sorted by expert, an expert's by row and then choice.
+
+    Anything outside [0, experts) is no choice.  Every expert has a multiple of `align` places, as tiles of a product need them.  The number of places is that of the worst
+    case, so that nothing waits for the device: rows * k without `align`; those behind offsets[experts] are left over.  At most 1024 experts and 16 choices.
+    """
+    return Order._make(_ops.expert_order(index, experts, align))
+
+
+def dispatch_forward(x: torch.Tensor, order: Order) -> torch.Tensor:
+    """[places, n]: the row x[r] at every place of its choices, zeros at places without a choice.  x [rows, n] is float32, float16 or bfloat16."""
+    return _ops.dispatch_forward(x, order.position, order.source)
+
+
+def dispatch_backward(dy: torch.Tensor, order: Order) -> torch.Tensor:
+    """The gradient of `dispatch_forward`'s x from that of its places: every row's are added up."""
+    return _ops.combine_forward(dy, order.position, order.source, None)
+
+
+def combine_forward(y: torch.Tensor, order: Order, gate: torch.Tensor) -> torch.Tensor:
+    """[rows, n]: out[r] = sum of gate[r, j] * y[position[r, j]] over the choices of row r that have a place; y [places, n], gate float32 [rows, k]."""
+    if gate is None:
+        raise TrainerError("gate must be a tensor")
+    return _ops.combine_forward(y, order.position, order.source, gate)
+
+
+def combine_backward(dout: torch.Tensor, y: torch.Tensor, order: Order, gate: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(dy, dgate) of `combine_forward` from the gradient dout [rows, n] of its result: dy [places, n], zeros at places without a choice, and dgate float32 [rows, k], 0
+    where a choice has no place."""
+    return _ops.combine_backward(dout, y, order.position, order.source, gate)
+
+
+# ---- rows by token ------------------------------------------------------------------------------------------------------
+def embedding_forward(tokens: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """scale * table[tokens]: tokens int32 or int64 of any shape, table [rows, n] float32, float16 or bfloat16.  A token outside the table (-1 for padding) has a row of zeros."""
+    return _ops.embedding_forward(tokens, table, scale, out)
+
+
+def embedding_backward(dy: torch.Tensor, tokens: torch.Tensor, rows: int, *, scale: float = 1.0, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The gradient [rows, n] of `embedding_forward`'s table from dy (tokens' shape and n): scale * the sum of dy over the tokens of every row, zeros where there are none.
+
+    Sums are 32 bits wide in an order that depends on the tokens alone.  `dtype` is that of dy (the default) or float32.
+    """
+    if dtype not in (None, torch.float32, getattr(dy, "dtype", None)):
+        raise TrainerError("dtype must be that of dy or float32")
+    return _ops.embedding_backward(dy, tokens, rows, scale, dtype == torch.float32)
 
 
 # ---- orthogonalisation ------------------------------------------------------------------------------------------------
