@@ -16,6 +16,7 @@ namespace {
 
 #define EMBED_THREADS 256
 #define EMBED_WARPS 8
+#define EMBED_ROWS 8  // table rows per warp at most
 
 struct Tokens {
     const void* p;
@@ -32,7 +33,7 @@ struct Tokens {
 // L lanes take CH * VEC columns each of R tokens' rows
 template <typename T, int VEC, int L, int CH, int R>
 __global__ void __launch_bounds__(EMBED_THREADS)
-k_embed_forward(Tokens tokens, int64_t count, const T* __restrict__ table, int64_t table_stride, int n, int tiles, float scale, T* __restrict__ out, int64_t out_stride) {
+k_embed_forward(Tokens tokens, int64_t count, const T* table, int64_t table_stride, int n, int tiles, float scale, T* __restrict__ out, int64_t out_stride) {
     const int64_t unit = (int64_t)blockIdx.x * (EMBED_THREADS / L) + threadIdx.x / L, group = unit / tiles;
     const int t = threadIdx.x % L, first = ((int)(unit - group * tiles) * (L * CH) + t) * VEC;
     op_next_may_start();
@@ -62,21 +63,18 @@ k_embed_forward(Tokens tokens, int64_t count, const T* __restrict__ table, int64
 }
 
 // ---- the sort ----------------------------------------------------------------------------------------------------------------
-// the first digits, of the tokens themselves
-struct FirstKey {
+// the first digits, of the tokens themselves; a token outside the table is -1 and has no place
+struct FirstSource {
     Tokens tokens;
     int mask;
-    __device__ __forceinline__ int operator()(int64_t i) const {
-        const int t = tokens(i);
-        return t < 0 ? -1 : t & mask;
-    }
+    __device__ __forceinline__ int operator()(int64_t i) const { return tokens(i); }
+    __device__ __forceinline__ int key(int v) const { return v < 0 ? -1 : v & mask; }
 };
 struct FirstPut {
-    Tokens tokens;
     int *key, *id, *count;  // count: of the tokens in the table, and (zero here) of the long lists
-    __device__ __forceinline__ void operator()(int64_t i, int place) const {
+    __device__ __forceinline__ void operator()(int64_t i, int v, int place) const {
         if (place < 0) return;
-        key[place] = tokens(i);
+        key[place] = v;
         id[place] = (int)i;
     }
     __device__ __forceinline__ void rest(const int*, const int* begin, const SortPlan& p) const {
@@ -84,25 +82,29 @@ struct FirstPut {
     }
 };
 // further digits, of what the digits before have sorted
-struct NextKey {
-    const int *key, *count;
+struct NextSource {
+    const int *sorted, *count;
     int shift, mask;
-    __device__ __forceinline__ int operator()(int64_t i) const { return i < *count ? key[i] >> shift & mask : -1; }
+    __device__ __forceinline__ int operator()(int64_t i) const {
+        const int v = sorted[i];  // behind the last one anything
+        return i < *count ? v : -1;
+    }
+    __device__ __forceinline__ int key(int v) const { return v < 0 ? -1 : v >> shift & mask; }
 };
 struct NextPut {
-    const int *key_in, *id_in;
+    const int* id_in;
     int *key, *id;
-    __device__ __forceinline__ void operator()(int64_t i, int place) const {
+    __device__ __forceinline__ void operator()(int64_t i, int v, int place) const {
         if (place < 0) return;
-        key[place] = key_in[i];
+        key[place] = v;
         id[place] = id_in[i];
     }
     __device__ __forceinline__ void rest(const int*, const int*, const SortPlan&) const {}
 };
 
-// How many of the sorted keys are below v, by a warp: 32 of them are looked at at once
-__device__ __forceinline__ int embed_below(const int* __restrict__ key, int count, int v, int lane) {
-    unsigned lo = 0, hi = (unsigned)count;
+// The first of the sorted keys [from, to) that is v or more (to: none), by a warp: 32 of them are looked at at once
+__device__ __forceinline__ int embed_below(const int* key, int from, int to, int v, int lane) {
+    unsigned lo = (unsigned)from, hi = (unsigned)to;
     while (lo < hi) {
         const unsigned step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step - 1;  // below 2^32
         const unsigned below = __popc(__ballot_sync(0xffffffffu, at < hi && key[at] < v));
@@ -124,32 +126,28 @@ __device__ __forceinline__ void embed_store(O* p, const float (&from)[VEC]) {
     }
 }
 
-// acc += the rows of the entries [from, to) of the list, in order; a lane's columns are first + c * 32 * VEC
 template <typename T, int VEC, int CH>
-__device__ __forceinline__ void embed_add(float (&acc)[CH][VEC], const T* __restrict__ dy, int64_t dy_stride, const int* __restrict__ id, int from, int to, int first, int n, int lane) {
-    constexpr int U = CH * VEC * sizeof(T) >= 64 ? 2 : 4;  // rows on their way together
-    for (int i0 = from; i0 < to; i0 += 32) {
-        const int mine = i0 + lane < to ? id[i0 + lane] : 0, many = min(32, to - i0);
-        for (int j0 = 0; j0 < many; j0 += U) {
-            OpRaw<T, VEC> v[U][CH];
+__device__ __forceinline__ void embed_load(OpRaw<T, VEC> (&x)[CH], const T* dy, int64_t dy_stride, int row, bool there, int first, int n) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int row = __shfl_sync(0xffffffffu, mine, j0 + u);
-#pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    const int col = first + c * 32 * VEC;
-                    v[u][c].zero();
-                    if (j0 + u < many && col < n) v[u][c].load(dy + row * dy_stride + col);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int c = 0; c < CH; ++c)
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) acc[c][i] += v[u][c].get(i);
-        }
+    for (int c = 0; c < CH; ++c) {
+        const int col = first + c * 32 * VEC;
+        x[c].zero();
+        if (there && col < n) x[c].load(dy + row * dy_stride + col);
     }
+}
+template <typename T, int VEC, int CH>
+__device__ __forceinline__ void embed_add(float (&acc)[CH][VEC], const OpRaw<T, VEC> (&x)[CH]) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[c][i] += x[c].get(i);
+}
+template <int VEC, int CH>
+__device__ __forceinline__ void embed_zero(float (&acc)[CH][VEC]) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[c][i] = 0.0f;
 }
 
 struct EmbedLong {       // a token whose list is longer than a piece: its first sum, and the list's last piece
@@ -163,11 +161,12 @@ struct EmbedList {
     float* part;         // [pieces][2][n]: the sums of a piece's first and of its last token, where those have long lists
 };
 
-// Blocks below pieces * tiles: a piece of the list and a tile of columns.  The others: a table row and a tile per warp.
+// Blocks below pieces * tiles: a piece of the list and a tile of columns.  The others: `per` table rows and a tile per warp; it looks for the first row's place in the
+// list once and reads on from there, 32 entries at a time.
 template <typename T, typename O, int VEC, int CH>
-__global__ void __launch_bounds__(EMBED_THREADS)
-k_embed_rows(const T* __restrict__ dy, int64_t dy_stride, EmbedList list, int64_t rows, int n, int tiles, float scale, O* __restrict__ out, int64_t out_stride) {
-    constexpr int TILE = 32 * VEC * CH;
+__global__ void __launch_bounds__(EMBED_THREADS, 4)
+k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n, int tiles, int per, float scale, O* __restrict__ out, int64_t out_stride) {
+    constexpr int TILE = 32 * VEC * CH, U = CH == 1 ? 8 : CH == 2 ? 4 : 2;  // rows on their way together
     __shared__ float s_part[EMBED_WARPS][TILE];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, piece_blocks = list.pieces * tiles;
     op_next_may_start();
@@ -175,41 +174,81 @@ k_embed_rows(const T* __restrict__ dy, int64_t dy_stride, EmbedList list, int64_
     const int count = *list.count;
     float acc[CH][VEC];
     if ((int64_t)blockIdx.x >= piece_blocks) {
-        const int64_t unit = ((int64_t)blockIdx.x - piece_blocks) * EMBED_WARPS + warp, row = unit / tiles;
-        if (row >= rows) return;
-        const int first = ((int)(unit - row * tiles) * 32 * CH + lane) * VEC, v = (int)row;
-        const int from = embed_below(list.key, count, v, lane);
-        int to = from + __popc(__ballot_sync(0xffffffffu, from + lane < count && list.key[from + lane] == v));
-        if (to - from == 32) to = embed_below(list.key, count, v + 1, lane);
-        if (to - from > list.piece) return;
+        const int64_t unit = ((int64_t)blockIdx.x - piece_blocks) * EMBED_WARPS + warp, group = unit / tiles, row0 = group * per;
+        if (row0 >= rows) return;
+        const int first = ((int)(unit - group * tiles) * 32 * CH + lane) * VEC, many = (int)min((int64_t)per, rows - row0);
+        const int end_row = (int)row0 + many;
+        const auto store = [&](int64_t v) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
+            for (int c = 0; c < CH; ++c) {
+                const int col = first + c * 32 * VEC;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[c][i] = 0.0f;
-        embed_add<T, VEC, CH>(acc, dy, dy_stride, list.id, from, to, first, n, lane);
+                for (int i = 0; i < VEC; ++i) acc[c][i] *= scale;
+                if (col < n) embed_store<O, VEC>(out + v * out_stride + col, acc[c]);
+            }
+            embed_zero(acc);
+        };
+        int v = (int)row0, last = -1;  // acc is v's; the key before the window
+        embed_zero(acc);
+        for (int at = embed_below(list.key, 0, count, v, lane);;) {
+            const int key = lane < count - at ? list.key[at + lane] : INT32_MAX, id = lane < count - at ? list.id[at + lane] : 0;
+            const int ahead = list.piece < count - at - lane ? list.key[at + list.piece + lane] : -1, before = __shfl_up_sync(0xffffffffu, key, 1);
+            // up to the window's first list that is longer than a piece, which is added up by pieces
+            const unsigned longer = __ballot_sync(0xffffffffu, ahead == key && key != (lane ? before : last) && key < end_row);
+            const int mine = __popc(__ballot_sync(0xffffffffu, key < end_row)), here = longer ? __ffs(longer) - 1 : mine;
+            for (int j0 = 0; j0 < here; j0 += U) {
+                OpRaw<T, VEC> x[U][CH];
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int col = first + c * 32 * VEC;
+                for (int u = 0; u < U; ++u) embed_load<T, VEC, CH>(x[u], dy, dy_stride, __shfl_sync(0xffffffffu, id, j0 + u), j0 + u < here, first, n);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[c][i] *= scale;
-            if (col < n) embed_store<O, VEC>(out + row * out_stride + col, acc[c]);
+                for (int u = 0; u < U; ++u) {
+                    const int k = __shfl_sync(0xffffffffu, key, j0 + u);
+                    if (j0 + u >= here) break;
+                    for (; v < k; ++v) store(v);
+                    embed_add(acc, x[u]);
+                }
+            }
+            if (longer) {
+                last = __shfl_sync(0xffffffffu, key, here);
+                for (; v < last; ++v) store(v);
+                ++v;
+                at = embed_below(list.key, at + here, count, v, lane);
+            } else {
+                if (mine < 32) break;
+                last = __shfl_sync(0xffffffffu, key, 31);
+                at += 32;
+            }
         }
+        for (; v < end_row; ++v) store(v);
         return;
     }
     const int piece = blockIdx.x / tiles, tile = blockIdx.x - piece * tiles, first = (tile * 32 * CH + lane) * VEC;
-    const int64_t from = (int64_t)piece * list.piece;
-    if (from >= count) return;
-    const int to = (int)min(from + list.piece, (int64_t)count), first_key = list.key[from], last_key = list.key[to - 1];
+    if ((int64_t)piece * list.piece >= count) return;
+    const int from = piece * list.piece, to = list.piece < count - from ? from + list.piece : count, first_key = list.key[from], last_key = list.key[to - 1];
     for (int slot = 0; slot < (first_key == last_key ? 1 : 2); ++slot) {
-        const int v = slot ? last_key : first_key, begin = embed_below(list.key, count, v, lane), end = embed_below(list.key, count, v + 1, lane);
-        if (end - begin <= list.piece) continue;
-        if (begin >= from && tile == 0 && threadIdx.x == 0) list.lists[atomicAdd(list.count + 1, 1)] = {v, piece * 2 + slot, (end - 1) / list.piece};
-        const int b = max(begin, (int)from), e = min(end, to), share = (e - b + EMBED_WARPS - 1) / EMBED_WARPS;
+        // the token's entries of this piece, and whether the list is longer than a piece
+        const int v = slot ? last_key : first_key;
+        const int b = slot ? embed_below(list.key, from, to, v, lane) : from, e = slot || last_key == v ? to : embed_below(list.key, from, to, v + 1, lane);
+        const bool begins = slot || from == 0 || list.key[from - 1] != v;
+        const bool longer = begins ? list.piece < count - b && list.key[b + list.piece] == v : e - from == list.piece || list.key[e - 1 - list.piece] == v;
+        if (!longer) continue;
+        if (begins && tile == 0 && warp == 0) {
+            const int end = embed_below(list.key, to, count, v + 1, lane);
+            if (lane == 0) list.lists[atomicAdd(list.count + 1, 1)] = {v, piece * 2 + slot, (end - 1) / list.piece};
+        }
+        const int share = (e - b + EMBED_WARPS - 1) / EMBED_WARPS;
+        embed_zero(acc);
+        const int mine_to = min(b + (warp + 1) * share, e);
+        for (int i0 = b + warp * share; i0 < mine_to; i0 += 32) {
+            const int many = min(32, mine_to - i0), id = lane < many ? list.id[i0 + lane] : 0;
+            for (int j0 = 0; j0 < many; j0 += U) {
+                OpRaw<T, VEC> x[U][CH];
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
+                for (int u = 0; u < U; ++u) embed_load<T, VEC, CH>(x[u], dy, dy_stride, __shfl_sync(0xffffffffu, id, j0 + u), j0 + u < many, first, n);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[c][i] = 0.0f;
-        embed_add<T, VEC, CH>(acc, dy, dy_stride, list.id, min(b + warp * share, e), min(b + (warp + 1) * share, e), first, n, lane);
+                for (int u = 0; u < U; ++u) embed_add(acc, x[u]);
+            }
+        }
         __syncthreads();  // the sums of the slot before are read
 #pragma unroll
         for (int c = 0; c < CH; ++c)
@@ -298,8 +337,11 @@ struct EmbedBackward {
 template <typename T, typename O, int VEC, int CH>
 void embed_rows_go(const EmbedBackward& a) {
     const int tiles = (int)ceil_div64(a.n, 32 * VEC * CH);
-    const int64_t blocks = (int64_t)a.list.pieces * tiles + ceil_div64(a.rows * tiles, EMBED_WARPS);
-    op_launch_next(a.s, dim3((unsigned)blocks), dim3(EMBED_THREADS), 0, k_embed_rows<T, O, VEC, CH>, (const T*)a.dy, a.dys, a.list, a.rows, a.n, tiles, a.scale, (O*)a.out, a.os);
+    // several rows per warp where that leaves every SM's 32 warps a few turns: they share the search
+    const int64_t turns = a.rows * tiles / ((int64_t)sm_count() * 128);
+    const int per = (int)(turns < 1 ? 1 : turns > EMBED_ROWS ? EMBED_ROWS : turns);
+    const int64_t blocks = (int64_t)a.list.pieces * tiles + ceil_div64(ceil_div64(a.rows, per) * tiles, EMBED_WARPS);
+    op_launch_next(a.s, dim3((unsigned)blocks), dim3(EMBED_THREADS), 0, k_embed_rows<T, O, VEC, CH>, (const T*)a.dy, a.dys, a.list, a.rows, a.n, tiles, per, a.scale, (O*)a.out, a.os);
     if (a.list.pieces > 1) {
         const int columns = (int)ceil_div64(a.n, 32);
         const int64_t items = (int64_t)a.list.pieces * columns, most = 8 * (int64_t)sm_count();
@@ -308,12 +350,12 @@ void embed_rows_go(const EmbedBackward& a) {
 }
 template <typename T, typename O, int VEC>
 void embed_rows_pick(const EmbedBackward& a) {
-    // accesses per lane that leave the fewest lanes of the last tile without a column, more where equal
+    // up to sixteen columns a lane (more do not fit 64 registers with the rows on their way); three accesses where they leave no more lanes without a column than two
     const int units = (int)ceil_div64(a.n, 32 * VEC);
     if (units == 1) return embed_rows_go<T, O, VEC, 1>(a);
-    if (units == 2) return embed_rows_go<T, O, VEC, 2>(a);
-    if (units % 4 != 0 && units % 3 == 0) return embed_rows_go<T, O, VEC, 3>(a);
-    return embed_rows_go<T, O, VEC, 4>(a);
+    if constexpr (VEC < 8)
+        if (ceil_div(units, 3) * 3 <= ceil_div(units, 2) * 2) return embed_rows_go<T, O, VEC, 3>(a);
+    embed_rows_go<T, O, VEC, 2>(a);
 }
 template <typename T, int VEC>
 void embed_rows_type(const EmbedBackward& a, bool single, bool wide) {
@@ -402,9 +444,9 @@ extern "C" int tb_embedding_backward(const void* d_dy, int64_t dy_stride, int ty
     int *key = work + p.words, *id = key + p.list, *key2 = id + p.list, *id2 = key2 + p.list;
     const Tokens tokens = {d_tokens, token_bytes == 8, rows};
     const int mask = (1 << p.bits) - 1;
-    sort_launch(s, p.sort, FirstKey{tokens, mask}, count, work, FirstPut{tokens, key, id, total});
+    sort_launch(s, p.sort, FirstSource{tokens, mask}, count, work, FirstPut{key, id, total});
     for (int k = 1; k < p.passes; ++k) {
-        sort_launch(s, p.sort, NextKey{key, total, k * p.bits, mask}, count, work, NextPut{key, id, key2, id2});
+        sort_launch(s, p.sort, NextSource{key, total, k * p.bits, mask}, count, work, NextPut{id, key2, id2});
         std::swap(key, key2);
         std::swap(id, id2);
     }

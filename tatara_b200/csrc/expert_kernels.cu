@@ -15,14 +15,15 @@ namespace {
 
 #define EXPERT_MAX_K 16
 
-struct ExpertKey {
+struct ExpertSource {
     const int* index;
     __device__ __forceinline__ int operator()(int64_t i) const { return index[i]; }
+    __device__ __forceinline__ int key(int v) const { return v; }
 };
 struct ExpertPut {
     int *position, *source, *offsets;
     int64_t slots;
-    __device__ __forceinline__ void operator()(int64_t i, int place) const {
+    __device__ __forceinline__ void operator()(int64_t i, int, int place) const {
         position[i] = place;
         if (place >= 0) source[place] = (int)i;
     }
@@ -43,7 +44,7 @@ struct ExpertPut {
 // A row is n units U of memory: 16 bytes, or an element where rows do not start on 16-byte boundaries.  L lanes take CH units each of a row's tile.
 template <typename U, int L, int CH>
 __global__ void __launch_bounds__(EXPERT_THREADS)
-k_dispatch(const U* __restrict__ x, int64_t x_stride, int64_t rows, int n, int tiles, int k, const int* __restrict__ position, const int* __restrict__ source, U* __restrict__ out, int64_t out_stride,
+k_dispatch(const U* x, int64_t x_stride, int64_t rows, int n, int tiles, int k, const int* position, const int* source, U* __restrict__ out, int64_t out_stride,
            int64_t slots) {
     int64_t unit = (int64_t)blockIdx.x * (EXPERT_THREADS / L) + threadIdx.x / L;
     const int t = threadIdx.x % L;
@@ -76,7 +77,7 @@ k_dispatch(const U* __restrict__ x, int64_t x_stride, int64_t rows, int n, int t
 
 template <typename T, int VEC, int L, int CH>
 __global__ void __launch_bounds__(EXPERT_THREADS)
-k_combine(const T* __restrict__ y, int64_t y_stride, int64_t slots, int64_t rows, int n, int tiles, int k, const int* __restrict__ position, const float* __restrict__ gate, T* __restrict__ out,
+k_combine(const T* y, int64_t y_stride, int64_t slots, int64_t rows, int n, int tiles, int k, const int* position, const float* gate, T* __restrict__ out,
           int64_t out_stride) {
     constexpr int J = 4;  // choices whose rows are on their way together
     const int64_t unit = (int64_t)blockIdx.x * (EXPERT_THREADS / L) + threadIdx.x / L, row = unit / tiles;
@@ -124,8 +125,8 @@ k_combine(const T* __restrict__ y, int64_t y_stride, int64_t slots, int64_t rows
 // W warps (W = 1: L lanes) walk along a row; K >= k choices at once.
 template <typename T, int VEC, int W, int L, int K>
 __global__ void __launch_bounds__(EXPERT_THREADS)
-k_combine_backward(const T* __restrict__ dout, int64_t dout_stride, const T* __restrict__ y, int64_t y_stride, int64_t slots, int64_t rows, int n, int k, const int* __restrict__ position,
-                   const int* __restrict__ source, const float* __restrict__ gate, T* __restrict__ dy, int64_t dy_stride, float* __restrict__ dgate, int64_t row_blocks) {
+k_combine_backward(const T* dout, int64_t dout_stride, const T* y, int64_t y_stride, int64_t slots, int64_t rows, int n, int k, const int* position,
+                   const int* source, const float* gate, T* __restrict__ dy, int64_t dy_stride, float* __restrict__ dgate, int64_t row_blocks) {
     constexpr int LANES = W == 1 ? L : 32 * W, PER = EXPERT_THREADS / LANES;
     static_assert(W == 1 || 32 * W == EXPERT_THREADS, "a block per row");
     __shared__ float s_dot[K][W];
@@ -308,7 +309,7 @@ extern "C" int tb_expert_order(const int32_t* d_index, int64_t rows, int k, int 
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "the workspace must be aligned and hold %lld bytes (got %lld)", (long long)need, (long long)work_bytes);
     const OpRows ix = op_vector(d_index, rows * k), po = op_vector(d_position, rows * k), so = op_vector(d_source, slots), of = op_vector(d_offsets, experts + 1);
     if (op_meets(ix, {po, so, of}) || op_meets(po, {so, of}) || op_meets(so, {of})) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "a result overlaps another tensor");
-    sort_launch(static_cast<cudaStream_t>(stream), sort_plan(rows * k, experts, align), ExpertKey{d_index}, rows * k, static_cast<int*>(d_work), ExpertPut{d_position, d_source, d_offsets, slots});
+    sort_launch(static_cast<cudaStream_t>(stream), sort_plan(rows * k, experts, align), ExpertSource{d_index}, rows * k, static_cast<int*>(d_work), ExpertPut{d_position, d_source, d_offsets, slots});
     return op_launched(err, err_len);
 }
 

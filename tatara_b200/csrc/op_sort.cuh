@@ -3,10 +3,12 @@
 //   count of key e, begin_e = sum of the counts before it (each rounded up to a multiple of `align`), place of entry i = begin_key(i) + how many
 //   entries before i have its key.  Entries whose key is outside [0, E) have no place.
 //
-// A block of eight warps owns a piece of the entries, a warp an eighth of it.  First launch: the blocks' counts.  Last launch: every block adds up the counts
-// ahead of its own, its warps count their eighths again into shared memory, turn the counts into places and walk their eighths once more, 32 entries at a time
-// (a match over the warp's keys ranks them).  Where blocks times keys are many, a launch between the two adds the counts up once for all blocks; where all
-// entries fit a block, the last launch is the only one.  No atomics on global memory, places do not depend on timing.
+// A block of eight warps owns a piece of the entries, a warp an eighth of it, 32 entries a step.  First launch: the blocks' counts.  Last launch: the warps count
+// their eighths again into shared memory, every block adds up the counts ahead of its own, turns the counts into places, and its warps give every entry its own (votes over
+// the warp's keys rank 32 entries at once).  Where blocks times keys are many, a launch between the two adds the counts up once for all
+// blocks; where all entries fit a block, the last launch is the only one.  No atomics on global memory, places do not depend on timing.
+//
+// What bounds it is latency: an eighth's entries are loaded together (one step at a time cost a microsecond each) and stay in registers up to SORT_STEPS steps.
 #pragma once
 #include "op_common.cuh"
 
@@ -15,77 +17,131 @@ namespace {
 #define SORT_THREADS 256
 #define SORT_WARPS 8
 #define SORT_MAX_E 1024
+#define SORT_STEPS 8          // of a warp, whose entries are in registers together
 #define SORT_ONE 4096         // entries of a single block's sort
-#define SORT_SCAN 16384       // blocks * keys above which a launch of its own adds up the counts
+#define SORT_SCAN 8192        // blocks * keys above which a launch of its own adds up the counts
 
 struct SortPlan {
     int blocks, keys, align;
-    int64_t piece;            // entries per block
+    int bits;                 // of a key
+    int steps;                // of every warp; a block's piece is SORT_THREADS * steps entries
     bool scan;
 };
 inline SortPlan sort_plan(int64_t entries, int keys, int align) {
     SortPlan p;
     p.keys = keys;
     p.align = align;
-    if (entries <= SORT_ONE) p.blocks = 1, p.piece = (entries > 0 ? entries + SORT_THREADS - 1 : SORT_THREADS) / SORT_THREADS * SORT_THREADS, p.scan = false;
-    else {
-        // as many blocks as there are SMs, of 1024 entries or more; more keys make every block's tables dearer
-        const int64_t least = keys <= 64 ? 1024 : keys <= 512 ? 4096 : 8192, most = 2 * (int64_t)sm_count();
-        const int64_t want = (entries + least - 1) / least, b = want < most ? want : most;
-        p.piece = ((entries + b - 1) / b + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS;
-        p.blocks = (int)((entries + p.piece - 1) / p.piece);
-        p.scan = (int64_t)p.blocks * keys > SORT_SCAN;
-    }
+    for (p.bits = 0; 1 << p.bits < keys; ++p.bits) {}
+    // four steps up to a block per SM, then up to SORT_STEPS with more blocks, then longer pieces
+    const int64_t rows = (entries + SORT_THREADS - 1) / SORT_THREADS, sms = sm_count();
+    int64_t steps = rows <= 4 * sms ? 4 : rows <= 2 * SORT_STEPS * sms ? SORT_STEPS : (rows + 2 * sms - 1) / (2 * sms);
+    if (entries <= SORT_ONE) steps = rows < 1 ? 1 : rows;
+    p.steps = (int)steps;
+    p.blocks = entries <= SORT_ONE ? 1 : (int)((rows + steps - 1) / steps);
+    p.scan = p.blocks > 1 && (int64_t)p.blocks * keys > SORT_SCAN;
     return p;
 }
 // 32-bit words of workspace: the blocks' counts and, with a scan, the keys' counts
 inline int64_t sort_words(const SortPlan& p) { return p.blocks == 1 ? 0 : ((int64_t)p.blocks + (p.scan ? 1 : 0)) * p.keys; }
 
-// Walks the entries [from, to) of a warp, 32 at a time: f(entry, key or -1, lanes with the same key)
-template <typename Key, typename F>
-__device__ __forceinline__ void sort_walk(const Key& key, int keys, int64_t from, int64_t to, int lane, F f) {
-    for (int64_t i0 = from; i0 < to; i0 += 32) {
-        const int64_t i = i0 + lane;
-        int e = i < to ? key(i) : -1;
-        if ((unsigned)e >= (unsigned)keys) e = -1;
-        f(i, e, __match_any_sync(0xffffffffu, e));
+// The lanes whose key is this lane's, by a vote per bit: a third of the time of the match instruction for keys that differ
+__device__ __forceinline__ unsigned sort_peers(int e, int bits) {
+    unsigned peers = __ballot_sync(0xffffffffu, e >= 0);
+    if (e < 0) peers = ~peers;
+    for (int b = 0; b < bits; ++b) {
+        const unsigned set = __ballot_sync(0xffffffffu, e >> b & 1);
+        peers &= e >> b & 1 ? set : ~set;
     }
+    return peers;
 }
 
-template <typename Key>
-__global__ void __launch_bounds__(SORT_THREADS) k_sort_count(Key key, int64_t entries, SortPlan p, int* __restrict__ part) {
+// The entries of a warp, SORT_STEPS steps at a time.
+template <typename Source>
+struct SortWalk {
+    const Source& source;
+    int keys, steps, bits, lane;
+    int64_t first, entries;
+    int v[SORT_STEPS], rank[SORT_STEPS];
+    __device__ __forceinline__ SortWalk(const Source& src, int64_t n, const SortPlan& p)
+        : source(src), keys(p.keys), steps(p.steps), bits(p.bits), lane(threadIdx.x & 31),
+          first(((int64_t)blockIdx.x * SORT_WARPS + (threadIdx.x >> 5)) * p.steps * 32), entries(n) {}
+    __device__ __forceinline__ void load(int s0) {
+#pragma unroll
+        for (int s = 0; s < SORT_STEPS; ++s) {
+            const int64_t i = first + (int64_t)(s0 + s) * 32 + lane;
+            v[s] = -1;
+            if (s0 + s < steps && i < entries) v[s] = source(i);
+        }
+    }
+    __device__ __forceinline__ int key(int s) const {
+        const int e = source.key(v[s]);
+        return (unsigned)e < (unsigned)keys ? e : -1;
+    }
+    // count[key] += 1 for every entry, in order; rank: what the count was before it
+    __device__ __forceinline__ void add(int s0, int* count) {
+#pragma unroll
+        for (int s = 0; s < SORT_STEPS; ++s) {
+            if (s0 + s >= steps) break;
+            const int e = key(s);
+            const unsigned peers = sort_peers(e, bits);
+            const int leader = __ffs(peers) - 1;
+            int before = 0;
+            if (lane == leader && e >= 0) before = atomicAdd(&count[e], __popc(peers));
+            rank[s] = __shfl_sync(0xffffffffu, before, leader) + __popc(peers & ((1u << lane) - 1u));
+        }
+    }
+};
+
+template <typename Source>
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_count(Source source, int64_t entries, SortPlan p, int* __restrict__ part) {
     extern __shared__ int s_count[];
     op_next_may_start();
     for (int e = threadIdx.x; e < p.keys; e += SORT_THREADS) s_count[e] = 0;
     __syncthreads();
     op_wait_for_previous();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t first = (int64_t)blockIdx.x * p.piece + warp * (p.piece / SORT_WARPS), last = min(first + p.piece / SORT_WARPS, entries);
-    sort_walk(key, p.keys, first, last, lane, [&](int64_t, int e, unsigned peers) {
-        if (e >= 0 && lane == __ffs(peers) - 1) atomicAdd(&s_count[e], __popc(peers));
-    });
+    SortWalk<Source> w(source, entries, p);
+    for (int s0 = 0; s0 < p.steps; s0 += SORT_STEPS) {
+        w.load(s0);
+        w.add(s0, s_count);
+    }
     __syncthreads();
     for (int e = threadIdx.x; e < p.keys; e += SORT_THREADS) part[(int64_t)blockIdx.x * p.keys + e] = s_count[e];
 }
 
-// the counts of the blocks before each block, in place, and the keys' counts behind them; a warp per 32 keys, its lanes a key each
-__global__ void __launch_bounds__(32) k_sort_scan(SortPlan p, int* __restrict__ part) {
+// The counts of the blocks before each block, in place, and the keys' counts behind them.  A block per 32 keys, a lane per key, the warps a share of the blocks each.
+__global__ void __launch_bounds__(1024) k_sort_scan(SortPlan p, int* __restrict__ part) {
+    constexpr int U = 8;
+    __shared__ int s_sum[32][32];
     op_next_may_start();
     op_wait_for_previous();
-    const int e = blockIdx.x * 32 + threadIdx.x;
-    if (e >= p.keys) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
+    const int share = (p.blocks + 31) / 32, from = min(warp * share, p.blocks), to = min(from + share, p.blocks);
+    int* at = part + (int64_t)from * p.keys + e;
+    int sum = 0;
+    for (int b0 = 0; b0 < to - from; b0 += U) {
+        int c[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) c[i] = b0 + i < to - from && e < p.keys ? at[(int64_t)(b0 + i) * p.keys] : 0;
+#pragma unroll
+        for (int i = 0; i < U; ++i) sum += c[i];
+    }
+    s_sum[warp][lane] = sum;
+    __syncthreads();
     int run = 0;
-    for (int b0 = 0; b0 < p.blocks; b0 += 16) {
-        int c[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) c[i] = b0 + i < p.blocks ? part[(int64_t)(b0 + i) * p.keys + e] : 0;
+    for (int w = 0; w < 32; ++w) run += w < warp ? s_sum[w][lane] : 0;
+    if (e >= p.keys) return;
+    for (int b0 = 0; b0 < to - from; b0 += U) {
+        int c[U];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if (b0 + i < p.blocks) part[(int64_t)(b0 + i) * p.keys + e] = run;
+        for (int i = 0; i < U; ++i) c[i] = b0 + i < to - from ? at[(int64_t)(b0 + i) * p.keys] : 0;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (b0 + i < to - from) at[(int64_t)(b0 + i) * p.keys] = run;
             run += c[i];
         }
     }
-    part[(int64_t)p.blocks * p.keys + e] = run;
+    if (warp == 31) part[(int64_t)p.blocks * p.keys + e] = run;
 }
 
 // Where the experts begin from their counts, both [keys] in shared memory (s_begin[keys] too: the end), by all threads of the block
@@ -120,79 +176,94 @@ __device__ __forceinline__ void sort_begins(const int* s_total, int* s_begin, co
     __syncthreads();
 }
 
-// Key: entry -> key; Put: put(entry, place) for every entry (-1: no place), and put.rest(...) by every block with the begins in shared memory
-template <typename Key, typename Put>
-__global__ void __launch_bounds__(SORT_THREADS) k_sort_place(Key key, int64_t entries, SortPlan p, const int* __restrict__ part, Put put) {
+// Source: the value of an entry, and the key in a value; Put: put(entry, value, place) for every entry (-1: no place), and put.rest(counts, begins, plan) by every block
+template <typename Source, typename Put>
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_place(Source source, int64_t entries, SortPlan p, const int* part, Put put) {
     extern __shared__ int s_mem[];
-    int *s_total = s_mem, *s_begin = s_total + p.keys, *s_next = s_begin + p.keys + 1;  // s_next: [SORT_WARPS][keys]
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, keys = p.keys;
+    // s_total, s_ahead: a key's entries, those in the blocks before this one; s_next: [SORT_WARPS][keys]
+    int *s_total = s_mem, *s_ahead = s_total + p.keys, *s_begin = s_ahead + p.keys, *s_next = s_begin + p.keys + 1;
+    const int keys = p.keys;
     op_next_may_start();
+    for (int i = threadIdx.x; i < 2 * keys; i += SORT_THREADS) s_total[i] = 0;
     for (int i = threadIdx.x; i < SORT_WARPS * keys; i += SORT_THREADS) s_next[i] = 0;
-    __syncthreads();
     op_wait_for_previous();
-    const int64_t first = (int64_t)blockIdx.x * p.piece + warp * (p.piece / SORT_WARPS), last = min(first + p.piece / SORT_WARPS, entries);
-    int* next = s_next + warp * keys;
-    sort_walk(key, keys, first, last, lane, [&](int64_t, int e, unsigned peers) {
-        if (e >= 0 && lane == __ffs(peers) - 1) next[e] += __popc(peers);  // a warp's leaders have keys of their own
-        __syncwarp();
-    });
+    SortWalk<Source> w(source, entries, p);
+    w.load(0);
     __syncthreads();
-    // a key's places: its begin, the blocks before this one, the warps before this one
-    int ahead[SORT_MAX_E / SORT_THREADS];
-#pragma unroll
-    for (int i = 0; i < SORT_MAX_E / SORT_THREADS; ++i) {
-        const int e = threadIdx.x + i * SORT_THREADS;
-        ahead[i] = 0;
-        if (e >= keys) continue;
-        int total = 0;
-        if (p.blocks == 1) {
-            for (int w = 0; w < SORT_WARPS; ++w) total += s_next[w * keys + e];
-        } else if (p.scan) {
-            ahead[i] = part[(int64_t)blockIdx.x * keys + e];
-            total = part[(int64_t)p.blocks * keys + e];
-        } else {
+    int* next = s_next + (threadIdx.x >> 5) * keys;
+    if (p.blocks > 1 && p.scan) {
+        for (int e = threadIdx.x; e < keys; e += SORT_THREADS) {
+            s_ahead[e] = part[(int64_t)blockIdx.x * keys + e];
+            s_total[e] = part[(int64_t)p.blocks * keys + e];
+        }
+    } else if (p.blocks > 1) {
+        // keys side by side, the threads that are left share the blocks
+        int width = 32;
+        while (width < keys && width < SORT_THREADS) width *= 2;
+        for (int e = threadIdx.x % width; e < keys; e += width) {
+            const int step = SORT_THREADS / width;
+            int total = 0, ahead = 0;
 #pragma unroll 8
-            for (int b = 0; b < p.blocks; ++b) {
+            for (int b = threadIdx.x / width; b < p.blocks; b += step) {
                 const int c = part[(int64_t)b * keys + e];
                 total += c;
-                if (b < (int)blockIdx.x) ahead[i] += c;
+                if (b < (int)blockIdx.x) ahead += c;
             }
+            atomicAdd(&s_total[e], total);
+            atomicAdd(&s_ahead[e], ahead);
         }
-        s_total[e] = total;
+    }
+    w.add(0, next);
+    for (int s0 = SORT_STEPS; s0 < p.steps; s0 += SORT_STEPS) {
+        w.load(s0);
+        w.add(s0, next);
     }
     __syncthreads();
-    sort_begins(s_total, s_begin, p);
+    if (p.blocks == 1) {
+        for (int e = threadIdx.x; e < keys; e += SORT_THREADS) {
+            int total = 0;
 #pragma unroll
-    for (int i = 0; i < SORT_MAX_E / SORT_THREADS; ++i) {
-        const int e = threadIdx.x + i * SORT_THREADS;
-        if (e >= keys) continue;
-        int run = s_begin[e] + ahead[i];
-        for (int w = 0; w < SORT_WARPS; ++w) {
-            const int c = s_next[w * keys + e];
-            s_next[w * keys + e] = run;
+            for (int k = 0; k < SORT_WARPS; ++k) total += s_next[k * keys + e];
+            s_total[e] = total;
+        }
+        __syncthreads();
+    }
+    sort_begins(s_total, s_begin, p);
+    // a key's places: its begin, the blocks before this one, the warps before this one
+    for (int e = threadIdx.x; e < keys; e += SORT_THREADS) {
+        int run = s_begin[e] + s_ahead[e];
+#pragma unroll
+        for (int k = 0; k < SORT_WARPS; ++k) {
+            const int c = s_next[k * keys + e];
+            s_next[k * keys + e] = run;
             run += c;
         }
     }
     __syncthreads();
-    sort_walk(key, keys, first, last, lane, [&](int64_t i, int e, unsigned peers) {
-        int place = -1;
-        if (e >= 0) place = next[e] + __popc(peers & ((1u << lane) - 1u));
-        __syncwarp();
-        if (e >= 0 && lane == __ffs(peers) - 1) next[e] += __popc(peers);
-        __syncwarp();
-        if (i < last) put(i, place);
-    });
+    for (int s0 = 0; s0 < p.steps; s0 += SORT_STEPS) {
+        const bool again = p.steps > SORT_STEPS;  // counted on from the places themselves; otherwise the ranks are still there
+        if (again) {
+            w.load(s0);
+            w.add(s0, next);
+        }
+#pragma unroll
+        for (int s = 0; s < SORT_STEPS; ++s) {
+            const int64_t i = w.first + (int64_t)(s0 + s) * 32 + w.lane;
+            const int e = w.key(s);
+            if (s0 + s < p.steps && i < entries) put(i, w.v[s], e < 0 ? -1 : again ? w.rank[s] : next[e] + w.rank[s]);
+        }
+    }
     put.rest(s_total, s_begin, p);
 }
 
-template <typename Key, typename Put>
-void sort_launch(cudaStream_t s, const SortPlan& p, const Key& key, int64_t entries, int* work, const Put& put) {
+template <typename Source, typename Put>
+void sort_launch(cudaStream_t s, const SortPlan& p, const Source& source, int64_t entries, int* work, const Put& put) {
     if (p.blocks > 1) {
-        op_launch_next(s, dim3((unsigned)p.blocks), dim3(SORT_THREADS), (size_t)p.keys * 4, k_sort_count<Key>, key, entries, p, work);
-        if (p.scan) op_launch_next(s, dim3((unsigned)((p.keys + 31) / 32)), dim3(32), 0, k_sort_scan, p, work);
+        op_launch_next(s, dim3((unsigned)p.blocks), dim3(SORT_THREADS), (size_t)p.keys * 4, k_sort_count<Source>, source, entries, p, work);
+        if (p.scan) op_launch_next(s, dim3((unsigned)((p.keys + 31) / 32)), dim3(1024), 0, k_sort_scan, p, work);
     }
-    // at most 40 KB: 1024 keys of eight warps and two tables
-    op_launch_next(s, dim3((unsigned)p.blocks), dim3(SORT_THREADS), (size_t)((SORT_WARPS + 2) * p.keys + 1) * 4, k_sort_place<Key, Put>, key, entries, p, (const int*)work, put);
+    // at most 44 KB: 1024 keys of eight warps and three tables
+    op_launch_next(s, dim3((unsigned)p.blocks), dim3(SORT_THREADS), (size_t)((SORT_WARPS + 3) * p.keys + 1) * 4, k_sort_place<Source, Put>, source, entries, p, (const int*)work, put);
 }
 
 }  // namespace

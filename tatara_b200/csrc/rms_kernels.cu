@@ -20,32 +20,137 @@ namespace {
 #define RMS_LEAST 1.17549435e-38f  // 2^-126: the smallest scale
 
 // 1 / sqrt(mean of squares + eps) by `sum(f)`, the row's sum of (f h)^2 over its threads, the same in all of them; `any(c)`: whether c holds in a row that
-// shares the sums' barriers or shuffles.  Squares overflow above 2^63 and lose bits below 2^-75, which counts where eps is no larger.
+// shares the sums' barriers or shuffles.  Squares overflow above 2^63 and lose bits below 2^-75, which counts where eps is no larger.  `scale` is the f
+// that was taken, and what comes back is 1 / rms of f h: the row's own is f times that.
 template <typename Sum, typename Any>
-__device__ __forceinline__ float rms_rstd(int n, float eps, Sum sum, Any any) {
+__device__ __forceinline__ float rms_factor(int n, float eps, float& scale, Sum sum, Any any) {
     float ss = sum(1.0f), f = 1.0f;
     const bool large = ss > 8.5e37f, small = ss < 8e-25f && eps < 8e-31f;
     if (any(large || small)) {
         f = large ? 7.888609052e-31f : small ? 1.2676506002e30f : 1.0f;  // 2^-100, 2^100
         ss = sum(f);
     }
-    return f / sqrtf(ss / (float)n + eps * f * f);
+    scale = f;
+    return 1.0f / sqrtf(ss / (float)n + eps * f * f);
 }
 
-__device__ __forceinline__ unsigned rms_magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }  // ordered like |v|, NaN above all
-// the scale of a group from its largest magnitude; NaN stays NaN
-__device__ __forceinline__ float rms_scale(unsigned most) {
-    const float s = __uint_as_float(most) / RMS_MOST;
+// two fp32 operations at once
+__device__ __forceinline__ uint64_t rms_pair(float a, float b) { return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a); }
+template <int N>
+__device__ __forceinline__ void rms_multiply(float (&v)[N], const float (&w)[N]) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            uint64_t r;
+            asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(rms_pair(v[i], v[i + 1])), "l"(rms_pair(w[i], w[i + 1])));
+            v[i] = __uint_as_float((unsigned)r), v[i + 1] = __uint_as_float((unsigned)(r >> 32));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= w[i];
+    }
+}
+template <int N>
+__device__ __forceinline__ void rms_multiply(float (&v)[N], float by) {
+    float w[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = by;
+    rms_multiply<N>(v, w);
+}
+// the sum of squares of a thread's columns: two chains, the even and the odd ones
+template <int CH, int N>
+__device__ __forceinline__ float rms_squares(const float (&v)[CH][N]) {
+    if constexpr (N % 2 == 0) {
+        uint64_t sum = 0;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                const uint64_t p = rms_pair(v[c][i], v[c][i + 1]);
+                asm("fma.rn.f32x2 %0, %1, %1, %0;" : "+l"(sum) : "l"(p));
+            }
+        return __uint_as_float((unsigned)sum) + __uint_as_float((unsigned)(sum >> 32));
+    } else {
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum = fmaf(v[c][i], v[c][i], sum);
+        return sum;
+    }
+}
+// the largest magnitude; NaN if any is
+__device__ __forceinline__ float rms_larger(float a, float b, float c = 0.0f) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void rms_unpack(const OpRaw<T, N>& raw, float (&to)[N]) {
+    if constexpr (std::is_same<T, __half>::value && N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&raw.w[i / 2]));
+            to[i] = two.x, to[i + 1] = two.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) to[i] = raw.get(i);
+    }
+}
+// the scale of a group from its largest |y|; NaN stays NaN
+__device__ __forceinline__ float rms_scale(float most) {
+    const float s = most * (1.0f / RMS_MOST);
     return s < RMS_LEAST ? RMS_LEAST : s;
 }
+// Whether z of largest magnitude `most` may be multiplied with 448 / most for z r / s: to 2 ulp, where nothing leaves the range of that quotient and s is not the smallest scale.
+// (With divisions to the last bit for every group, 40000 x 1000 fp16 in groups of 128 took 40 us.)
+__device__ __forceinline__ bool rms_usual(float most, float r) { return most > 1e-30f && most < 1e30f && most * r > 1e-35f; }
 __device__ __forceinline__ uint8_t rms_q(float v) { return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
+// VEC numbers times `by` as adjacent bytes
+template <int VEC>
+__device__ __forceinline__ void rms_store_q(uint8_t* to, float (&v)[VEC], float by) {
+    rms_multiply<VEC>(v, by);
+    if constexpr (VEC == 1) {
+        *to = rms_q(v[0]);
+    } else {
+        OpVec<unsigned, VEC / 4> u;
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+            const unsigned low = __nv_cvt_float2_to_fp8x2(make_float2(v[i], v[i + 1]), __NV_SATFINITE, __NV_E4M3);
+            const unsigned high = __nv_cvt_float2_to_fp8x2(make_float2(v[i + 2], v[i + 3]), __NV_SATFINITE, __NV_E4M3);
+            u.v[i / 4] = low | high << 16;
+        }
+        *reinterpret_cast<OpVec<unsigned, VEC / 4>*>(to) = u;
+    }
+}
 
+// the largest of G lanes' magnitudes, whose bits are ordered like them with NaN above all
 template <int G>
-__device__ __forceinline__ unsigned rms_group_max(unsigned v) {
-    if constexpr (G == 32) return __reduce_max_sync(0xffffffffu, v);
+__device__ __forceinline__ float rms_group_max(float most) {
+    unsigned v = __float_as_uint(most);
+    if constexpr (G == 32) return __uint_as_float(__reduce_max_sync(0xffffffffu, v));
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+    return __uint_as_float(v);
+}
+
+// VEC columns of the weight in one access: 32 bytes of eight columns, as adjacent as the lanes are.  (Two of 16 bytes with gaps of 16 between the lanes cost four times the
+// wavefronts of the L1, more than all the rest of an 8-bit row: 40000 x 1000 fp16 37 us.)
+template <int VEC>
+__device__ __forceinline__ void rms_columns(const float* p, int col, float (&to)[VEC]) {
+    if constexpr (VEC == 8) {
+        if (p) {
+            asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                : "=f"(to[0]), "=f"(to[1]), "=f"(to[2]), "=f"(to[3]), "=f"(to[4]), "=f"(to[5]), "=f"(to[6]), "=f"(to[7])
+                : "l"(p + col));
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) to[i] = 1.0f;
+        }
+    } else {
+        norm_columns<VEC>(p, col, 1.0f, to);
+    }
 }
 
 struct RmsForward {
@@ -68,131 +173,157 @@ struct RmsForward {
 };
 
 // W warps per row, VEC adjacent columns per access, CH accesses per thread: a thread holds columns (c * LANES + t) * VEC + i.  With W = 1 a row has L lanes.
-// G: 0 for y of type T, 1 for 8 bits with a scale per row, else lanes that share a scale.
-template <typename T, int W, int L, int VEC, int CH, int G>
-__global__ void __launch_bounds__(W == 1 ? 128 : W * 32)
-k_rms_forward(const T* x, int64_t x_stride, const T* res, int64_t res_stride, const float* __restrict__ weight, float eps, int64_t rows, int n, void* y, int64_t y_stride,
+// G: 0 for y of type T, 1 for 8 bits with a scale per row, else lanes that share a scale.  FULL: accesses that are inside the row for every thread.  AHEAD: warps that walk down the rows, the next one's x on its way while they compute
+// (16-bit rows without a residual, where instructions take as long as the bytes); otherwise every group of lanes has one row.
+constexpr int rms_per_sm(int columns) { return columns <= 32 ? 7 : 5; }  // of blocks that walk down, by a thread's columns
+
+template <typename T, int W, int L, int VEC, int CH, int FULL, int G, bool AHEAD>
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, AHEAD ? rms_per_sm(CH * VEC) : 1)
+k_rms_forward(const T* x, int64_t x_stride, const T* res, int64_t res_stride, const float* weight, float eps, int64_t rows, int n, void* y, int64_t y_stride,
               T* h, int64_t h_stride, float* __restrict__ rstd_out, float* __restrict__ scale_out) {
     constexpr int LANES = W == 1 ? L : 32 * W, SUBS = W == 1 ? 32 / L : 1, RB = W == 1 ? 4 * SUBS : 1;  // rows per block
     __shared__ float s_sum[2][W];
-    __shared__ unsigned s_max[W];
+    __shared__ float s_max[W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = W == 1 ? lane % L : threadIdx.x;
-    const int64_t row = (int64_t)blockIdx.x * RB + (W == 1 ? warp * SUBS + lane / L : 0);
+    int64_t row = (int64_t)blockIdx.x * RB + (W == 1 ? warp * SUBS + lane / L : 0);
     op_next_may_start();
     if (L == 32 && row >= rows) return;  // by whole warps; lanes that share a warp stay for its sums
     const bool there = L == 32 || row < rows;
     OpRaw<T, VEC> xv[CH], rv[CH];
+    const auto load = [&](OpRaw<T, VEC>(&to)[CH], const T* from) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int col = (c * LANES + t) * VEC;
+            to[c].zero();
+            if (there && (c < FULL || col < n)) to[c].load(from + col);
+        }
+    };
     op_wait_for_previous();
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int col = (c * LANES + t) * VEC;
-        xv[c].zero();
-        if (there && col < n) xv[c].load(x + row * x_stride + col);
-    }
-    if (res) {
+    load(xv, x + row * x_stride);
+    do {
+        if (!AHEAD && res) load(rv, res + row * res_stride);
+        float v[CH][VEC];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int col = (c * LANES + t) * VEC;
-            rv[c].zero();
-            if (there && col < n) rv[c].load(res + row * res_stride + col);
+            rms_unpack(xv[c], v[c]);
+            if (!AHEAD && res) {
+                float u[VEC];
+                rms_unpack(rv[c], u);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) v[c][i] += u[i];
+            }
         }
-    }
-    float v[CH][VEC];
+        if (AHEAD && row + (int64_t)gridDim.x * RB < rows) load(xv, x + (row + (int64_t)gridDim.x * RB) * x_stride);
+        if (!AHEAD && h && there) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[c][i] = xv[c].get(i);
-        if (res) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v[c][i] += rv[c].get(i);
+            for (int c = 0; c < CH; ++c) {
+                const int col = (c * LANES + t) * VEC;
+                if (c < FULL || col < n) op_store<T, VEC>(h + row * h_stride + col, v[c]);
+            }
         }
-    }
-    int turn = 0;
-    const float rstd = rms_rstd(
-        n, eps,
-        [&](float f) {
-            float ss[1] = {0.0f};
+        int turn = 0;
+        float f;
+        const float r = rms_factor(
+            n, eps, f,
+            [&](float by) {
+                float ss[1];
+                if (turn) {  // the second sum: f h stays
 #pragma unroll
-            for (int c = 0; c < CH; ++c)
+                    for (int c = 0; c < CH; ++c) rms_multiply<VEC>(v[c], by);
+                }
+                ss[0] = rms_squares(v);
+                norm_rows_sum<W, L, 1>(ss, s_sum[turn++ & 1], warp, lane);
+                return ss[0];
+            },
+            [](bool c) { return W == 1 && L < 32 ? __any_sync(0xffffffffu, c) : c; });
+        if (t == 0 && there && rstd_out) rstd_out[row] = f * r;
+        if constexpr (G == 0) {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) ss[0] = fmaf(v[c][i] * f, v[c][i] * f, ss[0]);
-            norm_rows_sum<W, L, 1>(ss, s_sum[turn++ & 1], warp, lane);
-            return ss[0];
-        },
-        [](bool c) { return W == 1 && L < 32 ? __any_sync(0xffffffffu, c) : c; });
-    if (t == 0 && there && rstd_out) rstd_out[row] = rstd;
-    if (h && there) {
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int col = (c * LANES + t) * VEC;
-            if (col < n) op_store<T, VEC>(h + row * h_stride + col, v[c]);
-        }
-    }
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int col = (c * LANES + t) * VEC;
-        float w[VEC];
-        if (col < n) {
-            norm_columns<VEC>(weight, col, 1.0f, w);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v[c][i] = v[c][i] * rstd * w[i];
-            if (G == 0 && there) op_store<T, VEC>(static_cast<T*>(y) + row * y_stride + col, v[c]);
+            for (int c = 0; c < CH; ++c) {
+                const int col = (c * LANES + t) * VEC;
+                if (c >= FULL && col >= n) continue;
+                rms_multiply<VEC>(v[c], r);
+                if (weight) {
+                    float w[VEC];
+                    rms_columns<VEC>(weight, col, w);
+                    rms_multiply<VEC>(v[c], w);
+                }
+                if (there) op_store<T, VEC>(static_cast<T*>(y) + row * y_stride + col, v[c]);
+            }
         } else {
+            // z = f h * weight, y = z * r: one multiplication less for every column
+            if (weight) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[c][i] = 0.0f;
-        }
-    }
-    if constexpr (G == 0) return;
-    else {
-        unsigned most[CH];
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            most[c] = 0;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) most[c] = max(most[c], rms_magnitude(v[c][i]));
-        }
-        uint8_t* q = static_cast<uint8_t*>(y) + row * y_stride;
-        float s = 0.0f;
-        if constexpr (G == 1) {
-#pragma unroll
-            for (int c = 1; c < CH; ++c) most[0] = max(most[0], most[c]);
-            most[0] = rms_group_max<L>(most[0]);
-            if (W > 1) {
-                if (lane == 0) s_max[warp] = most[0];
-                __syncthreads();
-#pragma unroll
-                for (int w = 0; w < W; ++w) most[0] = max(most[0], s_max[w]);
+                for (int c = 0; c < CH; ++c) {
+                    const int col = (c * LANES + t) * VEC;
+                    if (c >= FULL && col >= n) continue;
+                    float w[VEC];
+                    rms_columns<VEC>(weight, col, w);
+                    rms_multiply<VEC>(v[c], w);
+                }
             }
-            s = rms_scale(most[0]);
-            if (t == 0 && there) scale_out[row] = s;
-        }
-        [[maybe_unused]] const int groups = G > 1 ? (n + G * VEC - 1) / (G * VEC) : 1;
+            float most[CH];  // columns that do not exist are zeros
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int col = (c * LANES + t) * VEC;
-            if constexpr (G > 1) {
-                s = rms_scale(rms_group_max<G>(most[c]));
-                if (there && col < n && t % G == 0) scale_out[row * groups + col / (G * VEC)] = s;
-            }
-            if (there && col < n) {
-                OpVec<uint8_t, VEC> u;
+            for (int c = 0; c < CH; ++c) {
+                most[c] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) u.v[i] = rms_q(v[c][i] / s);
-                *reinterpret_cast<OpVec<uint8_t, VEC>*>(q + col) = u;
+                for (int i = 0; i < VEC; i += 2) most[c] = rms_larger(most[c], v[c][i], VEC > 1 ? v[c][(i + 1) % VEC] : 0.0f);
+            }
+            uint8_t* q = static_cast<uint8_t*>(y) + row * y_stride;
+            const int groups = G > 1 ? (n + G * VEC - 1) / (G * VEC) : 1;
+            bool usual = true;
+            if constexpr (G == 1) {
+#pragma unroll
+                for (int c = 1; c < CH; ++c) most[0] = rms_larger(most[0], most[c]);
+                most[0] = rms_group_max<L>(most[0]);
+                if (W > 1) {
+                    if (lane == 0) s_max[warp] = most[0];
+                    __syncthreads();
+#pragma unroll
+                    for (int w = 0; w < W; ++w) most[0] = rms_larger(most[0], s_max[w]);
+                }
+                usual = rms_usual(most[0], r);
+                if (t == 0 && there) scale_out[row] = rms_scale(most[0] * r);
+            } else {
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int col = (c * LANES + t) * VEC;
+                    most[c] = rms_group_max<G>(most[c]);
+                    usual = usual && (rms_usual(most[c], r) || (c >= FULL && col >= n));
+                    if (there && (c < FULL || col < n) && t % G == 0) scale_out[row * groups + col / (G * VEC)] = rms_scale(most[c] * r);
+                }
+            }
+            if (__all_sync(0xffffffffu, usual || !there)) {
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int col = (c * LANES + t) * VEC;
+                    if (there && (c < FULL || col < n)) rms_store_q<VEC>(q + col, v[c], __fdividef(RMS_MOST, most[G == 1 ? 0 : c]));
+                }
+                continue;
+            }
+#pragma unroll 1
+            for (int c = 0; c < CH; ++c) {
+                const int col = (c * LANES + t) * VEC;
+#pragma unroll
+                for (int k = 0; k < CH; ++k) {
+                    if (k != c || !there || col >= n) continue;
+                    rms_multiply<VEC>(v[k], r);
+                    rms_store_q<VEC>(q + col, v[k], 1.0f / rms_scale(most[G == 1 ? 0 : k] * r));
+                }
             }
         }
-    }
+    } while (AHEAD && (row += (int64_t)gridDim.x * RB) < rows);
 }
 
 // Any row: a block per row that reads it again for every pass; thread t takes columns t, t + TH, ..  Rows longer than RMS_REG_N, and 8-bit rows that start anywhere.
 // C counts columns: int, or int64_t where the last step would go beyond 2^31.
 template <typename T, typename C, int TH>
 __global__ void __launch_bounds__(TH)
-k_rms_forward_long(const T* x, int64_t x_stride, const T* res, int64_t res_stride, const float* __restrict__ weight, float eps, int n, void* y, int64_t y_stride, T* h, int64_t h_stride,
+k_rms_forward_long(const T* x, int64_t x_stride, const T* res, int64_t res_stride, const float* weight, float eps, int n, void* y, int64_t y_stride, T* h, int64_t h_stride,
                    float* __restrict__ rstd_out, float* __restrict__ scale_out, int group) {
     constexpr int W = TH / 32;
     __shared__ float s_sum[2][W];
-    __shared__ unsigned s_max[W];
+    __shared__ float s_max[W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = blockIdx.x;
     const T *xr = x + row * x_stride, *rr = res + row * res_stride;
@@ -201,19 +332,20 @@ k_rms_forward_long(const T* x, int64_t x_stride, const T* res, int64_t res_strid
     op_wait_for_previous();
     const auto sum_at = [&](C c) { return res ? op_float(xr[c]) + op_float(rr[c]) : op_float(xr[c]); };
     int turn = 0;
-    const float rstd = rms_rstd(
-        n, eps,
-        [&](float f) {
+    float f;
+    const float r = rms_factor(
+        n, eps, f,
+        [&](float by) {
             float ss = 0.0f;
             for (C c = threadIdx.x; c < n; c += TH) {
-                const float v = sum_at(c) * f;
+                const float v = sum_at(c) * by;
                 ss = fmaf(v, v, ss);
             }
             return norm_row_sum<W>(ss, s_sum[turn++ & 1], warp, lane);
         },
         [](bool c) { return c; });
-    if (threadIdx.x == 0 && rstd_out) rstd_out[row] = rstd;
-    const auto y_at = [&](C c, float v) { return v * rstd * (weight ? weight[c] : 1.0f); };
+    if (threadIdx.x == 0 && rstd_out) rstd_out[row] = f * r;
+    const auto y_at = [&](C c, float v) { return v * f * r * (weight ? weight[c] : 1.0f); };
     if (group == 0) {
         T* yr = static_cast<T*>(y) + row * y_stride;
         for (C c = threadIdx.x; c < n; c += TH) {
@@ -225,19 +357,19 @@ k_rms_forward_long(const T* x, int64_t x_stride, const T* res, int64_t res_strid
     }
     uint8_t* q = static_cast<uint8_t*>(y) + row * y_stride;
     if (group >= n) {
-        unsigned most = 0;
-        for (C c = threadIdx.x; c < n; c += TH) most = max(most, rms_magnitude(y_at(c, sum_at(c))));
+        float most = 0.0f;
+        for (C c = threadIdx.x; c < n; c += TH) most = rms_larger(most, y_at(c, sum_at(c)));
         most = rms_group_max<32>(most);
         if (lane == 0) s_max[warp] = most;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < W; ++w) most = max(most, s_max[w]);
-        const float s = rms_scale(most);
+        for (int w = 0; w < W; ++w) most = rms_larger(most, s_max[w]);
+        const float s = rms_scale(most), inverse = 1.0f / s;
         if (threadIdx.x == 0) scale_out[row] = s;
         for (C c = threadIdx.x; c < n; c += TH) {
             const float v = sum_at(c);
             if (h) hr[c] = op_round<T>(v);
-            q[c] = rms_q(y_at(c, v) / s);
+            q[c] = rms_q(y_at(c, v) * inverse);
         }
         return;
     }
@@ -245,7 +377,7 @@ k_rms_forward_long(const T* x, int64_t x_stride, const T* res, int64_t res_strid
     const int groups = (int)(((C)n + group - 1) / group);
     for (int g = warp; g < groups; g += W) {
         float v[4];
-        unsigned most = 0;
+        float most = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const C c = (C)g * group + i * 32 + lane;
@@ -255,23 +387,28 @@ k_rms_forward_long(const T* x, int64_t x_stride, const T* res, int64_t res_strid
                 if (h) hr[c] = op_round<T>(u);
                 v[i] = y_at(c, u);
             }
-            most = max(most, rms_magnitude(v[i]));
+            most = rms_larger(most, v[i]);
         }
-        const float s = rms_scale(rms_group_max<32>(most));
+        const float s = rms_scale(rms_group_max<32>(most)), inverse = 1.0f / s;
         if (lane == 0) scale_out[row * groups + g] = s;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const C c = (C)g * group + i * 32 + lane;
-            if (i * 32 < group && c < n) q[c] = rms_q(v[i] / s);
+            if (i * 32 < group && c < n) q[c] = rms_q(v[i] * inverse);
         }
     }
 }
 
-template <typename T, int W, int L, int VEC, int CH, int G>
+template <typename T, int W, int L, int VEC, int CH, int FULL, int G>
 void rms_forward_go(const RmsForward& a) {
-    const int64_t per = W == 1 ? 128 / L : 1, blocks = (a.rows + per - 1) / per;
-    op_launch_next(a.s, dim3((unsigned)blocks), dim3(W == 1 ? 128 : W * 32), 0, k_rms_forward<T, W, L, VEC, CH, G>, (const T*)a.x, a.xs, (const T*)a.r, a.rs, a.w, a.eps, a.rows, a.n, a.y, a.ys, (T*)a.h,
-                   a.hs, a.rstd, a.scale);
+    const int64_t per = W == 1 ? 128 / L : 1, blocks = (a.rows + per - 1) / per, most = (int64_t)sm_count() * rms_per_sm(CH * VEC);
+#define RUN(AHEAD, BLOCKS)                                                                                                                                              \
+    op_launch_next(a.s, dim3((unsigned)(BLOCKS)), dim3(W == 1 ? 128 : W * 32), 0, k_rms_forward<T, W, L, VEC, CH, FULL, G, AHEAD>, (const T*)a.x, a.xs, (const T*)a.r, a.rs, a.w, a.eps, a.rows, a.n, a.y, \
+                   a.ys, (T*)a.h, a.hs, a.rstd, a.scale)
+    if constexpr (sizeof(T) == 2 && W == 1 && L == 32 && VEC > 1)
+        if (!a.r && blocks > most) return RUN(true, most);
+    RUN(false, blocks);
+#undef RUN
 }
 template <typename T>
 void rms_forward_any(const RmsForward& a) {
@@ -285,12 +422,13 @@ void rms_forward_any(const RmsForward& a) {
 }
 template <typename T, int VEC, int G>
 void rms_forward_pick(const RmsForward& a) {
-#define GO(W, L, K) \
-    if (a.n <= (W) * (K) * (L)) return rms_forward_go<T, W, L, VEC, ((K) + VEC - 1) / VEC, G>(a)
-    if constexpr (G <= 1 || G * VEC <= 32) GO(1, 8, 8);    // a group is shorter than the row
-    if constexpr (G <= 1 || G * VEC <= 64) GO(1, 16, 8);
-    GO(1, 32, 8); GO(1, 32, 16); GO(1, 32, 24); GO(1, 32, 32); GO(1, 32, 48);
-    GO(4, 32, 16); GO(4, 32, 32); GO(8, 32, 32); GO(16, 32, 32); GO(32, 32, 32);
+    // the rows over LO columns, up to W * K * L
+#define GO(LO, W, L, K) \
+    if (a.n <= (W) * (K) * (L)) return rms_forward_go<T, W, L, VEC, ((K) + VEC - 1) / VEC, (LO) / ((W) * (L) * VEC), G>(a)
+    if constexpr (G <= 1 || G * VEC <= 32) GO(0, 1, 8, 8);  // a group is shorter than the row
+    if constexpr (G <= 1 || G * VEC <= 64) GO(0, 1, 16, 8);
+    GO(0, 1, 32, 8); GO(256, 1, 32, 16); GO(512, 1, 32, 24); GO(768, 1, 32, 32); GO(1024, 1, 32, 48);
+    GO(1536, 4, 32, 16); GO(2048, 4, 32, 32); GO(4096, 8, 32, 32); GO(8192, 16, 32, 32); GO(16384, 32, 32, 32);
 #undef GO
     rms_forward_any<T>(a);
 }
@@ -310,7 +448,7 @@ constexpr int rms_per_sm_back(int warps) { return warps == 1 ? 4 : 24 / warps < 
 
 template <typename T, int W, int L, int VEC, int CH, int R>
 __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, rms_per_sm_back(W))
-k_rms_backward(const T* dy, int64_t dy_stride, const T* h, int64_t h_stride, const float* __restrict__ rstd, const float* __restrict__ weight, const T* dres, int64_t dres_stride, int64_t rows, int n,
+k_rms_backward(const T* dy, int64_t dy_stride, const T* h, int64_t h_stride, const float* rstd, const float* weight, const T* dres, int64_t dres_stride, int64_t rows, int n,
                T* dx, int64_t dx_stride, float* __restrict__ part_w) {
     constexpr int LANES = W == 1 ? L : 32 * W, SUBS = W == 1 ? 32 / L : 1, RB = W == 1 ? 4 * SUBS : 1;
     __shared__ float s_sum[2][R][W];
@@ -414,7 +552,7 @@ k_rms_backward(const T* dy, int64_t dy_stride, const T* h, int64_t h_stride, con
 // rows longer than RMS_REG_N_BACK: dx by a block per row, the columns' sums by threads that walk down stripes of rows
 template <typename T, typename C>
 __global__ void __launch_bounds__(1024)
-k_rms_backward_long(const T* dy, int64_t dy_stride, const T* h, int64_t h_stride, const float* __restrict__ rstd, const float* __restrict__ weight, const T* dres, int64_t dres_stride, int n, T* dx,
+k_rms_backward_long(const T* dy, int64_t dy_stride, const T* h, int64_t h_stride, const float* rstd, const float* weight, const T* dres, int64_t dres_stride, int n, T* dx,
                     int64_t dx_stride) {
     __shared__ float s_sum[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -432,7 +570,7 @@ k_rms_backward_long(const T* dy, int64_t dy_stride, const T* h, int64_t h_stride
 }
 template <typename T>
 __global__ void __launch_bounds__(256)
-k_rms_columns_long(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ h, int64_t h_stride, const float* __restrict__ rstd, int64_t rows, int n, float* __restrict__ part_w) {
+k_rms_columns_long(const T* dy, int64_t dy_stride, const T* h, int64_t h_stride, const float* rstd, int64_t rows, int n, float* __restrict__ part_w) {
     const unsigned at = blockIdx.x * 256 + threadIdx.x;  // may be beyond 2^31
     op_next_may_start();
     op_wait_for_previous();
@@ -531,7 +669,7 @@ int rms_forward_check(const RmsForward& a, int type, bool eight, char* err, size
 int rms_forward_run(const RmsForward& a, int type, char* err, size_t err_len) {
     const int size = op_type_size(type), vec = 16 / size;
     const bool out = a.group ? (uintptr_t)a.y % vec == 0 && a.ys % vec == 0 : norm_aligned(a.y, a.ys, size);
-    const bool wide = a.n % vec == 0 && norm_aligned(a.x, a.xs, size) && (!a.r || norm_aligned(a.r, a.rs, size)) && (!a.h || norm_aligned(a.h, a.hs, size)) && out && ((uintptr_t)a.w & 15) == 0;
+    const bool wide = a.n % vec == 0 && norm_aligned(a.x, a.xs, size) && (!a.r || norm_aligned(a.r, a.rs, size)) && (!a.h || norm_aligned(a.h, a.hs, size)) && out && (uintptr_t)a.w % (4 * vec) == 0;
     if (type == TB_TYPE_F32) rms_forward_type<float, 4>(a, wide);
     else if (type == TB_TYPE_F16) rms_forward_type<__half, 8>(a, wide);
     else rms_forward_type<__nv_bfloat16, 8>(a, wide);
