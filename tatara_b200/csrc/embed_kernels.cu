@@ -70,12 +70,22 @@ struct FirstSource {
     __device__ __forceinline__ int operator()(int64_t i) const { return tokens(i); }
     __device__ __forceinline__ int key(int v) const { return v < 0 ? -1 : v & mask; }
 };
+// counts for the sort by the next digits while the entries are placed: the blocks of that sort take `piece` places each.  (A launch of its own for it: 6 us.)
+struct NextCount {
+    int* part;  // NULL: none
+    int keys, piece, shift;
+    __device__ __forceinline__ void operator()(int v, int place) const {
+        if (part) atomicAdd(part + (int64_t)(place / piece) * keys + (v >> shift & (keys - 1)), 1);
+    }
+};
 struct FirstPut {
     int *key, *id, *count;  // count: of the tokens in the table, and (zero here) of the long lists
+    NextCount next;
     __device__ __forceinline__ void operator()(int64_t i, int v, int place) const {
         if (place < 0) return;
         key[place] = v;
         id[place] = (int)i;
+        next(v, place);
     }
     __device__ __forceinline__ void rest(const int*, const int* begin, const SortPlan& p) const {
         if (blockIdx.x == 0 && threadIdx.x == 0) count[0] = begin[p.keys], count[1] = 0;
@@ -94,10 +104,12 @@ struct NextSource {
 struct NextPut {
     const int* id_in;
     int *key, *id;
+    NextCount next;
     __device__ __forceinline__ void operator()(int64_t i, int v, int place) const {
         if (place < 0) return;
         key[place] = v;
         id[place] = id_in[i];
+        next(v, place);
     }
     __device__ __forceinline__ void rest(const int*, const int*, const SortPlan&) const {}
 };
@@ -265,7 +277,20 @@ k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n
     }
 }
 
-// The rows with long lists: a block adds up the pieces of a list for 32 columns, its warps a share of them each.
+// The rows with long lists, 32 columns at a time: a warp adds up a list's pieces, or a block's warps a share of them each where they are more than EMBED_ALONE.
+#define EMBED_ALONE 32
+template <int U>
+__device__ __forceinline__ float embed_pieces(const EmbedList& list, const EmbedLong& l, int from, int to, int col, int n) {
+    float sum = 0.0f;
+    for (int p0 = from; p0 < to; p0 += U) {
+        float t[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) t[i] = p0 + i < to && col < n ? list.part[(int64_t)(p0 + i == 0 ? l.first : (l.first / 2 + p0 + i) * 2) * n + col] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < U; ++i) sum += t[i];
+    }
+    return sum;
+}
 template <typename O>
 __global__ void __launch_bounds__(EMBED_THREADS)
 k_embed_join(EmbedList list, int n, int tiles, float scale, O* __restrict__ out, int64_t out_stride) {
@@ -274,22 +299,21 @@ k_embed_join(EmbedList list, int n, int tiles, float scale, O* __restrict__ out,
     op_next_may_start();
     op_wait_for_previous();
     const int64_t items = (int64_t)list.count[1] * tiles;
+    for (int64_t item = (int64_t)blockIdx.x * EMBED_WARPS + warp; item < items; item += (int64_t)gridDim.x * EMBED_WARPS) {
+        const EmbedLong l = list.lists[item / tiles];
+        const int col = (int)(item % tiles) * 32 + lane, sums = l.last - l.first / 2 + 1;
+        if (sums > EMBED_ALONE) continue;
+        const float sum = embed_pieces<8>(list, l, 0, sums, col, n);
+        if (col < n) out[(int64_t)l.token * out_stride + col] = op_round<O>(sum * scale);
+    }
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const EmbedLong l = list.lists[item / tiles];
-        const int col = (int)(item % tiles) * 32 + lane, piece = l.first / 2, sums = l.last - piece + 1, share = (sums + EMBED_WARPS - 1) / EMBED_WARPS;
-        const int to = min((warp + 1) * share, sums);
-        float sum = 0.0f;
-        for (int p0 = warp * share; p0 < to; p0 += 16) {
-            float t[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) t[i] = p0 + i < to && col < n ? list.part[(int64_t)(p0 + i == 0 ? l.first : (piece + p0 + i) * 2) * n + col] : 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sum += t[i];
-        }
-        s_part[warp][lane] = sum;
+        const int col = (int)(item % tiles) * 32 + lane, sums = l.last - l.first / 2 + 1, share = (sums + EMBED_WARPS - 1) / EMBED_WARPS;
+        if (sums <= EMBED_ALONE) continue;
+        s_part[warp][lane] = embed_pieces<16>(list, l, warp * share, min((warp + 1) * share, sums), col, n);
         __syncthreads();
         if (warp == 0 && col < n) {
-            sum = s_part[0][lane];
+            float sum = s_part[0][lane];
 #pragma unroll
             for (int w = 1; w < EMBED_WARPS; ++w) sum += s_part[w][lane];
             out[(int64_t)l.token * out_stride + col] = op_round<O>(sum * scale);
@@ -316,7 +340,7 @@ bool embed_plan(int64_t count, int64_t rows, int n, EmbedPlan* p) {
     p->piece = 32;
     while (count > (int64_t)p->piece * 2048) p->piece *= 2;
     p->pieces = (int)((count + p->piece - 1) / p->piece);
-    p->words = (sort_words(p->sort) + 2 + 7) / 8 * 8;
+    p->words = (p->passes * sort_words(p->sort) + 2 + 7) / 8 * 8;
     p->list = (count + 7) / 8 * 8;
     // what one launch takes; tensors that fit a GPU are far below
     return (p->pieces + rows / EMBED_WARPS + 2) * ceil_div64(n, 32) <= INT32_MAX;
@@ -444,9 +468,13 @@ extern "C" int tb_embedding_backward(const void* d_dy, int64_t dy_stride, int ty
     int *key = work + p.words, *id = key + p.list, *key2 = id + p.list, *id2 = key2 + p.list;
     const Tokens tokens = {d_tokens, token_bytes == 8, rows};
     const int mask = (1 << p.bits) - 1;
-    sort_launch(s, p.sort, FirstSource{tokens, mask}, count, work, FirstPut{key, id, total});
+    // the counts of the sort by digit k: [k] of as many tables
+    const int64_t table = sort_words(p.sort);
+    const auto next = [&](int k) { return NextCount{k < p.passes && table ? work + k * table : nullptr, p.sort.keys, SORT_THREADS * p.sort.steps, k * p.bits}; };
+    sort_count(s, p.sort, FirstSource{tokens, mask}, count, work, work + table, (p.passes - 1) * table);
+    sort_place(s, p.sort, FirstSource{tokens, mask}, count, work, FirstPut{key, id, total, next(1)});
     for (int k = 1; k < p.passes; ++k) {
-        sort_launch(s, p.sort, NextSource{key, total, k * p.bits, mask}, count, work, NextPut{id, key2, id2});
+        sort_place(s, p.sort, NextSource{key, total, k * p.bits, mask}, count, work + k * table, NextPut{id, key2, id2, next(k + 1)});
         std::swap(key, key2);
         std::swap(id, id2);
     }

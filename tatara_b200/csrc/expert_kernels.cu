@@ -309,7 +309,10 @@ extern "C" int tb_expert_order(const int32_t* d_index, int64_t rows, int k, int 
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "the workspace must be aligned and hold %lld bytes (got %lld)", (long long)need, (long long)work_bytes);
     const OpRows ix = op_vector(d_index, rows * k), po = op_vector(d_position, rows * k), so = op_vector(d_source, slots), of = op_vector(d_offsets, experts + 1);
     if (op_meets(ix, {po, so, of}) || op_meets(po, {so, of}) || op_meets(so, {of})) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "a result overlaps another tensor");
-    sort_launch(static_cast<cudaStream_t>(stream), sort_plan(rows * k, experts, align), ExpertSource{d_index}, rows * k, static_cast<int*>(d_work), ExpertPut{d_position, d_source, d_offsets, slots});
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const SortPlan plan = sort_plan(rows * k, experts, align);
+    sort_count(s, plan, ExpertSource{d_index}, rows * k, static_cast<int*>(d_work));
+    sort_place(s, plan, ExpertSource{d_index}, rows * k, static_cast<int*>(d_work), ExpertPut{d_position, d_source, d_offsets, slots});
     return op_launched(err, err_len);
 }
 

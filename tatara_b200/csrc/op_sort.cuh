@@ -44,30 +44,19 @@ inline SortPlan sort_plan(int64_t entries, int keys, int align) {
 // 32-bit words of workspace: the blocks' counts and, with a scan, the keys' counts
 inline int64_t sort_words(const SortPlan& p) { return p.blocks == 1 ? 0 : ((int64_t)p.blocks + (p.scan ? 1 : 0)) * p.keys; }
 
-// The lanes whose key is this lane's, by a vote per bit: a third of the time of the match instruction for keys that differ
-__device__ __forceinline__ unsigned sort_peers(int e, int bits) {
-    unsigned peers = __ballot_sync(0xffffffffu, e >= 0);
-    if (e < 0) peers = ~peers;
-    for (int b = 0; b < bits; ++b) {
-        const unsigned set = __ballot_sync(0xffffffffu, e >> b & 1);
-        peers &= e >> b & 1 ? set : ~set;
-    }
-    return peers;
-}
-
-// The entries of a warp, SORT_STEPS steps at a time.
-template <typename Source>
+// The entries of a warp, S steps at a time.
+template <typename Source, int S>
 struct SortWalk {
     const Source& source;
     int keys, steps, bits, lane;
     int64_t first, entries;
-    int v[SORT_STEPS], rank[SORT_STEPS];
+    int v[S], rank[S];
     __device__ __forceinline__ SortWalk(const Source& src, int64_t n, const SortPlan& p)
         : source(src), keys(p.keys), steps(p.steps), bits(p.bits), lane(threadIdx.x & 31),
           first(((int64_t)blockIdx.x * SORT_WARPS + (threadIdx.x >> 5)) * p.steps * 32), entries(n) {}
     __device__ __forceinline__ void load(int s0) {
 #pragma unroll
-        for (int s = 0; s < SORT_STEPS; ++s) {
+        for (int s = 0; s < S; ++s) {
             const int64_t i = first + (int64_t)(s0 + s) * 32 + lane;
             v[s] = -1;
             if (s0 + s < steps && i < entries) v[s] = source(i);
@@ -77,33 +66,51 @@ struct SortWalk {
         const int e = source.key(v[s]);
         return (unsigned)e < (unsigned)keys ? e : -1;
     }
-    // count[key] += 1 for every entry, in order; rank: what the count was before it
-    __device__ __forceinline__ void add(int s0, int* count) {
+    // count[key] += 1 for every entry, in order; rank: what the count was before it.  The lanes with the same key are found by a vote per bit, all steps side by side (the match
+    // instruction takes three times as long where keys differ).
+    __device__ __forceinline__ void add(int* count) {
+        unsigned peers[S];
+        int before[S];
 #pragma unroll
-        for (int s = 0; s < SORT_STEPS; ++s) {
-            if (s0 + s >= steps) break;
-            const int e = key(s);
-            const unsigned peers = sort_peers(e, bits);
-            const int leader = __ffs(peers) - 1;
-            int before = 0;
-            if (lane == leader && e >= 0) before = atomicAdd(&count[e], __popc(peers));
-            rank[s] = __shfl_sync(0xffffffffu, before, leader) + __popc(peers & ((1u << lane) - 1u));
+        for (int s = 0; s < S; ++s) {
+            const unsigned any = __ballot_sync(0xffffffffu, key(s) >= 0);
+            peers[s] = key(s) >= 0 ? any : ~any;
         }
+        for (int b = 0; b < bits; ++b)
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                const bool one = key(s) >> b & 1;
+                const unsigned set = __ballot_sync(0xffffffffu, one);
+                peers[s] &= one ? set : ~set;
+            }
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            before[s] = 0;
+            if (lane == __ffs(peers[s]) - 1 && key(s) >= 0) before[s] = atomicAdd(&count[key(s)], __popc(peers[s]));
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s) rank[s] = __shfl_sync(0xffffffffu, before[s], __ffs(peers[s]) - 1) + __popc(peers[s] & ((1u << lane) - 1u));
     }
 };
 
-template <typename Source>
-__global__ void __launch_bounds__(SORT_THREADS) k_sort_count(Source source, int64_t entries, SortPlan p, int* __restrict__ part) {
+// zero: further words to be set to zero, for whoever counts into them later
+template <typename Source, int S>
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_count(Source source, int64_t entries, SortPlan p, int* __restrict__ part, int* __restrict__ zero, int64_t zeros) {
     extern __shared__ int s_count[];
     op_next_may_start();
     for (int e = threadIdx.x; e < p.keys; e += SORT_THREADS) s_count[e] = 0;
     __syncthreads();
     op_wait_for_previous();
-    SortWalk<Source> w(source, entries, p);
-    for (int s0 = 0; s0 < p.steps; s0 += SORT_STEPS) {
+    SortWalk<Source, S> w(source, entries, p);
+    for (int s0 = 0; s0 < p.steps; s0 += S) {
         w.load(s0);
-        w.add(s0, s_count);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int e = w.key(s);
+            if (e >= 0) atomicAdd(&s_count[e], 1);
+        }
     }
+    for (int64_t i = (int64_t)blockIdx.x * SORT_THREADS + threadIdx.x; i < zeros; i += (int64_t)gridDim.x * SORT_THREADS) zero[i] = 0;
     __syncthreads();
     for (int e = threadIdx.x; e < p.keys; e += SORT_THREADS) part[(int64_t)blockIdx.x * p.keys + e] = s_count[e];
 }
@@ -177,7 +184,7 @@ __device__ __forceinline__ void sort_begins(const int* s_total, int* s_begin, co
 }
 
 // Source: the value of an entry, and the key in a value; Put: put(entry, value, place) for every entry (-1: no place), and put.rest(counts, begins, plan) by every block
-template <typename Source, typename Put>
+template <typename Source, typename Put, int S>
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_place(Source source, int64_t entries, SortPlan p, const int* part, Put put) {
     extern __shared__ int s_mem[];
     // s_total, s_ahead: a key's entries, those in the blocks before this one; s_next: [SORT_WARPS][keys]
@@ -187,7 +194,7 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_place(Source source, int6
     for (int i = threadIdx.x; i < 2 * keys; i += SORT_THREADS) s_total[i] = 0;
     for (int i = threadIdx.x; i < SORT_WARPS * keys; i += SORT_THREADS) s_next[i] = 0;
     op_wait_for_previous();
-    SortWalk<Source> w(source, entries, p);
+    SortWalk<Source, S> w(source, entries, p);
     w.load(0);
     __syncthreads();
     int* next = s_next + (threadIdx.x >> 5) * keys;
@@ -213,10 +220,10 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_place(Source source, int6
             atomicAdd(&s_ahead[e], ahead);
         }
     }
-    w.add(0, next);
-    for (int s0 = SORT_STEPS; s0 < p.steps; s0 += SORT_STEPS) {
+    w.add(next);
+    for (int s0 = S; s0 < p.steps; s0 += S) {
         w.load(s0);
-        w.add(s0, next);
+        w.add(next);
     }
     __syncthreads();
     if (p.blocks == 1) {
@@ -240,14 +247,14 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_place(Source source, int6
         }
     }
     __syncthreads();
-    for (int s0 = 0; s0 < p.steps; s0 += SORT_STEPS) {
-        const bool again = p.steps > SORT_STEPS;  // counted on from the places themselves; otherwise the ranks are still there
+    for (int s0 = 0; s0 < p.steps; s0 += S) {
+        const bool again = p.steps > S;  // counted on from the places themselves; otherwise the ranks are still there
         if (again) {
             w.load(s0);
-            w.add(s0, next);
+            w.add(next);
         }
 #pragma unroll
-        for (int s = 0; s < SORT_STEPS; ++s) {
+        for (int s = 0; s < S; ++s) {
             const int64_t i = w.first + (int64_t)(s0 + s) * 32 + w.lane;
             const int e = w.key(s);
             if (s0 + s < p.steps && i < entries) put(i, w.v[s], e < 0 ? -1 : again ? w.rank[s] : next[e] + w.rank[s]);
@@ -256,14 +263,18 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_place(Source source, int6
     put.rest(s_total, s_begin, p);
 }
 
+// The launches of a sort: the blocks' counts into `part` (unless a sort before has counted them), then their sums and the places.
+template <typename Source>
+void sort_count(cudaStream_t s, const SortPlan& p, const Source& source, int64_t entries, int* part, int* zero = nullptr, int64_t zeros = 0) {
+    if (p.blocks > 1)
+        op_launch_next(s, dim3((unsigned)p.blocks), dim3(SORT_THREADS), (size_t)p.keys * 4, p.steps <= 4 ? k_sort_count<Source, 4> : k_sort_count<Source, SORT_STEPS>, source, entries, p, part, zero, zeros);
+}
 template <typename Source, typename Put>
-void sort_launch(cudaStream_t s, const SortPlan& p, const Source& source, int64_t entries, int* work, const Put& put) {
-    if (p.blocks > 1) {
-        op_launch_next(s, dim3((unsigned)p.blocks), dim3(SORT_THREADS), (size_t)p.keys * 4, k_sort_count<Source>, source, entries, p, work);
-        if (p.scan) op_launch_next(s, dim3((unsigned)((p.keys + 31) / 32)), dim3(1024), 0, k_sort_scan, p, work);
-    }
+void sort_place(cudaStream_t s, const SortPlan& p, const Source& source, int64_t entries, int* part, const Put& put) {
+    if (p.scan) op_launch_next(s, dim3((unsigned)((p.keys + 31) / 32)), dim3(1024), 0, k_sort_scan, p, part);
     // at most 44 KB: 1024 keys of eight warps and three tables
-    op_launch_next(s, dim3((unsigned)p.blocks), dim3(SORT_THREADS), (size_t)((SORT_WARPS + 3) * p.keys + 1) * 4, k_sort_place<Source, Put>, source, entries, p, (const int*)work, put);
+    op_launch_next(s, dim3((unsigned)p.blocks), dim3(SORT_THREADS), (size_t)((SORT_WARPS + 3) * p.keys + 1) * 4, p.steps <= 4 ? k_sort_place<Source, Put, 4> : k_sort_place<Source, Put, SORT_STEPS>, source, entries,
+                   p, (const int*)part, put);
 }
 
 }  // namespace
