@@ -6,17 +6,19 @@
 // A token outside the table has a row of zeros and no gradient.  Both are bound by memory.  Backward, the tokens are sorted (op_sort.cuh, a stable sort by up
 // to ten bits at a time), so that a row's tokens lie together in ascending order.  A warp takes a table row: it finds its tokens in the sorted list
 // and adds their rows in registers.  Where that would be a long chain (more than `piece` tokens: a few tokens make up much of any text or board), the list's
-// pieces of that many tokens are added up by blocks of their own in the same launch, and a further launch adds up the pieces.  Sums are fp32 in an order that depends
+// pieces of that many tokens are added up by blocks of their own in the same launch, the last of which adds up the pieces.  Sums are fp32 in an order that depends
 // on the tokens alone, so results repeat bit for bit.
+#include "op_bulk.cuh"
 #include "op_sort.cuh"
 
+#include <atomic>
 #include <utility>
 
 namespace {
 
-#define EMBED_THREADS 256
-#define EMBED_WARPS 8
-#define EMBED_ROWS 8  // table rows per warp at most
+#define EMBED_THREADS 128
+#define EMBED_WARPS 4
+#define EMBED_ROWS 16  // table rows per warp at most
 
 struct Tokens {
     const void* p;
@@ -24,7 +26,9 @@ struct Tokens {
     int64_t rows;
     // -1 where the table has no such row
     __device__ __forceinline__ int operator()(int64_t i) const {
-        const int64_t t = wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int*>(p)[i];
+        int64_t t;
+        if (wide) t = static_cast<const int64_t*>(p)[i];
+        else t = static_cast<const int*>(p)[i];
         return t >= 0 && t < rows ? (int)t : -1;
     }
 };
@@ -79,7 +83,9 @@ struct NextCount {
     }
 };
 struct FirstPut {
-    int *key, *id, *count;  // count: of the tokens in the table, and (zero here) of the long lists
+    int *key, *id, *count;  // count: of the tokens in the table
+    int* zero;              // set to zero by a single block; by the launch that counts where there are more
+    int64_t zeros;
     NextCount next;
     __device__ __forceinline__ void operator()(int64_t i, int v, int place) const {
         if (place < 0) return;
@@ -88,7 +94,8 @@ struct FirstPut {
         next(v, place);
     }
     __device__ __forceinline__ void rest(const int*, const int* begin, const SortPlan& p) const {
-        if (blockIdx.x == 0 && threadIdx.x == 0) count[0] = begin[p.keys], count[1] = 0;
+        if (blockIdx.x == 0 && threadIdx.x == 0) *count = begin[p.keys];
+        for (int64_t i = threadIdx.x; gridDim.x == 1 && i < zeros; i += SORT_THREADS) zero[i] = 0;
     }
 };
 // further digits, of what the digits before have sorted
@@ -138,22 +145,6 @@ __device__ __forceinline__ void embed_store(O* p, const float (&from)[VEC]) {
     }
 }
 
-template <typename T, int VEC, int CH>
-__device__ __forceinline__ void embed_load(OpRaw<T, VEC> (&x)[CH], const T* dy, int64_t dy_stride, int row, bool there, int first, int n) {
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int col = first + c * 32 * VEC;
-        x[c].zero();
-        if (there && col < n) x[c].load(dy + row * dy_stride + col);
-    }
-}
-template <typename T, int VEC, int CH>
-__device__ __forceinline__ void embed_add(float (&acc)[CH][VEC], const OpRaw<T, VEC> (&x)[CH]) {
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[c][i] += x[c].get(i);
-}
 template <int VEC, int CH>
 __device__ __forceinline__ void embed_zero(float (&acc)[CH][VEC]) {
 #pragma unroll
@@ -162,64 +153,148 @@ __device__ __forceinline__ void embed_zero(float (&acc)[CH][VEC]) {
         for (int i = 0; i < VEC; ++i) acc[c][i] = 0.0f;
 }
 
-struct EmbedLong {       // a token whose list is longer than a piece: its first sum, and the list's last piece
-    int token, first, last;
-};
 struct EmbedList {
-    const int *key, *id;
-    int* count;          // of the tokens in the table, and of the long lists
-    int piece, pieces;   // tokens to a piece, and how many pieces there can be
-    EmbedLong* lists;    // the long ones in any order
-    float* part;         // [pieces][2][n]: the sums of a piece's first and of its last token, where those have long lists
+    const int *key, *id, *count;   // count: of the tokens in the table
+    int piece, pieces, together;   // tokens to a piece, how many pieces there can be, and how many of them a block looks at
+    float* part;                   // [pieces][2][n]: the sums of a piece's first and of its last token, where those have long lists
+    int* done;                     // [pieces][2][tiles]: how many of a list's sums are there, counted at its first one; zero at the start
 };
 
-// Blocks below pieces * tiles: a piece of the list and a tile of columns.  The others: `per` table rows and a tile per warp; it looks for the first row's place in the
+// acc += sums that other blocks have written
+template <int VEC>
+__device__ __forceinline__ void embed_add_sums(float (&acc)[VEC], const float* from) {
+    if constexpr (VEC == 1) {
+        acc[0] += __ldcg(from);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(from + i));
+            acc[i] += v.x, acc[i + 1] += v.y, acc[i + 2] += v.z, acc[i + 3] += v.w;
+        }
+    }
+}
+
+// How a warp gets the rows of a window of the list, `here` of them by the lanes' ids: f(j) for each in order, with its columns added to acc on the way.
+//
+// Rows on 16-byte boundaries come by asynchronous copies, several on their way for every warp whatever the lists' lengths, without registers.
+template <typename T, int VEC, int CH, int K>
+struct EmbedCopies {
+    static constexpr int TILE = 32 * VEC * CH, SLOT = TILE * (int)sizeof(T), SMEM = EMBED_WARPS * K * SLOT;
+    static_assert(SMEM >= EMBED_WARPS * TILE * 4 || K * sizeof(T) >= 4, "the warps' sums lie in the same memory");
+    BulkRing<K, SLOT> ring;
+    unsigned char* memory;
+    const T* dy;
+    int64_t stride;
+    unsigned bytes;
+    __device__ __forceinline__ EmbedCopies(unsigned char* smem, uint64_t* bars, const T* rows, int64_t row_stride, int column, int n)
+        : ring(smem + (threadIdx.x >> 5) * K * SLOT, bars + (threadIdx.x >> 5) * K), memory(smem + (threadIdx.x >> 5) * K * SLOT), dy(rows + column), stride(row_stride),
+          bytes((unsigned)(min(TILE, n - column) * (int)sizeof(T))) {}
+    template <typename F>
+    __device__ __forceinline__ void add(float (&acc)[CH][VEC], int id, int here, F f) {
+        const int lane = threadIdx.x & 31;
+        int sent = 0;
+        for (int j = 0; j < here; ++j) {
+            for (; sent < here && sent < j + K; ++sent) ring.put(dy + __shfl_sync(0xffffffffu, id, sent) * stride, bytes);
+            f(j);
+            const T* x = reinterpret_cast<const T*>(memory + ring.take() * SLOT) + lane * VEC;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                OpRaw<T, VEC> v;
+                v.load(x + c * 32 * VEC);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) acc[c][i] += v.get(i);
+            }
+            __syncwarp();
+        }
+    }
+    // of all sums from here on: NaN after a wait that has run out
+    __device__ __forceinline__ float factor() const { return ring.ok ? 1.0f : __int_as_float(0x7fc00000); }
+    __device__ __forceinline__ void end() { ring.end(); }
+};
+// Rows that start anywhere come through registers, an element at a time.
+template <typename T, int VEC, int CH, int K>
+struct EmbedLoads {
+    static constexpr int SMEM = 0;
+    const T* dy;
+    int64_t stride;
+    int n;
+    __device__ __forceinline__ EmbedLoads(unsigned char*, uint64_t*, const T* rows, int64_t row_stride, int column, int columns) : dy(rows + column), stride(row_stride), n(columns - column) {}
+    template <typename F>
+    __device__ __forceinline__ void add(float (&acc)[CH][VEC], int id, int here, F f) {
+        const int lane = threadIdx.x & 31;
+        for (int j0 = 0; j0 < here; j0 += K) {
+            OpRaw<T, VEC> x[K][CH];
+#pragma unroll
+            for (int u = 0; u < K; ++u) {
+                const int64_t row = __shfl_sync(0xffffffffu, id, j0 + u);
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int col = (c * 32 + lane) * VEC;
+                    x[u][c].zero();
+                    if (j0 + u < here && col < n) x[u][c].load(dy + row * stride + col);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < K; ++u) {
+                if (j0 + u >= here) break;
+                f(j0 + u);
+#pragma unroll
+                for (int c = 0; c < CH; ++c)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) acc[c][i] += x[u][c].get(i);
+            }
+        }
+    }
+    __device__ __forceinline__ float factor() const { return 1.0f; }
+    __device__ __forceinline__ void end() {}
+};
+
+// The first blocks: `together` pieces of the list and a tile of columns.  The others: `per` table rows and a tile per warp; it looks for the first row's place in the
 // list once and reads on from there, 32 entries at a time.
-template <typename T, typename O, int VEC, int CH>
+template <typename T, typename O, int VEC, int CH, int K, template <typename, int, int, int> class Rows>
 __global__ void __launch_bounds__(EMBED_THREADS, 4)
 k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n, int tiles, int per, float scale, O* __restrict__ out, int64_t out_stride) {
-    constexpr int TILE = 32 * VEC * CH, U = CH == 1 ? 8 : CH == 2 ? 4 : 2;  // rows on their way together
-    __shared__ float s_part[EMBED_WARPS][TILE];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, piece_blocks = list.pieces * tiles;
+    using From = Rows<T, VEC, CH, K>;
+    constexpr int TILE = 32 * VEC * CH;
+    extern __shared__ __align__(128) unsigned char s_rows[];
+    __shared__ uint64_t s_bars[EMBED_WARPS * K];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, piece_blocks = (list.pieces + list.together - 1) / list.together * tiles;
     op_next_may_start();
+    const bool piece_block = (int64_t)blockIdx.x < piece_blocks;
+    const int64_t unit = piece_block ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x - piece_blocks) * EMBED_WARPS + warp, group = unit / tiles;
+    const int column = (int)(unit - group * tiles) * TILE, first = column + lane * VEC;
+    __shared__ float s_few[From::SMEM ? 1 : EMBED_WARPS * TILE];
+    From from_rows(s_rows, s_bars, dy, dy_stride, column, n);
     op_wait_for_previous();
     const int count = *list.count;
     float acc[CH][VEC];
-    if ((int64_t)blockIdx.x >= piece_blocks) {
-        const int64_t unit = ((int64_t)blockIdx.x - piece_blocks) * EMBED_WARPS + warp, group = unit / tiles, row0 = group * per;
+    embed_zero(acc);
+    if (!piece_block) {
+        const int64_t row0 = group * per;
         if (row0 >= rows) return;
-        const int first = ((int)(unit - group * tiles) * 32 * CH + lane) * VEC, many = (int)min((int64_t)per, rows - row0);
-        const int end_row = (int)row0 + many;
+        const int end_row = (int)min(row0 + per, rows);
         const auto store = [&](int64_t v) {
+            const float by = scale * from_rows.factor();
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int col = first + c * 32 * VEC;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) acc[c][i] *= scale;
+                for (int i = 0; i < VEC; ++i) acc[c][i] *= by;
                 if (col < n) embed_store<O, VEC>(out + v * out_stride + col, acc[c]);
             }
             embed_zero(acc);
         };
         int v = (int)row0, last = -1;  // acc is v's; the key before the window
-        embed_zero(acc);
         for (int at = embed_below(list.key, 0, count, v, lane);;) {
             const int key = lane < count - at ? list.key[at + lane] : INT32_MAX, id = lane < count - at ? list.id[at + lane] : 0;
             const int ahead = list.piece < count - at - lane ? list.key[at + list.piece + lane] : -1, before = __shfl_up_sync(0xffffffffu, key, 1);
             // up to the window's first list that is longer than a piece, which is added up by pieces
             const unsigned longer = __ballot_sync(0xffffffffu, ahead == key && key != (lane ? before : last) && key < end_row);
             const int mine = __popc(__ballot_sync(0xffffffffu, key < end_row)), here = longer ? __ffs(longer) - 1 : mine;
-            for (int j0 = 0; j0 < here; j0 += U) {
-                OpRaw<T, VEC> x[U][CH];
-#pragma unroll
-                for (int u = 0; u < U; ++u) embed_load<T, VEC, CH>(x[u], dy, dy_stride, __shfl_sync(0xffffffffu, id, j0 + u), j0 + u < here, first, n);
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int k = __shfl_sync(0xffffffffu, key, j0 + u);
-                    if (j0 + u >= here) break;
-                    for (; v < k; ++v) store(v);
-                    embed_add(acc, x[u]);
-                }
-            }
+            from_rows.add(acc, id, here, [&](int j) {
+                const int k = __shfl_sync(0xffffffffu, key, j);
+                for (; v < k; ++v) store(v);
+            });
             if (longer) {
                 last = __shfl_sync(0xffffffffu, key, here);
                 for (; v < last; ++v) store(v);
@@ -232,105 +307,164 @@ k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n
             }
         }
         for (; v < end_row; ++v) store(v);
+        from_rows.end();
         return;
     }
-    const int piece = blockIdx.x / tiles, tile = blockIdx.x - piece * tiles, first = (tile * 32 * CH + lane) * VEC;
-    if ((int64_t)piece * list.piece >= count) return;
-    const int from = piece * list.piece, to = list.piece < count - from ? from + list.piece : count, first_key = list.key[from], last_key = list.key[to - 1];
-    for (int slot = 0; slot < (first_key == last_key ? 1 : 2); ++slot) {
-        // the token's entries of this piece, and whether the list is longer than a piece
-        const int v = slot ? last_key : first_key;
-        const int b = slot ? embed_below(list.key, from, to, v, lane) : from, e = slot || last_key == v ? to : embed_below(list.key, from, to, v + 1, lane);
-        const bool begins = slot || from == 0 || list.key[from - 1] != v;
-        const bool longer = begins ? list.piece < count - b && list.key[b + list.piece] == v : e - from == list.piece || list.key[e - 1 - list.piece] == v;
-        if (!longer) continue;
-        if (begins && tile == 0 && warp == 0) {
-            const int end = embed_below(list.key, to, count, v + 1, lane);
-            if (lane == 0) list.lists[atomicAdd(list.count + 1, 1)] = {v, piece * 2 + slot, (end - 1) / list.piece};
+    // Every warp looks at a piece: its first and its last token, and whether their lists are longer than a piece.
+    struct Sum {
+        int token, from, to, first, last;  // the token's entries in this piece, the list's first sum and its last piece
+    };
+    __shared__ Sum s_sums[EMBED_WARPS][2];
+    __shared__ bool s_last;
+    const int piece = (int)group * list.together + warp;
+    if (lane == 0) s_sums[warp][0].token = s_sums[warp][1].token = -1;
+    if (warp < list.together && (int64_t)piece * list.piece < count) {
+        const int from = piece * list.piece, to = list.piece < count - from ? from + list.piece : count, first_key = list.key[from], last_key = list.key[to - 1];
+        for (int slot = 0; slot < (first_key == last_key ? 1 : 2); ++slot) {
+            const int v = slot ? last_key : first_key;
+            const int b = slot ? embed_below(list.key, from, to, v, lane) : from, e = slot || last_key == v ? to : embed_below(list.key, from, to, v + 1, lane);
+            const bool begins = slot || from == 0 || list.key[from - 1] != v;
+            const bool longer = begins ? list.piece < count - b && list.key[b + list.piece] == v : e - from == list.piece || list.key[e - 1 - list.piece] == v;
+            if (!longer) continue;
+            const int begin = begins ? b : embed_below(list.key, 0, from, v, lane), end = e < to ? e : embed_below(list.key, to, count, v + 1, lane);
+            // a list that begins inside a piece is that piece's last one
+            if (lane == 0) s_sums[warp][slot] = {v, b, e, begin / list.piece * 2 + (begin % list.piece ? 1 : 0), (end - 1) / list.piece};
         }
-        const int share = (e - b + EMBED_WARPS - 1) / EMBED_WARPS;
-        embed_zero(acc);
-        const int mine_to = min(b + (warp + 1) * share, e);
-        for (int i0 = b + warp * share; i0 < mine_to; i0 += 32) {
-            const int many = min(32, mine_to - i0), id = lane < many ? list.id[i0 + lane] : 0;
-            for (int j0 = 0; j0 < many; j0 += U) {
-                OpRaw<T, VEC> x[U][CH];
-#pragma unroll
-                for (int u = 0; u < U; ++u) embed_load<T, VEC, CH>(x[u], dy, dy_stride, __shfl_sync(0xffffffffu, id, j0 + u), j0 + u < many, first, n);
-#pragma unroll
-                for (int u = 0; u < U; ++u) embed_add(acc, x[u]);
-            }
-        }
-        __syncthreads();  // the sums of the slot before are read
+    }
+    __syncthreads();
+    float* s_part = From::SMEM ? reinterpret_cast<float*>(s_rows) : s_few;
+    // the warps' sums of their columns, added up in order: column at of the tile
+    const auto share_out = [&](auto put) {
+        __syncthreads();
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) s_part[warp][(c * VEC + i) * 32 + lane] = acc[c][i];
+            for (int i = 0; i < VEC; ++i) s_part[warp * TILE + (c * VEC + i) * 32 + lane] = acc[c][i];
         __syncthreads();
         for (int at = threadIdx.x; at < TILE; at += EMBED_THREADS) {
-            float sum = s_part[0][at];
+            float sum = s_part[at];
 #pragma unroll
-            for (int w = 1; w < EMBED_WARPS; ++w) sum += s_part[w][at];
-            const int col = ((tile * CH + at / 32 / VEC) * 32 + at % 32) * VEC + at / 32 % VEC;
-            if (col < n) list.part[((int64_t)piece * 2 + slot) * n + col] = sum;
+            for (int w = 1; w < EMBED_WARPS; ++w) sum += s_part[w * TILE + at];
+            const int col = column + (at / 32 / VEC * 32 + at % 32) * VEC + at / 32 % VEC;
+            if (col < n) put(col, sum);
         }
+    };
+    for (int which = 0; which < 2 * list.together; ++which) {
+        const Sum sum = s_sums[which / 2][which % 2];
+        if (sum.token < 0) continue;
+        const int64_t number = 2 * (group * list.together + which / 2) + which % 2;
+        const int share = (sum.to - sum.from + EMBED_WARPS - 1) / EMBED_WARPS, mine_to = min(sum.from + (warp + 1) * share, sum.to);
+        embed_zero(acc);
+        for (int i0 = sum.from + warp * share; i0 < mine_to; i0 += 32) {
+            const int many = min(32, mine_to - i0), id = lane < many ? list.id[i0 + lane] : 0;
+            from_rows.add(acc, id, many, [](int) {});
+        }
+        const float by = from_rows.factor();
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[c][i] *= by;
+        share_out([&](int col, float x) { list.part[number * n + col] = x; });
+        // who writes the list's last sum adds them all up
+        __threadfence();
+        __syncthreads();
+        const int sums = sum.last - sum.first / 2 + 1;
+        if (threadIdx.x == 0) s_last = atomicAdd(list.done + (int64_t)sum.first * tiles + column / TILE, 1) == sums - 1;
+        __syncthreads();
+        if (s_last) {
+            __threadfence();
+            embed_zero(acc);
+            const int mine = (sums + EMBED_WARPS - 1) / EMBED_WARPS, to = min((warp + 1) * mine, sums);
+#pragma unroll 4
+            for (int k = warp * mine; k < to; ++k) {
+                const float* from = list.part + (int64_t)(k == 0 ? sum.first : (sum.first / 2 + k) * 2) * n;
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int col = first + c * 32 * VEC;
+                    if (col < n) embed_add_sums<VEC>(acc[c], from + col);
+                }
+            }
+            share_out([&](int col, float x) { out[(int64_t)sum.token * out_stride + col] = op_round<O>(x * scale); });
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // copies may follow
+        __syncthreads();
     }
+    from_rows.end();
 }
 
-// The rows with long lists, 32 columns at a time: a warp adds up a list's pieces, or a block's warps a share of them each where they are more than EMBED_ALONE.
-#define EMBED_ALONE 32
-template <int U>
-__device__ __forceinline__ float embed_pieces(const EmbedList& list, const EmbedLong& l, int from, int to, int col, int n) {
-    float sum = 0.0f;
-    for (int p0 = from; p0 < to; p0 += U) {
-        float t[U];
-#pragma unroll
-        for (int i = 0; i < U; ++i) t[i] = p0 + i < to && col < n ? list.part[(int64_t)(p0 + i == 0 ? l.first : (l.first / 2 + p0 + i) * 2) * n + col] : 0.0f;
-#pragma unroll
-        for (int i = 0; i < U; ++i) sum += t[i];
-    }
-    return sum;
-}
-template <typename O>
-__global__ void __launch_bounds__(EMBED_THREADS)
-k_embed_join(EmbedList list, int n, int tiles, float scale, O* __restrict__ out, int64_t out_stride) {
-    __shared__ float s_part[EMBED_WARPS][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Few tokens and a small table: a block per table row and tile looks through all tokens for its own, in order, and its warps take a share of them each.  One launch and
+// no workspace; 1000 tokens, 81 x 256 fp32: 3.7 us, by the sort 12 to 14.
+#define EMBED_FEW 1024
+#define EMBED_FEW_WARPS 8
+template <typename T, typename O, int VEC>
+__global__ void __launch_bounds__(EMBED_FEW_WARPS * 32)
+k_embed_few(Tokens tokens, int count, const T* dy, int64_t dy_stride, int n, int tiles, float scale, O* __restrict__ out, int64_t out_stride) {
+    constexpr int TILE = 32 * VEC, STEPS = EMBED_FEW / EMBED_FEW_WARPS / 32;
+    __shared__ float s_part[EMBED_FEW_WARPS * TILE];
+    __shared__ int s_id[EMBED_FEW], s_many[EMBED_FEW_WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x / tiles, column = (int)(blockIdx.x - row * tiles) * TILE;
     op_next_may_start();
+    // through registers, the copies' latency is longer
+    EmbedLoads<T, VEC, 1, 8> from_rows(nullptr, nullptr, dy, dy_stride, column, n);
     op_wait_for_previous();
-    const int64_t items = (int64_t)list.count[1] * tiles;
-    for (int64_t item = (int64_t)blockIdx.x * EMBED_WARPS + warp; item < items; item += (int64_t)gridDim.x * EMBED_WARPS) {
-        const EmbedLong l = list.lists[item / tiles];
-        const int col = (int)(item % tiles) * 32 + lane, sums = l.last - l.first / 2 + 1;
-        if (sums > EMBED_ALONE) continue;
-        const float sum = embed_pieces<8>(list, l, 0, sums, col, n);
-        if (col < n) out[(int64_t)l.token * out_stride + col] = op_round<O>(sum * scale);
-    }
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const EmbedLong l = list.lists[item / tiles];
-        const int col = (int)(item % tiles) * 32 + lane, sums = l.last - l.first / 2 + 1, share = (sums + EMBED_WARPS - 1) / EMBED_WARPS;
-        if (sums <= EMBED_ALONE) continue;
-        s_part[warp][lane] = embed_pieces<16>(list, l, warp * share, min((warp + 1) * share, sums), col, n);
-        __syncthreads();
-        if (warp == 0 && col < n) {
-            float sum = s_part[0][lane];
+    int token[STEPS];  // on their way together
 #pragma unroll
-            for (int w = 1; w < EMBED_WARPS; ++w) sum += s_part[w][lane];
-            out[(int64_t)l.token * out_stride + col] = op_round<O>(sum * scale);
-        }
-        __syncthreads();
+    for (int s = 0; s < STEPS; ++s) {
+        const int i = (warp * STEPS + s) * 32 + lane;
+        token[s] = tokens(min(i, count - 1));
+        if (i >= count) token[s] = -1;
+    }
+    unsigned found[STEPS];
+    int many = 0;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        found[s] = __ballot_sync(0xffffffffu, token[s] == row);
+        many += __popc(found[s]);
+    }
+    if (lane == 0) s_many[warp] = many;
+    __syncthreads();
+    int at = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < EMBED_FEW_WARPS; ++w) {
+        at += w < warp ? s_many[w] : 0;
+        all += s_many[w];
+    }
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        if (found[s] >> lane & 1) s_id[at + __popc(found[s] & ((1u << lane) - 1u))] = (warp * STEPS + s) * 32 + lane;
+        at += __popc(found[s]);
+    }
+    __syncthreads();
+    float acc[1][VEC];
+    embed_zero(acc);
+    const int share = (all + EMBED_FEW_WARPS - 1) / EMBED_FEW_WARPS, to = min((warp + 1) * share, all);
+    for (int i0 = warp * share; i0 < to; i0 += 32) {
+        const int here = min(32, to - i0), id = lane < here ? s_id[i0 + lane] : 0;
+        from_rows.add(acc, id, here, [](int) {});
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s_part[warp * TILE + lane * VEC + i] = acc[0][i];
+    __syncthreads();
+    for (int k = threadIdx.x; k < TILE; k += EMBED_FEW_WARPS * 32) {
+        float sum = s_part[k];
+#pragma unroll
+        for (int w = 1; w < EMBED_FEW_WARPS; ++w) sum += s_part[w * TILE + k];
+        if (column + k < n) out[(int64_t)row * out_stride + column + k] = op_round<O>(sum * scale);
     }
 }
 
 // ---- plans -------------------------------------------------------------------------------------------------------------------
 struct EmbedPlan {
+    bool few;            // no sort
     int passes, bits;    // of the sort
     SortPlan sort;
     int piece, pieces;
-    int64_t words, list; // 32-bit ones of the sort's workspace and the counts, of each sorted list; then the long lists and the pieces' sums
+    int64_t tables, done, words, list; // 32-bit ones of the sorts' counts, of the counted sums, of both and the count; of each sorted list, behind which the pieces' sums lie
 };
 bool embed_plan(int64_t count, int64_t rows, int n, EmbedPlan* p) {
     if (count < 0 || count > OP_MAX_ENTRIES || rows < 1 || rows > INT32_MAX || n < 1 || n > OP_MAX_COLUMNS) return false;
+    // every row's blocks look through all tokens: as long as that is less than the sort's launches
+    p->few = count > 0 && count <= EMBED_FEW && rows * ceil_div64(n, 128) <= 16 * (int64_t)sm_count();
     int bits = 1;
     while (((int64_t)1 << bits) < rows) ++bits;
     p->passes = (bits + 9) / 10;
@@ -340,16 +474,23 @@ bool embed_plan(int64_t count, int64_t rows, int n, EmbedPlan* p) {
     p->piece = 32;
     while (count > (int64_t)p->piece * 2048) p->piece *= 2;
     p->pieces = (int)((count + p->piece - 1) / p->piece);
-    p->words = (p->passes * sort_words(p->sort) + 2 + 7) / 8 * 8;
     p->list = (count + 7) / 8 * 8;
     // what one launch takes; tensors that fit a GPU are far below
-    return (p->pieces + rows / EMBED_WARPS + 2) * ceil_div64(n, 32) <= INT32_MAX;
+    const int64_t tiles = ceil_div64(n, 32);
+    if ((p->pieces + rows / EMBED_WARPS + 2) * tiles > INT32_MAX) return false;
+    // the tables of counts, those of the sums that are there, the count of tokens
+    p->tables = p->passes * sort_words(p->sort);
+    p->done = (int64_t)p->pieces * 2 * tiles;
+    p->words = (p->tables + p->done + 1 + 7) / 8 * 8;
+    return true;
 }
-int64_t embed_lists(const EmbedPlan& p) { return ((int64_t)p.pieces * 3 + 7) / 8 * 8; }
-int64_t embed_bytes(const EmbedPlan& p, int n) { return 4 * (p.words + (p.passes > 1 ? 4 : 2) * p.list + embed_lists(p) + (int64_t)p.pieces * 2 * n); }
+int64_t embed_bytes(const EmbedPlan& p, int n) { return p.few ? 0 : 4 * (p.words + (p.passes > 1 ? 4 : 2) * p.list + (int64_t)p.pieces * 2 * n); }
 
 struct EmbedBackward {
     cudaStream_t s;
+    Tokens tokens;
+    int64_t count;
+    bool few;
     const void* dy;
     int64_t dys, rows;
     int n;
@@ -358,28 +499,42 @@ struct EmbedBackward {
     int64_t os;
     EmbedList list;
 };
-template <typename T, typename O, int VEC, int CH>
+template <typename T, typename O, int VEC, int CH, int K, template <typename, int, int, int> class Rows>
 void embed_rows_go(const EmbedBackward& a) {
+    constexpr int SMEM = Rows<T, VEC, CH, K>::SMEM;
     const int tiles = (int)ceil_div64(a.n, 32 * VEC * CH);
-    // several rows per warp where that leaves every SM's 32 warps a few turns: they share the search
-    const int64_t turns = a.rows * tiles / ((int64_t)sm_count() * 128);
-    const int per = (int)(turns < 1 ? 1 : turns > EMBED_ROWS ? EMBED_ROWS : turns);
-    const int64_t blocks = (int64_t)a.list.pieces * tiles + ceil_div64(ceil_div64(a.rows, per) * tiles, EMBED_WARPS);
-    op_launch_next(a.s, dim3((unsigned)blocks), dim3(EMBED_THREADS), 0, k_embed_rows<T, O, VEC, CH>, (const T*)a.dy, a.dys, a.list, a.rows, a.n, tiles, per, a.scale, (O*)a.out, a.os);
-    if (a.list.pieces > 1) {
-        const int columns = (int)ceil_div64(a.n, 32);
-        const int64_t items = (int64_t)a.list.pieces * columns, most = 8 * (int64_t)sm_count();
-        op_launch_next(a.s, dim3((unsigned)(items < most ? items : most)), dim3(EMBED_THREADS), 0, k_embed_join<O>, a.list, a.n, columns, a.scale, (O*)a.out, a.os);
+    const auto kernel = k_embed_rows<T, O, VEC, CH, K, Rows>;
+    if (SMEM > 40 * 1024) {
+        static std::atomic<uint64_t> known{0};
+        op_allow_smem(kernel, SMEM, known);
     }
+    // several rows per warp where that leaves every SM's warps a few turns: they share the search
+    const int64_t turns = a.rows * tiles / ((int64_t)sm_count() * 64);
+    const int per = (int)(turns < 1 ? 1 : turns > EMBED_ROWS ? EMBED_ROWS : turns);
+    // pieces together where they are more than a few blocks per SM: most of them have no long list
+    EmbedList list = a.list;
+    const int64_t many = (int64_t)list.pieces * tiles / (2 * sm_count());
+    list.together = (int)(many < 1 ? 1 : many > EMBED_WARPS ? EMBED_WARPS : many);
+    const int64_t blocks = ceil_div64(list.pieces, list.together) * tiles + ceil_div64(ceil_div64(a.rows, per) * tiles, EMBED_WARPS);
+    op_launch_next(a.s, dim3((unsigned)blocks), dim3(EMBED_THREADS), SMEM, kernel, (const T*)a.dy, a.dys, list, a.rows, a.n, tiles, per, a.scale, (O*)a.out, a.os);
 }
 template <typename T, typename O, int VEC>
 void embed_rows_pick(const EmbedBackward& a) {
-    // up to sixteen columns a lane (more do not fit 64 registers with the rows on their way); three accesses where they leave no more lanes without a column than two
     const int units = (int)ceil_div64(a.n, 32 * VEC);
-    if (units == 1) return embed_rows_go<T, O, VEC, 1>(a);
-    if constexpr (VEC < 8)
-        if (ceil_div(units, 3) * 3 <= ceil_div(units, 2) * 2) return embed_rows_go<T, O, VEC, 3>(a);
-    embed_rows_go<T, O, VEC, 2>(a);
+    if (a.few) {
+        op_launch_next(a.s, dim3((unsigned)(a.rows * units)), dim3(EMBED_FEW_WARPS * 32), 0, k_embed_few<T, O, VEC>, a.tokens, (int)a.count, (const T*)a.dy, a.dys, a.n, units, a.scale, (O*)a.out, a.os);
+        return;
+    }
+    if constexpr (VEC == 1) {
+        if (units == 1) return embed_rows_go<T, O, 1, 1, 8, EmbedLoads>(a);
+        embed_rows_go<T, O, 1, 4, 4, EmbedLoads>(a);
+    } else {
+        // the whole row up to 3 KB, tiles of 2 KB above; as many copies per warp as leave an SM sixteen warps
+        if (units == 1) return embed_rows_go<T, O, VEC, 1, 8, EmbedCopies>(a);
+        if (units == 2) return embed_rows_go<T, O, VEC, 2, 8, EmbedCopies>(a);
+        if (units == 5 || units == 6) return embed_rows_go<T, O, VEC, 6, 4, EmbedCopies>(a);
+        embed_rows_go<T, O, VEC, 4, 4, EmbedCopies>(a);
+    }
 }
 template <typename T, int VEC>
 void embed_rows_type(const EmbedBackward& a, bool single, bool wide) {
@@ -461,26 +616,28 @@ extern "C" int tb_embedding_backward(const void* d_dy, int64_t dy_stride, int ty
     EmbedPlan p;
     if (!embed_plan(count, rows, n, &p)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "rows times columns are too many for one launch");
     const int64_t need = embed_bytes(p, n);
-    if (!d_work || work_bytes < need || ((uintptr_t)d_work & 31))
+    if (need > 0 && (!d_work || work_bytes < need || ((uintptr_t)d_work & 31)))
         return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "the workspace must be aligned and hold %lld bytes (got %lld)", (long long)need, (long long)work_bytes);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    int *work = static_cast<int*>(d_work), *total = work + p.words - 2;
-    int *key = work + p.words, *id = key + p.list, *key2 = id + p.list, *id2 = key2 + p.list;
     const Tokens tokens = {d_tokens, token_bytes == 8, rows};
-    const int mask = (1 << p.bits) - 1;
-    // the counts of the sort by digit k: [k] of as many tables
-    const int64_t table = sort_words(p.sort);
-    const auto next = [&](int k) { return NextCount{k < p.passes && table ? work + k * table : nullptr, p.sort.keys, SORT_THREADS * p.sort.steps, k * p.bits}; };
-    sort_count(s, p.sort, FirstSource{tokens, mask}, count, work, work + table, (p.passes - 1) * table);
-    sort_place(s, p.sort, FirstSource{tokens, mask}, count, work, FirstPut{key, id, total, next(1)});
-    for (int k = 1; k < p.passes; ++k) {
-        sort_place(s, p.sort, NextSource{key, total, k * p.bits, mask}, count, work + k * table, NextPut{id, key2, id2, next(k + 1)});
-        std::swap(key, key2);
-        std::swap(id, id2);
+    int *work = static_cast<int*>(d_work), *total = work + p.words - 1;
+    int *key = work + p.words, *id = key + p.list, *key2 = id + p.list, *id2 = key2 + p.list;
+    if (!p.few) {
+        const int mask = (1 << p.bits) - 1;
+        // the counts of the sort by digit k: [k] of as many tables
+        const int64_t table = sort_words(p.sort), zeros = p.tables - table + p.done;
+        const auto next = [&](int k) { return NextCount{k < p.passes && table ? work + k * table : nullptr, p.sort.keys, SORT_THREADS * p.sort.steps, k * p.bits}; };
+        sort_count(s, p.sort, FirstSource{tokens, mask}, count, work, work + table, zeros);
+        sort_place(s, p.sort, FirstSource{tokens, mask}, count, work, FirstPut{key, id, total, work + table, zeros, next(1)});
+        for (int k = 1; k < p.passes; ++k) {
+            sort_place(s, p.sort, NextSource{key, total, k * p.bits, mask}, count, work + k * table, NextPut{id, key2, id2, next(k + 1)});
+            std::swap(key, key2);
+            std::swap(id, id2);
+        }
     }
-    int* lists = work + p.words + (p.passes > 1 ? 4 : 2) * p.list;
+    float* part = reinterpret_cast<float*>(work + p.words + (p.passes > 1 ? 4 : 2) * p.list);
     const bool wide = n % (16 / size) == 0 && embed_aligned(d_dy, dy_stride, size) && embed_aligned(d_dtable, dtable_stride, out_size);
-    const EmbedBackward a = {s, d_dy, dy_stride, rows, n, scale, d_dtable, dtable_stride, {key, id, total, p.piece, p.pieces, reinterpret_cast<EmbedLong*>(lists), reinterpret_cast<float*>(lists + embed_lists(p))}};
+    const EmbedBackward a = {s, tokens, count, p.few, d_dy, dy_stride, rows, n, scale, d_dtable, dtable_stride, {key, id, total, p.piece, p.pieces, 1, part, work + p.tables}};
     const bool single = dtable_type == TB_TYPE_F32;
     if (type == TB_TYPE_F32) embed_rows_type<float, 4>(a, true, wide);
     else if (type == TB_TYPE_F16) embed_rows_type<__half, 8>(a, single, wide);

@@ -10,6 +10,7 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <atomic>
 #include <initializer_list>
 
 #define OP_MAX_ENTRIES (INT32_MAX - 1023)  // of operators that count entries in int: one step of a block beyond the last
@@ -107,6 +108,17 @@ static inline void op_launch_next(cudaStream_t s, dim3 grid, dim3 block, size_t 
     cfg.attrs = at;
     cfg.numAttrs = 1;
     op_note(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+}
+
+// Lets a kernel take that much shared memory on the current device; known: a bit for each device where it may already
+template <typename Kernel>
+static inline void op_allow_smem(Kernel kernel, int bytes, std::atomic<uint64_t>& known) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && known.load(std::memory_order_relaxed) >> dev & 1) return;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) known.fetch_or(1ull << dev);
+    op_note(e);
 }
 
 static inline int op_type_size(int type) { return type == TB_TYPE_F32 ? 4 : type == TB_TYPE_F16 || type == TB_TYPE_BF16 ? 2 : 0; }
