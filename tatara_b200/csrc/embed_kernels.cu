@@ -156,7 +156,7 @@ __device__ __forceinline__ void embed_zero(float (&acc)[CH][VEC]) {
 struct EmbedList {
     const int *key, *id, *count;   // count: of the tokens in the table
     int piece, pieces, together;   // tokens to a piece, how many pieces there can be, and how many of them a block looks at
-    float* part;                   // [pieces][2][n]: the sums of a piece's first and of its last token, where those have long lists
+    float* part;                   // [pieces][2][n]: the chunks' sums, at the piece and the end of it (first or last token) where the list's entries in the chunk begin
     int* done;                     // [pieces][2][tiles]: how many of a list's sums are there, counted at its first one; zero at the start
 };
 
@@ -176,11 +176,14 @@ __device__ __forceinline__ void embed_add_sums(float (&acc)[VEC], const float* f
 
 // How a warp gets the rows of a window of the list, `here` of them by the lanes' ids: f(j) for each in order, with its columns added to acc on the way.
 //
-// Rows on 16-byte boundaries come by asynchronous copies, several on their way for every warp whatever the lists' lengths, without registers.
+// By asynchronous copies: several are on their way for every warp whatever the lists' lengths, without registers.  Of a row that starts anywhere (VEC = 1) the 16-byte
+// pieces that hold its columns are copied, and its columns are read from where they lie in them.
 template <typename T, int VEC, int CH, int K>
 struct EmbedCopies {
-    static constexpr int TILE = 32 * VEC * CH, SLOT = TILE * (int)sizeof(T), SMEM = EMBED_WARPS * K * SLOT;
-    static_assert(SMEM >= EMBED_WARPS * TILE * 4 || K * sizeof(T) >= 4, "the warps' sums lie in the same memory");
+    static constexpr int TILE = 32 * VEC * CH, SLOT = TILE * (int)sizeof(T) + (VEC == 1 ? 16 : 0), SMEM = EMBED_WARPS * K * SLOT;
+    static_assert(K * sizeof(T) >= 4, "the warps' sums lie in the same memory");
+    // blocks per SM: what registers and memory allow
+    static constexpr int PER_SM = CH * VEC <= 8 && SMEM <= 24 * 1024 ? 8 : CH * VEC <= 16 ? 6 : 4;
     BulkRing<K, SLOT> ring;
     unsigned char* memory;
     const T* dy;
@@ -189,14 +192,19 @@ struct EmbedCopies {
     __device__ __forceinline__ EmbedCopies(unsigned char* smem, uint64_t* bars, const T* rows, int64_t row_stride, int column, int n)
         : ring(smem + (threadIdx.x >> 5) * K * SLOT, bars + (threadIdx.x >> 5) * K), memory(smem + (threadIdx.x >> 5) * K * SLOT), dy(rows + column), stride(row_stride),
           bytes((unsigned)(min(TILE, n - column) * (int)sizeof(T))) {}
+    __device__ __forceinline__ unsigned off(const T* row) const { return VEC == 1 ? (unsigned)(uintptr_t)row & 15u : 0u; }
     template <typename F>
     __device__ __forceinline__ void add(float (&acc)[CH][VEC], int id, int here, F f) {
         const int lane = threadIdx.x & 31;
         int sent = 0;
         for (int j = 0; j < here; ++j) {
-            for (; sent < here && sent < j + K; ++sent) ring.put(dy + __shfl_sync(0xffffffffu, id, sent) * stride, bytes);
+            for (; sent < here && sent < j + K; ++sent) {
+                const T* row = dy + __shfl_sync(0xffffffffu, id, sent) * stride;
+                ring.put(reinterpret_cast<const unsigned char*>(row) - off(row), VEC == 1 ? (bytes + off(row) + 15u) & ~15u : bytes);
+            }
             f(j);
-            const T* x = reinterpret_cast<const T*>(memory + ring.take() * SLOT) + lane * VEC;
+            const unsigned from = VEC == 1 ? off(dy + __shfl_sync(0xffffffffu, id, j) * stride) : 0u;
+            const T* x = reinterpret_cast<const T*>(memory + ring.take() * SLOT + from) + lane * VEC;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 OpRaw<T, VEC> v;
@@ -211,37 +219,32 @@ struct EmbedCopies {
     __device__ __forceinline__ float factor() const { return ring.ok ? 1.0f : __int_as_float(0x7fc00000); }
     __device__ __forceinline__ void end() { ring.end(); }
 };
-// Rows that start anywhere come through registers, an element at a time.
+// Through registers, K rows at a time: less latency where a warp has a few rows, and less to do for each where they are short.
 template <typename T, int VEC, int CH, int K>
 struct EmbedLoads {
-    static constexpr int SMEM = 0;
+    static constexpr int SMEM = EMBED_WARPS * 32 * VEC * 4, PER_SM = 8;
+    static_assert(CH == 1, "a lane has one access of a row");
     const T* dy;
     int64_t stride;
-    int n;
-    __device__ __forceinline__ EmbedLoads(unsigned char*, uint64_t*, const T* rows, int64_t row_stride, int column, int columns) : dy(rows + column), stride(row_stride), n(columns - column) {}
+    bool there;
+    __device__ __forceinline__ EmbedLoads(unsigned char*, uint64_t*, const T* rows, int64_t row_stride, int column, int n)
+        : dy(rows + column + (threadIdx.x & 31) * VEC), stride(row_stride), there(column + (int)(threadIdx.x & 31) * VEC < n) {}
     template <typename F>
-    __device__ __forceinline__ void add(float (&acc)[CH][VEC], int id, int here, F f) {
-        const int lane = threadIdx.x & 31;
+    __device__ __forceinline__ void add(float (&acc)[1][VEC], int id, int here, F f) {
         for (int j0 = 0; j0 < here; j0 += K) {
-            OpRaw<T, VEC> x[K][CH];
+            OpRaw<T, VEC> x[K];
 #pragma unroll
             for (int u = 0; u < K; ++u) {
                 const int64_t row = __shfl_sync(0xffffffffu, id, j0 + u);
-#pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    const int col = (c * 32 + lane) * VEC;
-                    x[u][c].zero();
-                    if (j0 + u < here && col < n) x[u][c].load(dy + row * stride + col);
-                }
+                x[u].zero();
+                if (j0 + u < here && there) x[u].load(dy + row * stride);
             }
 #pragma unroll
             for (int u = 0; u < K; ++u) {
                 if (j0 + u >= here) break;
                 f(j0 + u);
 #pragma unroll
-                for (int c = 0; c < CH; ++c)
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) acc[c][i] += x[u][c].get(i);
+                for (int i = 0; i < VEC; ++i) acc[0][i] += x[u].get(i);
             }
         }
     }
@@ -249,12 +252,11 @@ struct EmbedLoads {
     __device__ __forceinline__ void end() {}
 };
 
-// The first blocks: `together` pieces of the list and a tile of columns.  The others: `per` table rows and a tile per warp; it looks for the first row's place in the
+// The first blocks: a chunk of `together` pieces of the list and a tile of columns.  The others: `per` table rows and a tile per warp; it looks for the first row's place in the
 // list once and reads on from there, 32 entries at a time.
 template <typename T, typename O, int VEC, int CH, int K, template <typename, int, int, int> class Rows>
-__global__ void __launch_bounds__(EMBED_THREADS, 4)
+__global__ void __launch_bounds__(EMBED_THREADS, Rows<T, VEC, CH, K>::PER_SM)
 k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n, int tiles, int per, float scale, O* __restrict__ out, int64_t out_stride) {
-    using From = Rows<T, VEC, CH, K>;
     constexpr int TILE = 32 * VEC * CH;
     extern __shared__ __align__(128) unsigned char s_rows[];
     __shared__ uint64_t s_bars[EMBED_WARPS * K];
@@ -263,8 +265,7 @@ k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n
     const bool piece_block = (int64_t)blockIdx.x < piece_blocks;
     const int64_t unit = piece_block ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x - piece_blocks) * EMBED_WARPS + warp, group = unit / tiles;
     const int column = (int)(unit - group * tiles) * TILE, first = column + lane * VEC;
-    __shared__ float s_few[From::SMEM ? 1 : EMBED_WARPS * TILE];
-    From from_rows(s_rows, s_bars, dy, dy_stride, column, n);
+    Rows<T, VEC, CH, K> from_rows(s_rows, s_bars, dy, dy_stride, column, n);
     op_wait_for_previous();
     const int count = *list.count;
     float acc[CH][VEC];
@@ -312,7 +313,7 @@ k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n
     }
     // Every warp looks at a piece: its first and its last token, and whether their lists are longer than a piece.
     struct Sum {
-        int token, from, to, first, last;  // the token's entries in this piece, the list's first sum and its last piece
+        int token, from, to, first, last;  // the token's entries in this piece, the list's first sum, which is in the chunk where it begins, and its last piece
     };
     __shared__ Sum s_sums[EMBED_WARPS][2];
     __shared__ bool s_last;
@@ -332,7 +333,7 @@ k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n
         }
     }
     __syncthreads();
-    float* s_part = From::SMEM ? reinterpret_cast<float*>(s_rows) : s_few;
+    float* s_part = reinterpret_cast<float*>(s_rows);  // what the rows have come through
     // the warps' sums of their columns, added up in order: column at of the tile
     const auto share_out = [&](auto put) {
         __syncthreads();
@@ -349,9 +350,16 @@ k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n
             if (col < n) put(col, sum);
         }
     };
-    for (int which = 0; which < 2 * list.together; ++which) {
-        const Sum sum = s_sums[which / 2][which % 2];
+    for (int which = 0, next; which < 2 * list.together; which = next) {
+        Sum sum = s_sums[which / 2][which % 2];
+        next = which + 1;
         if (sum.token < 0) continue;
+        // the list's entries in the further pieces of this chunk follow
+        for (; next < 2 * list.together; ++next) {
+            const Sum more = s_sums[next / 2][next % 2];
+            if (more.token >= 0 && more.token != sum.token) break;
+            if (more.token >= 0) sum.to = more.to;
+        }
         const int64_t number = 2 * (group * list.together + which / 2) + which % 2;
         const int share = (sum.to - sum.from + EMBED_WARPS - 1) / EMBED_WARPS, mine_to = min(sum.from + (warp + 1) * share, sum.to);
         embed_zero(acc);
@@ -368,7 +376,7 @@ k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n
         // who writes the list's last sum adds them all up
         __threadfence();
         __syncthreads();
-        const int sums = sum.last - sum.first / 2 + 1;
+        const int chunk = sum.first / 2 / list.together, sums = sum.last / list.together - chunk + 1;
         if (threadIdx.x == 0) s_last = atomicAdd(list.done + (int64_t)sum.first * tiles + column / TILE, 1) == sums - 1;
         __syncthreads();
         if (s_last) {
@@ -377,7 +385,7 @@ k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n
             const int mine = (sums + EMBED_WARPS - 1) / EMBED_WARPS, to = min((warp + 1) * mine, sums);
 #pragma unroll 4
             for (int k = warp * mine; k < to; ++k) {
-                const float* from = list.part + (int64_t)(k == 0 ? sum.first : (sum.first / 2 + k) * 2) * n;
+                const float* from = list.part + (int64_t)(k == 0 ? sum.first : (chunk + k) * list.together * 2) * n;
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
                     const int col = first + c * 32 * VEC;
@@ -404,8 +412,6 @@ k_embed_few(Tokens tokens, int count, const T* dy, int64_t dy_stride, int n, int
     __shared__ int s_id[EMBED_FEW], s_many[EMBED_FEW_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x / tiles, column = (int)(blockIdx.x - row * tiles) * TILE;
     op_next_may_start();
-    // through registers, the copies' latency is longer
-    EmbedLoads<T, VEC, 1, 8> from_rows(nullptr, nullptr, dy, dy_stride, column, n);
     op_wait_for_previous();
     int token[STEPS];  // on their way together
 #pragma unroll
@@ -437,6 +443,7 @@ k_embed_few(Tokens tokens, int count, const T* dy, int64_t dy_stride, int n, int
     __syncthreads();
     float acc[1][VEC];
     embed_zero(acc);
+    EmbedLoads<T, VEC, 1, 8> from_rows(nullptr, nullptr, dy, dy_stride, column, n);
     const int share = (all + EMBED_FEW_WARPS - 1) / EMBED_FEW_WARPS, to = min((warp + 1) * share, all);
     for (int i0 = warp * share; i0 < to; i0 += 32) {
         const int here = min(32, to - i0), id = lane < here ? s_id[i0 + lane] : 0;
@@ -499,9 +506,9 @@ struct EmbedBackward {
     int64_t os;
     EmbedList list;
 };
-template <typename T, typename O, int VEC, int CH, int K, template <typename, int, int, int> class Rows>
+template <typename T, typename O, int VEC, int CH, int K, template <typename, int, int, int> class Rows = EmbedCopies>
 void embed_rows_go(const EmbedBackward& a) {
-    constexpr int SMEM = Rows<T, VEC, CH, K>::SMEM;
+    constexpr int SMEM = Rows<T, VEC, CH, K>::SMEM, PER_SM = Rows<T, VEC, CH, K>::PER_SM;
     const int tiles = (int)ceil_div64(a.n, 32 * VEC * CH);
     const auto kernel = k_embed_rows<T, O, VEC, CH, K, Rows>;
     if (SMEM > 40 * 1024) {
@@ -509,9 +516,9 @@ void embed_rows_go(const EmbedBackward& a) {
         op_allow_smem(kernel, SMEM, known);
     }
     // several rows per warp where that leaves every SM's warps a few turns: they share the search
-    const int64_t turns = a.rows * tiles / ((int64_t)sm_count() * 64);
+    const int64_t turns = a.rows * tiles / ((int64_t)sm_count() * PER_SM * EMBED_WARPS * 4);
     const int per = (int)(turns < 1 ? 1 : turns > EMBED_ROWS ? EMBED_ROWS : turns);
-    // pieces together where they are more than a few blocks per SM: most of them have no long list
+    // pieces together where they are more than a few blocks per SM: most of them have no long list, and a long one has fewer sums
     EmbedList list = a.list;
     const int64_t many = (int64_t)list.pieces * tiles / (2 * sm_count());
     list.together = (int)(many < 1 ? 1 : many > EMBED_WARPS ? EMBED_WARPS : many);
@@ -525,15 +532,20 @@ void embed_rows_pick(const EmbedBackward& a) {
         op_launch_next(a.s, dim3((unsigned)(a.rows * units)), dim3(EMBED_FEW_WARPS * 32), 0, k_embed_few<T, O, VEC>, a.tokens, (int)a.count, (const T*)a.dy, a.dys, a.n, units, a.scale, (O*)a.out, a.os);
         return;
     }
+    // a copy costs as much as a hundred bytes do: 132430 tokens of 17 fp16 columns 71 us by copies, 45 by loads; 22552 of 269 bf16 28 and 39
+    if (units == 1 && a.n * (int)sizeof(T) <= 256) return embed_rows_go<T, O, VEC, 1, 8, EmbedLoads>(a);
+    // the whole row up to 3 KB (512 columns where it starts anywhere), tiles of 2 KB (512 columns) above; as many copies per warp as leave an SM sixteen warps
     if constexpr (VEC == 1) {
-        if (units == 1) return embed_rows_go<T, O, 1, 1, 8, EmbedLoads>(a);
-        embed_rows_go<T, O, 1, 4, 4, EmbedLoads>(a);
+        if (units == 1) return embed_rows_go<T, O, 1, 1, 8>(a);
+        if (units == 2) return embed_rows_go<T, O, 1, 2, 8>(a);
+        if (units <= 4) return embed_rows_go<T, O, 1, 4, 8>(a);
+        if (units <= 8) return embed_rows_go<T, O, 1, 8, 8>(a);
+        embed_rows_go<T, O, 1, 16, 4>(a);
     } else {
-        // the whole row up to 3 KB, tiles of 2 KB above; as many copies per warp as leave an SM sixteen warps
-        if (units == 1) return embed_rows_go<T, O, VEC, 1, 8, EmbedCopies>(a);
-        if (units == 2) return embed_rows_go<T, O, VEC, 2, 8, EmbedCopies>(a);
-        if (units == 5 || units == 6) return embed_rows_go<T, O, VEC, 6, 4, EmbedCopies>(a);
-        embed_rows_go<T, O, VEC, 4, 4, EmbedCopies>(a);
+        if (units == 1) return embed_rows_go<T, O, VEC, 1, 8>(a);
+        if (units == 2) return embed_rows_go<T, O, VEC, 2, 8>(a);
+        if (units == 5 || units == 6) return embed_rows_go<T, O, VEC, 6, 4>(a);
+        embed_rows_go<T, O, VEC, 4, 4>(a);
     }
 }
 template <typename T, int VEC>

@@ -31,8 +31,16 @@ struct ExpertPut {
     __device__ __forceinline__ void rest(const int* total, const int* begin, const SortPlan& p) const {
         if (blockIdx.x == 0)
             for (int e = threadIdx.x; e <= p.keys; e += SORT_THREADS) offsets[e] = begin[e];
-        for (int e = blockIdx.x; e < p.keys && p.align > 1; e += gridDim.x)
-            for (int s = begin[e] + total[e] + threadIdx.x; s < begin[e + 1]; s += SORT_THREADS) source[s] = -1;
+        // experts that have not filled their last `align` places: one for each warp of the launch in turn, looked at 32 at once
+        const int lane = threadIdx.x & 31, warps = gridDim.x * SORT_WARPS;
+        for (int e0 = blockIdx.x * SORT_WARPS + threadIdx.x / 32; e0 < p.keys && p.align > 1; e0 += 32 * warps) {
+            const int e = e0 + lane * warps;
+            unsigned gaps = __ballot_sync(0xffffffffu, e < p.keys && begin[e] + total[e] < begin[e + 1]);
+            for (; gaps; gaps &= gaps - 1) {
+                const int g = e0 + (__ffs(gaps) - 1) * warps;
+                for (int s = begin[g] + total[g] + lane; s < begin[g + 1]; s += 32) source[s] = -1;
+            }
+        }
         for (int64_t s = begin[p.keys] + (int64_t)blockIdx.x * SORT_THREADS + threadIdx.x; s < slots; s += (int64_t)gridDim.x * SORT_THREADS) source[s] = -1;
     }
 };
@@ -193,14 +201,16 @@ k_combine_backward(const T* dout, int64_t dout_stride, const T* y, int64_t y_str
 }
 
 // ---- which kernel --------------------------------------------------------------------------------------------------------
-// f(lanes, units per lane) by a row's units: eight lanes up to 8 of them, then a warp with one to four each; longer rows are tiles of 128
-template <typename F>
+// f(lanes, units per lane) by a row's units: eight lanes up to 8 of them, then a warp with one to MOST each; longer rows are tiles.  Single elements are up to eight a lane, or too
+// few bytes are on their way (2386 columns of fp16: 59 us with two, 42 so).
+template <int MOST, typename F>
 void expert_with_shape(int units, F&& f) {
     using std::integral_constant;
     if (units <= 8) f(integral_constant<int, 8>(), integral_constant<int, 1>());
     else if (units <= 32) f(integral_constant<int, 32>(), integral_constant<int, 1>());
-    else if (units <= 64) f(integral_constant<int, 32>(), integral_constant<int, 2>());
-    else f(integral_constant<int, 32>(), integral_constant<int, 4>());
+    else if (units <= 64 || MOST == 2) f(integral_constant<int, 32>(), integral_constant<int, 2>());
+    else if (units <= 128 || MOST == 4) f(integral_constant<int, 32>(), integral_constant<int, 4>());
+    else f(integral_constant<int, 32>(), integral_constant<int, MOST>());
 }
 bool expert_blocks(int64_t units, int lanes, unsigned* blocks) {
     const int64_t b = (units + EXPERT_THREADS / lanes - 1) / (EXPERT_THREADS / lanes);
@@ -219,7 +229,7 @@ template <typename U>
 bool dispatch_go(const Experts& a, const void* x, int64_t xs, void* out, int64_t os, int per) {
     const int n = a.n / per;
     bool fits = true;
-    expert_with_shape(n, [&](auto l, auto ch) {
+    expert_with_shape<(sizeof(U) < 16 ? 8 : 4)>(n, [&](auto l, auto ch) {
         constexpr int L = decltype(l)::value, CH = decltype(ch)::value;
         const int tiles = (int)ceil_div64(n, L * CH);
         unsigned blocks;
@@ -232,8 +242,8 @@ bool dispatch_go(const Experts& a, const void* x, int64_t xs, void* out, int64_t
 template <typename T, int VEC>
 bool combine_go(const Experts& a, const void* y, int64_t ys, const float* gate, void* out, int64_t os) {
     bool fits = true;
-    expert_with_shape((int)ceil_div64(a.n, VEC), [&](auto l, auto ch) {
-        constexpr int L = decltype(l)::value, CH = decltype(ch)::value < 2 ? decltype(ch)::value : 2;
+    expert_with_shape<(VEC == 1 ? 8 : 2)>((int)ceil_div64(a.n, VEC), [&](auto l, auto ch) {
+        constexpr int L = decltype(l)::value, CH = decltype(ch)::value;
         const int tiles = (int)ceil_div64(a.n, L * CH * VEC);
         unsigned blocks;
         fits = expert_blocks(a.rows * tiles, L, &blocks);

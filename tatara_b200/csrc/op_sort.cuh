@@ -18,7 +18,7 @@ namespace {
 #define SORT_WARPS 8
 #define SORT_MAX_E 1024
 #define SORT_STEPS 8          // of a warp, whose entries are in registers together
-#define SORT_ONE 4096         // entries of a single block's sort
+#define SORT_ONE 2048         // entries of a single block's sort
 #define SORT_SCAN 8192        // blocks * keys above which a launch of its own adds up the counts
 
 struct SortPlan {

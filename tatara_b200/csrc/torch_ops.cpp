@@ -498,7 +498,11 @@ PyObject* expert_order(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const int64_t slots = tb_expert_slots(rows, k, experts, align);
     const On on(ix);
     const int64_t room = slots > 0 ? slots : 0;  // invalid sizes are refused below
-    const at::Tensor position = make(ix, {rows, k}, at::kInt), source = make(ix, {room}, at::kInt), offsets = make(ix, {experts > 0 ? experts + (int64_t)1 : 1}, at::kInt);
+    const int64_t begins = experts > 0 ? experts + (int64_t)1 : 1;
+    Shared all;
+    const int64_t position_at = all.place(rows * k), source_at = all.place(room), offsets_at = all.place(begins);
+    all.allocate(ix);
+    const at::Tensor position = all.tensor(position_at, {rows, k}, at::kInt), source = all.tensor(source_at, {room}, at::kInt), offsets = all.tensor(offsets_at, {begins}, at::kInt);
     const Work work(ix, tb_expert_order_workspace(rows, k, experts));
     char err[256];
     check(tb_expert_order(index, rows, k, experts, align, position.data_ptr<int>(), source.data_ptr<int>(), room, offsets.data_ptr<int>(), work.at(), work.bytes, on.stream, err, sizeof err),
