@@ -496,16 +496,16 @@ PyObject* expert_order(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const int32_t* index = static_cast<int32_t*>(vector_of(a[0], "index", ix, {rows, k}, at::kInt, true));
     const int experts = whole(a[1], "experts"), align = whole(a[2], "align");
     const int64_t slots = tb_expert_slots(rows, k, experts, align);
-    const On on(ix);
-    const int64_t room = slots > 0 ? slots : 0;  // invalid sizes are refused below
-    const int64_t begins = experts > 0 ? experts + (int64_t)1 : 1;
-    Shared all;
-    const int64_t position_at = all.place(rows * k), source_at = all.place(room), offsets_at = all.place(begins);
-    all.allocate(ix);
-    const at::Tensor position = all.tensor(position_at, {rows, k}, at::kInt), source = all.tensor(source_at, {room}, at::kInt), offsets = all.tensor(offsets_at, {begins}, at::kInt);
-    const Work work(ix, tb_expert_order_workspace(rows, k, experts));
     char err[256];
-    check(tb_expert_order(index, rows, k, experts, align, position.data_ptr<int>(), source.data_ptr<int>(), room, offsets.data_ptr<int>(), work.at(), work.bytes, on.stream, err, sizeof err),
+    if (slots < 0) check(tb_expert_order(nullptr, rows, k, experts, align, nullptr, nullptr, 0, nullptr, nullptr, 0, nullptr, err, sizeof err), "tb_expert_order", err);
+    const On on(ix);
+    const int64_t begins = experts + (int64_t)1;
+    Shared all;
+    const int64_t position_at = all.place(rows * k), source_at = all.place(slots), offsets_at = all.place(begins);
+    all.allocate(ix);
+    const at::Tensor position = all.tensor(position_at, {rows, k}, at::kInt), source = all.tensor(source_at, {slots}, at::kInt), offsets = all.tensor(offsets_at, {begins}, at::kInt);
+    const Work work(ix, tb_expert_order_workspace(rows, k, experts));
+    check(tb_expert_order(index, rows, k, experts, align, position.data_ptr<int>(), source.data_ptr<int>(), slots, offsets.data_ptr<int>(), work.at(), work.bytes, on.stream, err, sizeof err),
           "tb_expert_order", err);
     return tuple_of({position, source, offsets});
     BODY_END

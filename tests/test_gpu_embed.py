@@ -89,6 +89,33 @@ def test_lists_that_end_at_a_piece(count):
             check_backward(dy, tokens, rows, 1.0, ops().embedding_backward(dy, tokens, rows))
 
 
+# tiles of every width, one and several, rows on 16-byte boundaries and not, with lists that go over a piece, a chunk of pieces and much of the whole
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("count,rows,n", [(5000, 30, 777), (4000, 7, 768), (3000, 5, 1030), (2500, 3, 4100), (9000, 2, 513), (20000, 400, 96), (9000, 60, 128), (6000, 50, 200), (6000, 70, 250), (6000, 40, 1536),
+                                          (30000, 900, 768), (800_000, 5000, 4), (700_000, 3, 9)])
+def test_long_lists_of_wide_rows(count, rows, n, dtype):
+    dy, tokens = values(count, n, dtype, count + n), tokens_of(count, rows, n, 0.1)
+    got = ops().embedding_backward(dy, tokens, rows)
+    check_backward(dy, tokens, rows, 1.0, got)
+    assert torch.equal(ops().embedding_backward(dy, tokens.int(), rows), got)
+
+
+def test_a_first_call_may_be_captured():
+    """Nothing has to be set up before: a process of its own whose first calls go into a graph."""
+    import subprocess
+    import sys
+    from helpers import ROOT
+    code = ("import torch; from tatara_b200 import ops\n"
+            "t = torch.arange(5000, device='cuda') % 40; dy = torch.ones(5000, 768, device='cuda'); torch.cuda.synchronize()\n"
+            "g = torch.cuda.CUDAGraph()\n"
+            "with torch.cuda.graph(g):\n"
+            "    d = ops.embedding_backward(dy, t, 41); o = ops.expert_order(t.int()[:, None].contiguous(), 40); y = ops.rms_norm_forward(dy)[0]\n"
+            "g.replay(); torch.cuda.synchronize()\n"
+            "assert (d[:40] == 125).all() and (d[40] == 0).all() and (o.offsets.cpu() == torch.arange(41) * 125).all() and ((y - 1).abs() < 1e-5).all()\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("offset", [1, 8])
 def test_rows_of_a_wider_buffer(dtype, offset):

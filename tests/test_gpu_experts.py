@@ -74,6 +74,24 @@ def test_align_of_more_than_all_entries():
     assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("rows,k,experts", [(400_001, 2, 9), (350_000, 4, 1000), (2_500_000, 1, 33)])
+def test_orders_of_many_choices(rows, k, experts):
+    """Blocks whose entries do not fit their registers; against a stable sort, which is exact."""
+    index = torch.randint(-1, experts, (rows, k), generator=torch.Generator("cuda").manual_seed(rows), device="cuda", dtype=torch.int32)
+    index[1000:200_000] = experts // 2   # a long run of one expert
+    got = ops().expert_order(index, experts, align=64)
+    flat = torch.where(index.flatten() < 0, experts, index.flatten())
+    by = flat.sort(stable=True)
+    counts = torch.bincount(flat, minlength=experts + 1)[:experts]
+    begins = torch.cat([counts.new_zeros(1), ((counts + 63) // 64 * 64).cumsum(0)])
+    assert torch.equal(got.offsets.long(), begins)
+    ok = by.values < experts
+    place = begins[by.values[ok].long()] + torch.arange(int(ok.sum()), device="cuda") - torch.cat([counts.new_zeros(1), counts.cumsum(0)])[by.values[ok].long()]
+    position = torch.full_like(flat, -1).index_copy_(0, by.indices[ok], place.int())
+    source = torch.full_like(got.source, -1).index_copy_(0, place, by.indices[ok].int())
+    assert torch.equal(got.position.flatten(), position) and torch.equal(got.source, source)
+
+
 def rows_of(rows, n, dtype, seed, pad=0, offset=0):
     g = torch.Generator("cuda").manual_seed(seed)
     return torch.randn(rows, n + pad + offset, generator=g, device="cuda").to(dtype)[:, offset:offset + n]
