@@ -72,6 +72,7 @@ struct FirstSource {
     Tokens tokens;
     int mask;
     __device__ __forceinline__ int operator()(int64_t i) const { return tokens(i); }
+    __device__ __forceinline__ int id(int64_t i) const { return (int)i; }
     __device__ __forceinline__ int key(int v) const { return v < 0 ? -1 : v & mask; }
 };
 // counts for the sort by the next digits while the entries are placed: the blocks of that sort take `piece` places each.  (A launch of its own for it: 6 us.)
@@ -87,10 +88,10 @@ struct FirstPut {
     int* zero;              // set to zero by a single block; by the launch that counts where there are more
     int64_t zeros;
     NextCount next;
-    __device__ __forceinline__ void operator()(int64_t i, int v, int place) const {
+    __device__ __forceinline__ void operator()(int i, int v, int place) const {
         if (place < 0) return;
         key[place] = v;
-        id[place] = (int)i;
+        id[place] = i;
         next(v, place);
     }
     __device__ __forceinline__ void rest(const int*, const int* begin, const SortPlan& p) const {
@@ -100,22 +101,22 @@ struct FirstPut {
 };
 // further digits, of what the digits before have sorted
 struct NextSource {
-    const int *sorted, *count;
+    const int *sorted, *ids, *count;
     int shift, mask;
     __device__ __forceinline__ int operator()(int64_t i) const {
         const int v = sorted[i];  // behind the last one anything
         return i < *count ? v : -1;
     }
+    __device__ __forceinline__ int id(int64_t i) const { return ids[i]; }
     __device__ __forceinline__ int key(int v) const { return v < 0 ? -1 : v >> shift & mask; }
 };
 struct NextPut {
-    const int* id_in;
     int *key, *id;
     NextCount next;
-    __device__ __forceinline__ void operator()(int64_t i, int v, int place) const {
+    __device__ __forceinline__ void operator()(int i, int v, int place) const {
         if (place < 0) return;
         key[place] = v;
-        id[place] = id_in[i];
+        id[place] = i;
         next(v, place);
     }
     __device__ __forceinline__ void rest(const int*, const int*, const SortPlan&) const {}
@@ -219,32 +220,39 @@ struct EmbedCopies {
     __device__ __forceinline__ float factor() const { return ring.ok ? 1.0f : __int_as_float(0x7fc00000); }
     __device__ __forceinline__ void end() { ring.end(); }
 };
-// Through registers, K rows at a time: less latency where a warp has a few rows, and less to do for each where they are short.
+// Through registers, K rows at a time: less latency where a warp has a few rows, and as many short ones as there are (an SM starts a copy every 90 cycles or so).
 template <typename T, int VEC, int CH, int K>
 struct EmbedLoads {
-    static constexpr int SMEM = EMBED_WARPS * 32 * VEC * 4, PER_SM = 8;
-    static_assert(CH == 1, "a lane has one access of a row");
+    static constexpr int TILE = 32 * VEC * CH, SMEM = EMBED_WARPS * TILE * 4;
+    static constexpr int HELD = K * CH * ((VEC * (int)sizeof(T) + 3) / 4) + CH * VEC;  // registers
+    static constexpr int PER_SM = HELD <= 28 ? 8 : HELD <= 48 ? 6 : 4;
     const T* dy;
     int64_t stride;
-    bool there;
-    __device__ __forceinline__ EmbedLoads(unsigned char*, uint64_t*, const T* rows, int64_t row_stride, int column, int n)
-        : dy(rows + column + (threadIdx.x & 31) * VEC), stride(row_stride), there(column + (int)(threadIdx.x & 31) * VEC < n) {}
+    int n;  // columns from the tile's first
+    __device__ __forceinline__ EmbedLoads(unsigned char*, uint64_t*, const T* rows, int64_t row_stride, int column, int columns) : dy(rows + column), stride(row_stride), n(columns - column) {}
     template <typename F>
-    __device__ __forceinline__ void add(float (&acc)[1][VEC], int id, int here, F f) {
+    __device__ __forceinline__ void add(float (&acc)[CH][VEC], int id, int here, F f) {
+        const int lane = threadIdx.x & 31;
         for (int j0 = 0; j0 < here; j0 += K) {
-            OpRaw<T, VEC> x[K];
+            OpRaw<T, VEC> x[K][CH];
 #pragma unroll
             for (int u = 0; u < K; ++u) {
-                const int64_t row = __shfl_sync(0xffffffffu, id, j0 + u);
-                x[u].zero();
-                if (j0 + u < here && there) x[u].load(dy + row * stride);
+                const T* row = dy + __shfl_sync(0xffffffffu, id, j0 + u) * stride;
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int col = (c * 32 + lane) * VEC;
+                    x[u][c].zero();
+                    if (j0 + u < here && col < n) x[u][c].load(row + col);
+                }
             }
 #pragma unroll
             for (int u = 0; u < K; ++u) {
                 if (j0 + u >= here) break;
                 f(j0 + u);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) acc[0][i] += x[u].get(i);
+                for (int c = 0; c < CH; ++c)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) acc[c][i] += x[u][c].get(i);
             }
         }
     }
@@ -402,43 +410,51 @@ k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n
 
 // Few tokens and a small table: a block per table row and tile looks through all tokens for its own, in order, and its warps take a share of them each.  One launch and
 // no workspace; 1000 tokens, 81 x 256 fp32: 3.7 us, by the sort 12 to 14.
-#define EMBED_FEW 1024
+#define EMBED_FEW 2048
 #define EMBED_FEW_WARPS 8
 template <typename T, typename O, int VEC>
 __global__ void __launch_bounds__(EMBED_FEW_WARPS * 32)
 k_embed_few(Tokens tokens, int count, const T* dy, int64_t dy_stride, int n, int tiles, float scale, O* __restrict__ out, int64_t out_stride) {
-    constexpr int TILE = 32 * VEC, STEPS = EMBED_FEW / EMBED_FEW_WARPS / 32;
+    constexpr int TILE = 32 * VEC, STEPS = 4;
     __shared__ float s_part[EMBED_FEW_WARPS * TILE];
     __shared__ int s_id[EMBED_FEW], s_many[EMBED_FEW_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x / tiles, column = (int)(blockIdx.x - row * tiles) * TILE;
     op_next_may_start();
     op_wait_for_previous();
-    int token[STEPS];  // on their way together
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-        const int i = (warp * STEPS + s) * 32 + lane;
-        token[s] = tokens(min(i, count - 1));
-        if (i >= count) token[s] = -1;
-    }
+    // a warp's eighth of the tokens, STEPS * 32 of them at a time
+    const int rounds = (count + EMBED_FEW_WARPS * STEPS * 32 - 1) / (EMBED_FEW_WARPS * STEPS * 32);
     unsigned found[STEPS];
-    int many = 0;
+    int many = 0, at = 0, all = 0;
+    const auto look = [&](int round) {
+        int token[STEPS];  // on their way together
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-        found[s] = __ballot_sync(0xffffffffu, token[s] == row);
-        many += __popc(found[s]);
+        for (int s = 0; s < STEPS; ++s) {
+            const int i = ((warp * rounds + round) * STEPS + s) * 32 + lane;
+            token[s] = tokens(min(i, count - 1));
+            if (i >= count) token[s] = -1;
+        }
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) found[s] = __ballot_sync(0xffffffffu, token[s] == row);
+    };
+    for (int round = 0; round < rounds; ++round) {
+        look(round);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) many += __popc(found[s]);
     }
     if (lane == 0) s_many[warp] = many;
     __syncthreads();
-    int at = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < EMBED_FEW_WARPS; ++w) {
         at += w < warp ? s_many[w] : 0;
         all += s_many[w];
     }
+    for (int round = 0; round < rounds; ++round) {
+        if (rounds > 1) look(round);
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-        if (found[s] >> lane & 1) s_id[at + __popc(found[s] & ((1u << lane) - 1u))] = (warp * STEPS + s) * 32 + lane;
-        at += __popc(found[s]);
+        for (int s = 0; s < STEPS; ++s) {
+            if (found[s] >> lane & 1) s_id[at + __popc(found[s] & ((1u << lane) - 1u))] = ((warp * rounds + round) * STEPS + s) * 32 + lane;
+            at += __popc(found[s]);
+        }
     }
     __syncthreads();
     float acc[1][VEC];
@@ -470,8 +486,9 @@ struct EmbedPlan {
 };
 bool embed_plan(int64_t count, int64_t rows, int n, EmbedPlan* p) {
     if (count < 0 || count > OP_MAX_ENTRIES || rows < 1 || rows > INT32_MAX || n < 1 || n > OP_MAX_COLUMNS) return false;
-    // every row's blocks look through all tokens: as long as that is less than the sort's launches
-    p->few = count > 0 && count <= EMBED_FEW && rows * ceil_div64(n, 128) <= 16 * (int64_t)sm_count();
+    // every row's blocks look through all tokens: as long as they, and what they read, are less than the sort's launches
+    const int64_t blocks = rows * ceil_div64(n, 128);
+    p->few = count > 0 && count <= EMBED_FEW && blocks <= 16 * (int64_t)sm_count() && blocks * count <= 16 * 1024 * (int64_t)sm_count();
     int bits = 1;
     while (((int64_t)1 << bits) < rows) ++bits;
     p->passes = (bits + 9) / 10;
@@ -515,8 +532,8 @@ void embed_rows_go(const EmbedBackward& a) {
         static std::atomic<uint64_t> known{0};
         op_allow_smem(kernel, SMEM, known);
     }
-    // several rows per warp where that leaves every SM's warps a few turns: they share the search
-    const int64_t turns = a.rows * tiles / ((int64_t)sm_count() * PER_SM * EMBED_WARPS * 4);
+    // Several rows per warp share the search: as many as leave every warp four turns, or one turn of short rows, which take no longer than the search.
+    const int64_t turns = a.rows * tiles / ((int64_t)sm_count() * PER_SM * EMBED_WARPS * (a.n * (int)sizeof(T) <= 256 ? 1 : 4));
     const int per = (int)(turns < 1 ? 1 : turns > EMBED_ROWS ? EMBED_ROWS : turns);
     // pieces together where they are more than a few blocks per SM: most of them have no long list, and a long one has fewer sums
     EmbedList list = a.list;
@@ -532,20 +549,19 @@ void embed_rows_pick(const EmbedBackward& a) {
         op_launch_next(a.s, dim3((unsigned)(a.rows * units)), dim3(EMBED_FEW_WARPS * 32), 0, k_embed_few<T, O, VEC>, a.tokens, (int)a.count, (const T*)a.dy, a.dys, a.n, units, a.scale, (O*)a.out, a.os);
         return;
     }
-    // a copy costs as much as a hundred bytes do: 132430 tokens of 17 fp16 columns 71 us by copies, 45 by loads; 22552 of 269 bf16 28 and 39
-    if (units == 1 && a.n * (int)sizeof(T) <= 256) return embed_rows_go<T, O, VEC, 1, 8, EmbedLoads>(a);
-    // the whole row up to 3 KB (512 columns where it starts anywhere), tiles of 2 KB (512 columns) above; as many copies per warp as leave an SM sixteen warps
+    // Rows up to 2 KB by loads (125143 tokens evenly over 3640 x 384 fp32: 73 us, by copies 85), longer ones and their tiles of 2 KB by copies (73305 x 768: 136, by loads
+    // 143); rows that start anywhere up to 128 columns by loads, by copies above (3640 x 222: 80 us, by loads 60 where tokens are even and 154 where they are not).
     if constexpr (VEC == 1) {
-        if (units == 1) return embed_rows_go<T, O, 1, 1, 8>(a);
-        if (units == 2) return embed_rows_go<T, O, 1, 2, 8>(a);
-        if (units <= 4) return embed_rows_go<T, O, 1, 4, 8>(a);
-        if (units <= 8) return embed_rows_go<T, O, 1, 8, 8>(a);
-        embed_rows_go<T, O, 1, 16, 4>(a);
+        if (units == 1) return embed_rows_go<T, O, 1, 1, 8, EmbedLoads>(a);
+        if (units == 2) return embed_rows_go<T, O, 1, 2, 8, EmbedLoads>(a);
+        if (units <= 4) return embed_rows_go<T, O, 1, 4, 4, EmbedLoads>(a);
+        if (units <= 8) return embed_rows_go<T, O, 1, 8, 8, EmbedCopies>(a);
+        embed_rows_go<T, O, 1, 16, 4, EmbedCopies>(a);
     } else {
-        if (units == 1) return embed_rows_go<T, O, VEC, 1, 8>(a);
-        if (units == 2) return embed_rows_go<T, O, VEC, 2, 8>(a);
-        if (units == 5 || units == 6) return embed_rows_go<T, O, VEC, 6, 4>(a);
-        embed_rows_go<T, O, VEC, 4, 4>(a);
+        if (units == 1) return embed_rows_go<T, O, VEC, 1, 8, EmbedLoads>(a);
+        if (units <= 4) return embed_rows_go<T, O, VEC, 2, 4, EmbedLoads>(a);
+        if (units == 5 || units == 6) return embed_rows_go<T, O, VEC, 6, 4, EmbedCopies>(a);
+        embed_rows_go<T, O, VEC, 4, 4, EmbedCopies>(a);
     }
 }
 template <typename T, int VEC>
@@ -565,6 +581,12 @@ bool embed_forward_go(cudaStream_t s, const Tokens& tokens, int64_t count, const
         op_launch_next(s, dim3((unsigned)blocks), dim3(EMBED_THREADS), 0, k_embed_forward<T, VEC, L, CH, R>, tokens, count, (const T*)table, ts, n, tiles, scale, (T*)out, os); \
         return true;                                                                                                                                              \
     } while (0)
+    if constexpr (VEC == 1) {  // single elements: more of them on their way (146325 x 294 fp16: 114 us with four a lane, 40 with sixteen)
+        if (units <= 8) GO(8, 1, 8);
+        if (units <= 32) GO(32, 1, 8);
+        if (units <= 64) GO(32, 2, 8);
+        GO(32, 4, 4);
+    }
     if (units <= 8) GO(8, 1, 4);
     if (units <= 32) GO(32, 1, 4);
     if (units <= 64) GO(32, 2, 2);
@@ -642,7 +664,7 @@ extern "C" int tb_embedding_backward(const void* d_dy, int64_t dy_stride, int ty
         sort_count(s, p.sort, FirstSource{tokens, mask}, count, work, work + table, zeros);
         sort_place(s, p.sort, FirstSource{tokens, mask}, count, work, FirstPut{key, id, total, work + table, zeros, next(1)});
         for (int k = 1; k < p.passes; ++k) {
-            sort_place(s, p.sort, NextSource{key, total, k * p.bits, mask}, count, work + k * table, NextPut{id, key2, id2, next(k + 1)});
+            sort_place(s, p.sort, NextSource{key, id, total, k * p.bits, mask}, count, work + k * table, NextPut{key2, id2, next(k + 1)});
             std::swap(key, key2);
             std::swap(id, id2);
         }

@@ -18,14 +18,15 @@ namespace {
 struct ExpertSource {
     const int* index;
     __device__ __forceinline__ int operator()(int64_t i) const { return index[i]; }
+    __device__ __forceinline__ int id(int64_t i) const { return (int)i; }
     __device__ __forceinline__ int key(int v) const { return v; }
 };
 struct ExpertPut {
     int *position, *source, *offsets;
     int64_t slots;
-    __device__ __forceinline__ void operator()(int64_t i, int, int place) const {
+    __device__ __forceinline__ void operator()(int i, int, int place) const {
         position[i] = place;
-        if (place >= 0) source[place] = (int)i;
+        if (place >= 0) source[place] = i;
     }
     // the begins, and -1 at every place that no choice has taken
     __device__ __forceinline__ void rest(const int* total, const int* begin, const SortPlan& p) const {
@@ -201,12 +202,13 @@ k_combine_backward(const T* dout, int64_t dout_stride, const T* y, int64_t y_str
 }
 
 // ---- which kernel --------------------------------------------------------------------------------------------------------
-// f(lanes, units per lane) by a row's units: eight lanes up to 8 of them, then a warp with one to MOST each; longer rows are tiles.  Single elements are up to eight a lane, or too
+// f(lanes, units per lane) by a row's units: 8 or 16 lanes up to as many of them, then a warp with one to MOST each; longer rows are tiles.  Single elements are up to eight a lane, or too
 // few bytes are on their way (2386 columns of fp16: 59 us with two, 42 so).
 template <int MOST, typename F>
 void expert_with_shape(int units, F&& f) {
     using std::integral_constant;
     if (units <= 8) f(integral_constant<int, 8>(), integral_constant<int, 1>());
+    else if (units <= 16) f(integral_constant<int, 16>(), integral_constant<int, 1>());
     else if (units <= 32) f(integral_constant<int, 32>(), integral_constant<int, 1>());
     else if (units <= 64 || MOST == 2) f(integral_constant<int, 32>(), integral_constant<int, 2>());
     else if (units <= 128 || MOST == 4) f(integral_constant<int, 32>(), integral_constant<int, 4>());
@@ -267,7 +269,8 @@ void combine_backward_go(const Experts& a, const void* dout, int64_t ds, const v
 }
 template <typename T, int VEC>
 void combine_backward_pick(const Experts& a, const void* dout, int64_t ds, const void* y, int64_t ys, const float* gate, void* dy, int64_t dys, float* dgate) {
-    if (a.n <= 8 * VEC) combine_backward_go<T, VEC, 1, 8>(a, dout, ds, y, ys, gate, dy, dys, dgate);
+    // eight lanes for short rows: fewer of them for a sum over the lanes (55049 x 59 bf16, k = 5: 52 us, with a warp per row 60)
+    if (a.n <= 8 * VEC || (VEC == 1 && a.n <= 64)) combine_backward_go<T, VEC, 1, 8>(a, dout, ds, y, ys, gate, dy, dys, dgate);
     else if (a.n <= 64 * VEC || a.rows >= 8 * (int64_t)sm_count()) combine_backward_go<T, VEC, 1, 32>(a, dout, ds, y, ys, gate, dy, dys, dgate);
     else combine_backward_go<T, VEC, 8, 32>(a, dout, ds, y, ys, gate, dy, dys, dgate);
 }
@@ -300,7 +303,9 @@ extern "C" int64_t tb_expert_slots(int64_t rows, int k, int experts, int align) 
 }
 extern "C" int64_t tb_expert_order_workspace(int64_t rows, int k, int experts) {
     if (tb_expert_slots(rows, k, experts, 1) < 0) return TB_ERR_INVALID_ARGUMENT;
-    return sort_words(sort_plan(rows * k, experts, 1)) * 4;
+    // for any align: more blocks fill the places that are left over where those are many
+    const int64_t usual = sort_words(sort_plan(rows * k, experts, 1)), filling = sort_words(sort_plan(rows * k, experts, 1, INT32_MAX));
+    return (usual > filling ? usual : filling) * 4;
 }
 
 extern "C" int tb_expert_order(const int32_t* d_index, int64_t rows, int k, int experts, int align, int32_t* d_position, int32_t* d_source, int64_t slots, int32_t* d_offsets, void* d_work,
@@ -320,7 +325,7 @@ extern "C" int tb_expert_order(const int32_t* d_index, int64_t rows, int k, int 
     const OpRows ix = op_vector(d_index, rows * k), po = op_vector(d_position, rows * k), so = op_vector(d_source, slots), of = op_vector(d_offsets, experts + 1);
     if (op_meets(ix, {po, so, of}) || op_meets(po, {so, of}) || op_meets(so, {of})) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "a result overlaps another tensor");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const SortPlan plan = sort_plan(rows * k, experts, align);
+    const SortPlan plan = sort_plan(rows * k, experts, align, slots - rows * k);
     sort_count(s, plan, ExpertSource{d_index}, rows * k, static_cast<int*>(d_work));
     sort_place(s, plan, ExpertSource{d_index}, rows * k, static_cast<int*>(d_work), ExpertPut{d_position, d_source, d_offsets, slots});
     return op_launched(err, err_len);

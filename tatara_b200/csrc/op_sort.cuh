@@ -27,7 +27,8 @@ struct SortPlan {
     int steps;                // of every warp; a block's piece is SORT_THREADS * steps entries
     bool scan;
 };
-inline SortPlan sort_plan(int64_t entries, int keys, int align) {
+// fill: places that may be left over, for the same blocks to fill
+inline SortPlan sort_plan(int64_t entries, int keys, int align, int64_t fill = 0) {
     SortPlan p;
     p.keys = keys;
     p.align = align;
@@ -35,9 +36,11 @@ inline SortPlan sort_plan(int64_t entries, int keys, int align) {
     // four steps up to a block per SM, then up to SORT_STEPS with more blocks, then longer pieces
     const int64_t rows = (entries + SORT_THREADS - 1) / SORT_THREADS, sms = sm_count();
     int64_t steps = rows <= 4 * sms ? 4 : rows <= 2 * SORT_STEPS * sms ? SORT_STEPS : (rows + 2 * sms - 1) / (2 * sms);
-    if (entries <= SORT_ONE) steps = rows < 1 ? 1 : rows;
+    const bool one = entries <= SORT_ONE && fill <= 16 * SORT_ONE;
+    if (one) steps = rows < 1 ? 1 : rows;
+    else if (fill > 16 * SORT_ONE && rows < sms) steps = 1;
     p.steps = (int)steps;
-    p.blocks = entries <= SORT_ONE ? 1 : (int)((rows + steps - 1) / steps);
+    p.blocks = one || rows < 1 ? 1 : (int)((rows + steps - 1) / steps);
     p.scan = p.blocks > 1 && (int64_t)p.blocks * keys > SORT_SCAN;
     return p;
 }
@@ -50,7 +53,7 @@ struct SortWalk {
     const Source& source;
     int keys, steps, bits, lane;
     int64_t first, entries;
-    int v[S], rank[S];
+    int v[S], id[S], rank[S];
     __device__ __forceinline__ SortWalk(const Source& src, int64_t n, const SortPlan& p)
         : source(src), keys(p.keys), steps(p.steps), bits(p.bits), lane(threadIdx.x & 31),
           first(((int64_t)blockIdx.x * SORT_WARPS + (threadIdx.x >> 5)) * p.steps * 32), entries(n) {}
@@ -58,8 +61,8 @@ struct SortWalk {
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             const int64_t i = first + (int64_t)(s0 + s) * 32 + lane;
-            v[s] = -1;
-            if (s0 + s < steps && i < entries) v[s] = source(i);
+            v[s] = -1, id[s] = 0;
+            if (s0 + s < steps && i < entries) v[s] = source(i), id[s] = source.id(i);
         }
     }
     __device__ __forceinline__ int key(int s) const {
@@ -183,7 +186,7 @@ __device__ __forceinline__ void sort_begins(const int* s_total, int* s_begin, co
     __syncthreads();
 }
 
-// Source: the value of an entry, and the key in a value; Put: put(entry, value, place) for every entry (-1: no place), and put.rest(counts, begins, plan) by every block
+// Source: the value and the identity of an entry, and the key in a value; Put: put(identity, value, place) for every entry (-1: no place), and put.rest(counts, begins, plan) by every block
 template <typename Source, typename Put, int S>
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_place(Source source, int64_t entries, SortPlan p, const int* part, Put put) {
     extern __shared__ int s_mem[];
@@ -210,7 +213,7 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_place(Source source, int6
         for (int e = threadIdx.x % width; e < keys; e += width) {
             const int step = SORT_THREADS / width;
             int total = 0, ahead = 0;
-#pragma unroll 8
+#pragma unroll 16
             for (int b = threadIdx.x / width; b < p.blocks; b += step) {
                 const int c = part[(int64_t)b * keys + e];
                 total += c;
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_place(Source source, int6
         for (int s = 0; s < S; ++s) {
             const int64_t i = w.first + (int64_t)(s0 + s) * 32 + w.lane;
             const int e = w.key(s);
-            if (s0 + s < p.steps && i < entries) put(i, w.v[s], e < 0 ? -1 : again ? w.rank[s] : next[e] + w.rank[s]);
+            if (s0 + s < p.steps && i < entries) put(w.id[s], w.v[s], e < 0 ? -1 : again ? w.rank[s] : next[e] + w.rank[s]);
         }
     }
     put.rest(s_total, s_begin, p);
