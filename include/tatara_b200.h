@@ -358,7 +358,8 @@ int tb_combine_backward(const void* d_dout, int64_t dout_stride, const void* d_y
 int tb_embedding_forward(const void* d_tokens, int token_bytes, int64_t count, const void* d_table, int64_t table_stride, int type, int64_t rows, int n, float scale,
                          void* d_out, int64_t out_stride, void* stream, char* err, size_t err_len);
 int64_t tb_embedding_backward_workspace(int64_t count, int64_t rows, int n);
-/* dtable [rows, n] = scale * the sum of dy over the tokens of every row, written (not added to), zeros where there are none; of type dtable_type: that of dy, or TB_TYPE_F32. */
+/* dtable [rows, n] = scale * the sum of dy over the tokens of every row, written (not added to), zeros where there are none; of type dtable_type: that of dy, or TB_TYPE_F32.  The
+ * 16-byte pieces of memory that hold a row of dy may be read whole. */
 int tb_embedding_backward(const void* d_dy, int64_t dy_stride, int type, const void* d_tokens, int token_bytes, int64_t count, int64_t rows, int n, float scale,
                           void* d_dtable, int64_t dtable_stride, int dtable_type, void* d_work, int64_t work_bytes, void* stream, char* err, size_t err_len);
 

@@ -9,6 +9,9 @@
 // All are bound by memory: rows go by the order of the tokens, so a token's row is read once for all of its places; the places' rows are read or written
 // once each, wherever they lie, in whole 16-byte accesses.  A group of lanes takes a row or a tile of its columns.  Sums are fp32: the choices in ascending order; a
 // dot product's columns per thread in ascending order, then halves of the lanes, then the warps in order.
+//
+// Measured: dispatch 65536 x 1536 bf16 to two places each 95.5 us (6.3 TB/s); combination of 30011 x 1000 fp16 from eight places each 95 us (5.4 TB/s: gathers of 2000 bytes), its gradient for
+// 40000 x 768 fp32 and two places 95.5 us (6.4 TB/s); the order of 65536 x 2 choices of 9 6 us, of 40000 x 8 of 256 15.6 us (launches that wait for one another).
 #include "op_sort.cuh"
 
 namespace {

@@ -6,7 +6,7 @@
 // A block of eight warps owns a piece of the entries, a warp an eighth of it, 32 entries a step.  First launch: the blocks' counts.  Last launch: the warps count
 // their eighths again into shared memory, every block adds up the counts ahead of its own, turns the counts into places, and its warps give every entry its own (votes over
 // the warp's keys rank 32 entries at once).  Where blocks times keys are many, a launch between the two adds the counts up once for all
-// blocks; where all entries fit a block, the last launch is the only one.  No atomics on global memory, places do not depend on timing.
+// blocks; where all entries fit a block, the last launch is the only one.  Places do not depend on timing.
 //
 // What bounds it is latency: an eighth's entries are loaded together (one step at a time cost a microsecond each) and stay in registers up to SORT_STEPS steps.
 #pragma once
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(1024) k_sort_scan(SortPlan p, int* __restrict_
     if (warp == 31) part[(int64_t)p.blocks * p.keys + e] = run;
 }
 
-// Where the experts begin from their counts, both [keys] in shared memory (s_begin[keys] too: the end), by all threads of the block
+// Where the keys begin from their counts, both [keys] in shared memory (s_begin[keys] too: the end), by all threads of the block
 __device__ __forceinline__ void sort_begins(const int* s_total, int* s_begin, const SortPlan& p) {
     __shared__ int s_warp[SORT_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
