@@ -99,7 +99,7 @@ void* vector_of(PyObject* o, const char* name, const at::Tensor& like, at::IntAr
     return t.data_ptr();
 }
 at::Tensor make(const at::Tensor& like, at::IntArrayRef shape, at::ScalarType type) { return at::detail::empty_cuda(shape, type, like.device(), std::nullopt); }
-// Small results of one call from one allocation (one each costs 0.5 us): places of 128 bytes' alignment, and the tensors there.
+// Small results of one call, and what is kept together, from one allocation (one each costs 0.5 us): places of 128 bytes' alignment, and the tensors there.
 struct Shared {
     int64_t bytes = 0;
     at::Tensor base;
@@ -429,9 +429,19 @@ PyObject* rms_norm(PyObject* const* a, bool eight) {
     const int group = !eight ? 0 : a[4] == Py_None ? n : whole(a[4], "group");
     if (eight && group != 32 && group != 64 && group != 128 && group != n) refuse("group must be 32, 64, 128 or the number of columns (got %d)", group);
     const On on(x);
-    const at::Tensor h = r.defined() ? output_named(a[5], x, "residual_out") : at::Tensor();
+    at::Tensor h, rstd;
+    if (r.defined() && a[5] == Py_None) {  // what the backward pass takes, from one allocation
+        Shared both;
+        const int64_t h_at = both.place((rows * n * x.element_size() + 3) / 4), rstd_at = both.place(rows);
+        both.allocate(x);
+        h = both.tensor(h_at, x.sizes(), x.scalar_type());
+        rstd = both.tensor(rstd_at, {rows}, at::kFloat);
+    } else {
+        if (r.defined()) h = output_named(a[5], x, "residual_out");
+        rstd = make(x, {rows}, at::kFloat);
+    }
     const int64_t hs = h.defined() ? rows_of(h, "residual_out") : 0;
-    const at::Tensor y = eight ? make(x, x.sizes(), at::kFloat8_e4m3fn) : output(a[4], x), rstd = make(x, {rows}, at::kFloat);
+    const at::Tensor y = eight ? make(x, x.sizes(), at::kFloat8_e4m3fn) : output(a[4], x);
     const int64_t ys = rows_of(y, "out");
     char err[256];
     if (eight) {

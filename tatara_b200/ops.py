@@ -3,7 +3,7 @@ by expert and back, rows of a table by token, Newton-Schulz orthogonalisation an
 
 The functions check their arguments, take outputs and workspaces from torch's allocator and enqueue kernels of libtatara_b200.so on torch's current
 stream of the tensors' device (csrc/torch_ops.cpp).  Nothing is synchronised and nothing is kept between calls.  Wrong arguments raise
-`TrainerError`.  Small results of one call (mean and rstd; dweight and dbias; a routing's counts, rows, prob_mean and losses; an order's three) are parts of one
+`TrainerError`.  Small results of one call (mean and rstd; dweight and dbias; a routing's counts, rows, prob_mean and losses; an order's three; a residual stream's h and rstd) are parts of one
 allocation: clone what is to outlive the others by long.  Gradients are what the *_backward functions return; torch's automatic differentiation
 does not see these calls, but it refuses to use what it saved of a tensor that one of them has written since (`out`, or a Muon step's weight and momentum).  This module needs torch; the rest of the package does not.
 """

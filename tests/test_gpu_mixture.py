@@ -206,6 +206,20 @@ def test_an_order_s_results_are_tensors_of_their_own():
         t.copy_(keep[i])
 
 
+def test_the_stream_and_its_rstd_are_tensors_of_their_own():
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.randn(7, 33, device="cuda").to(dtype)
+        y, h, rstd = ops().rms_norm_forward(x, residual=x)
+        q, scale, h8, rstd8 = ops().rms_norm_quantised(x, residual=x)
+        for a, b in ((h, rstd), (h8, rstd8)):
+            keep = a.clone(), b.clone()
+            assert a.is_contiguous() and b.is_contiguous() and a.dtype == dtype and b.dtype == torch.float32 and torch.equal(keep[0], (2 * x.float()).to(dtype))
+            a.fill_(3)
+            assert torch.equal(b, keep[1])
+            b.fill_(4)
+            assert (a == 3).all()
+
+
 def test_tensors_of_another_device_are_refused():
     x = torch.zeros(4, 8, device="cuda")
     for bad in (lambda: ops().rms_norm_forward(x, torch.zeros(8)), lambda: ops().dispatch_forward(x, ops().Order(torch.zeros(4, 1, dtype=torch.int32), torch.zeros(4, dtype=torch.int32), None)),
