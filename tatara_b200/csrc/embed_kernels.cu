@@ -497,9 +497,9 @@ bool embed_plan(int64_t count, int64_t rows, int n, EmbedPlan* p) {
     p->passes = (bits + 9) / 10;
     p->bits = (bits + p->passes - 1) / p->passes;
     p->sort = sort_plan(count, 1 << p->bits, 1);
-    // pieces of 32 tokens, or more where there were over 2048 of them: their sums are one chain per warp when they are joined
+    // pieces of 32 tokens, or more where there were over 4096 of them: their sums are one chain per warp when they are joined
     p->piece = 32;
-    while (count > (int64_t)p->piece * 2048) p->piece *= 2;
+    while (count > (int64_t)p->piece * 4096) p->piece *= 2;
     p->pieces = (int)((count + p->piece - 1) / p->piece);
     p->list = (count + 7) / 8 * 8;
     // what one launch takes; tensors that fit a GPU are far below

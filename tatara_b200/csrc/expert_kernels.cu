@@ -10,7 +10,7 @@
 // once each, wherever they lie, in whole 16-byte accesses.  A group of lanes takes a row or a tile of its columns.  Sums are fp32: the choices in ascending order; a
 // dot product's columns per thread in ascending order, then halves of the lanes, then the warps in order.
 //
-// Measured: dispatch 65536 x 1536 bf16 to two places each 95.5 us (6.3 TB/s); combination of 30011 x 1000 fp16 from eight places each 95 us (5.4 TB/s: gathers of 2000 bytes), its gradient for
+// Measured: dispatch 65536 x 1536 bf16 to two places each 95.5 us (6.3 TB/s); combination of 30011 x 1000 fp16 from eight places each 88 us (5.9 TB/s: gathers of 2000 bytes), its gradient for
 // 40000 x 768 fp32 and two places 95.5 us (6.4 TB/s); the order of 65536 x 2 choices of 9 6 us, of 40000 x 8 of 256 15.6 us (launches that wait for one another).
 #include "op_sort.cuh"
 
@@ -52,6 +52,7 @@ struct ExpertPut {
 // ---- rows to their places ------------------------------------------------------------------------------------------------
 #define EXPERT_THREADS 256
 #define EXPERT_ZEROS 8  // places that a group looks at for rows of zeros
+#define COMBINE_THREADS 128
 
 // A row is n units U of memory: 16 bytes, or an element where rows do not start on 16-byte boundaries.  L lanes take CH units each of a row's tile.
 template <typename U, int L, int CH>
@@ -87,12 +88,13 @@ k_dispatch(const U* x, int64_t x_stride, int64_t rows, int n, int tiles, int k, 
     }
 }
 
-template <typename T, int VEC, int L, int CH>
-__global__ void __launch_bounds__(EXPERT_THREADS)
+// J choices' rows are on their way together: of one or two choices with four accesses a lane, of more four with two (30011 x 1000 fp16, k = 8: 88 us; two with four accesses 92, eight with two
+// 92; 65536 x 1536 bf16, k = 2: 113 and 118).  Blocks of four warps: of eight 95 us, the former.
+template <typename T, int VEC, int L, int CH, int J>
+__global__ void __launch_bounds__(COMBINE_THREADS)
 k_combine(const T* y, int64_t y_stride, int64_t slots, int64_t rows, int n, int tiles, int k, const int* position, const float* gate, T* __restrict__ out,
           int64_t out_stride) {
-    constexpr int J = 4;  // choices whose rows are on their way together
-    const int64_t unit = (int64_t)blockIdx.x * (EXPERT_THREADS / L) + threadIdx.x / L, row = unit / tiles;
+    const int64_t unit = (int64_t)blockIdx.x * (COMBINE_THREADS / L) + threadIdx.x / L, row = unit / tiles;
     const int t = threadIdx.x % L, first = ((int)(unit - row * tiles) * (L * CH) + t) * VEC;
     op_next_may_start();
     op_wait_for_previous();
@@ -217,8 +219,8 @@ void expert_with_shape(int units, F&& f) {
     else if (units <= 128 || MOST == 4) f(integral_constant<int, 32>(), integral_constant<int, 4>());
     else f(integral_constant<int, 32>(), integral_constant<int, MOST>());
 }
-bool expert_blocks(int64_t units, int lanes, unsigned* blocks) {
-    const int64_t b = (units + EXPERT_THREADS / lanes - 1) / (EXPERT_THREADS / lanes);
+bool expert_blocks(int64_t units, int lanes, int threads, unsigned* blocks) {
+    const int64_t b = (units + threads / lanes - 1) / (threads / lanes);
     *blocks = (unsigned)b;
     return b <= INT32_MAX;
 }
@@ -238,23 +240,27 @@ bool dispatch_go(const Experts& a, const void* x, int64_t xs, void* out, int64_t
         constexpr int L = decltype(l)::value, CH = decltype(ch)::value;
         const int tiles = (int)ceil_div64(n, L * CH);
         unsigned blocks;
-        fits = expert_blocks((a.rows + (a.slots + EXPERT_ZEROS - 1) / EXPERT_ZEROS) * tiles, L, &blocks);
+        fits = expert_blocks((a.rows + (a.slots + EXPERT_ZEROS - 1) / EXPERT_ZEROS) * tiles, L, EXPERT_THREADS, &blocks);
         if (fits)
             op_launch_next(a.s, dim3(blocks), dim3(EXPERT_THREADS), 0, k_dispatch<U, L, CH>, (const U*)x, xs / per, a.rows, n, tiles, a.k, a.position, a.source, (U*)out, os / per, a.slots);
     });
     return fits;
 }
-template <typename T, int VEC>
+template <typename T, int VEC, int J>
 bool combine_go(const Experts& a, const void* y, int64_t ys, const float* gate, void* out, int64_t os) {
     bool fits = true;
-    expert_with_shape<(VEC == 1 ? 8 : 2)>((int)ceil_div64(a.n, VEC), [&](auto l, auto ch) {
+    expert_with_shape<(VEC == 1 ? 8 : J == 4 ? 2 : 4)>((int)ceil_div64(a.n, VEC), [&](auto l, auto ch) {
         constexpr int L = decltype(l)::value, CH = decltype(ch)::value;
         const int tiles = (int)ceil_div64(a.n, L * CH * VEC);
         unsigned blocks;
-        fits = expert_blocks(a.rows * tiles, L, &blocks);
-        if (fits) op_launch_next(a.s, dim3(blocks), dim3(EXPERT_THREADS), 0, k_combine<T, VEC, L, CH>, (const T*)y, ys, a.slots, a.rows, a.n, tiles, a.k, a.position, gate, (T*)out, os);
+        fits = expert_blocks(a.rows * tiles, L, COMBINE_THREADS, &blocks);
+        if (fits) op_launch_next(a.s, dim3(blocks), dim3(COMBINE_THREADS), 0, k_combine<T, VEC, L, CH, J>, (const T*)y, ys, a.slots, a.rows, a.n, tiles, a.k, a.position, gate, (T*)out, os);
     });
     return fits;
+}
+template <typename T, int VEC>
+bool combine_pick(const Experts& a, const void* y, int64_t ys, const float* gate, void* out, int64_t os) {
+    return a.k == 1 ? combine_go<T, VEC, 1>(a, y, ys, gate, out, os) : a.k == 2 ? combine_go<T, VEC, 2>(a, y, ys, gate, out, os) : combine_go<T, VEC, 4>(a, y, ys, gate, out, os);
 }
 template <typename T, int VEC, int W, int L>
 void combine_backward_go(const Experts& a, const void* dout, int64_t ds, const void* y, int64_t ys, const float* gate, void* dy, int64_t dys, float* dgate) {
@@ -366,7 +372,7 @@ extern "C" int tb_combine_forward(const void* d_y, int64_t y_stride, int type, i
     if (rows == 0) return TB_OK;
     if (op_extents_meet(outr, {yr, op_vector(d_position, rows * k), op_vector(d_gate, rows * k)})) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_out overlaps another tensor");
     const bool wide = n % (16 / size) == 0 && expert_aligned(d_y, y_stride, size) && expert_aligned(d_out, out_stride, size);
-#define GO(T, VEC) (wide ? combine_go<T, VEC>(a, d_y, y_stride, d_gate, d_out, out_stride) : combine_go<T, 1>(a, d_y, y_stride, d_gate, d_out, out_stride))
+#define GO(T, VEC) (wide ? combine_pick<T, VEC>(a, d_y, y_stride, d_gate, d_out, out_stride) : combine_pick<T, 1>(a, d_y, y_stride, d_gate, d_out, out_stride))
     const bool fits = type == TB_TYPE_F32 ? GO(float, 4) : type == TB_TYPE_F16 ? GO(__half, 8) : GO(__nv_bfloat16, 8);
 #undef GO
     return fits ? op_launched(err, err_len) : expert_too_many(err, err_len);
