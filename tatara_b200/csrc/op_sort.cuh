@@ -90,6 +90,7 @@ struct SortWalk {
         for (int s = 0; s < S; ++s) {
             before[s] = 0;
             if (lane == __ffs(peers[s]) - 1 && key(s) >= 0) before[s] = atomicAdd(&count[key(s)], __popc(peers[s]));
+            __syncwarp();  // another lane may add for the same key in the next step, and has to find this one's sum
         }
 #pragma unroll
         for (int s = 0; s < S; ++s) rank[s] = __shfl_sync(0xffffffffu, before[s], __ffs(peers[s]) - 1) + __popc(peers[s] & ((1u << lane) - 1u));
