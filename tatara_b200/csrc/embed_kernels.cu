@@ -22,6 +22,7 @@ namespace {
 #define EMBED_THREADS 128
 #define EMBED_WARPS 4
 #define EMBED_ROWS 16  // table rows per warp at most
+#define EMBED_NAN __int_as_float(0x7fc00000)  // what sums are after a wait that has run out
 
 struct Tokens {
     const void* p;
@@ -219,8 +220,7 @@ struct EmbedCopies {
             __syncwarp();
         }
     }
-    // of all sums from here on: NaN after a wait that has run out
-    __device__ __forceinline__ float factor() const { return ring.ok ? 1.0f : __int_as_float(0x7fc00000); }
+    __device__ __forceinline__ bool failed() const { return !ring.ok; }  // a wait has run out: of all sums from here on
     __device__ __forceinline__ void end() { ring.end(); }
 };
 // Through registers, K rows at a time: less latency where a warp has a few rows, and as many short ones as there are (an SM starts a copy every 90 cycles or so).
@@ -259,7 +259,7 @@ struct EmbedLoads {
             }
         }
     }
-    __device__ __forceinline__ float factor() const { return 1.0f; }
+    __device__ __forceinline__ bool failed() const { return false; }
     __device__ __forceinline__ void end() {}
 };
 
@@ -286,7 +286,7 @@ k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n
         if (row0 >= rows) return;
         const int end_row = (int)min(row0 + per, rows);
         const auto store = [&](int64_t v) {
-            const float by = scale * from_rows.factor();
+            const float by = from_rows.failed() ? EMBED_NAN : scale;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int col = first + c * 32 * VEC;
@@ -327,8 +327,9 @@ k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n
         int token, from, to, first, last;  // the token's entries in this piece, the list's first sum, which is in the chunk where it begins, and its last piece
     };
     __shared__ Sum s_sums[EMBED_WARPS][2];
-    __shared__ bool s_last;
+    __shared__ bool s_last, s_failed;
     const int piece = (int)group * list.together + warp;
+    if (threadIdx.x == 0) s_failed = false;
     if (lane == 0) s_sums[warp][0].token = s_sums[warp][1].token = -1;
     if (warp < list.together && (int64_t)piece * list.piece < count) {
         const int from = piece * list.piece, to = list.piece < count - from ? from + list.piece : count, first_key = list.key[from], last_key = list.key[to - 1];
@@ -345,8 +346,11 @@ k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n
     }
     __syncthreads();
     float* s_part = reinterpret_cast<float*>(s_rows);  // what the rows have come through
-    // the warps' sums of their columns, added up in order: column at of the tile
+    // The warps' sums of their columns, added up in order: column at of the tile.  After a wait that has run out in any warp, copies may still have been on their way to where the sums
+    // lie; they are waited for, and what the block puts out from there on is NaN by a mark that lies elsewhere.
     const auto share_out = [&](auto put) {
+        from_rows.end();
+        if (from_rows.failed()) s_failed = true;
         __syncthreads();
 #pragma unroll
         for (int c = 0; c < CH; ++c)
@@ -358,7 +362,7 @@ k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n
 #pragma unroll
             for (int w = 1; w < EMBED_WARPS; ++w) sum += s_part[w * TILE + at];
             const int col = column + (at / 32 / VEC * 32 + at % 32) * VEC + at / 32 % VEC;
-            if (col < n) put(col, sum);
+            if (col < n) put(col, s_failed ? EMBED_NAN : sum);
         }
     };
     for (int which = 0, next; which < 2 * list.together; which = next) {
@@ -378,11 +382,6 @@ k_embed_rows(const T* dy, int64_t dy_stride, EmbedList list, int64_t rows, int n
             const int many = min(32, mine_to - i0), id = lane < many ? list.id[i0 + lane] : 0;
             from_rows.add(acc, id, many, [](int) {});
         }
-        const float by = from_rows.factor();
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[c][i] *= by;
         share_out([&](int col, float x) { list.part[number * n + col] = x; });
         // who writes the list's last sum adds them all up
         __threadfence();

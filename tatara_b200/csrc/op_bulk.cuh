@@ -4,7 +4,10 @@
 
 namespace {
 
-#define BULK_WAIT_LIMIT (1 << 20)  // tries before a wait gives up
+enum { BULK_COPY, BULK_END };
+#ifndef BULK_WAIT_LIMIT  // tries before a wait gives up; the one at the end outlasts the others
+#define BULK_WAIT_LIMIT(role) ((role) == BULK_END ? 1 << 22 : 1 << 20)
+#endif
 
 __device__ __forceinline__ unsigned bulk_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 
@@ -32,9 +35,9 @@ struct BulkRing {
         }
         ++put_count;
     }
-    __device__ __forceinline__ bool arrived(unsigned limit) {
+    __device__ __forceinline__ bool arrived(int limit) {
         const unsigned bar = bars + 8 * (taken % K), parity = taken / K & 1;
-        for (unsigned i = 0; i < limit; ++i) {
+        for (int i = 0; i < limit; ++i) {
             unsigned there;
             asm volatile(
                 "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -48,14 +51,14 @@ struct BulkRing {
     // the slot of the next copy, once it is there
     __device__ __forceinline__ unsigned take() {
         const unsigned k = taken % K;
-        if (ok) ok = __all_sync(0xffffffffu, arrived(BULK_WAIT_LIMIT));
+        if (ok) ok = __all_sync(0xffffffffu, arrived(BULK_WAIT_LIMIT(BULK_COPY)));
         if (ok) ++taken;
         return k;
     }
-    // before the block ends: nothing is on its way any more
+    // Before the slots hold anything else, and before the block ends: nothing is on its way any more.  There is something only after a wait that has run out.
     __device__ __forceinline__ void end() {
         for (; taken < put_count; ++taken)
-            if (!arrived(BULK_WAIT_LIMIT << 2)) break;
+            if (!arrived(BULK_WAIT_LIMIT(BULK_END))) put_count = taken;  // not waited for again
     }
 };
 
