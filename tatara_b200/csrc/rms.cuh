@@ -116,9 +116,9 @@ __device__ __forceinline__ float rms_scale(float most) {
     const float s = most * (1.0f / RMS_MOST);
     return s < RMS_LEAST ? RMS_LEAST : s;
 }
-// Whether z of largest magnitude `most` may be multiplied with 448 / most for z r / s: to 2 ulp, where nothing leaves the range of that quotient and s is not the smallest scale.
+// Whether z of largest magnitude `most` may be multiplied with 448 / most for z late / s: to 2 ulp, where nothing leaves the range of that quotient and s is not the smallest scale.
 // (With divisions to the last bit for every group, 40000 x 1000 fp16 in groups of 128 took 40 us.)
-__device__ __forceinline__ bool rms_usual(float most, float r) { return most > 1e-30f && most < 1e30f && most * r > 1e-35f; }
+__device__ __forceinline__ bool rms_usual(float most, float late) { return most > 1e-30f && most < 1e30f && most * late > 1e-35f; }
 __device__ __forceinline__ uint8_t rms_q(float v) { return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
 // VEC numbers times `by` as adjacent bytes
 template <int VEC>
@@ -246,7 +246,14 @@ k_rms_forward(const T* x, int64_t x_stride, const T* res, int64_t res_stride, co
                 if (there) op_store<T, VEC>(static_cast<T*>(y) + row * y_stride + col, v[c]);
             }
         } else {
-            // z = f h * weight, y = z * r: one multiplication less for every column
+            // z = f h * weight, y = z * late.  h * weight may leave fp32's range, or lose bits, where y does not, so 1 / rms comes first; in the kernels that walk down it may come last, at
+            // one multiplication less per column, where z is no larger than y and less than 16 times smaller (40000 x 1000 fp16 in groups of 128: 24.7 us, 25.4 where it comes first).
+            const bool near = AHEAD && r >= 1.0f && r < 16.0f;
+            const float late = near ? r : 1.0f;
+            if (!near)
+#pragma unroll
+                for (int c = 0; c < CH; ++c)
+                    if (c < FULL || (c * LANES + t) * VEC < n) rms_multiply<VEC>(v[c], r);
             if (weight) {
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
@@ -279,8 +286,8 @@ k_rms_forward(const T* x, int64_t x_stride, const T* res, int64_t res_stride, co
 #pragma unroll
                     for (int w = 0; w < W; ++w) most[0] = rms_larger(most[0], s_max[w]);
                 }
-                usual = rms_usual(most[0], r);
-                if (t == 0 && there) scale_out[row] = rms_scale(most[0] * r);
+                usual = rms_usual(most[0], late);
+                if (t == 0 && there) scale_out[row] = rms_scale(most[0] * late);
             } else {
 #pragma unroll
                 for (int c = 0; c < CH; c += JOIN) {
@@ -292,8 +299,8 @@ k_rms_forward(const T* x, int64_t x_stride, const T* res, int64_t res_stride, co
 #pragma unroll
                     for (int k = 1; k < JOIN; ++k)
                         if (c + k < CH) most[c + k < CH ? c + k : 0] = most[c];
-                    usual = usual && (rms_usual(most[c], r) || (c >= FULL && col >= n));
-                    if (there && (c < FULL || col < n) && t % GL == 0) scale_out[row * groups + col / G] = rms_scale(most[c] * r);
+                    usual = usual && (rms_usual(most[c], late) || (c >= FULL && col >= n));
+                    if (there && (c < FULL || col < n) && t % GL == 0) scale_out[row * groups + col / G] = rms_scale(most[c] * late);
                 }
             }
             if (__all_sync(0xffffffffu, usual || !there)) {
@@ -310,8 +317,8 @@ k_rms_forward(const T* x, int64_t x_stride, const T* res, int64_t res_stride, co
 #pragma unroll
                 for (int k = 0; k < CH; ++k) {
                     if (k != c || !there || col >= n) continue;
-                    rms_multiply<VEC>(v[k], r);
-                    rms_store_q<VEC>(q + col, v[k], 1.0f / rms_scale(most[G == 1 ? 0 : k] * r));
+                    rms_multiply<VEC>(v[k], late);
+                    rms_store_q<VEC>(q + col, v[k], 1.0f / rms_scale(most[G == 1 ? 0 : k] * late));
                 }
             }
         }
