@@ -116,6 +116,8 @@ __device__ __forceinline__ float rms_scale(float most) {
     const float s = most * (1.0f / RMS_MOST);
     return s < RMS_LEAST ? RMS_LEAST : s;
 }
+// Its inverse, NaN of a scale that is infinite (0 would make the group's other numbers zeros)
+__device__ __forceinline__ float rms_inverse(float s) { return s < INFINITY ? 1.0f / s : __int_as_float(0x7fc00000); }
 // Whether z of largest magnitude `most` may be multiplied with 448 / most for z late / s: to 2 ulp, where nothing leaves the range of that quotient and s is not the smallest scale.
 // (With divisions to the last bit for every group, 40000 x 1000 fp16 in groups of 128 took 40 us.)
 __device__ __forceinline__ bool rms_usual(float most, float late) { return most > 1e-30f && most < 1e30f && most * late > 1e-35f; }
@@ -318,7 +320,7 @@ k_rms_forward(const T* x, int64_t x_stride, const T* res, int64_t res_stride, co
                 for (int k = 0; k < CH; ++k) {
                     if (k != c || !there || col >= n) continue;
                     rms_multiply<VEC>(v[k], late);
-                    rms_store_q<VEC>(q + col, v[k], 1.0f / rms_scale(most[G == 1 ? 0 : k] * late));
+                    rms_store_q<VEC>(q + col, v[k], rms_inverse(rms_scale(most[G == 1 ? 0 : k] * late)));
                 }
             }
         }
@@ -374,7 +376,7 @@ k_rms_forward_long(const T* x, int64_t x_stride, const T* res, int64_t res_strid
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < W; ++w) most = rms_larger(most, s_max[w]);
-        const float s = rms_scale(most), inverse = 1.0f / s;
+        const float s = rms_scale(most), inverse = rms_inverse(s);
         if (threadIdx.x == 0) scale_out[row] = s;
         for (C c = threadIdx.x; c < n; c += TH) {
             const float v = sum_at(c);
@@ -399,7 +401,7 @@ k_rms_forward_long(const T* x, int64_t x_stride, const T* res, int64_t res_strid
             }
             most = rms_larger(most, v[i]);
         }
-        const float s = rms_scale(rms_group_max<32>(most)), inverse = 1.0f / s;
+        const float s = rms_scale(rms_group_max<32>(most)), inverse = rms_inverse(s);
         if (lane == 0) scale_out[row * groups + g] = s;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

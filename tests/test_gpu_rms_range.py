@@ -1,8 +1,10 @@
-"""The root-mean-square norm in 8 bits where weights or squares leave the usual range."""
+"""The root-mean-square norm in 8 bits where weights, results or squares leave the usual range."""
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
-from test_gpu_rms import check_backward, check_quantised, make, ops, vector  # noqa: E402
+from test_gpu_rms import EPS, check_backward, check_quantised, make, ops, plain, vector  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 # rows, columns, type, first column in a wider buffer: lanes that share a warp, a warp per row, walking down, several warps, few rows with more, rows read again; and rows that start anywhere
@@ -33,3 +35,25 @@ def test_scales_and_gradients_of_rows_whose_squares_leave_fp32(n, offset):
             check_quantised(v, w, None, group, ops().rms_norm_quantised(v, w, eps=0.0, group=group), eps=0.0)
         h, rstd = ops().rms_norm_forward(v, w, eps=0.0)[1:]
         check_backward(dy, h, rstd, w, None, ops().rms_norm_backward(dy, h, rstd, w))
+
+
+def groups_of(n, group):
+    return torch.arange(n, device="cuda") // (n if group is None else group)
+
+
+@pytest.mark.parametrize("rows,n,dtype,offset", LAYOUTS)
+@pytest.mark.parametrize("group", [None, 32, 128])
+def test_a_group_with_an_infinity_from_the_weight(rows, n, dtype, offset, group):
+    x = make(rows, n, dtype, 1, offset, offset)
+    for odd in (math.inf, -math.inf, math.nan, 3e38):   # the last one makes y infinite wherever |h| / rms is above 1.2
+        w = vector(n, 2)
+        w[n // 2] = odd
+        q, scale, _, _ = ops().rms_norm_quantised(x, w, eps=EPS, group=group)
+        y = plain(x, w, None, EPS)[0].float()
+        column = groups_of(n, group)
+        most = torch.zeros(scale.shape, device="cuda").index_reduce_(1, column, y.abs(), "amax")
+        near = (plain(x, w, None, EPS)[0].abs() / torch.finfo(torch.float32).max - 1).abs().amin(1, keepdim=True) < 1e-3   # y may round to either side
+        bad = ~most.isfinite()
+        assert bad.any() and ((scale == math.inf) | scale.isnan() | ~bad | near).all()
+        assert (q.float().isnan() | ~bad[:, column] | near).all()
+        assert (q.float().isfinite() | bad[:, column] | near).all() and (scale.isfinite() | bad | near).all()
