@@ -111,7 +111,7 @@ struct Shared {
     void allocate(const at::Tensor& like) { base = make(like, {bytes}, at::kByte); }
     at::Tensor tensor(int64_t at, at::IntArrayRef shape, at::ScalarType type) const {
         at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(type));
-        t.unsafeGetTensorImpl()->set_storage_offset(at / 4);
+        t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(type));
         t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
         return t;
     }
