@@ -535,7 +535,7 @@ void embed_rows_go(const EmbedBackward& a) {
         op_allow_smem(kernel, SMEM, known);
     }
     // Several rows per warp share the search: as many as leave every warp four turns, or one turn of short rows, which take no longer than the search.
-    const int64_t turns = a.rows * tiles / ((int64_t)sm_count() * PER_SM * EMBED_WARPS * (a.n * (int)sizeof(T) <= 256 ? 1 : 4));
+    const int64_t turns = a.rows * tiles / ((int64_t)sm_count() * PER_SM * EMBED_WARPS * (a.n <= 256 / (int)sizeof(T) ? 1 : 4));
     const int per = (int)(turns < 1 ? 1 : turns > EMBED_ROWS ? EMBED_ROWS : turns);
     // pieces together where they are more than a few blocks per SM: most of them have no long list, and a long one has fewer sums
     EmbedList list = a.list;
