@@ -12,6 +12,8 @@
 #pragma once
 #include "op_common.cuh"
 
+#include <type_traits>
+
 namespace {
 
 #define SORT_THREADS 256
@@ -19,7 +21,9 @@ namespace {
 #define SORT_MAX_E 1024
 #define SORT_STEPS 8          // of a warp, whose entries are in registers together
 #define SORT_ONE 2048         // entries of a single block's sort
-#define SORT_SCAN 4096        // blocks * keys above which a launch of its own adds up the counts (5000 x 2 of 512, 20480 of them: 7.9 us, without it 10.2; 65536 x 2 of 20, 2560: 8.2 and 6.2)
+// Blocks * keys above which a launch of its own adds up the counts; with it and without, entries x keys: 80000 x 128 (10112) 8.2 and 7.0 us, 131072 x 128 (16384) 9.1 and 8.1, 320000 x 128 (20096) 11.7 and 11.6,
+// 40000 x 512 (20480) 8.3 and 8.9, 80000 x 256 (20224) 9.0 and 10.5, 131072 x 256 (32768) 9.5 and 17.5.
+#define SORT_SCAN 16384
 
 struct SortPlan {
     int blocks, keys, align;
@@ -208,18 +212,27 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_place(Source source, int6
             s_total[e] = part[(int64_t)p.blocks * keys + e];
         }
     } else if (p.blocks > 1) {
-        // keys side by side, the threads that are left share the blocks
+        // keys side by side, the threads that are left share the blocks; U blocks' counts are on their way together, those behind the last whole batch too (10000 entries of 512 keys, ten
+        // blocks: 6.4 us; with those behind it a load at a time 10.2)
         int width = 32;
         while (width < keys && width < SORT_THREADS) width *= 2;
+        constexpr int U = 16;
         for (int e = threadIdx.x % width; e < keys; e += width) {
             const int step = SORT_THREADS / width;
             int total = 0, ahead = 0;
-#pragma unroll 16
-            for (int b = threadIdx.x / width; b < p.blocks; b += step) {
-                const int c = part[(int64_t)b * keys + e];
-                total += c;
-                if (b < (int)blockIdx.x) ahead += c;
-            }
+            int b0 = threadIdx.x / width;
+            const auto batch = [&](auto whole) {
+                int c[U];
+#pragma unroll
+                for (int i = 0; i < U; ++i) c[i] = decltype(whole)::value || b0 + i * step < p.blocks ? part[(int64_t)(b0 + i * step) * keys + e] : 0;
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    total += c[i];
+                    if (b0 + i * step < (int)blockIdx.x) ahead += c[i];
+                }
+            };
+            for (; b0 + (U - 1) * step < p.blocks; b0 += U * step) batch(std::true_type());
+            if (b0 < p.blocks) batch(std::false_type());
             atomicAdd(&s_total[e], total);
             atomicAdd(&s_ahead[e], ahead);
         }
