@@ -316,11 +316,13 @@ int tb_muon_step(const tb_muon* cfg, const float* d_w, const float* d_m, const v
 
 /* Root-mean-square norm on a residual stream: h = x + residual, y = h * rstd * weight per row of n, rstd = 1 / sqrt(mean(h^2) + eps).  The norm is that of the fp32 sum;
  * d_h receives the sum rounded to the tensors' type, for the next layer and the backward pass.  residual may be NULL (h is x; d_h must be NULL then), weight (fp32 [n]), d_h and d_rstd
- * (fp32 [rows], kept for the backward pass) may be NULL.  All rows have the same type.  y and h may each be the memory of x or of the residual (not the same one). */
+ * (fp32 [rows], kept for the backward pass) may be NULL.  All rows have the same type.  y and h may each be the memory of x or of the residual (not the same one); the
+ * backward pass takes h, which is x where there is no residual: not for a y in its place.  Rows go by 16-byte accesses where they all start on such a boundary and n is a multiple, and the weight starts on 16 bytes for
+ * fp32 and 32 bytes for 16-bit rows (backward 16); otherwise by single elements, at two to three times the time. */
 int tb_rms_norm_forward(const void* d_x, int64_t x_stride, const void* d_residual, int64_t residual_stride, const float* d_weight, float eps, int type,
                         int64_t rows, int n, void* d_y, int64_t y_stride, void* d_h, int64_t h_stride, float* d_rstd, void* stream, char* err, size_t err_len);
 /* The same with y in 8 bits: q [rows, n] (e4m3 bytes) and scale [rows, ceil(n / group)] (fp32, contiguous) with y ~ q * scale; group: 32, 64, 128 columns, or n (a scale
- * per row).  scale = max(largest |y| of the group / 448, 2^-126), q = y / scale rounded to nearest.  A group with an infinity or a NaN has q NaN throughout.  q overlaps no other
+ * per row).  scale = max(largest |y| of the group / 448, 2^-126), q = y / scale rounded to nearest.  A group whose y holds an infinity or a NaN has q NaN throughout.  q overlaps no other
  * tensor; h may be the memory of x or of the residual. */
 int tb_rms_norm_quantised(const void* d_x, int64_t x_stride, const void* d_residual, int64_t residual_stride, const float* d_weight, float eps, int type,
                           int64_t rows, int n, int group, void* d_q, int64_t q_stride, float* d_scale, void* d_h, int64_t h_stride, float* d_rstd, void* stream,

@@ -21,7 +21,9 @@ namespace {
 
 #define EMBED_THREADS 128
 #define EMBED_WARPS 4
-#define EMBED_ROWS 16  // table rows per warp at most
+// table rows per warp at most; with 8 of them, 16 and 32: 1000000 x 1 fp32 from 5000 tokens 66, 49 and 42 us, 200000 x 128 fp32 from 20000 47, 43 and 43, 73305 x 32 fp32 from 131072 44, 46 and 48; above 2 KB 8 are better
+// (73305 x 1024 fp32 from 65536 141 and 154)
+#define EMBED_ROWS 16
 #define EMBED_NAN __int_as_float(0x7fc00000)  // what sums are after a wait that has run out
 
 struct Tokens {
@@ -488,7 +490,9 @@ struct EmbedPlan {
 };
 bool embed_plan(int64_t count, int64_t rows, int n, EmbedPlan* p) {
     if (count < 0 || count > OP_MAX_ENTRIES || rows < 1 || rows > INT32_MAX || n < 1 || n > OP_MAX_COLUMNS) return false;
-    // every row's blocks look through all tokens: as long as they, and what they read, are less than the sort's launches
+    // Every row's blocks look through all tokens: as long as they, and what they read, are less than the sort's launches.  They are counted as tiles of 128 columns, which is what fp32 rows of whole 16-byte
+    // accesses have, because the workspace's size may depend neither on the type nor on the alignment; 16-bit rows have half as many blocks, and rows that start anywhere four times as many (9 tokens,
+    // 122 x 1473 bf16: 12 us).
     const int64_t blocks = rows * ceil_div64(n, 128);
     p->few = count > 0 && count <= EMBED_FEW && blocks <= 16 * (int64_t)sm_count() && blocks * count <= 16 * 1024 * (int64_t)sm_count();
     int bits = 1;
@@ -551,8 +555,10 @@ void embed_rows_pick(const EmbedBackward& a) {
         op_launch_next(a.s, dim3((unsigned)(a.rows * units)), dim3(EMBED_FEW_WARPS * 32), 0, k_embed_few<T, O, VEC>, a.tokens, (int)a.count, (const T*)a.dy, a.dys, a.n, units, a.scale, (O*)a.out, a.os);
         return;
     }
-    // Rows up to 2 KB by loads (125143 tokens evenly over 3640 x 384 fp32: 73 us, by copies 85), longer ones and their tiles of 2 KB by copies (73305 x 768: 136, by loads
-    // 143); rows that start anywhere up to 128 columns by loads, by copies above (3640 x 222: 80 us, by loads 60 where tokens are even and 154 where they are not).
+    // Rows up to 2 KB by loads (125143 tokens evenly over 3640 x 384 fp32: 73 us, by copies 85), rows up to 3 KB by copies of the whole row, longer ones by copies of tiles of 2 KB.  65536 tokens of
+    // tables of 73305 and 3640 rows, whole rows of 3 KB and tiles of 2 KB: 640 fp32 111 and 63 us, 119 and 78; 768 fp32 118 and 71, 123 and 76; 1152 bf16 111 and 69, 114 and 72; 1536 bf16 122 and 81, 121 and
+    // 79.  Of longer rows, tiles of 3 KB take 16-bit ones no less time and fp32 ones some less, some more: 1024 fp32 182 and 79, by tiles of 2 KB 154 and 80; 1536 fp32 225 and 100, 243 and 115.
+    // Rows that start anywhere by loads up to 128 columns, by copies above (3640 x 222: 80 us, by loads 60 where tokens are even and 154 where they are not).
     if constexpr (VEC == 1) {
         if (units == 1) return embed_rows_go<T, O, 1, 1, 8, EmbedLoads>(a);
         if (units == 2) return embed_rows_go<T, O, 1, 2, 8, EmbedLoads>(a);
@@ -600,7 +606,7 @@ bool embed_aligned(const void* p, int64_t stride, int size) { return ((uintptr_t
 int embed_check(int type, int64_t count, int64_t rows, int n, int token_bytes, const void* tokens, char* err, size_t err_len) {
     if (!op_type_size(type)) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "type must be TB_TYPE_F32, TB_TYPE_F16 or TB_TYPE_BF16 (got %d)", type);
     if (token_bytes != 4 && token_bytes != 8) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "token_bytes must be 4 or 8 (got %d)", token_bytes);
-    if (count < 0 || count > OP_MAX_ENTRIES || rows < 1 || rows > INT32_MAX) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "count must be in [0, 2^31) and rows in [1, 2^31)");
+    if (count < 0 || count > OP_MAX_ENTRIES || rows < 1 || rows > INT32_MAX) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "count must be in [0, 2^31 - 1024] and rows in [1, 2^31)");
     if (n < 1 || n > OP_MAX_COLUMNS) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "n must be in [1, 2^30] (got %d)", n);
     if (count > 0 && !tokens) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "d_tokens is NULL");
     if ((uintptr_t)tokens % token_bytes) return op_report(err, err_len, TB_ERR_INVALID_ARGUMENT, "tensors must be aligned to their elements");

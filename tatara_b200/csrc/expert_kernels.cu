@@ -265,7 +265,7 @@ bool combine_pick(const Experts& a, const void* y, int64_t ys, const float* gate
 template <typename T, int VEC, int W, int L>
 void combine_backward_go(const Experts& a, const void* dout, int64_t ds, const void* y, int64_t ys, const float* gate, void* dy, int64_t dys, float* dgate) {
     constexpr int PER = EXPERT_THREADS / (W == 1 ? L : 32 * W);
-    const int64_t row_blocks = (a.rows + PER - 1) / PER, blocks = row_blocks + (a.slots + 31) / 32;  // below 2^31 + 2^26: rows * k is below 2^31
+    const int64_t row_blocks = (a.rows + PER - 1) / PER, blocks = row_blocks + (a.slots + 31) / 32;  // below 2^28 + 2^26: eight rows to a block or more, but where rows are few
 #define GO(K) \
     op_launch_next(a.s, dim3((unsigned)blocks), dim3(EXPERT_THREADS), 0, k_combine_backward<T, VEC, W, L, K>, (const T*)dout, ds, (const T*)y, ys, a.slots, a.rows, a.n, a.k, a.position, a.source, gate, \
                    (T*)dy, dys, dgate, row_blocks)

@@ -20,7 +20,9 @@ namespace {
 #define SORT_WARPS 8
 #define SORT_MAX_E 1024
 #define SORT_STEPS 8          // of a warp, whose entries are in registers together
-#define SORT_ONE 2048         // entries of a single block's sort
+// entries of a single block's sort: 1200 x 1 of 9 4.0 us (two blocks 4.7), 2000 x 1 of 1024 5.8 (7.0), 3000 x 1 of 256 10.3 (several blocks 5.4); where `align` leaves much to fill it is slower (276 x 6 of 215, align 16: 10.5, several
+// blocks 8.2)
+#define SORT_ONE 2048
 // Blocks * keys above which a launch of its own adds up the counts; with it and without, entries x keys: 80000 x 128 (10112) 8.2 and 7.0 us, 131072 x 128 (16384) 9.1 and 8.1, 320000 x 128 (20096) 11.7 and 11.6,
 // 40000 x 512 (20480) 8.3 and 8.9, 80000 x 256 (20224) 9.0 and 10.5, 131072 x 256 (32768) 9.5 and 17.5.
 #define SORT_SCAN 16384

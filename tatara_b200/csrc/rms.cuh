@@ -27,8 +27,9 @@ void rms_quantised_run(const RmsForward& a, int type, bool wide);  // rms_quanti
 
 namespace {
 
-#define RMS_REG_N 32768      // longest row that the forward pass keeps in registers
-#define RMS_REG_N_BACK 16384 // ... the backward pass
+// The longest row that the backward pass keeps in registers (the forward pass: 32768, the last of rms_forward_pick).  Kept and read again: forward 2000 x 17000 fp32 56 and 63 us, 24576 bf16 48 and 67; backward 2000 x
+// 16384 fp32 105 and 119, but 2000 x 10000 86 and 82, 200 x 12288 26 and 22.
+#define RMS_REG_N_BACK 16384
 #define RMS_MOST 448.0f      // the largest e4m3 number
 #define RMS_LEAST 1.17549435e-38f  // 2^-126: the smallest scale
 
@@ -327,7 +328,7 @@ k_rms_forward(const T* x, int64_t x_stride, const T* res, int64_t res_stride, co
     } while (AHEAD && (row += (int64_t)gridDim.x * RB) < rows);
 }
 
-// Any row: a block per row that reads it again for every pass; thread t takes columns t, t + TH, ..  Rows longer than RMS_REG_N, and 8-bit rows over 1536 columns that start anywhere.
+// Any row: a block per row that reads it again for every pass; thread t takes columns t, t + TH, ..  Rows longer than 32768, and 8-bit rows over 1536 columns that start anywhere.
 // C counts columns: int, or int64_t where the last step would go beyond 2^31.
 template <typename T, typename C, int TH>
 __global__ void __launch_bounds__(TH)
@@ -447,6 +448,8 @@ void rms_forward_pick(const RmsForward& a) {
     GO(0, 1, 32, 8); GO(256, 1, 32, 16);
     if constexpr (VEC > 1) { GO(512, 1, 32, 24); GO(768, 1, 32, 32); }
     else GO(512, 1, 32, 32);
+    // many rows of 16-byte accesses (65536 x 1088 bf16 48 us, four warps per row 70; 1536 fp32 119 and 116); not the best for some hundreds of rows (500 x 1536 fp32 4.4 and 2.5), nor for single elements (30000 x 1251 bf16 65
+    // and 48)
     GO(1024, 1, 32, 48);
     if constexpr (VEC > 1 || G <= 1) {
         if constexpr (G == 0) { GO(1536, 4, 32, 16); GO(2048, 4, 32, 32); }

@@ -78,7 +78,8 @@ def rms_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, 
 
     x, residual, y and h are of one type (float32, float16 or bfloat16) with any row strides, weight float32 [n].  y is the norm of the 32-bit sum, h the sum
     rounded to the type (x itself without a residual): the residual of the next layer.  h and rstd (float32 [rows]) are what `rms_norm_backward` takes.  `out` and
-    `residual_out` may be x or residual, not both the same.  Without `eps`, a row of zeros is NaN.
+    `residual_out` may be x or residual, not both the same.  Where y is written over x without a residual, h is that memory too and no longer what `rms_norm_backward` takes.  Without `eps`, a
+    row of zeros is NaN.
     """
     return _ops.rms_norm_forward(x, weight, residual, eps, out, residual_out)
 
@@ -88,7 +89,7 @@ def rms_norm_quantised(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *
     """(q, scale, h, rstd): `rms_norm_forward` with y ~ q * scale in 8 bits.
 
     q is float8_e4m3fn [rows, n], scale float32 [rows, ceil(n / group)]: the largest |y| of a row's group of 32, 64, 128 or (None) all columns over 448, at least
-    2^-126.  The backward pass is `rms_norm_backward`, as if y had not been rounded.  A group that holds an infinity or a NaN is NaN throughout.
+    2^-126.  The backward pass is `rms_norm_backward`, as if y had not been rounded.  A group whose y holds an infinity or a NaN is NaN throughout.
     """
     return _ops.rms_norm_quantised(x, weight, residual, eps, group, residual_out)
 
