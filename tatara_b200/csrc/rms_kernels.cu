@@ -10,7 +10,7 @@
 // scale of 2^-100 or 2^100, which costs the rows that need it nothing but instructions.
 //
 // Measured (inputs not in L2): 65536 x 1536 bf16 with a residual 118 us (6.8 TB/s), its backward pass in fp32 with the residual's gradient 242 us (6.7 TB/s, 7 of them the columns' sums);
-// 8 bits, 40000 x 1000 fp16 in groups of 128 25 us (4.9 TB/s: 410 instructions per row, issue slots at 63 %; 25.5 where rms is above 1).  16 x 1536: 1.8 us.
+// 8 bits, 40000 x 1000 fp16 in groups of 128 25 us (4.9 TB/s: 430 instructions per row, issue slots at 64 %; 25.5 where rms is above 1).  16 x 1536: 1.8 us.
 #include "rms.cuh"
 
 namespace {
